@@ -1,0 +1,702 @@
+// Key / value cache held in 4 bits: writing new tokens into it (with rotary embedding), reading them back, attention over it.
+//
+// Layout.  pages[n_pages][Hkv][page / 16][18 hd] bytes: a block of 16 tokens of one head is one contiguous piece that a single bulk copy fetches, so
+// that the page size only says how finely the pool is dealt out.  In a block: 16 rows of key codes (hd / 2 bytes each), 16 rows of value codes, 16
+// rows of key scales (NG = hd / 32 bf16), 16 rows of value scales.  32 neighbouring elements (a group g) of a row share the scale s; code c in 0..15
+// stands for (c - 8) s.  s = -m / 8 rounded to bf16, m the element of largest magnitude (of a tie the negative one): it gets code 0 and is held exactly
+// where s is, and the step is 1/8 of the largest magnitude instead of the 1/7 of a scale without a sign.
+// The order in a row is that of the matrix instructions' registers in the attention kernel (lane = 4 i + j):
+//   key row:   32-bit word j NG + g has the elements 32 g + 8 j + e, e = 0..7, in its e-th four bits
+//   value row: 16-bit word i NG + g has the elements 32 g + 4 i + e, e = 0..3
+#include "tc.cuh"
+
+namespace {
+
+MLB_DEFINE_ERROR_WORD(kv4)
+
+constexpr int TOK = 16;                 // tokens of a block
+template <int HD> struct Block {
+  static constexpr int NG = HD / 32, ROW = HD / 2, BYTES = 18 * HD;
+  static constexpr int V = 8 * HD, KS = 16 * HD, VS = 17 * HD;      // where value codes, key scales and value scales begin
+};
+constexpr float TINY = 7.52316385e-37f;      // 2^-120: a smaller scale is held as 0 (below it quotients would meet subnormal numbers)
+
+__device__ __forceinline__ float bf16_bits(uint32_t hi) { return __uint_as_float(hi << 16); }
+__device__ __forceinline__ float lo_bf16(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_bf16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// ------------------------------------------------------------------ append
+// A thread has 8 neighbouring elements of one head of one row, 4 threads a group.  Products and sums of the rotation are rounded one by one, so that
+// the value which is cut to 4 bits does not depend on what the compiler contracts.
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int k = 0; k < 4; k++) x[2 * k] = lo_bf16(u[k]), x[2 * k + 1] = hi_bf16(u[k]);
+}
+struct Group { uint32_t codes; uint16_t scale; };
+__device__ __forceinline__ Group to_codes(const float (&x)[8]) {
+  float hi = x[0], lo = x[0];
+  uint32_t mag = 0;      // the largest magnitude's bits: those of infinities and NaN are the highest
+#pragma unroll
+  for (int e = 0; e < 8; e++) hi = fmaxf(hi, x[e]), lo = fminf(lo, x[e]), mag = max(mag, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, o));
+  }
+  const bf16 sb = __float2bfloat16_rn((hi > -lo ? hi : lo) * -0.125f);
+  const float s = __bfloat162float(sb);
+  Group g{0x88888888u, __bfloat16_as_ushort(sb)};
+  if (mag >= 0x7F800000u) {
+    g.scale = 0x7FC0;      // NaN
+  } else if (fabsf(s) < TINY) {
+    g.scale = 0;
+  } else {
+    g.codes = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int c = min(max(__float2int_rn(__fdiv_rn(x[e], s)) + 8, 0), 15);
+      g.codes |= (uint32_t)c << (4 * e);
+    }
+  }
+  return g;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(256) kv4_append_k(uint8_t* __restrict__ pages, bf16* __restrict__ q_out, const bf16* __restrict__ qkv,
+                                                    const int* __restrict__ slots, const int* __restrict__ pos, const float* __restrict__ cos,
+                                                    const float* __restrict__ sin, long n_pages, int page, unsigned total, long stride, int H, int Hkv, int T) {
+  mlb_pdl_sync();
+  using L = Block<HD>;
+  constexpr unsigned PER = HD / 8;
+  const unsigned heads = H + 2 * Hkv;
+  const unsigned at = blockIdx.x * 256u + threadIdx.x, idx = min(at, total - 1);      // (all lanes stay for the shuffles)
+  const unsigned t = idx % PER, head = idx / PER % heads, row = idx / PER / heads;
+  const bf16* src = qkv + (long)row * stride + (long)head * HD;
+  float x[8];
+  unpack8(*reinterpret_cast<const uint4*>(src + 8 * t), x);
+  if (cos != nullptr && head < (unsigned)(H + Hkv)) {
+    constexpr unsigned HALF = PER / 2;
+    int p = pos[row];
+    if (p < 0 || p >= T) {
+      if (t == 0 && head == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC3);
+      p = 0;
+    }
+    float y[8], c[8], s[8];
+    unpack8(*reinterpret_cast<const uint4*>(src + 8 * (t < HALF ? t + HALF : t - HALF)), y);
+    const long a = (long)p * (HD / 2) + 8 * (t < HALF ? t : t - HALF);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const float4 cv = *reinterpret_cast<const float4*>(cos + a + 4 * k), sv = *reinterpret_cast<const float4*>(sin + a + 4 * k);
+      c[4 * k] = cv.x, c[4 * k + 1] = cv.y, c[4 * k + 2] = cv.z, c[4 * k + 3] = cv.w;
+      s[4 * k] = sv.x, s[4 * k + 1] = sv.y, s[4 * k + 2] = sv.z, s[4 * k + 3] = sv.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float u = __fmul_rn(x[e], c[e]), v = __fmul_rn(y[e], s[e]);
+      x[e] = t < HALF ? __fsub_rn(u, v) : __fadd_rn(u, v);
+    }
+  }
+  const Group g = to_codes(x);
+  if (at >= total) return;
+  if (head < (unsigned)H) {
+    if (q_out != nullptr) {
+      const uint4 w = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+      *reinterpret_cast<uint4*>(q_out + ((long)row * H + head) * HD + 8 * t) = w;
+    }
+    return;
+  }
+  const int slot = slots[row];
+  if (slot < 0) return;
+  if (slot / page >= n_pages) {
+    if (t == 0 && head == (unsigned)H) mlb_set_error(MLB_ERR_BOUNDS, 0xC2);
+    return;
+  }
+  const bool value = head >= (unsigned)(H + Hkv);
+  const int kv = (int)head - H - (value ? Hkv : 0), off = slot % page, r = off % TOK;
+  uint8_t* b = pages + (((long)(slot / page) * Hkv + kv) * (page / TOK) + off / TOK) * L::BYTES;
+  const int j = t & 3, gi = t >> 2;
+  if (!value) {
+    *reinterpret_cast<uint32_t*>(b + r * L::ROW + 4 * (j * L::NG + gi)) = g.codes;
+  } else {
+    uint16_t* v = reinterpret_cast<uint16_t*>(b + L::V + r * L::ROW);
+    v[2 * j * L::NG + gi] = (uint16_t)g.codes;
+    v[(2 * j + 1) * L::NG + gi] = (uint16_t)(g.codes >> 16);
+  }
+  if (j == 0) *reinterpret_cast<uint16_t*>(b + (value ? L::VS : L::KS) + 2 * (r * L::NG + gi)) = g.scale;
+}
+
+// ------------------------------------------------------------------ read
+template <int HD>
+__global__ void __launch_bounds__(256) kv4_read_k(bf16* __restrict__ k, bf16* __restrict__ v, const uint8_t* __restrict__ pages, const int* __restrict__ slots,
+                                                  long n_pages, int page, unsigned total, int Hkv) {
+  mlb_pdl_sync();
+  using L = Block<HD>;
+  constexpr unsigned PER = HD / 8;
+  const unsigned idx = blockIdx.x * 256u + threadIdx.x;
+  if (idx >= total) return;
+  const unsigned t = idx % PER, kv = idx / PER % Hkv, row = idx / PER / Hkv;
+  const int slot = slots[row];
+  uint4 wk = {0, 0, 0, 0}, wv = wk;
+  if (slot >= 0 && slot / page >= n_pages) {
+    if (t == 0 && kv == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC2);
+  } else if (slot >= 0) {
+    const int off = slot % page, r = off % TOK, j = t & 3, gi = t >> 2;
+    const uint8_t* b = pages + (((long)(slot / page) * Hkv + kv) * (page / TOK) + off / TOK) * L::BYTES;
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(b + L::V + r * L::ROW);
+    const uint32_t ck = *reinterpret_cast<const uint32_t*>(b + r * L::ROW + 4 * (j * L::NG + gi));
+    const uint32_t cv = h[2 * j * L::NG + gi] | (uint32_t)h[(2 * j + 1) * L::NG + gi] << 16;
+    const float sk = bf16_bits(*reinterpret_cast<const uint16_t*>(b + L::KS + 2 * (r * L::NG + gi)));
+    const float sv = bf16_bits(*reinterpret_cast<const uint16_t*>(b + L::VS + 2 * (r * L::NG + gi)));
+    auto val = [](uint32_t c, int e, float s) { return __fmul_rn((float)((int)(c >> (4 * e) & 15) - 8), s); };
+    auto word = [&](uint32_t c, float s, int e) { return pack_bf16(val(c, e, s), val(c, e + 1, s)); };
+    wk = {word(ck, sk, 0), word(ck, sk, 2), word(ck, sk, 4), word(ck, sk, 6)};
+    wv = {word(cv, sv, 0), word(cv, sv, 2), word(cv, sv, 4), word(cv, sv, 6)};
+  }
+  *reinterpret_cast<uint4*>(k + 8L * idx) = wk;
+  *reinterpret_cast<uint4*>(v + 8L * idx) = wv;
+}
+
+// ------------------------------------------------------------------ attention
+// O[r] = sum_t p_rt (c_t - 8) s_t / sum_t p_rt,  p_rt = exp(scale q_r . k_t - m_r), over the tokens t that query row r sees; r runs over the G = H / Hkv
+// heads and the Tq tokens that share a key / value head, 8 NT of them at a time.
+//
+// Bound by the cache's bytes (4.5 bits an element), as long as an SM's 4 issue slots keep up with the 23 bytes a clock that reach it: 16 tokens of
+// 128 + 128 elements are 98 clocks, 390 instructions.  So the tensor cores do both products (mma.sync, tokens or elements as the 16 rows, query rows as
+// the 8 columns: tcgen05 would want 128 rows and its operands unpacked to shared memory), and codes go into them as the whole numbers they are:
+//   K: 128 + c is one bitwise instruction for two codes (the code put into the mantissa of 128).  The product starts from -136 sum(q) instead of
+//      subtracting 136 from each; every group's sum is scaled by s_t behind its two products, exactly, in fp32.
+//   V: c - 8 (one more instruction for two), with the scale in P, which is multiplied by it in fp32 before its one rounding to bf16.  That rounding,
+//      2^-8 of each weight at most and independent from token to token, is the only one on the way to O.
+// Scores stand transposed (token rows, query columns), so that softmax weights become the second product's operand by two matrix transpositions in
+// registers.  The running maximum m is the reference of all weights so far and moves only when a score passes it by 8 (weights up to 2^8, O and the
+// sums then rescaled): most blocks need a vote instead of two reductions over the warp.
+//
+// Work: all sequences' blocks of 16 tokens stand in one row of `total`, each thread block takes an equal piece of it whatever the lengths are, and its 4 warps
+// a quarter each of every sequence's share.  A warp fetches its own blocks by bulk copies through a ring of its own.  A head whose blocks are shared is
+// put together by the thread block that comes last, in the order of the pieces.
+struct AttnArgs {
+  bf16* out;
+  float* lse;
+  const bf16* q;
+  const uint8_t* pages;
+  const int *table, *lens;
+  float* part;
+  int* count;
+  long q_stride, n_pages;
+  int B, Tq, G, Hkv, width, page_log;
+  float scale_log2;            // > 0: a negative scale turns the queries' signs, and none makes them zeros
+  uint32_t q_keep, q_flip;
+};
+constexpr int WARPS = 4;
+constexpr int MAX_B = 2048;       // sequences of a launch: their first blocks' numbers stand in shared memory
+template <int HD> struct Ring { static constexpr int N = HD == 128 ? 5 : HD == 96 ? 6 : 8; };
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t codes128(uint32_t w) { return (w & 0x000F000Fu) | 0x43004300u; }      // two codes as bf16 128 + c
+__device__ __forceinline__ uint32_t codes_minus8(uint32_t w) {
+  const uint32_t x = codes128(w), k = 0x43084308u;      // 136
+  const bf162 y = __hsub2(*reinterpret_cast<const bf162*>(&x), *reinterpret_cast<const bf162*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int N> struct Words { uint32_t w[N]; };
+template <int N> __device__ __forceinline__ Words<N> load_words(const uint8_t* p) {      // N 32-bit words at a multiple of 4 N bytes (3: of 4)
+  Words<N> r;
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    r.w[0] = v.x, r.w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; k++) r.w[k] = *reinterpret_cast<const uint32_t*>(p + 4 * k);
+  }
+  return r;
+}
+template <int N> __device__ __forceinline__ void load_halves(const uint8_t* p, uint32_t (&h)[N]) {      // N 16-bit words: value h[g] in the low half
+  if constexpr (N % 2 == 0) {
+    const auto r = load_words<N / 2>(p);
+#pragma unroll
+    for (int k = 0; k < N; k++) h[k] = k % 2 ? r.w[k / 2] >> 16 : r.w[k / 2];
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; k++) h[k] = *reinterpret_cast<const uint16_t*>(p + 2 * k);
+  }
+}
+template <int N> __device__ __forceinline__ void load_scales(const uint8_t* p, float (&s)[N]) {
+  uint32_t h[N];
+  load_halves<N>(p, h);
+#pragma unroll
+  for (int k = 0; k < N; k++) s[k] = bf16_bits(h[k]);
+}
+
+template <int HD, int NT> struct Rows {      // a warp's share of 8 NT query rows
+  float o[NT][HD / 16][4];
+  float m[NT][2], neg[NT][2], l[NT][2];      // reference maximum, -m scale (0 where m = -inf), sum of this thread's tokens
+};
+template <int HD, int NT> struct Queries {
+  uint32_t b[NT][HD / 16][2];
+  float start[NT][HD / 32][2];      // -136 sum over a group of the query
+};
+
+// One block of 16 tokens.  first: its first token; seen[n][c]: tokens that column c sees; masked: not every column sees all 16.
+template <int HD, int NT>
+__device__ __forceinline__ void attend(Rows<HD, NT>& a, const Queries<HD, NT>& q, const uint8_t* blk, int first, bool masked, const int (&seen)[NT][2], float c,
+                                       int i, int j) {
+  using L = Block<HD>;
+  constexpr int NG = L::NG;
+  // Row r of the products is token r ^ (r / 2 & 1): the tokens whose values a lane reads are then of both parities in each load, half the conflicts
+  const int ta = i ^ (i >> 1 & 1), v0 = 2 * j + (j & 1), v1 = 2 * j + 1 - (j & 1);
+  float s[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int k = 0; k < 4; k++) s[n][k] = 0.f;
+  {
+    const auto ka = load_words<NG>(blk + ta * L::ROW + 4 * j * NG), kb = load_words<NG>(blk + (ta + 8) * L::ROW + 4 * j * NG);
+    float sa[NG], sb[NG];
+    load_scales<NG>(blk + L::KS + 2 * ta * NG, sa);
+    load_scales<NG>(blk + L::KS + 2 * (ta + 8) * NG, sb);
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      float d[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; n++) d[n][0] = d[n][2] = q.start[n][g][0], d[n][1] = d[n][3] = q.start[n][g][1];
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const uint32_t a0 = codes128(ka.w[g] >> 8 * k), a1 = codes128(kb.w[g] >> 8 * k), a2 = codes128(ka.w[g] >> (8 * k + 4)),
+                       a3 = codes128(kb.w[g] >> (8 * k + 4));
+#pragma unroll
+        for (int n = 0; n < NT; n++) mma16816(d[n], a0, a1, a2, a3, q.b[n][2 * g + k][0], q.b[n][2 * g + k][1]);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        s[n][0] = fmaf(sa[g], d[n][0], s[n][0]), s[n][1] = fmaf(sa[g], d[n][1], s[n][1]);
+        s[n][2] = fmaf(sb[g], d[n][2], s[n][2]), s[n][3] = fmaf(sb[g], d[n][3], s[n][3]);
+      }
+    }
+  }
+  const int t0 = first + ta, t1 = t0 + 8;
+  if (masked) {
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      if (t0 >= seen[n][0]) s[n][0] = -INFINITY;
+      if (t0 >= seen[n][1]) s[n][1] = -INFINITY;
+      if (t1 >= seen[n][0]) s[n][2] = -INFINITY;
+      if (t1 >= seen[n][1]) s[n][3] = -INFINITY;
+    }
+  }
+  bool grown = false;
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) grown |= (fmaxf(s[n][h], s[n][h + 2]) - a.m[n][h]) * c > 8.f;      // (m = -inf: true from the first score on)
+  if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float x = fmaxf(s[n][h], s[n][h + 2]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+        x = fmaxf(x, a.m[n][h]);
+        const float f = a.m[n][h] == x ? 1.f : ex2((a.m[n][h] - x) * c);      // (from -inf: 0)
+        a.m[n][h] = x;
+        a.neg[n][h] = x == -INFINITY ? 0.f : -x * c;
+        a.l[n][h] *= f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) a.o[n][d][h] *= f, a.o[n][d][h + 2] *= f;
+      }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      s[n][k] = ex2(fmaf(s[n][k], c, a.neg[n][k & 1]));
+      a.l[n][k & 1] += s[n][k];
+    }
+  float sa[NG], sb[NG];
+  load_scales<NG>(blk + L::VS + 2 * ta * NG, sa);
+  load_scales<NG>(blk + L::VS + 2 * (ta + 8) * NG, sb);
+  uint32_t w0[NG], w1[NG], w2[NG], w3[NG];
+  load_halves<NG>(blk + L::V + v0 * L::ROW + 2 * i * NG, w0);
+  load_halves<NG>(blk + L::V + v1 * L::ROW + 2 * i * NG, w1);
+  load_halves<NG>(blk + L::V + (v0 + 8) * L::ROW + 2 * i * NG, w2);
+  load_halves<NG>(blk + L::V + (v1 + 8) * L::ROW + 2 * i * NG, w3);
+#pragma unroll
+  for (int g = 0; g < NG; g++) {
+    uint32_t b0[NT], b1[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      float p[4] = {s[n][0] * sa[g], s[n][1] * sa[g], s[n][2] * sb[g], s[n][3] * sb[g]};
+      if (masked) {      // (a scale that no column sees may be anything)
+        if (t0 >= seen[n][0]) p[0] = 0.f;
+        if (t0 >= seen[n][1]) p[1] = 0.f;
+        if (t1 >= seen[n][0]) p[2] = 0.f;
+        if (t1 >= seen[n][1]) p[3] = 0.f;
+      }
+      b0[n] = transposed(pack_bf16(p[0], p[1]));
+      b1[n] = transposed(pack_bf16(p[2], p[3]));
+    }
+    const uint32_t x0 = __byte_perm(w0[g], w1[g], 0x5410), x1 = __byte_perm(w2[g], w3[g], 0x5410);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint32_t a0 = codes_minus8(x0 >> 8 * h), a1 = codes_minus8(x0 >> (8 * h + 4)), a2 = codes_minus8(x1 >> 8 * h), a3 = codes_minus8(x1 >> (8 * h + 4));
+#pragma unroll
+      for (int n = 0; n < NT; n++) mma16816(a.o[n][2 * g + h], a0, a1, a2, a3, b0[n], b1[n]);
+    }
+  }
+}
+
+template <int HD, int NT> constexpr int merge_floats() { return 8 * NT * (HD + 2); }
+template <int HD, int NT> constexpr int attn_ring() {      // bytes of the rings, and of the warps' shares that take their place
+  const int ring = WARPS * Ring<HD>::N * Block<HD>::BYTES, merge = WARPS * merge_floats<HD, NT>() * 4;
+  return ring > merge ? ring : merge;
+}
+template <int HD, int NT> int attn_smem(int B) { return attn_ring<HD, NT>() + (B + 1) * 4; }
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const AttnArgs A) {
+  using L = Block<HD>;
+  constexpr int NG = L::NG, NST = Ring<HD>::N, R = 8 * NT, PART = merge_floats<HD, NT>();
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[WARPS][NST];
+  __shared__ int scan[WARPS], last;
+  int* start = reinterpret_cast<int*>(smem + attn_ring<HD, NT>());
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane >> 2, j = lane & 3;
+  if (lane == 0) {
+    for (int k = 0; k < NST; k++) tc::mbar_init(&bars[warp][k], 1);
+    tc::mbar_fence_init();
+  }
+  mlb_pdl_sync();
+  // first blocks of the sequences, per key / value head: an empty one has a block of its own, which writes its zeros
+  const int longest = A.width << A.page_log;
+  int done = 0;
+  for (int b = 0; b < A.B; b += WARPS * 32) {
+    int n = 0;
+    if (b + tid < A.B) {
+      n = A.lens[b + tid];
+      if (n > longest && blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC4);
+      n = max(1, (min(n, longest) + TOK - 1) / TOK);
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    int before = done;
+    for (int w = 0; w < WARPS; w++) {
+      if (w < warp) before += scan[w];
+      done += scan[w];
+    }
+    if (b + tid < A.B) start[b + tid] = before + x - n;
+    __syncthreads();
+  }
+  if (tid == 0) start[A.B] = done;
+  __syncthreads();
+  const long total = (long)done * A.Hkv;
+  const long per = max((long)WARPS, (total + gridDim.x - 1) / gridDim.x);
+  long s = per * blockIdx.x;
+  const long e = min(total, s + per);
+  const int rows = A.G * A.Tq, row0 = blockIdx.y * R;
+  uint8_t* ring = smem + warp * NST * L::BYTES;
+  float* mrg = reinterpret_cast<float*>(smem);
+  const int bpl = A.page_log - 4;      // log2 of the blocks of a page
+  int count = 0;                       // blocks that this warp has taken from its ring
+  bool dead = false;
+  int b = 0;
+  if (s < e) {      // the sequence of the first block
+    int hi = A.B;
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if ((long)start[mid] * A.Hkv <= s) b = mid;
+      else hi = mid;
+    }
+  }
+  while (s < e) {
+    while ((long)start[b + 1] * A.Hkv <= s) b++;
+    const int nb = start[b + 1] - start[b];
+    const long base = (long)start[b] * A.Hkv;
+    const int kv = (int)((s - base) / nb);
+    const long item0 = base + (long)kv * nb, item1 = item0 + nb;
+    const int u0 = (int)(s - item0), u1 = (int)(min(e, item1) - item0);
+    const int len = max(0, min(A.lens[b], longest));
+
+    // ---- this warp's blocks [w0, w1)
+    const int w0 = u0 + (int)((long)(u1 - u0) * warp / WARPS), w1 = u0 + (int)((long)(u1 - u0) * (warp + 1) / WARPS);
+    Rows<HD, NT> acc;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) acc.o[n][d][k] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; h++) acc.m[n][h] = -INFINITY, acc.neg[n][h] = 0.f, acc.l[n][h] = 0.f;
+    }
+    if (w0 < w1 && len > 0) {
+      const int* trow = A.table + (long)b * A.width;
+      int have = -1, ids = 0;      // page numbers [have, have + 32) of the table, one a lane
+      uint32_t there = 0;          // blocks in the ring whose page is one of the pool
+      auto fetch = [&](int u, int n) {      // block u into place n
+        const int p = u >> bpl;
+        if (have < 0 || p >= have + 32) {
+          have = p;
+          ids = p + lane < A.width ? trow[p + lane] : -1;
+        }
+        const int id = __shfl_sync(0xffffffffu, ids, p - have);
+        const bool ok = id >= 0 && id < A.n_pages;
+        const int k = n % NST;
+        there = ok ? there | 1u << k : there & ~(1u << k);
+        if (lane == 0) {
+          if (ok) {
+            tc::mbar_expect_tx(&bars[warp][k], L::BYTES);
+            tc::bulk_load(ring + k * L::BYTES, A.pages + ((((long)id * A.Hkv + kv) << bpl) + (u & ((1 << bpl) - 1))) * L::BYTES, L::BYTES, &bars[warp][k]);
+          } else {
+            mlb_set_error(MLB_ERR_BOUNDS, 0xC1);
+            tc::mbar_arrive(&bars[warp][k]);
+          }
+        }
+      };
+      const int ahead = min(w1 - w0, NST);
+      if (!dead)
+        for (int k = 0; k < ahead; k++) fetch(w0 + k, count + k);
+      // ---- the queries, while the first blocks are on their way
+      Queries<HD, NT> q;
+      int seen[NT][2];
+      int all = len;      // tokens that every column sees
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const int r = row0 + 8 * n + i;
+        float sum[NG];
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+          uint4 w = {0, 0, 0, 0};
+          if (r < rows) w = *reinterpret_cast<const uint4*>(A.q + ((long)b * A.Tq + r / A.G) * A.q_stride + ((long)kv * A.G + r % A.G) * HD + 32 * g + 8 * j);
+          w.x = (w.x & A.q_keep) ^ A.q_flip, w.y = (w.y & A.q_keep) ^ A.q_flip, w.z = (w.z & A.q_keep) ^ A.q_flip, w.w = (w.w & A.q_keep) ^ A.q_flip;
+          q.b[n][2 * g][0] = __byte_perm(w.x, w.z, 0x5410), q.b[n][2 * g][1] = __byte_perm(w.x, w.z, 0x7632);
+          q.b[n][2 * g + 1][0] = __byte_perm(w.y, w.w, 0x5410), q.b[n][2 * g + 1][1] = __byte_perm(w.y, w.w, 0x7632);
+          float x[8];
+          unpack8(w, x);
+          float y = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; k++) y += x[k];
+          y += __shfl_xor_sync(0xffffffffu, y, 1);
+          y += __shfl_xor_sync(0xffffffffu, y, 2);
+          sum[g] = -136.f * y;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+          for (int g = 0; g < NG; g++) q.start[n][g][h] = __shfl_sync(0xffffffffu, sum[g], (2 * j + h) * 4);
+          const int col = row0 + 8 * n + 2 * j + h;
+          seen[n][h] = col < rows ? len - A.Tq + col / A.G + 1 : len;
+        }
+      }
+      if (row0 < rows) all = len - A.Tq + row0 / A.G + 1;      // (the first row of the tile sees the fewest)
+      for (int u = w0; u < w1 && !dead; u++, count++) {
+        const int k = count % NST;
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(&bars[warp][k], count / NST & 1, 0xD1))) {
+          dead = true;      // no more is fetched; what is on its way is waited for
+          for (int x = 1; x < min(NST, w1 - u); x++) tc::mbar_wait(&bars[warp][(count + x) % NST], (count + x) / NST & 1, 0xD2);
+          __syncwarp();
+          break;
+        }
+        if (there >> k & 1) attend<HD, NT>(acc, q, ring + k * L::BYTES, u * TOK, u * TOK + TOK > all, seen, A.scale_log2, i, j);
+        __syncwarp();
+        if (u + NST < w1) fetch(u + NST, count + NST);
+      }
+    }
+    // ---- the warps' shares put together (in the rings' memory, which nothing is on its way to)
+    __syncthreads();
+    float* mine = mrg + warp * PART;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float l = acc.l[n][h];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const int col = 8 * n + 2 * j + h;
+        if (i == 0) mine[col] = acc.m[n][h], mine[R + col] = l;
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+          *reinterpret_cast<float4*>(mine + 2 * R + col * HD + 32 * g + 4 * i) =
+              make_float4(acc.o[n][2 * g][h], acc.o[n][2 * g][h + 2], acc.o[n][2 * g + 1][h], acc.o[n][2 * g + 1][h + 2]);
+      }
+    __syncthreads();
+    const int live = min(R, rows - row0);
+    const long c0 = item0 / per, c1 = (item1 - 1) / per;      // the thread blocks that share this head
+    const int item = (int)(blockIdx.y * (long)A.B * A.Hkv + (long)b * A.Hkv + kv);
+    float* part = A.part + ((long)blockIdx.y * gridDim.x * 2) * PART;
+    float* my = part + (blockIdx.x * 2 + (s == per * blockIdx.x ? 0 : 1)) * (long)PART;
+    const int n_shares = (int)(c1 - c0 + 1);
+    auto finish = [&](int r, int d, float m, float l, const float4& o) {      // elements 4 d ... of row r, whole
+      const int head = kv * A.G + (row0 + r) % A.G, tok = (row0 + r) / A.G;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (nothing seen: zeros; NaN stays)
+      bf16* out = A.out + ((long)b * A.Tq + tok) * A.G * A.Hkv * HD + (long)head * HD + 4 * d;
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+      if (d == 0 && A.lse != nullptr)
+        A.lse[((long)b * A.G * A.Hkv + head) * A.Tq + tok] = l == 0.f ? -INFINITY : (m * A.scale_log2 + log2f(l)) * 0.693147180559945f;
+    };
+    for (int x = tid; x < live * (HD / 4); x += WARPS * 32) {
+      const int r = x / (HD / 4), d = x % (HD / 4);
+      float m = -INFINITY, l = 0.f;
+      for (int w = 0; w < WARPS; w++) m = fmaxf(m, mrg[w * PART + r]);
+      float4 o = {0, 0, 0, 0};
+      for (int w = 0; w < WARPS; w++) {
+        const float mw = mrg[w * PART + r], f = mw == m ? (m == -INFINITY ? 0.f : 1.f) : ex2((mw - m) * A.scale_log2);
+        const float4 v = *reinterpret_cast<const float4*>(mrg + w * PART + 2 * R + r * HD + 4 * d);
+        l = fmaf(f, mrg[w * PART + R + r], l);
+        o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+      }
+      if (n_shares > 1) {
+        if (d == 0) my[r] = m, my[R + r] = l;
+        *reinterpret_cast<float4*>(my + 2 * R + r * HD + 4 * d) = o;
+      } else {
+        finish(r, d, m, l, o);
+      }
+    }
+    if (n_shares > 1) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) last = atomicAdd(A.count + item, 1) == n_shares - 1;
+      __syncthreads();
+      if (last) {
+        __threadfence();
+        if (tid == 0) A.count[item] = 0;      // for the next call
+        for (int x = tid; x < live * (HD / 4); x += WARPS * 32) {
+          const int r = x / (HD / 4), d = x % (HD / 4);
+          auto share = [&](long c) { return part + (c * 2 + (c > c0 || item0 == c * per ? 0 : 1)) * (long)PART; };
+          float m = -INFINITY, l = 0.f;
+          for (long c = c0; c <= c1; c++) m = fmaxf(m, __ldcg(share(c) + r));
+          float4 o = {0, 0, 0, 0};
+          for (long c = c0; c <= c1; c++) {
+            const float* p = share(c);
+            const float mw = __ldcg(p + r), f = mw == m ? (m == -INFINITY ? 0.f : 1.f) : ex2((mw - m) * A.scale_log2);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + 2 * R + r * HD + 4 * d));
+            l = fmaf(f, __ldcg(p + R + r), l);
+            o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+          }
+          finish(r, d, m, l, o);
+        }
+      }
+    }
+    tc::fence_async_smem();      // (bulk copies will write where the shares were)
+    __syncthreads();
+    s = min(e, item1);
+  }
+}
+
+template <int HD, int NT>
+cudaError_t launch_attn(const AttnArgs& a, int grid, int tiles, cudaStream_t st) {
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = mlb_allow_smem(kv4_attn_k<HD, NT>, attn_smem<HD, NT>(MAX_B), allowed);
+  if (e != cudaSuccess) return e;
+  return mlb_launch(kv4_attn_k<HD, NT>, dim3(grid, tiles), dim3(WARPS * 32), attn_smem<HD, NT>(a.B), st, a);
+}
+bool known_head(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128; }
+int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1; }
+// query rows a thread block takes at a time: 8 where that is all of them, else 16
+int row_tiles(long rows, int& nt) {
+  nt = rows <= 8 ? 1 : 2;
+  return (int)((rows + 8 * nt - 1) / (8 * nt));
+}
+int attn_grid(long B, int Hkv, int width, int page, int nt) {
+  const long most = B * Hkv * (((long)width * page + TOK - 1) / TOK);      // (a thread block has a block of tokens for each warp)
+  const long all = (nt == 1 ? 4 : 3) * (long)mlb_sm_count(), want = (most + WARPS - 1) / WARPS;
+  return (int)(want < all ? (want > 0 ? want : 1) : all);
+}
+#define MLB_BY_HEAD(hd, F) \
+  switch (hd) {            \
+    case 32: F(32); break; \
+    case 64: F(64); break; \
+    case 96: F(96); break; \
+    default: F(128);       \
+  }
+
+}  // namespace
+
+// qkv[N] rows of (H + 2 Hkv) heads, `stride` elements apart: queries (and keys) rotated by cos / sin[pos] (null: not) go to q_out[N, H hd] (null: nowhere), keys and
+// values to the slots of the pool; a negative slot is none.  Returns -7 for what the kernel does not take.
+MLB_API int mlb_kv4_append(uint8_t* pages, void* q_out, const void* qkv, const int* slots, const int* pos, const float* cos, const float* sin, long n_pages,
+                           int page, long N, long stride, int H, int Hkv, int hd, int T, cudaStream_t st) {
+  if (!known_head(hd) || page_shift(page) < 0 || stride % 8 != 0 || H < 0 || Hkv < 1) return -7;
+  const long per_row = (long)(H + 2 * Hkv) * (hd / 8), rows = (1L << 30) / per_row;
+  if (rows < 1) return -7;
+  cudaError_t e = cudaSuccess;
+  for (long r = 0; r < N && e == cudaSuccess; r += rows) {
+    const unsigned total = (unsigned)((N - r < rows ? N - r : rows) * per_row);
+#define MLB_GO(HD)                                                                                                                            \
+  e = mlb_launch(kv4_append_k<HD>, dim3((total + 255) / 256), dim3(256), 0, st, pages, q_out ? (bf16*)q_out + r * H * HD : nullptr,          \
+                 (const bf16*)qkv + r * stride, slots + r, cos ? pos + r : nullptr, cos, sin, n_pages, page, total, stride, H, Hkv, T)
+    MLB_BY_HEAD(hd, MLB_GO)
+#undef MLB_GO
+  }
+  return (int)e;
+}
+
+// k, v[N, Hkv, hd]: what the slots hold; zeros for a negative slot
+MLB_API int mlb_kv4_read(void* k, void* v, const uint8_t* pages, const int* slots, long n_pages, int page, long N, int Hkv, int hd, cudaStream_t st) {
+  if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1) return -7;
+  const long per_row = (long)Hkv * (hd / 8), rows = (1L << 30) / per_row;
+  if (rows < 1) return -7;
+  cudaError_t e = cudaSuccess;
+  for (long r = 0; r < N && e == cudaSuccess; r += rows) {
+    const unsigned total = (unsigned)((N - r < rows ? N - r : rows) * per_row);
+#define MLB_GO(HD)                                                                                                                            \
+  e = mlb_launch(kv4_read_k<HD>, dim3((total + 255) / 256), dim3(256), 0, st, (bf16*)k + r * Hkv * HD, (bf16*)v + r * Hkv * HD, pages, slots + r, \
+                 n_pages, page, total, Hkv)
+    MLB_BY_HEAD(hd, MLB_GO)
+#undef MLB_GO
+  }
+  return (int)e;
+}
+
+// fp32 words of workspace that attention wants, and (negative) nothing for sizes that it does not take; counters: B Hkv row tiles, zero before the first call
+MLB_API long mlb_kv4_attn_scratch(int B, int Tq, int H, int Hkv, int hd, int width, int page) {
+  if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1 || H % Hkv != 0) return -7;
+  int nt;
+  const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
+  return (long)attn_grid(B < MAX_B ? B : MAX_B, Hkv, width, page, nt) * tiles * 2 * 8 * nt * (hd + 2);
+}
+// out[B Tq, H hd] = attention of q (rows `q_stride` elements apart) over table[B, width], lens[B] tokens each; lse[B, H, Tq] or null
+MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pages, const int* table, const int* lens, float* part, int* count, long n_pages,
+                         long q_stride, int B, int Tq, int H, int Hkv, int hd, int width, int page, float scale, cudaStream_t st) {
+  const int shift = page_shift(page);
+  if (!known_head(hd) || shift < 0 || Hkv < 1 || H % Hkv != 0 || q_stride % 8 != 0) return -7;
+  int nt;
+  const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
+  if (tiles > 65535) return -7;
+  cudaError_t e = cudaSuccess;
+  for (int b = 0; b < B && e == cudaSuccess; b += MAX_B) {
+    const int n = B - b < MAX_B ? B - b : MAX_B;
+    const AttnArgs a{(bf16*)out + (long)b * Tq * H * hd, lse ? lse + (long)b * H * Tq : nullptr, (const bf16*)q + (long)b * Tq * q_stride, pages,
+                     table + (long)b * width, lens + b, part, count, q_stride, n_pages, n, Tq, H / Hkv, Hkv, width, shift, (scale == 0.f ? 1.f : fabsf(scale)) * 1.44269504088896f,
+                     scale == 0.f ? 0u : ~0u, scale < 0.f ? 0x80008000u : 0u};
+    const int grid = attn_grid(n, Hkv, width, page, nt);
+#define MLB_GO(HD) e = nt == 1 ? launch_attn<HD, 1>(a, grid, tiles, st) : launch_attn<HD, 2>(a, grid, tiles, st)
+    MLB_BY_HEAD(hd, MLB_GO)
+#undef MLB_GO
+  }
+  return (int)e;
+}

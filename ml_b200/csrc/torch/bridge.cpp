@@ -76,8 +76,18 @@ typedef std::optional<Tensor> Maybe;      // (an undefined tensor is no argument
   X(mlb_embed_bwd, int, (float*, const void*, const int*, long, int, int, int, int, St))                                                       \
   X(mlb_adamw, int, (float*, void*, const float*, float*, float*, long, float, float, float, float, float, float, float, float, const float*, St)) \
   X(mlb_sum_scale, int, (float*, const float*, long, float, St))
+// those of generation (the 4-bit cache, tables, beams)
+#define MLB_GENERATION(X)                                                                                                                      \
+  X(mlb_kv4_append, int, (uint8_t*, void*, const void*, const int*, const int*, const float*, const float*, long, int, long, long, int, int, int, int, St)) \
+  X(mlb_kv4_read, int, (void*, void*, const uint8_t*, const int*, long, int, long, int, int, St))                                              \
+  X(mlb_kv4_attn_scratch, long, (int, int, int, int, int, int, int))                                                                           \
+  X(mlb_kv4_attn, int, (void*, float*, const void*, const uint8_t*, const int*, const int*, float*, int*, long, long, int, int, int, int, int, int, int, float, St)) \
+  X(mlb_block_tables, int, (int*, int*, int*, int*, int*, int*, int*, const int*, const int*, const int*, const int*, int, int, int, int, int, St)) \
+  X(mlb_beam_select_pieces, int, (int, int, int))                                                                                              \
+  X(mlb_beam_select, int, (float*, int*, int*, int*, const void*, const float*, const int*, float*, float*, int*, int*, int, int, int, long, int, int, St)) \
+  X(mlb_beam_reorder, int, (uint8_t*, int*, int*, int*, const int*, const int*, const int*, const int*, const int*, const int*, int, long, int, int, int, int, int, int, int, St))
 #define MLB_POINTER(name, ret, args) ret(*name) args = nullptr;
-struct Entries { MLB_ENTRIES(MLB_POINTER) } K;
+struct Entries { MLB_ENTRIES(MLB_POINTER) MLB_GENERATION(MLB_POINTER) } K;
 
 PyObject* address_type = nullptr;  // ops.native.Address
 PyObject* settings = nullptr;      // the Python module whose variables FUSED_ATTN_BWD and FUSED_ATTN_BWD_MAX_SCRATCH bound attn_bwd's workspace
@@ -546,6 +556,7 @@ template <typename R, typename... A> struct typed_call<R(A...)> {
     END_HANDLE_TH_ERRORS                                                       \
   }
 MLB_ENTRIES(MLB_CALL)
+MLB_GENERATION(MLB_CALL)
 
 // bind(path, settings): the kernel library whose functions are called, the module with the variables above
 PyObject* py_bind(PyObject*, PyObject* args) {
@@ -559,6 +570,7 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   K.name = (ret(*) args)dlsym(h, #name);                             \
   TORCH_CHECK(K.name != nullptr, p, " has no function " #name);
   MLB_ENTRIES(MLB_LOOKUP)
+  MLB_GENERATION(MLB_LOOKUP)
   PyObject* address = PyObject_GetAttrString(module, "Address");
   if (!address) return nullptr;
   Py_XDECREF(address_type);
@@ -570,12 +582,19 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
-// signatures(): every entry point's parameters by name
+// signatures(), generation_signatures(): the entry points' parameters by name
+#define MLB_KINDS(name, ret, args) d[#name] = kinds_of(K.name);
 PyObject* py_signatures(PyObject*, PyObject*) {
   HANDLE_TH_ERRORS
   pybind11::dict d;
-#define MLB_KINDS(name, ret, args) d[#name] = kinds_of(K.name);
   MLB_ENTRIES(MLB_KINDS)
+  return d.release().ptr();
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_generation_signatures(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  pybind11::dict d;
+  MLB_GENERATION(MLB_KINDS)
   return d.release().ptr();
   END_HANDLE_TH_ERRORS
 }
@@ -583,7 +602,8 @@ PyObject* py_signatures(PyObject*, PyObject*) {
 #define MLB_FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 #define MLB_METHOD(name, ret, args) {#name, (PyCFunction)(void (*)(void))call_##name, METH_FASTCALL, nullptr},
 PyMethodDef methods[] = {MLB_FAST(linear), MLB_FAST(rmsnorm), MLB_FAST(layer_norm), MLB_FAST(swiglu), MLB_FAST(rope_causal_attention), MLB_FAST(bidir_attention),
-                         MLB_FAST(cross_entropy), MLB_ENTRIES(MLB_METHOD) {"bind", py_bind, METH_VARARGS, nullptr}, {"signatures", py_signatures, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+                         MLB_FAST(cross_entropy), MLB_ENTRIES(MLB_METHOD) MLB_GENERATION(MLB_METHOD) {"bind", py_bind, METH_VARARGS, nullptr}, {"signatures", py_signatures, METH_NOARGS, nullptr},
+                         {"generation_signatures", py_generation_signatures, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mlb_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

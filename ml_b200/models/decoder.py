@@ -474,34 +474,54 @@ class GPT:
         return self.mean_loss(B=B, valid_tokens=valid)
 
     @torch.no_grad()
-    def generate(self, prompt: torch.Tensor, n_new: int, temperature: float = 0.0, top_k: int = 0, seed: int = 0) -> torch.Tensor:
+    def generate(self, prompt: torch.Tensor, n_new: int, temperature: float = 0.0, top_k: int = 0, seed: int = 0, kv: Optional[str] = None,
+                 beams: int = 1, eos: int = -1, page: int = 64, length_penalty: float = 0.0) -> torch.Tensor:
         """Continues `prompt` [b, P] (token ids, b <= B, P >= 1) by `n_new` tokens with the training forward pass: every
         new token is one forward over the whole window (there is no key / value cache - this is a way to look at what a
         checkpoint has learnt, not a serving path), the window slides once it is full.  temperature 0 = greedy; else
         softmax sampling at that temperature, over the `top_k` most likely tokens if top_k > 0, from a generator seeded
-        with `seed`.  The reference has no sampling mode; needs materialised logits (no chunked LM head)."""
-        if self.logits is None:
-            raise ValueError("generate() reads the [B*T, V] logits: build the model without lmce_chunk")
+        with `seed`.  The reference has no sampling mode; needs materialised logits (no chunked LM head).
+
+        kv="4bit": keys and values are cached in 4 bits, in pages of `page` tokens (ml_b200.models.generation): a token costs one pass over itself, any
+        number of prompts, P + n_new within the window.  beams > 1 (with the cache): the most likely of `beams` continuations that are
+        carried along, ended by `eos` (-1: never) and compared by log-probability / length ** length_penalty."""
         c = self.cfg
         b, P = prompt.shape
+        gen = torch.Generator(device="cpu").manual_seed(seed)
+
+        def choose(logits):
+            if temperature <= 0:
+                return logits.argmax(-1)
+            logits = logits / temperature
+            if top_k > 0:
+                kth = logits.topk(min(top_k, c.V), dim=-1).values[:, -1:]
+                logits = logits.masked_fill(logits < kth, float("-inf"))
+            return torch.multinomial(torch.softmax(logits, -1).cpu(), 1, generator=gen).view(-1).to(self.device)
+
+        if kv not in (None, "4bit"):
+            raise ValueError(f"kv={kv!r}: None or '4bit'")
+        if kv is not None:
+            from . import generation
+            if b < 1 or P < 1 or n_new < 0:
+                raise ValueError(f"{b} prompts of {P} tokens, {n_new} more")
+            if beams > 1 and n_new:
+                if temperature > 0:
+                    raise ValueError("beams and sampling exclude each other")
+                return generation.beam_search(self, prompt, n_new, beams, eos, page, length_penalty)[0][:, 0]
+            return generation.sample(self, prompt, n_new, choose, page)
+        if beams != 1:
+            raise ValueError("beams need the cache: kv='4bit'")
+        if self.logits is None:
+            raise ValueError("generate() reads the [B*T, V] logits: build the model without lmce_chunk")
         assert 1 <= b <= self.B and P >= 1
         out = prompt.to(self.device).long()
-        gen = torch.Generator(device="cpu").manual_seed(seed)
         ids = torch.zeros(b, c.T, dtype=torch.int32, device=self.device)
         for _ in range(n_new):
             ctx = out[:, -c.T:]
             n = ctx.shape[1]
             ids.zero_()
             ids[:, :n] = ctx.to(torch.int32)       # positions past n hold padding: causal attention keeps it out of row n - 1
-            logits = self.forward(ids.view(-1), B=b).view(b, c.T, c.V)[:, n - 1].float()
-            if temperature <= 0:
-                nxt = logits.argmax(-1)
-            else:
-                logits = logits / temperature
-                if top_k > 0:
-                    kth = logits.topk(min(top_k, c.V), dim=-1).values[:, -1:]
-                    logits = logits.masked_fill(logits < kth, float("-inf"))
-                nxt = torch.multinomial(torch.softmax(logits, -1).cpu(), 1, generator=gen).view(-1).to(self.device)
+            nxt = choose(self.forward(ids.view(-1), B=b).view(b, c.T, c.V)[:, n - 1].float())
             out = torch.cat([out, nxt.view(b, 1)], dim=1)
         return out
 

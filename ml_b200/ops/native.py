@@ -41,7 +41,15 @@ _KINDS = {
     "attn_bwd_scratch_bytes": "nnnn", "attn_bwd": "bbbbffbnnnnffs", "attn_bwd_have_delta": "bbbbffbnnnnffs",
     "attn_bidir_fwd": "bfbnnnns", "attn_bidir_bwd": "bbbbffnnnns", "ce_mean": "fffbbilns", "ce_fwd_bwd": "fbilnldns",
     "scale_dev": "bbfls", "embed_fwd": "bbilnns", "embed_bwd": "fbilnnnns", "adamw": "fbffflddddddddfs", "sum_scale": "fflds"}
+# ... and those of generation: the 4-bit key / value cache, tables, beams (ops/native_gen.py)
+_GEN_KINDS = {
+    "kv4_append": "ubbiifflnllnnnns", "kv4_read": "bbuilnlnns", "kv4_attn_scratch": "nnnnnnn", "kv4_attn": "bfbuiifillnnnnnnnds",
+    "block_tables": "iiiiiiiiiiinnnnns", "beam_select_pieces": "nnn", "beam_select": "fiiibfiffiinnnlnns",
+    "beam_reorder": "uiiiiiiiiinlnnnnnnns"}
 _CTYPES = {"n": _i32, "l": _i64, "d": _f32}      # (else a pointer)
+
+
+_ERROR_WORDS = ("gemm", "attn", "elementwise", "comm", "kv4", "beam")      # one of each source of kernels
 
 
 @lru_cache(maxsize=1)
@@ -86,14 +94,14 @@ def lib():
         "mlb_cast_bf16_fp8": [_vp, _vp, _i64, _f32, _vp],
         "mlb_adamw_fp8": [_vp] * 6 + [_i64] + [_f32] * 9 + [_vp, _vp],
     }
-    sig.update({"mlb_" + name: [_CTYPES.get(k, _vp) for k in kinds] for name, kinds in _KINDS.items()})
+    sig.update({"mlb_" + name: [_CTYPES.get(k, _vp) for k in kinds] for name, kinds in {**_KINDS, **_GEN_KINDS}.items()})
     for name, args in sig.items():
         fn = getattr(L, name)
         fn.argtypes = args
         fn.restype = _i32
-    L.mlb_attn_bwd_scratch_bytes.restype = _i64
+    L.mlb_attn_bwd_scratch_bytes.restype = L.mlb_kv4_attn_scratch.restype = _i64
     L.mlb_capture_id.restype = C.c_ulonglong
-    for tag in ("gemm", "attn", "elementwise", "comm"):
+    for tag in _ERROR_WORDS:
         for pre in ("mlb_get_error_", "mlb_clear_error_"):
             if hasattr(L, pre + tag):
                 getattr(L, pre + tag).restype = _i32
@@ -183,7 +191,7 @@ def _cuda_err(rc):
 def get_error() -> int:
     """Non-zero if a kernel gave up on a bounded wait: (code << 24) | detail, see csrc/common.cuh."""
     L = lib()
-    for tag in ("gemm", "attn", "elementwise", "comm"):
+    for tag in _ERROR_WORDS:
         if hasattr(L, "mlb_get_error_" + tag):
             v = getattr(L, "mlb_get_error_" + tag)()
             if v:
@@ -195,6 +203,11 @@ _ERR_CODES = {1: "an mbarrier wait inside a kernel's pipeline ran out", 2: "a wa
               3: "an index was out of range"}
 _ERR_BOUNDS = {0xE1: "token id outside the vocabulary (embedding forward)", 0xE2: "token id outside the vocabulary (embedding backward)",
                0xCE: "target outside the vocabulary (cross-entropy)",
+               0xB1: "request of negative length, of more new tokens than the slot map has places, or more free pages than the stack (block tables)",
+               0xB2: "more new tokens than the slot map has places (block tables)", 0xB3: "parent that is no beam of the request (beam reordering)",
+               0xB4: "page outside the pool (beam reordering)", 0xC1: "page outside the pool (attention over the 4-bit cache)",
+               0xC2: "slot outside the pool (4-bit cache)", 0xC3: "position outside the rotary tables (4-bit cache)",
+               0xC4: "sequence longer than its row of the block table (attention over the 4-bit cache)",
                0xA1: "shared memory of the attention backward (head size 128) does not start on a 1024-byte boundary",
                0xA2: "shared memory of the attention backward (head size 64) does not start on a 1024-byte boundary"}
 
@@ -222,7 +235,7 @@ def read_errors_async(host_words: torch.Tensor):
 
 def clear_error():
     L = lib()
-    for tag in ("gemm", "attn", "elementwise", "comm"):
+    for tag in _ERROR_WORDS:
         if hasattr(L, "mlb_clear_error_" + tag):
             getattr(L, "mlb_clear_error_" + tag)()
 
@@ -246,7 +259,7 @@ class _Ctypes:
     """The entry points as the extension module has them, through ctypes."""
 
     def __getattr__(self, name):
-        fn, kinds, to = getattr(lib(), name), _KINDS[name[4:]], {"b": _b, "f": _f, "i": _i, "u": _u8}
+        fn, kinds, to = getattr(lib(), name), _KINDS.get(name[4:]) or _GEN_KINDS[name[4:]], {"b": _b, "f": _f, "i": _i, "u": _u8}
 
         def call(*args):
             a = [to[k](x) if k in to and type(x) is not Address else x for k, x in zip(kinds, args, strict=kinds[-1] != "s")]
@@ -769,3 +782,7 @@ def zero_(x):
 
 def scale_(x, s):
     _chk(lib().mlb_scale_f32(_f(x), x.numel(), s, _st()), "scale_f32")
+
+
+# ------------------------------------------------------------------ generation
+from .native_gen import beam_reorder, beam_select, block_tables, kv4_append, kv4_attn, kv4_read  # noqa: E402,F401

@@ -406,3 +406,6 @@ def sum_scale(out, x, scale):
 
 def zero_(x):
     x.zero_()
+
+
+from .ref_gen import beam_reorder, beam_select, block_tables, kv4_append, kv4_attn, kv4_read  # noqa: E402,F401
