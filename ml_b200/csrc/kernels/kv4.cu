@@ -8,6 +8,8 @@
 // The order in a row is that of the matrix instructions' registers in the attention kernel (lane = 4 i + j):
 //   key row:   32-bit word j NG + g has the elements 32 g + 8 j + e, e = 0..7, in its e-th four bits
 //   value row: 16-bit word i NG + g has the elements 32 g + 4 i + e, e = 0..3
+#include <cuda_fp16.h>
+
 #include "tc.cuh"
 
 namespace {
@@ -164,14 +166,17 @@ __global__ void __launch_bounds__(256) kv4_read_k(bf16* __restrict__ k, bf16* __
 //
 // Bound by the cache's bytes (4.5 bits an element), as long as an SM's 4 issue slots keep up with the 23 bytes a clock that reach it: 16 tokens of
 // 128 + 128 elements are 98 clocks, 390 instructions.  So the tensor cores do both products (mma.sync, tokens or elements as the 16 rows, query rows as
-// the 8 columns: tcgen05 would want 128 rows and its operands unpacked to shared memory), and codes go into them as the whole numbers they are:
-//   K: 128 + c is one bitwise instruction for two codes (the code put into the mantissa of 128).  The product starts from -136 sum(q) instead of
-//      subtracting 136 from each; every group's sum is scaled by s_t behind its two products, exactly, in fp32.
-//   V: c - 8 (one more instruction for two), with the scale in P, which is multiplied by it in fp32 before its one rounding to bf16.  That rounding,
-//      2^-8 of each weight at most and independent from token to token, is the only one on the way to O.
+// the 8 columns: tcgen05 would want 128 rows and its operands unpacked to shared memory).  What the codes become is as few instructions as can be:
+//   K: four bits at the bottom of a 16-bit word are the fp16 number c 2^-24, the next four c 2^-20 (both subnormal, both exact), so one bitwise instruction
+//      makes two operands and only the upper byte's codes need a shift; the factor 16 is taken out of the queries, which a power of two of each row brings to fp16
+//      exactly.  The product starts from -8 sum(q) instead of subtracting 8 from each code; every group's sum is scaled by s_t behind its two
+//      products, in fp32.  (The tensor core lines products up by their operands' nominal exponents, 2^-14 for a subnormal: a score is off by some 2^-16 of |q| s.)
+//   V: the bits put into the mantissa of 128 in bf16, less 136: c - 8 by two instructions for two codes, so that what is 0 adds 0.  The scale goes into P, in
+//      fp32 before its one rounding to bf16 (which has the range for weights and scales of any size).  That rounding, 2^-8 of each weight at most and independent
+//      from token to token, is the only one on the way to O.
 // Scores stand transposed (token rows, query columns), so that softmax weights become the second product's operand by two matrix transpositions in
-// registers.  The running maximum m is the reference of all weights so far and moves only when a score passes it by 8 (weights up to 2^8, O and the
-// sums then rescaled): most blocks need a vote instead of two reductions over the warp.
+// registers.  The largest score m is the reference of all weights so far and moves only when a score passes it by 2^8 (O and the sums are then rescaled): most
+// blocks need a vote instead of reductions over the warp.
 //
 // Work: all sequences' blocks of 16 tokens stand in one row of `total`, each thread block takes an equal piece of it whatever the lengths are, and its 4 warps
 // a quarter each of every sequence's share.  A warp fetches its own blocks by bulk copies through a ring of its own.  A head whose blocks are shared is
@@ -193,7 +198,14 @@ constexpr int WARPS = 4;
 constexpr int MAX_B = 2048;       // sequences of a launch: their first blocks' numbers stand in shared memory
 template <int HD> struct Ring { static constexpr int N = HD == 128 ? 5 : HD == 96 ? 6 : 8; };
 
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// D = A B + C: keys' codes and queries in fp16, values' codes and weights in bf16
+__device__ __forceinline__ void mma_keys(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2,
+                                         float c3) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ void mma_values(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -203,11 +215,16 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t codes128(uint32_t w) { return (w & 0x000F000Fu) | 0x43004300u; }      // two codes as bf16 128 + c
-__device__ __forceinline__ uint32_t codes_minus8(uint32_t w) {
-  const uint32_t x = codes128(w), k = 0x43084308u;      // 136
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000F000Fu; }       // two codes as fp16 c 2^-24
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00F000F0u; }      // c 2^-20
+__device__ __forceinline__ uint32_t value_codes(uint32_t w) {      // two codes as bf16 c - 8
+  const uint32_t x = low_codes(w) | 0x43004300u, k = 0x43084308u;      // 128 + c, 136
   const bf162 y = __hsub2(*reinterpret_cast<const bf162*>(&x), *reinterpret_cast<const bf162*>(&k));
   return *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -248,26 +265,23 @@ template <int N> __device__ __forceinline__ void load_scales(const uint8_t* p, f
 
 template <int HD, int NT> struct Rows {      // a warp's share of 8 NT query rows
   float o[NT][HD / 16][4];
-  float m[NT][2], neg[NT][2], l[NT][2];      // reference maximum, -m scale (0 where m = -inf), sum of this thread's tokens
+  float m[NT][2], neg[NT][2], l[NT][2];      // largest score (scaled), -m (NONE before the first one), sum of this thread's tokens
 };
+constexpr float NONE = 1e30f;      // in place of -m: any score passes it, and -inf with it is -inf
 template <int HD, int NT> struct Queries {
   uint32_t b[NT][HD / 16][2];
-  float start[NT][HD / 32][2];      // -136 sum over a group of the query
+  float start[NT][HD / 32][2];      // -8 2^-24 sum over a group of the query
+  float c[NT][2];                   // score = c * product
 };
 
 // One block of 16 tokens.  first: its first token; seen[n][c]: tokens that column c sees; masked: not every column sees all 16.
 template <int HD, int NT>
-__device__ __forceinline__ void attend(Rows<HD, NT>& a, const Queries<HD, NT>& q, const uint8_t* blk, int first, bool masked, const int (&seen)[NT][2], float c,
-                                       int i, int j) {
+__device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q, const uint8_t* blk, int first, bool masked, const int (&seen)[NT][2], int i, int j) {
   using L = Block<HD>;
   constexpr int NG = L::NG;
   // Row r of the products is token r ^ (r / 2 & 1): the tokens whose values a lane reads are then of both parities in each load, half the conflicts
   const int ta = i ^ (i >> 1 & 1), v0 = 2 * j + (j & 1), v1 = 2 * j + 1 - (j & 1);
   float s[NT][4];
-#pragma unroll
-  for (int n = 0; n < NT; n++)
-#pragma unroll
-    for (int k = 0; k < 4; k++) s[n][k] = 0.f;
   {
     const auto ka = load_words<NG>(blk + ta * L::ROW + 4 * j * NG), kb = load_words<NG>(blk + (ta + 8) * L::ROW + 4 * j * NG);
     float sa[NG], sb[NG];
@@ -275,61 +289,59 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& a, const Queries<HD, NT>& q
     load_scales<NG>(blk + L::KS + 2 * (ta + 8) * NG, sb);
 #pragma unroll
     for (int g = 0; g < NG; g++) {
-      float d[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; n++) d[n][0] = d[n][2] = q.start[n][g][0], d[n][1] = d[n][3] = q.start[n][g][1];
-#pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const uint32_t a0 = codes128(ka.w[g] >> 8 * k), a1 = codes128(kb.w[g] >> 8 * k), a2 = codes128(ka.w[g] >> (8 * k + 4)),
-                       a3 = codes128(kb.w[g] >> (8 * k + 4));
-#pragma unroll
-        for (int n = 0; n < NT; n++) mma16816(d[n], a0, a1, a2, a3, q.b[n][2 * g + k][0], q.b[n][2 * g + k][1]);
-      }
+      const uint32_t xa = ka.w[g], xb = kb.w[g], ya = xa >> 8, yb = xb >> 8;
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        s[n][0] = fmaf(sa[g], d[n][0], s[n][0]), s[n][1] = fmaf(sa[g], d[n][1], s[n][1]);
-        s[n][2] = fmaf(sb[g], d[n][2], s[n][2]), s[n][3] = fmaf(sb[g], d[n][3], s[n][3]);
+        float d[4];
+        const float s0 = q.start[n][g][0], s1 = q.start[n][g][1];
+        mma_keys(d, low_codes(xa), low_codes(xb), high_codes(xa), high_codes(xb), q.b[n][2 * g][0], q.b[n][2 * g][1], s0, s1, s0, s1);
+        mma_keys(d, low_codes(ya), low_codes(yb), high_codes(ya), high_codes(yb), q.b[n][2 * g + 1][0], q.b[n][2 * g + 1][1], d[0], d[1], d[2], d[3]);
+        s[n][0] = g ? fmaf(sa[g], d[0], s[n][0]) : sa[g] * d[0], s[n][1] = g ? fmaf(sa[g], d[1], s[n][1]) : sa[g] * d[1];
+        s[n][2] = g ? fmaf(sb[g], d[2], s[n][2]) : sb[g] * d[2], s[n][3] = g ? fmaf(sb[g], d[3], s[n][3]) : sb[g] * d[3];
       }
     }
   }
   const int t0 = first + ta, t1 = t0 + 8;
   if (masked) {
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-      if (t0 >= seen[n][0]) s[n][0] = -INFINITY;
-      if (t0 >= seen[n][1]) s[n][1] = -INFINITY;
-      if (t1 >= seen[n][0]) s[n][2] = -INFINITY;
-      if (t1 >= seen[n][1]) s[n][3] = -INFINITY;
-    }
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (t0 >= seen[n][h]) s[n][h] = -INFINITY;
+        if (t1 >= seen[n][h]) s[n][h + 2] = -INFINITY;
+      }
   }
-  bool grown = false;
+  float y[NT][4], top = -INFINITY;
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int h = 0; h < 2; h++) grown |= (fmaxf(s[n][h], s[n][h + 2]) - a.m[n][h]) * c > 8.f;      // (m = -inf: true from the first score on)
-  if (__any_sync(0xffffffffu, grown)) {
+    for (int k = 0; k < 4; k++) y[n][k] = fmaf(s[n][k], q.c[n][k & 1], r.neg[n][k & 1]), top = fmaxf(top, y[n][k]);
+  if (__any_sync(0xffffffffu, top > 8.f)) {
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        float x = fmaxf(s[n][h], s[n][h + 2]);
+        float x = fmaxf(s[n][h], s[n][h + 2]) * q.c[n][h];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-        x = fmaxf(x, a.m[n][h]);
-        const float f = a.m[n][h] == x ? 1.f : ex2((a.m[n][h] - x) * c);      // (from -inf: 0)
-        a.m[n][h] = x;
-        a.neg[n][h] = x == -INFINITY ? 0.f : -x * c;
-        a.l[n][h] *= f;
+        x = fmaxf(x, r.m[n][h]);
+        if (x > -INFINITY) {
+          const float f = ex2(r.m[n][h] - x);      // (from -inf: 0)
+          r.m[n][h] = x;
+          r.neg[n][h] = -x;
+          r.l[n][h] *= f;
 #pragma unroll
-        for (int d = 0; d < HD / 16; d++) a.o[n][d][h] *= f, a.o[n][d][h + 2] *= f;
+          for (int d = 0; d < HD / 16; d++) r.o[n][d][h] *= f, r.o[n][d][h + 2] *= f;
+        }
+        y[n][h] = fmaf(s[n][h], q.c[n][h], r.neg[n][h]), y[n][h + 2] = fmaf(s[n][h + 2], q.c[n][h], r.neg[n][h]);
       }
   }
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      s[n][k] = ex2(fmaf(s[n][k], c, a.neg[n][k & 1]));
-      a.l[n][k & 1] += s[n][k];
+      y[n][k] = ex2(y[n][k]);
+      r.l[n][k & 1] += y[n][k];
     }
   float sa[NG], sb[NG];
   load_scales<NG>(blk + L::VS + 2 * ta * NG, sa);
@@ -341,29 +353,25 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& a, const Queries<HD, NT>& q
   load_halves<NG>(blk + L::V + (v1 + 8) * L::ROW + 2 * i * NG, w3);
 #pragma unroll
   for (int g = 0; g < NG; g++) {
-    uint32_t b0[NT], b1[NT];
+    const uint32_t x0 = __byte_perm(w0[g], w1[g], 0x5410), x1 = __byte_perm(w2[g], w3[g], 0x5410);
+    uint32_t a[8];
+#pragma unroll
+    for (int e = 0; e < 4; e++) a[e / 2 * 4 + e % 2] = value_codes(x0 >> 4 * e), a[e / 2 * 4 + 2 + e % 2] = value_codes(x1 >> 4 * e);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-      float p[4] = {s[n][0] * sa[g], s[n][1] * sa[g], s[n][2] * sb[g], s[n][3] * sb[g]};
-      if (masked) {      // (a scale that no column sees may be anything)
+      float p[4] = {y[n][0] * sa[g], y[n][1] * sa[g], y[n][2] * sb[g], y[n][3] * sb[g]};
+      if (masked) {      // (a scale that is not seen may be anything)
         if (t0 >= seen[n][0]) p[0] = 0.f;
         if (t0 >= seen[n][1]) p[1] = 0.f;
         if (t1 >= seen[n][0]) p[2] = 0.f;
         if (t1 >= seen[n][1]) p[3] = 0.f;
       }
-      b0[n] = transposed(pack_bf16(p[0], p[1]));
-      b1[n] = transposed(pack_bf16(p[2], p[3]));
-    }
-    const uint32_t x0 = __byte_perm(w0[g], w1[g], 0x5410), x1 = __byte_perm(w2[g], w3[g], 0x5410);
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint32_t a0 = codes_minus8(x0 >> 8 * h), a1 = codes_minus8(x0 >> (8 * h + 4)), a2 = codes_minus8(x1 >> 8 * h), a3 = codes_minus8(x1 >> (8 * h + 4));
-#pragma unroll
-      for (int n = 0; n < NT; n++) mma16816(a.o[n][2 * g + h], a0, a1, a2, a3, b0[n], b1[n]);
+      const uint32_t b0 = transposed(pack_bf16(p[0], p[1])), b1 = transposed(pack_bf16(p[2], p[3]));
+      mma_values(r.o[n][2 * g], a[0], a[1], a[2], a[3], b0, b1);
+      mma_values(r.o[n][2 * g + 1], a[4], a[5], a[6], a[7], b0, b1);
     }
   }
 }
-
 template <int HD, int NT> constexpr int merge_floats() { return 8 * NT * (HD + 2); }
 template <int HD, int NT> constexpr int attn_ring() {      // bytes of the rings, and of the warps' shares that take their place
   const int ring = WARPS * Ring<HD>::N * Block<HD>::BYTES, merge = WARPS * merge_floats<HD, NT>() * 4;
@@ -451,7 +459,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
 #pragma unroll
         for (int k = 0; k < 4; k++) acc.o[n][d][k] = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; h++) acc.m[n][h] = -INFINITY, acc.neg[n][h] = 0.f, acc.l[n][h] = 0.f;
+      for (int h = 0; h < 2; h++) acc.m[n][h] = -INFINITY, acc.neg[n][h] = NONE, acc.l[n][h] = 0.f;
     }
     if (w0 < w1 && len > 0) {
       const int* trow = A.table + (long)b * A.width;
@@ -487,27 +495,42 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         const int r = row0 + 8 * n + i;
+        uint4 w[NG];
+        uint32_t top = 0;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+          w[g] = {0, 0, 0, 0};
+          if (r < rows) w[g] = *reinterpret_cast<const uint4*>(A.q + ((long)b * A.Tq + r / A.G) * A.q_stride + ((long)kv * A.G + r % A.G) * HD + 32 * g + 8 * j);
+          w[g].x = (w[g].x & A.q_keep) ^ A.q_flip, w[g].y = (w[g].y & A.q_keep) ^ A.q_flip, w[g].z = (w[g].z & A.q_keep) ^ A.q_flip, w[g].w = (w[g].w & A.q_keep) ^ A.q_flip;
+          const uint32_t u[4] = {w[g].x, w[g].y, w[g].z, w[g].w};
+#pragma unroll
+          for (int k = 0; k < 4; k++) top = max(top, max(u[k] << 16 & 0x7F800000u, u[k] & 0x7F800000u));
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the row's largest element comes to 2^13 ... 2^14: exact for all elements above 2^-23 of it.  A row of zeros, or below 2^-100, as if its exponent were that
+        const int e = min(max((int)(top >> 23), 27), 243);
+        const float f = __uint_as_float((uint32_t)(267 - e) << 23), back = A.scale_log2 * __uint_as_float((uint32_t)(e + 11) << 23);
         float sum[NG];
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-          uint4 w = {0, 0, 0, 0};
-          if (r < rows) w = *reinterpret_cast<const uint4*>(A.q + ((long)b * A.Tq + r / A.G) * A.q_stride + ((long)kv * A.G + r % A.G) * HD + 32 * g + 8 * j);
-          w.x = (w.x & A.q_keep) ^ A.q_flip, w.y = (w.y & A.q_keep) ^ A.q_flip, w.z = (w.z & A.q_keep) ^ A.q_flip, w.w = (w.w & A.q_keep) ^ A.q_flip;
-          q.b[n][2 * g][0] = __byte_perm(w.x, w.z, 0x5410), q.b[n][2 * g][1] = __byte_perm(w.x, w.z, 0x7632);
-          q.b[n][2 * g + 1][0] = __byte_perm(w.y, w.w, 0x5410), q.b[n][2 * g + 1][1] = __byte_perm(w.y, w.w, 0x7632);
           float x[8];
-          unpack8(w, x);
+          unpack8(w[g], x);
           float y = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; k++) y += x[k];
+          for (int k = 0; k < 8; k++) x[k] *= f, y += x[k];
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+            q.b[n][2 * g + k][0] = pack_half(x[2 * k], x[2 * k + 4]), q.b[n][2 * g + k][1] = pack_half(x[2 * k + 1] * 0.0625f, x[2 * k + 5] * 0.0625f);
           y += __shfl_xor_sync(0xffffffffu, y, 1);
           y += __shfl_xor_sync(0xffffffffu, y, 2);
-          sum[g] = -136.f * y;
+          sum[g] = y * -4.76837158203125e-7f;      // -8 2^-24
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
 #pragma unroll
           for (int g = 0; g < NG; g++) q.start[n][g][h] = __shfl_sync(0xffffffffu, sum[g], (2 * j + h) * 4);
+          q.c[n][h] = __shfl_sync(0xffffffffu, back, (2 * j + h) * 4);
           const int col = row0 + 8 * n + 2 * j + h;
           seen[n][h] = col < rows ? len - A.Tq + col / A.G + 1 : len;
         }
@@ -521,13 +544,14 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
           __syncwarp();
           break;
         }
-        if (there >> k & 1) attend<HD, NT>(acc, q, ring + k * L::BYTES, u * TOK, u * TOK + TOK > all, seen, A.scale_log2, i, j);
+        if (there >> k & 1) attend<HD, NT>(acc, q, ring + k * L::BYTES, u * TOK, u * TOK + TOK > all, seen, i, j);
         __syncwarp();
         if (u + NST < w1) fetch(u + NST, count + NST);
       }
     }
     // ---- the warps' shares put together (in the rings' memory, which nothing is on its way to)
     __syncthreads();
+    const int live = min(R, rows - row0);
     float* mine = mrg + warp * PART;
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -539,12 +563,13 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
         const int col = 8 * n + 2 * j + h;
         if (i == 0) mine[col] = acc.m[n][h], mine[R + col] = l;
 #pragma unroll
-        for (int g = 0; g < NG; g++)
-          *reinterpret_cast<float4*>(mine + 2 * R + col * HD + 32 * g + 4 * i) =
-              make_float4(acc.o[n][2 * g][h], acc.o[n][2 * g][h + 2], acc.o[n][2 * g + 1][h], acc.o[n][2 * g + 1][h + 2]);
+        for (int g = 0; g < NG; g++) {
+          if (col < live)
+            *reinterpret_cast<float4*>(mine + 2 * R + col * HD + 32 * g + 4 * i) =
+                make_float4(acc.o[n][2 * g][h], acc.o[n][2 * g][h + 2], acc.o[n][2 * g + 1][h], acc.o[n][2 * g + 1][h + 2]);
+        }
       }
     __syncthreads();
-    const int live = min(R, rows - row0);
     const long c0 = item0 / per, c1 = (item1 - 1) / per;      // the thread blocks that share this head
     const int item = (int)(blockIdx.y * (long)A.B * A.Hkv + (long)b * A.Hkv + kv);
     float* part = A.part + ((long)blockIdx.y * gridDim.x * 2) * PART;
@@ -556,7 +581,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
       bf16* out = A.out + ((long)b * A.Tq + tok) * A.G * A.Hkv * HD + (long)head * HD + 4 * d;
       *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
       if (d == 0 && A.lse != nullptr)
-        A.lse[((long)b * A.G * A.Hkv + head) * A.Tq + tok] = l == 0.f ? -INFINITY : (m * A.scale_log2 + log2f(l)) * 0.693147180559945f;
+        A.lse[((long)b * A.G * A.Hkv + head) * A.Tq + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
     };
     for (int x = tid; x < live * (HD / 4); x += WARPS * 32) {
       const int r = x / (HD / 4), d = x % (HD / 4);
@@ -564,7 +589,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
       for (int w = 0; w < WARPS; w++) m = fmaxf(m, mrg[w * PART + r]);
       float4 o = {0, 0, 0, 0};
       for (int w = 0; w < WARPS; w++) {
-        const float mw = mrg[w * PART + r], f = mw == m ? (m == -INFINITY ? 0.f : 1.f) : ex2((mw - m) * A.scale_log2);
+        const float mw = mrg[w * PART + r], f = mw == m ? (m == -INFINITY ? 0.f : 1.f) : ex2(mw - m);
         const float4 v = *reinterpret_cast<const float4*>(mrg + w * PART + 2 * R + r * HD + 4 * d);
         l = fmaf(f, mrg[w * PART + R + r], l);
         o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
@@ -592,7 +617,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
           float4 o = {0, 0, 0, 0};
           for (long c = c0; c <= c1; c++) {
             const float* p = share(c);
-            const float mw = __ldcg(p + r), f = mw == m ? (m == -INFINITY ? 0.f : 1.f) : ex2((mw - m) * A.scale_log2);
+            const float mw = __ldcg(p + r), f = mw == m ? (m == -INFINITY ? 0.f : 1.f) : ex2(mw - m);
             const float4 v = __ldcg(reinterpret_cast<const float4*>(p + 2 * R + r * HD + 4 * d));
             l = fmaf(f, __ldcg(p + R + r), l);
             o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
