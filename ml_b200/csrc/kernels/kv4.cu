@@ -196,7 +196,10 @@ struct AttnArgs {
 };
 constexpr int WARPS = 4;
 constexpr int MAX_B = 2048;       // sequences of a launch: their first blocks' numbers stand in shared memory
-template <int HD> struct Ring { static constexpr int N = HD == 128 ? 5 : HD == 96 ? 6 : 8; };
+// A warp's ring: N places of STEP blocks (hd = 128: 4 thread blocks' rings fill an SM's shared memory)
+constexpr int STEP = 2;
+constexpr int per_sm(int nt) { return nt == 1 ? 3 : 3; }      // thread blocks that an SM holds
+template <int HD> struct Ring { static constexpr int N = HD == 128 ? 3 : HD == 96 ? 4 : HD == 64 ? 6 : 8, BYTES = STEP * Block<HD>::BYTES; };
 
 // D = A B + C: keys' codes and queries in fp16, values' codes and weights in bf16
 __device__ __forceinline__ void mma_keys(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2,
@@ -274,19 +277,21 @@ template <int HD, int NT> struct Queries {
   float c[NT][2];                   // score = c * product
 };
 
-// One block of 16 tokens.  first: its first token; seen[n][c]: tokens that column c sees; masked: not every column sees all 16.
-template <int HD, int NT>
-__device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q, const uint8_t* blk, int first, bool masked, const int (&seen)[NT][2], int i, int j) {
+// NB blocks of 16 tokens, one behind the other.  first: their first token; seen[n][c]: tokens that column c sees, asked only where MASKED.
+template <int HD, int NT, int NB, bool MASKED>
+__device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q, const uint8_t* blk, int first, const int (&seen)[NT][2], int i, int j) {
   using L = Block<HD>;
   constexpr int NG = L::NG;
-  // Row r of the products is token r ^ (r / 2 & 1): the tokens whose values a lane reads are then of both parities in each load, half the conflicts
+  // Row x of the products is token x ^ (x / 2 & 1): the tokens whose values a lane reads are then of both parities in each load, half the conflicts
   const int ta = i ^ (i >> 1 & 1), v0 = 2 * j + (j & 1), v1 = 2 * j + 1 - (j & 1);
-  float s[NT][4];
-  {
-    const auto ka = load_words<NG>(blk + ta * L::ROW + 4 * j * NG), kb = load_words<NG>(blk + (ta + 8) * L::ROW + 4 * j * NG);
+  float s[NB][NT][4];
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    const uint8_t* at = blk + b * L::BYTES;
+    const auto ka = load_words<NG>(at + ta * L::ROW + 4 * j * NG), kb = load_words<NG>(at + (ta + 8) * L::ROW + 4 * j * NG);
     float sa[NG], sb[NG];
-    load_scales<NG>(blk + L::KS + 2 * ta * NG, sa);
-    load_scales<NG>(blk + L::KS + 2 * (ta + 8) * NG, sb);
+    load_scales<NG>(at + L::KS + 2 * ta * NG, sa);
+    load_scales<NG>(at + L::KS + 2 * (ta + 8) * NG, sb);
 #pragma unroll
     for (int g = 0; g < NG; g++) {
       const uint32_t xa = ka.w[g], xb = kb.w[g], ya = xa >> 8, yb = xb >> 8;
@@ -296,32 +301,36 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
         const float s0 = q.start[n][g][0], s1 = q.start[n][g][1];
         mma_keys(d, low_codes(xa), low_codes(xb), high_codes(xa), high_codes(xb), q.b[n][2 * g][0], q.b[n][2 * g][1], s0, s1, s0, s1);
         mma_keys(d, low_codes(ya), low_codes(yb), high_codes(ya), high_codes(yb), q.b[n][2 * g + 1][0], q.b[n][2 * g + 1][1], d[0], d[1], d[2], d[3]);
-        s[n][0] = g ? fmaf(sa[g], d[0], s[n][0]) : sa[g] * d[0], s[n][1] = g ? fmaf(sa[g], d[1], s[n][1]) : sa[g] * d[1];
-        s[n][2] = g ? fmaf(sb[g], d[2], s[n][2]) : sb[g] * d[2], s[n][3] = g ? fmaf(sb[g], d[3], s[n][3]) : sb[g] * d[3];
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[b][n][k] = g ? fmaf(k < 2 ? sa[g] : sb[g], d[k], s[b][n][k]) : (k < 2 ? sa[g] : sb[g]) * d[k];
       }
     }
   }
-  const int t0 = first + ta, t1 = t0 + 8;
-  if (masked) {
+  const int t0 = first + ta;      // token of block 0's elements 0 and 1; 2 and 3: 8 on
+  if constexpr (MASKED) {
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (t0 + 16 * b + k / 2 * 8 >= seen[n][k & 1]) s[b][n][k] = -INFINITY;
+  }
+  float y[NB][NT][4], top = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < NB; b++)
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if (t0 >= seen[n][h]) s[n][h] = -INFINITY;
-        if (t1 >= seen[n][h]) s[n][h + 2] = -INFINITY;
-      }
-  }
-  float y[NT][4], top = -INFINITY;
-#pragma unroll
-  for (int n = 0; n < NT; n++)
-#pragma unroll
-    for (int k = 0; k < 4; k++) y[n][k] = fmaf(s[n][k], q.c[n][k & 1], r.neg[n][k & 1]), top = fmaxf(top, y[n][k]);
+      for (int k = 0; k < 4; k++) y[b][n][k] = fmaf(s[b][n][k], q.c[n][k & 1], r.neg[n][k & 1]), top = fmaxf(top, y[b][n][k]);
   if (__any_sync(0xffffffffu, top > 8.f)) {
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        float x = fmaxf(s[n][h], s[n][h + 2]) * q.c[n][h];
+        float x = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < NB; b++) x = fmaxf(x, fmaxf(s[b][n][h], s[b][n][h + 2]) * q.c[n][h]);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
         x = fmaxf(x, r.m[n][h]);
@@ -333,54 +342,61 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
 #pragma unroll
           for (int d = 0; d < HD / 16; d++) r.o[n][d][h] *= f, r.o[n][d][h + 2] *= f;
         }
-        y[n][h] = fmaf(s[n][h], q.c[n][h], r.neg[n][h]), y[n][h + 2] = fmaf(s[n][h + 2], q.c[n][h], r.neg[n][h]);
+#pragma unroll
+        for (int b = 0; b < NB; b++) y[b][n][h] = fmaf(s[b][n][h], q.c[n][h], r.neg[n][h]), y[b][n][h + 2] = fmaf(s[b][n][h + 2], q.c[n][h], r.neg[n][h]);
       }
   }
 #pragma unroll
-  for (int n = 0; n < NT; n++)
+  for (int b = 0; b < NB; b++)
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      y[n][k] = ex2(y[n][k]);
-      r.l[n][k & 1] += y[n][k];
-    }
-  float sa[NG], sb[NG];
-  load_scales<NG>(blk + L::VS + 2 * ta * NG, sa);
-  load_scales<NG>(blk + L::VS + 2 * (ta + 8) * NG, sb);
-  uint32_t w0[NG], w1[NG], w2[NG], w3[NG];
-  load_halves<NG>(blk + L::V + v0 * L::ROW + 2 * i * NG, w0);
-  load_halves<NG>(blk + L::V + v1 * L::ROW + 2 * i * NG, w1);
-  load_halves<NG>(blk + L::V + (v0 + 8) * L::ROW + 2 * i * NG, w2);
-  load_halves<NG>(blk + L::V + (v1 + 8) * L::ROW + 2 * i * NG, w3);
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-  for (int g = 0; g < NG; g++) {
-    const uint32_t x0 = __byte_perm(w0[g], w1[g], 0x5410), x1 = __byte_perm(w2[g], w3[g], 0x5410);
-    uint32_t a[8];
-#pragma unroll
-    for (int e = 0; e < 4; e++) a[e / 2 * 4 + e % 2] = value_codes(x0 >> 4 * e), a[e / 2 * 4 + 2 + e % 2] = value_codes(x1 >> 4 * e);
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      float p[4] = {y[n][0] * sa[g], y[n][1] * sa[g], y[n][2] * sb[g], y[n][3] * sb[g]};
-      if (masked) {      // (a scale that is not seen may be anything)
-        if (t0 >= seen[n][0]) p[0] = 0.f;
-        if (t0 >= seen[n][1]) p[1] = 0.f;
-        if (t1 >= seen[n][0]) p[2] = 0.f;
-        if (t1 >= seen[n][1]) p[3] = 0.f;
+      for (int k = 0; k < 4; k++) {
+        y[b][n][k] = ex2(y[b][n][k]);
+        r.l[n][k & 1] += y[b][n][k];
       }
-      const uint32_t b0 = transposed(pack_bf16(p[0], p[1])), b1 = transposed(pack_bf16(p[2], p[3]));
-      mma_values(r.o[n][2 * g], a[0], a[1], a[2], a[3], b0, b1);
-      mma_values(r.o[n][2 * g + 1], a[4], a[5], a[6], a[7], b0, b1);
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    const uint8_t* at = blk + b * L::BYTES;
+    float sa[NG], sb[NG];
+    load_scales<NG>(at + L::VS + 2 * ta * NG, sa);
+    load_scales<NG>(at + L::VS + 2 * (ta + 8) * NG, sb);
+    uint32_t w0[NG], w1[NG], w2[NG], w3[NG];
+    load_halves<NG>(at + L::V + v0 * L::ROW + 2 * i * NG, w0);
+    load_halves<NG>(at + L::V + v1 * L::ROW + 2 * i * NG, w1);
+    load_halves<NG>(at + L::V + (v0 + 8) * L::ROW + 2 * i * NG, w2);
+    load_halves<NG>(at + L::V + (v1 + 8) * L::ROW + 2 * i * NG, w3);
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      const uint32_t x0 = __byte_perm(w0[g], w1[g], 0x5410), x1 = __byte_perm(w2[g], w3[g], 0x5410);
+      uint32_t a[8];
+#pragma unroll
+      for (int e = 0; e < 4; e++) a[e / 2 * 4 + e % 2] = value_codes(x0 >> 4 * e), a[e / 2 * 4 + 2 + e % 2] = value_codes(x1 >> 4 * e);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        float p[4] = {y[b][n][0] * sa[g], y[b][n][1] * sa[g], y[b][n][2] * sb[g], y[b][n][3] * sb[g]};
+        if constexpr (MASKED) {      // (a scale that is not seen may be anything)
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (t0 + 16 * b + k / 2 * 8 >= seen[n][k & 1]) p[k] = 0.f;
+        }
+        const uint32_t b0 = transposed(pack_bf16(p[0], p[1])), b1 = transposed(pack_bf16(p[2], p[3]));
+        mma_values(r.o[n][2 * g], a[0], a[1], a[2], a[3], b0, b1);
+        mma_values(r.o[n][2 * g + 1], a[4], a[5], a[6], a[7], b0, b1);
+      }
     }
   }
 }
+
 template <int HD, int NT> constexpr int merge_floats() { return 8 * NT * (HD + 2); }
 template <int HD, int NT> constexpr int attn_ring() {      // bytes of the rings, and of the warps' shares that take their place
-  const int ring = WARPS * Ring<HD>::N * Block<HD>::BYTES, merge = WARPS * merge_floats<HD, NT>() * 4;
+  const int ring = WARPS * Ring<HD>::N * Ring<HD>::BYTES, merge = WARPS * merge_floats<HD, NT>() * 4;
   return ring > merge ? ring : merge;
 }
 template <int HD, int NT> int attn_smem(int B) { return attn_ring<HD, NT>() + (B + 1) * 4; }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const AttnArgs A) {
+__global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnArgs A) {
   using L = Block<HD>;
   constexpr int NG = L::NG, NST = Ring<HD>::N, R = 8 * NT, PART = merge_floats<HD, NT>();
   extern __shared__ __align__(128) uint8_t smem[];
@@ -421,36 +437,33 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
   }
   if (tid == 0) start[A.B] = done;
   __syncthreads();
-  const long total = (long)done * A.Hkv;
-  const long per = max((long)WARPS, (total + gridDim.x - 1) / gridDim.x);
-  long s = per * blockIdx.x;
-  const long e = min(total, s + per);
+  const unsigned total = (unsigned)done * A.Hkv, per = max((unsigned)WARPS, (total + gridDim.x - 1) / gridDim.x);      // (the host sees to it that total fits)
+  unsigned s = per * blockIdx.x;
+  const unsigned e = min(total, s + per);
   const int rows = A.G * A.Tq, row0 = blockIdx.y * R;
-  uint8_t* ring = smem + warp * NST * L::BYTES;
+  uint8_t* ring = smem + warp * NST * Ring<HD>::BYTES;
   float* mrg = reinterpret_cast<float*>(smem);
   const int bpl = A.page_log - 4;      // log2 of the blocks of a page
-  int count = 0;                       // blocks that this warp has taken from its ring
+  int count = 0;                       // places that this warp has taken from its ring
   bool dead = false;
   int b = 0;
   if (s < e) {      // the sequence of the first block
     int hi = A.B;
     while (hi - b > 1) {
       const int mid = (b + hi) >> 1;
-      if ((long)start[mid] * A.Hkv <= s) b = mid;
+      if ((unsigned)start[mid] * A.Hkv <= s) b = mid;
       else hi = mid;
     }
   }
   while (s < e) {
-    while ((long)start[b + 1] * A.Hkv <= s) b++;
-    const int nb = start[b + 1] - start[b];
-    const long base = (long)start[b] * A.Hkv;
-    const int kv = (int)((s - base) / nb);
-    const long item0 = base + (long)kv * nb, item1 = item0 + nb;
+    while ((unsigned)start[b + 1] * A.Hkv <= s) b++;
+    const unsigned nb = start[b + 1] - start[b], kv = (s - (unsigned)start[b] * A.Hkv) / nb;
+    const unsigned item0 = (unsigned)start[b] * A.Hkv + kv * nb, item1 = item0 + nb;
     const int u0 = (int)(s - item0), u1 = (int)(min(e, item1) - item0);
     const int len = max(0, min(A.lens[b], longest));
 
     // ---- this warp's blocks [w0, w1)
-    const int w0 = u0 + (int)((long)(u1 - u0) * warp / WARPS), w1 = u0 + (int)((long)(u1 - u0) * (warp + 1) / WARPS);
+    const int w0 = u0 + (u1 - u0) * warp / WARPS, w1 = u0 + (u1 - u0) * (warp + 1) / WARPS;
     Rows<HD, NT> acc;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -464,30 +477,29 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
     if (w0 < w1 && len > 0) {
       const int* trow = A.table + (long)b * A.width;
       int have = -1, ids = 0;      // page numbers [have, have + 32) of the table, one a lane
-      uint32_t there = 0;          // blocks in the ring whose page is one of the pool
-      auto fetch = [&](int u, int n) {      // block u into place n
-        const int p = u >> bpl;
-        if (have < 0 || p >= have + 32) {
-          have = p;
-          ids = p + lane < A.width ? trow[p + lane] : -1;
+      uint32_t there = 0;          // blocks in the ring whose page is one of the pool, STEP bits a place
+      const uint8_t* base = A.pages + ((long)kv << bpl) * L::BYTES;
+      auto fetch = [&](int u, int n) {      // blocks u ... u + STEP - 1 into place n, a lane each
+        const int p0 = u >> bpl, mine = u + lane, p = mine >> bpl;
+        if (have < 0 || ((min(u + STEP, w1) - 1) >> bpl) >= have + 32) {
+          have = p0;
+          ids = p0 + lane < A.width ? trow[p0 + lane] : -1;
         }
         const int id = __shfl_sync(0xffffffffu, ids, p - have);
-        const bool ok = id >= 0 && id < A.n_pages;
+        const bool wanted = lane < STEP && mine < w1, ok = wanted && id >= 0 && id < A.n_pages;
+        const uint32_t oks = __ballot_sync(0xffffffffu, ok);
         const int k = n % NST;
-        there = ok ? there | 1u << k : there & ~(1u << k);
-        if (lane == 0) {
-          if (ok) {
-            tc::mbar_expect_tx(&bars[warp][k], L::BYTES);
-            tc::bulk_load(ring + k * L::BYTES, A.pages + ((((long)id * A.Hkv + kv) << bpl) + (u & ((1 << bpl) - 1))) * L::BYTES, L::BYTES, &bars[warp][k]);
-          } else {
-            mlb_set_error(MLB_ERR_BOUNDS, 0xC1);
-            tc::mbar_arrive(&bars[warp][k]);
-          }
-        }
+        there = (there & ~(((1u << STEP) - 1) << k * STEP)) | oks << k * STEP;
+        if (lane == 0) tc::mbar_expect_tx(&bars[warp][k], __popc(oks) * L::BYTES);
+        __syncwarp();
+        if (ok)
+          tc::bulk_load(ring + k * Ring<HD>::BYTES + lane * L::BYTES, base + ((((long)id * A.Hkv) << bpl) + (mine & ((1 << bpl) - 1))) * L::BYTES, L::BYTES, &bars[warp][k]);
+        else if (wanted)
+          mlb_set_error(MLB_ERR_BOUNDS, 0xC1);
       };
-      const int ahead = min(w1 - w0, NST);
+      const int places = (w1 - w0 + STEP - 1) / STEP;
       if (!dead)
-        for (int k = 0; k < ahead; k++) fetch(w0 + k, count + k);
+        for (int k = 0; k < min(places, NST); k++) fetch(w0 + k * STEP, count + k);
       // ---- the queries, while the first blocks are on their way
       Queries<HD, NT> q;
       int seen[NT][2];
@@ -536,17 +548,25 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
         }
       }
       if (row0 < rows) all = len - A.Tq + row0 / A.G + 1;      // (the first row of the tile sees the fewest)
-      for (int u = w0; u < w1 && !dead; u++, count++) {
+      for (int u = w0; u < w1 && !dead; u += STEP, count++) {
         const int k = count % NST;
         if (!__all_sync(0xffffffffu, tc::mbar_wait(&bars[warp][k], count / NST & 1, 0xD1))) {
           dead = true;      // no more is fetched; what is on its way is waited for
-          for (int x = 1; x < min(NST, w1 - u); x++) tc::mbar_wait(&bars[warp][(count + x) % NST], (count + x) / NST & 1, 0xD2);
+          for (int x = 1; x < min(NST, (w1 - u + STEP - 1) / STEP); x++) tc::mbar_wait(&bars[warp][(count + x) % NST], (count + x) / NST & 1, 0xD2);
           __syncwarp();
           break;
         }
-        if (there >> k & 1) attend<HD, NT>(acc, q, ring + k * L::BYTES, u * TOK, u * TOK + TOK > all, seen, i, j);
+        const uint32_t oks = there >> k * STEP & ((1u << STEP) - 1);
+        const uint8_t* blk = ring + k * Ring<HD>::BYTES;
+        if (oks == (1u << STEP) - 1 && (u + STEP) * TOK <= all) {
+          attend<HD, NT, STEP, false>(acc, q, blk, u * TOK, seen, i, j);
+        } else {
+#pragma unroll 1
+          for (int x = 0; x < STEP; x++)
+            if (oks >> x & 1) attend<HD, NT, 1, true>(acc, q, blk + x * L::BYTES, (u + x) * TOK, seen, i, j);
+        }
         __syncwarp();
-        if (u + NST < w1) fetch(u + NST, count + NST);
+        if (u + NST * STEP < w1) fetch(u + NST * STEP, count + NST);
       }
     }
     // ---- the warps' shares put together (in the rings' memory, which nothing is on its way to)
@@ -570,11 +590,10 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
         }
       }
     __syncthreads();
-    const long c0 = item0 / per, c1 = (item1 - 1) / per;      // the thread blocks that share this head
-    const int item = (int)(blockIdx.y * (long)A.B * A.Hkv + (long)b * A.Hkv + kv);
-    float* part = A.part + ((long)blockIdx.y * gridDim.x * 2) * PART;
+    const unsigned c0 = item0 / per, c1 = (item1 - 1) / per;      // the thread blocks that share this head
+    const int item = (int)((blockIdx.y * (unsigned)A.B + b) * A.Hkv + kv), n_shares = (int)(c1 - c0 + 1);
+    float* part = A.part + (long)blockIdx.y * gridDim.x * 2 * PART;
     float* my = part + (blockIdx.x * 2 + (s == per * blockIdx.x ? 0 : 1)) * (long)PART;
-    const int n_shares = (int)(c1 - c0 + 1);
     auto finish = [&](int r, int d, float m, float l, const float4& o) {      // elements 4 d ... of row r, whole
       const int head = kv * A.G + (row0 + r) % A.G, tok = (row0 + r) / A.G;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (nothing seen: zeros; NaN stays)
@@ -602,27 +621,65 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv4_attn_k(const 
       }
     }
     if (n_shares > 1) {
-      __threadfence();
       __syncthreads();
-      if (tid == 0) last = atomicAdd(A.count + item, 1) == n_shares - 1;
+      if (tid == 0) {
+        __threadfence();      // (the block's shares before the count)
+        last = atomicAdd(A.count + item, 1) == n_shares - 1;
+        __threadfence();
+      }
       __syncthreads();
       if (last) {
-        __threadfence();
         if (tid == 0) A.count[item] = 0;      // for the next call
-        for (int x = tid; x < live * (HD / 4); x += WARPS * 32) {
-          const int r = x / (HD / 4), d = x % (HD / 4);
-          auto share = [&](long c) { return part + (c * 2 + (c > c0 || item0 == c * per ? 0 : 1)) * (long)PART; };
+        // elements to the threads; few elements: the shares too, `ways` threads an element
+        const int elems = live * (HD / 4), ways = elems >= WARPS * 32 ? 1 : WARPS * 32 / elems;
+        for (int x = tid; x < elems * ways; x += WARPS * 32) {
+          const int way = x / elems, r = x % elems / (HD / 4), d = x % elems % (HD / 4);
           float m = -INFINITY, l = 0.f;
-          for (long c = c0; c <= c1; c++) m = fmaxf(m, __ldcg(share(c) + r));
           float4 o = {0, 0, 0, 0};
-          for (long c = c0; c <= c1; c++) {
-            const float* p = share(c);
-            const float mw = __ldcg(p + r), f = mw == m ? (m == -INFINITY ? 0.f : 1.f) : ex2(mw - m);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + 2 * R + r * HD + 4 * d));
-            l = fmaf(f, __ldcg(p + R + r), l);
-            o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+          constexpr int BATCH = 8;      // shares on their way at a time
+          for (int c = way; c < n_shares; c += ways * BATCH) {
+            float ms[BATCH], ls[BATCH];
+            float4 os[BATCH];
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+              const int z = c + k * ways;
+              ms[k] = -INFINITY, ls[k] = 0.f, os[k] = make_float4(0, 0, 0, 0);
+              if (z < n_shares) {
+                const float* p = part + ((c0 + z) * 2 + (z > 0 || item0 == c0 * per ? 0 : 1)) * (long)PART;
+                ms[k] = __ldcg(p + r), ls[k] = __ldcg(p + R + r), os[k] = __ldcg(reinterpret_cast<const float4*>(p + 2 * R + r * HD + 4 * d));
+              }
+            }
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) top = fmaxf(top, ms[k]);
+            const float g = top == -INFINITY ? 1.f : ex2(m - top);
+            l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, m = top;
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+              const float f = top == -INFINITY ? 0.f : ex2(ms[k] - top);
+              l = fmaf(f, ls[k], l), o.x = fmaf(f, os[k].x, o.x), o.y = fmaf(f, os[k].y, o.y), o.z = fmaf(f, os[k].z, o.z), o.w = fmaf(f, os[k].w, o.w);
+            }
           }
-          finish(r, d, m, l, o);
+          if (ways == 1) {
+            finish(r, d, m, l, o);
+          } else {      // (the warps' shares in shared memory have been read)
+            float* t = mrg + x * 6;
+            t[0] = m, t[1] = l, t[2] = o.x, t[3] = o.y, t[4] = o.z, t[5] = o.w;
+          }
+        }
+        if (ways > 1) {
+          __syncthreads();
+          if (tid < elems) {
+            float m = -INFINITY, l = 0.f;
+            float4 o = {0, 0, 0, 0};
+            for (int w = 0; w < ways; w++) m = fmaxf(m, mrg[(w * elems + tid) * 6]);
+            for (int w = 0; w < ways; w++) {
+              const float* t = mrg + (w * elems + tid) * 6;
+              const float f = m == -INFINITY ? 0.f : ex2(t[0] - m);
+              l = fmaf(f, t[1], l), o.x = fmaf(f, t[2], o.x), o.y = fmaf(f, t[3], o.y), o.z = fmaf(f, t[4], o.z), o.w = fmaf(f, t[5], o.w);
+            }
+            finish(tid / (HD / 4), tid % (HD / 4), m, l, o);
+          }
         }
       }
     }
@@ -648,7 +705,7 @@ int row_tiles(long rows, int& nt) {
 }
 int attn_grid(long B, int Hkv, int width, int page, int nt) {
   const long most = B * Hkv * (((long)width * page + TOK - 1) / TOK);      // (a thread block has a block of tokens for each warp)
-  const long all = (nt == 1 ? 4 : 3) * (long)mlb_sm_count(), want = (most + WARPS - 1) / WARPS;
+  const long all = per_sm(nt) * (long)mlb_sm_count(), want = (most + WARPS - 1) / WARPS;
   return (int)(want < all ? (want > 0 ? want : 1) : all);
 }
 #define MLB_BY_HEAD(hd, F) \
@@ -711,7 +768,7 @@ MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pa
   if (!known_head(hd) || shift < 0 || Hkv < 1 || H % Hkv != 0 || q_stride % 8 != 0) return -7;
   int nt;
   const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
-  if (tiles > 65535) return -7;
+  if (tiles > 65535 || ((long)width * page / TOK + 1) * (B < MAX_B ? B : MAX_B) * Hkv >= 1L << 31) return -7;
   cudaError_t e = cudaSuccess;
   for (int b = 0; b < B && e == cudaSuccess; b += MAX_B) {
     const int n = B - b < MAX_B ? B - b : MAX_B;
