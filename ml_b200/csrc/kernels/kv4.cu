@@ -193,11 +193,12 @@ struct AttnArgs {
   int B, Tq, G, Hkv, width, page_log;
   float scale_log2;            // > 0: a negative scale turns the queries' signs, and none makes them zeros
   uint32_t q_keep, q_flip;
+  float inv_g;
 };
 constexpr int WARPS = 4;
 constexpr int MAX_B = 2048;       // sequences of a launch: their first blocks' numbers stand in shared memory
 // A warp's ring: N places of STEP blocks (hd = 128: 4 thread blocks' rings fill an SM's shared memory)
-constexpr int STEP = 2;
+constexpr int STEP = 2, PAD = 12;
 constexpr int per_sm(int nt) { return nt == 1 ? 3 : 3; }      // thread blocks that an SM holds
 template <int HD> struct Ring { static constexpr int N = HD == 128 ? 3 : HD == 96 ? 4 : HD == 64 ? 6 : 8, BYTES = STEP * Block<HD>::BYTES; };
 
@@ -271,41 +272,46 @@ template <int HD, int NT> struct Rows {      // a warp's share of 8 NT query row
   float m[NT][2], neg[NT][2], l[NT][2];      // largest score (scaled), -m (NONE before the first one), sum of this thread's tokens
 };
 constexpr float NONE = 1e30f;      // in place of -m: any score passes it, and -inf with it is -inf
-template <int HD, int NT> struct Queries {
-  uint32_t b[NT][HD / 16][2];
-  float start[NT][HD / 32][2];      // -8 2^-24 sum over a group of the query
-  float c[NT][2];                   // score = c * product
+template <int HD, int NT> struct Queries {      // of a thread block's query rows, in shared memory
+  uint4 b[NT][HD / 32][32];          // a lane's operands of a group's two products
+  float2 start[NT][HD / 32][4];      // -8 2^-24 sum over a group of the query: of columns 2 j, 2 j + 1
+  float back[NT][8];                 // score of a column = back * product
 };
 
 // NB blocks of 16 tokens, one behind the other.  first: their first token; seen[n][c]: tokens that column c sees, asked only where MASKED.
 template <int HD, int NT, int NB, bool MASKED>
-__device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q, const uint8_t* blk, int first, const int (&seen)[NT][2], int i, int j) {
+__device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q, const float (&c)[NT][2], const uint8_t* blk, int first,
+                                       const int (&seen)[NT][2], int i, int j) {
   using L = Block<HD>;
   constexpr int NG = L::NG;
   // Row x of the products is token x ^ (x / 2 & 1): the tokens whose values a lane reads are then of both parities in each load, half the conflicts
   const int ta = i ^ (i >> 1 & 1), v0 = 2 * j + (j & 1), v1 = 2 * j + 1 - (j & 1);
   float s[NB][NT][4];
+  Words<NG> ka[NB], kb[NB];
+  float ska[NB][NG], skb[NB][NG];
 #pragma unroll
   for (int b = 0; b < NB; b++) {
     const uint8_t* at = blk + b * L::BYTES;
-    const auto ka = load_words<NG>(at + ta * L::ROW + 4 * j * NG), kb = load_words<NG>(at + (ta + 8) * L::ROW + 4 * j * NG);
-    float sa[NG], sb[NG];
-    load_scales<NG>(at + L::KS + 2 * ta * NG, sa);
-    load_scales<NG>(at + L::KS + 2 * (ta + 8) * NG, sb);
+    ka[b] = load_words<NG>(at + ta * L::ROW + 4 * j * NG), kb[b] = load_words<NG>(at + (ta + 8) * L::ROW + 4 * j * NG);
+    load_scales<NG>(at + L::KS + 2 * ta * NG, ska[b]);
+    load_scales<NG>(at + L::KS + 2 * (ta + 8) * NG, skb[b]);
+  }
 #pragma unroll
-    for (int g = 0; g < NG; g++) {
-      const uint32_t xa = ka.w[g], xb = kb.w[g], ya = xa >> 8, yb = xb >> 8;
+  for (int g = 0; g < NG; g++)
 #pragma unroll
-      for (int n = 0; n < NT; n++) {
+    for (int n = 0; n < NT; n++) {
+      const uint4 qb = q.b[n][g][i * 4 + j];
+      const float2 st = q.start[n][g][j];
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        const uint32_t xa = ka[b].w[g], xb = kb[b].w[g], ya = xa >> 8, yb = xb >> 8;
         float d[4];
-        const float s0 = q.start[n][g][0], s1 = q.start[n][g][1];
-        mma_keys(d, low_codes(xa), low_codes(xb), high_codes(xa), high_codes(xb), q.b[n][2 * g][0], q.b[n][2 * g][1], s0, s1, s0, s1);
-        mma_keys(d, low_codes(ya), low_codes(yb), high_codes(ya), high_codes(yb), q.b[n][2 * g + 1][0], q.b[n][2 * g + 1][1], d[0], d[1], d[2], d[3]);
+        mma_keys(d, low_codes(xa), low_codes(xb), high_codes(xa), high_codes(xb), qb.x, qb.y, st.x, st.y, st.x, st.y);
+        mma_keys(d, low_codes(ya), low_codes(yb), high_codes(ya), high_codes(yb), qb.z, qb.w, d[0], d[1], d[2], d[3]);
 #pragma unroll
-        for (int k = 0; k < 4; k++) s[b][n][k] = g ? fmaf(k < 2 ? sa[g] : sb[g], d[k], s[b][n][k]) : (k < 2 ? sa[g] : sb[g]) * d[k];
+        for (int k = 0; k < 4; k++) s[b][n][k] = g ? fmaf(k < 2 ? ska[b][g] : skb[b][g], d[k], s[b][n][k]) : (k < 2 ? ska[b][g] : skb[b][g]) * d[k];
       }
     }
-  }
   const int t0 = first + ta;      // token of block 0's elements 0 and 1; 2 and 3: 8 on
   if constexpr (MASKED) {
 #pragma unroll
@@ -322,7 +328,7 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) y[b][n][k] = fmaf(s[b][n][k], q.c[n][k & 1], r.neg[n][k & 1]), top = fmaxf(top, y[b][n][k]);
+      for (int k = 0; k < 4; k++) y[b][n][k] = fmaf(s[b][n][k], c[n][k & 1], r.neg[n][k & 1]), top = fmaxf(top, y[b][n][k]);
   if (__any_sync(0xffffffffu, top > 8.f)) {
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -330,7 +336,7 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
       for (int h = 0; h < 2; h++) {
         float x = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < NB; b++) x = fmaxf(x, fmaxf(s[b][n][h], s[b][n][h + 2]) * q.c[n][h]);
+        for (int b = 0; b < NB; b++) x = fmaxf(x, fmaxf(s[b][n][h], s[b][n][h + 2]) * c[n][h]);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
         x = fmaxf(x, r.m[n][h]);
@@ -343,7 +349,7 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
           for (int d = 0; d < HD / 16; d++) r.o[n][d][h] *= f, r.o[n][d][h + 2] *= f;
         }
 #pragma unroll
-        for (int b = 0; b < NB; b++) y[b][n][h] = fmaf(s[b][n][h], q.c[n][h], r.neg[n][h]), y[b][n][h + 2] = fmaf(s[b][n][h + 2], q.c[n][h], r.neg[n][h]);
+        for (int b = 0; b < NB; b++) y[b][n][h] = fmaf(s[b][n][h], c[n][h], r.neg[n][h]), y[b][n][h + 2] = fmaf(s[b][n][h + 2], c[n][h], r.neg[n][h]);
       }
   }
 #pragma unroll
@@ -393,7 +399,7 @@ template <int HD, int NT> constexpr int attn_ring() {      // bytes of the rings
   const int ring = WARPS * Ring<HD>::N * Ring<HD>::BYTES, merge = WARPS * merge_floats<HD, NT>() * 4;
   return ring > merge ? ring : merge;
 }
-template <int HD, int NT> int attn_smem(int B) { return attn_ring<HD, NT>() + (B + 1) * 4; }
+template <int HD, int NT> int attn_smem(int B) { return attn_ring<HD, NT>() + (int)sizeof(Queries<HD, NT>) + (B + 1) * 4; }
 
 template <int HD, int NT>
 __global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnArgs A) {
@@ -402,14 +408,15 @@ __global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnA
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[WARPS][NST];
   __shared__ int scan[WARPS], last;
-  int* start = reinterpret_cast<int*>(smem + attn_ring<HD, NT>());
+  Queries<HD, NT>& q = *reinterpret_cast<Queries<HD, NT>*>(smem + attn_ring<HD, NT>());
+  int* start = reinterpret_cast<int*>(smem + attn_ring<HD, NT>() + sizeof(q));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane >> 2, j = lane & 3;
   if (lane == 0) {
     for (int k = 0; k < NST; k++) tc::mbar_init(&bars[warp][k], 1);
     tc::mbar_fence_init();
   }
   mlb_pdl_sync();
-  // first blocks of the sequences, per key / value head: an empty one has a block of its own, which writes its zeros
+  // first units of work of the sequences, per key / value head: its blocks and PAD, what it takes to begin and end one; an empty one has a unit, for its zeros
   const int longest = A.width << A.page_log;
   int done = 0;
   for (int b = 0; b < A.B; b += WARPS * 32) {
@@ -417,7 +424,7 @@ __global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnA
     if (b + tid < A.B) {
       n = A.lens[b + tid];
       if (n > longest && blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC4);
-      n = max(1, (min(n, longest) + TOK - 1) / TOK);
+      n = n <= 0 ? 1 : (min(n, longest) + TOK - 1) / TOK + PAD;
     }
     int x = n;
 #pragma unroll
@@ -444,7 +451,8 @@ __global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnA
   uint8_t* ring = smem + warp * NST * Ring<HD>::BYTES;
   float* mrg = reinterpret_cast<float*>(smem);
   const int bpl = A.page_log - 4;      // log2 of the blocks of a page
-  int count = 0;                       // places that this warp has taken from its ring
+  const unsigned page_bytes = (unsigned)A.Hkv * L::BYTES << bpl;      // of all heads (below 2^32: a page is at most 128 tokens)
+  uint32_t parity = 0;                 // of the next phase of each place of this warp's ring
   bool dead = false;
   int b = 0;
   if (s < e) {      // the sequence of the first block
@@ -459,8 +467,24 @@ __global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnA
     while ((unsigned)start[b + 1] * A.Hkv <= s) b++;
     const unsigned nb = start[b + 1] - start[b], kv = (s - (unsigned)start[b] * A.Hkv) / nb;
     const unsigned item0 = (unsigned)start[b] * A.Hkv + kv * nb, item1 = item0 + nb;
-    const int u0 = (int)(s - item0), u1 = (int)(min(e, item1) - item0);
-    const int len = max(0, min(A.lens[b], longest));
+    const int len = max(0, min(A.lens[b], longest)), blocks = (len + TOK - 1) / TOK;
+    const int u0 = (int)(s - item0), u1 = min((int)(min(e, item1) - item0), blocks);
+    auto token = [&](int r) { return (int)(((float)r + 0.5f) * A.inv_g); };      // r / G (exact: r < 2^20)
+    auto finish = [&](int r, int d, float m, float l, const float4& o) {         // elements 4 d ... of row r, whole
+      const int tok = token(row0 + r), head = (int)kv * A.G + row0 + r - tok * A.G;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (nothing seen: zeros; NaN stays)
+      bf16* out = A.out + ((long)b * A.Tq + tok) * A.G * A.Hkv * HD + (long)head * HD + 4 * d;
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+      if (d == 0 && A.lse != nullptr)
+        A.lse[((long)b * A.G * A.Hkv + head) * A.Tq + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
+    };
+    const int live = min(R, rows - row0);
+    if (u0 >= u1) {
+      if (blocks == 0)
+        for (int x = tid; x < live * (HD / 4); x += WARPS * 32) finish(x / (HD / 4), x % (HD / 4), 0.f, 0.f, make_float4(0, 0, 0, 0));
+      s = min(e, item1);
+      continue;
+    }
 
     // ---- this warp's blocks [w0, w1)
     const int w0 = u0 + (u1 - u0) * warp / WARPS, w1 = u0 + (u1 - u0) * (warp + 1) / WARPS;
@@ -474,104 +498,110 @@ __global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnA
 #pragma unroll
       for (int h = 0; h < 2; h++) acc.m[n][h] = -INFINITY, acc.neg[n][h] = NONE, acc.l[n][h] = 0.f;
     }
-    if (w0 < w1 && len > 0) {
-      const int* trow = A.table + (long)b * A.width;
-      int have = -1, ids = 0;      // page numbers [have, have + 32) of the table, one a lane
-      uint32_t there = 0;          // blocks in the ring whose page is one of the pool, STEP bits a place
-      const uint8_t* base = A.pages + ((long)kv << bpl) * L::BYTES;
-      auto fetch = [&](int u, int n) {      // blocks u ... u + STEP - 1 into place n, a lane each
-        const int p0 = u >> bpl, mine = u + lane, p = mine >> bpl;
-        if (have < 0 || ((min(u + STEP, w1) - 1) >> bpl) >= have + 32) {
-          have = p0;
-          ids = p0 + lane < A.width ? trow[p0 + lane] : -1;
-        }
-        const int id = __shfl_sync(0xffffffffu, ids, p - have);
-        const bool wanted = lane < STEP && mine < w1, ok = wanted && id >= 0 && id < A.n_pages;
-        const uint32_t oks = __ballot_sync(0xffffffffu, ok);
-        const int k = n % NST;
-        there = (there & ~(((1u << STEP) - 1) << k * STEP)) | oks << k * STEP;
-        if (lane == 0) tc::mbar_expect_tx(&bars[warp][k], __popc(oks) * L::BYTES);
-        __syncwarp();
-        if (ok)
-          tc::bulk_load(ring + k * Ring<HD>::BYTES + lane * L::BYTES, base + ((((long)id * A.Hkv) << bpl) + (mine & ((1 << bpl) - 1))) * L::BYTES, L::BYTES, &bars[warp][k]);
-        else if (wanted)
-          mlb_set_error(MLB_ERR_BOUNDS, 0xC1);
-      };
-      const int places = (w1 - w0 + STEP - 1) / STEP;
-      if (!dead)
-        for (int k = 0; k < min(places, NST); k++) fetch(w0 + k * STEP, count + k);
-      // ---- the queries, while the first blocks are on their way
-      Queries<HD, NT> q;
-      int seen[NT][2];
-      int all = len;      // tokens that every column sees
+    const bool some = w0 < w1;
+    const int* trow = A.table + (long)b * A.width;
+    int have = 0, ids = -1;      // page numbers [have, have + 32) of the table, one a lane
+    uint32_t there = 0;          // blocks in the ring whose page is one of the pool, STEP bits a place
+    const uint8_t* base = A.pages + (size_t)(kv << bpl) * L::BYTES;
+    auto names = [&](int p) {
+      have = p;
+      ids = p + lane < A.width ? trow[p + lane] : -1;
+    };
+    auto fetch = [&](int u, int k) {      // blocks u ... u + STEP - 1 into place k, a lane each
+      const int mine = u + lane;
+      if (((min(u + STEP, w1) - 1) >> bpl) >= have + 32) names(u >> bpl);
+      const int id = __shfl_sync(0xffffffffu, ids, (mine >> bpl) - have);
+      const bool wanted = lane < STEP && mine < w1, ok = wanted && (unsigned)id < (unsigned)A.n_pages;
+      const uint32_t oks = __ballot_sync(0xffffffffu, ok);
+      there = (there & ~(((1u << STEP) - 1) << k * STEP)) | oks << k * STEP;
+      if (lane == 0) tc::mbar_expect_tx(&bars[warp][k], __popc(oks) * L::BYTES);
+      __syncwarp();
+      if (ok)
+        tc::bulk_load(ring + k * Ring<HD>::BYTES + lane * L::BYTES, base + (size_t)(unsigned)id * page_bytes + (mine & ((1 << bpl) - 1)) * L::BYTES, L::BYTES,
+                      &bars[warp][k]);
+      else if (wanted)
+        mlb_set_error(MLB_ERR_BOUNDS, 0xC1);
+    };
+    if (some && !dead) {
+      names(w0 >> bpl);
 #pragma unroll
-      for (int n = 0; n < NT; n++) {
-        const int r = row0 + 8 * n + i;
-        uint4 w[NG];
-        uint32_t top = 0;
+      for (int k = 0; k < NST; k++)
+        if (w0 + k * STEP < w1) fetch(w0 + k * STEP, k);
+    }
+    // ---- the queries, while the first blocks are on their way: a group and tile of 8 rows a warp
+#pragma unroll 1
+    for (int x = warp; x < NT * NG; x += WARPS) {
+      const int n = x / NG, own = x % NG, r = row0 + 8 * n + i, tok = token(r);
+      const bf16* src = A.q + ((long)b * A.Tq + tok) * A.q_stride + ((int)kv * A.G + r - tok * A.G) * HD + 8 * j;
+      uint32_t top = 0;
+      uint4 w = {0, 0, 0, 0};
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-          w[g] = {0, 0, 0, 0};
-          if (r < rows) w[g] = *reinterpret_cast<const uint4*>(A.q + ((long)b * A.Tq + r / A.G) * A.q_stride + ((long)kv * A.G + r % A.G) * HD + 32 * g + 8 * j);
-          w[g].x = (w[g].x & A.q_keep) ^ A.q_flip, w[g].y = (w[g].y & A.q_keep) ^ A.q_flip, w[g].z = (w[g].z & A.q_keep) ^ A.q_flip, w[g].w = (w[g].w & A.q_keep) ^ A.q_flip;
-          const uint32_t u[4] = {w[g].x, w[g].y, w[g].z, w[g].w};
+      for (int g = 0; g < NG; g++) {
+        uint4 v = {0, 0, 0, 0};
+        if (r < rows) v = *reinterpret_cast<const uint4*>(src + 32 * g);
+        if (g == own) w = v;
+        const uint32_t u[4] = {v.x & A.q_keep, v.y & A.q_keep, v.z & A.q_keep, v.w & A.q_keep};
 #pragma unroll
-          for (int k = 0; k < 4; k++) top = max(top, max(u[k] << 16 & 0x7F800000u, u[k] & 0x7F800000u));
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the row's largest element comes to 2^13 ... 2^14: exact for all elements above 2^-23 of it.  A row of zeros, or below 2^-100, as if its exponent were that
-        const int e = min(max((int)(top >> 23), 27), 243);
-        const float f = __uint_as_float((uint32_t)(267 - e) << 23), back = A.scale_log2 * __uint_as_float((uint32_t)(e + 11) << 23);
-        float sum[NG];
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-          float x[8];
-          unpack8(w[g], x);
-          float y = 0.f;
-#pragma unroll
-          for (int k = 0; k < 8; k++) x[k] *= f, y += x[k];
-#pragma unroll
-          for (int k = 0; k < 2; k++)
-            q.b[n][2 * g + k][0] = pack_half(x[2 * k], x[2 * k + 4]), q.b[n][2 * g + k][1] = pack_half(x[2 * k + 1] * 0.0625f, x[2 * k + 5] * 0.0625f);
-          y += __shfl_xor_sync(0xffffffffu, y, 1);
-          y += __shfl_xor_sync(0xffffffffu, y, 2);
-          sum[g] = y * -4.76837158203125e-7f;      // -8 2^-24
-        }
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-#pragma unroll
-          for (int g = 0; g < NG; g++) q.start[n][g][h] = __shfl_sync(0xffffffffu, sum[g], (2 * j + h) * 4);
-          q.c[n][h] = __shfl_sync(0xffffffffu, back, (2 * j + h) * 4);
-          const int col = row0 + 8 * n + 2 * j + h;
-          seen[n][h] = col < rows ? len - A.Tq + col / A.G + 1 : len;
-        }
+        for (int k = 0; k < 4; k++) top = max(top, max(u[k] << 16 & 0x7F800000u, u[k] & 0x7F800000u));
       }
-      if (row0 < rows) all = len - A.Tq + row0 / A.G + 1;      // (the first row of the tile sees the fewest)
-      for (int u = w0; u < w1 && !dead; u += STEP, count++) {
-        const int k = count % NST;
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(&bars[warp][k], count / NST & 1, 0xD1))) {
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the row's largest element comes to 2^13 ... 2^14: exact for all elements above 2^-23 of it.  A row of zeros, or below 2^-100, as if its exponent were that
+      const int ex = min(max((int)(top >> 23), 27), 243);
+      const float f = __uint_as_float((uint32_t)(267 - ex) << 23);
+      w.x = (w.x & A.q_keep) ^ A.q_flip, w.y = (w.y & A.q_keep) ^ A.q_flip, w.z = (w.z & A.q_keep) ^ A.q_flip, w.w = (w.w & A.q_keep) ^ A.q_flip;
+      float v[8], y = 0.f;
+      unpack8(w, v);
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] *= f, y += v[k];
+      q.b[n][own][lane] = {pack_half(v[0], v[4]), pack_half(v[1] * 0.0625f, v[5] * 0.0625f), pack_half(v[2], v[6]), pack_half(v[3] * 0.0625f, v[7] * 0.0625f)};
+      y += __shfl_xor_sync(0xffffffffu, y, 1);
+      y += __shfl_xor_sync(0xffffffffu, y, 2);
+      if (j == 0) {
+        reinterpret_cast<float*>(q.start[n][own])[i] = y * -4.76837158203125e-7f;      // -8 2^-24
+        q.back[n][i] = A.scale_log2 * __uint_as_float((uint32_t)(ex + 11) << 23);
+      }
+    }
+    float c[NT][2];
+    int seen[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int col = row0 + 8 * n + 2 * j + h;
+        seen[n][h] = col < rows ? len - A.Tq + token(col) + 1 : len;
+      }
+    const int all = len - A.Tq + token(row0) + 1;      // tokens that every column sees: the first row of the tile sees the fewest
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; n++) c[n][0] = q.back[n][2 * j], c[n][1] = q.back[n][2 * j + 1];
+    if (some && !dead) {
+      int k = 0;
+#pragma unroll 1
+      for (int u = w0; u < w1; u += STEP) {
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(&bars[warp][k], parity >> k & 1, 0xD1))) {
           dead = true;      // no more is fetched; what is on its way is waited for
-          for (int x = 1; x < min(NST, (w1 - u + STEP - 1) / STEP); x++) tc::mbar_wait(&bars[warp][(count + x) % NST], (count + x) / NST & 1, 0xD2);
+          for (int x = 1; x < NST && u + x * STEP < w1; x++) tc::mbar_wait(&bars[warp][(k + x) % NST], parity >> (k + x) % NST & 1, 0xD2);
           __syncwarp();
           break;
         }
+        parity ^= 1u << k;
         const uint32_t oks = there >> k * STEP & ((1u << STEP) - 1);
         const uint8_t* blk = ring + k * Ring<HD>::BYTES;
         if (oks == (1u << STEP) - 1 && (u + STEP) * TOK <= all) {
-          attend<HD, NT, STEP, false>(acc, q, blk, u * TOK, seen, i, j);
+          attend<HD, NT, STEP, false>(acc, q, c, blk, u * TOK, seen, i, j);
         } else {
 #pragma unroll 1
           for (int x = 0; x < STEP; x++)
-            if (oks >> x & 1) attend<HD, NT, 1, true>(acc, q, blk + x * L::BYTES, (u + x) * TOK, seen, i, j);
+            if (oks >> x & 1) attend<HD, NT, 1, true>(acc, q, c, blk + x * L::BYTES, (u + x) * TOK, seen, i, j);
         }
         __syncwarp();
-        if (u + NST * STEP < w1) fetch(u + NST * STEP, count + NST);
+        if (u + NST * STEP < w1) fetch(u + NST * STEP, k);
+        k = k + 1 == NST ? 0 : k + 1;
       }
     }
     // ---- the warps' shares put together (in the rings' memory, which nothing is on its way to)
     __syncthreads();
-    const int live = min(R, rows - row0);
     float* mine = mrg + warp * PART;
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -590,18 +620,10 @@ __global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnA
         }
       }
     __syncthreads();
-    const unsigned c0 = item0 / per, c1 = (item1 - 1) / per;      // the thread blocks that share this head
+    const unsigned c0 = item0 / per, c1 = (item0 + blocks - 1) / per;      // the thread blocks that share this head
     const int item = (int)((blockIdx.y * (unsigned)A.B + b) * A.Hkv + kv), n_shares = (int)(c1 - c0 + 1);
     float* part = A.part + (long)blockIdx.y * gridDim.x * 2 * PART;
     float* my = part + (blockIdx.x * 2 + (s == per * blockIdx.x ? 0 : 1)) * (long)PART;
-    auto finish = [&](int r, int d, float m, float l, const float4& o) {      // elements 4 d ... of row r, whole
-      const int head = kv * A.G + (row0 + r) % A.G, tok = (row0 + r) / A.G;
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (nothing seen: zeros; NaN stays)
-      bf16* out = A.out + ((long)b * A.Tq + tok) * A.G * A.Hkv * HD + (long)head * HD + 4 * d;
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-      if (d == 0 && A.lse != nullptr)
-        A.lse[((long)b * A.G * A.Hkv + head) * A.Tq + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
-    };
     for (int x = tid; x < live * (HD / 4); x += WARPS * 32) {
       const int r = x / (HD / 4), d = x % (HD / 4);
       float m = -INFINITY, l = 0.f;
@@ -704,7 +726,7 @@ int row_tiles(long rows, int& nt) {
   return (int)((rows + 8 * nt - 1) / (8 * nt));
 }
 int attn_grid(long B, int Hkv, int width, int page, int nt) {
-  const long most = B * Hkv * (((long)width * page + TOK - 1) / TOK);      // (a thread block has a block of tokens for each warp)
+  const long most = B * Hkv * (((long)width * page + TOK - 1) / TOK + PAD);      // (a thread block has a unit for each warp)
   const long all = per_sm(nt) * (long)mlb_sm_count(), want = (most + WARPS - 1) / WARPS;
   return (int)(want < all ? (want > 0 ? want : 1) : all);
 }
@@ -768,13 +790,13 @@ MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pa
   if (!known_head(hd) || shift < 0 || Hkv < 1 || H % Hkv != 0 || q_stride % 8 != 0) return -7;
   int nt;
   const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
-  if (tiles > 65535 || ((long)width * page / TOK + 1) * (B < MAX_B ? B : MAX_B) * Hkv >= 1L << 31) return -7;
+  if (tiles > 65535 || (long)n_pages > 0x7FFFFFFFL || (long)Hkv * page * hd * 9 / 8 >= 1L << 32 || ((long)width * page / TOK + PAD) * (B < MAX_B ? B : MAX_B) * Hkv >= 1L << 31) return -7;
   cudaError_t e = cudaSuccess;
   for (int b = 0; b < B && e == cudaSuccess; b += MAX_B) {
     const int n = B - b < MAX_B ? B - b : MAX_B;
     const AttnArgs a{(bf16*)out + (long)b * Tq * H * hd, lse ? lse + (long)b * H * Tq : nullptr, (const bf16*)q + (long)b * Tq * q_stride, pages,
                      table + (long)b * width, lens + b, part, count, q_stride, n_pages, n, Tq, H / Hkv, Hkv, width, shift, (scale == 0.f ? 1.f : fabsf(scale)) * 1.44269504088896f,
-                     scale == 0.f ? 0u : ~0u, scale < 0.f ? 0x80008000u : 0u};
+                     scale == 0.f ? 0u : ~0u, scale < 0.f ? 0x80008000u : 0u, 1.f / (H / Hkv)};
     const int grid = attn_grid(n, Hkv, width, page, nt);
 #define MLB_GO(HD) e = nt == 1 ? launch_attn<HD, 1>(a, grid, tiles, st) : launch_attn<HD, 2>(a, grid, tiles, st)
     MLB_BY_HEAD(hd, MLB_GO)
