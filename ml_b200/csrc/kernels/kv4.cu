@@ -274,7 +274,7 @@ template <int HD, int NT> struct Rows {      // a warp's share of 8 NT query row
 constexpr float NONE = 1e30f;      // in place of -m: any score passes it, and -inf with it is -inf
 template <int HD, int NT> struct Queries {      // of a thread block's query rows, in shared memory
   uint4 b[NT][HD / 32][32];          // a lane's operands of a group's two products
-  float2 start[NT][HD / 32][4];      // -8 2^-24 sum over a group of the query: of columns 2 j, 2 j + 1
+  float4 start[NT][HD / 32][4];      // -8 2^-24 sum over a group of the query: of columns 2 j, 2 j + 1, twice (an accumulator's four)
   float back[NT][8];                 // score of a column = back * product
 };
 
@@ -301,12 +301,12 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       const uint4 qb = q.b[n][g][i * 4 + j];
-      const float2 st = q.start[n][g][j];
+      const float4 st = q.start[n][g][j];
 #pragma unroll
       for (int b = 0; b < NB; b++) {
         const uint32_t xa = ka[b].w[g], xb = kb[b].w[g], ya = xa >> 8, yb = xb >> 8;
         float d[4];
-        mma_keys(d, low_codes(xa), low_codes(xb), high_codes(xa), high_codes(xb), qb.x, qb.y, st.x, st.y, st.x, st.y);
+        mma_keys(d, low_codes(xa), low_codes(xb), high_codes(xa), high_codes(xb), qb.x, qb.y, st.x, st.y, st.z, st.w);
         mma_keys(d, low_codes(ya), low_codes(yb), high_codes(ya), high_codes(yb), qb.z, qb.w, d[0], d[1], d[2], d[3]);
 #pragma unroll
         for (int k = 0; k < 4; k++) s[b][n][k] = g ? fmaf(k < 2 ? ska[b][g] : skb[b][g], d[k], s[b][n][k]) : (k < 2 ? ska[b][g] : skb[b][g]) * d[k];
@@ -558,7 +558,8 @@ __global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnA
       y += __shfl_xor_sync(0xffffffffu, y, 1);
       y += __shfl_xor_sync(0xffffffffu, y, 2);
       if (j == 0) {
-        reinterpret_cast<float*>(q.start[n][own])[i] = y * -4.76837158203125e-7f;      // -8 2^-24
+        float* st = reinterpret_cast<float*>(&q.start[n][own][i / 2]) + i % 2;
+        st[0] = st[2] = y * -4.76837158203125e-7f;      // -8 2^-24
         q.back[n][i] = A.scale_log2 * __uint_as_float((uint32_t)(ex + 11) << 23);
       }
     }
