@@ -24,6 +24,9 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
+#include <vector>
+
 namespace {
 
 using at::Tensor;
@@ -558,6 +561,182 @@ template <typename R, typename... A> struct typed_call<R(A...)> {
 MLB_ENTRIES(MLB_CALL)
 MLB_GENERATION(MLB_CALL)
 
+// ------------------------------------------------------------------ generation
+// The operators of ops/native_gen.py for contiguous tensors of exactly the sizes that belong together, outside a graph capture; whatever else comes is handed
+// back, and Python looks for what is wrong with it.  A step of generation is a chain of kernels of 3 to 10 us, each of which would wait for 11 us of interpreter.
+bool sized(const Tensor& t, std::initializer_list<int64_t> sizes) { return t.sizes() == at::IntArrayRef(sizes.begin(), sizes.size()) && t.is_contiguous(); }
+bool given(PyObject* o, Tensor& t, at::ScalarType type, std::initializer_list<int64_t> sizes) { return plain(o, t, type, (int)sizes.size()) && sized(t, sizes); }
+// bf16 rows that a kernel reads 16 bytes at a time
+bool rows_given(PyObject* o, Tensor& t, int64_t rows, int64_t cols) {
+  return plain(o, t, at::kBFloat16, 2) && t.size(0) == rows && t.size(1) == cols && t.stride(1) == 1 && t.stride(0) % 8 == 0 && aligned(t);
+}
+struct Pool { Tensor t; long n, Hkv, page, hd; };
+bool pool_given(PyObject* o, Pool& p, int dim) {
+  if (!plain(o, p.t, at::kByte, dim) || !p.t.is_contiguous() || !aligned(p.t)) return false;
+  const long b = p.t.size(dim - 1), blocks = p.t.size(dim - 2);
+  p.n = p.t.size(dim - 4), p.Hkv = p.t.size(dim - 3), p.page = 16 * blocks, p.hd = b / 18;
+  return b % 18 == 0 && (p.hd == 32 || p.hd == 64 || p.hd == 96 || p.hd == 128) && (blocks == 1 || blocks == 2 || blocks == 4 || blocks == 8) && p.n * p.page < (1L << 31);
+}
+// Workspace of the calling thread on its current stream, kept from call to call; counters are zero between calls (never given back: the thread may end after torch)
+struct Kept { int op; c10::DeviceIndex device; St st; Tensor part, count; };
+enum { KEPT_ATTN, KEPT_TABLES, KEPT_SELECT };
+Kept& kept(int op, const Tensor& like, St st, long floats, long counters) {
+  static thread_local auto* all = new std::vector<Kept>();
+  Kept* k = nullptr;
+  for (Kept& x : *all)
+    if (x.op == op && x.st == st && x.device == like.get_device()) k = &x;
+  if (!k) {
+    all->push_back({op, (c10::DeviceIndex)like.get_device(), st, Tensor(), Tensor()});
+    k = &all->back();
+  }
+  if (floats > 0 && (!k->part.defined() || k->part.numel() < floats)) k->part = at::empty({floats}, like.options().dtype(at::kFloat));
+  if (!k->count.defined() || k->count.numel() < counters) k->count = at::zeros({counters}, like.options().dtype(at::kInt));
+  return *k;
+}
+template <typename F>
+PyObject* launched(const char* what, F&& f) {
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    rc = f();
+  }
+  if (rc == -7) return declined();
+  check(rc, what);
+  Py_RETURN_NONE;
+}
+template <typename T> T* at_(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
+
+PyObject* py_kv4_append(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd)
+  HANDLE_TH_ERRORS
+  Pool p;
+  Tensor q, qkv, slots, pos, cos, sin;
+  long H, Hkv, hd;
+  if (n != 10 || transformed() || !pool_given(a[0], p, 4) || !plain(a[3], slots, at::kInt, 1) || !slots.is_contiguous() || !int_arg(a[7], H) || !int_arg(a[8], Hkv) ||
+      !int_arg(a[9], hd) || p.Hkv != Hkv || p.hd != hd)
+    return declined();
+  const long N = slots.size(0);
+  if (!rows_given(a[2], qkv, N, (H + 2 * Hkv) * hd) || (a[1] != Py_None && !given(a[1], q, at::kBFloat16, {N, H * hd}))) return declined();
+  if ((a[5] == Py_None) != (a[6] == Py_None)) return declined();
+  if (a[5] != Py_None) {
+    if (!plain(a[5], cos, at::kFloat, 2) || !sized(cos, {cos.size(0), hd / 2}) || !given(a[6], sin, at::kFloat, {cos.size(0), hd / 2}) || !given(a[4], pos, at::kInt, {N}) ||
+        !aligned(cos) || !aligned(sin) || cos.size(0) >= (1L << 31))
+      return declined();
+  }
+  if (q.defined() && !aligned(q)) return declined();
+  return launched("kv4_append", [&] {
+    return K.mlb_kv4_append(at_<uint8_t>(p.t), at_<void>(q), at_<void>(qkv), at_<int>(slots), at_<int>(pos), at_<float>(cos), at_<float>(sin), p.n, (int)p.page, N,
+                            qkv.stride(0), (int)H, (int)Hkv, (int)hd, cos.defined() ? (int)cos.size(0) : 0, stream());
+  });
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_kv4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (k, v, pages, slots)
+  HANDLE_TH_ERRORS
+  Pool p;
+  Tensor k, v, slots;
+  if (n != 4 || transformed() || !pool_given(a[2], p, 4) || !plain(a[3], slots, at::kInt, 1) || !slots.is_contiguous()) return declined();
+  const long N = slots.size(0);
+  if (!given(a[0], k, at::kBFloat16, {N, p.Hkv * p.hd}) || !given(a[1], v, at::kBFloat16, {N, p.Hkv * p.hd}) || !aligned(k) || !aligned(v)) return declined();
+  return launched("kv4_read", [&] {
+    return K.mlb_kv4_read(at_<void>(k), at_<void>(v), at_<uint8_t>(p.t), at_<int>(slots), p.n, (int)p.page, N, (int)p.Hkv, (int)p.hd, stream());
+  });
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_kv4_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale)
+  HANDLE_TH_ERRORS
+  Pool p;
+  Tensor out, lse, q, table, lens;
+  long Tq, H, Hkv, hd;
+  if (n != 11 || transformed() || !pool_given(a[3], p, 4) || !plain(a[5], lens, at::kInt, 1) || !lens.is_contiguous() || !int_arg(a[6], Tq) || !int_arg(a[7], H) ||
+      !int_arg(a[8], Hkv) || !int_arg(a[9], hd) || p.Hkv != Hkv || p.hd != hd || Tq < 1 || H < 1 || H % Hkv != 0)
+    return declined();
+  double scale = 1.0 / std::sqrt((double)hd);
+  if (a[10] != Py_None) {
+    if (!PyFloat_CheckExact(a[10])) return declined();
+    scale = PyFloat_AS_DOUBLE(a[10]);
+    if (!std::isfinite(scale)) return declined();
+  }
+  const long B = lens.size(0);
+  if (!plain(a[4], table, at::kInt, 2) || !sized(table, {B, table.size(1)}) || !rows_given(a[2], q, B * Tq, H * hd) || !given(a[0], out, at::kBFloat16, {B * Tq, H * hd}) ||
+      !aligned(out) || (a[1] != Py_None && !given(a[1], lse, at::kFloat, {B, H, Tq})))
+    return declined();
+  const St st = stream();
+  const long floats = K.mlb_kv4_attn_scratch((int)B, (int)Tq, (int)H, (int)Hkv, (int)hd, (int)table.size(1), (int)p.page);
+  if (floats < 0 || K.mlb_capture_id(st) != 0) return declined();
+  const Kept& w = kept(KEPT_ATTN, lens, st, floats, B * Hkv * ((H / Hkv * Tq + 7) / 8));
+  return launched("kv4_attn", [&] {
+    return K.mlb_kv4_attn(at_<void>(out), at_<float>(lse), at_<void>(q), at_<uint8_t>(p.t), at_<int>(table), at_<int>(lens), at_<float>(w.part), at_<int>(w.count), p.n,
+                          q.stride(0), (int)B, (int)Tq, (int)H, (int)Hkv, (int)hd, (int)table.size(1), (int)p.page, (float)scale, st);
+  });
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (table, slots, pos, starts, new_lens, left, lens, new, free, n_free, page)
+  HANDLE_TH_ERRORS
+  Tensor table, slots, pos, starts, new_lens, left, lens, news, stack, n_free;
+  long page;
+  if (n != 11 || transformed() || !plain(a[6], lens, at::kInt, 1) || !lens.is_contiguous() || !plain(a[1], slots, at::kInt, 1) || !slots.is_contiguous() ||
+      !plain(a[8], stack, at::kInt, 1) || !stack.is_contiguous() || !int_arg(a[10], page))
+    return declined();
+  const long B = lens.size(0), rows = slots.size(0);
+  if (!plain(a[0], table, at::kInt, 2) || !sized(table, {B, table.size(1)}) || !given(a[2], pos, at::kInt, {rows}) || !given(a[3], starts, at::kInt, {B + 1}) ||
+      !given(a[4], new_lens, at::kInt, {B}) || !given(a[5], left, at::kInt, {1}) || !given(a[7], news, at::kInt, {B}) || !given(a[9], n_free, at::kInt, {1}))
+    return declined();
+  const St st = stream();
+  if (K.mlb_capture_id(st) != 0) return declined();
+  const Kept& w = kept(KEPT_TABLES, lens, st, 0, 1);
+  return launched("block_tables", [&] {
+    return K.mlb_block_tables(at_<int>(table), at_<int>(slots), at_<int>(pos), at_<int>(starts), at_<int>(new_lens), at_<int>(left), at_<int>(w.count), at_<int>(lens),
+                              at_<int>(news), at_<int>(stack), at_<int>(n_free), (int)B, (int)table.size(1), (int)page, (int)rows, (int)stack.size(0), st);
+  });
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (scores, tokens, parents, done_out, logits, prev, done, eos)
+  HANDLE_TH_ERRORS
+  Tensor scores, tokens, parents, done_out, z, prev, done;
+  if (n != 8 || transformed() || !plain(a[5], prev, at::kFloat, 2) || !prev.is_contiguous() || !PyLong_CheckExact(a[7])) return declined();
+  int over = 0;
+  const long B = prev.size(0), Kb = prev.size(1), rows = B * Kb, eos = PyLong_AsLongAndOverflow(a[7], &over);
+  const bool half = plain(a[4], z, at::kBFloat16, 2);
+  if (over != 0 || eos < -(1L << 31) || eos >= (1L << 31) || (!half && !plain(a[4], z, at::kFloat, 2)) || z.size(0) != rows || z.size(1) >= (1L << 31) || (z.size(1) > 1 && z.stride(1) != 1) ||
+      !given(a[0], scores, at::kFloat, {B, Kb}) || !given(a[1], tokens, at::kInt, {B, Kb}) || !given(a[2], parents, at::kInt, {B, Kb}) ||
+      !given(a[3], done_out, at::kInt, {B, Kb}) || !given(a[6], done, at::kInt, {B, Kb}) || rows >= (1L << 31))
+    return declined();
+  const St st = stream();
+  const long V = z.size(1), pieces = K.mlb_beam_select_pieces((int)rows, (int)Kb, (int)V);
+  if (pieces < 0 || K.mlb_capture_id(st) != 0) return declined();
+  const long m = rows * pieces;
+  const Kept& w = kept(KEPT_SELECT, prev, st, m * (2 + 2 * Kb), B);
+  float* part = at_<float>(w.part);
+  return launched("beam_select", [&] {
+    return K.mlb_beam_select(at_<float>(scores), at_<int>(tokens), at_<int>(parents), at_<int>(done_out), at_<void>(z), at_<float>(prev), at_<int>(done), part, part + 2 * m,
+                             (int*)(part + 2 * m + m * Kb), at_<int>(w.count), (int)rows, (int)Kb, (int)V, z.stride(0), (int)eos, half ? 16 : 32, st);
+  });
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, page)
+  HANDLE_TH_ERRORS
+  Pool p{Tensor(), 0, 0, 0, 0};
+  Tensor table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens;
+  if (n != 11 || transformed() || !plain(a[8], parents, at::kInt, 2) || !parents.is_contiguous() || !plain(a[4], table, at::kInt, 2) || !plain(a[7], hist, at::kInt, 2))
+    return declined();
+  const long B = parents.size(0), Kb = parents.size(1), rows = B * Kb, width = table.size(1), T = hist.size(1);
+  long page = 0;
+  if (a[10] != Py_None && !int_arg(a[10], page)) return declined();
+  if (a[0] != Py_None) {
+    if (!pool_given(a[0], p, 5) || (a[10] != Py_None && page != p.page)) return declined();
+    page = p.page;
+  }
+  if (page < 16 || page % 16 != 0 || !sized(table, {rows, width}) || !sized(hist, {rows, T}) || !given(a[1], table_out, at::kInt, {rows, width}) ||
+      !given(a[2], spare_out, at::kInt, {rows}) || !given(a[3], hist_out, at::kInt, {rows, T}) || !given(a[5], spare, at::kInt, {rows}) || !given(a[6], lens, at::kInt, {rows}) ||
+      !given(a[9], tokens, at::kInt, {B, Kb}) || table.data_ptr() == table_out.data_ptr() || spare.data_ptr() == spare_out.data_ptr() || hist.data_ptr() == hist_out.data_ptr())
+    return declined();
+  return launched("beam_reorder", [&] {
+    return K.mlb_beam_reorder(at_<uint8_t>(p.t), at_<int>(table_out), at_<int>(spare_out), at_<int>(hist_out), at_<int>(table), at_<int>(spare), at_<int>(lens), at_<int>(hist),
+                              at_<int>(parents), at_<int>(tokens), p.t.defined() ? (int)p.t.size(0) : 0, p.n, (int)p.Hkv, (int)page, p.t.defined() ? (int)(18 * p.hd) : 16, (int)B, (int)Kb,
+                              (int)width, (int)T, stream());
+  });
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(path, settings): the kernel library whose functions are called, the module with the variables above
 PyObject* py_bind(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
@@ -602,7 +781,8 @@ PyObject* py_generation_signatures(PyObject*, PyObject*) {
 #define MLB_FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 #define MLB_METHOD(name, ret, args) {#name, (PyCFunction)(void (*)(void))call_##name, METH_FASTCALL, nullptr},
 PyMethodDef methods[] = {MLB_FAST(linear), MLB_FAST(rmsnorm), MLB_FAST(layer_norm), MLB_FAST(swiglu), MLB_FAST(rope_causal_attention), MLB_FAST(bidir_attention),
-                         MLB_FAST(cross_entropy), MLB_ENTRIES(MLB_METHOD) MLB_GENERATION(MLB_METHOD) {"bind", py_bind, METH_VARARGS, nullptr}, {"signatures", py_signatures, METH_NOARGS, nullptr},
+                         MLB_FAST(cross_entropy), MLB_FAST(kv4_append), MLB_FAST(kv4_read), MLB_FAST(kv4_attn), MLB_FAST(block_tables), MLB_FAST(beam_select), MLB_FAST(beam_reorder),
+                         MLB_ENTRIES(MLB_METHOD) MLB_GENERATION(MLB_METHOD) {"bind", py_bind, METH_VARARGS, nullptr}, {"signatures", py_signatures, METH_NOARGS, nullptr},
                          {"generation_signatures", py_generation_signatures, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mlb_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

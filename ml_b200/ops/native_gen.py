@@ -1,5 +1,6 @@
 """The operators of generation on the kernels of csrc/kernels/kv4.cu and beam.cu: arguments looked at, workspace fetched, one launch each on the current
-stream, nothing read back.  What they do stands with their plain forms in `ops.ref_gen`."""
+stream, nothing read back.  What they do stands with their plain forms in `ops.ref_gen`.  The extension module takes plain calls whole and hands back the
+others (ops/autograd.py has its operators the same way); a step of generation is bound by what its launches cost the host."""
 from __future__ import annotations
 
 import math
@@ -33,7 +34,17 @@ def _here(*ts):
             raise ValueError(f"a tensor is on device {t.get_device()}, the current one is {dev}")
 
 
+def _plain(name, *args):
+    e = _n._entries()
+    if e is not _n.bridge() or getattr(e, name)(*args) is NotImplemented:
+        return False
+    _n.LAUNCHES += 1
+    return True
+
+
 def kv4_append(pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd):
+    if _plain('kv4_append', pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd):
+        return
     n, page, N = check_append(pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd)
     _here(pages, q_out, qkv, slots, pos, cos, sin)
     if N == 0:
@@ -44,6 +55,8 @@ def kv4_append(pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd):
 
 
 def kv4_read(k, v, pages, slots):
+    if _plain('kv4_read', k, v, pages, slots):
+        return
     n, Hkv, page, hd, N = check_read(k, v, pages, slots)
     _here(k, v, pages, slots)
     if N:
@@ -51,6 +64,8 @@ def kv4_read(k, v, pages, slots):
 
 
 def kv4_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale=None):
+    if _plain('kv4_attn', out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale):
+        return
     n, page, B = check_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale)
     _here(out, lse, q, pages, table, lens)
     if B == 0:
@@ -63,6 +78,8 @@ def kv4_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale=None):
 
 
 def block_tables(table, slots, pos, starts, new_lens, left, lens, new, free, n_free, page):
+    if _plain('block_tables', table, slots, pos, starts, new_lens, left, lens, new, free, n_free, page):
+        return
     B = check_tables(table, slots, pos, starts, new_lens, left, lens, new, free, n_free, page)
     _here(table, slots, pos, starts, new_lens, left, lens, new, free, n_free)
     ticket = _n.scratch("tables_ticket", 1, I32, table.device, zero=True)
@@ -71,6 +88,8 @@ def block_tables(table, slots, pos, starts, new_lens, left, lens, new, free, n_f
 
 
 def beam_select(scores, tokens, parents, done_out, logits, prev, done, eos):
+    if _plain('beam_select', scores, tokens, parents, done_out, logits, prev, done, eos):
+        return
     B, K, V = check_select(scores, tokens, parents, done_out, logits, prev, done)
     _here(scores, tokens, parents, done_out, logits, prev, done)
     if B == 0:
@@ -89,6 +108,8 @@ def beam_select(scores, tokens, parents, done_out, logits, prev, done, eos):
 
 
 def beam_reorder(pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, page=None):
+    if _plain('beam_reorder', pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, page):
+        return
     layers, n, Hkv, page, block, B, K = check_reorder(pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, page)
     _here(pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens)
     if B * K == 0:
