@@ -1,6 +1,6 @@
 // What a generation step decides on the GPU: which cache pages and slots the new tokens get, which continuations of the beams are kept, and the beams' tables,
 // histories and half-filled pages in the order of their parents.  Nothing here is read back by the host.
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace {
 
@@ -133,12 +133,21 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
 // beam that has ended goes on as itself: its one continuation is (eos, prev[k]).  Within a row the order of the scores is that of the logits, so a row's K
 // best can be found before its lse is known, in the one pass that reads it.
 //
-// Bound by the logits' bytes, then by an exponential for each.  A row is cut into pieces of at most 8192 logits (so many that the machine is filled), a thread
-// block keeps its piece in registers.  The K-th largest of 8 (K > 8: 32) maxima of parts of the piece is a bound below which nothing is among its K largest: one comparison beside
-// the exponential leaves a handful of candidates, which one warp sorts out.  Too many of them (logits all alike) take K rounds over the registers
-// instead.  The request's last thread block merges the pieces' sorted lists.
-constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_E = 32, SEL_PIECE = SEL_THREADS * SEL_E, SEL_MAX_K = 32, SEL_CAND = 256, SEL_LISTS = 8192, SEL_HELD = 2048;
+// Bound by the logits' bytes, then by an exponential for each.  A row is cut into as many pieces as fill the machine once, and a thread block fetches up to 32 KB of
+// its piece at a time into shared memory, by one bulk copy: many bytes on their way, and loops that are short (they run a few times only, so that instructions
+// fetched for the first time are a good part of a call).  The K-th largest of 8 (K > 4: 32) maxima of parts of what came first is a bound below which nothing
+// is among the piece's K largest: one comparison for 8 logits leaves some tens of candidates.  Where they become many, those behind the K-th go and it
+// is the bound from then on.  A candidate's place is the number of those before it.  More candidates at a time than there is room for (logits all alike) are forgotten:
+// then K rounds over the piece find its K largest.  The request's last thread block finds its K best among the pieces' sorted lists in the same way,
+// the bound being of its threads' best.
+constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_BYTES = 32768, SEL_MAX_K = 32, SEL_CAND = 512, SEL_HELD = 1024;
+constexpr int SEL_PER_SM = 6, SEL_LEAST = 2048;      // thread blocks that an SM holds; the smallest piece
 typedef unsigned long long u64;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 struct SelectArgs {
   float* scores;
   int *tokens, *parents, *done_out;
@@ -175,218 +184,301 @@ __device__ __forceinline__ u64 block_best(u64 k, u64* red) {
   for (int w = 1; w < SEL_WARPS; w++) k = max(k, red[w]);
   return k;
 }
-__device__ __forceinline__ float logit(float x) { return x != x ? -INFINITY : x; }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(SEL_THREADS) beam_select_k(const SelectArgs A) {
-  mlb_pdl_sync();
-  __shared__ float smax[32], ssum[SEL_WARPS];
-  __shared__ u64 cand[SEL_CAND], red[SEL_WARPS];
+// 8 neighbouring logits in shared memory, -inf for NaN, and the largest
+template <typename T> struct Eight;
+template <> struct Eight<bf16> {
+  uint32_t w[4];
+  __device__ __forceinline__ float load(const bf16* p) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    bf162 m;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const uint32_t ninf = 0xFF80FF80u;
+      const bf162 x = __hmax2(*reinterpret_cast<bf162*>(&w[k]), *reinterpret_cast<const bf162*>(&ninf));
+      w[k] = *reinterpret_cast<const uint32_t*>(&x);
+      m = k ? __hmax2(m, x) : x;
+    }
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  __device__ __forceinline__ float get(int k) const { return __uint_as_float(k % 2 ? w[k / 2] & 0xFFFF0000u : w[k / 2] << 16); }
+};
+template <> struct Eight<float> {
+  float x[8];
+  __device__ __forceinline__ float load(const float* p) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + k);
+      x[k] = fmaxf(v.x, -INFINITY), x[k + 1] = fmaxf(v.y, -INFINITY), x[k + 2] = fmaxf(v.z, -INFINITY), x[k + 3] = fmaxf(v.w, -INFINITY);
+      m = fmaxf(m, fmaxf(fmaxf(x[k], x[k + 1]), fmaxf(x[k + 2], x[k + 3])));
+    }
+    return m;
+  }
+  __device__ __forceinline__ float get(int k) const { return x[k]; }
+};
+// Number of the n keys at `keys` that come before `mine`; keys are distinct
+__device__ __forceinline__ int place_of(u64 mine, const u64* keys, int n) {
+  int before = 0;
+  for (int c = 0; c < n; c++) before += keys[c] > mine;
+  return before;
+}
+
+// The K-th largest of the maxima of 8 (K > 4: 32) parts of the threads' values: K of these are not below it.  tops: 32 values of shared memory
+template <typename X, typename Max>
+__device__ __forceinline__ X kth_of_parts(X m, int K, X* tops, Max larger) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = K <= 4 ? SEL_WARPS : 32;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (parts == SEL_WARPS) m = larger(m, __shfl_xor_sync(0xffffffffu, m, 8)), m = larger(m, __shfl_xor_sync(0xffffffffu, m, 16));
+  if (parts == SEL_WARPS ? lane == 0 : lane % 8 == 0) tops[parts == SEL_WARPS ? warp : warp * 4 + lane / 8] = m;
+  __syncthreads();
+  m = tops[lane % parts];
+  int better = 0;
+#pragma unroll 8
+  for (int o = 0; o < parts; o++) {
+    const X y = tops[o];
+    better += y > m || (y == m && o < lane);
+  }
+  return __shfl_sync(0xffffffffu, m, __ffs(__ballot_sync(0xffffffffu, better == K - 1)) - 1);
+}
+// Natural logarithm of a normal number, off by 2^-22 and a rounding: the exponent's part apart from that of a number of 1 ... 2
+__device__ __forceinline__ float log_of(float x) {
+  const int e = (int)(__float_as_uint(x) >> 23) - 127;
+  const float f = __uint_as_float((__float_as_uint(x) & 0x007FFFFFu) | 0x3F800000u);
+  return fmaf((float)e, 0.693145751953125f, fmaf((float)e, 1.42860682e-6f, __log2f(f) * 0.693147181f));
+}
+
+// BULK: rows begin on 16-byte boundaries
+template <typename T, bool BULK>
+__global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const SelectArgs A) {
+  extern __shared__ __align__(128) uint8_t fetched[];
+  __shared__ uint64_t bar;
+  __shared__ float tops[32], sums[SEL_WARPS];
+  __shared__ u64 cand[SEL_HELD], red[32];
   __shared__ int n_cand, last;
-  __shared__ float prev[SEL_MAX_K], lse[SEL_MAX_K];
-  __shared__ int ended[SEL_MAX_K];
-  __shared__ uint8_t head[SEL_LISTS];
-  __shared__ u64 held[SEL_HELD];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = A.K, V = A.V;
   const int row = blockIdx.y, req = row / K;
   const long list = (long)row * A.pieces + blockIdx.x;
+  if (tid == 0) {
+    n_cand = 0;
+    tc::mbar_init(&bar, 1);
+    tc::mbar_fence_init();
+  }
+  __syncthreads();
+  mlb_pdl_sync();
   if (!A.done[row]) {
+    constexpr int CHUNK = SEL_CHUNK_BYTES / sizeof(T);
+    T* data = reinterpret_cast<T*>(fetched);
     const int begin = blockIdx.x * A.piece, n = min(A.piece, V - begin);
     const T* z = reinterpret_cast<const T*>(A.logits) + row * A.stride + begin;
-    float x[SEL_E];
-    auto at = [&](int k) { return VEC ? (k / 8 * SEL_THREADS + tid) * 8 + k % 8 : k * SEL_THREADS + tid; };      // place of element k in the piece
+    float m = -INFINITY, s = 0.f, bound = -INFINITY;
+    int most = 0;      // candidates up to and with this thread's last
+    bool over = false;
+    uint32_t parity = 0;
+    for (int c = 0; c < n; c += CHUNK, parity ^= 1) {
+      const int count = min(CHUNK, n - c), whole = BULK ? (int)(count * sizeof(T) / 16 * 16 / sizeof(T)) : 0;
+      if (BULK && tid == 0 && whole > 0) {
+        tc::mbar_expect_tx(&bar, whole * sizeof(T));
+        tc::bulk_load(data, z + c, whole * sizeof(T), &bar);
+      }
+      for (int e = whole + tid; e < count; e += SEL_THREADS) data[e] = z[c + e];
+      if (tid < 8 && count + tid < (count + 7) / 8 * 8) data[count + tid] = (T)-INFINITY;
+      if (BULK && whole > 0) {
+        tc::mbar_wait(&bar, parity, 0xD3);
+        __syncwarp();
+      }
+      __syncthreads();
+      float top = -INFINITY;
+      Eight<T> x;
+#pragma unroll 2
+      for (int e = tid * 8; e < count; e += SEL_THREADS * 8) top = fmaxf(top, x.load(data + e));
+      const float kth = kth_of_parts(top, K, tops, [](float a, float b) { return fmaxf(a, b); });
+      if (c == 0) bound = kth;
+      top = warp_max(tops[lane % (K <= 4 ? SEL_WARPS : 32)]);
+      if (top > m) s *= ex2((m - top) * 1.44269504088896f), m = top;      // (from -inf: 0 times 0)
+      const float mm = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+      for (int e = tid * 8; e < count; e += SEL_THREADS * 8) {
+        const float best = x.load(data + e);
 #pragma unroll
-    for (int g = 0; g < SEL_E / 8; g++) {
-#pragma unroll
-      for (int k = 0; k < 8; k++) x[8 * g + k] = -INFINITY;
-      if (g * SEL_THREADS * 8 < n) {
-        if constexpr (VEC) {
-          const int p = at(8 * g);
-          if (p + 8 <= n) {
-            if constexpr (sizeof(T) == 2) {
-              const uint4 w = *reinterpret_cast<const uint4*>(z + p);
-              const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-              for (int k = 0; k < 4; k++) x[8 * g + 2 * k] = __uint_as_float(u[k] << 16), x[8 * g + 2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 2; k++) {
-                const float4 w = *reinterpret_cast<const float4*>(z + p + 4 * k);
-                x[8 * g + 4 * k] = w.x, x[8 * g + 4 * k + 1] = w.y, x[8 * g + 4 * k + 2] = w.z, x[8 * g + 4 * k + 3] = w.w;
-              }
+        for (int k = 0; k < 8; k++) s += ex2((x.get(k) - mm) * 1.44269504088896f);
+        if (best >= bound && !over)
+#pragma unroll 1
+          for (int k = 0; k < min(8, count - e); k++) {
+            const float v = fmaxf((float)data[e + k], -INFINITY);
+            if (v >= bound) {
+              most = atomicAdd(&n_cand, 1) + 1;
+              if (most <= SEL_CAND) cand[most - 1] = rank_of(v, begin + c + e + k);
             }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-              if (p + k < n) x[8 * g + k] = (float)z[p + k];
           }
-        } else {
+      }
+      const bool more = c + CHUNK < n;
+      if (__syncthreads_or(most > (more ? 2 * K : SEL_CAND))) {
+        over |= __syncthreads_or(most > SEL_CAND) != 0;
+        if (!over && more) {      // the K best of them stay
+          const int found = n_cand;
+          u64 mine[SEL_CAND / SEL_THREADS];
+          int place[SEL_CAND / SEL_THREADS];
 #pragma unroll
-          for (int k = 0; k < 8; k++)
-            if (at(8 * g + k) < n) x[8 * g + k] = (float)z[at(8 * g + k)];
+          for (int h = 0; h < SEL_CAND / SEL_THREADS; h++) {
+            const int e = tid + h * SEL_THREADS;
+            mine[h] = e < found ? cand[e] : 0ull;
+            place[h] = e < found ? place_of(mine[h], cand, found) : K;
+          }
+          __syncthreads();
+#pragma unroll
+          for (int h = 0; h < SEL_CAND / SEL_THREADS; h++)
+            if (place[h] < K) cand[place[h]] = mine[h];
+          if (tid == 0) n_cand = K;
+          __syncthreads();
+          bound = unordered((uint32_t)(cand[K - 1] >> 32));
+          __syncthreads();
         }
+        most = 0;
       }
+      tc::fence_async_smem();      // (the next bulk copy writes what has been read)
+      if (more) __syncthreads();
     }
-    float m = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < SEL_E; k++) x[k] = logit(x[k]), m = fmaxf(m, x[k]);
-    // maxima of 32 parts of the piece: a part is 8 threads
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((lane & 7) == 0) smax[warp * 4 + (lane >> 3)] = m;
-    if (tid == 0) n_cand = 0;
-    __syncthreads();
-    m = smax[lane];
-    int better = 0;
-#pragma unroll
-    for (int o = 1; o < 32; o++) {
-      const float y = __shfl_xor_sync(0xffffffffu, m, o);
-      better += y > m || (y == m && (lane ^ o) < lane);
-    }
-    const float bound = __shfl_sync(0xffffffffu, m, __ffs(__ballot_sync(0xffffffffu, better == K - 1)) - 1);
-    m = warp_max(m);
-    const float mm = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < SEL_E; k++) {
-      s += exp2f((x[k] - mm) * 1.44269504088896f);
-      if (x[k] >= bound && at(k) < n) {
-        const int c = atomicAdd(&n_cand, 1);
-        if (c < SEL_CAND) cand[c] = rank_of(x[k], begin + at(k));
-      }
-    }
+    // the piece's sum
     s = warp_sum(s);
-    if (lane == 0) ssum[warp] = s;
+    if (lane == 0) sums[warp] = s;
     __syncthreads();
     if (tid == 0) {
       s = 0.f;
-      for (int w = 0; w < SEL_WARPS; w++) s += ssum[w];
+#pragma unroll
+      for (int w = 0; w < SEL_WARPS; w++) s += sums[w];
       A.stats[list] = make_float2(m, s);
     }
-    if (n_cand <= SEL_CAND) {
-      if (warp == 0) {
-        u64 mine[SEL_CAND / 32];
-#pragma unroll
-        for (int c = 0; c < SEL_CAND / 32; c++) mine[c] = c * 32 + lane < n_cand ? cand[c * 32 + lane] : 0ull;
-        for (int k = 0; k < K; k++) {
-          u64 best = 0;
-#pragma unroll
-          for (int c = 0; c < SEL_CAND / 32; c++) best = max(best, mine[c]);
-          best = warp_best(best);
-#pragma unroll
-          for (int c = 0; c < SEL_CAND / 32; c++)
-            if (mine[c] == best) mine[c] = 0;
-          if (lane == 0) {
-            A.values[list * K + k] = best ? unordered((uint32_t)(best >> 32)) : -INFINITY;
-            A.ids[list * K + k] = best ? (int)~(uint32_t)best : -1;
-          }
-        }
+    if (!over) {
+      const int found = n_cand;
+      for (int e = tid; e < found; e += SEL_THREADS) {
+        const u64 mine = cand[e];
+        const int k = place_of(mine, cand, found);
+        if (k < K) A.values[list * K + k] = unordered((uint32_t)(mine >> 32)), A.ids[list * K + k] = (int)~(uint32_t)mine;
       }
+      if (tid >= found && tid < K) A.ids[list * K + tid] = -1;      // (a piece of fewer than K logits)
     } else {
       u64 prior = ~0ull;
       for (int k = 0; k < K; k++) {
         u64 best = 0;
-#pragma unroll
-        for (int c = 0; c < SEL_E; c++) {
-          const u64 r = at(c) < n ? rank_of(x[c], begin + at(c)) : 0ull;
+        for (int e = tid; e < n; e += SEL_THREADS) {
+          const u64 r = rank_of(fmaxf((float)z[e], -INFINITY), begin + e);
           if (r < prior) best = max(best, r);
         }
         prior = best = block_best(best, red);
-        if (tid == 0) {
-          A.values[list * K + k] = best ? unordered((uint32_t)(best >> 32)) : -INFINITY;
-          A.ids[list * K + k] = best ? (int)~(uint32_t)best : -1;
-        }
+        if (tid == 0) A.values[list * K + k] = unordered((uint32_t)(best >> 32)), A.ids[list * K + k] = (int)~(uint32_t)best;
       }
     }
   }
   // ---- the request's last thread block merges
-  __threadfence();
   __syncthreads();
-  if (tid == 0) last = atomicAdd(A.ticket + req, 1) == A.pieces * K - 1;
+  if (tid == 0) {
+    __threadfence();      // (the block's list before the count)
+    last = atomicAdd(A.ticket + req, 1) == A.pieces * K - 1;
+    __threadfence();
+  }
   __syncthreads();
   if (!last) return;
-  __threadfence();
-  if (tid == 0) A.ticket[req] = 0;
+  __shared__ float prev[SEL_MAX_K], lse[SEL_MAX_K];
+  __shared__ int ended[SEL_MAX_K];
+  const int lists = K * A.pieces;
+  if (tid == 0) A.ticket[req] = 0, n_cand = 0;
+  // the lists' entries, their first ones before their second ones
+  constexpr int HELD = SEL_HELD / SEL_THREADS;
+  const float per_list = 1.f / lists, per_beam = 1.f / A.pieces;      // ((x + 1/2) / n rounded down is exact for the few thousands that these are)
+  float val[HELD];
+  int tok[HELD];
+#pragma unroll
+  for (int h = 0; h < HELD; h++) {
+    const int e = tid + h * SEL_THREADS;
+    tok[h] = -1, val[h] = 0.f;
+    if (e < lists * K) {
+      const int nth = (int)((e + 0.5f) * per_list);
+      const long a = ((long)req * lists + e - nth * lists) * K + nth;
+      tok[h] = __ldcg(A.ids + a), val[h] = __ldcg(A.values + a);
+    }
+  }
   if (tid < K) prev[tid] = A.prev[req * K + tid], ended[tid] = A.done[req * K + tid] != 0;
   for (int k = warp; k < K; k += SEL_WARPS) {
     if (A.done[req * K + k]) continue;
     const float2* st = A.stats + (long)(req * K + k) * A.pieces;
+    float2 v[2];      // (pieces past 64 are read again)
     float m = -INFINITY;
-    for (int p = lane; p < A.pieces; p += 32) m = fmaxf(m, __ldcg(st + p).x);
+#pragma unroll
+    for (int h = 0; h < 2; h++) v[h] = lane + 32 * h < A.pieces ? __ldcg(st + lane + 32 * h) : make_float2(-INFINITY, 0.f), m = fmaxf(m, v[h].x);
+    for (int p = lane + 64; p < A.pieces; p += 32) m = fmaxf(m, __ldcg(st + p).x);
     m = warp_max(m);
-    float s = 0.f;
-    for (int p = lane; p < A.pieces; p += 32) {
-      const float2 v = __ldcg(st + p);
-      s += v.x == m ? v.y : v.y * exp2f((v.x - m) * 1.44269504088896f);
-    }
+    auto term = [&](const float2& t) { return t.x == m ? t.y : t.y * ex2((t.x - m) * 1.44269504088896f); };
+    float s = (lane < A.pieces ? term(v[0]) : 0.f) + (lane + 32 < A.pieces ? term(v[1]) : 0.f);
+    for (int p = lane + 64; p < A.pieces; p += 32) s += term(__ldcg(st + p));
     s = warp_sum(s);
-    if (lane == 0) lse[k] = m + (float)log((double)s);
+    if (lane == 0) lse[k] = s > 0.f ? m + log_of(s) : -INFINITY;
   }
-  const int lists = K * A.pieces;
-  for (int l = tid; l < lists; l += SEL_THREADS) head[l] = 0;
   __syncthreads();
-  // a beam of no continuation: it was nothing, or its logits have no logarithm of a sum
-  auto dead = [&](int k) { return !ended[k] && !(prev[k] > -INFINITY && fabsf(lse[k]) < INFINITY); };
-  auto rank = [&](int l, int h) -> u64 {      // entry h of list l, 0: no more
-    const int k = l / A.pieces, p = l % A.pieces;
-    float x;
-    int tok;
-    if (ended[k] || dead(k)) {
-      if (p != 0) return 0;
-      if (ended[k] && A.eos >= 0 && A.eos < V) {
-        tok = h == 0 ? A.eos : h - 1 < A.eos ? h - 1 : h;
-        x = h == 0 ? prev[k] : -INFINITY;
-        if (x != x) x = -INFINITY;
+  u64 key[HELD], best = 0;
+#pragma unroll
+  for (int h = 0; h < HELD; h++) {
+    const int e = tid + h * SEL_THREADS;
+    key[h] = 0;
+    if (e < lists * K) {
+      const int nth = (int)((e + 0.5f) * per_list), l = e - nth * lists, k = (int)((l + 0.5f) * per_beam);
+      int t = tok[h];
+      float x = val[h];
+      // a beam that has ended, and one of no continuation: it was nothing, or its logits have no logarithm of a sum
+      const bool end = ended[k] != 0, dead = !end && !(prev[k] > -INFINITY && fabsf(lse[k]) < INFINITY);
+      if (end || dead) {
+        x = -INFINITY, t = nth;
+        if (end && A.eos >= 0 && A.eos < V) {
+          t = nth == 0 ? A.eos : nth - 1 < A.eos ? nth - 1 : nth;
+          if (nth == 0) x = prev[k];
+        }
+        if (l != k * A.pieces || t >= V) t = -1;
       } else {
-        tok = h, x = -INFINITY;
+        x = __fadd_rn(prev[k], __fsub_rn(x, lse[k]));
       }
-      if (tok >= V) return 0;
-    } else {
-      const long a = ((long)(req * K + k) * A.pieces + p) * K + h;
-      tok = __ldcg(A.ids + a);
-      if (tok < 0) return 0;
-      x = __fadd_rn(prev[k], __fsub_rn(__ldcg(A.values + a), lse[k]));
-      if (x != x) x = -INFINITY;
+      if (t >= 0) key[h] = rank_of(x != x ? -INFINITY : x, (uint32_t)k * (uint32_t)V + (uint32_t)t);
     }
-    return rank_of(x, (uint32_t)k * (uint32_t)V + (uint32_t)tok);
-  };
-  const bool keep = lists * K <= SEL_HELD;
-  if (keep)
-    for (int e = tid; e < lists * K; e += SEL_THREADS) held[e] = rank(e / K, e % K);
+    best = max(best, key[h]);
+  }
+  const u64 bound = kth_of_parts(best, K, red, [](u64 a, u64 b) { return a > b ? a : b; });
+#pragma unroll
+  for (int h = 0; h < HELD; h++)
+    if (key[h] != 0 && key[h] >= bound) cand[atomicAdd(&n_cand, 1)] = key[h];
   __syncthreads();
-  u64 best = 0;      // the best head of this thread's lists, and whose it is
-  int mine = -1;
-  auto choose = [&] {
-    best = 0;
-    for (int l = tid; l < lists; l += SEL_THREADS) {
-      const int h = head[l];
-      const u64 r = h >= K ? 0ull : keep ? held[l * K + h] : rank(l, h);
-      if (r > best) best = r, mine = l;
+  const int found = n_cand;
+  for (int e = tid; e < found; e += SEL_THREADS) {
+    const u64 mine = cand[e];
+    const int k = place_of(mine, cand, found);
+    if (k < K) {
+      const uint32_t flat = ~(uint32_t)mine;
+      const int from = (int)(flat / (uint32_t)V), t = (int)(flat % (uint32_t)V), o = req * K + k;
+      A.scores[o] = unordered((uint32_t)(mine >> 32));
+      A.tokens[o] = t, A.parents[o] = from, A.done_out[o] = ended[from] || t == A.eos;
     }
-  };
-  choose();
-  for (int k = 0; k < K; k++) {
-    const u64 top = block_best(best, red);
-    if (best == top && top != 0) {
-      const uint32_t flat = ~(uint32_t)top;
-      const int from = (int)(flat / (uint32_t)V), tok = (int)(flat % (uint32_t)V), o = req * K + k;
-      A.scores[o] = unordered((uint32_t)(top >> 32));
-      A.tokens[o] = tok, A.parents[o] = from, A.done_out[o] = ended[from] || tok == A.eos;
-      head[mine]++;
-      choose();
-    }
-    if (top == 0 && tid == 0) {      // fewer continuations than beams (V < K)
-      const int o = req * K + k;
-      A.scores[o] = -INFINITY, A.tokens[o] = A.eos, A.parents[o] = 0, A.done_out[o] = 1;
-    }
+  }
+  if (tid >= found && tid < K) {      // fewer continuations than beams (V < K)
+    const int o = req * K + tid;
+    A.scores[o] = -INFINITY, A.tokens[o] = A.eos, A.parents[o] = 0, A.done_out[o] = 1;
   }
 }
 
-// Logits of a piece, a multiple of 8: at least a wave of thread blocks (4 an SM) where the rows give as much, 1024 logits and more each
-int select_piece(int rows, int V) {
-  const long least = (V + SEL_PIECE - 1) / SEL_PIECE, most = (V + 1023) / 1024, want = (4L * mlb_sm_count() + rows - 1) / rows;
-  const long n = want < least ? least : want > most ? most : want;
+// Logits of a piece, a multiple of 8: the machine's thread blocks once over the rows, but no more of a row than one fetch where there are enough of them, SEL_LEAST
+// logits and more each, and no more lists than a thread block holds to merge
+int select_piece(int rows, int K, int V, int bits) {
+  const long fill = (long)SEL_PER_SM * mlb_sm_count() / rows, one = ((long)V * (bits / 8) + SEL_CHUNK_BYTES - 1) / SEL_CHUNK_BYTES, most = (V + SEL_LEAST - 1) / SEL_LEAST,
+             held = SEL_HELD / (K * K);
+  long n = fill > one ? fill : one;
+  n = n < most ? n : most;
+  n = n < held ? n : held;
+  n = n < 1 ? 1 : n;
   return (int)((V + n - 1) / n + 7) / 8 * 8;
+}
+template <typename T, bool BULK>
+cudaError_t launch_select(const SelectArgs& a, int rows, cudaStream_t st) {
+  const int bytes = a.piece * (int)sizeof(T) < SEL_CHUNK_BYTES ? a.piece * (int)sizeof(T) : SEL_CHUNK_BYTES;
+  return mlb_launch(beam_select_k<T, BULK>, dim3(a.pieces, rows), dim3(SEL_THREADS), (bytes + 127) / 128 * 128, st, a);
 }
 
 // ------------------------------------------------------------------ beams in the order of their parents
@@ -447,21 +539,20 @@ MLB_API int mlb_block_tables(int* table, int* slots, int* pos, int* starts, int*
 }
 
 // Pieces that a row of V logits is cut into, and (-7) nothing for what the kernel does not take
-MLB_API int mlb_beam_select_pieces(int rows, int K, int V) {
+MLB_API int mlb_beam_select_pieces(int rows, int K, int V, int bits) {
   if (K < 1 || K > SEL_MAX_K || V < 1 || rows < 1 || rows > 65535 || (long)K * V >= 0xFFFFFFFFL) return -7;
-  const int piece = select_piece(rows, V), pieces = (V + piece - 1) / piece;
-  return (long)pieces * K > SEL_LISTS ? -7 : pieces;
+  const int piece = select_piece(rows, K, V, bits);
+  return (V + piece - 1) / piece;
 }
 // bits: 16 (bf16) or 32 (fp32) logits, rows `stride` elements apart
 MLB_API int mlb_beam_select(float* scores, int* tokens, int* parents, int* done_out, const void* logits, const float* prev, const int* done, float* stats,
                             float* values, int* ids, int* ticket, int rows, int K, int V, long stride, int eos, int bits, cudaStream_t st) {
-  const int pieces = mlb_beam_select_pieces(rows, K, V);
+  const int pieces = mlb_beam_select_pieces(rows, K, V, bits);
   if (pieces < 0 || rows % K != 0) return -7;
-  const SelectArgs a{scores, tokens, parents, done_out, logits, prev, done, (float2*)stats, values, ids, ticket, stride, K, V, eos, pieces, select_piece(rows, V)};
-  const bool vec = ((uintptr_t)logits & 15) == 0 && stride * (bits / 8) % 16 == 0;
-  const dim3 grid(pieces, rows), block(SEL_THREADS);
-  if (bits == 16) return (int)(vec ? mlb_launch(beam_select_k<bf16, true>, grid, block, 0, st, a) : mlb_launch(beam_select_k<bf16, false>, grid, block, 0, st, a));
-  return (int)(vec ? mlb_launch(beam_select_k<float, true>, grid, block, 0, st, a) : mlb_launch(beam_select_k<float, false>, grid, block, 0, st, a));
+  const SelectArgs a{scores, tokens, parents, done_out, logits, prev, done, (float2*)stats, values, ids, ticket, stride, K, V, eos, pieces, select_piece(rows, K, V, bits)};
+  const bool bulk = ((uintptr_t)logits & 15) == 0 && stride * (bits / 8) % 16 == 0;
+  if (bits == 16) return (int)(bulk ? launch_select<bf16, true>(a, rows, st) : launch_select<bf16, false>(a, rows, st));
+  return (int)(bulk ? launch_select<float, true>(a, rows, st) : launch_select<float, false>(a, rows, st));
 }
 
 // pages null: no cache to copy in; block_bytes of 16 tokens of a head

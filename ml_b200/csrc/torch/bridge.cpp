@@ -86,7 +86,7 @@ typedef std::optional<Tensor> Maybe;      // (an undefined tensor is no argument
   X(mlb_kv4_attn_scratch, long, (int, int, int, int, int, int, int))                                                                           \
   X(mlb_kv4_attn, int, (void*, float*, const void*, const uint8_t*, const int*, const int*, float*, int*, long, long, int, int, int, int, int, int, int, float, St)) \
   X(mlb_block_tables, int, (int*, int*, int*, int*, int*, int*, int*, const int*, const int*, const int*, const int*, int, int, int, int, int, St)) \
-  X(mlb_beam_select_pieces, int, (int, int, int))                                                                                              \
+  X(mlb_beam_select_pieces, int, (int, int, int, int))                                                                                              \
   X(mlb_beam_select, int, (float*, int*, int*, int*, const void*, const float*, const int*, float*, float*, int*, int*, int, int, int, long, int, int, St)) \
   X(mlb_beam_reorder, int, (uint8_t*, int*, int*, int*, const int*, const int*, const int*, const int*, const int*, const int*, int, long, int, int, int, int, int, int, int, St))
 #define MLB_POINTER(name, ret, args) ret(*name) args = nullptr;
@@ -701,7 +701,7 @@ PyObject* py_beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {      // 
       !given(a[3], done_out, at::kInt, {B, Kb}) || !given(a[6], done, at::kInt, {B, Kb}) || rows >= (1L << 31))
     return declined();
   const St st = stream();
-  const long V = z.size(1), pieces = K.mlb_beam_select_pieces((int)rows, (int)Kb, (int)V);
+  const long V = z.size(1), pieces = K.mlb_beam_select_pieces((int)rows, (int)Kb, (int)V, half ? 16 : 32);
   if (pieces < 0 || K.mlb_capture_id(st) != 0) return declined();
   const long m = rows * pieces;
   const Kept& w = kept(KEPT_SELECT, prev, st, m * (2 + 2 * Kb), B);

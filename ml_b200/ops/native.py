@@ -44,7 +44,7 @@ _KINDS = {
 # ... and those of generation: the 4-bit key / value cache, tables, beams (ops/native_gen.py)
 _GEN_KINDS = {
     "kv4_append": "ubbiifflnllnnnns", "kv4_read": "bbuilnlnns", "kv4_attn_scratch": "nnnnnnn", "kv4_attn": "bfbuiifillnnnnnnnds",
-    "block_tables": "iiiiiiiiiiinnnnns", "beam_select_pieces": "nnn", "beam_select": "fiiibfiffiinnnlnns",
+    "block_tables": "iiiiiiiiiiinnnnns", "beam_select_pieces": "nnnn", "beam_select": "fiiibfiffiinnnlnns",
     "beam_reorder": "uiiiiiiiiinlnnnnnnns"}
 _CTYPES = {"n": _i32, "l": _i64, "d": _f32}      # (else a pointer)
 

@@ -96,15 +96,15 @@ def beam_select(scores, tokens, parents, done_out, logits, prev, done, eos):
         return
     if V > 1 and logits.stride(1) != 1:
         raise ValueError("logits: need rows of neighbouring elements")
-    e, dev, rows = _n._entries(), logits.device, B * K
-    pieces = e.mlb_beam_select_pieces(rows, K, V)
+    e, dev, rows, bits = _n._entries(), logits.device, B * K, 16 if logits.dtype == torch.bfloat16 else 32
+    pieces = e.mlb_beam_select_pieces(rows, K, V, bits)
     if pieces < 0:
-        raise ValueError(f"{B} x {K} beams of {V} logits: at most 65535 rows, and 8192 pieces of 8192 logits in a request")
+        raise ValueError(f"{B} x {K} beams: at most 65535 rows")
     part = _n.scratch("select_part", rows * pieces * (2 + 2 * K), F32, dev)
     ticket = _n.scratch("select_ticket", B, I32, dev, zero=True)
     base, n = part.data_ptr(), rows * pieces
     _n._chk(e.mlb_beam_select(scores, tokens, parents, done_out, Address(logits.data_ptr()), prev, done, part, Address(base + 8 * n), Address(base + 8 * n + 4 * n * K),
-                              ticket, rows, K, V, logits.stride(0), eos, 16 if logits.dtype == torch.bfloat16 else 32), "beam_select")
+                              ticket, rows, K, V, logits.stride(0), eos, bits), "beam_select")
 
 
 def beam_reorder(pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, page=None):
