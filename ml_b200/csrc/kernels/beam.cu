@@ -135,10 +135,10 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
 //
 // Bound by the logits' bytes, then by an exponential for each.  A row is cut into as many pieces as fill the machine once, and a thread block fetches up to 32 KB of
 // its piece at a time into shared memory, by one bulk copy: many bytes on their way, and loops that are short (they run a few times only, so that instructions
-// fetched for the first time are a good part of a call).  The K-th largest of 8 (K > 4: 32) maxima of parts of what came first is a bound below which nothing
+// fetched for the first time are a good part of a call).  The K-th largest of the maxima of 8 to 32 parts of what came first is a bound below which nothing
 // is among the piece's K largest: one comparison for 8 logits leaves some tens of candidates.  Where they become many, those behind the K-th go and it
 // is the bound from then on.  A candidate's place is the number of those before it.  More candidates at a time than there is room for (logits all alike) are forgotten:
-// then K rounds over the piece find its K largest.  The request's last thread block finds its K best among the pieces' sorted lists in the same way,
+// then K rounds over the piece find its K largest.  The request's last thread block finds its K best among the pieces' lists in the same way,
 // the bound being of its threads' best.
 constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_BYTES = 32768, SEL_MAX_K = 32, SEL_CAND = 512, SEL_HELD = 1024;
 constexpr int SEL_PER_SM = 6, SEL_LEAST = 2048;      // thread blocks that an SM holds; the smallest piece
@@ -155,11 +155,11 @@ struct SelectArgs {
   const float* prev;
   const int* done;
   float2* stats;      // [rows][pieces]: maximum, sum of exponentials
-  float* values;      // [rows][pieces][K], largest first
-  int* ids;           // [rows][pieces][K], -1: no more
+  float* values;      // [rows][pieces][L]: the K best and maybe others
+  int* ids;           // [rows][pieces][L], -1: none
   int* ticket;
   long stride;
-  int K, V, eos, pieces, piece;
+  int K, L, V, eos, pieces, piece;
 };
 // Order of candidates as whole numbers: larger value first, then the lower index
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -221,18 +221,21 @@ template <> struct Eight<float> {
 // Number of the n keys at `keys` that come before `mine`; keys are distinct
 __device__ __forceinline__ int place_of(u64 mine, const u64* keys, int n) {
   int before = 0;
+#pragma unroll 8
   for (int c = 0; c < n; c++) before += keys[c] > mine;
   return before;
 }
 
-// The K-th largest of the maxima of 8 (K > 4: 32) parts of the threads' values: K of these are not below it.  tops: 32 values of shared memory
+// Parts of a thread block whose maxima bound its K largest: warps, halves or quarters of them
+__device__ __forceinline__ int parts_for(int K) { return K <= SEL_WARPS / 2 ? SEL_WARPS : K <= SEL_WARPS ? 2 * SEL_WARPS : 4 * SEL_WARPS; }
+// The K-th largest of the maxima of the parts' values: K of these are not below it.  tops: 32 values of shared memory
 template <typename X, typename Max>
 __device__ __forceinline__ X kth_of_parts(X m, int K, X* tops, Max larger) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = K <= 4 ? SEL_WARPS : 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = parts_for(K), each = SEL_THREADS / parts;      // 8, 16 or 32 threads
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (parts == SEL_WARPS) m = larger(m, __shfl_xor_sync(0xffffffffu, m, 8)), m = larger(m, __shfl_xor_sync(0xffffffffu, m, 16));
-  if (parts == SEL_WARPS ? lane == 0 : lane % 8 == 0) tops[parts == SEL_WARPS ? warp : warp * 4 + lane / 8] = m;
+  for (int o = 8; o < each; o <<= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane % each == 0) tops[(warp * 32 + lane) / each] = m;
   __syncthreads();
   m = tops[lane % parts];
   int better = 0;
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
       for (int e = tid * 8; e < count; e += SEL_THREADS * 8) top = fmaxf(top, x.load(data + e));
       const float kth = kth_of_parts(top, K, tops, [](float a, float b) { return fmaxf(a, b); });
       if (c == 0) bound = kth;
-      top = warp_max(tops[lane % (K <= 4 ? SEL_WARPS : 32)]);
+      top = warp_max(tops[lane % parts_for(K)]);
       if (top > m) s *= ex2((m - top) * 1.44269504088896f), m = top;      // (from -inf: 0 times 0)
       const float mm = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
@@ -304,15 +307,17 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
         const float best = x.load(data + e);
 #pragma unroll
         for (int k = 0; k < 8; k++) s += ex2((x.get(k) - mm) * 1.44269504088896f);
-        if (best >= bound && !over)
-#pragma unroll 1
-          for (int k = 0; k < min(8, count - e); k++) {
-            const float v = fmaxf((float)data[e + k], -INFINITY);
-            if (v >= bound) {
-              most = atomicAdd(&n_cand, 1) + 1;
-              if (most <= SEL_CAND) cand[most - 1] = rank_of(v, begin + c + e + k);
-            }
+        if (best >= bound && !over) {
+          uint32_t hits = 0;
+#pragma unroll
+          for (int k = 0; k < 8; k++) hits |= (x.get(k) >= bound ? 1u : 0u) << k;
+          hits &= 0xFFu >> max(0, 8 - (count - e));
+          for (; hits != 0; hits &= hits - 1) {
+            const int k = __ffs(hits) - 1;
+            most = atomicAdd(&n_cand, 1) + 1;
+            if (most <= SEL_CAND) cand[most - 1] = rank_of(fmaxf((float)data[e + k], -INFINITY), begin + c + e + k);
           }
+        }
       }
       const bool more = c + CHUNK < n;
       if (__syncthreads_or(most > (more ? 2 * K : SEL_CAND))) {
@@ -351,14 +356,15 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
       for (int w = 0; w < SEL_WARPS; w++) s += sums[w];
       A.stats[list] = make_float2(m, s);
     }
+    const int L = A.L;
     if (!over) {
       const int found = n_cand;
       for (int e = tid; e < found; e += SEL_THREADS) {
         const u64 mine = cand[e];
-        const int k = place_of(mine, cand, found);
-        if (k < K) A.values[list * K + k] = unordered((uint32_t)(mine >> 32)), A.ids[list * K + k] = (int)~(uint32_t)mine;
+        const int k = found <= L ? e : place_of(mine, cand, found);      // (the merge needs no order)
+        if (k < L) A.values[list * L + k] = unordered((uint32_t)(mine >> 32)), A.ids[list * L + k] = (int)~(uint32_t)mine;
       }
-      if (tid >= found && tid < K) A.ids[list * K + tid] = -1;      // (a piece of fewer than K logits)
+      if (tid >= found && tid < L) A.ids[list * L + tid] = -1;
     } else {
       u64 prior = ~0ull;
       for (int k = 0; k < K; k++) {
@@ -368,8 +374,9 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
           if (r < prior) best = max(best, r);
         }
         prior = best = block_best(best, red);
-        if (tid == 0) A.values[list * K + k] = unordered((uint32_t)(best >> 32)), A.ids[list * K + k] = (int)~(uint32_t)best;
+        if (tid == 0) A.values[list * L + k] = unordered((uint32_t)(best >> 32)), A.ids[list * L + k] = (int)~(uint32_t)best;
       }
+      if (tid >= K && tid < L) A.ids[list * L + tid] = -1;
     }
   }
   // ---- the request's last thread block merges
@@ -383,7 +390,7 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
   if (!last) return;
   __shared__ float prev[SEL_MAX_K], lse[SEL_MAX_K];
   __shared__ int ended[SEL_MAX_K];
-  const int lists = K * A.pieces;
+  const int lists = K * A.pieces, L = A.L;
   if (tid == 0) A.ticket[req] = 0, n_cand = 0;
   // the lists' entries, their first ones before their second ones
   constexpr int HELD = SEL_HELD / SEL_THREADS;
@@ -394,9 +401,9 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
   for (int h = 0; h < HELD; h++) {
     const int e = tid + h * SEL_THREADS;
     tok[h] = -1, val[h] = 0.f;
-    if (e < lists * K) {
+    if (e < lists * L) {
       const int nth = (int)((e + 0.5f) * per_list);
-      const long a = ((long)req * lists + e - nth * lists) * K + nth;
+      const long a = ((long)req * lists + e - nth * lists) * L + nth;
       tok[h] = __ldcg(A.ids + a), val[h] = __ldcg(A.values + a);
     }
   }
@@ -422,7 +429,7 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
   for (int h = 0; h < HELD; h++) {
     const int e = tid + h * SEL_THREADS;
     key[h] = 0;
-    if (e < lists * K) {
+    if (e < lists * L) {
       const int nth = (int)((e + 0.5f) * per_list), l = e - nth * lists, k = (int)((l + 0.5f) * per_beam);
       int t = tok[h];
       float x = val[h];
@@ -466,9 +473,10 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
 
 // Logits of a piece, a multiple of 8: the machine's thread blocks once over the rows, but no more of a row than one fetch where there are enough of them, SEL_LEAST
 // logits and more each, and no more lists than a thread block holds to merge
+int select_list(int K) { return K <= 16 ? 2 * K : K; }      // entries of a piece's list: usually all its candidates, which then need no places
 int select_piece(int rows, int K, int V, int bits) {
   const long fill = (long)SEL_PER_SM * mlb_sm_count() / rows, one = ((long)V * (bits / 8) + SEL_CHUNK_BYTES - 1) / SEL_CHUNK_BYTES, most = (V + SEL_LEAST - 1) / SEL_LEAST,
-             held = SEL_HELD / (K * K);
+             held = SEL_HELD / (K * select_list(K));
   long n = fill > one ? fill : one;
   n = n < most ? n : most;
   n = n < held ? n : held;
@@ -549,7 +557,7 @@ MLB_API int mlb_beam_select(float* scores, int* tokens, int* parents, int* done_
                             float* values, int* ids, int* ticket, int rows, int K, int V, long stride, int eos, int bits, cudaStream_t st) {
   const int pieces = mlb_beam_select_pieces(rows, K, V, bits);
   if (pieces < 0 || rows % K != 0) return -7;
-  const SelectArgs a{scores, tokens, parents, done_out, logits, prev, done, (float2*)stats, values, ids, ticket, stride, K, V, eos, pieces, select_piece(rows, K, V, bits)};
+  const SelectArgs a{scores, tokens, parents, done_out, logits, prev, done, (float2*)stats, values, ids, ticket, stride, K, select_list(K), V, eos, pieces, select_piece(rows, K, V, bits)};
   const bool bulk = ((uintptr_t)logits & 15) == 0 && stride * (bits / 8) % 16 == 0;
   if (bits == 16) return (int)(bulk ? launch_select<bf16, true>(a, rows, st) : launch_select<bf16, false>(a, rows, st));
   return (int)(bulk ? launch_select<float, true>(a, rows, st) : launch_select<float, false>(a, rows, st));
