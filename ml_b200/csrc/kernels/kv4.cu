@@ -27,106 +27,129 @@ __device__ __forceinline__ float bf16_bits(uint32_t hi) { return __uint_as_float
 __device__ __forceinline__ float lo_bf16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_bf16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000F000Fu; }       // two codes as fp16 c 2^-24
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00F000F0u; }      // c 2^-20
+__device__ __forceinline__ uint32_t value_codes(uint32_t w) {      // two codes as bf16 c - 8
+  const uint32_t x = low_codes(w) | 0x43004300u, k = 0x43084308u;      // 128 + c, 136
+  const bf162 y = __hsub2(*reinterpret_cast<const bf162*>(&x), *reinterpret_cast<const bf162*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
 // ------------------------------------------------------------------ append
-// A thread has 8 neighbouring elements of one head of one row, 4 threads a group.  Products and sums of the rotation are rounded one by one, so that
-// the value which is cut to 4 bits does not depend on what the compiler contracts.
+// A thread has 8 neighbouring elements of one head, 4 threads a group, and goes over rows.  Products and sums of the rotation are rounded one by one, so that the value
+// which is cut to 4 bits does not depend on what the compiler contracts.  Bound by the bytes of the rows, and about as much by instructions: 100 for 8
+// elements, so the quotients share a reciprocal and the codes are put together by multiply-adds.
 __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int k = 0; k < 4; k++) x[2 * k] = lo_bf16(u[k]), x[2 * k + 1] = hi_bf16(u[k]);
 }
 struct Group { uint32_t codes; uint16_t scale; };
-__device__ __forceinline__ Group to_codes(const float (&x)[8]) {
-  float hi = x[0], lo = x[0];
-  uint32_t mag = 0;      // the largest magnitude's bits: those of infinities and NaN are the highest
+// x / s as rounded to nearest: the rounded reciprocal's product corrected by its remainder is that (Markstein, Computation of elementary functions on the IBM RISC
+// System/6000 processor, 1990), as long as nothing on the way is subnormal
+__device__ __forceinline__ float quotient(float x, float s, float rs) {
+  const float q = x * rs;
+  return fmaf(fmaf(-q, s, x), rs, q);
+}
+__device__ __forceinline__ Group to_codes(const float (&x)[8], unsigned mask) {
+  // a number's bits turned left by one have its magnitude above its sign: the largest are of the largest magnitude, of a tie the negative one's
+  uint32_t top = 0;
 #pragma unroll
-  for (int e = 0; e < 8; e++) hi = fmaxf(hi, x[e]), lo = fminf(lo, x[e]), mag = max(mag, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, o));
-  }
-  const bf16 sb = __float2bfloat16_rn((hi > -lo ? hi : lo) * -0.125f);
+  for (int e = 0; e < 8; e++) top = max(top, __funnelshift_l(__float_as_uint(x[e]), __float_as_uint(x[e]), 1));
+  top = max(top, __shfl_xor_sync(mask, top, 1));
+  top = max(top, __shfl_xor_sync(mask, top, 2));
+  const bf16 sb = __float2bfloat16_rn(__uint_as_float(__funnelshift_r(top, top, 1)) * -0.125f);
   const float s = __bfloat162float(sb);
   Group g{0x88888888u, __bfloat16_as_ushort(sb)};
-  if (mag >= 0x7F800000u) {
+  if (top >= 0xFF000000u) {      // an infinity or NaN among them
     g.scale = 0x7FC0;      // NaN
   } else if (fabsf(s) < TINY) {
     g.scale = 0;
   } else {
-    g.codes = 0;
+    // Quotients go from -8 to 8 and the scale's rounding: 8 alone is one code too many.  1.5 2^23 + 8: the sum's last bits are the quotient rounded to nearest even, + 8
+    uint32_t w = 0;
+    auto add = [&](float q) { w = w * 16u + __float_as_uint(fminf(q, 7.f) + 12582920.f); };
+    if (fabsf(s) >= 8.67361738e-19f) {      // 2^-60
+      const float rs = __frcp_rn(s);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int c = min(max(__float2int_rn(__fdiv_rn(x[e], s)) + 8, 0), 15);
-      g.codes |= (uint32_t)c << (4 * e);
+      for (int e = 7; e >= 0; e--) add(quotient(x[e], s, rs));
+    } else {
+#pragma unroll 1
+      for (int e = 7; e >= 0; e--) add(__fdiv_rn(x[e], s));
     }
+    g.codes = w - 0x3F400000u;      // (the constant's other bits, 0x4B400000 at each of the 8 places, modulo 2^32)
   }
   return g;
 }
 
 template <int HD>
-__global__ void __launch_bounds__(256) kv4_append_k(uint8_t* __restrict__ pages, bf16* __restrict__ q_out, const bf16* __restrict__ qkv,
+__global__ void __launch_bounds__(512, 2) kv4_append_k(uint8_t* __restrict__ pages, bf16* __restrict__ q_out, const bf16* __restrict__ qkv,
                                                     const int* __restrict__ slots, const int* __restrict__ pos, const float* __restrict__ cos,
-                                                    const float* __restrict__ sin, long n_pages, int page, unsigned total, long stride, int H, int Hkv, int T) {
+                                                    const float* __restrict__ sin, long n_pages, int page_log, int N, long stride, int H, int Hkv, int T) {
   mlb_pdl_sync();
   using L = Block<HD>;
-  constexpr unsigned PER = HD / 8;
-  const unsigned heads = H + 2 * Hkv;
-  const unsigned at = blockIdx.x * 256u + threadIdx.x, idx = min(at, total - 1);      // (all lanes stay for the shuffles)
-  const unsigned t = idx % PER, head = idx / PER % heads, row = idx / PER / heads;
-  const bf16* src = qkv + (long)row * stride + (long)head * HD;
-  float x[8];
-  unpack8(*reinterpret_cast<const uint4*>(src + 8 * t), x);
-  if (cos != nullptr && head < (unsigned)(H + Hkv)) {
-    constexpr unsigned HALF = PER / 2;
-    int p = pos[row];
-    if (p < 0 || p >= T) {
-      if (t == 0 && head == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC3);
-      p = 0;
-    }
-    float y[8], c[8], s[8];
-    unpack8(*reinterpret_cast<const uint4*>(src + 8 * (t < HALF ? t + HALF : t - HALF)), y);
-    const long a = (long)p * (HD / 2) + 8 * (t < HALF ? t : t - HALF);
+  constexpr int PER = HD / 8, HALF = PER / 2, NG = L::NG;
+  const int idx = blockIdx.x * blockDim.x + threadIdx.x, head = idx / PER, t = idx % PER, j = t & 3, g = t >> 2;
+  const bool any = head < H + 2 * Hkv, query = head < H, value = head >= H + Hkv, turn = cos != nullptr && head < H + Hkv;
+  const int kv = head - H - (value ? Hkv : 0);
+  const unsigned group = __ballot_sync(0xffffffffu, any && !query);      // lanes that cut their elements to codes
+  if (!any || (query && q_out == nullptr)) return;
+  const int other = 8 * (t < HALF ? t + HALF : t - HALF), angle = 8 * (t < HALF ? t : t - HALF);
+  const uint32_t minus = t < HALF ? 0x80008000u : 0u;      // the first half loses what the second one gains
+  for (int row = blockIdx.y; row < N; row += gridDim.y) {
+    const bf16* src = qkv + row * stride + (long)head * HD;
+    const int slot = slots[row];
+    float x[8];
+    unpack8(*reinterpret_cast<const uint4*>(src + 8 * t), x);
+    if (turn) {
+      int p = pos[row];
+      if (p < 0 || p >= T) {
+        if (t == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC3);
+        p = 0;
+      }
+      float y[8];
+      uint4 far = *reinterpret_cast<const uint4*>(src + other);
+      far.x ^= minus, far.y ^= minus, far.z ^= minus, far.w ^= minus;
+      unpack8(far, y);
+      const float4* cp = reinterpret_cast<const float4*>(cos + (long)p * (HD / 2) + angle);
+      const float4* sp = reinterpret_cast<const float4*>(sin + (long)p * (HD / 2) + angle);
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-      const float4 cv = *reinterpret_cast<const float4*>(cos + a + 4 * k), sv = *reinterpret_cast<const float4*>(sin + a + 4 * k);
-      c[4 * k] = cv.x, c[4 * k + 1] = cv.y, c[4 * k + 2] = cv.z, c[4 * k + 3] = cv.w;
-      s[4 * k] = sv.x, s[4 * k + 1] = sv.y, s[4 * k + 2] = sv.z, s[4 * k + 3] = sv.w;
-    }
+      for (int k = 0; k < 2; k++) {
+        const float4 cv = cp[k], sv = sp[k];
+        const float c[4] = {cv.x, cv.y, cv.z, cv.w}, s[4] = {sv.x, sv.y, sv.z, sv.w};
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float u = __fmul_rn(x[e], c[e]), v = __fmul_rn(y[e], s[e]);
-      x[e] = t < HALF ? __fsub_rn(u, v) : __fadd_rn(u, v);
+        for (int e = 0; e < 4; e++) {
+          x[4 * k + e] = __fadd_rn(__fmul_rn(x[4 * k + e], c[e]), __fmul_rn(y[4 * k + e], s[e]));
+        }
+      }
     }
-  }
-  const Group g = to_codes(x);
-  if (at >= total) return;
-  if (head < (unsigned)H) {
-    if (q_out != nullptr) {
+    if (query) {
       const uint4 w = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
       *reinterpret_cast<uint4*>(q_out + ((long)row * H + head) * HD + 8 * t) = w;
+      continue;
     }
-    return;
+    if (slot < 0) continue;      // (all lanes of a row's group go together)
+    const int pg = slot >> page_log, off = slot & ((1 << page_log) - 1), r = off % TOK;
+    if (pg >= n_pages) {
+      if (t == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC2);
+      continue;
+    }
+    const Group c = to_codes(x, group);
+    uint8_t* b = pages + ((((long)pg * Hkv + kv) << (page_log - 4)) + off / TOK) * L::BYTES;
+    if (!value) {
+      *reinterpret_cast<uint32_t*>(b + r * L::ROW + 4 * (j * NG + g)) = c.codes;
+    } else {
+      uint8_t* v = b + L::V + r * L::ROW;
+      if constexpr (NG % 2 == 0) {      // a whole 32-bit word a thread: groups g and g ^ 1 swap halves
+        const uint32_t got = __shfl_xor_sync(group, g % 2 == 0 ? c.codes >> 16 : c.codes & 0xFFFFu, 4);
+        const uint32_t w = g % 2 == 0 ? (c.codes & 0xFFFFu) | got << 16 : got | (c.codes & 0xFFFF0000u);
+        *reinterpret_cast<uint32_t*>(v + 2 * ((2 * j + g % 2) * NG + g / 2 * 2)) = w;
+      } else {
+        *reinterpret_cast<uint16_t*>(v + 2 * (2 * j * NG + g)) = (uint16_t)c.codes;
+        *reinterpret_cast<uint16_t*>(v + 2 * ((2 * j + 1) * NG + g)) = (uint16_t)(c.codes >> 16);
+      }
+    }
+    if (j == 0) *reinterpret_cast<uint16_t*>(b + (value ? L::VS : L::KS) + 2 * (r * NG + g)) = c.scale;
   }
-  const int slot = slots[row];
-  if (slot < 0) return;
-  if (slot / page >= n_pages) {
-    if (t == 0 && head == (unsigned)H) mlb_set_error(MLB_ERR_BOUNDS, 0xC2);
-    return;
-  }
-  const bool value = head >= (unsigned)(H + Hkv);
-  const int kv = (int)head - H - (value ? Hkv : 0), off = slot % page, r = off % TOK;
-  uint8_t* b = pages + (((long)(slot / page) * Hkv + kv) * (page / TOK) + off / TOK) * L::BYTES;
-  const int j = t & 3, gi = t >> 2;
-  if (!value) {
-    *reinterpret_cast<uint32_t*>(b + r * L::ROW + 4 * (j * L::NG + gi)) = g.codes;
-  } else {
-    uint16_t* v = reinterpret_cast<uint16_t*>(b + L::V + r * L::ROW);
-    v[2 * j * L::NG + gi] = (uint16_t)g.codes;
-    v[(2 * j + 1) * L::NG + gi] = (uint16_t)(g.codes >> 16);
-  }
-  if (j == 0) *reinterpret_cast<uint16_t*>(b + (value ? L::VS : L::KS) + 2 * (r * L::NG + gi)) = g.scale;
 }
 
 // ------------------------------------------------------------------ read
@@ -149,12 +172,19 @@ __global__ void __launch_bounds__(256) kv4_read_k(bf16* __restrict__ k, bf16* __
     const uint16_t* h = reinterpret_cast<const uint16_t*>(b + L::V + r * L::ROW);
     const uint32_t ck = *reinterpret_cast<const uint32_t*>(b + r * L::ROW + 4 * (j * L::NG + gi));
     const uint32_t cv = h[2 * j * L::NG + gi] | (uint32_t)h[(2 * j + 1) * L::NG + gi] << 16;
-    const float sk = bf16_bits(*reinterpret_cast<const uint16_t*>(b + L::KS + 2 * (r * L::NG + gi)));
-    const float sv = bf16_bits(*reinterpret_cast<const uint16_t*>(b + L::VS + 2 * (r * L::NG + gi)));
-    auto val = [](uint32_t c, int e, float s) { return __fmul_rn((float)((int)(c >> (4 * e) & 15) - 8), s); };
-    auto word = [&](uint32_t c, float s, int e) { return pack_bf16(val(c, e, s), val(c, e + 1, s)); };
-    wk = {word(ck, sk, 0), word(ck, sk, 2), word(ck, sk, 4), word(ck, sk, 6)};
-    wv = {word(cv, sv, 0), word(cv, sv, 2), word(cv, sv, 4), word(cv, sv, 6)};
+    const uint32_t sk = *reinterpret_cast<const uint16_t*>(b + L::KS + 2 * (r * L::NG + gi)) * 0x10001u;
+    const uint32_t sv = *reinterpret_cast<const uint16_t*>(b + L::VS + 2 * (r * L::NG + gi)) * 0x10001u;
+    // (c - 8) s rounded once: both factors are bf16 numbers
+    auto values = [](uint32_t c, uint32_t s) {
+      const uint32_t a = value_codes(c), b = value_codes(c >> 4), d = value_codes(c >> 8), e = value_codes(c >> 12);      // elements 0 4, 1 5, 2 6, 3 7
+      auto times = [&](uint32_t x) {
+        const bf162 y = __hmul2(*reinterpret_cast<const bf162*>(&x), *reinterpret_cast<const bf162*>(&s));
+        return *reinterpret_cast<const uint32_t*>(&y);
+      };
+      return make_uint4(times(__byte_perm(a, b, 0x5410)), times(__byte_perm(d, e, 0x5410)), times(__byte_perm(a, b, 0x7632)), times(__byte_perm(d, e, 0x7632)));
+    };
+    wk = values(ck, sk);
+    wv = values(cv, sv);
   }
   *reinterpret_cast<uint4*>(k + 8L * idx) = wk;
   *reinterpret_cast<uint4*>(v + 8L * idx) = wv;
@@ -218,13 +248,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000F000Fu; }       // two codes as fp16 c 2^-24
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00F000F0u; }      // c 2^-20
-__device__ __forceinline__ uint32_t value_codes(uint32_t w) {      // two codes as bf16 c - 8
-  const uint32_t x = low_codes(w) | 0x43004300u, k = 0x43084308u;      // 128 + c, 136
-  const bf162 y = __hsub2(*reinterpret_cast<const bf162*>(&x), *reinterpret_cast<const bf162*>(&k));
-  return *reinterpret_cast<const uint32_t*>(&y);
 }
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -746,17 +769,17 @@ int attn_grid(long B, int Hkv, int width, int page, int nt) {
 MLB_API int mlb_kv4_append(uint8_t* pages, void* q_out, const void* qkv, const int* slots, const int* pos, const float* cos, const float* sin, long n_pages,
                            int page, long N, long stride, int H, int Hkv, int hd, int T, cudaStream_t st) {
   if (!known_head(hd) || page_shift(page) < 0 || stride % 8 != 0 || H < 0 || Hkv < 1) return -7;
-  const long per_row = (long)(H + 2 * Hkv) * (hd / 8), rows = (1L << 30) / per_row;
-  if (rows < 1) return -7;
+  if (N < 1) return 0;
+  // a row is a block or several of up to 512 threads; as many rows at a time as fill the machine, each block 4 of them and more where there are enough
+  const long per_row = (long)(H + 2 * Hkv) * (hd / 8), blocks = (per_row + 511) / 512, threads = ((per_row + blocks - 1) / blocks + 31) / 32 * 32;
+  const long room = 2048L / threads * mlb_sm_count() / blocks + 1, want = N < room ? N : (N + 3) / 4 > room ? (N + 3) / 4 : room;
+  if (per_row >= 1L << 30 || N >= 1L << 31) return -7;
   cudaError_t e = cudaSuccess;
-  for (long r = 0; r < N && e == cudaSuccess; r += rows) {
-    const unsigned total = (unsigned)((N - r < rows ? N - r : rows) * per_row);
 #define MLB_GO(HD)                                                                                                                            \
-  e = mlb_launch(kv4_append_k<HD>, dim3((total + 255) / 256), dim3(256), 0, st, pages, q_out ? (bf16*)q_out + r * H * HD : nullptr,          \
-                 (const bf16*)qkv + r * stride, slots + r, cos ? pos + r : nullptr, cos, sin, n_pages, page, total, stride, H, Hkv, T)
-    MLB_BY_HEAD(hd, MLB_GO)
+  e = mlb_launch(kv4_append_k<HD>, dim3((unsigned)blocks, (unsigned)(want < 65535 ? want : 65535)), dim3((unsigned)threads), 0, st, pages, (bf16*)q_out,  \
+                 (const bf16*)qkv, slots, pos, cos, sin, n_pages, page_shift(page), (int)N, stride, H, Hkv, T)
+  MLB_BY_HEAD(hd, MLB_GO)
 #undef MLB_GO
-  }
   return (int)e;
 }
 
