@@ -43,12 +43,30 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
 #pragma unroll
   for (int k = 0; k < 4; k++) x[2 * k] = lo_bf16(u[k]), x[2 * k + 1] = hi_bf16(u[k]);
 }
+// Two numbers an instruction, each rounded as by itself
+struct Pair { unsigned long long v; };
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void split(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair p;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair p;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return p;
+}
 struct Group { uint32_t codes; uint16_t scale; };
 // x / s as rounded to nearest: the rounded reciprocal's product corrected by its remainder is that (Markstein, Computation of elementary functions on the IBM RISC
 // System/6000 processor, 1990), as long as nothing on the way is subnormal
-__device__ __forceinline__ float quotient(float x, float s, float rs) {
-  const float q = x * rs;
-  return fmaf(fmaf(-q, s, x), rs, q);
+__device__ __forceinline__ Pair quotients(Pair x, Pair minus_s, Pair rs) {
+  const Pair q = mul2(x, rs);
+  return fma2(fma2(q, minus_s, x), rs, q);
 }
 __device__ __forceinline__ Group to_codes(const float (&x)[8], unsigned mask) {
   // a number's bits turned left by one have its magnitude above its sign: the largest are of the largest magnitude, of a tie the negative one's
@@ -70,8 +88,13 @@ __device__ __forceinline__ Group to_codes(const float (&x)[8], unsigned mask) {
     auto add = [&](float q) { w = w * 16u + __float_as_uint(fminf(q, 7.f) + 12582920.f); };
     if (fabsf(s) >= 8.67361738e-19f) {      // 2^-60
       const float rs = __frcp_rn(s);
+      const Pair rr = pair(rs, rs), ms = pair(-s, -s);
 #pragma unroll
-      for (int e = 7; e >= 0; e--) add(quotient(x[e], s, rs));
+      for (int e = 6; e >= 0; e -= 2) {
+        float a, b;
+        split(quotients(pair(x[e], x[e + 1]), ms, rr), a, b);
+        add(b), add(a);
+      }
     } else {
 #pragma unroll 1
       for (int e = 7; e >= 0; e--) add(__fdiv_rn(x[e], s));
@@ -95,40 +118,50 @@ __global__ void __launch_bounds__(512, 2) kv4_append_k(uint8_t* __restrict__ pag
   if (!any || (query && q_out == nullptr)) return;
   const int other = 8 * (t < HALF ? t + HALF : t - HALF), angle = 8 * (t < HALF ? t : t - HALF);
   const uint32_t minus = t < HALF ? 0x80008000u : 0u;      // the first half loses what the second one gains
-  for (int row = blockIdx.y; row < N; row += gridDim.y) {
-    const bf16* src = qkv + row * stride + (long)head * HD;
-    const int slot = slots[row];
+  const bf16* src = qkv + (long)head * HD;
+  // the next row is on its way while one is worked on
+  int row = blockIdx.y, slot = 0, p = 0;
+  uint4 near = {0, 0, 0, 0}, far = near;
+  auto fetch = [&] {
+    if (row >= N) return;
+    const bf16* r = src + row * stride;
+    near = *reinterpret_cast<const uint4*>(r + 8 * t);
+    if (turn) far = *reinterpret_cast<const uint4*>(r + other), p = pos[row];
+    if (!query) slot = slots[row];
+  };
+  fetch();
+#pragma unroll 1
+  for (int now = row; now < N; now = row) {
     float x[8];
-    unpack8(*reinterpret_cast<const uint4*>(src + 8 * t), x);
+    unpack8(near, x);
+    const int here = slot;
     if (turn) {
-      int p = pos[row];
       if (p < 0 || p >= T) {
         if (t == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC3);
         p = 0;
       }
       float y[8];
-      uint4 far = *reinterpret_cast<const uint4*>(src + other);
       far.x ^= minus, far.y ^= minus, far.z ^= minus, far.w ^= minus;
       unpack8(far, y);
       const float4* cp = reinterpret_cast<const float4*>(cos + (long)p * (HD / 2) + angle);
       const float4* sp = reinterpret_cast<const float4*>(sin + (long)p * (HD / 2) + angle);
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        const float4 cv = cp[k], sv = sp[k];
-        const float c[4] = {cv.x, cv.y, cv.z, cv.w}, s[4] = {sv.x, sv.y, sv.z, sv.w};
+        const float4 c = cp[k], s = sp[k];
+        const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          x[4 * k + e] = __fadd_rn(__fmul_rn(x[4 * k + e], c[e]), __fmul_rn(y[4 * k + e], s[e]));
-        }
+        for (int e = 0; e < 4; e++) x[4 * k + e] = __fadd_rn(__fmul_rn(x[4 * k + e], cc[e]), __fmul_rn(y[4 * k + e], ss[e]));
       }
     }
+    row += gridDim.y;
+    fetch();
     if (query) {
       const uint4 w = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
-      *reinterpret_cast<uint4*>(q_out + ((long)row * H + head) * HD + 8 * t) = w;
+      *reinterpret_cast<uint4*>(q_out + ((long)now * H + head) * HD + 8 * t) = w;
       continue;
     }
-    if (slot < 0) continue;      // (all lanes of a row's group go together)
-    const int pg = slot >> page_log, off = slot & ((1 << page_log) - 1), r = off % TOK;
+    if (here < 0) continue;      // (all lanes of a row's group go together)
+    const int pg = here >> page_log, off = here & ((1 << page_log) - 1), r = off % TOK;
     if (pg >= n_pages) {
       if (t == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC2);
       continue;
@@ -154,40 +187,43 @@ __global__ void __launch_bounds__(512, 2) kv4_append_k(uint8_t* __restrict__ pag
 
 // ------------------------------------------------------------------ read
 template <int HD>
-__global__ void __launch_bounds__(256) kv4_read_k(bf16* __restrict__ k, bf16* __restrict__ v, const uint8_t* __restrict__ pages, const int* __restrict__ slots,
-                                                  long n_pages, int page, unsigned total, int Hkv) {
+__global__ void __launch_bounds__(512, 3) kv4_read_k(bf16* __restrict__ k, bf16* __restrict__ v, const uint8_t* __restrict__ pages, const int* __restrict__ slots,
+                                                     long n_pages, int page_log, int N, int Hkv) {
   mlb_pdl_sync();
   using L = Block<HD>;
-  constexpr unsigned PER = HD / 8;
-  const unsigned idx = blockIdx.x * 256u + threadIdx.x;
-  if (idx >= total) return;
-  const unsigned t = idx % PER, kv = idx / PER % Hkv, row = idx / PER / Hkv;
-  const int slot = slots[row];
-  uint4 wk = {0, 0, 0, 0}, wv = wk;
-  if (slot >= 0 && slot / page >= n_pages) {
-    if (t == 0 && kv == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC2);
-  } else if (slot >= 0) {
-    const int off = slot % page, r = off % TOK, j = t & 3, gi = t >> 2;
-    const uint8_t* b = pages + (((long)(slot / page) * Hkv + kv) * (page / TOK) + off / TOK) * L::BYTES;
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(b + L::V + r * L::ROW);
-    const uint32_t ck = *reinterpret_cast<const uint32_t*>(b + r * L::ROW + 4 * (j * L::NG + gi));
-    const uint32_t cv = h[2 * j * L::NG + gi] | (uint32_t)h[(2 * j + 1) * L::NG + gi] << 16;
-    const uint32_t sk = *reinterpret_cast<const uint16_t*>(b + L::KS + 2 * (r * L::NG + gi)) * 0x10001u;
-    const uint32_t sv = *reinterpret_cast<const uint16_t*>(b + L::VS + 2 * (r * L::NG + gi)) * 0x10001u;
-    // (c - 8) s rounded once: both factors are bf16 numbers
-    auto values = [](uint32_t c, uint32_t s) {
-      const uint32_t a = value_codes(c), b = value_codes(c >> 4), d = value_codes(c >> 8), e = value_codes(c >> 12);      // elements 0 4, 1 5, 2 6, 3 7
-      auto times = [&](uint32_t x) {
-        const bf162 y = __hmul2(*reinterpret_cast<const bf162*>(&x), *reinterpret_cast<const bf162*>(&s));
-        return *reinterpret_cast<const uint32_t*>(&y);
+  constexpr int PER = HD / 8;
+  const int idx = blockIdx.x * blockDim.x + threadIdx.x, t = idx % PER, kv = idx / PER, j = t & 3, gi = t >> 2;
+  if (kv >= Hkv) return;
+#pragma unroll 1
+  for (int row = blockIdx.y; row < N; row += gridDim.y) {
+    const int slot = slots[row], pg = slot >> page_log;
+    uint4 wk = {0, 0, 0, 0}, wv = wk;
+    if (slot >= 0 && pg >= n_pages) {
+      if (t == 0 && kv == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xC2);
+    } else if (slot >= 0) {
+      const int off = slot & ((1 << page_log) - 1), r = off % TOK;
+      const uint8_t* b = pages + ((((long)pg * Hkv + kv) << (page_log - 4)) + off / TOK) * L::BYTES;
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(b + L::V + r * L::ROW);
+      const uint32_t ck = *reinterpret_cast<const uint32_t*>(b + r * L::ROW + 4 * (j * L::NG + gi));
+      const uint32_t cv = h[2 * j * L::NG + gi] | (uint32_t)h[(2 * j + 1) * L::NG + gi] << 16;
+      const uint32_t sk = *reinterpret_cast<const uint16_t*>(b + L::KS + 2 * (r * L::NG + gi)) * 0x10001u;
+      const uint32_t sv = *reinterpret_cast<const uint16_t*>(b + L::VS + 2 * (r * L::NG + gi)) * 0x10001u;
+      // (c - 8) s rounded once: both factors are bf16 numbers
+      auto values = [](uint32_t c, uint32_t s) {
+        const uint32_t a = value_codes(c), b = value_codes(c >> 4), d = value_codes(c >> 8), e = value_codes(c >> 12);      // elements 0 4, 1 5, 2 6, 3 7
+        auto times = [&](uint32_t x) {
+          const bf162 y = __hmul2(*reinterpret_cast<const bf162*>(&x), *reinterpret_cast<const bf162*>(&s));
+          return *reinterpret_cast<const uint32_t*>(&y);
+        };
+        return make_uint4(times(__byte_perm(a, b, 0x5410)), times(__byte_perm(d, e, 0x5410)), times(__byte_perm(a, b, 0x7632)), times(__byte_perm(d, e, 0x7632)));
       };
-      return make_uint4(times(__byte_perm(a, b, 0x5410)), times(__byte_perm(d, e, 0x5410)), times(__byte_perm(a, b, 0x7632)), times(__byte_perm(d, e, 0x7632)));
-    };
-    wk = values(ck, sk);
-    wv = values(cv, sv);
+      wk = values(ck, sk);
+      wv = values(cv, sv);
+    }
+    const long to = ((long)row * Hkv + kv) * HD + 8 * t;
+    *reinterpret_cast<uint4*>(k + to) = wk;
+    *reinterpret_cast<uint4*>(v + to) = wv;
   }
-  *reinterpret_cast<uint4*>(k + 8L * idx) = wk;
-  *reinterpret_cast<uint4*>(v + 8L * idx) = wv;
 }
 
 // ------------------------------------------------------------------ attention
@@ -754,6 +790,14 @@ int attn_grid(long B, int Hkv, int width, int page, int nt) {
   const long all = per_sm(nt) * (long)mlb_sm_count(), want = (most + WARPS - 1) / WARPS;
   return (int)(want < all ? (want > 0 ? want : 1) : all);
 }
+// Threads of a row (`per_row`) in blocks of up to 512, and as many rows at a time as fill the machine; where there are many, a block goes over 4 of them and more
+struct Shape { dim3 grid; unsigned threads; };
+Shape rows_shape(long per_row, long N) {
+  if (per_row < 1 || per_row >= 1L << 30 || N < 1 || N >= 1L << 31) return {dim3(), 0};
+  const long blocks = (per_row + 511) / 512, threads = ((per_row + blocks - 1) / blocks + 31) / 32 * 32;
+  const long room = 2048L / threads * mlb_sm_count() / blocks + 1, many = (N + 3) / 4 > room ? (N + 3) / 4 : room, rows = N < many ? N : many;
+  return {dim3((unsigned)blocks, (unsigned)(rows < 65535 ? rows : 65535)), (unsigned)threads};
+}
 #define MLB_BY_HEAD(hd, F) \
   switch (hd) {            \
     case 32: F(32); break; \
@@ -769,15 +813,12 @@ int attn_grid(long B, int Hkv, int width, int page, int nt) {
 MLB_API int mlb_kv4_append(uint8_t* pages, void* q_out, const void* qkv, const int* slots, const int* pos, const float* cos, const float* sin, long n_pages,
                            int page, long N, long stride, int H, int Hkv, int hd, int T, cudaStream_t st) {
   if (!known_head(hd) || page_shift(page) < 0 || stride % 8 != 0 || H < 0 || Hkv < 1) return -7;
-  if (N < 1) return 0;
-  // a row is a block or several of up to 512 threads; as many rows at a time as fill the machine, each block 4 of them and more where there are enough
-  const long per_row = (long)(H + 2 * Hkv) * (hd / 8), blocks = (per_row + 511) / 512, threads = ((per_row + blocks - 1) / blocks + 31) / 32 * 32;
-  const long room = 2048L / threads * mlb_sm_count() / blocks + 1, want = N < room ? N : (N + 3) / 4 > room ? (N + 3) / 4 : room;
-  if (per_row >= 1L << 30 || N >= 1L << 31) return -7;
+  const Shape z = rows_shape((long)(H + 2 * Hkv) * (hd / 8), N);
+  if (z.threads == 0) return -7;
   cudaError_t e = cudaSuccess;
 #define MLB_GO(HD)                                                                                                                            \
-  e = mlb_launch(kv4_append_k<HD>, dim3((unsigned)blocks, (unsigned)(want < 65535 ? want : 65535)), dim3((unsigned)threads), 0, st, pages, (bf16*)q_out,  \
-                 (const bf16*)qkv, slots, pos, cos, sin, n_pages, page_shift(page), (int)N, stride, H, Hkv, T)
+  e = mlb_launch(kv4_append_k<HD>, z.grid, dim3(z.threads), 0, st, pages, (bf16*)q_out, (const bf16*)qkv, slots, pos, cos, sin, n_pages, page_shift(page), (int)N, stride, H, \
+                 Hkv, T)
   MLB_BY_HEAD(hd, MLB_GO)
 #undef MLB_GO
   return (int)e;
@@ -786,17 +827,12 @@ MLB_API int mlb_kv4_append(uint8_t* pages, void* q_out, const void* qkv, const i
 // k, v[N, Hkv, hd]: what the slots hold; zeros for a negative slot
 MLB_API int mlb_kv4_read(void* k, void* v, const uint8_t* pages, const int* slots, long n_pages, int page, long N, int Hkv, int hd, cudaStream_t st) {
   if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1) return -7;
-  const long per_row = (long)Hkv * (hd / 8), rows = (1L << 30) / per_row;
-  if (rows < 1) return -7;
+  const Shape z = rows_shape((long)Hkv * (hd / 8), N);
+  if (z.threads == 0) return -7;
   cudaError_t e = cudaSuccess;
-  for (long r = 0; r < N && e == cudaSuccess; r += rows) {
-    const unsigned total = (unsigned)((N - r < rows ? N - r : rows) * per_row);
-#define MLB_GO(HD)                                                                                                                            \
-  e = mlb_launch(kv4_read_k<HD>, dim3((total + 255) / 256), dim3(256), 0, st, (bf16*)k + r * Hkv * HD, (bf16*)v + r * Hkv * HD, pages, slots + r, \
-                 n_pages, page, total, Hkv)
-    MLB_BY_HEAD(hd, MLB_GO)
+#define MLB_GO(HD) e = mlb_launch(kv4_read_k<HD>, z.grid, dim3(z.threads), 0, st, (bf16*)k, (bf16*)v, pages, slots, n_pages, page_shift(page), (int)N, Hkv)
+  MLB_BY_HEAD(hd, MLB_GO)
 #undef MLB_GO
-  }
   return (int)e;
 }
 
