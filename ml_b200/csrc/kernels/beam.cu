@@ -498,13 +498,14 @@ struct OrderArgs {
   int *table_out, *spare_out, *hist_out;
   const int *table, *spare, *lens, *hist, *parents, *tokens;
   long n_pages;
-  int K, Hkv, page, block_vecs, width, T;      // block_vecs: 16-byte words of a block of 16 tokens
+  int K, Hkv, page, block_vecs, width, T, parts;      // block_vecs: 16-byte words of a block of 16 tokens; parts: thread blocks that copy a layer's page
 };
 constexpr int ORDER_THREADS = 256;
 __global__ void __launch_bounds__(ORDER_THREADS) beam_reorder_k(const OrderArgs A) {
   mlb_pdl_sync();
   const int row = blockIdx.x, tid = threadIdx.x;
   int parent = A.parents[row];
+  const int spare = A.spare[row];
   if (parent < 0 || parent >= A.K) {
     if (tid == 0 && blockIdx.y == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xB3);
     parent = row % A.K;
@@ -514,25 +515,36 @@ __global__ void __launch_bounds__(ORDER_THREADS) beam_reorder_k(const OrderArgs 
   const bool moved = rest > 0 && src != row;
   if (blockIdx.y == 0) {
     for (int p = tid; p < A.width; p += ORDER_THREADS)
-      A.table_out[(long)row * A.width + p] = moved && p == full ? A.spare[row] : A.table[(long)(p < full ? src : row) * A.width + p];
-    if (tid == 0) A.spare_out[row] = moved ? A.table[(long)row * A.width + full] : A.spare[row];
+      A.table_out[(long)row * A.width + p] = moved && p == full ? spare : A.table[(long)(p < full ? src : row) * A.width + p];
+    if (tid == 0) A.spare_out[row] = moved ? A.table[(long)row * A.width + full] : spare;
     for (int t = tid; t < min(len, A.T); t += ORDER_THREADS) A.hist_out[(long)row * A.T + t] = A.hist[(long)src * A.T + t];
     if (tid == 0 && len < A.T) A.hist_out[(long)row * A.T + len] = A.tokens[row];
     return;
   }
   if (!moved) return;
-  const int from = A.table[(long)src * A.width + full], to = A.spare[row];
+  const int from = A.table[(long)src * A.width + full], to = spare;
   if (from < 0 || from >= A.n_pages || to < 0 || to >= A.n_pages) {
     if (tid == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xB4);
     return;
   }
-  const int blocks = A.page / 16, each = (rest + 15) / 16 * A.block_vecs;
-  const long base = (long)(blockIdx.y - 1) * A.n_pages, head = (long)blocks * A.block_vecs;
-  const uint4* f = reinterpret_cast<const uint4*>(A.pages) + (base + from) * A.Hkv * head;
-  uint4* t = reinterpret_cast<uint4*>(A.pages) + (base + to) * A.Hkv * head;
-  for (int v = tid; v < A.Hkv * each; v += ORDER_THREADS) {
-    const long a = v / each * head + v % each;
-    t[a] = f[a];
+  // `parts` blocks a layer: this one's words of the Hkv heads' tokens, 4 on their way at a time
+  const int layer = (blockIdx.y - 1) / A.parts, part = (blockIdx.y - 1) % A.parts;
+  const unsigned blocks = A.page / 16, each = (rest + 15) / 16 * A.block_vecs, head = blocks * A.block_vecs, total = A.Hkv * each;
+  const unsigned v0 = (unsigned)((unsigned long long)total * part / A.parts), v1 = (unsigned)((unsigned long long)total * (part + 1) / A.parts);
+  const uint4* f = reinterpret_cast<const uint4*>(A.pages) + ((long)layer * A.n_pages + from) * A.Hkv * head;
+  uint4* t = reinterpret_cast<uint4*>(A.pages) + ((long)layer * A.n_pages + to) * A.Hkv * head;
+  for (unsigned v = v0 + tid; v < v1; v += 4 * ORDER_THREADS) {
+    uint4 w[4];
+    unsigned at[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const unsigned x = v + k * ORDER_THREADS;
+      at[k] = x / each * head + x % each;      // (a page of all heads is below 2^32 bytes)
+      if (x < v1) w[k] = f[at[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (v + k * ORDER_THREADS < v1) t[at[k]] = w[k];
   }
 }
 
@@ -568,6 +580,10 @@ MLB_API int mlb_beam_reorder(uint8_t* pages, int* table_out, int* spare_out, int
                              const int* parents, const int* tokens, int layers, long n_pages, int Hkv, int page, int block_bytes, int B, int K, int width, int T,
                              cudaStream_t st) {
   if (page < 16 || page % 16 != 0 || block_bytes % 16 != 0 || K < 1 || width < 1 || layers > 65534) return -7;
-  const OrderArgs a{pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, n_pages, K, Hkv, page, block_bytes / 16, width, T};
-  return (int)mlb_launch(beam_reorder_k, dim3(B * K, pages ? layers + 1 : 1), dim3(ORDER_THREADS), 0, st, a);
+  // a part is 1024 words (16 KB) of a page or more
+  const long words = (long)Hkv * (page / 16) * (block_bytes / 16), most = layers > 0 ? 65534 / layers : 1;
+  if (words >= 1L << 28) return -7;
+  const int parts = (int)(words / 1024 < 1 ? 1 : words / 1024 < most ? words / 1024 : most);
+  const OrderArgs a{pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, n_pages, K, Hkv, page, block_bytes / 16, width, T, parts};
+  return (int)mlb_launch(beam_reorder_k, dim3(B * K, pages ? layers * parts + 1 : 1), dim3(ORDER_THREADS), 0, st, a);
 }
