@@ -263,10 +263,10 @@ struct AttnArgs {
 };
 constexpr int WARPS = 4;
 constexpr int MAX_B = 2048;       // sequences of a launch: their first blocks' numbers stand in shared memory
-// A warp's ring: N places of STEP blocks (hd = 128: 4 thread blocks' rings fill an SM's shared memory)
-constexpr int STEP = 2, PAD = 12;
-constexpr int per_sm(int nt) { return nt == 1 ? 3 : 3; }      // thread blocks that an SM holds
-template <int HD> struct Ring { static constexpr int N = HD == 128 ? 3 : HD == 96 ? 4 : HD == 64 ? 6 : 8, BYTES = STEP * Block<HD>::BYTES; };
+// A warp's ring: N places of STEP blocks (hd = 128: 3 thread blocks' rings fill an SM's shared memory), which are worked on two at a time.  PAD: see the kernel
+constexpr int STEP = 4, PAD = 12;
+constexpr int PER_SM = 3;      // thread blocks that an SM holds
+template <int HD> struct Ring { static constexpr int N = HD == 64 ? 4 : HD == 32 ? 6 : 2, BYTES = STEP * Block<HD>::BYTES; };
 
 // D = A B + C: keys' codes and queries in fp16, values' codes and weights in bf16
 __device__ __forceinline__ void mma_keys(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2,
@@ -461,7 +461,7 @@ template <int HD, int NT> constexpr int attn_ring() {      // bytes of the rings
 template <int HD, int NT> int attn_smem(int B) { return attn_ring<HD, NT>() + (int)sizeof(Queries<HD, NT>) + (B + 1) * 4; }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnArgs A) {
+__global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs A) {
   using L = Block<HD>;
   constexpr int NG = L::NG, NST = Ring<HD>::N, R = 8 * NT, PART = merge_floats<HD, NT>();
   extern __shared__ __align__(128) uint8_t smem[];
@@ -648,12 +648,15 @@ __global__ void __launch_bounds__(WARPS * 32, per_sm(NT)) kv4_attn_k(const AttnA
         parity ^= 1u << k;
         const uint32_t oks = there >> k * STEP & ((1u << STEP) - 1);
         const uint8_t* blk = ring + k * Ring<HD>::BYTES;
-        if (oks == (1u << STEP) - 1 && (u + STEP) * TOK <= all) {
-          attend<HD, NT, STEP, false>(acc, q, c, blk, u * TOK, seen, i, j);
-        } else {
 #pragma unroll 1
-          for (int x = 0; x < STEP; x++)
-            if (oks >> x & 1) attend<HD, NT, 1, true>(acc, q, c, blk + x * L::BYTES, (u + x) * TOK, seen, i, j);
+        for (int x = 0; x < STEP; x += 2) {
+          if ((oks >> x & 3) == 3 && (u + x + 2) * TOK <= all) {
+            attend<HD, NT, 2, false>(acc, q, c, blk + x * L::BYTES, (u + x) * TOK, seen, i, j);
+          } else {
+#pragma unroll 1
+            for (int y = x; y < x + 2; y++)
+              if (oks >> y & 1) attend<HD, NT, 1, true>(acc, q, c, blk + y * L::BYTES, (u + y) * TOK, seen, i, j);
+          }
         }
         __syncwarp();
         if (u + NST * STEP < w1) fetch(u + NST * STEP, k);
@@ -785,9 +788,9 @@ int row_tiles(long rows, int& nt) {
   nt = rows <= 8 ? 1 : 2;
   return (int)((rows + 8 * nt - 1) / (8 * nt));
 }
-int attn_grid(long B, int Hkv, int width, int page, int nt) {
+int attn_grid(long B, int Hkv, int width, int page) {
   const long most = B * Hkv * (((long)width * page + TOK - 1) / TOK + PAD);      // (a thread block has a unit for each warp)
-  const long all = per_sm(nt) * (long)mlb_sm_count(), want = (most + WARPS - 1) / WARPS;
+  const long all = PER_SM * (long)mlb_sm_count(), want = (most + WARPS - 1) / WARPS;
   return (int)(want < all ? (want > 0 ? want : 1) : all);
 }
 // Threads of a row (`per_row`) in blocks of up to 512, and as many rows at a time as fill the machine; where there are many, a block goes over 4 of them and more
@@ -841,7 +844,7 @@ MLB_API long mlb_kv4_attn_scratch(int B, int Tq, int H, int Hkv, int hd, int wid
   if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1 || H % Hkv != 0) return -7;
   int nt;
   const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
-  return (long)attn_grid(B < MAX_B ? B : MAX_B, Hkv, width, page, nt) * tiles * 2 * 8 * nt * (hd + 2);
+  return (long)attn_grid(B < MAX_B ? B : MAX_B, Hkv, width, page) * tiles * 2 * 8 * nt * (hd + 2);
 }
 // out[B Tq, H hd] = attention of q (rows `q_stride` elements apart) over table[B, width], lens[B] tokens each; lse[B, H, Tq] or null
 MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pages, const int* table, const int* lens, float* part, int* count, long n_pages,
@@ -857,7 +860,7 @@ MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pa
     const AttnArgs a{(bf16*)out + (long)b * Tq * H * hd, lse ? lse + (long)b * H * Tq : nullptr, (const bf16*)q + (long)b * Tq * q_stride, pages,
                      table + (long)b * width, lens + b, part, count, q_stride, n_pages, n, Tq, H / Hkv, Hkv, width, shift, (scale == 0.f ? 1.f : fabsf(scale)) * 1.44269504088896f,
                      scale == 0.f ? 0u : ~0u, scale < 0.f ? 0x80008000u : 0u, 1.f / (H / Hkv)};
-    const int grid = attn_grid(n, Hkv, width, page, nt);
+    const int grid = attn_grid(n, Hkv, width, page);
 #define MLB_GO(HD) e = nt == 1 ? launch_attn<HD, 1>(a, grid, tiles, st) : launch_attn<HD, 2>(a, grid, tiles, st)
     MLB_BY_HEAD(hd, MLB_GO)
 #undef MLB_GO
