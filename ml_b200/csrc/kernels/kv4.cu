@@ -265,8 +265,8 @@ constexpr int WARPS = 4;
 constexpr int MAX_B = 2048;       // sequences of a launch: their first blocks' numbers stand in shared memory
 // A warp's ring: N places of STEP blocks (hd = 128: 3 thread blocks' rings fill an SM's shared memory), which are worked on two at a time.  PAD: see the kernel
 constexpr int STEP = 4, PAD = 12;
-constexpr int PER_SM = 3;      // thread blocks that an SM holds
-template <int HD> struct Ring { static constexpr int N = HD == 64 ? 4 : HD == 32 ? 6 : 2, BYTES = STEP * Block<HD>::BYTES; };
+constexpr int PER_SM = 3;      // thread blocks that an SM holds (of 2 where the sequences' numbers leave no room for the third's ring)
+template <int HD> struct Ring { static constexpr int N = HD == 64 ? 3 : HD == 32 ? 6 : 2, BYTES = STEP * Block<HD>::BYTES; };
 
 // D = A B + C: keys' codes and queries in fp16, values' codes and weights in bf16
 __device__ __forceinline__ void mma_keys(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2,
@@ -788,10 +788,24 @@ int row_tiles(long rows, int& nt) {
   nt = rows <= 8 ? 1 : 2;
   return (int)((rows + 8 * nt - 1) / (8 * nt));
 }
-int attn_grid(long B, int Hkv, int width, int page) {
-  const long most = B * Hkv * (((long)width * page + TOK - 1) / TOK + PAD);      // (a thread block has a unit for each warp)
-  const long all = PER_SM * (long)mlb_sm_count(), want = (most + WARPS - 1) / WARPS;
+// Shared memory of a thread block: for the grid, which has to be resident at once to be worth its division of the work
+int attn_smem_of(int hd, int nt, int B) {
+#define MLB_SMEM(HD) return nt == 1 ? attn_smem<HD, 1>(B) : attn_smem<HD, 2>(B)
+  switch (hd) {
+    case 32: MLB_SMEM(32);
+    case 64: MLB_SMEM(64);
+    case 96: MLB_SMEM(96);
+    default: MLB_SMEM(128);
+  }
+#undef MLB_SMEM
+}
+int attn_most(long B, int Hkv, int width, int page) {      // a thread block has a unit for each warp
+  const long most = B * Hkv * (((long)width * page + TOK - 1) / TOK + PAD), all = (long)PER_SM * mlb_sm_count(), want = (most + WARPS - 1) / WARPS;
   return (int)(want < all ? (want > 0 ? want : 1) : all);
+}
+int attn_grid(long B, int Hkv, int width, int page, int hd, int nt) {
+  const long fit = 228L * 1024 / (attn_smem_of(hd, nt, (int)B) + 1024 + 128) * mlb_sm_count(), want = attn_most(B, Hkv, width, page);      // (1 KB of a block's is the system's)
+  return (int)(want < fit ? want : fit);
 }
 // Threads of a row (`per_row`) in blocks of up to 512, and as many rows at a time as fill the machine; where there are many, a block goes over 4 of them and more
 struct Shape { dim3 grid; unsigned threads; };
@@ -844,7 +858,7 @@ MLB_API long mlb_kv4_attn_scratch(int B, int Tq, int H, int Hkv, int hd, int wid
   if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1 || H % Hkv != 0) return -7;
   int nt;
   const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
-  return (long)attn_grid(B < MAX_B ? B : MAX_B, Hkv, width, page) * tiles * 2 * 8 * nt * (hd + 2);
+  return (long)attn_most(B < MAX_B ? B : MAX_B, Hkv, width, page) * tiles * 2 * 8 * nt * (hd + 2);
 }
 // out[B Tq, H hd] = attention of q (rows `q_stride` elements apart) over table[B, width], lens[B] tokens each; lse[B, H, Tq] or null
 MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pages, const int* table, const int* lens, float* part, int* count, long n_pages,
@@ -860,7 +874,7 @@ MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pa
     const AttnArgs a{(bf16*)out + (long)b * Tq * H * hd, lse ? lse + (long)b * H * Tq : nullptr, (const bf16*)q + (long)b * Tq * q_stride, pages,
                      table + (long)b * width, lens + b, part, count, q_stride, n_pages, n, Tq, H / Hkv, Hkv, width, shift, (scale == 0.f ? 1.f : fabsf(scale)) * 1.44269504088896f,
                      scale == 0.f ? 0u : ~0u, scale < 0.f ? 0x80008000u : 0u, 1.f / (H / Hkv)};
-    const int grid = attn_grid(n, Hkv, width, page);
+    const int grid = attn_grid(n, Hkv, width, page, hd, nt);
 #define MLB_GO(HD) e = nt == 1 ? launch_attn<HD, 1>(a, grid, tiles, st) : launch_attn<HD, 2>(a, grid, tiles, st)
     MLB_BY_HEAD(hd, MLB_GO)
 #undef MLB_GO
