@@ -269,9 +269,12 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
     tc::mbar_init(&bar, 1);
     tc::mbar_fence_init();
   }
-  __syncthreads();
   mlb_pdl_sync();
-  if (!A.done[row]) {
+  __shared__ float prev[SEL_MAX_K], lse[SEL_MAX_K];      // the request's beams, which the merge will want
+  __shared__ int ended[SEL_MAX_K];
+  if (tid < K) prev[tid] = A.prev[req * K + tid], ended[tid] = A.done[req * K + tid] != 0;
+  __syncthreads();
+  if (!ended[row - req * K]) {
     constexpr int CHUNK = SEL_CHUNK_BYTES / sizeof(T);
     T* data = reinterpret_cast<T*>(fetched);
     const int begin = blockIdx.x * A.piece, n = min(A.piece, V - begin);
@@ -388,8 +391,6 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
   }
   __syncthreads();
   if (!last) return;
-  __shared__ float prev[SEL_MAX_K], lse[SEL_MAX_K];
-  __shared__ int ended[SEL_MAX_K];
   const int lists = K * A.pieces, L = A.L;
   if (tid == 0) A.ticket[req] = 0, n_cand = 0;
   // the lists' entries, their first ones before their second ones
@@ -407,9 +408,7 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
       tok[h] = __ldcg(A.ids + a), val[h] = __ldcg(A.values + a);
     }
   }
-  if (tid < K) prev[tid] = A.prev[req * K + tid], ended[tid] = A.done[req * K + tid] != 0;
-  for (int k = warp; k < K; k += SEL_WARPS) {
-    if (A.done[req * K + k]) continue;
+  for (int k = warp; k < K; k += SEL_WARPS) {      // (an ended beam's are nothing, and not asked for)
     const float2* st = A.stats + (long)(req * K + k) * A.pieces;
     float2 v[2];      // (pieces past 64 are read again)
     float m = -INFINITY;
