@@ -393,21 +393,6 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
   if (!last) return;
   const int lists = K * A.pieces, L = A.L;
   if (tid == 0) A.ticket[req] = 0, n_cand = 0;
-  // the lists' entries, their first ones before their second ones
-  constexpr int HELD = SEL_HELD / SEL_THREADS;
-  const float per_list = 1.f / lists, per_beam = 1.f / A.pieces;      // ((x + 1/2) / n rounded down is exact for the few thousands that these are)
-  float val[HELD];
-  int tok[HELD];
-#pragma unroll
-  for (int h = 0; h < HELD; h++) {
-    const int e = tid + h * SEL_THREADS;
-    tok[h] = -1, val[h] = 0.f;
-    if (e < lists * L) {
-      const int nth = (int)((e + 0.5f) * per_list);
-      const long a = ((long)req * lists + e - nth * lists) * L + nth;
-      tok[h] = __ldcg(A.ids + a), val[h] = __ldcg(A.values + a);
-    }
-  }
   for (int k = warp; k < K; k += SEL_WARPS) {      // (an ended beam's are nothing, and not asked for)
     const float2* st = A.stats + (long)(req * K + k) * A.pieces;
     float2 v[2];      // (pieces past 64 are read again)
@@ -423,35 +408,38 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
     if (lane == 0) lse[k] = s > 0.f ? m + log_of(s) : -INFINITY;
   }
   __syncthreads();
-  u64 key[HELD], best = 0;
-#pragma unroll
-  for (int h = 0; h < HELD; h++) {
-    const int e = tid + h * SEL_THREADS;
-    key[h] = 0;
-    if (e < lists * L) {
-      const int nth = (int)((e + 0.5f) * per_list), l = e - nth * lists, k = (int)((l + 0.5f) * per_beam);
-      int t = tok[h];
-      float x = val[h];
-      // a beam that has ended, and one of no continuation: it was nothing, or its logits have no logarithm of a sum
-      const bool end = ended[k] != 0, dead = !end && !(prev[k] > -INFINITY && fabsf(lse[k]) < INFINITY);
-      if (end || dead) {
-        x = -INFINITY, t = nth;
-        if (end && A.eos >= 0 && A.eos < V) {
-          t = nth == 0 ? A.eos : nth - 1 < A.eos ? nth - 1 : nth;
-          if (nth == 0) x = prev[k];
-        }
-        if (l != k * A.pieces || t >= V) t = -1;
-      } else {
-        x = __fadd_rn(prev[k], __fsub_rn(x, lse[k]));
+  // the lists' entries, their first ones before their second ones: loops kept short, since each runs once or twice
+  u64* keys = reinterpret_cast<u64*>(fetched);
+  u64 best = 0;
+  const float per_list = 1.f / lists, per_beam = 1.f / A.pieces;      // ((x + 1/2) / n rounded down is exact for the few thousands that these are)
+#pragma unroll 1
+  for (int e = tid; e < lists * L; e += SEL_THREADS) {
+    const int nth = (int)((e + 0.5f) * per_list), l = e - nth * lists, k = (int)((l + 0.5f) * per_beam);
+    const long a = ((long)req * lists + l) * L + nth;
+    int t = __ldcg(A.ids + a);
+    float x = __ldcg(A.values + a);
+    // a beam that has ended, and one of no continuation: it was nothing, or its logits have no logarithm of a sum
+    const bool end = ended[k] != 0, dead = !end && !(prev[k] > -INFINITY && fabsf(lse[k]) < INFINITY);
+    if (end || dead) {
+      x = -INFINITY, t = nth;
+      if (end && A.eos >= 0 && A.eos < V) {
+        t = nth == 0 ? A.eos : nth - 1 < A.eos ? nth - 1 : nth;
+        if (nth == 0) x = prev[k];
       }
-      if (t >= 0) key[h] = rank_of(x != x ? -INFINITY : x, (uint32_t)k * (uint32_t)V + (uint32_t)t);
+      if (l != k * A.pieces || t >= V) t = -1;
+    } else {
+      x = __fadd_rn(prev[k], __fsub_rn(x, lse[k]));
     }
-    best = max(best, key[h]);
+    const u64 key = t < 0 ? 0ull : rank_of(x != x ? -INFINITY : x, (uint32_t)k * (uint32_t)V + (uint32_t)t);
+    keys[e] = key;
+    best = max(best, key);
   }
   const u64 bound = kth_of_parts(best, K, red, [](u64 a, u64 b) { return a > b ? a : b; });
-#pragma unroll
-  for (int h = 0; h < HELD; h++)
-    if (key[h] != 0 && key[h] >= bound) cand[atomicAdd(&n_cand, 1)] = key[h];
+#pragma unroll 1
+  for (int e = tid; e < lists * L; e += SEL_THREADS) {
+    const u64 key = keys[e];
+    if (key != 0 && key >= bound) cand[atomicAdd(&n_cand, 1)] = key;
+  }
   __syncthreads();
   const int found = n_cand;
   for (int e = tid; e < found; e += SEL_THREADS) {
@@ -485,7 +473,8 @@ int select_piece(int rows, int K, int V, int bits) {
 template <typename T, bool BULK>
 cudaError_t launch_select(const SelectArgs& a, int rows, cudaStream_t st) {
   const int bytes = a.piece * (int)sizeof(T) < SEL_CHUNK_BYTES ? a.piece * (int)sizeof(T) : SEL_CHUNK_BYTES;
-  return mlb_launch(beam_select_k<T, BULK>, dim3(a.pieces, rows), dim3(SEL_THREADS), (bytes + 127) / 128 * 128, st, a);
+  const int least = SEL_HELD * (int)sizeof(u64);      // (the merge's)
+  return mlb_launch(beam_select_k<T, BULK>, dim3(a.pieces, rows), dim3(SEL_THREADS), bytes > least ? (bytes + 127) / 128 * 128 : least, st, a);
 }
 
 // ------------------------------------------------------------------ beams in the order of their parents
