@@ -204,6 +204,14 @@ def test_attention_of_more_sequences_than_a_launch_takes(B):
     close(*attend(lens, 1, 1, 1, 32, 16, seed=1, spoil=False))
 
 
+def test_attention_of_many_sequences_at_head_size_128():
+    """More sequences than leave room for a third thread block's ring on an SM, short and long ones, empty ones among them."""
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 40, (700,), generator=g).tolist()
+    lens[13], lens[500] = 1500, 900
+    close(*attend(lens, 1, 2, 1, 128, 64, seed=2, spoil=False))
+
+
 def test_attention_of_no_sequence_and_without_lse():
     pages = oracle.random_pages(1, 1, 16, 64, 0).to(dev())
     ops.kv4_attn(torch.empty(0, 64, dtype=torch.bfloat16, device=dev()), None, torch.empty(0, 64, dtype=torch.bfloat16, device=dev()), pages, ints([]).view(0, 1), ints([]), 1, 1, 1, 64)
@@ -424,6 +432,21 @@ def test_beam_select_of_equal_logits_masks_and_nan(dtype):
     assert 2 not in p.tolist()[0]
     check_choice(z, torch.full((1, K), -math.inf), done, 5)
     check_choice(z, prev, torch.ones_like(done), 5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,K,V,stride", [(1, 32, 50304, 0), (2, 16, 70001, 7), (1000, 1, 300, 0), (3, 24, 40000, 0)])
+def test_beam_select_of_pieces_that_are_fetched_in_parts(dtype, B, K, V, stride):
+    """Many beams: few pieces, several fetches each, the bound moving from one to the next; and logits all alike in the second half, which leave no room for
+    candidates there."""
+    torch.manual_seed(V)
+    logits = (torch.randn(B * K, V) * 3).to(dtype)
+    prev, done = -10 * torch.rand(B, K), torch.zeros(B, K, dtype=I32)
+    check_choice(logits, prev, done, 7, stride=stride)
+    logits[:, V // 2:] = 20.0
+    check_choice(logits, prev, done, 7, stride=stride)
+    logits[:, -1] = 21.0
+    check_choice(logits, prev, done, 7, stride=stride)
 
 
 def test_beam_select_in_a_graph():
