@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
 // then K rounds over the piece find its K largest.  The request's last thread block finds its K best among the pieces' lists in the same way,
 // the bound being of its threads' best.
 constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_BYTES = 32768, SEL_MAX_K = 32, SEL_CAND = 512, SEL_HELD = 1024;
-constexpr int SEL_PER_SM = 6, SEL_LEAST = 2048;      // thread blocks that an SM holds; the smallest piece
+constexpr int SEL_PER_SM = 6, SEL_LEAST = 4096;      // thread blocks that an SM holds; the smallest piece
 typedef unsigned long long u64;
 __device__ __forceinline__ float ex2(float x) {
   float y;
