@@ -717,39 +717,57 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
         if (tid == 0) A.count[item] = 0;      // for the next call
         // elements to the threads; few elements: the shares too, `ways` threads an element
         const int elems = live * (HD / 4), ways = elems >= WARPS * 32 ? 1 : WARPS * 32 / elems;
-        for (int x = tid; x < elems * ways; x += WARPS * 32) {
-          const int way = x / elems, r = x % elems / (HD / 4), d = x % elems % (HD / 4);
-          float m = -INFINITY, l = 0.f;
-          float4 o = {0, 0, 0, 0};
+        for (int x = tid; x < elems * ways; x += NT * WARPS * 32) {      // (of two tiles of rows two elements a thread, their loads on their way together)
           constexpr int BATCH = 8;      // shares on their way at a time
+          const int way = ways > 1 ? x / elems : 0;
+          int row[NT], word[NT];
+          bool is[NT];
+          float m[NT], l[NT];
+          float4 o[NT];
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            const int y = x - way * elems + n * WARPS * 32;
+            is[n] = n == 0 || (ways == 1 && y < elems);
+            row[n] = y / (HD / 4), word[n] = y % (HD / 4);
+            m[n] = -INFINITY, l[n] = 0.f, o[n] = make_float4(0, 0, 0, 0);
+          }
           for (int c = way; c < n_shares; c += ways * BATCH) {
-            float ms[BATCH], ls[BATCH];
-            float4 os[BATCH];
+            float ms[NT][BATCH], ls[NT][BATCH];
+            float4 os[NT][BATCH];
 #pragma unroll
             for (int k = 0; k < BATCH; k++) {
               const int z = c + k * ways;
-              ms[k] = -INFINITY, ls[k] = 0.f, os[k] = make_float4(0, 0, 0, 0);
-              if (z < n_shares) {
-                const float* p = part + ((c0 + z) * 2 + (z > 0 || item0 == c0 * per ? 0 : 1)) * (long)PART;
-                ms[k] = __ldcg(p + r), ls[k] = __ldcg(p + R + r), os[k] = __ldcg(reinterpret_cast<const float4*>(p + 2 * R + r * HD + 4 * d));
+              const float* p = part + ((c0 + z) * 2 + (z > 0 || item0 == c0 * per ? 0 : 1)) * (long)PART;
+#pragma unroll
+              for (int n = 0; n < NT; n++) {
+                ms[n][k] = -INFINITY, ls[n][k] = 0.f, os[n][k] = make_float4(0, 0, 0, 0);
+                if (z < n_shares && is[n])
+                  ms[n][k] = __ldcg(p + row[n]), ls[n][k] = __ldcg(p + R + row[n]), os[n][k] = __ldcg(reinterpret_cast<const float4*>(p + 2 * R + row[n] * HD + 4 * word[n]));
               }
             }
-            float top = m;
 #pragma unroll
-            for (int k = 0; k < BATCH; k++) top = fmaxf(top, ms[k]);
-            const float g = top == -INFINITY ? 1.f : ex2(m - top);
-            l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, m = top;
+            for (int n = 0; n < NT; n++) {
+              float top = m[n];
 #pragma unroll
-            for (int k = 0; k < BATCH; k++) {
-              const float f = top == -INFINITY ? 0.f : ex2(ms[k] - top);
-              l = fmaf(f, ls[k], l), o.x = fmaf(f, os[k].x, o.x), o.y = fmaf(f, os[k].y, o.y), o.z = fmaf(f, os[k].z, o.z), o.w = fmaf(f, os[k].w, o.w);
+              for (int k = 0; k < BATCH; k++) top = fmaxf(top, ms[n][k]);
+              const float g = top == -INFINITY ? 1.f : ex2(m[n] - top);
+              l[n] *= g, o[n].x *= g, o[n].y *= g, o[n].z *= g, o[n].w *= g, m[n] = top;
+#pragma unroll
+              for (int k = 0; k < BATCH; k++) {
+                const float f = top == -INFINITY ? 0.f : ex2(ms[n][k] - top);
+                const float4 v = os[n][k];
+                l[n] = fmaf(f, ls[n][k], l[n]);
+                o[n].x = fmaf(f, v.x, o[n].x), o[n].y = fmaf(f, v.y, o[n].y), o[n].z = fmaf(f, v.z, o[n].z), o[n].w = fmaf(f, v.w, o[n].w);
+              }
             }
           }
           if (ways == 1) {
-            finish(r, d, m, l, o);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+              if (is[n]) finish(row[n], word[n], m[n], l[n], o[n]);
           } else {      // (the warps' shares in shared memory have been read)
             float* t = mrg + x * 6;
-            t[0] = m, t[1] = l, t[2] = o.x, t[3] = o.y, t[4] = o.z, t[5] = o.w;
+            t[0] = m[0], t[1] = l[0], t[2] = o[0].x, t[3] = o[0].y, t[4] = o[0].z, t[5] = o[0].w;
           }
         }
         if (ways > 1) {
