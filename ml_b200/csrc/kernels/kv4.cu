@@ -36,8 +36,9 @@ __device__ __forceinline__ uint32_t value_codes(uint32_t w) {      // two codes 
 }
 // ------------------------------------------------------------------ append
 // A thread has 8 neighbouring elements of one head, 4 threads a group, and goes over rows.  Products and sums of the rotation are rounded one by one, so that the value
-// which is cut to 4 bits does not depend on what the compiler contracts.  Bound by the bytes of the rows, and about as much by instructions: 100 for 8
-// elements, so the quotients share a reciprocal and the codes are put together by multiply-adds.
+// which is cut to 4 bits does not depend on what the compiler contracts (a packed product and sum of two values did come out contracted).  Bound by the bytes of the
+// rows, and as much by instructions, some 200 for 8 elements, so the quotients share a reciprocal and the codes are put together by multiply-adds.
+// 8192 rows of 12 + 24 heads of 64, written and read back by the kernel below: 25.4 us, 3.5 TB/s of what has to move; 16 rows of 16 + 32 heads of 128: 3.5 us.
 __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(512, 2) kv4_append_k(uint8_t* __restrict__ pag
 }
 
 // Head sizes 64 and 128, whose halves are whole groups: a thread has the 8 elements of both halves that the rotation mixes, so rows, angles and addresses are fetched and
-// unpacked once for 16 elements (8192 rows of 36 heads of 64: 19 us instead of 23 with 8 a thread).
+// unpacked once for 16 elements (8192 rows of 36 heads of 64, written and read back: 25.4 us against 27.7 with 8 a thread).
 template <int HD>
 __global__ void __launch_bounds__(512, 2) kv4_append_halves_k(uint8_t* __restrict__ pages, bf16* __restrict__ q_out, const bf16* __restrict__ qkv,
                                                               const int* __restrict__ slots, const int* __restrict__ pos, const float* __restrict__ cos,
@@ -328,9 +329,16 @@ __global__ void __launch_bounds__(512, 3) kv4_read_k(bf16* __restrict__ k, bf16*
 // registers.  The largest score m is the reference of all weights so far and moves only when a score passes it by 2^8 (O and the sums are then rescaled): most
 // blocks need a vote instead of reductions over the warp.
 //
-// Work: all sequences' blocks of 16 tokens stand in one row of `total`, each thread block takes an equal piece of it whatever the lengths are, and its 4 warps
-// a quarter each of every sequence's share.  A warp fetches its own blocks by bulk copies through a ring of its own.  A head whose blocks are shared is
-// put together by the thread block that comes last, in the order of the pieces.
+// Work: all heads' blocks of 16 tokens stand in one row of units, each thread block takes an equal piece of it whatever the lengths are, and its 4 warps a quarter
+// each of every head's part in it.  A head has PAD more units, which stand for what it costs to begin and end one (without them, 16 sequences of up to 2048 tokens
+// took 39 us where two of them were empty, and 23 with 2 units).  A warp fetches its own blocks by bulk copies through a ring of its own.  A head whose blocks are
+// shared is put together by the thread block that comes last, in the order of the pieces, so that a call repeats its bits.
+//
+// Measured: 64 sequences of 1024 to 8192 tokens, 32 heads over 8 of 128: 92 us, 3.8 TB/s (58 % of the measured copy rate; 60 us with the arithmetic left out, so
+// that half of what is missing is instructions: 366 a block, of which 200 on the pipe of bitwise operations and shifts, 88 of these and of the FMA pipe's for the
+// values' codes; moving their shifts to multiplications made it 100).  16 sequences of up to 2048 tokens, 16 heads of 128: 23 us, of which 11 are that
+// arithmetic and 8 beginnings, ends and the joining of shares.  One sequence of 1000 tokens, 12 heads of 64: 6.8 us, 1.4 of them an empty kernel's, 2.6 the joining
+// (a fence, a counter, another block's results).  12 warps an SM: 8 or 16 (with 128 registers) are 4 to 8 % slower.
 struct AttnArgs {
   bf16* out;
   float* lse;
@@ -912,7 +920,7 @@ int attn_grid(long B, int Hkv, int width, int page, int hd, int nt) {
 // Threads of a row (`per_row`) in blocks of up to 512, and as many rows at a time as fill the machine; where there are many, a block goes over 4 of them and more
 struct Shape { dim3 grid; unsigned threads; };
 Shape rows_shape(long per_row, long N) {
-  if (per_row < 1 || per_row >= 1L << 30 || N < 1 || N >= 1L << 31) return {dim3(), 0};
+  if (per_row < 1 || per_row >= 1L << 30 || N < 1 || N >= (1L << 31) - 65536) return {dim3(), 0};
   const long blocks = (per_row + 511) / 512, threads = ((per_row + blocks - 1) / blocks + 31) / 32 * 32;
   const long room = 2048L / threads * mlb_sm_count() / blocks + 1, many = (N + 3) / 4 > room ? (N + 3) / 4 : room, rows = N < many ? N : many;
   return {dim3((unsigned)blocks, (unsigned)(rows < 65535 ? rows : 65535)), (unsigned)threads};

@@ -14,12 +14,13 @@ from .. import ops
 
 
 class Cache4:
-    """Pool of pages for `layers` layers, block tables of `rows` sequences of up to `tokens` tokens, and one spare page a sequence where they are beams."""
+    """Pool of pages for `layers` layers, block tables of `rows` sequences of up to `tokens` tokens, and one spare page a sequence where they are beams; `shared`:
+    full pages of a sequence that are another one's too (a prompt's, of all beams of a request but the first), for `sharing` sequences."""
 
-    def __init__(self, layers: int, rows: int, tokens: int, Hkv: int, hd: int, page: int = 64, device="cpu", spares: bool = False):
+    def __init__(self, layers: int, rows: int, tokens: int, Hkv: int, hd: int, page: int = 64, device="cpu", spares: bool = False, shared: int = 0, sharing: int = 0):
         i32 = dict(dtype=torch.int32, device=device)
         self.page, self.width = page, -(-tokens // page)
-        n = rows * (self.width + int(spares))
+        n = rows * (self.width + int(spares)) - shared * sharing
         self.pages = torch.empty(layers, n, Hkv, page // 16, 18 * hd, dtype=torch.uint8, device=device)
         self.table = torch.full((rows, self.width), -1, **i32)
         self.lens = torch.zeros(rows, **i32)
@@ -45,14 +46,14 @@ class Cache4:
 class CachedDecoder:
     """A `GPT`'s weights behind a 4-bit cache of `rows` sequences."""
 
-    def __init__(self, gpt, rows: int, tokens: int, page: int = 64, spares: bool = False):
+    def __init__(self, gpt, rows: int, tokens: int, page: int = 64, spares: bool = False, shared: int = 0, sharing: int = 0):
         c = gpt.cfg
         if gpt.sharded or gpt.cp is not None:
             raise ValueError("generation from the cache needs the whole model on this device")
         if tokens > c.T:
             raise ValueError(f"{tokens} tokens: the model's window has {c.T}")
         self.gpt, self.c, self.dev, self.dtype = gpt, c, gpt.device, gpt.dtype
-        self.cache = Cache4(c.L, rows, tokens, c.H, c.hd, page, gpt.device, spares)
+        self.cache = Cache4(c.L, rows, tokens, c.H, c.hd, page, gpt.device, spares, shared, sharing)
 
     def _new(self, *shape, dtype=None):
         return torch.empty(*shape, dtype=dtype or self.dtype, device=self.dev)
@@ -132,7 +133,7 @@ def beam_search(gpt, prompt, n_new, beams, eos=-1, page=64, length_penalty=0.0):
     has chosen `eos` is filled up with it; beams are compared by log-probability / length^length_penalty at the end (length: up to and with the first eos)."""
     b, P = prompt.shape
     rows = b * beams
-    m = CachedDecoder(gpt, rows, P + n_new, page, spares=True)
+    m = CachedDecoder(gpt, rows, P + n_new, page, True, P // page, rows - b)
     k, dev = m.cache, m.dev
     i32 = dict(dtype=torch.int32, device=dev)
     ids = prompt.to(dev).int()

@@ -27,6 +27,12 @@ def _pool(pages):
     return pages
 
 
+def _took(rc, name):
+    if rc == -7:
+        raise ValueError(f"{name}: sizes past what the kernel counts in 32 bits")
+    _n._chk(rc, name)
+
+
 def _here(*ts):
     dev = torch._C._cuda_getDevice()
     for t in ts:
@@ -50,7 +56,7 @@ def kv4_append(pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd):
     if N == 0:
         return
     rope = cos is not None
-    _n._chk(_n._entries().mlb_kv4_append(_pool(pages), NONE if q_out is None else q_out, _rows(qkv, "qkv"), slots, pos if rope else NONE, cos if rope else NONE,
+    _took(_n._entries().mlb_kv4_append(_pool(pages), NONE if q_out is None else q_out, _rows(qkv, "qkv"), slots, pos if rope else NONE, cos if rope else NONE,
                                          sin if rope else NONE, n, page, N, qkv.stride(0), H, Hkv, hd, cos.shape[0] if rope else 0), "kv4_append")
 
 
@@ -60,7 +66,7 @@ def kv4_read(k, v, pages, slots):
     n, Hkv, page, hd, N = check_read(k, v, pages, slots)
     _here(k, v, pages, slots)
     if N:
-        _n._chk(_n._entries().mlb_kv4_read(k, v, _pool(pages), slots, n, page, N, Hkv, hd), "kv4_read")
+        _took(_n._entries().mlb_kv4_read(k, v, _pool(pages), slots, n, page, N, Hkv, hd), "kv4_read")
 
 
 def kv4_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale=None):
@@ -71,9 +77,9 @@ def kv4_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale=None):
     if B == 0:
         return
     e, dev, width = _n._entries(), q.device, table.shape[1]
-    part = _n.scratch("kv4_part", e.mlb_kv4_attn_scratch(B, Tq, H, Hkv, hd, width, page), F32, dev)
+    part = _n.scratch("kv4_part", max(0, e.mlb_kv4_attn_scratch(B, Tq, H, Hkv, hd, width, page)), F32, dev)
     count = _n.scratch("kv4_count", B * Hkv * -(-H // Hkv * Tq // 8), I32, dev, zero=True)
-    _n._chk(e.mlb_kv4_attn(out, NONE if lse is None else lse, _rows(q, "q"), _pool(pages), table, lens, part, count, n, q.stride(0), B, Tq, H, Hkv, hd, width, page,
+    _took(e.mlb_kv4_attn(out, NONE if lse is None else lse, _rows(q, "q"), _pool(pages), table, lens, part, count, n, q.stride(0), B, Tq, H, Hkv, hd, width, page,
                            1.0 / math.sqrt(hd) if scale is None else scale), "kv4_attn")
 
 
@@ -83,7 +89,7 @@ def block_tables(table, slots, pos, starts, new_lens, left, lens, new, free, n_f
     B = check_tables(table, slots, pos, starts, new_lens, left, lens, new, free, n_free, page)
     _here(table, slots, pos, starts, new_lens, left, lens, new, free, n_free)
     ticket = _n.scratch("tables_ticket", 1, I32, table.device, zero=True)
-    _n._chk(_n._entries().mlb_block_tables(table, slots, pos, starts, new_lens, left, ticket, lens, new, free, n_free, B, table.shape[1], page, slots.numel(),
+    _took(_n._entries().mlb_block_tables(table, slots, pos, starts, new_lens, left, ticket, lens, new, free, n_free, B, table.shape[1], page, slots.numel(),
                                            free.numel()), "block_tables")
 
 
@@ -103,7 +109,7 @@ def beam_select(scores, tokens, parents, done_out, logits, prev, done, eos):
     part = _n.scratch("select_part", rows * pieces * (2 + 4 * K), F32, dev)
     ticket = _n.scratch("select_ticket", B, I32, dev, zero=True)
     base, n = part.data_ptr(), rows * pieces
-    _n._chk(e.mlb_beam_select(scores, tokens, parents, done_out, Address(logits.data_ptr()), prev, done, part, Address(base + 8 * n), Address(base + 8 * n + 8 * n * K),
+    _took(e.mlb_beam_select(scores, tokens, parents, done_out, Address(logits.data_ptr()), prev, done, part, Address(base + 8 * n), Address(base + 8 * n + 8 * n * K),
                               ticket, rows, K, V, logits.stride(0), eos, bits), "beam_select")
 
 
@@ -114,5 +120,5 @@ def beam_reorder(pages, table_out, spare_out, hist_out, table, spare, lens, hist
     _here(pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens)
     if B * K == 0:
         return
-    _n._chk(_n._entries().mlb_beam_reorder(NONE if pages is None else _pool(pages), table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, layers, n,
+    _took(_n._entries().mlb_beam_reorder(NONE if pages is None else _pool(pages), table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, layers, n,
                                            Hkv, page, block, B, K, table.shape[1], hist.shape[1]), "beam_reorder")
