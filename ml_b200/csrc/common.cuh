@@ -123,6 +123,13 @@ __device__ __forceinline__ void mlb_set_error(int code, int detail) {
   atomicCAS(&g_mlb_error, 0, (code << 24) | (detail & 0xFFFFFF));
 }
 
+// One more at a counter of blocks, by one thread between two barriers of its block: what the block wrote before is there for the block that finds the count full.
+__device__ __forceinline__ int mlb_count_block(int* counter) {
+  int before;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
+}
+
 static inline int ceil_div_i(long a, long b) { return (int)((a + b - 1) / b); }
 
 __device__ __forceinline__ float warp_sum(float v) {

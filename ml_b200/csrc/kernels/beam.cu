@@ -113,9 +113,8 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
   if (blockIdx.x == 0)
     for (int r = tid; r <= A.B; r += TAB_THREADS) A.starts[r] = start[r];
   if (gridDim.x > 1) {
-    __threadfence();
     __syncthreads();
-    if (tid == 0) last = atomicAdd(A.ticket, 1) == (int)gridDim.x - 1;
+    if (tid == 0) last = mlb_count_block(A.ticket) == (int)gridDim.x - 1;
     __syncthreads();
     if (!last) return;
     if (tid == 0) *A.ticket = 0;
@@ -387,11 +386,7 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
   }
   // ---- the request's last thread block merges
   __syncthreads();
-  if (tid == 0) {
-    __threadfence();      // (the block's list before the count)
-    last = atomicAdd(A.ticket + req, 1) == A.pieces * K - 1;
-    __threadfence();
-  }
+  if (tid == 0) last = mlb_count_block(A.ticket + req) == A.pieces * K - 1;
   __syncthreads();
   if (!last) return;
   const int lists = K * A.pieces, L = A.L;

@@ -799,11 +799,7 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
     }
     if (n_shares > 1) {
       __syncthreads();
-      if (tid == 0) {
-        __threadfence();      // (the block's shares before the count)
-        last = atomicAdd(A.count + item, 1) == n_shares - 1;
-        __threadfence();
-      }
+      if (tid == 0) last = mlb_count_block(A.count + item) == n_shares - 1;
       __syncthreads();
       if (last) {
         if (tid == 0) A.count[item] = 0;      // for the next call
