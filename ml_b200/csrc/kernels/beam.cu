@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
         add = 0;
       } else if ((long)len + add <= (long)A.width * A.page) {
         fits = true;
-        need = (len + add + A.page - 1) / A.page - (len + A.page - 1) / A.page;
+        need = ((unsigned)len + add + A.page - 1) / A.page - ((unsigned)len + A.page - 1) / A.page;
       }
     }
     Two total;
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
         else hi = mid;
       }
       if (first[r] >= 0) {
-        const int len = A.lens[r], has = (len + A.page - 1) / A.page;
+        const int len = A.lens[r], has = ((unsigned)len + A.page - 1) / A.page;
         at = len + row - start[r];
         const int p = at / A.page, off = at - p * A.page;
         int id;
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
           id = A.stack[n_free - 1 - (first[r] + p - has)];
           if (off == 0) A.table[(long)r * A.width + p] = id;
         }
-        slot = id < 0 ? -1 : id * A.page + off;
+        slot = id < 0 ? -1 : (int)min((long)id * A.page + off, 0x7FFFFFFFL);      // (the last number is no slot of any pool)
       }
     }
     A.slots[row] = slot;
@@ -460,13 +460,13 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
 // logits and more each, and no more lists than a thread block holds to merge
 int select_list(int K) { return K <= 16 ? 2 * K : K; }      // entries of a piece's list: usually all its candidates, which then need no places
 int select_piece(int rows, int K, int V, int bits) {
-  const long fill = (long)SEL_PER_SM * mlb_sm_count() / rows, one = ((long)V * (bits / 8) + SEL_CHUNK_BYTES - 1) / SEL_CHUNK_BYTES, most = (V + SEL_LEAST - 1) / SEL_LEAST,
+  const long fill = (long)SEL_PER_SM * mlb_sm_count() / rows, one = ((long)V * (bits / 8) + SEL_CHUNK_BYTES - 1) / SEL_CHUNK_BYTES, most = (V - 1) / SEL_LEAST + 1,
              held = SEL_HELD / (K * select_list(K));
   long n = fill > one ? fill : one;
   n = n < most ? n : most;
   n = n < held ? n : held;
   n = n < 1 ? 1 : n;
-  return (int)((V + n - 1) / n + 7) / 8 * 8;
+  return (int)(((V + n - 1) / n + 7) / 8 * 8);
 }
 template <typename T, bool BULK>
 cudaError_t launch_select(const SelectArgs& a, int rows, cudaStream_t st) {
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(ORDER_THREADS) beam_reorder_k(const OrderArgs 
 
 MLB_API int mlb_block_tables(int* table, int* slots, int* pos, int* starts, int* new_lens, int* left, int* ticket, const int* lens, const int* news,
                              const int* stack, const int* n_free, int B, int width, int page, int rows, int stack_size, cudaStream_t st) {
-  if (B < 1 || B > TAB_MAX_B || page < 1 || width < 1 || rows < 0 || rows > TAB_MAX_ROWS || (long)B * width >= 1L << 31) return -7;
+  if (B < 1 || B > TAB_MAX_B || page < 1 || width < 1 || rows < 0 || rows > TAB_MAX_ROWS || (long)B * width >= 1L << 31 || (long)width * page >= 1L << 31) return -7;
   const int want = (rows + TAB_THREADS - 1) / TAB_THREADS, most = 2 * mlb_sm_count();
   const TableArgs a{table, slots, pos, starts, new_lens, left, ticket, lens, news, stack, n_free, B, width, page, rows, stack_size};
   return (int)mlb_launch(block_tables_k, dim3(want < 1 ? 1 : want < most ? want : most), dim3(TAB_THREADS), (2 * B + 1) * sizeof(int), st, a);
@@ -549,7 +549,7 @@ MLB_API int mlb_block_tables(int* table, int* slots, int* pos, int* starts, int*
 MLB_API int mlb_beam_select_pieces(int rows, int K, int V, int bits) {
   if (K < 1 || K > SEL_MAX_K || V < 1 || rows < 1 || rows > 65535 || (long)K * V >= 0xFFFFFFFFL) return -7;
   const int piece = select_piece(rows, K, V, bits);
-  return (V + piece - 1) / piece;
+  return (V - 1) / piece + 1;
 }
 // bits: 16 (bf16) or 32 (fp32) logits, rows `stride` elements apart
 MLB_API int mlb_beam_select(float* scores, int* tokens, int* parents, int* done_out, const void* logits, const float* prev, const int* done, float* stats,
@@ -566,7 +566,7 @@ MLB_API int mlb_beam_select(float* scores, int* tokens, int* parents, int* done_
 MLB_API int mlb_beam_reorder(uint8_t* pages, int* table_out, int* spare_out, int* hist_out, const int* table, const int* spare, const int* lens, const int* hist,
                              const int* parents, const int* tokens, int layers, long n_pages, int Hkv, int page, int block_bytes, int B, int K, int width, int T,
                              cudaStream_t st) {
-  if (page < 16 || page % 16 != 0 || block_bytes % 16 != 0 || K < 1 || width < 1 || layers > 65534) return -7;
+  if (page < 16 || page % 16 != 0 || block_bytes % 16 != 0 || K < 1 || width < 1 || layers > 65534 || (long)width * page >= 1L << 31) return -7;
   // a part is 1024 words (16 KB) of a page or more
   const long words = (long)Hkv * (page / 16) * (block_bytes / 16), most = layers > 0 ? 65534 / layers : 1;
   if (words >= 1L << 28) return -7;

@@ -976,7 +976,7 @@ MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pa
   if (!known_head(hd) || shift < 0 || Hkv < 1 || H % Hkv != 0 || q_stride % 8 != 0) return -7;
   int nt;
   const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
-  if (tiles > 65535 || (long)n_pages > 0x7FFFFFFFL || (long)Hkv * page * hd * 9 / 8 >= 1L << 32 || ((long)width * page / TOK + PAD) * (B < MAX_B ? B : MAX_B) * Hkv >= 1L << 31) return -7;
+  if (tiles > 65535 || (long)n_pages > 0x7FFFFFFFL || (long)width * page >= 1L << 31 || (long)Hkv * page * hd * 9 / 8 >= 1L << 32 || ((long)width * page / TOK + PAD) * (B < MAX_B ? B : MAX_B) * Hkv >= 1L << 31) return -7;
   cudaError_t e = cudaSuccess;
   for (int b = 0; b < B && e == cudaSuccess; b += MAX_B) {
     const int n = B - b < MAX_B ? B - b : MAX_B;

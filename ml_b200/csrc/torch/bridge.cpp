@@ -656,7 +656,7 @@ PyObject* py_kv4_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (ou
     if (!std::isfinite(scale)) return declined();
   }
   const long B = lens.size(0);
-  if (!plain(a[4], table, at::kInt, 2) || !sized(table, {B, table.size(1)}) || !rows_given(a[2], q, B * Tq, H * hd) || !given(a[0], out, at::kBFloat16, {B * Tq, H * hd}) ||
+  if (!plain(a[4], table, at::kInt, 2) || !sized(table, {B, table.size(1)}) || table.numel() >= (1L << 31) || !rows_given(a[2], q, B * Tq, H * hd) || !given(a[0], out, at::kBFloat16, {B * Tq, H * hd}) ||
       !aligned(out) || (a[1] != Py_None && !given(a[1], lse, at::kFloat, {B, H, Tq})))
     return declined();
   const St st = stream();
@@ -677,7 +677,7 @@ PyObject* py_block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {      //
       !plain(a[8], stack, at::kInt, 1) || !stack.is_contiguous() || !int_arg(a[10], page))
     return declined();
   const long B = lens.size(0), rows = slots.size(0);
-  if (!plain(a[0], table, at::kInt, 2) || !sized(table, {B, table.size(1)}) || !given(a[2], pos, at::kInt, {rows}) || !given(a[3], starts, at::kInt, {B + 1}) ||
+  if (!plain(a[0], table, at::kInt, 2) || !sized(table, {B, table.size(1)}) || table.numel() >= (1L << 31) || !given(a[2], pos, at::kInt, {rows}) || !given(a[3], starts, at::kInt, {B + 1}) ||
       !given(a[4], new_lens, at::kInt, {B}) || !given(a[5], left, at::kInt, {1}) || !given(a[7], news, at::kInt, {B}) || !given(a[9], n_free, at::kInt, {1}))
     return declined();
   const St st = stream();
@@ -725,7 +725,7 @@ PyObject* py_beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {      //
     if (!pool_given(a[0], p, 5) || (a[10] != Py_None && page != p.page)) return declined();
     page = p.page;
   }
-  if (page < 16 || page % 16 != 0 || !sized(table, {rows, width}) || !sized(hist, {rows, T}) || !given(a[1], table_out, at::kInt, {rows, width}) ||
+  if (page < 16 || page % 16 != 0 || !sized(table, {rows, width}) || !sized(hist, {rows, T}) || table.numel() >= (1L << 31) || T >= (1L << 31) || !given(a[1], table_out, at::kInt, {rows, width}) ||
       !given(a[2], spare_out, at::kInt, {rows}) || !given(a[3], hist_out, at::kInt, {rows, T}) || !given(a[5], spare, at::kInt, {rows}) || !given(a[6], lens, at::kInt, {rows}) ||
       !given(a[9], tokens, at::kInt, {B, Kb}) || table.data_ptr() == table_out.data_ptr() || spare.data_ptr() == spare_out.data_ptr() || hist.data_ptr() == hist_out.data_ptr())
     return declined();

@@ -38,6 +38,11 @@ def need(t, shape, what, dtype=None):
         raise ValueError(f"{what} {tuple(t.shape)} {t.dtype}: need {tuple(shape)}" + (f" {dtype}" if dtype is not None else ""))
 
 
+def _row_tokens(table, page):
+    if table.shape[1] * page >= 1 << 31:
+        raise ValueError(f"rows of {table.shape[1]} pages of {page} tokens: places in a sequence are 32-bit numbers")
+
+
 def check_append(pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd):
     n, heads, page, _ = pages_shape(pages, hd)
     if H < 0 or heads != Hkv:
@@ -75,6 +80,7 @@ def check_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale):
     need(lens, (B,), "lens", torch.int32)
     if table.dim() != 2 or table.shape[0] != B or table.dtype != torch.int32:
         raise ValueError(f"table {tuple(table.shape)} {table.dtype}: need int32 [{B}, pages of a sequence]")
+    _row_tokens(table, page)
     need(q, (B * Tq, H * hd), "q")
     need(out, (B * Tq, H * hd), "out", q.dtype)
     if lse is not None:
@@ -88,6 +94,7 @@ def check_tables(table, slots, pos, starts, new_lens, left, lens, new, free, n_f
         raise ValueError(f"{B} requests, {slots.numel()} places, pages of {page}: 1 to 4096 requests and 2^22 places at most")
     if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1:
         raise ValueError(f"table {tuple(table.shape)}: need [{B}, pages of a request]")
+    _row_tokens(table, page)
     for t, s, n in ((table, table.shape, "table"), (slots, (slots.numel(),), "slots"), (pos, (slots.numel(),), "pos"), (starts, (B + 1,), "starts"), (new_lens, (B,), "new_lens"),
                     (left, (1,), "left"), (lens, (B,), "lens"), (new, (B,), "new"), (free, (free.numel(),), "free"), (n_free, (1,), "n_free")):
         need(t, s, n, torch.int32)
@@ -102,8 +109,8 @@ def check_select(scores, tokens, parents, done_out, logits, prev, done):
         raise ValueError(f"{K} beams: 1 to 32 a request")
     if logits.dim() != 2 or logits.shape[0] != B * K or logits.shape[1] < 1 or logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"logits {tuple(logits.shape)} {logits.dtype}: need bfloat16 or float32 [{B * K}, V]")
-    if K * logits.shape[1] >= 0xFFFFFFFF:
-        raise ValueError(f"{K} beams of {logits.shape[1]} logits: their product has to stay below 2^32")
+    if K * logits.shape[1] >= 0xFFFFFFFF or logits.shape[1] >= 1 << 31:
+        raise ValueError(f"{K} beams of {logits.shape[1]} logits: their product has to stay below 2^32, and the logits below 2^31")
     for t, n, d in ((scores, "scores", torch.float32), (prev, "prev", torch.float32), (tokens, "tokens", torch.int32), (parents, "parents", torch.int32),
                     (done_out, "done_out", torch.int32), (done, "done", torch.int32)):
         need(t, (B, K), n, d)
@@ -127,12 +134,14 @@ def check_reorder(pages, table_out, spare_out, hist_out, table, spare, lens, his
     if pages is None:
         if page is None or page < 16 or page % 16:
             raise ValueError(f"page = {page}: without pages the tokens of a page have to be given, a multiple of 16")
+        _row_tokens(table, page)
         return 0, 0, 0, page, 16, B, K
     if pages.dim() != 5:
         raise ValueError(f"pages {tuple(pages.shape)}: need [layers, n_pages, Hkv, page / 16, 18 hd]")
     n, Hkv, size, hd = pages_shape(pages[0] if pages.shape[0] else pages.new_empty(pages.shape[1:]))
     if page is not None and page != size:
         raise ValueError(f"page = {page}, and pages of {size} tokens")
+    _row_tokens(table, size)
     return pages.shape[0], n, Hkv, size, 18 * hd, B, K
 
 
@@ -292,7 +301,7 @@ def block_tables(table, slots, pos, starts, new_lens, left, lens, new, free, n_f
             taken = max(taken, asked)
             t = torch.arange(L[r], L[r] + N[r], device=table.device)
             ids = table[r, t // page]
-            slots[at:at + N[r]] = torch.where(ids < 0, -1, ids * page + t % page).int()
+            slots[at:at + N[r]] = torch.where(ids < 0, -1, (ids.long() * page + t % page).clamp(max=(1 << 31) - 1)).int()
             pos[at:at + N[r]] = t.int()
             L[r] += N[r]
         at += N[r]

@@ -8,7 +8,7 @@ import torch
 
 from ml_b200 import Config, ops
 from ml_b200.models import GPT, generation
-from ml_b200.ops import ref
+from ml_b200.ops import ref, ref_gen
 from tests import generation_oracle as oracle
 
 I32 = torch.int32
@@ -71,6 +71,35 @@ def test_plain_tables(B, page, width, old, new, free):
     slots, pos, starts = torch.empty(rows, dtype=I32), torch.empty(rows, dtype=I32), torch.empty(B + 1, dtype=I32)
     ops.block_tables(t, slots, pos, starts, l, nf, l, ints(news), ints(stack), nf, page)
     assert (t.tolist(), slots.tolist(), pos.tolist(), starts.tolist(), l.tolist(), int(nf)) == oracle.tables(table, lens, news, stack, free, page, rows)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """A place in a sequence, a slot and a token are 32-bit numbers."""
+    one, wide = torch.zeros(1, dtype=I32), lambda n: torch.empty(1, n, dtype=I32)
+    x = torch.zeros(1, 64)
+    pages = torch.zeros(4, 1, 8, 18 * 64, dtype=torch.uint8)
+    attn = lambda n: ref_gen.check_attn(x, None, x, pages, wide(n), one, 1, 1, 1, 64, None)
+    tables = lambda n, page: ref_gen.check_tables(wide(n), one, one, ints([0, 0]), one, one, one, one, one, one, page)
+    order = lambda n, pool, page: ref_gen.check_reorder(pool, wide(n), one, ints([[0]]), wide(n), ints([0]), one, ints([[0]]), ints([[0]]), ints([[0]]), page)
+    select = lambda V: ref_gen.check_select(torch.zeros(1, 1), one[None], one[None], one[None], torch.empty(1, V, device="meta"), torch.zeros(1, 1), one[None])
+    for f in (attn, lambda n: tables(n, 128), lambda n: order(n, pages[None], None), lambda n: order(n, None, 128)):
+        f((1 << 24) - 1)
+        with pytest.raises(ValueError, match="32-bit"):
+            f(1 << 24)
+    tables(1, (1 << 31) - 1)
+    with pytest.raises(ValueError, match="32-bit"):
+        tables(1, 1 << 31)
+    select((1 << 31) - 1)
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        select(1 << 31)
+
+
+def test_a_page_number_whose_slot_passes_32_bits_gets_a_slot_of_no_pool():
+    """... and not another page's."""
+    table, slots, pos = ints([[-1, -1]]), ints([0] * 70), ints([0] * 70)
+    ops.block_tables(table, slots, pos, ints([0, 0]), ints([0]), ints([0]), ints([0]), ints([70]), ints([1 << 26, 1 << 24]), ints([2]), 64)
+    assert table.tolist() == [[1 << 24, 1 << 26]]
+    assert slots.tolist() == [(1 << 30) + t for t in range(64)] + [(1 << 31) - 1] * 6
 
 
 @pytest.mark.parametrize("B,K,V", [(1, 1, 1), (1, 4, 3), (3, 5, 200)])

@@ -330,6 +330,27 @@ def test_block_tables(B, page, width, most_old, most_new, free, alias):
         assert g == w, name
 
 
+def test_a_page_number_whose_slot_passes_32_bits_gets_a_slot_of_no_pool():
+    """... and not another page's."""
+    table, slots, pos = ints([[-1, -1]]), ints([0] * 70), ints([0] * 70)
+    ops.block_tables(table, slots, pos, ints([0, 0]), ints([0]), ints([0]), ints([0]), ints([70]), ints([1 << 26, 1 << 24]), ints([2]), 64)
+    assert table.tolist() == [[1 << 24, 1 << 26]]
+    assert slots.tolist() == [(1 << 30) + t for t in range(64)] + [(1 << 31) - 1] * 6
+
+
+def test_tables_past_32_bits_are_refused():
+    x = torch.zeros(1, 64, dtype=torch.bfloat16, device=dev())
+    pages = torch.zeros(4, 1, 8, 18 * 64, dtype=torch.uint8, device=dev())
+    wide, other = (torch.zeros(1, 1 << 24, dtype=I32, device=dev()) for _ in range(2))
+    calls = [lambda t: ops.kv4_attn(torch.empty_like(x), None, x, pages, t, ints([0]), 1, 1, 1, 64),
+             lambda t: ops.block_tables(t, ints([0]), ints([0]), ints([0, 0]), ints([0]), ints([0]), ints([0]), ints([0]), ints([0]), ints([1]), 128),
+             lambda t: ops.beam_reorder(pages[None], other[:, :t.shape[1]], ints([0]), ints([[0]]), t, ints([0]), ints([0]), ints([[0]]), ints([[0]]), ints([[0]]))]
+    for f in calls:
+        f(wide[:, :-1])
+        with pytest.raises(ValueError, match="32-bit"):
+            f(wide)
+
+
 def test_block_tables_report_what_does_not_fit():
     def call(lens, new, places, n_free=4):
         t, s, p, st = torch.full((len(lens), 3), -1, dtype=I32, device=dev()), torch.zeros(places, dtype=I32, device=dev()), torch.zeros(places, dtype=I32, device=dev()), torch.zeros(len(lens) + 1, dtype=I32, device=dev())
