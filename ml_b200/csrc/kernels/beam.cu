@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
     if (key != 0 && key >= bound) cand[atomicAdd(&n_cand, 1)] = key;
   }
   __syncthreads();
-  const int found = n_cand;
+  const int found = n_cand;      // (K or more: every beam has a continuation, if one of -inf)
   for (int e = tid; e < found; e += SEL_THREADS) {
     const u64 mine = cand[e];
     const int k = place_of(mine, cand, found);
@@ -449,10 +449,6 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
       A.scores[o] = unordered((uint32_t)(mine >> 32));
       A.tokens[o] = t, A.parents[o] = from, A.done_out[o] = ended[from] || t == A.eos;
     }
-  }
-  if (tid >= found && tid < K) {      // fewer continuations than beams (V < K)
-    const int o = req * K + tid;
-    A.scores[o] = -INFINITY, A.tokens[o] = A.eos, A.parents[o] = 0, A.done_out[o] = 1;
   }
 }
 

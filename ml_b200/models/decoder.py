@@ -502,8 +502,8 @@ class GPT:
             raise ValueError(f"kv={kv!r}: None or '4bit'")
         if kv is not None:
             from . import generation
-            if b < 1 or P < 1 or n_new < 0:
-                raise ValueError(f"{b} prompts of {P} tokens, {n_new} more")
+            if b < 1 or P < 1 or n_new < 0 or beams < 1:
+                raise ValueError(f"{b} prompts of {P} tokens, {n_new} more, {beams} beams")
             if beams > 1 and n_new:
                 if temperature > 0:
                     raise ValueError("beams and sampling exclude each other")

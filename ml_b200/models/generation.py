@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
+from ..ops.ref_gen import HEADS, PAGES
 
 
 class Cache4:
@@ -18,6 +19,10 @@ class Cache4:
     full pages of a sequence that are another one's too (a prompt's, of all beams of a request but the first), for `sharing` sequences."""
 
     def __init__(self, layers: int, rows: int, tokens: int, Hkv: int, hd: int, page: int = 64, device="cpu", spares: bool = False, shared: int = 0, sharing: int = 0):
+        if page not in PAGES:
+            raise ValueError(f"pages of {page} tokens: the 4-bit cache has {PAGES}")
+        if hd not in HEADS:
+            raise ValueError(f"head size {hd}: the 4-bit cache has {HEADS}")
         i32 = dict(dtype=torch.int32, device=device)
         self.page, self.width = page, -(-tokens // page)
         n = rows * (self.width + int(spares)) - shared * sharing

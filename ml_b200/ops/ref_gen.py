@@ -16,6 +16,7 @@ import torch
 
 TOK = 16             # tokens of a block
 TINY = 2.0 ** -120   # a smaller scale is held as 0
+HEADS, PAGES = (32, 64, 96, 128), (16, 32, 64, 128)      # head sizes, tokens of a page
 
 
 # ------------------------------------------------------------------ checks
@@ -24,10 +25,10 @@ def pages_shape(pages, hd=None):
     if pages.dim() != 4 or pages.dtype != torch.uint8 or pages.shape[3] % 18 or (hd is not None and pages.shape[3] != 18 * hd):
         raise ValueError(f"pages {tuple(pages.shape)} {pages.dtype}: need uint8 [n_pages, Hkv, page / 16, 18 hd]" + (f" with hd = {hd}" if hd else ""))
     n, Hkv, blocks, b = pages.shape
-    if b // 18 not in (32, 64, 96, 128):
-        raise ValueError(f"head size {b // 18}: the 4-bit cache has 32, 64, 96 and 128")
-    if blocks not in (1, 2, 4, 8):
-        raise ValueError(f"pages of {16 * blocks} tokens: the 4-bit cache has 16, 32, 64 and 128")
+    if b // 18 not in HEADS:
+        raise ValueError(f"head size {b // 18}: the 4-bit cache has {HEADS}")
+    if TOK * blocks not in PAGES:
+        raise ValueError(f"pages of {TOK * blocks} tokens: the 4-bit cache has {PAGES}")
     if n * blocks * TOK >= 1 << 31:
         raise ValueError(f"{n} pages of {16 * blocks} tokens: slots are 32-bit numbers")
     return n, Hkv, TOK * blocks, b // 18
@@ -327,15 +328,11 @@ def beam_select(scores, tokens, parents, done_out, logits, prev, done, eos):
     kept = torch.where(torch.arange(V, device=z.device) == eos, prev[..., None], torch.full_like(s, ninf))
     s = torch.where((done != 0)[..., None], torch.where(torch.isnan(kept), torch.full_like(s, ninf), kept), s).view(B, K * V)
     best, at = torch.sort(s, dim=1, descending=True, stable=True)
-    n = min(K, K * V)
-    at = at[:, :n]
+    best, at = best[:, :K], at[:, :K]
     par, tok = at // V, at % V
     ended = (done != 0).gather(1, par) | (tok == eos)
-    scores.fill_(ninf)
-    tokens.fill_(eos)
-    parents.zero_()
-    done_out.fill_(1)
-    scores[:, :n], tokens[:, :n], parents[:, :n], done_out[:, :n] = best[:, :n], tok.int(), par.int(), ended.int()
+    for out, x in ((scores, best), (tokens, tok), (parents, par), (done_out, ended)):
+        out.copy_(x)
 
 
 def beam_reorder(pages, table_out, spare_out, hist_out, table, spare, lens, hist, parents, tokens, page=None):

@@ -215,6 +215,33 @@ def test_generate_refuses_what_the_cache_has_not():
         odd.generate(p, 2, kv="4bit")
 
 
+@pytest.mark.parametrize("page", [-64, 0, 8, 24, 48, 100, 256])
+def test_pages_of_other_sizes_are_refused_before_anything_is_laid_out(page):
+    """A pool cut down to whole blocks would not be the one that slots are counted in."""
+    with pytest.raises(ValueError, match="pages of"):
+        generation.Cache4(1, 1, 100, 1, 64, page)
+    with pytest.raises(ValueError, match="pages of"):
+        small().generate(torch.zeros(1, 10, dtype=torch.long), 4, kv="4bit", page=page)
+
+
+def test_no_beam_is_refused():
+    for n in (0, 4):
+        with pytest.raises(ValueError, match="0 beams"):
+            small().generate(torch.zeros(1, 10, dtype=torch.long), n, kv="4bit", beams=0)
+
+
+@pytest.mark.parametrize("B,K,V,eos", [(2, 5, 1, 0), (2, 32, 3, -1), (1, 4, 2, 7)])
+def test_plain_selection_over_fewer_tokens_than_beams(B, K, V, eos):
+    torch.manual_seed(K)
+    z, prev, done = torch.randn(B * K, V), torch.randn(B, K), (torch.rand(B, K) < 0.5).int()
+    z[0] = float("-inf")
+    got = torch.empty(B, K), ints([[9] * K] * B), ints([[9] * K] * B), ints([[9] * K] * B)
+    ops.beam_select(*got, z, prev, done, eos)
+    assert ((0 <= got[1]) & (got[1] < V) & (0 <= got[2]) & (got[2] < K)).all() and not torch.isnan(got[0]).any()
+    flat = got[2].long() * V + got[1]
+    assert all(len(set(r)) == K for r in flat.tolist())
+
+
 def test_generate_mode_reads_the_cache(tmp_path):
     import os
     import subprocess

@@ -455,6 +455,16 @@ def test_beam_select_of_equal_logits_masks_and_nan(dtype):
     check_choice(z, prev, torch.ones_like(done), 5)
 
 
+@pytest.mark.parametrize("B,K,V,eos", [(2, 5, 1, 0), (2, 32, 3, -1), (1, 4, 2, 7), (3, 17, 16, 15)])
+def test_beam_select_over_fewer_tokens_than_beams(B, K, V, eos):
+    torch.manual_seed(K)
+    logits, prev, done = torch.randn(B * K, V).bfloat16(), -10 * torch.rand(B, K), (torch.rand(B, K) < 0.5).int()
+    logits[0] = -math.inf
+    check_choice(logits, prev, done, eos)
+    prev[:, 1:] = -math.inf
+    check_choice(logits, prev, torch.zeros_like(done), eos)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("B,K,V,stride", [(1, 32, 50304, 0), (2, 16, 70001, 7), (1000, 1, 300, 0), (3, 24, 40000, 0)])
 def test_beam_select_of_pieces_that_are_fetched_in_parts(dtype, B, K, V, stride):
