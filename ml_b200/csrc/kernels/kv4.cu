@@ -38,7 +38,7 @@ __device__ __forceinline__ uint32_t value_codes(uint32_t w) {      // two codes 
 // A thread has 8 neighbouring elements of one head, 4 threads a group, and goes over rows.  Products and sums of the rotation are rounded one by one, so that the value
 // which is cut to 4 bits does not depend on what the compiler contracts (a packed product and sum of two values did come out contracted).  Bound by the bytes of the
 // rows, and as much by instructions, some 200 for 8 elements, so the quotients share a reciprocal and the codes are put together by multiply-adds.
-// 8192 rows of 12 + 24 heads of 64, written and read back by the kernel below: 25.4 us, 3.5 TB/s of what has to move; 16 rows of 16 + 32 heads of 128: 3.5 us.
+// 8192 rows of 12 + 24 heads of 64, written and read back by the kernel below: 23.6 us, 3.8 TB/s of what has to move; 16 rows of 16 + 32 heads of 128: 3.6 us.
 __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(512, 2) kv4_append_k(uint8_t* __restrict__ pag
 }
 
 // Head sizes 64 and 128, whose halves are whole groups: a thread has the 8 elements of both halves that the rotation mixes, so rows, angles and addresses are fetched and
-// unpacked once for 16 elements (8192 rows of 36 heads of 64, written and read back: 25.4 us against 27.7 with 8 a thread).
+// unpacked once for 16 elements (8192 rows of 36 heads of 64, written and read back: 25.4 us then, 27.7 with 8 a thread).
 template <int HD>
 __global__ void __launch_bounds__(512, 2) kv4_append_halves_k(uint8_t* __restrict__ pages, bf16* __restrict__ q_out, const bf16* __restrict__ qkv,
                                                               const int* __restrict__ slots, const int* __restrict__ pos, const float* __restrict__ cos,
@@ -913,13 +913,15 @@ int attn_grid(long B, int Hkv, int width, int page, int hd, int nt) {
   const long fit = 228L * 1024 / (attn_smem_of(hd, nt, (int)B) + 1024 + 128) * mlb_sm_count(), want = attn_most(B, Hkv, width, page);      // (1 KB of a block's is the system's)
   return (int)(want < fit ? want : fit);
 }
-// Threads of a row (`per_row`) in blocks of up to 512, and as many rows at a time as fill the machine; where there are many, a block goes over 4 of them and more
+// Threads of a row (`per_row`) in blocks of up to 512, and rows twice as often as the machine holds 1024 threads an SM (append's registers: two waves; reading back: one).  Blocks
+// go over the rows in equal steps, so that a wave of a few blocks more is what costs: 8192 rows of 12 + 24 heads of 64 written and read 23.6 us (25.3 once, 25.3
+// three times, 25.8 with 4 rows a block), of 16 + 32 heads of 128 54.7 (63.7, 56.2, 59.3), 4096 rows of 32 + 16 heads of 128 27.0 (28.0, 28.0, 30.3)
 struct Shape { dim3 grid; unsigned threads; };
 Shape rows_shape(long per_row, long N) {
   if (per_row < 1 || per_row >= 1L << 30 || N < 1 || N >= (1L << 31) - 65536) return {dim3(), 0};
   const long blocks = (per_row + 511) / 512, threads = ((per_row + blocks - 1) / blocks + 31) / 32 * 32;
-  const long room = 2048L / threads * mlb_sm_count() / blocks + 1, many = (N + 3) / 4 > room ? (N + 3) / 4 : room, rows = N < many ? N : many;
-  return {dim3((unsigned)blocks, (unsigned)(rows < 65535 ? rows : 65535)), (unsigned)threads};
+  const long fit = 2 * (1024 / threads) * mlb_sm_count() / blocks, rows = N < fit ? N : fit > 1 ? fit : 1;
+  return {dim3((unsigned)blocks, (unsigned)rows), (unsigned)threads};
 }
 #define MLB_BY_HEAD(hd, F) \
   switch (hd) {            \
