@@ -10,6 +10,8 @@
 //   value row: 16-bit word i NG + g has the elements 32 g + 4 i + e, e = 0..3
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "tc.cuh"
 
 namespace {
@@ -29,9 +31,14 @@ __device__ __forceinline__ float hi_bf16(uint32_t w) { return __uint_as_float(w 
 
 __device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000F000Fu; }       // two codes as fp16 c 2^-24
 __device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00F000F0u; }      // c 2^-20
-__device__ __forceinline__ uint32_t value_codes(uint32_t w) {      // two codes as bf16 c - 8
-  const uint32_t x = low_codes(w) | 0x43004300u, k = 0x43084308u;      // 128 + c, 136
+__device__ __forceinline__ uint32_t less(uint32_t x, uint32_t k) {      // of two bf16 numbers
   const bf162 y = __hsub2(*reinterpret_cast<const bf162*>(&x), *reinterpret_cast<const bf162*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ uint32_t value_codes(uint32_t w) { return less(low_codes(w) | 0x43004300u, 0x43084308u); }      // two codes as bf16 c - 8: 128 + c, 136
+__device__ __forceinline__ uint32_t sixteen_times(uint32_t w) {
+  const uint32_t k = 0x41804180u;
+  const bf162 y = __hmul2(*reinterpret_cast<const bf162*>(&w), *reinterpret_cast<const bf162*>(&k));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 // ------------------------------------------------------------------ append
@@ -322,9 +329,13 @@ __global__ void __launch_bounds__(512, 3) kv4_read_k(bf16* __restrict__ k, bf16*
 //      makes two operands and only the upper byte's codes need a shift; the factor 16 is taken out of the queries, which a power of two of each row brings to fp16
 //      exactly.  The product starts from -8 sum(q) instead of subtracting 8 from each code; every group's sum is scaled by s_t behind its two
 //      products, in fp32.  (The tensor core lines products up by their operands' nominal exponents, 2^-14 for a subnormal: a score is off by some 2^-16 of |q| s.)
-//   V: the bits put into the mantissa of 128 in bf16, less 136: c - 8 by two instructions for two codes, so that what is 0 adds 0.  The scale goes into P, in
-//      fp32 before its one rounding to bf16 (which has the range for weights and scales of any size).  That rounding, 2^-8 of each weight at most and independent
-//      from token to token, is the only one on the way to O.
+//   V: the same bits as bf16 numbers are c 2^-133 and 16 c 2^-133 (these reach into the exponent's last bit, and are counted on without a gap there), less 8 and 128
+//      of which all is exact and what is 0 adds 0: two instructions for two codes, a shift for eight.  For the products' sake the weights are 2^88 times what they are
+//      (a sum of 2^31 of them, each up to 2^8, still is a number), O is 2^-45 times: what a token adds below 2^-81 is lost.  With a scale of 2^31 and more a weight
+//      may pass bf16's range.  Then O is not finite, the warp sees it and goes over its blocks once more with codes as numbers of the size that they are.
+//      The scale goes into P, in fp32 before its one rounding to bf16.  That rounding, 2^-8 of each weight at most and independent from token to token, is
+//      the only one on the way to O.  (Codes as 128 + c less 136 with the weights as they are, a shift for each two: 64 x 8192 tokens, below, 91 us instead of 79.  The
+//      8 or 128 taken off by a product with a constant was no faster, 82, and leaves 2^-24 of a weight where the code stands for 0.)
 // Scores stand transposed (token rows, query columns), so that softmax weights become the second product's operand by two matrix transpositions in
 // registers.  The largest score m is the reference of all weights so far and moves only when a score passes it by 2^8 (O and the sums are then rescaled): most
 // blocks need a vote instead of reductions over the warp.
@@ -334,7 +345,7 @@ __global__ void __launch_bounds__(512, 3) kv4_read_k(bf16* __restrict__ k, bf16*
 // took 39 us where two of them were empty, and 23 with 2 units).  A warp fetches its own blocks by bulk copies through a ring of its own.  A head whose blocks are
 // shared is put together by the thread block that comes last, in the order of the pieces, so that a call repeats its bits.
 //
-// Measured: 64 sequences of 1024 to 8192 tokens, 32 heads over 8 of 128: 92 us, 3.8 TB/s (58 % of the measured copy rate; 60 us with the arithmetic left out, so
+// Measured: 64 sequences of 1024 to 8192 tokens, 32 heads over 8 of 128: 79 us, 4.4 TB/s (67 % of the measured copy rate; 60 us with the arithmetic left out, so
 // that half of what is missing is instructions: 366 a block, of which 200 on the pipe of bitwise operations and shifts, 88 of these and of the FMA pipe's for the
 // values' codes; moving their shifts to multiplications made it 100).  16 sequences of up to 2048 tokens, 16 heads of 128: 23 us, of which 11 are that
 // arithmetic and 8 beginnings, ends and the joining of shares.  One sequence of 1000 tokens, 12 heads of 64: 6.8 us, 1.4 of them an empty kernel's, 2.6 the joining
@@ -429,8 +440,12 @@ template <int HD, int NT> struct Queries {      // of a thread block's query row
   float back[NT][8];                 // score of a column = back * product
 };
 
-// NB blocks of 16 tokens, one behind the other.  first: their first token; seen[n][c]: tokens that column c sees, asked only where MASKED.
-template <int HD, int NT, int NB, bool MASKED>
+// Weights are 2^UP times what they are, so that with the values' codes as subnormal numbers, c 2^-133 (of odd elements 16 times that), O is VALUE times what it is
+constexpr float UP = 88.f, BACK_DOWN = 3.23117426778526e-27f;      // 2^-88
+constexpr float VALUE = 2.8421709430404007e-14f, BACK_EVEN = 35184372088832.f, BACK_ODD = 2199023255552.f;      // 2^(88 - 133), its inverse, a 16th of that
+
+// NB blocks of 16 tokens, one behind the other.  first: their first token; seen[n][c]: tokens that column c sees, asked only where MASKED.  WIDE: scales of 2^31 and more
+template <int HD, int NT, int NB, bool MASKED, bool WIDE>
 __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q, const float (&c)[NT][2], const uint8_t* blk, int first,
                                        const int (&seen)[NT][2], int i, int j) {
   using L = Block<HD>;
@@ -480,7 +495,7 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
     for (int n = 0; n < NT; n++)
 #pragma unroll
       for (int k = 0; k < 4; k++) y[b][n][k] = fmaf(s[b][n][k], c[n][k & 1], r.neg[n][k & 1]), top = fmaxf(top, y[b][n][k]);
-  if (__any_sync(0xffffffffu, top > 8.f)) {
+  if (__any_sync(0xffffffffu, top > UP + 8.f)) {
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -494,7 +509,7 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
         if (x > -INFINITY) {
           const float f = ex2(r.m[n][h] - x);      // (from -inf: 0)
           r.m[n][h] = x;
-          r.neg[n][h] = -x;
+          r.neg[n][h] = UP - x;
           r.l[n][h] *= f;
 #pragma unroll
           for (int d = 0; d < HD / 16; d++) r.o[n][d][h] *= f, r.o[n][d][h + 2] *= f;
@@ -528,10 +543,18 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
       const uint32_t x0 = __byte_perm(w0[g], w1[g], 0x5410), x1 = __byte_perm(w2[g], w3[g], 0x5410);
       uint32_t a[8];
 #pragma unroll
-      for (int e = 0; e < 4; e++) a[e / 2 * 4 + e % 2] = value_codes(x0 >> 4 * e), a[e / 2 * 4 + 2 + e % 2] = value_codes(x1 >> 4 * e);
+      for (int e = 0; e < 4; e += 2) {
+        const uint32_t u = x0 >> 4 * e, v = x1 >> 4 * e;
+        if constexpr (WIDE)
+          a[2 * e] = value_codes(u), a[2 * e + 1] = sixteen_times(value_codes(u >> 4)), a[2 * e + 2] = value_codes(v), a[2 * e + 3] = sixteen_times(value_codes(v >> 4));
+        else
+          a[2 * e] = less(low_codes(u), 0x00080008u), a[2 * e + 1] = less(high_codes(u), 0x00800080u), a[2 * e + 2] = less(low_codes(v), 0x00080008u), a[2 * e + 3] = less(high_codes(v), 0x00800080u);
+      }
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        float p[4] = {y[b][n][0] * sa[g], y[b][n][1] * sa[g], y[b][n][2] * sb[g], y[b][n][3] * sb[g]};
+        float p[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[k] = (WIDE ? y[b][n][k] * BACK_DOWN * VALUE : y[b][n][k]) * (k < 2 ? sa[g] : sb[g]);
         if constexpr (MASKED) {      // (a scale that is not seen may be anything)
 #pragma unroll
           for (int k = 0; k < 4; k++)
@@ -622,10 +645,11 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
     const int u0 = (int)(s - item0), u1 = min((int)(min(e, item1) - item0), blocks);
     auto token = [&](int r) { return (int)(((float)r + 0.5f) * A.inv_g); };      // r / G (exact: r < 2^20)
     auto finish = [&](int r, int d, float m, float l, const float4& o) {         // elements 4 d ... of row r, whole
+      l *= BACK_DOWN;
       const int tok = token(row0 + r), head = (int)kv * A.G + row0 + r - tok * A.G;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (nothing seen: zeros; NaN stays)
       bf16* out = A.out + ((long)b * A.Tq + tok) * A.G * A.Hkv * HD + (long)head * HD + 4 * d;
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv * BACK_EVEN, o.y * inv * BACK_ODD), pack_bf16(o.z * inv * BACK_EVEN, o.w * inv * BACK_ODD));
       if (d == 0 && A.lse != nullptr)
         A.lse[((long)b * A.G * A.Hkv + head) * A.Tq + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
     };
@@ -640,15 +664,18 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
     // ---- this warp's blocks [w0, w1)
     const int w0 = u0 + (u1 - u0) * warp / WARPS, w1 = u0 + (u1 - u0) * (warp + 1) / WARPS;
     Rows<HD, NT> acc;
+    auto clear = [&] {
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
+      for (int n = 0; n < NT; n++) {
 #pragma unroll
-      for (int d = 0; d < HD / 16; d++)
+        for (int d = 0; d < HD / 16; d++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) acc.o[n][d][k] = 0.f;
+          for (int k = 0; k < 4; k++) acc.o[n][d][k] = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; h++) acc.m[n][h] = -INFINITY, acc.neg[n][h] = NONE, acc.l[n][h] = 0.f;
-    }
+        for (int h = 0; h < 2; h++) acc.m[n][h] = -INFINITY, acc.neg[n][h] = NONE, acc.l[n][h] = 0.f;
+      }
+    };
+    clear();
     const bool some = w0 < w1;
     const int* trow = A.table + (long)b * A.width;
     int have = 0, ids = -1;      // page numbers [have, have + 32) of the table, one a lane
@@ -673,12 +700,13 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
       else if (wanted)
         mlb_set_error(MLB_ERR_BOUNDS, 0xC1);
     };
-    if (some && !dead) {
+    auto begin = [&] {
       names(w0 >> bpl);
 #pragma unroll
       for (int k = 0; k < NST; k++)
         if (w0 + k * STEP < w1) fetch(w0 + k * STEP, k);
-    }
+    };
+    if (some && !dead) begin();
     // ---- the queries, while the first blocks are on their way: a group and tile of 8 rows a warp
 #pragma unroll 1
     for (int x = warp; x < NT * NG; x += WARPS) {
@@ -727,7 +755,8 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; n++) c[n][0] = q.back[n][2 * j], c[n][1] = q.back[n][2 * j + 1];
-    if (some && !dead) {
+    auto walk = [&](auto wide) {
+      constexpr bool WIDE = decltype(wide)::value;
       int k = 0;
 #pragma unroll 1
       for (int u = w0; u < w1; u += STEP) {
@@ -742,17 +771,33 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
         const uint8_t* blk = ring + k * Ring<HD>::BYTES;
 #pragma unroll 1
         for (int x = 0; x < STEP; x += 2) {
-          if ((oks >> x & 3) == 3 && (u + x + 2) * TOK <= all) {
-            attend<HD, NT, 2, false>(acc, q, c, blk + x * L::BYTES, (u + x) * TOK, seen, i, j);
+          if (!WIDE && (oks >> x & 3) == 3 && (u + x + 2) * TOK <= all) {
+            attend<HD, NT, 2, false, false>(acc, q, c, blk + x * L::BYTES, (u + x) * TOK, seen, i, j);
           } else {
 #pragma unroll 1
             for (int y = x; y < x + 2; y++)
-              if (oks >> y & 1) attend<HD, NT, 1, true>(acc, q, c, blk + y * L::BYTES, (u + y) * TOK, seen, i, j);
+              if (oks >> y & 1) attend<HD, NT, 1, true, WIDE>(acc, q, c, blk + y * L::BYTES, (u + y) * TOK, seen, i, j);
           }
         }
         __syncwarp();
         if (u + NST * STEP < w1) fetch(u + NST * STEP, k);
         k = k + 1 == NST ? 0 : k + 1;
+      }
+    };
+    if (some && !dead) {
+      walk(std::false_type());
+      // A scale of 2^31 or more may have made a weight infinite, and then it made all rows of the group's O infinite or NaN: once more, slower
+      float x = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int g = 0; g < NG; g++) x = fmaf(acc.o[n][2 * g][0], 0.f, fmaf(acc.o[n][2 * g][1], 0.f, x));
+      if (!dead && __any_sync(0xffffffffu, x != 0.f)) {
+        clear();
+        tc::fence_async_smem();
+        __syncwarp();
+        begin();
+        walk(std::true_type());
       }
     }
     // ---- the warps' shares put together (in the rings' memory, which nothing is on its way to)

@@ -253,6 +253,24 @@ def test_nan_and_infinity_reach_the_rows_that_see_them_and_no_others():
     close(out[:2].cpu().double().numpy().reshape(o.shape), lse[..., :2].cpu().double().numpy(), o, l, tol, ltol)
 
 
+@pytest.mark.parametrize("hd,size", [(64, 1e9), (64, 3e10), (128, 1e11), (32, 1e20), (96, 1e36), (128, 1e36), (64, 1e-10), (128, 1e-20)])
+@pytest.mark.parametrize("T,Tq,H", [(700, 1, 4), (90, 5, 8)])
+def test_attention_over_values_of_any_size(hd, size, T, Tq, H):
+    """Large ones, some tokens' among ordinary ones: weights times scales pass the range that the sums are kept in at first."""
+    torch.manual_seed(hd)
+    Hkv, page, n = 2, 32, -(-T // 32)
+    pages, table, slots = torch.zeros(n, Hkv, page // 16, 18 * hd, dtype=torch.uint8, device=dev()), torch.randperm(n), torch.arange(T)
+    qkv = torch.randn(T, 2 * Hkv * hd)
+    v = qkv[:, Hkv * hd:]
+    v *= size if size < 1 else torch.where(torch.rand(T, 1) < 0.1, size, 1.0)
+    ops.kv4_append(pages, None, qkv.bfloat16().to(dev()), (table[slots // page] * page + slots % page).int().to(dev()), None, None, None, 0, Hkv, hd)
+    q = torch.randn(Tq, H * hd).bfloat16()
+    out, lse = torch.empty(Tq, H * hd, dtype=torch.bfloat16, device=dev()), torch.empty(1, H, Tq, device=dev())
+    ops.kv4_attn(out, lse, q.to(dev()), pages, ints(table[None].tolist()), ints([T]), Tq, H, Hkv, hd)
+    o, l, tol, ltol = oracle.attention(q, pages.cpu(), table[None].numpy(), [T], Tq, H, Hkv, hd)
+    close(out.cpu().double().numpy().reshape(o.shape), lse.cpu().double().numpy(), o, l, tol, ltol)
+
+
 def test_cache_past_4_gigabytes():
     """Pages whose bytes lie past 2^32, written, read and attended to."""
     hd, page, Hkv = 128, 128, 8
