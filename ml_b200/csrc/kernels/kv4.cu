@@ -345,11 +345,11 @@ __global__ void __launch_bounds__(512, 3) kv4_read_k(bf16* __restrict__ k, bf16*
 // took 39 us where two of them were empty, and 23 with 2 units).  A warp fetches its own blocks by bulk copies through a ring of its own.  A head whose blocks are
 // shared is put together by the thread block that comes last, in the order of the pieces, so that a call repeats its bits.
 //
-// Measured: 64 sequences of 1024 to 8192 tokens, 32 heads over 8 of 128: 79 us, 4.4 TB/s (67 % of the measured copy rate; 60 us with the arithmetic left out, so
-// that half of what is missing is instructions: 366 a block, of which 200 on the pipe of bitwise operations and shifts, 88 of these and of the FMA pipe's for the
-// values' codes; moving their shifts to multiplications made it 100).  16 sequences of up to 2048 tokens, 16 heads of 128: 23 us, of which 11 are that
-// arithmetic and 8 beginnings, ends and the joining of shares.  One sequence of 1000 tokens, 12 heads of 64: 6.8 us, 1.4 of them an empty kernel's, 2.6 the joining
-// (a fence, a counter, another block's results).  12 warps an SM: 8 or 16 (with 128 registers) are 4 to 8 % slower.
+// Measured: 64 sequences of 1024 to 8192 tokens, 32 heads over 8 of 128: 79 us, 4.4 TB/s (67 % of the measured copy rate; 60 us with the arithmetic left out.  What is
+// missing is instructions, 306 a block, of which 146 go through the pipe of bitwise operations and shifts at half the rate, and that three warps an issue slot
+// leave 44 % of the slots empty).  16 sequences of up to 2048 tokens, 16 heads of 128: 20.7 us, of which some 9 are that arithmetic and 8 beginnings, ends and
+// the joining of shares.  One sequence of 1000 tokens, 12 heads of 64: 6.6 us, 1.4 of them an empty kernel's, 2.4 the joining (a counter, another block's
+// results).  12 warps an SM: 8 are 4 to 8 % slower, 16 (of 128 registers, with places of 32 tokens) 79 -> 85.
 struct AttnArgs {
   bf16* out;
   float* lse;
