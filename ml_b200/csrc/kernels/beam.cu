@@ -298,17 +298,19 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
         __syncwarp();
       }
       __syncthreads();
+      // Too few logits for all threads go to all parts alike (to neighbours 32 eights apart, which only so few can afford: they meet in the same banks)
+      const int mine = count < SEL_THREADS * 8 ? 8 * ((lane & 7) * 32 + warp * 4 + (lane >> 3)) : 8 * tid;
       float top = -INFINITY;
       Eight<T> x;
 #pragma unroll 2
-      for (int e = tid * 8; e < count; e += SEL_THREADS * 8) top = fmaxf(top, x.load(data + e));
+      for (int e = mine; e < count; e += SEL_THREADS * 8) top = fmaxf(top, x.load(data + e));
       const float kth = kth_of_parts(top, K, tops, [](float a, float b) { return fmaxf(a, b); });
       if (c == 0) bound = kth;
       top = warp_max(tops[lane % parts_for(K)]);
       if (top > m) s *= ex2((m - top) * 1.44269504088896f), m = top;      // (from -inf: 0 times 0)
       const float mm = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
-      for (int e = tid * 8; e < count; e += SEL_THREADS * 8) {
+      for (int e = mine; e < count; e += SEL_THREADS * 8) {
         const float best = x.load(data + e);
 #pragma unroll
         for (int k = 0; k < 8; k++) s += ex2((x.get(k) - mm) * 1.44269504088896f);
