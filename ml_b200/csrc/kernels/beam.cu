@@ -10,8 +10,8 @@ MLB_DEFINE_ERROR_WORD(beam)
 // Request r holds lens[r] tokens and gets news[r] more.  It needs ceil((lens + news) / page) - ceil(lens / page) pages, which it gets from the top of the free
 // stack if the needs of the requests up to it do not pass what lies there.  Every thread block adds up all requests for itself (12 bytes each: cheaper than
 // another launch or a wait for one block that does it) and then writes its share of the slots; the thread that has a page's first token writes the page into
-// the table.  What may be an input too (new_lens, left) is written by the block that comes last.  Bound by latency: 64 requests of one token 3.0 us, 300 requests
-// of 154 thousand tokens 5.9 (of 0.2 for their bytes).
+// the table.  What may be an input too (new_lens, left) is written by the block that comes last.  Bound by latency: 64 requests of one token 2.9 us, 300 requests
+// of 154 thousand tokens 6.3 (of 0.2 for their bytes).
 constexpr int TAB_THREADS = 256, TAB_MAX_B = 4096, TAB_MAX_ROWS = 1 << 22;
 struct TableArgs {
   int *table, *slots, *pos, *starts, *new_lens, *left, *ticket;
@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
 // is the bound from then on.  A candidate's place is the number of those before it.  More candidates at a time than there is room for (logits all alike) are forgotten:
 // then K rounds over the piece find its K largest.  The request's last thread block finds its K best among the pieces' lists in the same way,
 // the bound being of its threads' best.
-// 32 x 8 beams of 50304 bf16 logits, a quarter of them ended: 14.9 us (1.7 TB/s), of which fetching and the maximum 6.2, the exponentials 1, candidates and their
-// bound 2.6, the counters 1.7, the merge 3.  1 x 4 beams: 6.8 us (2.3, then 1 for the counters, 3 for the merge): latencies one behind the other.
+// 32 x 8 beams of 50304 bf16 logits, a quarter of them ended: 15.1 us (1.7 TB/s), of which fetching and the maximum 6.2, the exponentials 1, candidates and their
+// bound 2.6, the counters 1.9, the merge 3.  1 x 4 beams: 6.8 us (2.3, then 1 for the counters, 3 for the merge): latencies one behind the other.
 constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_BYTES = 32768, SEL_MAX_K = 32, SEL_CAND = 512, SEL_HELD = 1024;
 constexpr int SEL_PER_SM = 6, SEL_LEAST = 4096;      // thread blocks that an SM holds; the smallest piece
 typedef unsigned long long u64;
@@ -477,7 +477,7 @@ cudaError_t launch_select(const SelectArgs& a, int rows, cudaStream_t st) {
 // Row b K + k continues row b K + parents[b, k].  Full pages are shared: their numbers are copied from the parent's table.  The page that is being filled belongs to one
 // row alone, so a row that continues another one gets that one's tokens copied to its spare page, and the page it had is its spare from then on: nothing
 // that is read is written, whatever the order of the rows.  Bound by the copied bytes: 128 beams of 12 layers of 12 heads of 64, 52 tokens of a page each for 44 % of
-// them, 15.1 us (74 MB moved, 4.9 TB/s); 4 beams 3.0 us.
+// them, 15.3 us (74 MB moved, 4.8 TB/s); 4 beams 3.1 us.
 struct OrderArgs {
   uint8_t* pages;
   int *table_out, *spare_out, *hist_out;
