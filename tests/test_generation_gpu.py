@@ -253,6 +253,12 @@ def test_nan_and_infinity_reach_the_rows_that_see_them_and_no_others():
     close(out[:2].cpu().double().numpy().reshape(o.shape), lse[..., :2].cpu().double().numpy(), o, l, tol, ltol)
 
 
+@pytest.mark.parametrize("lens,Tq,H,Hkv,hd,page", [([1000], 950, 8, 1, 32, 64), ([130, 0, 90], 120, 6, 2, 96, 16), ([300, 41], 40, 16, 2, 128, 32), ([200], 200, 3, 3, 64, 128)])
+def test_attention_of_more_row_tiles_than_there_are_multiprocessors(lens, Tq, H, Hkv, hd, page):
+    """Prompts' worth of new tokens: few thread blocks for each tile of rows, down to one."""
+    close(*attend(lens, Tq, H, Hkv, hd, page, seed=7))
+
+
 @pytest.mark.parametrize("hd,size", [(64, 1e9), (64, 3e10), (128, 1e11), (32, 1e20), (96, 1e36), (128, 1e36), (64, 1e-10), (128, 1e-20)])
 @pytest.mark.parametrize("T,Tq,H", [(700, 1, 4), (90, 5, 8)])
 def test_attention_over_values_of_any_size(hd, size, T, Tq, H):
