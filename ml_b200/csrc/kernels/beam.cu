@@ -11,7 +11,7 @@ MLB_DEFINE_ERROR_WORD(beam)
 // stack if the needs of the requests up to it do not pass what lies there.  Every thread block adds up all requests for itself (12 bytes each: cheaper than
 // another launch or a wait for one block that does it) and then writes its share of the slots; the thread that has a page's first token writes the page into
 // the table.  What may be an input too (new_lens, left) is written by the block that comes last.  Bound by latency: 64 requests of one token 2.9 us, 300 requests
-// of 154 thousand tokens 6.3 (of 0.2 for their bytes).
+// of 154 thousand tokens 5.7 (of 0.2 for their bytes; 6.3 with sums over 256 requests at a time).
 constexpr int TAB_THREADS = 256, TAB_MAX_B = 4096, TAB_MAX_ROWS = 1 << 22;
 struct TableArgs {
   int *table, *slots, *pos, *starts, *new_lens, *left, *ticket;
@@ -49,34 +49,35 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
     if (tid == 0 && blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xB1);
     n_free = max(0, min(n_free, A.stack_size));
   }
-  Two done = {0, 0};
-  int taken = 0;
-  for (int r0 = 0; r0 < A.B; r0 += TAB_THREADS) {
-    const int r = r0 + tid;
-    int len = 0, add = 0, need = 0;
-    bool fits = false;
-    if (r < A.B) {
-      len = A.lens[r], add = A.news[r];
-      if (len < 0 || add < 0 || add > A.rows) {
-        if (blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xB1);
-        add = 0;
-      } else if ((long)len + add <= (long)A.width * A.page) {
-        fits = true;
-        need = ((unsigned)len + add + A.page - 1) / A.page - ((unsigned)len + A.page - 1) / A.page;
-      }
+  // a thread has `per` requests, one behind the other: their needs (-1: too long for the table's row) and new tokens, then the sums over those before
+  const int per = (A.B + TAB_THREADS - 1) / TAB_THREADS, r0 = tid * per, r1 = min(r0 + per, A.B);
+  Two own = {0, 0}, done;
+#pragma unroll 1
+  for (int r = r0; r < r1; r++) {
+    const int len = A.lens[r];
+    int add = A.news[r], need = -1;
+    if (len < 0 || add < 0 || add > A.rows) {
+      if (blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xB1);
+      add = 0;
+    } else if ((long)len + add <= (long)A.width * A.page) {
+      need = ((unsigned)len + add + A.page - 1) / A.page - ((unsigned)len + A.page - 1) / A.page;
     }
-    Two total;
-    const Two upto = block_scan({need, add}, warps, total);
-    if (r < A.B) {
-      const int pages = done.a + upto.a, rows = done.b + upto.b;
-      if (rows > A.rows && blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xB2);
-      const bool got = fits && pages <= n_free && rows <= A.rows;
-      start[r] = rows - add;
-      first[r] = got ? pages - need : -1;
-      if (got) taken = max(taken, pages);
-    }
-    done.a += total.a, done.b = min(done.b + total.b, A.rows + 1);      // (past the last place nothing fits any more: no sum overflows)
+    start[r] = add, first[r] = need;
+    own.a += max(need, 0), own.b = min(own.b + add, A.rows + 1);      // (past the last place nothing fits any more: no sum overflows)
   }
+  const Two upto = block_scan(own, warps, done);
+  int pages = upto.a - own.a, rows = upto.b - own.b, taken = 0;
+#pragma unroll 1
+  for (int r = r0; r < r1; r++) {
+    const int add = start[r], need = first[r];
+    start[r] = rows;
+    pages += max(need, 0), rows = min(rows + add, A.rows + 1);
+    const bool got = need >= 0 && pages <= n_free && rows <= A.rows;
+    first[r] = got ? pages - need : -1;
+    if (got) taken = max(taken, pages);
+    if (rows > A.rows && blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xB2);
+  }
+  done.b = min(done.b, A.rows + 1);
   if (tid == 0) start[A.B] = done.b;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) taken = max(taken, __shfl_xor_sync(0xffffffffu, taken, o));
