@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
 // is the bound from then on.  A candidate's place is the number of those before it.  More candidates at a time than there is room for (logits all alike) are forgotten:
 // then K rounds over the piece find its K largest.  The request's last thread block finds its K best among the pieces' lists in the same way,
 // the bound being of its threads' best.
-// 32 x 8 beams of 50304 bf16 logits, a quarter of them ended: 15.1 us (1.7 TB/s), of which fetching and the maximum 6.2, the exponentials 1, candidates and their
+// 32 x 8 beams of 50304 bf16 logits, a quarter of them ended: 15.2 us (1.7 TB/s), of which fetching and the maximum 6.2, the exponentials 1, candidates and their
 // bound 2.6, the counters 1.9, the merge 3.  1 x 4 beams: 6.8 us (2.3, then 1 for the counters, 3 for the merge): latencies one behind the other.
 constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_BYTES = 32768, SEL_MAX_K = 32, SEL_CAND = 512, SEL_HELD = 1024;
 constexpr int SEL_PER_SM = 6, SEL_LEAST = 4096;      // thread blocks that an SM holds; the smallest piece
@@ -409,13 +409,17 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
     if (lane == 0) lse[k] = s > 0.f ? m + log_of(s) : -INFINITY;
   }
   __syncthreads();
-  // the lists' entries, their first ones before their second ones: loops kept short, since each runs once or twice
+  // The lists' entries.  Of up to 4 beams the lists' first ones go before their second ones: many lists, so that every part has some of each beam.  Of more beams
+  // a list's entries go to as many parts of the thread block as there are, so that the parts' best are a bound also where one beam has all of the K best (8 x 32
+  // beams of 50304 logits 33 us, the other way 67; 8 x 8 beams 13.4, 14.5; 1 x 4 beams 7.1, 6.8).  Loops kept short, since each runs once or twice.
+  const bool few = K <= 4;
+  const int mine = few ? tid : warp + 8 * (lane >> 4) + 16 * (lane >> 3 & 1) + 32 * (lane & 7), inner = few ? lists : L;
   u64* keys = reinterpret_cast<u64*>(fetched);
   u64 best = 0;
-  const float per_list = 1.f / lists, per_beam = 1.f / A.pieces;      // ((x + 1/2) / n rounded down is exact for the few thousands that these are)
+  const float per_inner = 1.f / inner, per_beam = 1.f / A.pieces;      // ((x + 1/2) / n rounded down is exact for the few thousands that these are)
 #pragma unroll 1
-  for (int e = tid; e < lists * L; e += SEL_THREADS) {
-    const int nth = (int)((e + 0.5f) * per_list), l = e - nth * lists, k = (int)((l + 0.5f) * per_beam);
+  for (int e = mine; e < lists * L; e += SEL_THREADS) {
+    const int outer = (int)((e + 0.5f) * per_inner), rest = e - outer * inner, l = few ? rest : outer, nth = few ? outer : rest, k = (int)((l + 0.5f) * per_beam);
     const long a = ((long)req * lists + l) * L + nth;
     int t = __ldcg(A.ids + a);
     float x = __ldcg(A.values + a);
