@@ -569,7 +569,7 @@ MLB_API int mlb_beam_select(float* scores, int* tokens, int* parents, int* done_
 MLB_API int mlb_beam_reorder(uint8_t* pages, int* table_out, int* spare_out, int* hist_out, const int* table, const int* spare, const int* lens, const int* hist,
                              const int* parents, const int* tokens, int layers, long n_pages, int Hkv, int page, int block_bytes, int B, int K, int width, int T,
                              cudaStream_t st) {
-  if (page < 16 || page % 16 != 0 || block_bytes % 16 != 0 || K < 1 || width < 1 || layers > 65534 || (long)width * page >= 1L << 31) return -7;
+  if (page < 16 || page % 16 != 0 || block_bytes % 16 != 0 || ((uintptr_t)pages & 15) != 0 || K < 1 || width < 1 || layers > 65534 || (long)width * page >= 1L << 31) return -7;
   // a part is 1024 words (16 KB) of a page or more
   const long words = (long)Hkv * (page / 16) * (block_bytes / 16), most = layers > 0 ? 65534 / layers : 1;
   if (words >= 1L << 28) return -7;

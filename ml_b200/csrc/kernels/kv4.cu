@@ -970,6 +970,8 @@ Shape rows_shape(long per_row, long N) {
   const long fit = 2 * (1024 / threads) * mlb_sm_count() / blocks, rows = N < fit ? N : fit > 1 ? fit : 1;
   return {dim3((unsigned)blocks, (unsigned)rows), (unsigned)threads};
 }
+// Rows, tables and workspaces are read and written 16 bytes at a time (null: none)
+template <typename... P> bool on_16_bytes(P... p) { return ((... | (uintptr_t)p) & 15) == 0; }
 #define MLB_BY_HEAD(hd, F) \
   switch (hd) {            \
     case 32: F(32); break; \
@@ -984,7 +986,7 @@ Shape rows_shape(long per_row, long N) {
 // values to the slots of the pool; a negative slot is none.  Returns -7 for what the kernel does not take.
 MLB_API int mlb_kv4_append(uint8_t* pages, void* q_out, const void* qkv, const int* slots, const int* pos, const float* cos, const float* sin, long n_pages,
                            int page, long N, long stride, int H, int Hkv, int hd, int T, cudaStream_t st) {
-  if (!known_head(hd) || page_shift(page) < 0 || stride % 8 != 0 || H < 0 || Hkv < 1) return -7;
+  if (!known_head(hd) || page_shift(page) < 0 || stride % 8 != 0 || H < 0 || Hkv < 1 || !on_16_bytes(pages, q_out, qkv, cos, sin)) return -7;
   const bool halves = hd % 64 == 0;
   const Shape z = rows_shape((long)(H + 2 * Hkv) * (hd / (halves ? 16 : 8)), N);
   if (z.threads == 0) return -7;
@@ -1001,7 +1003,7 @@ MLB_API int mlb_kv4_append(uint8_t* pages, void* q_out, const void* qkv, const i
 
 // k, v[N, Hkv, hd]: what the slots hold; zeros for a negative slot
 MLB_API int mlb_kv4_read(void* k, void* v, const uint8_t* pages, const int* slots, long n_pages, int page, long N, int Hkv, int hd, cudaStream_t st) {
-  if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1) return -7;
+  if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1 || !on_16_bytes(k, v, pages)) return -7;
   const Shape z = rows_shape((long)Hkv * (hd / 8), N);
   if (z.threads == 0) return -7;
   cudaError_t e = cudaSuccess;
@@ -1022,7 +1024,7 @@ MLB_API long mlb_kv4_attn_scratch(int B, int Tq, int H, int Hkv, int hd, int wid
 MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pages, const int* table, const int* lens, float* part, int* count, long n_pages,
                          long q_stride, int B, int Tq, int H, int Hkv, int hd, int width, int page, float scale, cudaStream_t st) {
   const int shift = page_shift(page);
-  if (!known_head(hd) || shift < 0 || Hkv < 1 || H % Hkv != 0 || q_stride % 8 != 0) return -7;
+  if (!known_head(hd) || shift < 0 || Hkv < 1 || H % Hkv != 0 || q_stride % 8 != 0 || !on_16_bytes(out, q, pages, part)) return -7;
   int nt;
   const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
   if (tiles > 65535 || (long)n_pages > 0x7FFFFFFFL || (long)width * page >= 1L << 31 || (long)Hkv * page * hd * 9 / 8 >= 1L << 32 || ((long)width * page / TOK + PAD) * (B < MAX_B ? B : MAX_B) * Hkv >= 1L << 31) return -7;

@@ -21,6 +21,13 @@ def _rows(t, what):
     return Address(t.data_ptr())
 
 
+def _on_16_bytes(**tensors):
+    """Other tensors that a kernel reads or writes 16 bytes at a time."""
+    for what, t in tensors.items():
+        if t is not None and t.data_ptr() % 16:
+            raise ValueError(f"{what}: need memory that begins on a 16-byte boundary")
+
+
 def _pool(pages):
     if not pages.is_cuda or not pages.is_contiguous() or pages.data_ptr() % 16:
         raise ValueError("pages: need contiguous CUDA memory on a 16-byte boundary")
@@ -29,7 +36,7 @@ def _pool(pages):
 
 def _took(rc, name):
     if rc == -7:
-        raise ValueError(f"{name}: sizes past what the kernel counts in 32 bits")
+        raise ValueError(f"{name}: sizes past what the kernel counts in 32 bits, or memory off a 16-byte boundary")
     _n._chk(rc, name)
 
 
@@ -52,6 +59,7 @@ def kv4_append(pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd):
     if _plain('kv4_append', pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd):
         return
     n, page, N = check_append(pages, q_out, qkv, slots, pos, cos, sin, H, Hkv, hd)
+    _on_16_bytes(q_out=q_out, cos=cos, sin=sin)
     _here(pages, q_out, qkv, slots, pos, cos, sin)
     if N == 0:
         return
@@ -64,6 +72,7 @@ def kv4_read(k, v, pages, slots):
     if _plain('kv4_read', k, v, pages, slots):
         return
     n, Hkv, page, hd, N = check_read(k, v, pages, slots)
+    _on_16_bytes(k=k, v=v)
     _here(k, v, pages, slots)
     if N:
         _took(_n._entries().mlb_kv4_read(k, v, _pool(pages), slots, n, page, N, Hkv, hd), "kv4_read")
@@ -73,6 +82,7 @@ def kv4_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale=None):
     if _plain('kv4_attn', out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale):
         return
     n, page, B = check_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale)
+    _on_16_bytes(out=out)
     _here(out, lse, q, pages, table, lens)
     if B == 0:
         return

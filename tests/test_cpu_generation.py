@@ -132,6 +132,43 @@ def test_generation_entry_points_have_one_signature():
         assert all(d == k or (d == "p" and k in "bfiu") for d, k in zip(defined["mlb_" + name], kinds)), name
 
 
+def test_entries_refuse_addresses_off_16_bytes():
+    """The kernels read and write 16 bytes at a time: -7, before anything is launched (without a device a launch answers with another code)."""
+    from ml_b200.ops import native
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are nobody's memory: asked only where no kernel can run")
+    L, ok, off = native.lib(), 1 << 20, (1 << 20) + 2
+    append = lambda **kw: L.mlb_kv4_append(*{**dict(pages=ok, q=ok, qkv=ok, slots=ok, pos=ok, cos=ok, sin=ok), **kw}.values(), 4, 16, 3, 512, 4, 2, 64, 9, None)
+    read = lambda **kw: L.mlb_kv4_read(*{**dict(k=ok, v=ok, pages=ok, slots=ok), **kw}.values(), 4, 16, 3, 2, 64, None)
+    attn = lambda **kw: L.mlb_kv4_attn(*{**dict(out=ok, lse=None, q=ok, pages=ok, table=ok, lens=ok, part=ok, count=ok), **kw}.values(), 4, 256, 1, 1, 4, 2, 64, 1, 16, 0.125, None)
+    order = lambda **kw: L.mlb_beam_reorder(*{**dict(pages=ok), **kw}.values(), *[ok] * 9, 1, 4, 2, 16, 18 * 64, 1, 2, 2, 9, None)
+    for call, names in ((append, ("pages", "q", "qkv", "cos", "sin")), (read, ("k", "v", "pages")), (attn, ("out", "q", "pages", "part")), (order, ("pages",))):
+        assert call() > 0      # (no device)
+        for name in names:
+            assert call(**{name: off}) == -7, name
+
+
+def test_tensors_off_16_bytes_are_refused_by_name():
+    """Views that begin in the middle of a buffer, before anything else is asked of them."""
+    from ml_b200.ops import native_gen
+    bf, hd = torch.bfloat16, 64
+    whole = lambda *s, dtype=bf: torch.zeros(*s, dtype=dtype)
+    off = lambda t: torch.zeros(t.numel() + 1, dtype=t.dtype)[1:].view(t.shape)
+    pages, x, slots, pos = whole(4, 2, 1, 18 * hd, dtype=torch.uint8), whole(3, 8 * hd), ints([0, 1, 2]), ints([0, 1, 2])
+    a = dict(pages=pages, q_out=whole(3, 4 * hd), qkv=x, slots=slots, pos=pos, cos=whole(9, hd // 2, dtype=torch.float32), sin=whole(9, hd // 2, dtype=torch.float32))
+    r = dict(k=whole(3, 2 * hd), v=whole(3, 2 * hd), pages=pages, slots=slots)
+    t = dict(out=whole(1, 4 * hd), lse=None, q=whole(1, 4 * hd), pages=pages, table=ints([[0]]), lens=ints([1]))
+    calls = ((lambda **kw: native_gen.kv4_append(**{**a, **kw}, H=4, Hkv=2, hd=hd), a, ("q_out", "cos", "sin")),
+             (lambda **kw: native_gen.kv4_read(**{**r, **kw}), r, ("k", "v")),
+             (lambda **kw: native_gen.kv4_attn(**{**t, **kw}, Tq=1, H=4, Hkv=2, hd=hd), t, ("out",)))
+    for call, args, names in calls:
+        for name in names:
+            view = off(args[name])
+            assert view.is_contiguous() and view.data_ptr() % 16
+            with pytest.raises(ValueError, match=rf"\b{name}\b.*16-byte"):
+                call(**{name: view})
+
+
 # ------------------------------------------------------------------ the whole path
 def small(V=50, T=80, hd=32, H=2, L=2):
     g = GPT(Config(V=V, C=H * hd, L=L, H=H, I=48, T=T), 2, "cpu")

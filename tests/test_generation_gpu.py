@@ -606,6 +606,32 @@ def test_refusals():
             pytest.fail(f"call {k} was taken")
 
 
+@pytest.mark.parametrize("module", [True, False])
+def test_views_that_begin_off_16_bytes_are_refused(monkeypatch, module):
+    """Contiguous ones too, by the argument's name, on both ways into the library; nothing is launched."""
+    n, bf, hd = nat(), torch.bfloat16, 64
+    if not module:
+        monkeypatch.setattr(n, "_E", n._Ctypes())
+    new = lambda *s, dtype=bf: torch.zeros(*s, dtype=dtype, device=dev())
+    off = lambda t: torch.zeros(t.numel() + 1, dtype=t.dtype, device=dev())[1:].view(t.shape)
+    pages, s = new(4, 2, 1, 18 * hd, dtype=torch.uint8), ints([0, 1, 2])
+    q, x, a, k, o = new(3, 4 * hd), new(3, 8 * hd), new(9, hd // 2, dtype=torch.float32), new(3, 2 * hd), new(1, 4 * hd)
+    calls = {
+        "q_out": lambda: ops.kv4_append(pages, off(q), x, s, None, None, None, 4, 2, hd),
+        "qkv": lambda: ops.kv4_append(pages, q, off(x), s, None, None, None, 4, 2, hd),
+        "cos": lambda: ops.kv4_append(pages, q, x, s, s, off(a), a, 4, 2, hd),
+        "sin": lambda: ops.kv4_append(pages, q, x, s, s, a, off(a), 4, 2, hd),
+        "k": lambda: ops.kv4_read(off(k), k, pages, s),
+        "v": lambda: ops.kv4_read(k, off(k), pages, s),
+        "pages": lambda: ops.kv4_read(k, k, off(pages), s),
+        "out": lambda: ops.kv4_attn(off(o), None, o, pages, ints([[0]]), ints([1]), 1, 4, 2, hd),
+        "q": lambda: ops.kv4_attn(o, None, off(o), pages, ints([[0]]), ints([1]), 1, 4, 2, hd),
+    }
+    for name, call in calls.items():
+        with pytest.raises(ValueError, match=rf"\b{name}\b.*16-byte"):
+            call()
+
+
 def test_generation_entry_points_through_ctypes_and_through_the_module(monkeypatch):
     """The same bits through the extension module and through ctypes."""
     n, seen = nat(), set()
