@@ -146,6 +146,8 @@ def beam_search(gpt, prompt, n_new, beams, eos=-1, page=64, length_penalty=0.0):
     lead = torch.arange(rows, device=dev) % beams == 0
     k.lens = torch.where(lead, 0, P // page * page).int()
     slots, _, starts = k.grow(torch.where(lead, P, P % page).int(), b * P + (rows - b) * (P % page))
+    table = k.table.view(b, beams, -1)
+    table[:, 1:, :P // page] = table[:, :1, :P // page].clone()      # (a beam that the first choice leaves without a continuation reads them too)
     at = starts[:-1].view(b, beams)[:, :1] + torch.arange(P, **i32)
     logits = m.prompt(ids, slots[at.long()].view(-1).contiguous())
     logits = logits.repeat_interleave(beams, 0)

@@ -238,6 +238,30 @@ def test_beam_search_on_cpu(page, P):
     assert torch.equal(g.generate(prompt, n, kv="4bit", beams=K, page=page), hist[:, 0])
 
 
+@pytest.mark.parametrize("V,K", [(3, 4), (4, 4), (8, 4), (2, 9)])
+@pytest.mark.parametrize("P", [5, 16, 20, 48])
+def test_beam_search_with_more_beams_than_continuations(V, K, P):
+    """A first step that has fewer continuations than beams leaves rows on beams that are none: those hold the prompt as well, shorter than a page, as long as one
+    and longer.  What is kept in the end are the best continuations; enough beams keep them all."""
+    g = small(V=V)
+    torch.manual_seed(V + P)
+    prompt = torch.randint(0, V, (2, P))
+    n = 3
+    hist, scores = generation.beam_search(g, prompt, n, K, page=16)
+    assert hist.shape == (2, K, P + n) and torch.equal(hist[:, :, :P], prompt[:, None].expand(2, K, P)) and not torch.isnan(scores).any()
+    live = torch.isfinite(scores)
+    assert live.sum(1).tolist() == [min(K, V ** n)] * 2
+    m = generation.CachedDecoder(g, 2 * K, P + n, 32)
+    rows = hist.view(2 * K, -1)
+    slots, _, _ = m.cache.grow(torch.full((2 * K,), P, dtype=I32), 2 * K * P)
+    logits, total = m.prompt(rows[:, :P].int().contiguous(), slots), torch.zeros(2 * K)
+    for t in range(P, P + n):
+        total += torch.log_softmax(logits, -1).gather(1, rows[:, t:t + 1]).view(-1)
+        if t + 1 < P + n:
+            logits = m.step(rows[:, t].int().contiguous())
+    assert torch.allclose(scores.view(-1)[live.view(-1)], total[live.view(-1)], atol=1e-3)
+
+
 def test_generate_refuses_what_the_cache_has_not():
     g = small()
     p = torch.zeros(1, 10, dtype=torch.long)

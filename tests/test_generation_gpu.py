@@ -724,6 +724,20 @@ def test_beam_search_scores_are_those_of_its_tokens(page, P):
     assert torch.equal(top, hist[:, 0])
 
 
+@pytest.mark.parametrize("V,K,P,page", [(3, 4, 20, 16), (3, 4, 16, 16), (8, 4, 48, 16), (2, 9, 70, 32), (3, 4, 5, 16)])
+def test_beam_search_with_more_beams_than_continuations(V, K, P, page):
+    """Rows on beams that are none hold the prompt too; the kernels find no page outside the pool (asked after every test)."""
+    from ml_b200 import Config
+    from ml_b200.models import GPT, generation
+    g = GPT(Config(V=V, C=128, L=2, H=2, I=192, T=160), 2, "cuda:0")
+    g.init_weights(7)
+    torch.manual_seed(V + P)
+    prompt, n = torch.randint(0, V, (2, P)), 4
+    hist, scores = generation.beam_search(g, prompt, n, K, page=page)
+    assert torch.equal(hist[:, :, :P].cpu(), prompt[:, None].expand(2, K, P)) and torch.isfinite(scores).all()
+    assert all(len({tuple(r) for r in h}) == K for h in hist.tolist())
+
+
 def test_beams_end():
     from ml_b200.models import generation
     g = small()
