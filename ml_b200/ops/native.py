@@ -221,12 +221,20 @@ def describe_error(err: int) -> str:
     return f"{text}, detail {detail:#x}"
 
 
+def error_words(pinned=True) -> torch.Tensor:
+    """Host memory for read_errors_async: int32, one word of each source of kernels."""
+    w = torch.zeros(len(_ERROR_WORDS), dtype=torch.int32)
+    return w.pin_memory() if pinned else w
+
+
 def read_errors_async(host_words: torch.Tensor):
-    """The four error words copied into `host_words` (pinned int32[4]) behind the current stream's work, without a
+    """The error words copied into `host_words` (error_words()) behind the current stream's work, without a
     synchronisation of their own: a caller that synchronises the stream anyway (to read a loss) checks them for free."""
+    if host_words.numel() != len(_ERROR_WORDS) or host_words.dtype != torch.int32:
+        raise ValueError(f"host_words: need int32[{len(_ERROR_WORDS)}]")
     L = lib()
     base = host_words.data_ptr()
-    for i, tag in enumerate(("gemm", "attn", "elementwise", "comm")):
+    for i, tag in enumerate(_ERROR_WORDS):
         fn = getattr(L, "mlb_read_error_async_" + tag)
         fn.argtypes = [_vp, _vp]
         fn.restype = _i32

@@ -252,7 +252,7 @@ class Trainer:
             # the kernels' error words ride behind the loss: one synchronisation for both
             from .ops import native
             if self.h_err is None:
-                self.h_err = torch.zeros(4, dtype=torch.int32).pin_memory()
+                self.h_err = native.error_words()
             native.read_errors_async(self.h_err)
             torch.cuda.current_stream().synchronize()
             if bool(self.h_err.any()):

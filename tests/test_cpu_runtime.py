@@ -632,3 +632,34 @@ def test_entry_points_refuse_numbers_for_tensors():
                 entries.mlb_swiglu_fwd(*args)
     with pytest.raises(AssertionError):
         native.bridge().mlb_swiglu_fwd(torch.zeros(16, 8, dtype=torch.bfloat16), native.NONE, 16, 8)      # (of the host)
+
+
+def test_a_step_copies_the_error_words_of_all_sources_of_kernels(monkeypatch):
+    """Every word that get_error() asks for, each to a place of its own."""
+    from ml_b200 import build
+    from ml_b200.ops import native
+    import re
+    asked = {}
+
+    class Read:
+        def __init__(self, tag):
+            self.tag = tag
+
+        def __call__(self, at, stream):
+            asked[self.tag] = at
+            return 0
+
+    class Lib:
+        def __getattr__(self, name):
+            assert name.startswith("mlb_read_error_async_")
+            return Read(name.rsplit("_", 1)[1])
+
+    defined = {t for src in (build.CSRC / "kernels").glob("*.cu") for t in re.findall(r"^MLB_DEFINE_ERROR_WORD\((\w+)\)", src.read_text(), re.M)}
+    monkeypatch.setattr(native, "lib", Lib)
+    monkeypatch.setattr(native, "_st", lambda: 0)
+    words = native.error_words(pinned=False)
+    native.read_errors_async(words)
+    assert set(asked) == defined == set(native._ERROR_WORDS)
+    assert sorted(asked.values()) == [words.data_ptr() + 4 * i for i in range(words.numel())]
+    with pytest.raises(ValueError):
+        native.read_errors_async(words[:-1])
