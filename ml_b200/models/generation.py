@@ -4,7 +4,7 @@
 through the training kernels (attention over its unrounded keys and values) and leaves its keys and values in the cache; after it every step reads the
 cache: slots for the new tokens (`ops.block_tables`), keys and values into them (`ops.kv4_append`), attention over what is there (`ops.kv4_attn`), and with beams
 the choice of continuations (`ops.beam_select`) and their state in the order of their parents (`ops.beam_reorder`).  Nothing is read back by the
-host before the end, except to sample.
+host before the end, except to sample; there the kernels' error words are (`CachedDecoder.check`).
 """
 from __future__ import annotations
 
@@ -115,6 +115,12 @@ class CachedDecoder:
 
         return self._layers(ids, attention)
 
+    def check(self):
+        """Waits for the steps so far, and raises what their kernels have reported (CPU tensors raise where they stand)."""
+        if self.dev.type == "cuda":
+            torch.cuda.current_stream(self.dev).synchronize()
+            ops.native_module().raise_error("generation")
+
 
 @torch.no_grad()
 def sample(gpt, prompt, n_new, choose, page=64):
@@ -129,6 +135,7 @@ def sample(gpt, prompt, n_new, choose, page=64):
         out = torch.cat([out, nxt.view(b, 1)], dim=1)
         if k + 1 < n_new:
             logits = m.step(nxt.int())
+    m.check()
     return out
 
 
@@ -162,6 +169,7 @@ def beam_search(gpt, prompt, n_new, beams, eos=-1, page=64, length_penalty=0.0):
         hist = k.reorder(hist, parents, tokens, copy=more)
         if more:
             logits = m.step(tokens.view(-1))
+    m.check()
     hist = hist.view(b, beams, -1)
     if length_penalty:
         new = hist[:, :, P:]

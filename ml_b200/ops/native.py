@@ -248,6 +248,14 @@ def clear_error():
             getattr(L, "mlb_clear_error_" + tag)()
 
 
+def raise_error(what: str):
+    """Raises what a kernel has reported, if any has, and clears it.  For callers behind a synchronisation of the streams that they used."""
+    err = get_error()
+    if err:
+        clear_error()
+        raise RuntimeError(f"{what}: kernel error word {err:#x} ({describe_error(err)}); results since the last check are invalid")
+
+
 def _b(t, name="tensor"):
     assert t.is_cuda and t.dtype == torch.bfloat16 and t.is_contiguous(), f"{name}: need contiguous CUDA bf16"
     return t.data_ptr()

@@ -262,6 +262,27 @@ def test_beam_search_with_more_beams_than_continuations(V, K, P):
     assert torch.allclose(scores.view(-1)[live.view(-1)], total[live.view(-1)], atol=1e-3)
 
 
+@pytest.mark.parametrize("beams", [1, 3])
+def test_generation_asks_for_the_kernels_errors_once_at_its_end(monkeypatch, beams):
+    asked = []
+    monkeypatch.setattr(generation.CachedDecoder, "check", lambda self: asked.append(len(steps)), raising=False)
+    steps, step = [], generation.CachedDecoder.step
+    monkeypatch.setattr(generation.CachedDecoder, "step", lambda self, ids: steps.append(1) or step(self, ids))
+    g = small()
+    g.generate(torch.zeros(1, 10, dtype=torch.long), 4, kv="4bit", beams=beams)
+    assert asked == [3]
+
+
+def test_an_error_word_is_raised_in_words_and_cleared(monkeypatch):
+    from ml_b200.ops import native
+    words = [3 << 24 | 0xC1]
+    monkeypatch.setattr(native, "get_error", lambda: words[0])
+    monkeypatch.setattr(native, "clear_error", lambda: words.__setitem__(0, 0))
+    with pytest.raises(RuntimeError, match="page outside the pool"):
+        native.raise_error("generation")
+    native.raise_error("generation")
+
+
 def test_generate_refuses_what_the_cache_has_not():
     g = small()
     p = torch.zeros(1, 10, dtype=torch.long)

@@ -738,6 +738,34 @@ def test_beam_search_with_more_beams_than_continuations(V, K, P, page):
     assert all(len({tuple(r) for r in h}) == K for h in hist.tolist())
 
 
+@pytest.mark.parametrize("beams", [1, 3])
+def test_generation_raises_what_its_kernels_report(beams):
+    """A token outside the vocabulary: an error in words, as CPU tensors give one, and no word left for whoever looks next."""
+    g = small()
+    prompt = torch.randint(0, 500, (2, 20))
+    prompt[1, 7] = 500
+    with pytest.raises(RuntimeError, match="token id outside the vocabulary"):
+        g.generate(prompt, 5, kv="4bit", beams=beams)
+    assert nat().get_error() == 0
+    assert g.generate(prompt[:1], 5, kv="4bit", beams=beams).shape == (1, 25)
+
+
+def test_a_step_outside_the_pool_is_reported():
+    """A block table that names no page, which the kernels leave out: generation does not hand on what came of it."""
+    from ml_b200.models import generation
+    g = small()
+    m = generation.CachedDecoder(g, 2, 30, 16)
+    ids = torch.randint(0, 500, (2, 20), dtype=I32, device=dev())
+    slots, _, _ = m.cache.grow(ints([20, 20]), 40)
+    m.prompt(ids, slots)
+    m.cache.table[1, 0] = -1
+    m.step(ids[:, 0].contiguous())
+    with pytest.raises(RuntimeError, match="page outside the pool"):
+        m.check()
+    assert nat().get_error() == 0
+    m.check()
+
+
 def test_beams_end():
     from ml_b200.models import generation
     g = small()
