@@ -1013,12 +1013,18 @@ MLB_API int mlb_kv4_read(void* k, void* v, const uint8_t* pages, const int* slot
   return (int)e;
 }
 
-// fp32 words of workspace that attention wants, and (negative) nothing for sizes that it does not take; counters: B Hkv row tiles, zero before the first call
+// fp32 words of workspace that attention wants - two shares of each thread block of its launches - and (negative) nothing for sizes that it does not take; counters:
+// B Hkv row tiles, zero before the first call
 MLB_API long mlb_kv4_attn_scratch(int B, int Tq, int H, int Hkv, int hd, int width, int page) {
   if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1 || H % Hkv != 0) return -7;
   int nt;
   const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
-  return (long)attn_most(B < MAX_B ? B : MAX_B, Hkv, width, page) * tiles * 2 * 8 * nt * (hd + 2);
+  int grid = attn_grid(B < MAX_B ? B : MAX_B, Hkv, width, page, hd, nt, tiles);
+  if (B > MAX_B && B % MAX_B != 0) {      // the last launch: fewer sequences, whose numbers leave room for more blocks
+    const int last = attn_grid(B % MAX_B, Hkv, width, page, hd, nt, tiles);
+    grid = last > grid ? last : grid;
+  }
+  return (long)grid * tiles * 2 * 8 * nt * (hd + 2);
 }
 // out[B Tq, H hd] = attention of q (rows `q_stride` elements apart) over table[B, width], lens[B] tokens each; lse[B, H, Tq] or null
 MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pages, const int* table, const int* lens, float* part, int* count, long n_pages,

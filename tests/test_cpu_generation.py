@@ -148,6 +148,17 @@ def test_entries_refuse_addresses_off_16_bytes():
             assert call(**{name: off}) == -7, name
 
 
+@pytest.mark.parametrize("B,Tq,H,Hkv,hd", [(8, 1024, 32, 8, 128), (1, 8192, 32, 8, 128), (2, 5000, 4, 4, 32), (64, 300, 12, 4, 96), (2100, 16, 8, 2, 64)])
+def test_attention_workspace_is_that_of_the_blocks_that_run(B, Tq, H, Hkv, hd):
+    """Two shares a thread block, of which all tiles of rows together have no more than the machine holds (8 an SM at most) and one more a tile."""
+    from ml_b200.ops import native
+    L, rows = native.lib(), H // Hkv * Tq
+    tiles, share = -(-rows // 16), 16 * (hd + 2)
+    for width in (1, 3, 512):
+        got = L.mlb_kv4_attn_scratch(B, Tq, H, Hkv, hd, width, 16)
+        assert tiles * 2 * share <= got <= (8 * 148 + tiles) * 2 * share
+
+
 def test_tensors_off_16_bytes_are_refused_by_name():
     """Views that begin in the middle of a buffer, before anything else is asked of them."""
     from ml_b200.ops import native_gen

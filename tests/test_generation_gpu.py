@@ -259,6 +259,25 @@ def test_attention_of_more_row_tiles_than_there_are_multiprocessors(lens, Tq, H,
     close(*attend(lens, Tq, H, Hkv, hd, page, seed=7))
 
 
+@pytest.mark.parametrize("B,T,Tq,H,Hkv,hd", [(1, 900, 1, 4, 4, 64), (16, 700, 1, 8, 4, 128), (3, 900, 40, 8, 2, 32), (2, 1300, 1300, 4, 2, 128), (2500, 20, 2, 2, 1, 64), (2049, 300, 9, 2, 1, 128)])
+def test_attention_stays_in_its_workspace(B, T, Tq, H, Hkv, hd):
+    """What the library says it wants is enough: nothing behind it is written, and the answer is the one of a call of the operator."""
+    n, page = nat(), 64
+    width = -(-T // page)
+    pages = oracle.random_pages(width, Hkv, page, hd, 3).to(dev())
+    table, lens = ints([list(range(width))]).repeat(B, 1), torch.randint(T // 2, T + 1, (B,), dtype=I32, device=dev())
+    q = torch.randn(B * Tq, H * hd, device=dev()).bfloat16()
+    want, got = torch.empty_like(q), torch.empty_like(q)
+    ops.kv4_attn(want, None, q, pages, table, lens, Tq, H, Hkv, hd)
+    e = n._entries()
+    floats = e.mlb_kv4_attn_scratch(B, Tq, H, Hkv, hd, width, page)
+    part = torch.full((floats + 65536,), 7.25, device=dev())
+    count = torch.zeros(B * Hkv * (-(-H // Hkv * Tq // 8) + 1), dtype=I32, device=dev())
+    n._chk(e.mlb_kv4_attn(got, n.NONE, q, pages, table, lens, part, count, width, q.stride(0), B, Tq, H, Hkv, hd, width, page, hd ** -0.5), "kv4_attn")
+    torch.cuda.synchronize()
+    assert bool((part[floats:] == 7.25).all()) and torch.equal(want, got) and int(count.abs().sum()) == 0
+
+
 @pytest.mark.parametrize("hd,size", [(64, 1e9), (64, 3e10), (128, 1e11), (32, 1e20), (96, 1e36), (128, 1e36), (64, 1e-10), (128, 1e-20)])
 @pytest.mark.parametrize("T,Tq,H", [(700, 1, 4), (90, 5, 8)])
 def test_attention_over_values_of_any_size(hd, size, T, Tq, H):
