@@ -1016,7 +1016,7 @@ MLB_API int mlb_kv4_read(void* k, void* v, const uint8_t* pages, const int* slot
 // fp32 words of workspace that attention wants - two shares of each thread block of its launches - and (negative) nothing for sizes that it does not take; counters:
 // B Hkv row tiles, zero before the first call
 MLB_API long mlb_kv4_attn_scratch(int B, int Tq, int H, int Hkv, int hd, int width, int page) {
-  if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1 || H % Hkv != 0) return -7;
+  if (!known_head(hd) || page_shift(page) < 0 || Hkv < 1 || H < 1 || H % Hkv != 0 || Tq < 1) return -7;
   int nt;
   const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
   int grid = attn_grid(B < MAX_B ? B : MAX_B, Hkv, width, page, hd, nt, tiles);
@@ -1030,7 +1030,7 @@ MLB_API long mlb_kv4_attn_scratch(int B, int Tq, int H, int Hkv, int hd, int wid
 MLB_API int mlb_kv4_attn(void* out, float* lse, const void* q, const uint8_t* pages, const int* table, const int* lens, float* part, int* count, long n_pages,
                          long q_stride, int B, int Tq, int H, int Hkv, int hd, int width, int page, float scale, cudaStream_t st) {
   const int shift = page_shift(page);
-  if (!known_head(hd) || shift < 0 || Hkv < 1 || H % Hkv != 0 || q_stride % 8 != 0 || !on_16_bytes(out, q, pages, part)) return -7;
+  if (!known_head(hd) || shift < 0 || Hkv < 1 || H < 1 || H % Hkv != 0 || Tq < 1 || q_stride % 8 != 0 || !on_16_bytes(out, q, pages, part)) return -7;
   int nt;
   const int tiles = row_tiles((long)(H / Hkv) * Tq, nt);
   if (tiles > 65535 || (long)n_pages > 0x7FFFFFFFL || (long)width * page >= 1L << 31 || (long)Hkv * page * hd * 9 / 8 >= 1L << 32 || ((long)width * page / TOK + PAD) * (B < MAX_B ? B : MAX_B) * Hkv >= 1L << 31) return -7;

@@ -159,6 +159,16 @@ def test_attention_workspace_is_that_of_the_blocks_that_run(B, Tq, H, Hkv, hd):
         assert tiles * 2 * share <= got <= (8 * 148 + tiles) * 2 * share
 
 
+def test_attention_entries_refuse_no_tokens_and_no_heads():
+    """... with their code, and do not divide by what there is none of."""
+    from ml_b200.ops import native
+    L, ok = native.lib(), 1 << 20
+    for Tq, H, Hkv in ((0, 4, 2), (1, 0, 2), (-1, 4, 2), (1, 4, 0)):
+        assert L.mlb_kv4_attn_scratch(1, Tq, H, Hkv, 64, 1, 16) == -7
+        if not torch.cuda.is_available():
+            assert L.mlb_kv4_attn(ok, None, ok, ok, ok, ok, ok, ok, 4, 256, 1, Tq, H, Hkv, 64, 1, 16, 0.125, None) == -7
+
+
 def test_tensors_off_16_bytes_are_refused_by_name():
     """Views that begin in the middle of a buffer, before anything else is asked of them."""
     from ml_b200.ops import native_gen
