@@ -488,13 +488,17 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
         for (int k = 0; k < 4; k++)
           if (t0 + 16 * b + k / 2 * 8 >= seen[n][k & 1]) s[b][n][k] = -INFINITY;
   }
+  auto power = [&](int b, int n, int k) {      // (a masked token's is -inf where a tiny scale's c has become 0 too)
+    const float x = fmaf(s[b][n][k], c[n][k & 1], r.neg[n][k & 1]);
+    return MASKED && s[b][n][k] == -INFINITY ? -INFINITY : x;
+  };
   float y[NB][NT][4], top = -INFINITY;
 #pragma unroll
   for (int b = 0; b < NB; b++)
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) y[b][n][k] = fmaf(s[b][n][k], c[n][k & 1], r.neg[n][k & 1]), top = fmaxf(top, y[b][n][k]);
+      for (int k = 0; k < 4; k++) y[b][n][k] = power(b, n, k), top = fmaxf(top, y[b][n][k]);
   if (__any_sync(0xffffffffu, top > UP + 8.f)) {
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -515,7 +519,7 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
           for (int d = 0; d < HD / 16; d++) r.o[n][d][h] *= f, r.o[n][d][h + 2] *= f;
         }
 #pragma unroll
-        for (int b = 0; b < NB; b++) y[b][n][h] = fmaf(s[b][n][h], c[n][h], r.neg[n][h]), y[b][n][h + 2] = fmaf(s[b][n][h + 2], c[n][h], r.neg[n][h]);
+        for (int b = 0; b < NB; b++) y[b][n][h] = power(b, n, h), y[b][n][h + 2] = power(b, n, h + 2);
       }
   }
 #pragma unroll

@@ -192,6 +192,20 @@ def test_attention_of_strided_queries_with_a_scale():
     close(*attend([90, 31], 1, 4, 2, 64, 32, seed=6, scale=0.0))
 
 
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("size,scale", [(0.0, 1e-12), (1e-30, 1e-13), (1.0, 1e-30), (1.0, -1e-42), (0.0, 1e-45)])
+def test_attention_with_scales_that_leave_nothing_of_scores(hd, size, scale):
+    """Scores of 0 or next to it: seen tokens count alike, the others, in the last block and behind a query's own token, not at all."""
+    lens, Tq, H, Hkv, page = [20, 37, 2], 3, 4, 2, 16
+    pages = oracle.random_pages(6, Hkv, page, hd, 11)
+    table = np.array([[0, 1, 0], [2, 3, 4], [5, 0, 0]])
+    q = (torch.randn(len(lens) * Tq, H * hd, generator=torch.Generator().manual_seed(hd)) * size).bfloat16()
+    out, lse = torch.empty_like(q, device=dev()), torch.empty(len(lens), H, Tq, device=dev())
+    ops.kv4_attn(out, lse, q.to(dev()), pages.to(dev()), ints(table.tolist()), ints(lens), Tq, H, Hkv, hd, scale)
+    o, l, tol, ltol = oracle.attention(q, pages, table, lens, Tq, H, Hkv, hd, scale)
+    close(out.cpu().double().numpy().reshape(o.shape), lse.cpu().double().numpy(), o, l, tol, ltol)
+
+
 def test_attention_with_large_scores():
     """Scores in the hundreds: most weights vanish, the running maximum moves block by block."""
     close(*attend([500, 37], 1, 4, 2, 64, 32, seed=8, spread=30.0))
