@@ -653,7 +653,7 @@ PyObject* py_kv4_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (ou
   if (a[10] != Py_None) {
     if (!PyFloat_CheckExact(a[10])) return declined();
     scale = PyFloat_AS_DOUBLE(a[10]);
-    if (!std::isfinite(scale)) return declined();
+    if (!(std::fabs(scale) <= 0x1p127)) return declined();
   }
   const long B = lens.size(0);
   if (!plain(a[4], table, at::kInt, 2) || !sized(table, {B, table.size(1)}) || table.numel() >= (1L << 31) || !rows_given(a[2], q, B * Tq, H * hd) || !given(a[0], out, at::kBFloat16, {B * Tq, H * hd}) ||

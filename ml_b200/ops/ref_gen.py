@@ -72,8 +72,8 @@ def check_read(k, v, pages, slots):
 
 
 def check_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale):
-    if scale is not None and not math.isfinite(scale):
-        raise ValueError(f"scale = {scale}")
+    if scale is not None and not abs(scale) <= 2.0 ** 127:      # (times log2 e it still is an fp32 number)
+        raise ValueError(f"scale = {scale}: need 2^127 at most")
     n, heads, page, _ = pages_shape(pages, hd)
     if Hkv < 1 or heads != Hkv or H % Hkv or H < 1 or Tq < 1:
         raise ValueError(f"{H} query heads over {Hkv} key / value heads (pages of {heads}), {Tq} tokens a sequence")

@@ -169,6 +169,15 @@ def test_attention_entries_refuse_no_tokens_and_no_heads():
             assert L.mlb_kv4_attn(ok, None, ok, ok, ok, ok, ok, ok, 4, 256, 1, Tq, H, Hkv, 64, 1, 16, 0.125, None) == -7
 
 
+@pytest.mark.parametrize("scale", [2e38, -1e300, math.inf, math.nan])
+def test_scales_past_32_bits_are_refused(scale):
+    """A kernel has the scale times log2 e as an fp32 number: one that becomes infinite there is none."""
+    x, pages = torch.zeros(1, 64), torch.zeros(4, 1, 1, 18 * 64, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="scale"):
+        ops.kv4_attn(torch.empty_like(x), None, x, pages, ints([[0]]), ints([1]), 1, 1, 1, 64, scale)
+    ops.kv4_attn(torch.empty_like(x), None, x, pages, ints([[0]]), ints([1]), 1, 1, 1, 64, 2.0 ** 127)
+
+
 def test_tensors_off_16_bytes_are_refused_by_name():
     """Views that begin in the middle of a buffer, before anything else is asked of them."""
     from ml_b200.ops import native_gen

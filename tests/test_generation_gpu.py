@@ -639,6 +639,13 @@ def test_refusals():
             pytest.fail(f"call {k} was taken")
 
 
+@pytest.mark.parametrize("scale", [2e38, -1e300, math.inf, math.nan])
+def test_scales_past_32_bits_are_refused(scale):
+    x, pages = torch.zeros(1, 64, dtype=torch.bfloat16, device=dev()), torch.zeros(4, 1, 1, 18 * 64, dtype=torch.uint8, device=dev())
+    with pytest.raises(ValueError, match="scale"):
+        ops.kv4_attn(torch.empty_like(x), None, x, pages, ints([[0]]), ints([1]), 1, 1, 1, 64, scale)
+
+
 @pytest.mark.parametrize("module", [True, False])
 def test_views_that_begin_off_16_bytes_are_refused(monkeypatch, module):
     """Contiguous ones too, by the argument's name, on both ways into the library; nothing is launched."""
