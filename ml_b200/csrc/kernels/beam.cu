@@ -1,5 +1,7 @@
 // What a generation step decides on the GPU: which cache pages and slots the new tokens get, which continuations of the beams are kept, and the beams' tables,
 // histories and half-filled pages in the order of their parents.  Nothing here is read back by the host.
+#include <type_traits>
+
 #include "tc.cuh"
 
 namespace {
@@ -131,18 +133,22 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
 
 // ------------------------------------------------------------------ beam selection
 // score(k, v) = prev[k] + (z[k, v] - lse[k]), lse[k] = log sum_v exp z[k, v]; of the K V scores of a request the K largest, equal ones by the lowest k V + v.  A
-// beam that has ended goes on as itself: its one continuation is (eos, prev[k]).  Within a row the order of the scores is that of the logits, so a row's K
-// best can be found before its lse is known, in the one pass that reads it.
+// beam that has ended goes on as itself: its one continuation is (eos, prev[k]).  Within a row a larger logit has no smaller score, so a row's K
+// best can be found before its lse is known, in the one pass that reads it - but for logits that differ and have equal scores after both roundings, of which the lowest
+// index counts and not the largest logit.  So a piece also gives a limit that no logit passes which it has left out.  Only where the limit's score is the K-th best of all
+// can something of a lower index have been left out; then a warp looks closer (some 2 us: 32 beams of bf16 logits, of which many are alike, in a search's first step),
+// and if need be goes over the request's rows in order (1 x 4 beams of 50304 with 40 equal scores a row 75 us).
 //
 // Bound by the logits' bytes, then by an exponential for each.  A row is cut into as many pieces as fill the machine once, and a thread block fetches up to 32 KB of
 // its piece at a time into shared memory, by one bulk copy: many bytes on their way, and loops that are short (they run a few times only, so that instructions
-// fetched for the first time are a good part of a call).  The K-th largest of the maxima of 8 to 32 parts of what came first is a bound below which nothing
-// is among the piece's K largest: one comparison for 8 logits leaves some tens of candidates.  Where they become many, those behind the K-th go and it
+// fetched for the first time are a good part of a call).  The (K + 1)-th largest of the maxima of 8 to 32 parts of what came first is a bound below which
+// nothing is among the piece's K + 1 largest: one comparison for 8 logits leaves some tens of candidates.  Where they become many, those behind the (K + 1)-th go and it
 // is the bound from then on.  A candidate's place is the number of those before it.  More candidates at a time than there is room for (logits all alike) are forgotten:
 // then K rounds over the piece find its K largest.  The request's last thread block finds its K best among the pieces' lists in the same way,
 // the bound being of its threads' best.
-// 32 x 8 beams of 50304 bf16 logits, a quarter of them ended: 15.2 us (1.7 TB/s), of which fetching and the maximum 6.2, the exponentials 1, candidates and their
-// bound 2.6, the counters 1.9, the merge 3.  1 x 4 beams: 6.8 us (2.3, then 1 for the counters, 3 for the merge): latencies one behind the other.
+// 32 x 8 beams of 50304 bf16 logits, a quarter of them ended: 15.6 us (1.7 TB/s), of which fetching and the maximum 6.2, the exponentials 1, candidates and their
+// bound 2.6, the counters 1.9, the merge 3.4.  1 x 4 beams: 7.2 us (2.3, then 1 for the counters, 3.4 for the merge): latencies one behind the other.  fp32 logits: 1 x 4
+// beams 7.2, 32 x 8 with none ended 25.8 (bf16: 17.9), 8 x 32 44.6 (33.8).
 constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_BYTES = 32768, SEL_MAX_K = 32, SEL_CAND = 512, SEL_HELD = 1024;
 constexpr int SEL_PER_SM = 6, SEL_LEAST = 4096;      // thread blocks that an SM holds; the smallest piece
 typedef unsigned long long u64;
@@ -158,8 +164,8 @@ struct SelectArgs {
   const float* prev;
   const int* done;
   float2* stats;      // [rows][pieces]: maximum, sum of exponentials
-  float* values;      // [rows][pieces][L]: the K best and maybe others
-  int* ids;           // [rows][pieces][L], -1: none
+  float* values;      // [rows][pieces][L + 1]: the K best and maybe others, and last what no logit passes that is not among them
+  int* ids;           // [rows][pieces][L + 1], -1: none
   int* ticket;
   long stride;
   int K, L, V, eos, pieces, piece;
@@ -233,8 +239,8 @@ __device__ __forceinline__ int place_of(u64 mine, const u64* keys, int n) {
 __device__ __forceinline__ int parts_for(int K) { return K <= SEL_WARPS / 2 ? SEL_WARPS : K <= SEL_WARPS ? 2 * SEL_WARPS : 4 * SEL_WARPS; }
 // The K-th largest of the maxima of the parts' values: K of these are not below it.  tops: 32 values of shared memory
 template <typename X, typename Max>
-__device__ __forceinline__ X kth_of_parts(X m, int K, X* tops, Max larger) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = parts_for(K), each = SEL_THREADS / parts;      // 8, 16 or 32 threads
+__device__ __forceinline__ X kth_of_parts(X m, int K, int parts, X* tops, Max larger) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, each = SEL_THREADS / parts;      // 8, 16 or 32 threads
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o));
   for (int o = 8; o < each; o <<= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -256,14 +262,86 @@ __device__ __forceinline__ float log_of(float x) {
   return fmaf((float)e, 0.693145751953125f, fmaf((float)e, 1.42860682e-6f, __log2f(f) * 0.693147181f));
 }
 
+__device__ __forceinline__ float score_of(float z, float prev, float lse) {      // NaN: there is none
+  const float x = __fadd_rn(prev, __fsub_rn(z, lse));
+  return x != x ? -INFINITY : x;
+}
+constexpr uint32_t NOTHING = 0x007FFFFFu;      // -inf, `ordered`
+template <typename T> __device__ __forceinline__ uint32_t next_below(uint32_t u) {      // the next smaller number of the type, `ordered` (below 0: nothing larger than that)
+  return u <= NOTHING ? NOTHING : u - (std::is_same<T, float>::value ? 1u : 0x10000u);
+}
+// Scores equal to the K-th best one S, for which a warp answers: whether a list has left out one that counts, and the places of those of the lowest indices.
+// (As a function that is called it costs 0.3 us of every call, in this place 0.1.)
+template <typename T>
+__device__ __forceinline__ void equal_scores(const SelectArgs& A, int req, uint32_t S, const u64* keys, bool few, const u64* cand, int found, const float* prev, const float* lse, const int* ended) {
+  const int lane = threadIdx.x & 31, K = A.K, V = A.V, lists = K * A.pieces;
+  auto dead = [&](int k) { return !(prev[k] > -INFINITY && fabsf(lse[k]) < INFINITY); };
+  auto put = [&](int place, int k, int t) {
+    const int o = req * K + place;
+    A.scores[o] = unordered(S);
+    A.tokens[o] = t, A.parents[o] = k, A.done_out[o] = ended[k] || t == A.eos;
+  };
+  // A list of such a limit has entries of score S itself, or there would be K better ones.  If these are one logit, the limit, what it has left out of that logit has higher
+  // indices and does not count; smaller logits do if the next smaller number still has that score
+  bool counts = false;
+#pragma unroll 1
+  for (int e = lane; e < lists * A.L; e += 32)
+    if (const u64 key = keys[e]; (uint32_t)(key >> 32) == S) {
+      const int l = few ? e % lists : e / A.L, nth = few ? e / lists : e % A.L, k = l / A.pieces;
+      if (ended[k] || dead(k)) continue;
+      const long list = ((long)req * lists + l) * (A.L + 1);
+      const uint32_t z = ordered(__ldcg(A.values + list + nth)), d = ordered(__ldcg(A.values + list + A.L));
+      if (d > NOTHING && ordered(score_of(unordered(d), prev[k], lse[k])) == S)
+        counts |= z != d || ordered(score_of(unordered(next_below<T>(d)), prev[k], lse[k])) == S;
+    }
+  if (!__any_sync(0xffffffffu, counts)) {
+#pragma unroll 1
+    for (int e = lane; e < found; e += 32)
+      if (const u64 mine = cand[e]; (uint32_t)(mine >> 32) == S) {
+        const uint32_t flat = ~(uint32_t)mine;
+        const int place = place_of(mine, cand, found);
+        if (place < K) put(place, (int)(flat / (uint32_t)V), (int)(flat % (uint32_t)V));
+      }
+    return;
+  }
+  int at = 0;      // better ones, all of them candidates
+#pragma unroll 1
+  for (int e = lane; e < found; e += 32) at += (uint32_t)(cand[e] >> 32) > S;
+  at = __reduce_add_sync(0xffffffffu, at);
+  for (int k = 0; k < K && at < K; k++) {
+    const T* z = reinterpret_cast<const T*>(A.logits) + ((long)req * K + k) * A.stride;
+    const bool end = ended[k] != 0, none = end || dead(k);
+    for (long v = 0; v < V && at < K; v += 256) {
+      uint32_t hits = 0;
+#pragma unroll 8
+      for (int e = 0; e < 8; e++) {      // (logits 32 apart: a hit's index is v + 32 e + lane)
+        const long t = v + 32 * e + lane;
+        float x = -INFINITY;
+        if (t < V && !none) x = score_of(fmaxf((float)z[t], -INFINITY), prev[k], lse[k]);
+        if (end && t == A.eos && prev[k] > -INFINITY) x = prev[k];
+        hits |= t < V && ordered(x) == S ? 1u << e : 0u;
+      }
+      if (!__any_sync(0xffffffffu, hits != 0)) continue;
+#pragma unroll 1
+      for (int e = 0; e < 8; e++) {
+        const uint32_t those = __ballot_sync(0xffffffffu, hits >> e & 1);
+        const int to = at + __popc(those & ((1u << lane) - 1));
+        if ((hits >> e & 1) && to < K) put(to, k, (int)v + 32 * e + lane);
+        at += __popc(those);
+      }
+    }
+  }
+}
+
 // BULK: rows begin on 16-byte boundaries
 template <typename T, bool BULK>
-__global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const SelectArgs A) {
+__global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const __grid_constant__ SelectArgs A) {
   extern __shared__ __align__(128) uint8_t fetched[];
   __shared__ uint64_t bar;
   __shared__ float tops[32], sums[SEL_WARPS];
   __shared__ u64 cand[SEL_HELD], red[32];
   __shared__ int n_cand, last;
+  __shared__ uint32_t limit;      // the largest score of what lists have left out, `ordered`
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = A.K, V = A.V;
   const int row = blockIdx.y, req = row / K;
   const long list = (long)row * A.pieces + blockIdx.x;
@@ -283,6 +361,10 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
     const int begin = blockIdx.x * A.piece, n = min(A.piece, V - begin);
     const T* z = reinterpret_cast<const T*>(A.logits) + row * A.stride + begin;
     float m = -INFINITY, s = 0.f, bound = -INFINITY;
+    // Candidates are down to the N-th: one more than are wanted, so that what is left out has the K-th one's score only if the next one has, too (32 beams have no part more
+    // to bound that one by).  What no logit passes that is left out: the bound, where candidates that may be as large have gone, else the next smaller number
+    const int parts = parts_for(K), N = K + 1;
+    bool cut = false;
     int most = 0;      // candidates up to and with this thread's last
     bool over = false;
     uint32_t parity = 0;
@@ -305,9 +387,9 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
       Eight<T> x;
 #pragma unroll 2
       for (int e = mine; e < count; e += SEL_THREADS * 8) top = fmaxf(top, x.load(data + e));
-      const float kth = kth_of_parts(top, K, tops, [](float a, float b) { return fmaxf(a, b); });
+      const float kth = kth_of_parts(top, min(N, parts), parts, tops, [](float a, float b) { return fmaxf(a, b); });
       if (c == 0) bound = kth;
-      top = warp_max(tops[lane % parts_for(K)]);
+      top = warp_max(tops[lane % parts]);
       if (top > m) s *= ex2((m - top) * 1.44269504088896f), m = top;      // (from -inf: 0 times 0)
       const float mm = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
@@ -330,7 +412,7 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
       const bool more = c + CHUNK < n;
       if (__syncthreads_or(most > (more ? 2 * K : SEL_CAND))) {
         over |= __syncthreads_or(most > SEL_CAND) != 0;
-        if (!over && more) {      // the K best of them stay
+        if (!over && more) {      // the N best of them stay
           const int found = n_cand;
           u64 mine[SEL_CAND / SEL_THREADS];
           int place[SEL_CAND / SEL_THREADS];
@@ -338,15 +420,16 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
           for (int h = 0; h < SEL_CAND / SEL_THREADS; h++) {
             const int e = tid + h * SEL_THREADS;
             mine[h] = e < found ? cand[e] : 0ull;
-            place[h] = e < found ? place_of(mine[h], cand, found) : K;
+            place[h] = e < found ? place_of(mine[h], cand, found) : N;
           }
           __syncthreads();
 #pragma unroll
           for (int h = 0; h < SEL_CAND / SEL_THREADS; h++)
-            if (place[h] < K) cand[place[h]] = mine[h];
-          if (tid == 0) n_cand = K;
+            if (place[h] < N) cand[place[h]] = mine[h];
+          if (tid == 0) n_cand = N;
           __syncthreads();
-          bound = unordered((uint32_t)(cand[K - 1] >> 32));
+          bound = unordered((uint32_t)(cand[N - 1] >> 32));
+          cut = true;
           __syncthreads();
         }
         most = 0;
@@ -370,21 +453,23 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
       for (int e = tid; e < found; e += SEL_THREADS) {
         const u64 mine = cand[e];
         const int k = found <= L ? e : place_of(mine, cand, found);      // (the merge needs no order)
-        if (k < L) A.values[list * L + k] = unordered((uint32_t)(mine >> 32)), A.ids[list * L + k] = (int)~(uint32_t)mine;
+        if (k <= L) A.values[list * (L + 1) + k] = unordered((uint32_t)(mine >> 32)), A.ids[list * (L + 1) + k] = (int)~(uint32_t)mine;
       }
-      if (tid >= found && tid < L) A.ids[list * L + tid] = -1;
+      if (tid >= found && tid < L) A.ids[list * (L + 1) + tid] = -1;
+      if (tid == L && found <= L) A.values[list * (L + 1) + L] = cut ? bound : unordered(next_below<T>(ordered(bound)));
     } else {
       u64 prior = ~0ull;
-      for (int k = 0; k < K; k++) {
+      for (int k = 0; k <= K; k++) {      // (one more: the largest that is left out)
         u64 best = 0;
         for (int e = tid; e < n; e += SEL_THREADS) {
           const u64 r = rank_of(fmaxf((float)z[e], -INFINITY), begin + e);
           if (r < prior) best = max(best, r);
         }
         prior = best = block_best(best, red);
-        if (tid == 0) A.values[list * L + k] = unordered((uint32_t)(best >> 32)), A.ids[list * L + k] = (int)~(uint32_t)best;
+        const long a = list * (L + 1) + (k < K ? k : L);
+        if (tid == 0) A.values[a] = best == 0 ? -INFINITY : unordered((uint32_t)(best >> 32)), A.ids[a] = (int)~(uint32_t)best;
       }
-      if (tid >= K && tid < L) A.ids[list * L + tid] = -1;
+      if (tid >= K && tid < L) A.ids[list * (L + 1) + tid] = -1;
     }
   }
   // ---- the request's last thread block merges
@@ -393,7 +478,7 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
   __syncthreads();
   if (!last) return;
   const int lists = K * A.pieces, L = A.L;
-  if (tid == 0) A.ticket[req] = 0, n_cand = 0;
+  if (tid == 0) A.ticket[req] = 0, n_cand = 0, limit = 0;
   for (int k = warp; k < K; k += SEL_WARPS) {      // (an ended beam's are nothing, and not asked for)
     const float2* st = A.stats + (long)(req * K + k) * A.pieces;
     float2 v[2];      // (pieces past 64 are read again)
@@ -416,13 +501,14 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
   const int mine = few ? tid : warp + 8 * (lane >> 4) + 16 * (lane >> 3 & 1) + 32 * (lane & 7), inner = few ? lists : L;
   u64* keys = reinterpret_cast<u64*>(fetched);
   u64 best = 0;
+  uint32_t most_left = 0;
   const float per_inner = 1.f / inner, per_beam = 1.f / A.pieces;      // ((x + 1/2) / n rounded down is exact for the few thousands that these are)
 #pragma unroll 1
   for (int e = mine; e < lists * L; e += SEL_THREADS) {
     const int outer = (int)((e + 0.5f) * per_inner), rest = e - outer * inner, l = few ? rest : outer, nth = few ? outer : rest, k = (int)((l + 0.5f) * per_beam);
-    const long a = ((long)req * lists + l) * L + nth;
+    const long a = ((long)req * lists + l) * (L + 1) + nth;
     int t = __ldcg(A.ids + a);
-    float x = __ldcg(A.values + a);
+    float x = __ldcg(A.values + a), y = nth == L - 1 ? __ldcg(A.values + a + 1) : -INFINITY;
     // a beam that has ended, and one of no continuation: it was nothing, or its logits have no logarithm of a sum
     const bool end = ended[k] != 0, dead = !end && !(prev[k] > -INFINITY && fabsf(lse[k]) < INFINITY);
     if (end || dead) {
@@ -433,13 +519,16 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
       }
       if (l != k * A.pieces || t >= V) t = -1;
     } else {
-      x = __fadd_rn(prev[k], __fsub_rn(x, lse[k]));
+      x = score_of(x, prev[k], lse[k]), y = score_of(y, prev[k], lse[k]);
+      if (y > -INFINITY) most_left = max(most_left, ordered(y));
     }
     const u64 key = t < 0 ? 0ull : rank_of(x != x ? -INFINITY : x, (uint32_t)k * (uint32_t)V + (uint32_t)t);
     keys[e] = key;
     best = max(best, key);
   }
-  const u64 bound = kth_of_parts(best, K, red, [](u64 a, u64 b) { return a > b ? a : b; });
+  most_left = __reduce_max_sync(0xffffffffu, most_left);
+  if (lane == 0 && most_left != 0) atomicMax(&limit, most_left);
+  const u64 bound = kth_of_parts(best, K, parts_for(K), red, [](u64 a, u64 b) { return a > b ? a : b; });
 #pragma unroll 1
   for (int e = tid; e < lists * L; e += SEL_THREADS) {
     const u64 key = keys[e];
@@ -447,21 +536,28 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const S
   }
   __syncthreads();
   const int found = n_cand;      // (K or more: every beam has a continuation, if one of -inf)
+  // What lists have left out scores S at most, S being the K-th best score.  If one does score S, the warp that has the K-th decides on all of that score
+  most_left = limit;
+  bool tied = false;
   for (int e = tid; e < found; e += SEL_THREADS) {
     const u64 mine = cand[e];
     const int k = place_of(mine, cand, found);
-    if (k < K) {
-      const uint32_t flat = ~(uint32_t)mine;
-      const int from = (int)(flat / (uint32_t)V), t = (int)(flat % (uint32_t)V), o = req * K + k;
-      A.scores[o] = unordered((uint32_t)(mine >> 32));
-      A.tokens[o] = t, A.parents[o] = from, A.done_out[o] = ended[from] || t == A.eos;
+    if (k >= K) continue;
+    if ((uint32_t)(mine >> 32) == most_left) {
+      tied |= k == K - 1;
+      continue;
     }
+    const uint32_t flat = ~(uint32_t)mine;
+    const int from = (int)(flat / (uint32_t)V), t = (int)(flat % (uint32_t)V), o = req * K + k;
+    A.scores[o] = unordered((uint32_t)(mine >> 32));
+    A.tokens[o] = t, A.parents[o] = from, A.done_out[o] = ended[from] || t == A.eos;
   }
+  if (__any_sync(0xffffffffu, tied)) equal_scores<T>(A, req, most_left, keys, few, cand, found, prev, lse, ended);
 }
 
 // Logits of a piece, a multiple of 8: the machine's thread blocks once over the rows, but no more of a row than one fetch where there are enough of them, SEL_LEAST
 // logits and more each, and no more lists than a thread block holds to merge
-int select_list(int K) { return K <= 16 ? 2 * K : K; }      // entries of a piece's list: usually all its candidates, which then need no places
+int select_list(int K) { return K <= 16 ? 2 * K : K; }      // entries of a piece's list, the limit apart: usually all its candidates, which then need no places
 int select_piece(int rows, int K, int V, int bits) {
   const long fill = (long)SEL_PER_SM * mlb_sm_count() / rows, one = ((long)V * (bits / 8) + SEL_CHUNK_BYTES - 1) / SEL_CHUNK_BYTES, most = (V - 1) / SEL_LEAST + 1,
              held = SEL_HELD / (K * select_list(K));
@@ -554,7 +650,7 @@ MLB_API int mlb_beam_select_pieces(int rows, int K, int V, int bits) {
   const int piece = select_piece(rows, K, V, bits);
   return (V - 1) / piece + 1;
 }
-// bits: 16 (bf16) or 32 (fp32) logits, rows `stride` elements apart
+// bits: 16 (bf16) or 32 (fp32) logits, rows `stride` elements apart; stats: 2 floats for each piece of each row, values and ids 2 K + 1
 MLB_API int mlb_beam_select(float* scores, int* tokens, int* parents, int* done_out, const void* logits, const float* prev, const int* done, float* stats,
                             float* values, int* ids, int* ticket, int rows, int K, int V, long stride, int eos, int bits, cudaStream_t st) {
   const int pieces = mlb_beam_select_pieces(rows, K, V, bits);

@@ -704,11 +704,11 @@ PyObject* py_beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {      // 
   const long V = z.size(1), pieces = K.mlb_beam_select_pieces((int)rows, (int)Kb, (int)V, half ? 16 : 32);
   if (pieces < 0 || K.mlb_capture_id(st) != 0) return declined();
   const long m = rows * pieces;
-  const Kept& w = kept(KEPT_SELECT, prev, st, m * (2 + 4 * Kb), B);
+  const Kept& w = kept(KEPT_SELECT, prev, st, m * (4 + 4 * Kb), B);
   float* part = at_<float>(w.part);
   return launched("beam_select", [&] {
     return K.mlb_beam_select(at_<float>(scores), at_<int>(tokens), at_<int>(parents), at_<int>(done_out), at_<void>(z), at_<float>(prev), at_<int>(done), part, part + 2 * m,
-                             (int*)(part + 2 * m + 2 * m * Kb), at_<int>(w.count), (int)rows, (int)Kb, (int)V, z.stride(0), (int)eos, half ? 16 : 32, st);
+                             (int*)(part + 2 * m + m * (2 * Kb + 1)), at_<int>(w.count), (int)rows, (int)Kb, (int)V, z.stride(0), (int)eos, half ? 16 : 32, st);
   });
   END_HANDLE_TH_ERRORS
 }

@@ -116,10 +116,10 @@ def beam_select(scores, tokens, parents, done_out, logits, prev, done, eos):
     pieces = e.mlb_beam_select_pieces(rows, K, V, bits)
     if pieces < 0:
         raise ValueError(f"{B} x {K} beams: at most 65535 rows")
-    part = _n.scratch("select_part", rows * pieces * (2 + 4 * K), F32, dev)
+    part = _n.scratch("select_part", rows * pieces * (4 + 4 * K), F32, dev)
     ticket = _n.scratch("select_ticket", B, I32, dev, zero=True)
     base, n = part.data_ptr(), rows * pieces
-    _took(e.mlb_beam_select(scores, tokens, parents, done_out, Address(logits.data_ptr()), prev, done, part, Address(base + 8 * n), Address(base + 8 * n + 8 * n * K),
+    _took(e.mlb_beam_select(scores, tokens, parents, done_out, Address(logits.data_ptr()), prev, done, part, Address(base + 8 * n), Address(base + 8 * n + 4 * n * (2 * K + 1)),
                               ticket, rows, K, V, logits.stride(0), eos, bits), "beam_select")
 
 

@@ -537,6 +537,76 @@ def test_beam_select_of_pieces_that_are_fetched_in_parts(dtype, B, K, V, stride)
     check_choice(logits, prev, done, 7, stride=stride)
 
 
+def rounded_scores(logits, prev, done, eos, lse_by=1.0):
+    """Scores as 32-bit numbers, prev + (logit - lse) rounded operation by operation; lse from 64 bits, off by a factor."""
+    B, K = prev.shape
+    z = logits.float().view(B, K, -1)
+    lse = torch.logsumexp(z.double(), -1, keepdim=True)
+    s = prev[..., None] + (z - (lse * lse_by).float())
+    s = torch.where((done != 0)[..., None], torch.where(torch.arange(z.shape[-1]) == eos, prev[..., None], -math.inf), s)
+    return s.view(B, -1)
+
+
+def check_ties(logits, prev, done, eos, stride=0):
+    """The choice is that of the plain form, to the index: the largest 32-bit scores, equal ones by the lowest index.  (Inputs whose choice does not hang on a logarithm
+    that is off by a few of its last bits.)"""
+    B, K = prev.shape
+    V = logits.shape[1]
+    order = [torch.sort(rounded_scores(logits, prev, done, eos, 1 + e * 2.0 ** -22), dim=1, descending=True, stable=True).indices[:, :K] for e in (0, -2, -1, 1, 2)]
+    assert all(torch.equal(order[0], o) for o in order[1:])
+    plain = torch.empty(B, K), *(torch.empty(B, K, dtype=I32) for _ in range(3))
+    ref.beam_select(*plain, logits, prev, done, eos)
+    s, t, p, e = choose(logits, prev, done, eos, stride=stride)
+    assert torch.equal(plain[2].long() * V + plain[1], order[0])
+    assert torch.equal(p.long() * V + t, order[0]) and torch.equal(e, plain[3])
+
+
+@pytest.mark.parametrize("B,K,V,stride", [(1, 1, 1000, 0), (2, 4, 3000, 0), (1, 4, 50304, 0), (3, 20, 9001, 1), (1, 32, 50304, 0), (40, 3, 20000, 0), (2, 16, 70001, 7)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("near", [3, 40, 900])
+def test_beam_select_of_scores_that_rounding_makes_equal(dtype, B, K, V, stride, near):
+    """Logits that differ, `near` of them so little beside a beam's large score that theirs are equal: the lowest indices, not the largest logits."""
+    g = torch.Generator().manual_seed(V + K + near)
+    logits = torch.full((B * K, V), -5.0)
+    for r in range(B * K):
+        at = torch.randperm(V, generator=g)[:near]
+        step = 2.0 ** -26 if dtype == torch.bfloat16 else 2.0 ** -23
+        logits[r, at] = (2.0 ** -12 if dtype == torch.bfloat16 else 1.0) + step * (128 // 8 if dtype == torch.bfloat16 else 1) * torch.randperm(near, generator=g) % 2.0 ** -11
+    logits = logits.to(dtype)
+    prev, done = torch.full((B, K), -20000.0), torch.zeros(B, K, dtype=I32)
+    check_ties(logits, prev, done, 7, stride)
+    prev[:, 1:] = -math.inf
+    check_ties(logits, prev, done, 7, stride)
+    prev[:, 1:] = -20000.0
+    done[:, K // 2:] = 1
+    check_ties(logits, prev, done, V - 1, stride)
+
+
+@pytest.mark.parametrize("K,V", [(16, 70001), (9, 150000), (32, 70001), (4, 400000)])
+@pytest.mark.parametrize("live", [1, 4])
+def test_beam_select_of_two_logits_with_one_score(K, V, live):
+    """A few of the larger logit behind many of the smaller one, all in what is fetched first: candidates that go when room is made for the next part are as good as what stays.
+    (The next smaller bf16 number has another score: the counts of logits at 0 put a boundary of rounding below the two.)"""
+    hi, lo, unit = 1 + 2.0 ** -7, 1.0, 2.0 ** -6      # (scores of 2^17 ... 2^18 are multiples of 2^-6)
+    lse = lambda m: math.log(10 * math.exp(hi) + 60 * math.exp(lo) + m + (V - 70 - m) * math.exp(-5))
+    m = next(m for m in range(1000) if 0.55 < (lo - lse(m)) / unit % 1 < 0.65)
+    z = torch.full((K, V), -5.0)
+    z[:, V - m:] = 0.0
+    at = torch.randperm(4000, generator=torch.Generator().manual_seed(K))[:70].sort().values
+    z[:, at[:60]], z[:, at[60:]] = lo, hi
+    prev = torch.full((1, K), -math.inf)
+    prev[0, :live] = -150000.0
+    check_ties(z.bfloat16(), prev, torch.zeros(1, K, dtype=I32), 7)
+
+
+@pytest.mark.parametrize("B,K,V", [(2, 4, 50304), (1, 32, 50304), (4, 1, 30000), (2, 9, 12345)])
+def test_beam_select_of_random_logits_behind_large_scores(B, K, V):
+    """Random fp32 logits, scores some ten of which are equal at the top."""
+    torch.manual_seed(V + K)
+    logits = torch.randn(B * K, V) * 3
+    check_ties(logits, torch.full((B, K), -300000.0) - 0.25 * torch.arange(K), torch.zeros(B, K, dtype=I32), 3)
+
+
 def test_beam_select_in_a_graph():
     torch.manual_seed(1)
     z = torch.randn(8, 5000, device=dev()).bfloat16()
