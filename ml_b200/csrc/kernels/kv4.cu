@@ -331,8 +331,10 @@ __global__ void __launch_bounds__(512, 3) kv4_read_k(bf16* __restrict__ k, bf16*
 //      products, in fp32.  (The tensor core lines products up by their operands' nominal exponents, 2^-14 for a subnormal: a score is off by some 2^-16 of |q| s.)
 //   V: the same bits as bf16 numbers are c 2^-133 and 16 c 2^-133 (these reach into the exponent's last bit, and are counted on without a gap there), less 8 and 128
 //      of which all is exact and what is 0 adds 0: two instructions for two codes, a shift for eight.  For the products' sake the weights are 2^88 times what they are
-//      (a sum of 2^31 of them, each up to 2^8, still is a number), O is 2^-45 times: what a token adds below 2^-81 is lost.  With a scale of 2^31 and more a weight
-//      may pass bf16's range.  Then O is not finite, the warp sees it and goes over its blocks once more with codes as numbers of the size that they are.
+//      (a sum of 2^31 of them, each up to 2^8, still is a number), O is 2^-45 times: what a token adds below 2^-81 is lost, and with a scale of 2^31 and more a weight
+//      may pass bf16's range.  So a warp looks at its O.  Where that is not finite, or below 2^-50 in a group (zeros are, too), it goes over its blocks once more with codes as numbers of
+//      the size that they are, and O 2^-45 or 2^48 times.  Shares are averages times 2^-5 and the power of two that brings their sum of weights to 1 ... 2: the
+//      cache's smallest number, 2^-120, and its largest ones stay what they are.  (Beside elements above some 2^50, which 2^48 times would pass fp32's range, those below 2^-81 are lost.)
 //      The scale goes into P, in fp32 before its one rounding to bf16.  That rounding, 2^-8 of each weight at most and independent from token to token, is
 //      the only one on the way to O.  (Codes as 128 + c less 136 with the weights as they are, a shift for each two: 64 x 8192 tokens, below, 91 us instead of 79.  The
 //      8 or 128 taken off by a product with a constant was no faster, 82, and leaves 2^-24 of a weight where the code stands for 0.)
@@ -347,8 +349,8 @@ __global__ void __launch_bounds__(512, 3) kv4_read_k(bf16* __restrict__ k, bf16*
 //
 // Measured: 64 sequences of 1024 to 8192 tokens, 32 heads over 8 of 128: 79 us, 4.4 TB/s (67 % of the measured copy rate; 60 us with the arithmetic left out.  What is
 // missing is instructions, 306 a block, of which 146 go through the pipe of bitwise operations and shifts at half the rate, and that three warps an issue slot
-// leave 44 % of the slots empty).  16 sequences of up to 2048 tokens, 16 heads of 128: 20.7 us, of which some 9 are that arithmetic and 8 beginnings, ends and
-// the joining of shares.  One sequence of 1000 tokens, 12 heads of 64: 6.6 us, 1.4 of them an empty kernel's, 2.4 the joining (a counter, another block's
+// leave 44 % of the slots empty).  16 sequences of up to 2048 tokens, 16 heads of 128: 21.1 us, of which some 9 are that arithmetic and 8 beginnings, ends and
+// the joining of shares.  One sequence of 1000 tokens, 12 heads of 64: 6.8 us, 1.4 of them an empty kernel's, 2.4 the joining (a counter, another block's
 // results).  12 warps an SM: 8 are 4 to 8 % slower, 16 (of 128 registers, with places of 32 tokens) 79 -> 85.
 struct AttnArgs {
   bf16* out;
@@ -440,14 +442,17 @@ template <int HD, int NT> struct Queries {      // of a thread block's query row
   float back[NT][8];                 // score of a column = back * product
 };
 
-// Weights are 2^UP times what they are, so that with the values' codes as subnormal numbers, c 2^-133 (of odd elements 16 times that), O is VALUE times what it is
-constexpr float UP = 88.f, BACK_DOWN = 3.23117426778526e-27f;      // 2^-88
-constexpr float VALUE = 2.8421709430404007e-14f, BACK_EVEN = 35184372088832.f, BACK_ODD = 2199023255552.f;      // 2^(88 - 133), its inverse, a 16th of that
+// Weights are 2^UP times what they are, so that with the values' codes as subnormal numbers, c 2^-133 (of odd elements 16 times that), O is 2^-45 times what it is
+constexpr float UP = 88.f;
+// With codes as they are: weights times this, and O is 2^-45 or 2^48 times what it is (in two factors: one would be subnormal)
+struct Size { float a, b; };
+__device__ __forceinline__ Size size_for(bool large) { return large ? Size{3.23117426778526e-27f, 2.8421709430404007e-14f} : Size{9.094947017729282e-13f, 1.f}; }      // 2^-88 2^-45, 2^-40
+constexpr int SHARE = -5;      // shares' O is 2^SHARE times an average
 
-// NB blocks of 16 tokens, one behind the other.  first: their first token; seen[n][c]: tokens that column c sees, asked only where MASKED.  WIDE: scales of 2^31 and more
+// NB blocks of 16 tokens, one behind the other.  first: their first token; seen[n][c]: tokens that column c sees, asked only where MASKED.  WIDE: codes as they are
 template <int HD, int NT, int NB, bool MASKED, bool WIDE>
 __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q, const float (&c)[NT][2], const uint8_t* blk, int first,
-                                       const int (&seen)[NT][2], int i, int j) {
+                                       const int (&seen)[NT][2], Size size, int i, int j) {
   using L = Block<HD>;
   constexpr int NG = L::NG;
   // Row x of the products is token x ^ (x / 2 & 1): the tokens whose values a lane reads are then of both parities in each load, half the conflicts
@@ -558,7 +563,7 @@ __device__ __forceinline__ void attend(Rows<HD, NT>& r, const Queries<HD, NT>& q
       for (int n = 0; n < NT; n++) {
         float p[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) p[k] = (WIDE ? y[b][n][k] * BACK_DOWN * VALUE : y[b][n][k]) * (k < 2 ? sa[g] : sb[g]);
+        for (int k = 0; k < 4; k++) p[k] = (WIDE ? y[b][n][k] * size.a * size.b : y[b][n][k]) * (k < 2 ? sa[g] : sb[g]);
         if constexpr (MASKED) {      // (a scale that is not seen may be anything)
 #pragma unroll
           for (int k = 0; k < 4; k++)
@@ -649,11 +654,10 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
     const int u0 = (int)(s - item0), u1 = min((int)(min(e, item1) - item0), blocks);
     auto token = [&](int r) { return (int)(((float)r + 0.5f) * A.inv_g); };      // r / G (exact: r < 2^20)
     auto finish = [&](int r, int d, float m, float l, const float4& o) {         // elements 4 d ... of row r, whole
-      l *= BACK_DOWN;
       const int tok = token(row0 + r), head = (int)kv * A.G + row0 + r - tok * A.G;
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (nothing seen: zeros; NaN stays)
+      const float inv = l > 0.f ? (float)(1 << -SHARE) / l : (l == 0.f ? 0.f : l);      // (nothing seen: zeros; NaN stays)
       bf16* out = A.out + ((long)b * A.Tq + tok) * A.G * A.Hkv * HD + (long)head * HD + 4 * d;
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv * BACK_EVEN, o.y * inv * BACK_ODD), pack_bf16(o.z * inv * BACK_EVEN, o.w * inv * BACK_ODD));
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
       if (d == 0 && A.lse != nullptr)
         A.lse[((long)b * A.G * A.Hkv + head) * A.Tq + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
     };
@@ -759,7 +763,7 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; n++) c[n][0] = q.back[n][2 * j], c[n][1] = q.back[n][2 * j + 1];
-    auto walk = [&](auto wide) {
+    auto walk = [&](auto wide, Size size) {
       constexpr bool WIDE = decltype(wide)::value;
       int k = 0;
 #pragma unroll 1
@@ -776,11 +780,11 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
 #pragma unroll 1
         for (int x = 0; x < STEP; x += 2) {
           if (!WIDE && (oks >> x & 3) == 3 && (u + x + 2) * TOK <= all) {
-            attend<HD, NT, 2, false, false>(acc, q, c, blk + x * L::BYTES, (u + x) * TOK, seen, i, j);
+            attend<HD, NT, 2, false, false>(acc, q, c, blk + x * L::BYTES, (u + x) * TOK, seen, size, i, j);
           } else {
 #pragma unroll 1
             for (int y = x; y < x + 2; y++)
-              if (oks >> y & 1) attend<HD, NT, 1, true, WIDE>(acc, q, c, blk + y * L::BYTES, (u + y) * TOK, seen, i, j);
+              if (oks >> y & 1) attend<HD, NT, 1, true, WIDE>(acc, q, c, blk + y * L::BYTES, (u + y) * TOK, seen, size, i, j);
           }
         }
         __syncwarp();
@@ -788,20 +792,51 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
         k = k + 1 == NST ? 0 : k + 1;
       }
     };
+    bool small = false;
     if (some && !dead) {
-      walk(std::false_type());
-      // A scale of 2^31 or more may have made a weight infinite, and then it made all rows of the group's O infinite or NaN: once more, slower
-      float x = 0.f;
+      walk(std::false_type(), Size{});
+      // A scale of 2^31 or more may have made a weight infinite, and then it made all rows of the group's O infinite or NaN.  What is tiny or 0 may be so because it was lost.
+      // First a look at one element in two, whose numbers without their signs lie in one range if all is well
+      constexpr uint32_t LOW = 32u << 24, HIGH = 255u << 24;      // 2^-95 (O of 2^-50), infinity
+      uint32_t far = 0;
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int g = 0; g < NG; g++) x = fmaf(acc.o[n][2 * g][0], 0.f, fmaf(acc.o[n][2 * g][1], 0.f, x));
-      if (!dead && __any_sync(0xffffffffu, x != 0.f)) {
-        clear();
-        tc::fence_async_smem();
-        __syncwarp();
-        begin();
-        walk(std::true_type());
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) far = max(far, 2u * __float_as_uint(acc.o[n][2 * g][h]) - LOW);
+      if (__any_sync(0xffffffffu, far >= HIGH - LOW)) {
+        auto endless = [&] {
+          float x = 0.f;
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int g = 0; g < NG; g++) x = fmaf(acc.o[n][2 * g][0], 0.f, fmaf(acc.o[n][2 * g][1], 0.f, x));
+          return __any_sync(0xffffffffu, x != 0.f) != 0;
+        };
+        uint32_t least = ~0u;      // of the largest of the four elements that a thread has of a group
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+              uint32_t top = 0;
+#pragma unroll
+              for (int e = 0; e < 4; e++) top = max(top, 2u * __float_as_uint(acc.o[n][2 * g + e / 2][h + e % 2 * 2]));
+              if (acc.m[n][h] > -INFINITY) least = min(least, top);
+            }
+        bool large = endless();
+        small = !large && __any_sync(0xffffffffu, least < LOW);
+        while (!dead && (large || small)) {
+          clear();
+          tc::fence_async_smem();
+          __syncwarp();
+          begin();
+          walk(std::true_type(), size_for(large));
+          if (large || !endless()) break;
+          large = true, small = false;
+        }
       }
     }
     // ---- the warps' shares put together (in the rings' memory, which nothing is on its way to)
@@ -815,12 +850,16 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         const int col = 8 * n + 2 * j + h;
-        if (i == 0) mine[col] = acc.m[n][h], mine[R + col] = l;
+        // l is 2^UP times the sum of weights (88 + 127 is 1's exponent): the power of two that brings it to 1 ... 2 goes to m, and with those of O and of the share into the factor
+        const int ex = min(max((int)(__float_as_uint(l) >> 23), 200), 253);
+        const float even = __uint_as_float((uint32_t)(127 + 215 + SHARE + (small ? -48 : 45) - ex) << 23), odd = even * 0.0625f;
+        l *= __uint_as_float((uint32_t)(254 - ex) << 23);
+        if (i == 0) mine[col] = acc.m[n][h] + (float)(ex - 215), mine[R + col] = l;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
           if (col < live)
             *reinterpret_cast<float4*>(mine + 2 * R + col * HD + 32 * g + 4 * i) =
-                make_float4(acc.o[n][2 * g][h], acc.o[n][2 * g][h + 2], acc.o[n][2 * g + 1][h], acc.o[n][2 * g + 1][h + 2]);
+                make_float4(acc.o[n][2 * g][h] * even, acc.o[n][2 * g][h + 2] * odd, acc.o[n][2 * g + 1][h] * even, acc.o[n][2 * g + 1][h + 2] * odd);
         }
       }
     __syncthreads();

@@ -232,7 +232,10 @@ def kv4_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale=None):
     """Attention of the newest Tq tokens of every sequence over its cached keys and values.  q, out [B Tq, H hd]; table int32 [B, pages of a sequence] has the
     page numbers of a sequence's tokens in order, lens int32 [B] how many tokens it has, the Tq newest (already appended) among them: query token i
     sees the tokens before lens - Tq + i + 1.  Every key / value head serves H / Hkv consecutive query heads; scale: 1 / sqrt(hd).  A query
-    that sees nothing gets zeros.  (The kernel loses what a token adds below 2^-81.)  lse fp32 [B, H, Tq] (or None): log of the sum of the exponentials, -inf where nothing is seen."""
+    that sees nothing gets zeros.  lse fp32 [B, H, Tq] (or None): log of the sum of the exponentials, -inf where nothing is seen.
+
+    The kernel adds up in 32 bits.  It rounds to fewer: weights times values' scales to bf16, once, and of queries what lies below 2^-23 of a row's largest element; a score
+    is off by some 2^-16 of max |q| times a scale.  Values of any size that the cache holds come out, but those below 2^-81 beside others above 2^50."""
     n, page, B = check_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale)
     scale = 1.0 / math.sqrt(hd) if scale is None else scale
     G = H // Hkv

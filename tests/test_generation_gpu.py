@@ -310,6 +310,38 @@ def test_attention_over_values_of_any_size(hd, size, T, Tq, H):
     close(out.cpu().double().numpy().reshape(o.shape), lse.cpu().double().numpy(), o, l, tol, ltol)
 
 
+@pytest.mark.parametrize("hd,size", [(32, 1e-22), (64, 1e-25), (96, 1e-30), (128, 1e-33), (64, 1e-33)])
+@pytest.mark.parametrize("T,Tq,H", [(1, 1, 2), (16, 1, 4), (700, 1, 4), (90, 5, 8), (3000, 20, 4)])
+@pytest.mark.parametrize("part", ["all", "group", "tokens"])
+def test_attention_over_tiny_values(hd, size, T, Tq, H, part):
+    """What the cache holds reaches the output, whatever its size: all values, those of one group of 32 beside ordinary ones, those of the first tokens.  (Held to the bound
+    of the elements themselves; a scale's smallest number is 2^-120, half of what adding up may lose.)"""
+    torch.manual_seed(hd + T)
+    Hkv, page, n = 2, 32, -(-T // 32)
+    pages, table, slots = torch.zeros(n, Hkv, page // 16, 18 * hd, dtype=torch.uint8, device=dev()), torch.randperm(n), torch.arange(T)
+    qkv = torch.randn(T, 2 * Hkv * hd)
+    v = qkv[:, Hkv * hd:].view(T, Hkv, hd)
+    (v if part == "all" else v[:, 1, -32:] if part == "group" else v[:T // 3]).mul_(size)
+    ops.kv4_append(pages, None, qkv.bfloat16().to(dev()), (table[slots // page] * page + slots % page).int().to(dev()), None, None, None, 0, Hkv, hd)
+    q = torch.randn(Tq, H * hd).bfloat16()
+    out, lse = torch.empty(Tq, H * hd, dtype=torch.bfloat16, device=dev()), torch.empty(1, H, Tq, device=dev())
+    ops.kv4_attn(out, lse, q.to(dev()), pages, ints(table[None].tolist()), ints([T]), Tq, H, Hkv, hd)
+    o, l, tol, ltol = oracle.attention(q, pages.cpu(), table[None].numpy(), [T], Tq, H, Hkv, hd)
+    close(out.cpu().double().numpy().reshape(o.shape), lse.cpu().double().numpy(), o, l, tol, ltol)
+
+
+def test_attention_over_values_that_are_zero():
+    """Exact zeros stay zeros."""
+    hd, T = 64, 90
+    pages = torch.zeros(3, 1, 2, 18 * hd, dtype=torch.uint8, device=dev())
+    kv = torch.randn(T, 2 * hd, device=dev()).bfloat16()
+    kv[:, hd:] = 0
+    ops.kv4_append(pages, None, kv, ints(list(range(T))), None, None, None, 0, 1, hd)
+    out = torch.full((1, hd), 7.0, dtype=torch.bfloat16, device=dev())
+    ops.kv4_attn(out, None, torch.randn(1, hd, device=dev()).bfloat16(), pages, ints([[0, 1, 2]]), ints([T]), 1, 1, 1, hd)
+    assert bool((out == 0).all())
+
+
 def test_cache_past_4_gigabytes():
     """Pages whose bytes lie past 2^32, written, read and attended to."""
     hd, page, Hkv = 128, 128, 8
