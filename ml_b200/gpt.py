@@ -779,7 +779,7 @@ def mode_export(argv):
 
 
 def mode_generate(argv):
-    """`generate --ckpt-dir DIR [--step N] --prompt "12 7 99" [--n 32] [--temperature 0] [--top-k 0] [--seed 0] [--kv 4bit [--beams 4 [--eos ID]
+    """`generate --ckpt-dir DIR [--step N] --prompt "12 7 99" [--n 32] [--temperature 0] [--top-k 0] [--seed 0] [--eos ID] [--kv 4bit [--beams 4
     [--length-penalty 0]] [--page 64]]`: loads the fp32 master weights of a checkpoint written by `train` (model shape from the ENTROPY_* variables, as there) and
     prints the prompt's continuation as token ids (this package has no tokenizer).  Not a mode of the reference."""
     import argparse
@@ -797,7 +797,7 @@ def mode_generate(argv):
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--kv", choices=("4bit",), default=None, help="keys and values cached in 4 bits instead of a pass over the window for each token")
     ap.add_argument("--beams", type=int, default=1)
-    ap.add_argument("--eos", type=int, default=-1, help="token that ends a beam")
+    ap.add_argument("--eos", type=int, default=-1, help="token that ends a continuation")
     ap.add_argument("--length-penalty", type=float, default=0.0)
     ap.add_argument("--page", type=int, default=64, help="tokens of a page of the cache")
     a = ap.parse_args(argv)

@@ -480,23 +480,27 @@ class GPT:
         new token is one forward over the whole window (there is no key / value cache - this is a way to look at what a
         checkpoint has learnt, not a serving path), the window slides once it is full.  temperature 0 = greedy; else
         softmax sampling at that temperature, over the `top_k` most likely tokens if top_k > 0, from a generator seeded
-        with `seed`.  The reference has no sampling mode; needs materialised logits (no chunked LM head).
+        with `seed`.  A row that has chosen `eos` (-1: none) is filled up with it.  The reference has no sampling mode; needs materialised
+        logits (no chunked LM head).
 
         kv="4bit": keys and values are cached in 4 bits, in pages of `page` tokens (ml_b200.models.generation): a token costs one pass over itself, any
         number of prompts, P + n_new within the window.  beams > 1 (with the cache): the most likely of `beams` continuations that are
-        carried along, ended by `eos` (-1: never) and compared by log-probability / length ** length_penalty."""
+        carried along, ended by `eos` and compared by log-probability / length ** length_penalty (one alone is compared with nothing).  Raises what
+        its kernels report."""
         c = self.cfg
         b, P = prompt.shape
         gen = torch.Generator(device="cpu").manual_seed(seed)
 
-        def choose(logits):
+        def choose(logits, new):
             if temperature <= 0:
-                return logits.argmax(-1)
-            logits = logits / temperature
-            if top_k > 0:
-                kth = logits.topk(min(top_k, c.V), dim=-1).values[:, -1:]
-                logits = logits.masked_fill(logits < kth, float("-inf"))
-            return torch.multinomial(torch.softmax(logits, -1).cpu(), 1, generator=gen).view(-1).to(self.device)
+                nxt = logits.argmax(-1)
+            else:
+                logits = logits / temperature
+                if top_k > 0:
+                    kth = logits.topk(min(top_k, c.V), dim=-1).values[:, -1:]
+                    logits = logits.masked_fill(logits < kth, float("-inf"))
+                nxt = torch.multinomial(torch.softmax(logits, -1).cpu(), 1, generator=gen).view(-1).to(self.device)
+            return nxt if eos < 0 else torch.where((new == eos).any(-1), eos, nxt)
 
         if kv not in (None, "4bit"):
             raise ValueError(f"kv={kv!r}: None or '4bit'")
@@ -521,7 +525,7 @@ class GPT:
             n = ctx.shape[1]
             ids.zero_()
             ids[:, :n] = ctx.to(torch.int32)       # positions past n hold padding: causal attention keeps it out of row n - 1
-            nxt = choose(self.forward(ids.view(-1), B=b).view(b, c.T, c.V)[:, n - 1].float())
+            nxt = choose(self.forward(ids.view(-1), B=b).view(b, c.T, c.V)[:, n - 1].float(), out[:, P:])
             out = torch.cat([out, nxt.view(b, 1)], dim=1)
         return out
 

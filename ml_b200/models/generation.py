@@ -124,14 +124,14 @@ class CachedDecoder:
 
 @torch.no_grad()
 def sample(gpt, prompt, n_new, choose, page=64):
-    """`prompt` [b, P] and n_new tokens more, the next one of every row by choose(logits fp32 [b, V]) -> int64 [b]."""
+    """`prompt` [b, P] and n_new tokens more, the next one of every row by choose(logits fp32 [b, V], new tokens so far) -> int64 [b]."""
     b, P = prompt.shape
     m = CachedDecoder(gpt, b, P + n_new, page)
     out = prompt.to(m.dev).long()
     slots, _, _ = m.cache.grow(torch.full((b,), P, dtype=torch.int32, device=m.dev), b * P)
     logits = m.prompt(out.int(), slots)
     for k in range(n_new):
-        nxt = choose(logits.float())
+        nxt = choose(logits.float(), out[:, P:])
         out = torch.cat([out, nxt.view(b, 1)], dim=1)
         if k + 1 < n_new:
             logits = m.step(nxt.int())

@@ -313,6 +313,26 @@ def test_an_error_word_is_raised_in_words_and_cleared(monkeypatch):
     native.raise_error("generation")
 
 
+@pytest.mark.parametrize("kv", [None, "4bit"])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_eos_ends_a_single_continuation_too(kv, temperature):
+    """What follows the first eos is eos, and what stands before it is what comes without one."""
+    g = small()
+    torch.manual_seed(4)
+    prompt = torch.randint(0, 50, (2, 12))
+    kw = dict(kv=kv, temperature=temperature, seed=6)
+    free = g.generate(prompt, 20, **kw)
+    eos = int(free[0, 16])
+    ended = g.generate(prompt, 20, eos=eos, **kw)
+    for r, (a, b) in enumerate(zip(free[:, 12:].tolist(), ended[:, 12:].tolist())):
+        n = a.index(eos) if eos in a else 20
+        assert b[:n] == a[:n] and set(b[n:]) <= {eos}, r
+    assert not torch.equal(free, ended) or set(free[0, 16:].tolist()) == {eos}
+    assert torch.equal(g.generate(prompt, 20, **kw), free)
+    if kv and not temperature:
+        assert torch.equal(generation.beam_search(g, prompt, 20, 1, eos=eos)[0][:, 0], ended)
+
+
 def test_generate_refuses_what_the_cache_has_not():
     g = small()
     p = torch.zeros(1, 10, dtype=torch.long)
