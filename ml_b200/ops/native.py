@@ -238,7 +238,9 @@ def read_errors_async(host_words: torch.Tensor):
         fn = getattr(L, "mlb_read_error_async_" + tag)
         fn.argtypes = [_vp, _vp]
         fn.restype = _i32
-        _chk(fn(base + 4 * i, _st()), "read_error_async")
+        rc = fn(base + 4 * i, _st())
+        if rc != 0:
+            raise RuntimeError(f"read_error_async failed: code {rc} ({_cuda_err(rc)})")
 
 
 def clear_error():

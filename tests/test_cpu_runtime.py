@@ -663,3 +663,17 @@ def test_a_step_copies_the_error_words_of_all_sources_of_kernels(monkeypatch):
     assert sorted(asked.values()) == [words.data_ptr() + 4 * i for i in range(words.numel())]
     with pytest.raises(ValueError):
         native.read_errors_async(words[:-1])
+
+
+def test_reading_the_error_words_counts_as_no_launch(monkeypatch):
+    """`LAUNCHES` is the number of kernels that a step launches; a copy is none."""
+    from ml_b200.ops import native
+    rc = [0]
+    monkeypatch.setattr(native, "lib", lambda: type("Lib", (), {"__getattr__": lambda self, name: type("Read", (), {"__call__": lambda self, at, stream: rc[0]})()})())
+    monkeypatch.setattr(native, "_st", lambda: 0)
+    before = native.LAUNCHES
+    native.read_errors_async(native.error_words(pinned=False))
+    assert native.LAUNCHES == before
+    rc[0] = 999
+    with pytest.raises(RuntimeError, match="read_error_async"):
+        native.read_errors_async(native.error_words(pinned=False))
