@@ -146,11 +146,13 @@ __global__ void __launch_bounds__(TAB_THREADS) block_tables_k(const TableArgs A)
 // is the bound from then on.  A candidate's place is the number of those before it.  More candidates at a time than there is room for (logits all alike) are forgotten:
 // then K rounds over the piece find its K largest.  The request's last thread block finds its K best among the pieces' lists in the same way,
 // the bound being of its threads' best.
-// 32 x 8 beams of 50304 bf16 logits, a quarter of them ended: 15.6 us (1.7 TB/s), of which fetching and the maximum 6.2, the exponentials 1, candidates and their
-// bound 2.6, the counters 1.9, the merge 3.4.  1 x 4 beams: 7.2 us (2.3, then 1 for the counters, 3.4 for the merge): latencies one behind the other.  fp32 logits: 1 x 4
+// 32 x 8 beams of 50304 bf16 logits, a quarter of them ended: 15.5 us (1.7 TB/s), of which fetching and the maximum 6.2, the exponentials 1, candidates and their
+// bound 2.6, the counters 1.9, the merge 3.4.  1 x 4 beams: 7.1 us (2.3, then 1 for the counters, 3.4 for the merge): latencies one behind the other.  fp32 logits: 1 x 4
 // beams 7.2, 32 x 8 with none ended 25.8 (bf16: 17.9), 8 x 32 44.6 (33.8).
 constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_BYTES = 32768, SEL_MAX_K = 32, SEL_CAND = 512, SEL_HELD = 1024;
-constexpr int SEL_PER_SM = 6, SEL_LEAST = 4096;      // thread blocks that an SM holds; the smallest piece
+// Thread blocks that an SM has registers for (shared memory leaves room for five whose fetches are whole 32 KB: counted as six, 256 rows of 50304 logits are four pieces a
+// row, 1024 blocks, of which 740 are resident at once); the smallest piece
+constexpr int SEL_PER_SM = 6, SEL_LEAST = 4096;
 typedef unsigned long long u64;
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -255,7 +257,8 @@ __device__ __forceinline__ X kth_of_parts(X m, int K, int parts, X* tops, Max la
   }
   return __shfl_sync(0xffffffffu, m, __ffs(__ballot_sync(0xffffffffu, better == K - 1)) - 1);
 }
-// Natural logarithm of a normal number, off by 2^-22 and a rounding: the exponent's part apart from that of a number of 1 ... 2
+// Natural logarithm of a normal number, off by 2^-22 and a rounding: the exponent's part apart from that of a number of 1 ... 2, ln 2 in two parts of which the first has
+// few bits, so that its multiples are exact (Cody and Waite, Software Manual for the Elementary Functions, 1980)
 __device__ __forceinline__ float log_of(float x) {
   const int e = (int)(__float_as_uint(x) >> 23) - 127;
   const float f = __uint_as_float((__float_as_uint(x) & 0x007FFFFFu) | 0x3F800000u);
