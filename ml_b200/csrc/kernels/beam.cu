@@ -369,18 +369,19 @@ __global__ void __launch_bounds__(SEL_THREADS, SEL_PER_SM) beam_select_k(const _
     const int parts = parts_for(K), N = K + 1;
     bool cut = false;
     int most = 0;      // candidates up to and with this thread's last
-    bool over = false;
+    bool over = false, late = false;
     uint32_t parity = 0;
     for (int c = 0; c < n; c += CHUNK, parity ^= 1) {
       const int count = min(CHUNK, n - c), whole = BULK ? (int)(count * sizeof(T) / 16 * 16 / sizeof(T)) : 0;
-      if (BULK && tid == 0 && whole > 0) {
+      if (BULK && tid == 0 && whole > 0 && !late) {
         tc::mbar_expect_tx(&bar, whole * sizeof(T));
         tc::bulk_load(data, z + c, whole * sizeof(T), &bar);
       }
       for (int e = whole + tid; e < count; e += SEL_THREADS) data[e] = z[c + e];
       if (tid < 8 && count + tid < (count + 7) / 8 * 8) data[count + tid] = (T)-INFINITY;
-      if (BULK && whole > 0) {
-        tc::mbar_wait(&bar, parity, 0xD3);
+      if (BULK && whole > 0 && !late && !__all_sync(0xffffffffu, tc::mbar_wait(&bar, parity, 0xD3))) {
+        late = true;      // nothing more is fetched, and what is on its way is waited for once more
+        tc::mbar_wait(&bar, parity, 0xD4);
         __syncwarp();
       }
       __syncthreads();

@@ -769,8 +769,8 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
 #pragma unroll 1
       for (int u = w0; u < w1; u += STEP) {
         if (!__all_sync(0xffffffffu, tc::mbar_wait(&bars[warp][k], parity >> k & 1, 0xD1))) {
-          dead = true;      // no more is fetched; what is on its way is waited for
-          for (int x = 1; x < NST && u + x * STEP < w1; x++) tc::mbar_wait(&bars[warp][(k + x) % NST], parity >> (k + x) % NST & 1, 0xD2);
+          dead = true;      // no more is fetched; what is on its way is waited for, the late one once more
+          for (int x = 0; x < NST && u + x * STEP < w1; x++) tc::mbar_wait(&bars[warp][(k + x) % NST], parity >> (k + x) % NST & 1, 0xD2);
           __syncwarp();
           break;
         }

@@ -105,3 +105,28 @@ def test_every_refused_index_has_its_words():
     details = {int(d, 16) for path in KERNELS.glob("*.cu*") for d in re.findall(r"MLB_ERR_BOUNDS, (0x[0-9A-Fa-f]+)\)", path.read_text())}
     assert 0xE1 in details
     assert not [hex(d) for d in details if describe_error(3 << 24 | d).endswith(f"detail {d:#x}")]
+
+
+def test_untiled_copies_on_their_way_are_waited_for_when_a_wait_has_run_out():
+    """A copy that is late still writes to shared memory.  Behind a wait that ran out all that is on its way is waited for, the late one as well, and nothing is fetched on
+    top of it."""
+    seen = set()
+    for file, name, body, _ in _kernels():
+        if "bulk_load(" not in body:
+            continue
+        waits = [m for m in WAIT.finditer(body) if "mbar_wait" in m.group(0)]
+        asked = [m for m in waits if list(_heads(body, m.start()))[0].rstrip().endswith("__all_sync(0xffffffffu,")]
+        assert len(asked) == 1 and len(waits) == 2, (file, name)      # the one whose answer decides, and the one behind it
+        again = body[asked[0].end():]
+        depth, end = 0, again.index("{")
+        for end in range(end, len(again)):
+            depth += {"{": 1, "}": -1}.get(again[end], 0)
+            if depth == 0:
+                break
+        block = again[again.index("{"):end]
+        assert "mbar_wait(" in block and re.search(r"\b(dead|late) = true;", block), (file, name)
+        loop = re.search(r"for \(int x = (\d)", block)
+        assert loop is None or loop.group(1) == "0", (file, name)
+        assert re.search(r"some && !dead|tid == 0 && whole > 0 && !late", body), (file, name)
+        seen.add(name)
+    assert seen == {"kv4_attn_k", "beam_select_k"}
