@@ -372,7 +372,7 @@ def run_ours(args):
         step = lambda i: tr.step()
         step_host = lambda i: tr.step_host(*h_in[i % pool])
         launches = lambda l0: tr.launches_per_step * args.steps if tr.use_graph else native.LAUNCHES - l0
-        d2h, api = 4 + 16, "ml_b200.trainer.Trainer.step_host"      # the loss, and the kernels' four error words read behind it
+        d2h, api = 4 + 4 * len(native._ERROR_WORDS), "ml_b200.trainer.Trainer.step_host"      # the loss, and the kernels' error words read behind it
         fl = flops_per_step(cfg, B) * world * accum
         tokens = B * T * world * accum
         loss_fn = lambda: tr.loss()
