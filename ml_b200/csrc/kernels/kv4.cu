@@ -332,9 +332,10 @@ __global__ void __launch_bounds__(512, 3) kv4_read_k(bf16* __restrict__ k, bf16*
 //   V: the same bits as bf16 numbers are c 2^-133 and 16 c 2^-133 (these reach into the exponent's last bit, and are counted on without a gap there), less 8 and 128
 //      of which all is exact and what is 0 adds 0: two instructions for two codes, a shift for eight.  For the products' sake the weights are 2^88 times what they are
 //      (a sum of 2^31 of them, each up to 2^8, still is a number), O is 2^-45 times: what a token adds below 2^-81 is lost, and with a scale of 2^31 and more a weight
-//      may pass bf16's range.  So a warp looks at its O.  Where that is not finite, or below 2^-50 in a group (zeros are, too), it goes over its blocks once more with codes as numbers of
-//      the size that they are, and O 2^-45 or 2^48 times.  Shares are averages times 2^-5 and the power of two that brings their sum of weights to 1 ... 2: the
-//      cache's smallest number, 2^-120, and its largest ones stay what they are.  (Beside elements above some 2^50, which 2^48 times would pass fp32's range, those below 2^-81 are lost.)
+//      may pass bf16's range.  So a warp looks at its O.  Where that is not finite, or all of a group below 2^-50 (zeros are, too), it goes over its blocks once more with codes as
+//      numbers of the size that they are, and O 2^-45 or 2^48 times.  Shares are averages times 2^-5 and the power of two that brings their sum of weights to 1 ... 2: the
+//      cache's smallest number, 2^-120, and its largest ones stay what they are.  (What is below 2^-81 stays lost beside more than 2^-50 in its own
+//      group, and beside more than some 2^50, which 2^48 times would pass fp32's range, in any.)
 //      The scale goes into P, in fp32 before its one rounding to bf16.  That rounding, 2^-8 of each weight at most and independent from token to token, is
 //      the only one on the way to O.  (Codes as 128 + c less 136 with the weights as they are, a shift for each two: 64 x 8192 tokens, below, 91 us instead of 79.  The
 //      8 or 128 taken off by a product with a constant was no faster, 82, and leaves 2^-24 of a weight where the code stands for 0.)
@@ -796,16 +797,26 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
     if (some && !dead) {
       walk(std::false_type(), Size{});
       // A scale of 2^31 or more may have made a weight infinite, and then it made all rows of the group's O infinite or NaN.  What is tiny or 0 may be so because it was lost.
-      // First a look at one element in two, whose numbers without their signs lie in one range if all is well
+      // First a look at one element in four, then at all, whose numbers without their signs lie in one range if all is well (together they are below it only if each is)
       constexpr uint32_t LOW = 32u << 24, HIGH = 255u << 24;      // 2^-95 (O of 2^-50), infinity
-      uint32_t far = 0;
+      auto outside = [&](auto every) {
+        uint32_t far = 0;
 #pragma unroll
-      for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int g = 0; g < NG; g++)
+          for (int h = 0; h < 2; h++) {
+            uint32_t f = 0;
 #pragma unroll
-          for (int h = 0; h < 2; h++) far = max(far, 2u * __float_as_uint(acc.o[n][2 * g][h]) - LOW);
-      if (__any_sync(0xffffffffu, far >= HIGH - LOW)) {
+            for (int g = 0; g < NG; g++) {
+              uint32_t x = __float_as_uint(acc.o[n][2 * g][h]);
+              if constexpr (decltype(every)::value) x |= __float_as_uint(acc.o[n][2 * g][h + 2]) | __float_as_uint(acc.o[n][2 * g + 1][h]) | __float_as_uint(acc.o[n][2 * g + 1][h + 2]);
+              f = max(f, 2u * x - LOW);
+            }
+            if (acc.m[n][h] > -INFINITY) far = max(far, f);      // (a row that sees nothing here has zeros)
+          }
+        return __any_sync(0xffffffffu, far >= HIGH - LOW) != 0;
+      };
+      if (outside(std::false_type()) && outside(std::true_type())) {
         auto endless = [&] {
           float x = 0.f;
 #pragma unroll
@@ -814,7 +825,7 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
             for (int g = 0; g < NG; g++) x = fmaf(acc.o[n][2 * g][0], 0.f, fmaf(acc.o[n][2 * g][1], 0.f, x));
           return __any_sync(0xffffffffu, x != 0.f) != 0;
         };
-        uint32_t least = ~0u;      // of the largest of the four elements that a thread has of a group
+        uint32_t least = ~0u;      // of the groups' largest elements
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -824,6 +835,8 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM) kv4_attn_k(const AttnArgs 
               uint32_t top = 0;
 #pragma unroll
               for (int e = 0; e < 4; e++) top = max(top, 2u * __float_as_uint(acc.o[n][2 * g + e / 2][h + e % 2 * 2]));
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
               if (acc.m[n][h] > -INFINITY) least = min(least, top);
             }
         bool large = endless();

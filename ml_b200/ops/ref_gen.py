@@ -235,7 +235,8 @@ def kv4_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale=None):
     that sees nothing gets zeros.  lse fp32 [B, H, Tq] (or None): log of the sum of the exponentials, -inf where nothing is seen.
 
     The kernel adds up in 32 bits.  It rounds to fewer: weights times values' scales to bf16, once, and of queries what lies below 2^-23 of a row's largest element; a score
-    is off by some 2^-16 of max |q| times a scale.  Values of any size that the cache holds come out, but those below 2^-81 beside others above 2^50."""
+    is off by some 2^-16 of max |q| times a scale.  Values of any size that the cache holds come out, but what is below 2^-81 beside more than 2^-50 in its
+    group, or than 2^50 in another."""
     n, page, B = check_attn(out, lse, q, pages, table, lens, Tq, H, Hkv, hd, scale)
     scale = 1.0 / math.sqrt(hd) if scale is None else scale
     G = H // Hkv
