@@ -89,8 +89,19 @@ typedef std::optional<Tensor> Maybe;      // (an undefined tensor is no argument
   X(mlb_beam_select_pieces, int, (int, int, int, int))                                                                                              \
   X(mlb_beam_select, int, (float*, int*, int*, int*, const void*, const float*, const int*, float*, float*, int*, int*, int, int, int, long, int, int, St)) \
   X(mlb_beam_reorder, int, (uint8_t*, int*, int*, int*, const int*, const int*, const int*, const int*, const int*, const int*, int, long, int, int, int, int, int, int, int, St))
+// those of the experts of a mixture
+#define MLB_MOE(X)                                                                                                                             \
+  X(mlb_moe_route_part, long, (long, int))                                                                                                     \
+  X(mlb_moe_route, int, (void*, int*, float*, float*, const void*, const float*, long, long, int, int, int, int, int, int, float, int, int, St)) \
+  X(mlb_moe_route_bwd, int, (void*, const void*, const float*, const void*, const int*, long, long, int, int, int, int, float, int, int, St))  \
+  X(mlb_moe_plan_ints, long, (long, int, int))                                                                                                 \
+  X(mlb_moe_plan_rows, long, (long, int, int))                                                                                                 \
+  X(mlb_moe_plan, int, (int*, const int*, long, int, int, St))                                                                                 \
+  X(mlb_moe_fwd, int, (void*, void*, void*, void*, void*, const void*, const void*, const void*, const void*, const int*, long, long, int, int, int, int, int, St)) \
+  X(mlb_moe_bwd, int, (void*, void*, void*, void*, void*, void*, void*, void*, void*, const void*, const void*, const void*, const void*, const void*, const void*, const int*, long, long, \
+                       int, int, int, int, int, St))
 #define MLB_POINTER(name, ret, args) ret(*name) args = nullptr;
-struct Entries { MLB_ENTRIES(MLB_POINTER) MLB_GENERATION(MLB_POINTER) } K;
+struct Entries { MLB_ENTRIES(MLB_POINTER) MLB_GENERATION(MLB_POINTER) MLB_MOE(MLB_POINTER) } K;
 
 PyObject* address_type = nullptr;  // ops.native.Address
 PyObject* settings = nullptr;      // the Python module whose variables FUSED_ATTN_BWD and FUSED_ATTN_BWD_MAX_SCRATCH bound attn_bwd's workspace
@@ -560,6 +571,7 @@ template <typename R, typename... A> struct typed_call<R(A...)> {
   }
 MLB_ENTRIES(MLB_CALL)
 MLB_GENERATION(MLB_CALL)
+MLB_MOE(MLB_CALL)
 
 // ------------------------------------------------------------------ generation
 // The operators of ops/native_gen.py for contiguous tensors of exactly the sizes that belong together, outside a graph capture; whatever else comes is handed
@@ -750,6 +762,7 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   TORCH_CHECK(K.name != nullptr, p, " has no function " #name);
   MLB_ENTRIES(MLB_LOOKUP)
   MLB_GENERATION(MLB_LOOKUP)
+  MLB_MOE(MLB_LOOKUP)
   PyObject* address = PyObject_GetAttrString(module, "Address");
   if (!address) return nullptr;
   Py_XDECREF(address_type);
@@ -761,7 +774,7 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
-// signatures(), generation_signatures(): the entry points' parameters by name
+// signatures(), generation_signatures(), moe_signatures(): the entry points' parameters by name
 #define MLB_KINDS(name, ret, args) d[#name] = kinds_of(K.name);
 PyObject* py_signatures(PyObject*, PyObject*) {
   HANDLE_TH_ERRORS
@@ -777,13 +790,20 @@ PyObject* py_generation_signatures(PyObject*, PyObject*) {
   return d.release().ptr();
   END_HANDLE_TH_ERRORS
 }
+PyObject* py_moe_signatures(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  pybind11::dict d;
+  MLB_MOE(MLB_KINDS)
+  return d.release().ptr();
+  END_HANDLE_TH_ERRORS
+}
 
 #define MLB_FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 #define MLB_METHOD(name, ret, args) {#name, (PyCFunction)(void (*)(void))call_##name, METH_FASTCALL, nullptr},
 PyMethodDef methods[] = {MLB_FAST(linear), MLB_FAST(rmsnorm), MLB_FAST(layer_norm), MLB_FAST(swiglu), MLB_FAST(rope_causal_attention), MLB_FAST(bidir_attention),
                          MLB_FAST(cross_entropy), MLB_FAST(kv4_append), MLB_FAST(kv4_read), MLB_FAST(kv4_attn), MLB_FAST(block_tables), MLB_FAST(beam_select), MLB_FAST(beam_reorder),
-                         MLB_ENTRIES(MLB_METHOD) MLB_GENERATION(MLB_METHOD) {"bind", py_bind, METH_VARARGS, nullptr}, {"signatures", py_signatures, METH_NOARGS, nullptr},
-                         {"generation_signatures", py_generation_signatures, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+                         MLB_ENTRIES(MLB_METHOD) MLB_GENERATION(MLB_METHOD) MLB_MOE(MLB_METHOD) {"bind", py_bind, METH_VARARGS, nullptr}, {"signatures", py_signatures, METH_NOARGS, nullptr},
+                         {"generation_signatures", py_generation_signatures, METH_NOARGS, nullptr}, {"moe_signatures", py_moe_signatures, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mlb_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -8,6 +8,9 @@ Two options of the reference's prototype model configuration (csrc/include/model
 QKV biases, Qwen2.5 style) exist only here: `Decoder(cfg, n_kv_heads=..., qkv_bias=True)`.  K / V heads are repeated up
 to the H query heads by the kernel that rotates Q and K, so the attention kernels see the usual [B*T, 3C] layout; such a
 module has no flat-buffer counterpart (`from_flat` / `load_flat` are for the default architecture).
+
+`Decoder(cfg, experts=dict(n_experts=8, top_k=2, ...))` has a mixture of experts (`ml_b200.models.moe.MoE`, whose arguments these are; I is the configuration's
+unless given) for each layer's feed-forward part; the loss then has `aux_coef` times the blocks' balancing losses added.
 """
 from __future__ import annotations
 
@@ -19,10 +22,11 @@ from .. import ops
 from ..config import Config
 from ..layout import DecoderLayout
 from ..ops import autograd as F
+from .moe import MoE
 
 
 class Block(nn.Module):
-    def __init__(self, cfg: Config, dtype, device, n_kv_heads=None, qkv_bias=False):
+    def __init__(self, cfg: Config, dtype, device, n_kv_heads=None, qkv_bias=False, experts=None):
         super().__init__()
         C, I, H, hd = cfg.C, cfg.I, cfg.H, cfg.hd
         self.Hkv = H if n_kv_heads is None else int(n_kv_heads)
@@ -31,7 +35,12 @@ class Block(nn.Module):
         mk = lambda *s: nn.Parameter(torch.empty(*s, dtype=dtype, device=device))
         self.ln1, self.qkv, self.o = mk(C), mk((H + 2 * self.Hkv) * hd, C), mk(C, C)
         self.qkv_bias = nn.Parameter(torch.zeros((H + 2 * self.Hkv) * hd, dtype=dtype, device=device)) if qkv_bias else None
-        self.ln2, self.gate_up, self.down = mk(C), mk(2 * I, C), mk(C, I)
+        self.ln2 = mk(C)
+        self.moe = None
+        if experts is None:
+            self.gate_up, self.down = mk(2 * I, C), mk(C, I)
+        else:
+            self.moe = MoE(**{"C": C, "I": I, "device": device, "dtype": dtype, **experts})
         self.cfg = cfg
 
     def forward(self, x, cos, sin, B):
@@ -41,20 +50,24 @@ class Block(nn.Module):
         a = F.rope_causal_attention(qkv, cos, sin, B, c.T, c.H, c.hd, self.Hkv)
         x = x + F.linear(a, self.o)
         h = F.rmsnorm(x, self.ln2, c.eps)
+        if self.moe is not None:
+            y, self.aux = self.moe(h)
+            return x + y
         return x + F.linear(F.swiglu(F.linear(h, self.gate_up)), self.down)
 
 
 class Decoder(nn.Module):
-    def __init__(self, cfg: Config, device="cpu", dtype=None, n_kv_heads=None, qkv_bias=False):
+    def __init__(self, cfg: Config, device="cpu", dtype=None, n_kv_heads=None, qkv_bias=False, experts=None, aux_coef=0.01):
         super().__init__()
         cfg.validate()
-        self.flat_compatible = (n_kv_heads in (None, cfg.H)) and not qkv_bias
+        self.flat_compatible = (n_kv_heads in (None, cfg.H)) and not qkv_bias and experts is None
+        self.aux_coef = aux_coef
         device = torch.device(device)
         if dtype is None:
             dtype = torch.bfloat16 if device.type == "cuda" else torch.float32
         self.cfg = cfg
         self.wte = nn.Parameter(torch.empty(cfg.V, cfg.C, dtype=dtype, device=device))
-        self.blocks = nn.ModuleList([Block(cfg, dtype, device, n_kv_heads, qkv_bias) for _ in range(cfg.L)])
+        self.blocks = nn.ModuleList([Block(cfg, dtype, device, n_kv_heads, qkv_bias, experts) for _ in range(cfg.L)])
         self.lnf = nn.Parameter(torch.empty(cfg.C, dtype=dtype, device=device))
         self.lm = nn.Parameter(torch.empty(cfg.V, cfg.C, dtype=dtype, device=device))
         cos, sin = ops.rope_tables(cfg.T, cfg.hd, cfg.rope_theta, device)
@@ -80,7 +93,7 @@ class Decoder(nn.Module):
     @torch.no_grad()
     def load_flat(self, flat: torch.Tensor):
         if not self.flat_compatible:
-            raise ValueError("grouped-query / biased modules have no flat-buffer layout")
+            raise ValueError("grouped-query / biased modules and those with experts have no flat-buffer layout")
         for p, off in self.named_flat():
             p.copy_(flat[off:off + p.numel()].view(p.shape))
 
@@ -93,4 +106,7 @@ class Decoder(nn.Module):
         logits = F.linear(F.rmsnorm(x, self.lnf, c.eps), self.lm)
         if tgt is None:
             return logits
-        return F.cross_entropy(logits, tgt.view(-1))
+        loss = F.cross_entropy(logits, tgt.view(-1))
+        if self.blocks[0].moe is not None:
+            loss = loss + self.aux_coef * sum(b.aux for b in self.blocks)
+        return loss

@@ -14,6 +14,7 @@ _NAMES = [
     "linear_fwd", "linear_bias_fwd", "linear_dx", "linear_dw", "linear_dw_cast", "gemm", "attn_fwd", "attn_bwd",
     "attn_bidir_fwd", "attn_bidir_bwd", "layernorm_fwd", "layernorm_bwd", "layernorm_bwd_cast",
     "kv4_append", "kv4_read", "kv4_attn", "block_tables", "beam_select", "beam_reorder",
+    "moe_route", "moe_route_bwd", "moe_mlp", "moe_mlp_fwd", "moe_mlp_bwd",
     "ce_fwd_bwd", "ce_mean", "scale_dev", "ce_chunk_stats", "ce_chunk_grad", "adamw", "patchify", "add_posembed", "posembed_grad", "residual_add", "cast", "fp8_qdq", "sum_scale", "zero_",
 ]
 

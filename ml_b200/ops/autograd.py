@@ -9,6 +9,7 @@ backward kernels need.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -203,6 +204,56 @@ class Embedding(torch.autograd.Function):
         return dw.to(ctx.dtype), None, None
 
 
+class MoERoute(torch.autograd.Function):
+    """logits [N, E] -> weights [N, k], idx int32 [N, k], mean fp32 [E] (ops/ref_moe.py has what they are).  The choice has no gradient, and neither has the bias."""
+
+    @staticmethod
+    def forward(ctx, logits, k, bias, score, groups, top_groups, renorm, scale, dtype):
+        N, E = logits.shape
+        weights, idx = _like(logits, N, k, dtype=dtype), _like(logits, N, k, dtype=torch.int32)
+        mean = _like(logits, E, dtype=torch.float32)
+        ops.moe_route(weights, idx, mean, logits, bias, score, groups, top_groups, renorm, scale)
+        ctx.save_for_backward(logits, idx)
+        ctx.how = (score, renorm, scale)
+        ctx.dtype = dtype
+        ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)
+        return weights, idx, mean
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dweights, _, dmean):
+        logits, idx = ctx.saved_tensors
+        if dweights is None and dmean is None:
+            return (None,) * 9
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dweights = torch.zeros(idx.shape, dtype=ctx.dtype, device=logits.device) if dweights is None else dweights.contiguous()
+        ops.moe_route_bwd(dlogits, dweights, None if dmean is None else dmean.contiguous(), logits, idx, *ctx.how)
+        return (dlogits,) + (None,) * 8
+
+
+class MoEMLP(torch.autograd.Function):
+    """x [N, C] through the experts idx [N, k] with weights [N, k]: sum_j w_nj down[e] (silu(gate) * up), [gate | up] = gate_up[e] x_n (ops/ref_moe.py)."""
+
+    @staticmethod
+    def forward(ctx, x, weights, idx, gate_up, down):
+        weights, idx, gate_up, down = weights.contiguous(), idx.contiguous(), gate_up.contiguous(), down.contiguous()
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        saved = ops.moe_mlp_fwd(out, x, weights, idx, gate_up, down)
+        ctx.save_for_backward(x, weights, idx, gate_up, down, *saved)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, weights, idx, gate_up, down, *saved = ctx.saved_tensors
+        new = lambda t, wanted=True: torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None
+        need = ctx.needs_input_grad
+        dx, dweights, dgate_up, ddown = new(x, need[0]), new(weights), new(gate_up, need[3]), new(down, need[4])
+        ops.moe_mlp_bwd(dx, dweights, dgate_up, ddown, dout.contiguous(), x, weights, idx, gate_up, down, saved)
+        return dx, dweights if need[1] else None, None, dgate_up, ddown
+
+
 # What programs call.  Plain calls on CUDA tensors go through the extension module (csrc/torch/bridge.cpp), which runs the same kernels
 # on the same saved tensors without the interpreter; it declines what is not plain, and that takes the Functions above.
 def _plain(name, x, *args):
@@ -248,3 +299,18 @@ def layer_norm(x, w, b, eps):
 
 
 embedding = Embedding.apply
+
+
+def moe_route(logits, k, bias=None, score="softmax", groups=1, top_groups=1, renorm=True, scale=1.0, dtype=None):
+    """(weights [N, k], idx int32 [N, k], mean fp32 [E]): each token's k experts, best first, their weights in `dtype` (None: that of the logits), and the experts' mean
+    probabilities, from which a loss that balances them is formed.  ops/ref_moe.py says what they are."""
+    return MoERoute.apply(logits, k, bias, score, groups, top_groups, renorm, scale, dtype or logits.dtype)
+
+
+def moe_mlp(x, weights, idx, gate_up, down):
+    """x [N, C] through the SwiGLU experts gate_up [E, 2 I, C], down [E, C, I] that `moe_route` chose, weighted and added up."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weights, gate_up, down)):
+        return MoEMLP.apply(x, weights, idx, gate_up, down)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    ops.moe_mlp(out, x, weights.contiguous(), idx.contiguous(), gate_up.contiguous(), down.contiguous())
+    return out

@@ -46,10 +46,14 @@ _GEN_KINDS = {
     "kv4_append": "ubbiifflnllnnnns", "kv4_read": "bbuilnlnns", "kv4_attn_scratch": "nnnnnnn", "kv4_attn": "bfbuiifillnnnnnnnds",
     "block_tables": "iiiiiiiiiiinnnnns", "beam_select_pieces": "nnnn", "beam_select": "fiiibfiffiinnnlnns",
     "beam_reorder": "uiiiiiiiiinlnnnnnnns"}
+# ... and those of the experts of a mixture (ops/native_moe.py)
+_MOE_KINDS = {
+    "moe_route_part": "ln", "moe_route": "biffbfllnnnnnndnns", "moe_route_bwd": "bbfbillnnnndnns", "moe_plan_ints": "lnn", "moe_plan_rows": "lnn", "moe_plan": "iilnns",
+    "moe_fwd": "bbbbbbbbbillnnnnns", "moe_bwd": "bbbbbbbbbbbbbbbillnnnnns"}
 _CTYPES = {"n": _i32, "l": _i64, "d": _f32}      # (else a pointer)
 
 
-_ERROR_WORDS = ("gemm", "attn", "elementwise", "comm", "kv4", "beam")      # one of each source of kernels
+_ERROR_WORDS = ("gemm", "attn", "elementwise", "comm", "kv4", "beam", "moe")      # one of each source of kernels
 
 
 @lru_cache(maxsize=1)
@@ -94,12 +98,13 @@ def lib():
         "mlb_cast_bf16_fp8": [_vp, _vp, _i64, _f32, _vp],
         "mlb_adamw_fp8": [_vp] * 6 + [_i64] + [_f32] * 9 + [_vp, _vp],
     }
-    sig.update({"mlb_" + name: [_CTYPES.get(k, _vp) for k in kinds] for name, kinds in {**_KINDS, **_GEN_KINDS}.items()})
+    sig.update({"mlb_" + name: [_CTYPES.get(k, _vp) for k in kinds] for name, kinds in {**_KINDS, **_GEN_KINDS, **_MOE_KINDS}.items()})
     for name, args in sig.items():
         fn = getattr(L, name)
         fn.argtypes = args
         fn.restype = _i32
     L.mlb_attn_bwd_scratch_bytes.restype = L.mlb_kv4_attn_scratch.restype = _i64
+    L.mlb_moe_route_part.restype = L.mlb_moe_plan_ints.restype = L.mlb_moe_plan_rows.restype = _i64
     L.mlb_capture_id.restype = C.c_ulonglong
     for tag in _ERROR_WORDS:
         for pre in ("mlb_get_error_", "mlb_clear_error_"):
@@ -208,6 +213,7 @@ _ERR_BOUNDS = {0xE1: "token id outside the vocabulary (embedding forward)", 0xE2
                0xB4: "page outside the pool (beam reordering)", 0xC1: "page outside the pool (attention over the 4-bit cache)",
                0xC2: "slot outside the pool (4-bit cache)", 0xC3: "position outside the rotary tables (4-bit cache)",
                0xC4: "sequence longer than its row of the block table (attention over the 4-bit cache)",
+               0xD1: "expert that there is not (sorting tokens by expert)", 0xD2: "expert that there is not (gradient of the routing)",
                0xA1: "shared memory of the attention backward (head size 128) does not start on a 1024-byte boundary",
                0xA2: "shared memory of the attention backward (head size 64) does not start on a 1024-byte boundary"}
 
@@ -277,7 +283,7 @@ class _Ctypes:
     """The entry points as the extension module has them, through ctypes."""
 
     def __getattr__(self, name):
-        fn, kinds, to = getattr(lib(), name), _KINDS.get(name[4:]) or _GEN_KINDS[name[4:]], {"b": _b, "f": _f, "i": _i, "u": _u8}
+        fn, kinds, to = getattr(lib(), name), _KINDS.get(name[4:]) or _GEN_KINDS.get(name[4:]) or _MOE_KINDS[name[4:]], {"b": _b, "f": _f, "i": _i, "u": _u8}
 
         def call(*args):
             a = [to[k](x) if k in to and type(x) is not Address else x for k, x in zip(kinds, args, strict=kinds[-1] != "s")]
@@ -804,3 +810,6 @@ def scale_(x, s):
 
 # ------------------------------------------------------------------ generation
 from .native_gen import beam_reorder, beam_select, block_tables, kv4_append, kv4_attn, kv4_read  # noqa: E402,F401
+
+# ------------------------------------------------------------------ experts
+from .native_moe import moe_mlp, moe_mlp_bwd, moe_mlp_fwd, moe_route, moe_route_bwd  # noqa: E402,F401

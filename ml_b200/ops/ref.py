@@ -409,3 +409,4 @@ def zero_(x):
 
 
 from .ref_gen import beam_reorder, beam_select, block_tables, kv4_append, kv4_attn, kv4_read  # noqa: E402,F401
+from .ref_moe import moe_mlp, moe_mlp_bwd, moe_mlp_fwd, moe_route, moe_route_bwd  # noqa: E402,F401

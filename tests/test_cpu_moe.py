@@ -1,0 +1,189 @@
+"""A mixture of experts on the CPU: the plain forms of routing and experts against the definitions in 64 bits, the block and the decoder with experts."""
+import math
+import re
+
+import pytest
+import torch
+
+from ml_b200 import ops
+from ml_b200.ops import autograd as F
+from tests import moe_oracle as oracle
+
+I32 = torch.int32
+
+
+def logits_of(N, E):
+    z = torch.randn(N, E, generator=torch.Generator().manual_seed(N + E)) * 2
+    if N > 5:
+        z[1], z[2, ::2], z[3, 1:], z[4] = -math.inf, math.nan, -math.inf, 0.5
+        z[5] = -95 - torch.arange(E) / 8
+    return z
+
+
+@pytest.mark.parametrize("N,E,k,groups,top", [(1, 1, 1, 1, 1), (9, 6, 2, 1, 1), (20, 33, 4, 1, 1), (12, 12, 3, 4, 2), (10, 64, 8, 8, 3), (8, 4, 1, 4, 1)])
+@pytest.mark.parametrize("score,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_plain_routing(N, E, k, groups, top, score, renorm, biased):
+    z = logits_of(N, E).requires_grad_()
+    bias = torch.randn(E) * 0.1 if biased else None
+    how = dict(score=score, groups=groups, top_groups=top, renorm=renorm, scale=1.5)
+    w, idx, mean = F.moe_route(z, k, bias=bias, **how)
+    zd = torch.where(torch.isfinite(z.detach()), z.detach().double(), -math.inf).requires_grad_()
+    ew, eidx, emean = oracle.route(zd, k, bias, **how)
+    assert torch.equal(idx, eidx)
+    assert torch.allclose(w.double(), ew, atol=1e-6) and torch.allclose(mean.double(), emean, atol=1e-6)
+    dw, dm = torch.randn(N, k), torch.randn(E)
+    dz, = torch.autograd.grad([w, mean], z, [dw, dm])
+    ez, = torch.autograd.grad([ew, emean], zd, [dw.double(), dm.double()])
+    assert torch.allclose(dz.double(), torch.nan_to_num(ez), atol=2e-6, rtol=1e-5)
+
+
+def test_routing_gradient_against_differences():
+    torch.manual_seed(3)
+    for score in ("softmax", "sigmoid"):
+        for renorm in (True, False):
+            z = torch.randn(4, 7, dtype=torch.float64)
+            dw, dm = torch.randn(4, 3, dtype=torch.float64), torch.randn(7, dtype=torch.float64)
+            f = lambda t: (lambda w, i, m: float((w * dw).sum() + (m * dm).sum()))(*oracle.route(t, 3, score=score, renorm=renorm))
+            zf = z.float().requires_grad_()
+            w, _, mean = F.moe_route(zf, 3, score=score, renorm=renorm)
+            dz, = torch.autograd.grad([w, mean], zf, [dw.float(), dm.float()])
+            for n, e in ((0, 0), (1, 3), (2, 6), (3, 1), (3, 5)):
+                up, lo = z.clone(), z.clone()
+                up[n, e] += 1e-5
+                lo[n, e] -= 1e-5
+                assert abs((f(up) - f(lo)) / 2e-5 - float(dz[n, e])) < 1e-5
+
+
+def case(N, E, k, C, I, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)
+    idx = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(N)]).to(I32)
+    if N > 3:
+        idx[1], idx[2, 0] = -1, -1
+    return r(N, C), torch.softmax(r(N, k), 1), idx, r(E, 2 * I, C) * C ** -0.5, r(E, C, I) * I ** -0.5
+
+
+@pytest.mark.parametrize("N,E,k,C,I", [(1, 1, 1, 16, 16), (7, 5, 2, 24, 40), (30, 4, 3, 16, 32)])
+def test_plain_experts(N, E, k, C, I):
+    x, w, idx, gate_up, down = leaves = case(N, E, k, C, I)
+    with torch.no_grad():
+        served = F.moe_mlp(*leaves)
+    for t in (x, w, gate_up, down):
+        t.requires_grad_()
+    dout = torch.randn(N, C)
+    out = F.moe_mlp(*leaves)
+    got = [out.detach(), *torch.autograd.grad(out, [x, w, gate_up, down], dout)]
+    assert torch.equal(served, got[0])
+    for a, b in zip(got, oracle.mlp_grads(dout, x, w, idx, gate_up, down)):
+        assert torch.allclose(a.double(), b, atol=1e-5, rtol=1e-4)
+
+
+def test_frozen_parts_get_no_gradient():
+    x, w, idx, gate_up, down = case(9, 4, 2, 16, 16)
+    y = F.moe_mlp(x, w, idx, gate_up.requires_grad_(), down)
+    want = oracle.mlp_grads(torch.ones_like(y), x, w, idx, gate_up, down)
+    assert torch.allclose(torch.autograd.grad(y.sum(), gate_up)[0].double(), want[3], atol=1e-5)
+
+
+def test_refusals():
+    x, w, idx, gate_up, down = case(9, 4, 2, 16, 16)
+    out = torch.empty_like(x)
+    for bad in (dict(x=x[:, :8]), dict(out=out[:5]), dict(idx=idx.long()), dict(idx=idx[:, 0]), dict(weights=w[:, :1]), dict(gate_up=gate_up[:, :-1]), dict(down=down.transpose(1, 2)[:, :8]),
+                dict(gate_up=gate_up.double()), dict(idx=idx + 4)):
+        a = {**dict(out=out, x=x, weights=w, idx=idx, gate_up=gate_up, down=down), **bad}
+        with pytest.raises(ValueError):
+            ops.moe_mlp(a["out"], a["x"], a["weights"], a["idx"], a["gate_up"], a["down"])
+    z, w, i = torch.zeros(4, 8), torch.empty(4, 2), torch.empty(4, 2, dtype=I32)
+    for bad in (dict(score="other"), dict(groups=3), dict(groups=4, top_groups=5), dict(groups=8, top_groups=1), dict(groups=0), dict(bias=torch.zeros(7)), dict(bias=torch.zeros(8).double())):
+        with pytest.raises(ValueError):
+            ops.moe_route(w, i, None, z, **bad)
+    for a in ((w.double(), i, None, z), (w, i.long(), None, z), (w, i, torch.empty(7), z), (w, i, None, z.double()), (w, i, None, torch.zeros(4, 2000)), (w, i, None, torch.zeros(8))):
+        with pytest.raises(ValueError):
+            ops.moe_route(*a)
+    for a in ((torch.empty(4, 7), w, None, z, i), (torch.empty(4, 8), w.double(), None, z, i), (torch.empty(4, 8), w, torch.empty(7), z, i), (torch.empty(4, 8), w, None, z, i.long())):
+        with pytest.raises(ValueError):
+            ops.moe_route_bwd(*a)
+
+
+def test_entry_points_have_one_signature():
+    """What ctypes declares, what the extension module calls and what the kernel library's sources define are the same, parameter by parameter."""
+    from ml_b200 import build
+    from ml_b200.ops import native
+    assert native.bridge().moe_signatures() == {"mlb_" + k: v for k, v in native._MOE_KINDS.items()}
+    letter = {"void*": "p", "float*": "f", "int*": "i", "uint8_t*": "u", "int": "n", "long": "l", "float": "d", "cudaStream_t": "s"}
+    defined = {}
+    for src in (build.CSRC / "kernels").glob("moe*.cu*"):
+        for name, args in re.findall(r"^MLB_API [\w ]+? (mlb_\w+)\(([^)]*)\)", src.read_text(), re.M):
+            types = [re.sub(r"\s*\w+$", "", a.replace("const ", "").strip()).replace(" *", "*") for a in args.split(",")]
+            defined[name] = "".join(letter.get(t, "?") for t in types)
+    assert set(defined) == {"mlb_" + k for k in native._MOE_KINDS}
+    for name, kinds in native._MOE_KINDS.items():
+        assert len(defined["mlb_" + name]) == len(kinds), name
+        assert all(d == k or (d == "p" and k in "bfiu") for d, k in zip(defined["mlb_" + name], kinds)), name
+
+
+# ------------------------------------------------------------------ the block, the decoder
+def test_block_gives_what_the_loop_over_experts_gives():
+    from ml_b200.models.moe import MoE, MoEBlock
+    torch.manual_seed(0)
+    loop, block = MoEBlock(24, 32, 5, 2, std=0.3), MoE(24, 32, 5, 2, std=0.3)
+    with torch.no_grad():
+        block.router.copy_(loop.router)
+        for e in range(5):
+            block.gate_up[e].copy_(loop.gate_up[e])
+            block.down[e].copy_(loop.down[e])
+    x = torch.randn(40, 24)
+    (a, la), (b, lb) = loop(x), block(x)
+    assert torch.allclose(a, b, atol=1e-5) and torch.allclose(la, lb, atol=1e-6)
+    (a.square().sum() + la).backward()
+    (b.square().sum() + lb).backward()
+    assert torch.allclose(loop.router.grad, block.router.grad, atol=1e-4)
+    assert torch.allclose(torch.stack([p.grad for p in loop.down]), block.down.grad, atol=1e-4)
+
+
+def test_balance_moves_the_choice():
+    from ml_b200.models.moe import MoE
+    torch.manual_seed(0)
+    m = MoE(16, 16, 4, 1, score="sigmoid", balanced=True)
+    with torch.no_grad():
+        m.router.zero_()
+    x = torch.randn(10, 16)
+    m(x)
+    assert m.load.tolist() == [10, 0, 0, 0]      # equal scores: the lowest index
+    m.balance(0.1)
+    assert m.bias.tolist() == pytest.approx([-0.1, 0.1, 0.1, 0.1])
+    m(x)
+    assert m.load.tolist() == [0, 10, 0, 0]
+    m.eval()
+    m(x[:2])
+    assert m.load.tolist() == [0, 10, 0, 0]
+    assert m.bfloat16().bias.dtype == torch.float32 and m.load.dtype == torch.float32
+    with pytest.raises(ValueError):
+        MoE(16, 16, 4, 1).balance()
+
+
+def test_decoder_with_experts_trains():
+    from ml_b200 import Config
+    from ml_b200.models.modules import Decoder
+    cfg = Config(V=61, C=32, L=2, H=2, I=48, T=16)
+    torch.manual_seed(0)
+    m = Decoder(cfg, experts=dict(n_experts=4, top_k=2, std=0.1))
+    for n, p in m.named_parameters():
+        if "moe" not in n:
+            torch.nn.init.normal_(p, std=0.1)
+    ids = torch.randint(0, 61, (2, 16), dtype=I32)
+    loss = m(ids, torch.roll(ids, -1))
+    loss.backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters())
+    assert all(b.moe.router.grad.abs().sum() > 0 for b in m.blocks)
+    with pytest.raises(ValueError):
+        m.load_flat(torch.zeros(1))
+    # the gradient of one weight against a difference
+    p, at = m.blocks[1].moe.gate_up, (int(m.blocks[1].moe.load.argmax()), 5, 7)
+    with torch.no_grad():
+        both = []
+        for d in (1e-2, -2e-2):
+            p[at] += d
+            both.append(float(m(ids, torch.roll(ids, -1))))
+    assert abs((both[0] - both[1]) / 2e-2 - float(p.grad[at])) < 1e-3

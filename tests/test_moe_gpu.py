@@ -1,0 +1,451 @@
+"""Kernels of a mixture of experts (routing, the experts' products and their gradients) against the definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from ml_b200 import ops
+from ml_b200.ops import autograd as F
+from tests import moe_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+HALF = {BF16: 2.0 ** -8, F32: 2.0 ** -24}      # half a step, relative: what one rounding is off by at most
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+def nat():
+    from ml_b200.ops import native
+    return native
+
+
+@pytest.fixture(autouse=True)
+def no_errors():
+    yield
+    torch.cuda.synchronize()
+    err = nat().get_error()
+    nat().clear_error()
+    assert err == 0, nat().describe_error(err)
+
+
+def raised(detail):
+    torch.cuda.synchronize()
+    err = nat().get_error()
+    nat().clear_error()
+    assert err == 3 << 24 | detail, hex(err)
+
+
+# ------------------------------------------------------------------ routing
+def logits_of(N, E, dtype, seed=0, special=True):
+    g = torch.Generator().manual_seed(1000 * N + E + seed)
+    z = (torch.randn(N, E, generator=g) * 2).to(dtype)
+    if special and N > 12:
+        z[1] = -math.inf                       # a token that goes nowhere
+        z[2, ::2] = math.nan                   # NaN is no expert
+        z[3, 1:] = -math.inf                   # one expert left
+        z[4] = 0.5                             # all equal
+        z[5, :E // 2] = z[5, E - E // 2:].clone()
+        z[6] = -90 - torch.arange(E, dtype=F32).to(dtype) / 8      # scores that vanish in 32 bits
+        z[7] = torch.where(torch.arange(E) % 3 == 0, 40.0, -40.0).to(dtype)
+        z[8] = torch.where(torch.arange(E) % 2 == 0, 0.0, -0.0).to(dtype)
+    return z
+
+
+def routed(z, k, wdtype=F32, mean=True, **how):
+    N, E = z.shape
+    w = torch.full((N, k), 7.0, dtype=wdtype, device=dev())
+    idx, m = torch.full((N, k), 77, dtype=I32, device=dev()), torch.full((E,), 7.0, device=dev()) if mean else None
+    b = how.pop("bias", None)
+    ops.moe_route(w, idx, m, z.to(dev()), None if b is None else b.to(dev()), **how)
+    return w, idx, m
+
+
+ROUTES = [(1, 1, 1), (1, 2, 2), (7, 8, 2), (40, 33, 5), (100, 64, 6), (33, 128, 8), (20, 200, 8), (70, 256, 8), (16, 500, 3), (16, 1024, 32)]
+
+
+@pytest.mark.parametrize("N,E,k", ROUTES)
+@pytest.mark.parametrize("score,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("biased", [False, True])
+def test_routing(N, E, k, score, renorm, dtype, biased):
+    z = logits_of(N, E, dtype)
+    bias = torch.randn(E, generator=torch.Generator().manual_seed(E)) * 0.1 if biased else None
+    how = dict(score=score, renorm=renorm, scale=1.5)
+    w, idx, mean = routed(z, k, bias=bias, **how)
+    ew, eidx, emean = oracle.route(z.double(), k, bias, **how)
+    assert torch.equal(idx.cpu(), eidx)
+    # exp: 3 steps of 2^-23 (its own 2, the split product 1); sums of E terms in a tree of 5 + E / 32 additions; a division, a product with the scale
+    tol = (6 + 2 * (5 + E / 32) + 4) * HALF[F32]
+    assert torch.all((w.cpu().double() - ew).abs() <= tol * ew.abs() + 1e-37)
+    # and N of them added up, N / 8 and more in each of some running sums
+    assert torch.all((mean.cpu().double() - emean).abs() <= (tol + (N / 8 + 16) * HALF[F32]) * emean + 1e-37)
+
+
+@pytest.mark.parametrize("N,E,k,groups,top", [(5, 4, 1, 4, 1), (40, 12, 3, 4, 2), (60, 64, 4, 8, 4), (30, 256, 8, 8, 4), (20, 60, 5, 6, 5), (20, 32, 2, 32, 3), (9, 1024, 8, 32, 7)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_routing_in_groups(N, E, k, groups, top, score, biased):
+    z = logits_of(N, E, F32, seed=3)
+    if N > 12:
+        z[9, E // groups:] = -math.inf                      # one group has experts
+        z[10, :E - 1] = -math.inf                           # and the last one a single one
+        z[11] = z[11, :E // groups].repeat(groups)          # equal groups
+    bias = torch.randn(E, generator=torch.Generator().manual_seed(E)) * 0.1 if biased else None
+    how = dict(score=score, groups=groups, top_groups=top)
+    w, idx, _ = routed(z, k, bias=bias, mean=False, **how)
+    ew, eidx, _ = oracle.route(z.double(), k, bias, **how)
+    assert torch.equal(idx.cpu(), eidx)
+    assert torch.all((w.cpu().double() - ew).abs() <= (6 + 2 * (5 + E / 32) + 4) * HALF[F32] * ew + 1e-37)
+
+
+def test_routing_next_to_a_border():
+    """Scores that 32 bits cannot tell apart are told apart, and equal ones go to the lowest index."""
+    E = 64
+    z = torch.zeros(3, E)
+    bias = torch.zeros(E)
+    bias[40], bias[3] = 1e-9, 5e-10                # beside scores of 0.5: one rounding of fp32 there is 3e-8
+    z[1, 50] = 2.0 ** -30
+    _, idx, _ = routed(z, 3, bias=bias, score="sigmoid")
+    assert idx.tolist() == [[40, 3, 0], [40, 3, 50], [40, 3, 0]]
+
+
+def test_routing_infinite_logits():
+    z = torch.randn(4, 40)
+    z[0, [7, 30]] = math.inf
+    z[1, 5] = math.inf
+    w, idx, _ = routed(z, 2)
+    assert idx[0].tolist() == [7, 30] and w[0].tolist() == [0.5, 0.5] and idx[1, 0] == 5 and w[1].tolist() == [1.0, 0.0]
+    w, _, mean = routed(z, 2, score="sigmoid", renorm=False)
+    assert w[0].tolist() == [1.0, 1.0] and bool(torch.isfinite(mean).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_routing_of_strided_logits_and_bf16_weights(dtype):
+    wide = logits_of(50, 90, dtype).to(dev())
+    z = wide[:, 11:71]
+    w, idx, mean = routed(z, 4, wdtype=BF16)
+    ew, eidx, emean = oracle.route(z.cpu().double(), 4)
+    assert torch.equal(idx.cpu(), eidx)
+    assert torch.all((w.cpu().double() - ew).abs() <= (HALF[BF16] + 1e-5) * ew)
+    d = torch.empty(50, 60, dtype=dtype, device=dev())
+    g = torch.randn(50, 4, device=dev())
+    ops.moe_route_bwd(d, g, None, z, idx)
+    e = torch.empty_like(d)
+    ops.moe_route_bwd(e, g, None, z.contiguous(), idx)
+    assert torch.equal(d, e)
+
+
+@pytest.mark.parametrize("N,E,k", ROUTES)
+@pytest.mark.parametrize("score,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradient_of_routing(N, E, k, score, renorm, dtype):
+    z = logits_of(N, E, dtype)
+    how = dict(score=score, renorm=renorm, scale=1.5)
+    zc = z.to(dev()).requires_grad_()
+    w, idx, mean = F.moe_route(zc, k, dtype=F32, **how)
+    dw, dm = torch.randn(N, k, device=dev()), torch.randn(E, device=dev()) * E
+    dz, = torch.autograd.grad([w, mean], [zc], [dw, dm])
+    zd = torch.where(torch.isfinite(z), z.double(), -math.inf).requires_grad_()
+    ew, eidx, emean = oracle.route(zd, k, **how)
+    ez, = torch.autograd.grad([ew, emean], [zd], [dw.cpu().double(), dm.cpu().double()])
+    ez = torch.nan_to_num(ez)
+    assert torch.equal(idx.cpu(), eidx)
+    # every gradient is a sum of two differences p (g - sum p g), whose terms are off by as much as a weight is: relative to the largest g of the row
+    p_tol = (6 + 2 * (5 + E / 32) + 8) * HALF[F32]
+    size = 1.5 * dw.abs().amax(1).cpu().double() + dm.abs().max().cpu().double() / N
+    err = (dz.cpu().double() - ez).abs()
+    assert torch.all(err <= HALF[dtype] * ez.abs() + 3 * p_tol * size[:, None] + 1e-37)
+
+
+def test_gradient_of_routing_of_one_output():
+    z = logits_of(30, 20, F32, special=False).to(dev()).requires_grad_()
+    for pick in (0, 2):
+        out = F.moe_route(z, 3)
+        g = torch.randn_like(out[pick])
+        dz, = torch.autograd.grad(out[pick], z, g)
+        zd = z.detach().cpu().double().requires_grad_()
+        ez, = torch.autograd.grad(oracle.route(zd, 3)[pick], zd, g.cpu().double())
+        assert torch.allclose(dz.cpu().double(), ez, atol=1e-6, rtol=1e-5)
+
+
+def test_routing_of_no_tokens():
+    w, idx, mean = routed(torch.empty(0, 8), 2)
+    assert w.shape == (0, 2) and mean.abs().sum() == 0
+    z = torch.empty(0, 8, device=dev(), requires_grad=True)
+    out = F.moe_route(z, 2)
+    assert torch.autograd.grad(out[0].sum() + out[2].sum(), z)[0].shape == (0, 8)
+
+
+def test_gradient_of_an_expert_that_there_is_not():
+    z = torch.zeros(2, 4, device=dev())
+    d = torch.empty_like(z)
+    ops.moe_route_bwd(d, torch.ones(2, 1, device=dev()), None, z, torch.tensor([[4], [-1]], dtype=I32, device=dev()))
+    raised(0xD2)
+    assert d.abs().sum() == 0
+
+
+# ------------------------------------------------------------------ the experts
+def experts(N, E, k, C, I, gates=BF16, seed=0, route="even", drop=0):
+    g = torch.Generator().manual_seed(seed + N + 10 * E + 100 * C + I)
+    r = lambda *s: torch.randn(*s, generator=g)
+    if route == "even":
+        idx = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(N)]) if N else torch.zeros(0, k)
+    else:                                        # most tokens to the first experts
+        idx = torch.topk(r(N, E) - 0.8 * torch.arange(E), k, 1).indices
+    idx = idx.to(I32)
+    w = torch.softmax(r(N, k), 1)
+    if drop:
+        lost = torch.randperm(N, generator=g)[:drop]
+        idx[lost, :(k + 1) // 2] = -1
+    to = lambda t: t.to(dev())
+    return to(r(N, C).to(BF16)), to(w.to(gates)), to(idx), to((r(E, 2 * I, C) * C ** -0.5).to(BF16)), to((r(E, C, I) * I ** -0.5).to(BF16))
+
+
+def close(got, want, roundings, what):
+    """All in all and row by row: `roundings` of half a step each, every one relative to what passes it."""
+    tol = roundings * HALF[BF16]
+    d = got.double() - want
+    assert torch.isfinite(d).all(), what
+    if d.numel():
+        assert float(d.norm()) <= tol * float(want.norm()) + 1e-30, (what, float(d.norm() / want.norm()), tol)
+        rows, size = d.flatten(0, -2).norm(dim=1), want.flatten(0, -2).norm(dim=1)
+        # (rows of few columns or nearly cancelled ones: relative to the ordinary row)
+        assert bool((rows <= tol * torch.maximum(size, want.norm() / max(1, len(size)) ** 0.5) + 1e-30).all()), what
+
+
+MLPS = [(1, 1, 1, 16, 16), (1, 4, 2, 64, 48), (3, 5, 2, 48, 80), (31, 2, 1, 64, 64), (33, 4, 2, 256, 128), (64, 3, 3, 128, 256), (257, 64, 8, 64, 96), (301, 8, 3, 336, 208),
+        (520, 2, 2, 272, 144), (700, 3, 1, 128, 272), (1500, 16, 4, 192, 160), (2500, 7, 2, 512, 320)]
+
+
+@pytest.mark.parametrize("N,E,k,C,I", MLPS)
+@pytest.mark.parametrize("gates", [BF16, F32])
+@pytest.mark.parametrize("route", ["even", "crowded"])
+def test_experts(N, E, k, C, I, gates, route):
+    x, w, idx, gate_up, down = experts(N, E, k, C, I, gates, route=route, drop=N // 9)
+    out = torch.full((N, C), 7.0, dtype=BF16, device=dev())
+    ops.moe_mlp(out, x, w, idx, gate_up, down)
+    want = oracle.mlp(x.double(), w.double(), idx, gate_up.double(), down.double())
+    close(out, want, 5, "out")                  # g and u (silu doubles that at most), h, y, out
+    gone = (idx < 0).all(1)
+    assert out[gone].abs().sum() == 0
+
+
+@pytest.mark.parametrize("N,E,k,C,I", MLPS)
+@pytest.mark.parametrize("gates", [BF16, F32])
+@pytest.mark.parametrize("route", ["even", "crowded"])
+def test_gradients_of_experts(N, E, k, C, I, gates, route):
+    x, w, idx, gate_up, down = leaves = experts(N, E, k, C, I, gates, route=route, drop=N // 9)
+    for t in (x, w, gate_up, down):
+        t.requires_grad_()
+    dout = torch.randn(N, C, generator=torch.Generator().manual_seed(N)).to(BF16).to(dev())
+    out = F.moe_mlp(*leaves)
+    grads = torch.autograd.grad(out, [x, w, gate_up, down], dout)
+    want = oracle.mlp_grads(dout, x, w, idx, gate_up, down)
+    close(out.detach(), want[0], 5, "out")
+    close(grads[0], want[1], 6, "dx")            # g and u 2, dh, dgu, dxs, dx
+    close(grads[1].reshape(1, -1), want[2].reshape(1, -1), 4, "dweights")
+    close(grads[2], want[3], 5, "dgate_up")      # g and u 2, dh, dgu, the result
+    close(grads[3], want[4], 4, "ddown")         # g and u 2, w h, the result
+    assert grads[1][idx < 0].abs().sum() == 0
+    unused = [e for e in range(E) if not bool((idx == e).any())]
+    assert grads[2][unused].abs().sum() == 0 and grads[3][unused].abs().sum() == 0
+
+
+@pytest.mark.parametrize("N,E,k", [(5000, 300, 2), (20000, 6, 1), (3000, 1024, 4)])
+def test_experts_of_many_copies(N, E, k):
+    """Copies enough for several thread blocks of the plan, and more experts than it has threads."""
+    x, w, idx, gate_up, down = leaves = experts(N, E, k, 32, 16, F32, route="even", drop=100)
+    for t in (x, w, gate_up, down):
+        t.requires_grad_()
+    out = F.moe_mlp(*leaves)
+    grads = torch.autograd.grad(out, [x, w, gate_up, down], dout := torch.randn(N, 32, device=dev()).to(BF16))
+    want = oracle.mlp_grads(dout, x, w, idx, gate_up, down)
+    for got, exact, n, what in zip((out.detach(), *grads), want, (5, 6, 4, 5, 4), ("out", "dx", "dweights", "dgate_up", "ddown")):
+        close(got.reshape(1, -1) if what == "dweights" else got, exact.reshape(1, -1) if what == "dweights" else exact, n, what)
+
+
+def test_the_same_expert_twice():
+    x, w, idx, gate_up, down = leaves = experts(40, 4, 2, 64, 64)
+    idx[:, 1] = idx[:, 0]
+    for t in (x, w, gate_up, down):
+        t.requires_grad_()
+    out = F.moe_mlp(*leaves)
+    grads = torch.autograd.grad(out, [x, w, gate_up, down], dout := torch.randn(40, 64, device=dev()).to(BF16))
+    want = oracle.mlp_grads(dout, x, w, idx, gate_up, down)
+    for got, exact, n, what in zip((out.detach(), *grads), want, (5, 6, 4, 5, 4), ("out", "dx", "dweights", "dgate_up", "ddown")):
+        close(got.reshape(1, -1) if what == "dweights" else got, exact.reshape(1, -1) if what == "dweights" else exact, n, what)
+
+
+def test_tokens_that_all_go_nowhere():
+    x, w, idx, gate_up, down = leaves = experts(20, 4, 2, 64, 64)
+    idx.fill_(-1)
+    for t in (x, w, gate_up, down):
+        t.requires_grad_()
+    out = F.moe_mlp(*leaves)
+    grads = torch.autograd.grad(out, [x, w, gate_up, down], torch.ones_like(out))
+    assert out.abs().sum() == 0 and all(g.abs().sum() == 0 for g in grads)
+
+
+def test_no_tokens():
+    leaves = experts(0, 4, 2, 64, 64)
+    for t in (leaves[0], leaves[1], leaves[3], leaves[4]):
+        t.requires_grad_()
+    out = F.moe_mlp(*leaves)
+    grads = torch.autograd.grad(out.sum(), [leaves[0], leaves[1], leaves[3], leaves[4]])
+    assert out.shape == (0, 64) and all(g.abs().sum() == 0 for g in grads)
+
+
+def test_an_expert_that_there_is_not():
+    x, w, idx, gate_up, down = experts(20, 4, 2, 64, 64)
+    out, clean = torch.empty_like(x), torch.empty_like(x)
+    bad = idx.clone()
+    bad[3, 1] = 4
+    ops.moe_mlp(out, x, w, bad, gate_up, down)
+    raised(0xD1)
+    idx[3, 1] = -1
+    ops.moe_mlp(clean, x, w, idx, gate_up, down)
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("N", [6, 200])
+def test_values_that_are_not_numbers_stay_with_their_token(N):
+    """NaN and infinities in a token reach its own row, and the gradients of the experts that it went to."""
+    x, w, idx, gate_up, down = experts(N, 6, 2, 64, 64)
+    idx[2], idx[4] = torch.tensor([0, 1]), torch.tensor([0, -1])
+    idx[idx[:, 0] != 0, :] = idx[idx[:, 0] != 0, :].clamp(min=2)
+    ref = torch.empty_like(x)
+    ops.moe_mlp(ref, x, w, idx, gate_up, down)
+    bad = x.clone()
+    bad[2], bad[4, 5] = math.nan, math.inf
+    out = torch.empty_like(x)
+    ops.moe_mlp(out, bad, w, idx, gate_up, down)
+    rest = [n for n in range(N) if n not in (2, 4)]
+    assert torch.equal(out[rest], ref[rest]) and bool(out[2].isnan().all())
+    leaves = [bad.requires_grad_(), w, gate_up.requires_grad_(), down.requires_grad_()]
+    y = F.moe_mlp(leaves[0], w, idx, gate_up, down)
+    dx, dgu, dd = torch.autograd.grad(y, [leaves[0], gate_up, down], torch.randn_like(y))
+    assert torch.isfinite(dx[rest]).all() and torch.isfinite(dgu[2:]).all() and torch.isfinite(dd[2:]).all()
+
+
+def test_rows_of_a_wider_tensor_and_frozen_weights():
+    x, w, idx, gate_up, down = experts(70, 4, 2, 64, 48)
+    wide = torch.zeros(70, 96, dtype=BF16, device=dev())
+    wide[:, 16:80] = x
+    part = wide[:, 16:80].requires_grad_()
+    out, ref = torch.empty_like(x), torch.empty_like(x)
+    ops.moe_mlp(out, part.detach(), w, idx, gate_up, down)
+    ops.moe_mlp(ref, x, w, idx, gate_up, down)
+    assert torch.equal(out, ref)
+    y = F.moe_mlp(part, w, idx, gate_up, down)      # only the tokens are trained
+    dx, = torch.autograd.grad(y, part, torch.ones_like(y[:1]).expand_as(y))
+    want = oracle.mlp_grads(torch.ones_like(y), x, w, idx, gate_up, down)
+    close(dx, want[1], 6, "dx")
+    y = F.moe_mlp(x, w, idx, gate_up, down.requires_grad_())
+    close(torch.autograd.grad(y, down, torch.ones_like(y))[0], want[4], 4, "ddown")
+
+
+@pytest.mark.parametrize("N,E,k,C,I", [(1, 8, 2, 256, 128), (16, 8, 2, 256, 128), (900, 8, 3, 128, 256)])
+def test_the_same_bits_on_every_run_and_from_a_graph(N, E, k, C, I):
+    x, w, idx, gate_up, down = leaves = experts(N, E, k, C, I, F32)
+    for t in (x, w, gate_up, down):
+        t.requires_grad_()
+    dout = torch.randn(N, C, device=dev()).to(BF16)
+
+    def step():
+        out = F.moe_mlp(*leaves)
+        return [out.detach(), *torch.autograd.grad(out, [x, w, gate_up, down], dout)]
+
+    def serve():
+        with torch.no_grad():
+            return F.moe_mlp(*leaves)
+
+    first, one = step(), serve()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, step())) and torch.equal(one, serve())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(), serve()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, out = step(), serve()
+    for t in (*got, out):
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, got)) and torch.equal(one, out)
+
+
+def test_experts_on_another_stream():
+    x, w, idx, gate_up, down = experts(300, 8, 2, 256, 128)
+    ref, out = torch.empty_like(x), torch.empty_like(x)
+    ops.moe_mlp(ref, x, w, idx, gate_up, down)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            ops.moe_mlp(out, x, w, idx, gate_up, down)
+    ops.moe_mlp(ref, x, w, idx, gate_up, down)      # at the same time
+    torch.cuda.synchronize()
+    assert torch.equal(ref, out)
+
+
+def test_a_token_costs_the_same_bits_in_any_batch_of_the_kind():
+    """What a token's experts give does not depend on who else is there (in the same form of the kernels)."""
+    x, w, idx, gate_up, down = experts(900, 8, 2, 128, 128)
+    all_, some = torch.empty_like(x), torch.empty_like(x[:700])
+    ops.moe_mlp(all_, x, w, idx, gate_up, down)
+    ops.moe_mlp(some, x[:700], w[:700], idx[:700], gate_up, down)
+    assert torch.equal(all_[:700], some)
+
+
+def test_refusals():
+    x, w, idx, gate_up, down = experts(20, 4, 2, 64, 64)
+    out = torch.empty_like(x)
+    ops_args = ("out", "x", "weights", "idx", "gate_up", "down")
+    def refused(**kw):
+        a = {**dict(zip(ops_args, (out, x, w, idx, gate_up, down))), **kw}
+        with pytest.raises(ValueError):
+            ops.moe_mlp(*(a[n] for n in ops_args))
+    refused(x=x.float()), refused(out=out.float()), refused(idx=idx.long()), refused(gate_up=gate_up[:, :-2]), refused(down=down.transpose(1, 2))
+    refused(weights=w[:, :1]), refused(out=torch.empty(64, 20, dtype=BF16, device=dev()).T), refused(x=torch.empty(64, 20, dtype=BF16, device=dev()).T)
+    refused(x=torch.empty(20 * 64 + 1, dtype=BF16, device=dev())[1:].view(20, 64))
+    refused(gate_up=torch.empty(4 * 128 * 64 + 1, dtype=BF16, device=dev())[1:].view(4, 128, 64))
+    odd = experts(20, 4, 2, 64, 64)
+    refused(gate_up=odd[3][:, :80].contiguous(), down=odd[4][:, :, :40].contiguous())      # 40 is no multiple of 16
+    refused(x=x[:, :56].contiguous(), out=out[:, :56].contiguous(), gate_up=gate_up[:, :, :56].contiguous(), down=down[:, :56].contiguous())
+    z = torch.zeros(4, 8, device=dev())
+    w8, i8 = torch.empty(4, 2, device=dev()), torch.empty(4, 2, dtype=I32, device=dev())
+    for bad in (dict(score="other"), dict(groups=3), dict(groups=4, top_groups=5), dict(groups=8, top_groups=1), dict(groups=0)):
+        with pytest.raises(ValueError):
+            ops.moe_route(w8, i8, None, z, **bad)
+    for a in ((w8.double(), i8, None, z), (w8, i8.long(), None, z), (w8, i8, torch.empty(7, device=dev()), z), (w8, i8, None, z.half()), (w8, i8, None, z, torch.zeros(9, device=dev())),
+              (w8, i8, None, torch.zeros(8, 4, device=dev()).T), (w8, i8, None, torch.zeros(4, 2000, device=dev()))):
+        with pytest.raises(ValueError):
+            ops.moe_route(*a)
+
+
+def test_entry_points_are_called_alike_through_python_and_the_extension_module(monkeypatch):
+    n = nat()
+    x, w, idx, gate_up, down = leaves = experts(50, 8, 2, 64, 64)
+    z = torch.randn(50, 8, device=dev()).requires_grad_()
+    for t in (x, w, gate_up, down):
+        t.requires_grad_()
+
+    def work():
+        rw, ridx, mean = F.moe_route(z, 2)
+        out = F.moe_mlp(*leaves)
+        served = torch.empty_like(x)
+        ops.moe_mlp(served, *(t.detach() for t in leaves))
+        return [rw.detach(), ridx, mean.detach(), out.detach(), served, *torch.autograd.grad([rw, mean], z, [torch.ones_like(rw), torch.ones_like(mean)]),
+                *torch.autograd.grad(out, [x, w, gate_up, down], torch.ones_like(out))]
+
+    outs = []
+    for entries in (n._Ctypes(), n.bridge()):
+        monkeypatch.setattr(n, "_E", entries)
+        outs.append(work())
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
