@@ -5,7 +5,8 @@
 // A copy of a token is a pair (token n, place j), numbered n k + j.  The plan puts the copies in rows by expert, each expert's rows beginning at a multiple of 32 and
 // filled up with empty rows, so that a product's tile and the reductions over tokens end where an expert does:
 //   forward    xs = rows of x;  [g | u] = xs Wgu^T, h = silu(g) u (one product, h formed from its accumulators);  y = h Wd^T;  out = weighted sums of y
-//   backward   ys = rows of dout;  dh = ys Wd;  dw = h . dh, dgu from w dh, hw = w h;  dxs = dgu Wgu, dx = sums of it;  dWgu = dgu^T xs;  dWd = ys^T hw
+//   backward   ys = rows of w dout, dw = dout . y;  dh = ys Wd and from it dgu;  dxs = dgu Wgu, dx = sums of it;  dWgu = dgu^T xs;  dWd = ys^T h
+// Of the forward pass xs, [g | u], h and y are kept: with h and y the gradient of a weight and that of Wd need neither SwiGLU again nor a second set of rows.
 // Counts are known on the device only: grids are sized by what there may be at most, and blocks that find nothing leave.
 #include "../tc.cuh"
 #include "moe_route.cuh"
@@ -18,7 +19,7 @@ constexpr int PAD = 32;            // an expert's rows begin at a multiple of th
 constexpr int TILE_TOKENS = 256;   // rows of a tile of the token products
 
 // ------------------------------------------------------------------ the plan
-// int32: start[E + 1], count[E], ntiles | tiles[maxT] {expert, first row, rows, 0} | place[N k] | source[R] | hist[blocks][E]
+// int32: start[E + 1], order[E], ntiles | tiles[maxT] {expert, first row, rows, 0} | place[N k] | source[R] | hist[blocks][E]
 struct PlanShape {
   long rows, tiles, place, source, hist, total;      // R; offsets of the parts in ints
   int max_tiles, blocks, per_block;
@@ -39,7 +40,7 @@ inline PlanShape plan_shape(long NK, int E) {
   return p;
 }
 struct PlanArgs {
-  int *start, *count, *ntiles;
+  int *start, *order, *ntiles;
   int4* tiles;
   int *place, *source, *hist;
   const int* idx;
@@ -139,7 +140,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_place_k(const PlanArgs A) {
   for (int e = e0; e < e1; e++) {
     const int n = total[e], padded = (n + PAD - 1) / PAD * PAD;
     if (writes) {
-      A.start[e] = row, A.count[e] = n;
+      A.start[e] = row;
+      int before = 0;      // experts with more rows: those come first in the weight gradients
+      for (int x = 0; x < E; x++) before += total[x] > n || (total[x] == n && x < e);
+      A.order[before] = e;
       for (int t = 0; t < n; t += TILE_TOKENS) A.tiles[tile++] = make_int4(e, row + t, min(TILE_TOKENS, n - t), 0);
       for (int t = n; t < padded; t++) A.source[row + t] = -1;
     }
@@ -171,6 +175,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_place_k(const PlanArgs A) {
 }
 
 // ------------------------------------------------------------------ tokens to rows, rows to tokens
+template <typename T> __device__ __forceinline__ float as_float(T v) { return (float)v; }
+template <> __device__ __forceinline__ float as_float<bf16>(bf16 v) { return __bfloat162float(v); }
 // out[r] = x[source[r] / k], empty rows 0; a warp to a row, 16 bytes a lane
 __global__ void __launch_bounds__(256) moe_dispatch_k(bf16* __restrict__ out, const bf16* __restrict__ x, const int* __restrict__ source, const int* __restrict__ rows, long ldx, int k,
                                                       int C) {
@@ -188,8 +194,6 @@ __global__ void __launch_bounds__(256) moe_dispatch_k(bf16* __restrict__ out, co
   for (int c = lane; c < C / 8; c += 32) o[c] = __ldg(in + c);
 }
 
-template <typename T> __device__ __forceinline__ float as_float(T v) { return (float)v; }
-template <> __device__ __forceinline__ float as_float<bf16>(bf16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void add8(float (&s)[8], const uint4& v, float w) {
   const uint32_t q[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -197,6 +201,45 @@ __device__ __forceinline__ void add8(float (&s)[8], const uint4& v, float w) {
     s[2 * i] = fmaf(__uint_as_float(q[i] << 16), w, s[2 * i]);
     s[2 * i + 1] = fmaf(__uint_as_float(q[i] & 0xffff0000u), w, s[2 * i + 1]);
   }
+}
+// backward: out[r] = w dout of its token, rounded once, and the weight's gradient dout . y; a warp to a copy.  What fills up the experts' rows is written as zeros
+// (the weight gradients add it up) by the warps behind the copies', a copy that goes nowhere has the gradient 0.
+template <typename W>
+__global__ void __launch_bounds__(256) moe_dispatch_bwd_k(bf16* __restrict__ out, W* __restrict__ dweights, const bf16* __restrict__ dout, const bf16* __restrict__ y,
+                                                          const W* __restrict__ weights, const int* __restrict__ place, const int* __restrict__ source, const int* __restrict__ rows,
+                                                          long ldo, long NK, int k, int C) {
+  mlb_pdl_sync();
+  const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (i >= NK) {
+    const long r = i - NK;
+    if (r >= *rows || source[r] >= 0) return;
+    for (int c = lane; c < C / 8; c += 32) reinterpret_cast<uint4*>(out + r * C)[c] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int r = place[i];
+  float dot = 0.f;
+  if (r >= 0) {
+    const float w = as_float(weights[i]);
+    const uint4 *in = reinterpret_cast<const uint4*>(dout + i / k * ldo), *yr = reinterpret_cast<const uint4*>(y + (long)r * C);
+    uint4* o = reinterpret_cast<uint4*>(out + (long)r * C);
+#pragma unroll 2
+    for (int c = lane; c < C / 8; c += 32) {
+      const uint4 a = __ldg(in + c), b = __ldg(yr + c);
+      const uint32_t aq[4] = {a.x, a.y, a.z, a.w}, bq[4] = {b.x, b.y, b.z, b.w};
+      uint32_t q[4];
+#pragma unroll
+      for (int v = 0; v < 4; v++) {
+        const float lo = __uint_as_float(aq[v] << 16), hi = __uint_as_float(aq[v] & 0xffff0000u);
+        dot = fmaf(lo, __uint_as_float(bq[v] << 16), dot);
+        dot = fmaf(hi, __uint_as_float(bq[v] & 0xffff0000u), dot);
+        q[v] = pack_bf16(w * lo, w * hi);
+      }
+      o[c] = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+    dot = warp_sum(dot);
+  }
+  if (lane == 0) dweights[i] = (W)dot;
 }
 // out[n] = sum_j w[n, j] y[place[n, j]] in the order of j, in fp32; without weights plain sums
 template <typename W>
@@ -216,132 +259,167 @@ __global__ void __launch_bounds__(256) moe_combine_k(bf16* __restrict__ out, con
   reinterpret_cast<uint4*>(out + n * C)[c] = make_uint4(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]), pack_bf16(s[4], s[5]), pack_bf16(s[6], s[7]));
 }
 
-// ------------------------------------------------------------------ SwiGLU backward with the weight of a row
-// gu and dgu have groups of 16 gate columns and their 16 up columns side by side.  Of a row with weight w and d = dh: s = sigmoid(g), h = g s u;
-//   dw = sum h d,  dg = w d u s (1 + g (1 - s)),  du = w d g s,  hw = w h.  Empty rows are written as zeros: the products over rows add them up.
-// A row to 128 threads, 8 columns of h a thread: bound by memory (12 bytes a column of h).
-template <typename W>
-__global__ void __launch_bounds__(128) moe_swiglu_bwd_k(bf16* __restrict__ dgu, bf16* __restrict__ hw, W* __restrict__ dweights, const bf16* __restrict__ dh, const bf16* __restrict__ gu,
-                                                        const W* __restrict__ weights, const int* __restrict__ source, const int* __restrict__ rows, int I) {
-  mlb_pdl_sync();
-  __shared__ float red[32];
-  const long r = blockIdx.x;
-  if (r >= *rows) return;
-  const int s = source[r];
-  const float w = s < 0 ? 0.f : as_float(weights[s]);
-  float dot = 0.f;
-  for (int c = threadIdx.x * 8; c < I; c += 128 * 8) {
-    const long at = r * 2 * I + (c >> 4) * 32 + (c & 8);
-    uint4 dg4 = make_uint4(0, 0, 0, 0), du4 = dg4, hw4 = dg4;
-    if (s >= 0) {
-      const uint4 g4 = __ldg(reinterpret_cast<const uint4*>(gu + at)), u4 = __ldg(reinterpret_cast<const uint4*>(gu + at + 16)), d4 = __ldg(reinterpret_cast<const uint4*>(dh + r * I + c));
-      const uint32_t gq[4] = {g4.x, g4.y, g4.z, g4.w}, uq[4] = {u4.x, u4.y, u4.z, u4.w}, dq[4] = {d4.x, d4.y, d4.z, d4.w};
-      uint32_t a[4], b[4], h4[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float dg[2], du[2], hh[2];
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const float g = __uint_as_float(x ? gq[i] & 0xffff0000u : gq[i] << 16), u = __uint_as_float(x ? uq[i] & 0xffff0000u : uq[i] << 16);
-          const float d = __uint_as_float(x ? dq[i] & 0xffff0000u : dq[i] << 16);
-          const float sg = 1.f / (1.f + __expf(-g)), silu = g * sg, h = silu * u;
-          dot = fmaf(h, d, dot);
-          const float wd = w * d;
-          dg[x] = wd * u * (sg + silu * (1.f - sg));
-          du[x] = wd * silu;
-          hh[x] = w * h;
-        }
-        a[i] = pack_bf16(dg[0], dg[1]), b[i] = pack_bf16(du[0], du[1]), h4[i] = pack_bf16(hh[0], hh[1]);
-      }
-      dg4 = make_uint4(a[0], a[1], a[2], a[3]), du4 = make_uint4(b[0], b[1], b[2], b[3]), hw4 = make_uint4(h4[0], h4[1], h4[2], h4[3]);
-    }
-    *reinterpret_cast<uint4*>(dgu + at) = dg4;
-    *reinterpret_cast<uint4*>(dgu + at + 16) = du4;
-    *reinterpret_cast<uint4*>(hw + r * I + c) = hw4;
-  }
-  dot = block_sum(dot, red);
-  if (threadIdx.x == 0 && s >= 0) dweights[s] = (W)dot;
-}
-// the gradient of the weight of a copy that goes nowhere
-template <typename W>
-__global__ void __launch_bounds__(256) moe_no_place_k(W* __restrict__ dweights, const int* __restrict__ place, long NK) {
-  mlb_pdl_sync();
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i < NK && place[i] < 0) dweights[i] = (W)0.f;
-}
-
 // ------------------------------------------------------------------ products
 // CTA pairs share a tile of 256 features x up to 256 tokens (token products) or 256 x 256 features (weight gradients): the leader issues tcgen05.mma.cta_group::2,
 // each CTA stages its 128 rows of A and its half of B and drains its own 128 tensor-memory lanes.  The weights are A and the tokens B, whose number
 // an instruction takes in steps of 32: an expert's last tile, and that of an expert with few tokens, is no wider than its rows.  Two accumulators, so that a tile's
 // epilogue runs under the next one's products.
-enum { GATE_UP, DOWN, DOWN_T, GATE_UP_T, D_GATE_UP, D_DOWN };
-constexpr int BK = 64, THREADS = 64 + 8 * 32;
+//   GATE_UP  [g | u] = xs Wgu^T, kept for backward or not, and h = silu(g) u
+//   DOWN     y = h Wd^T
+//   DOWN_T   dh = ys Wd, and from it dgu
+//   BACK     dWgu, dWd and dxs = dgu Wgu, one launch: tiles of all three behind one another, so that only one last wave leaves SMs idle
+enum { GATE_UP, DOWN, DOWN_T, BACK };
+constexpr int BK = 64;
+// An epilogue warp has 32 features, of CHUNK tokens at a time.  Its memory: GATE_UP, DOWN and BACK two places for what leaves (2 KB, and 1 KB for h), or one of 4 KB for a
+// weight gradient's rows; DOWN_T three places for [g | u], which arrive, become their gradients and leave, and one for dh.
+template <int MODE>
 struct Smem {
-  static constexpr int A_BYTES = 128 * BK * 2, STAGE_BYTES = 2 * A_BYTES, STAGES = 6, STAGING_BYTES = 8 * 4096;
-  static constexpr int TOTAL = STAGES * STAGE_BYTES + STAGING_BYTES + 256 + 1024;
+  static constexpr int EPI = MODE == DOWN_T ? 16 : 8, THREADS = 64 + 32 * EPI;      // epilogue warps
+  static constexpr int CHUNK = MODE == DOWN_T ? 16 : 32;
+  static constexpr int A_BYTES = 128 * BK * 2, STAGE_BYTES = 2 * A_BYTES, STAGES = MODE == DOWN_T ? 4 : MODE == GATE_UP ? 5 : 6;
+  static constexpr int PLACES = 2, PLACE = 128 * CHUNK, WARP_BYTES = MODE == DOWN_T ? PLACES * PLACE + PLACE / 2 : MODE == GATE_UP ? 2 * 2048 + 2 * 1024 : 4096;
+  static constexpr int TOTAL = STAGES * STAGE_BYTES + EPI * WARP_BYTES + 512 + 1024;
+  static_assert(WARP_BYTES % 1024 == 0 && TOTAL <= 232448, "shared memory of an SM");
 };
 struct GemmArgs {
-  const int* start;      // [E + 1] rows
+  const int *start, *order;      // rows of the experts [E + 1]; the experts, those with the most rows first
   const int4* tiles;
   const int* ntiles;
-  bf16 *out, *h;         // token products: [R, M]; h [R, M / 2] of GATE_UP, whose out may be null.  Weight gradients: [E, M, N]
-  int E, M, N, K;        // weight gradients: M x N each; token products: M features over K
-  int tiles_m, tiles_n;
+  bf16 *out, *h;         // [R, M]; GATE_UP (whose out may be null): h [R, M / 2].  DOWN_T: dgu [R, 2 M].  BACK: dxs
+  int E, M, K, tiles_m;  // token products: M features over K
+  // BACK
+  int C, I, per_gate_up, per_down;      // tiles of one expert (0: not asked for)
 };
-// A tile of the token products, or of one expert's weight gradient
-struct Item { int e, row0, rows, mt, nt; };
+enum { TOKENS, D_GATE_UP, D_DOWN };
+struct Item { int type, e, row0, rows, mt, nt; };
 template <int MODE>
 struct Items {      // items cid, cid + ncl, ... ; what the next one is read from memory is asked for ahead
-  static constexpr bool DW = MODE == D_GATE_UP || MODE == D_DOWN;
   const GemmArgs& g;
-  int i, step, n;
+  int i, step, n, grads;
   int4 ahead;
   __device__ __forceinline__ Items(const GemmArgs& g_, int cid, int ncl) : g(g_), i(cid), step(ncl) {
-    n = DW ? g.E * g.tiles_m * g.tiles_n : *g.ntiles * g.tiles_m;
+    grads = MODE == BACK ? g.E * (g.per_gate_up + g.per_down) : 0;
+    n = grads + (g.tiles_m > 0 ? *g.ntiles * g.tiles_m : 0);
     fetch();
   }
   __device__ __forceinline__ void fetch() {
     if (i >= n) return;
-    if (DW) {
-      const int e = i / (g.tiles_m * g.tiles_n);
+    if (MODE == BACK && i < grads) {
+      const int e = g.order[i / (g.per_gate_up + g.per_down)];
       ahead.x = e, ahead.y = g.start[e], ahead.z = g.start[e + 1];
     } else {
-      ahead = g.tiles[i / g.tiles_m];
+      ahead = g.tiles[(i - grads) / g.tiles_m];
     }
   }
   __device__ __forceinline__ bool next(Item& w) {
     if (i >= n) return false;
     w.e = ahead.x, w.row0 = ahead.y;
-    if (DW) {
-      const int x = i - w.e * g.tiles_m * g.tiles_n;
+    if (MODE == BACK && i < grads) {
+      const int x = i % (g.per_gate_up + g.per_down);
+      w.type = x < g.per_gate_up ? D_GATE_UP : D_DOWN;
       w.rows = ahead.z - ahead.y;
-      w.mt = x / g.tiles_n, w.nt = x - w.mt * g.tiles_n;
+      const int y = x < g.per_gate_up ? x : x - g.per_gate_up, nt = ((x < g.per_gate_up ? g.C : g.I) + 255) / 256;
+      w.mt = y / nt, w.nt = y - w.mt * nt;
     } else {
+      w.type = TOKENS;
       w.rows = ahead.z;
-      w.mt = i % g.tiles_m, w.nt = 0;
+      w.mt = (i - grads) % g.tiles_m, w.nt = 0;
     }
     i += step;
     fetch();
     return true;
   }
 };
-__device__ __forceinline__ float swiglu(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+// One warp's 32 x 64 accumulators (lane = row) as bf16 to its 4 KB buffer, from where they leave
+__device__ __forceinline__ void put_rows(uint8_t* buf, int lane, const uint32_t (&r)[32], const uint32_t (&r2)[32]) {
+  uint8_t* rowp = buf + lane * 128;
+#pragma unroll
+  for (int v = 0; v < 8; v++) {
+    const uint32_t* s = v < 4 ? &r[v * 8] : &r2[(v - 4) * 8];
+    uint4 pk;
+    pk.x = pack_bf16(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    pk.y = pack_bf16(__uint_as_float(s[2]), __uint_as_float(s[3]));
+    pk.z = pack_bf16(__uint_as_float(s[4]), __uint_as_float(s[5]));
+    pk.w = pack_bf16(__uint_as_float(s[6]), __uint_as_float(s[7]));
+    *reinterpret_cast<uint4*>(rowp + ((v ^ (lane & 7)) << 4)) = pk;
+  }
+}
+// What stands in a tile's place [token][32 features] of 64 bytes: unit u (8 features) of token t
+__device__ __forceinline__ int unit_at(int t, int u) { return t * 64 + ((u ^ ((t >> 1) & 3)) << 4); }
+
+// Two fp32 values an instruction
+typedef uint64_t Two;
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void parts(Two x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ Two two_bf16(uint32_t q) { return two(__uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t pack_two(Two x) {
+  float a, b;
+  parts(x, a, b);
+  return pack_bf16(a, b);
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ Two sigmoid2(Two g) {
+  float a, b;
+  parts(mul2(g, two(-1.44269504f, -1.44269504f)), a, b);
+  return two(rcp(1.f + ex2(a)), rcp(1.f + ex2(b)));
+}
+__device__ __forceinline__ Two swiglu2(Two g, Two u) { return mul2(mul2(g, sigmoid2(g)), u); }
+
+// SwiGLU's gradient, 8 neighbouring features of a row.  With s = sigmoid(g) and d = dh:  dg = d u s (1 + g (1 - s)),  du = d g s
+__device__ __forceinline__ void swiglu_bwd8(uint4& g4, uint4& u4, const uint4& d4) {
+  const uint32_t gq[4] = {g4.x, g4.y, g4.z, g4.w}, uq[4] = {u4.x, u4.y, u4.z, u4.w}, dq[4] = {d4.x, d4.y, d4.z, d4.w};
+  uint32_t a[4], b[4];
+  const Two one = two(1.f, 1.f), minus = two(-1.f, -1.f);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const Two g = two_bf16(gq[i]), u = two_bf16(uq[i]), d = two_bf16(dq[i]);
+    const Two s = sigmoid2(g), silu = mul2(g, s);
+    a[i] = pack_two(mul2(mul2(d, u), fma2(silu, fma2(s, minus, one), s)));
+    b[i] = pack_two(mul2(d, silu));
+  }
+  g4 = make_uint4(a[0], a[1], a[2], a[3]), u4 = make_uint4(b[0], b[1], b[2], b[3]);
+}
 
 template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmArgs g) {
-  constexpr bool DW = MODE == D_GATE_UP || MODE == D_DOWN, A_MN = MODE != GATE_UP && MODE != DOWN, B_MN = DW;
-  using S = Smem;
-  constexpr int STAGES = S::STAGES, ACC = 256;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Smem<MODE>::THREADS, 1)
+moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmB16, const __grid_constant__ CUtensorMap tmA1,
+           const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ CUtensorMap tmOut,
+           const __grid_constant__ CUtensorMap tmOut1, const __grid_constant__ CUtensorMap tmOut2, const GemmArgs g) {
+  using S = Smem<MODE>;
+  constexpr int STAGES = S::STAGES, ACC = 256, CHUNK = S::CHUNK, PASS = CHUNK * S::EPI / 4;
+  constexpr bool A_MN = MODE == DOWN_T || MODE == BACK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* staging = smem + STAGES * S::STAGE_BYTES;
-  uint64_t* full = (uint64_t*)(staging + S::STAGING_BYTES);
+  uint64_t* full = (uint64_t*)(staging + S::EPI * S::WARP_BYTES);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+  uint64_t* place_full = acc_empty + 2;      // [EPI][PLACES]
+  uint32_t* tmem_slot = (uint32_t*)(place_full + (MODE == DOWN_T ? S::EPI * S::PLACES : 0));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_ctarank();
@@ -349,7 +427,9 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; i++) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
-    for (int i = 0; i < 2; i++) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 16); }
+    for (int i = 0; i < 2; i++) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 2 * S::EPI); }
+    if (MODE == DOWN_T)
+      for (int i = 0; i < S::EPI * S::PLACES; i++) tc::mbar_init(&place_full[i], 1);
     tc::mbar_fence_init();
     tc::tma_prefetch_desc(&tmA);
     tc::tma_prefetch_desc(&tmB);
@@ -369,31 +449,36 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
       Items<MODE> items(g, cid, ncl);
       Item w;
       while (ok && items.next(w)) {
+        const bool grad = MODE == BACK && w.type != TOKENS;
         const int m0 = w.mt * 256 + (int)rank * 128;
-        const int kbs = DW ? (w.rows + BK - 1) / BK : (g.K + BK - 1) / BK;
+        const int kbs = ((grad ? w.rows : g.K) + BK - 1) / BK;
         const int half = ((w.rows + 31) & ~31) >> 1;      // token products: this CTA's tokens
+        const uint32_t bytes = 2 * (S::A_BYTES + (grad ? S::A_BYTES : half * 128));
         for (int kb = 0; kb < kbs; kb++) {
           if (!tc::mbar_wait(&empty[stage], phase ^ 1, 0x71)) { ok = false; break; }
           uint8_t* sA = smem + stage * S::STAGE_BYTES;
           uint8_t* sB = sA + S::A_BYTES;
           const uint32_t bar = tc::mapa_u32(tc::smem_u32(&full[stage]), 0);
-          if (rank == 0) tc::mbar_expect_tx(&full[stage], 2 * S::STAGE_BYTES);
-          if (MODE == GATE_UP) {      // rows in groups of 16 gate rows and the matching 16 up rows
-            tc::tma_load_5d_pair(sA, &tmA, bar, kb * BK, 0, 0, m0 / 32, w.e);
-          } else if (MODE == DOWN) {
-            tc::tma_load_3d_pair(sA, &tmA, bar, kb * BK, m0, w.e);
-          } else if (MODE == DOWN_T) {
-            for (int c = 0; c < 2; c++) tc::tma_load_3d_pair(sA + c * 8192, &tmA, bar, m0 + c * 64, kb * BK, w.e);
-          } else if (MODE == GATE_UP_T) {      // (K in the same groups)
-            for (int c = 0; c < 2; c++) tc::tma_load_5d_pair(sA + c * 8192, &tmA, bar, m0 + c * 64, 0, 0, kb * 2, w.e);
+          if (rank == 0) tc::mbar_expect_tx(&full[stage], bytes);
+          if (grad) {
+            const int y = w.row0 + kb * BK, n0 = w.nt * 256 + (int)rank * 128;
+            const CUtensorMap *a = w.type == D_GATE_UP ? &tmA1 : &tmA2, *b = w.type == D_GATE_UP ? &tmB1 : &tmB2;
+            for (int c = 0; c < 2; c++) tc::tma_load_2d_pair(sA + c * 8192, a, bar, m0 + c * 64, y);
+            for (int c = 0; c < 2; c++) tc::tma_load_2d_pair(sB + c * 8192, b, bar, n0 + c * 64, y);
           } else {
-            for (int c = 0; c < 2; c++) tc::tma_load_2d_pair(sA + c * 8192, &tmA, bar, m0 + c * 64, w.row0 + kb * BK);
-          }
-          if (DW) {
-            const int n0 = w.nt * 256 + (int)rank * 128;
-            for (int c = 0; c < 2; c++) tc::tma_load_2d_pair(sB + c * 8192, &tmB, bar, n0 + c * 64, w.row0 + kb * BK);
-          } else {
-            tc::tma_load_2d_pair(sB, &tmB, bar, kb * BK, w.row0 + (int)rank * half);
+            if (MODE == GATE_UP) {      // rows in groups of 16 gate rows and the matching 16 up rows
+              tc::tma_load_5d_pair(sA, &tmA, bar, kb * BK, 0, 0, m0 / 32, w.e);
+            } else if (MODE == DOWN) {
+              tc::tma_load_3d_pair(sA, &tmA, bar, kb * BK, m0, w.e);
+            } else if (MODE == DOWN_T) {
+              for (int c = 0; c < 2; c++) tc::tma_load_3d_pair(sA + c * 8192, &tmA, bar, m0 + c * 64, kb * BK, w.e);
+            } else {                    // (K in the same groups)
+              for (int c = 0; c < 2; c++) tc::tma_load_5d_pair(sA + c * 8192, &tmA, bar, m0 + c * 64, 0, 0, kb * 2, w.e);
+            }
+            const int y = w.row0 + (int)rank * half;
+            if (half == 128) tc::tma_load_2d_pair(sB, &tmB, bar, kb * BK, y);
+            else
+              for (int c = 0; c < half; c += 16) tc::tma_load_2d_pair(sB + c * 128, &tmB16, bar, kb * BK, y + c);
           }
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
@@ -407,9 +492,10 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
       Items<MODE> items(g, cid, ncl);
       Item w;
       while (ok && items.next(w)) {
-        const int kbs = DW ? (w.rows + BK - 1) / BK : (g.K + BK - 1) / BK;
+        const bool grad = MODE == BACK && w.type != TOKENS;
+        const int kbs = ((grad ? w.rows : g.K) + BK - 1) / BK;
         if (kbs == 0) continue;      // an expert without tokens
-        const uint32_t idesc = tc::idesc_bf16(256, DW ? 256 : (w.rows + 31) & ~31, A_MN ? 1 : 0, B_MN ? 1 : 0);
+        const uint32_t idesc = tc::idesc_bf16(256, grad ? 256 : (w.rows + 31) & ~31, A_MN ? 1 : 0, grad ? 1 : 0);
         const int acc = it & 1, acc_phase = (it >> 1) & 1;
         it++;
         if (!tc::mbar_wait(&acc_empty[acc], acc_phase ^ 1, 0x72)) { ok = false; break; }
@@ -420,12 +506,12 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
           tc::tc_fence_after();
           const uint32_t sA = tc::smem_u32(smem + stage * S::STAGE_BYTES);
           const uint32_t sB = sA + S::A_BYTES;
-          const int steps = DW ? min(BK, w.rows - kb * BK) / 16 : BK / 16;      // (the rows behind an expert's are another's)
+          const int steps = grad ? min(BK, w.rows - kb * BK) / 16 : BK / 16;      // (the rows behind an expert's are another's)
 #pragma unroll
           for (int k = 0; k < BK / 16; k++) {
-            if (DW && k >= steps) break;
+            if (MODE == BACK && k >= steps) break;
             const uint64_t da = A_MN ? tc::smem_desc_sw128(sA + k * 2048, 8192, 1024) : tc::smem_desc_sw128(sA + k * 32, 16, 1024);
-            const uint64_t db = B_MN ? tc::smem_desc_sw128(sB + k * 2048, 8192, 1024) : tc::smem_desc_sw128(sB + k * 32, 16, 1024);
+            const uint64_t db = grad ? tc::smem_desc_sw128(sB + k * 2048, 8192, 1024) : tc::smem_desc_sw128(sB + k * 32, 16, 1024);
             tc::mma_bf16_ss_pair(d_tmem, da, db, idesc, (kb > 0 || k > 0) ? 1u : 0u);
           }
           tc::mma_commit_pair(&empty[stage]);
@@ -435,80 +521,143 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
       }
     }
   } else {
-    // ---------------------------------------------------------------- epilogue (warps 2..9 of each CTA)
+    // ---------------------------------------------------------------- epilogue (warps 2 .. of each CTA): lanes 32 lg .., every EPI / 4-th chunk or half
     const int lg = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* buf = staging + (warp - 2) * 4096;
-    const uint32_t sbuf = tc::smem_u32(buf);
-    int it = 0;
+    uint8_t* buf = staging + (warp - 2) * S::WARP_BYTES;
+    const int tok = (lane >> 4) | (lane >> 1 & 6), unit = lane & 3;      // of four tokens 8 i + tok this lane has features m0 + 8 unit ... (tokens in an order that spares banks)
+    int it = 0, n = 0;      // items that had products; chunks of 32 tokens
     bool ok = true;
     Items<MODE> items(g, cid, ncl);
     Item w;
+    // DOWN_T: the products behind a chunk's gradients are asked for a chunk ahead
+    Items<MODE> ahead_items(g, cid, ncl);
+    Item ahead = {};
+    int ahead_c = 0, ahead_n = 0;
+    auto first_row = [&](const Item& x) { return x.mt * 256 + (int)rank * 128 + lg * 32; };
+    auto advance = [&]() {      // the next chunk of this warp; rows 0: there is none
+      ahead_c += PASS;
+      while (ahead_c >= ((ahead.rows + 31) & ~31) || first_row(ahead) >= g.M) {
+        if (!ahead_items.next(ahead)) { ahead.rows = 0; return; }
+        ahead_c = half * CHUNK;
+      }
+    };
+    auto ask = [&]() {
+      if (ahead.rows == 0) return;
+      if (lane == 0) {
+        uint64_t* bar = &place_full[(warp - 2) * S::PLACES + ahead_n % S::PLACES];
+        tc::mbar_expect_tx(bar, S::PLACE);
+        tc::tma_load_2d(buf + ahead_n % S::PLACES * S::PLACE, &tmA1, bar, 2 * first_row(ahead), ahead.row0 + ahead_c);
+      }
+      ahead_n++;
+      advance();
+    };
+    if constexpr (MODE == DOWN_T) {
+      advance();
+      ask();
+    }
     while (ok && items.next(w)) {
-      const int m0 = w.mt * 256 + (int)rank * 128 + lg * 32;
-      const bool some = !DW || w.rows > 0;
+      const bool grad = MODE == BACK && w.type != TOKENS;
+      const int m0 = first_row(w);
+      const bool some = !grad || w.rows > 0;
       const int acc = it & 1, acc_phase = (it >> 1) & 1;
+      const bool live = m0 < g.M;
       if (some) {
         it++;
         if (!__all_sync(0xffffffffu, tc::mbar_wait(&acc_full[acc], acc_phase, 0x74))) { ok = false; break; }
         tc::tc_fence_after();
       }
       const uint32_t taddr = tmem_base + ((uint32_t)(lg * 32) << 16) + acc * ACC;
-      if constexpr (!DW) {
-        const bool live = m0 < g.M;
-        const int unit = lane & 3, tok = lane >> 2;
-        for (int c = half * 32; c < w.rows; c += 64) {
-          uint32_t r[2][16];
+      if (!grad) {
+        const int last = (w.rows + 31) & ~31;      // (what fills up an expert's rows belongs to it)
+        for (int c = half * CHUNK; c < last; c += PASS) {
+          if (!live) break;      // (warp-uniform)
+          // what left two chunks ago (a tile's rows: before) has been read, its places are free
+          if constexpr (MODE != DOWN_T) {
+            if (lane == 0) tc::tma_wait_group_read<1>();
+            __syncwarp();
+          }
+          uint8_t* place = buf + (MODE == DOWN_T ? S::PLACES * S::PLACE : (n & 1) * 2048);
+          const uint32_t splace = tc::smem_u32(place);
+          uint32_t r[2][CHUNK / 2];
           tc::tmem_ld_frag_wait(taddr + c, r);
-          if (!live) continue;      // (warp-uniform)
-          uint32_t p[2][8];         // p[h][2 j + v]: tokens 8 j + 2 (lane % 4) + {0, 1} of feature 16 h + 8 v + lane / 4
-#pragma unroll
-          for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int q = 0; q < 8; q++) p[h][q] = pack_bf16(__uint_as_float(r[h][2 * q]), __uint_as_float(r[h][2 * q + 1]));
+          // r[h][4 j + 2 v + x]: token 8 j + 2 (lane % 4) + x of feature 16 h + 8 v + lane / 4
           if (MODE != GATE_UP || g.out != nullptr) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const int t = 8 * j + (lane & 7), u = lane >> 3;
-              tc::stmatrix_x4_trans(sbuf + t * 64 + ((u ^ ((t >> 1) & 3)) << 4), p[0][2 * j], p[0][2 * j + 1], p[1][2 * j], p[1][2 * j + 1]);
+            for (int j = 0; j < CHUNK / 8; j++) {
+              uint32_t p[4];
+#pragma unroll
+              for (int q = 0; q < 4; q++) p[q] = pack_bf16(__uint_as_float(r[q >> 1][4 * j + 2 * (q & 1)]), __uint_as_float(r[q >> 1][4 * j + 2 * (q & 1) + 1]));
+              tc::stmatrix_x4_trans(splace + unit_at(8 * j + (lane & 7), lane >> 3), p[0], p[1], p[2], p[3]);
             }
           }
           if constexpr (MODE == GATE_UP) {      // feature 8 v + lane / 4: h = 0 its gate, h = 1 its up value
+            uint8_t* hplace = buf + 2 * 2048 + (n & 1) * 1024;
             uint32_t x[8];
 #pragma unroll
             for (int q = 0; q < 8; q++)
-              x[q] = pack_bf16(swiglu(__uint_as_float(p[0][q] << 16), __uint_as_float(p[1][q] << 16)),
-                               swiglu(__uint_as_float(p[0][q] & 0xffff0000u), __uint_as_float(p[1][q] & 0xffff0000u)));
+              x[q] = pack_two(swiglu2(two(__uint_as_float(r[0][2 * q]), __uint_as_float(r[0][2 * q + 1])), two(__uint_as_float(r[1][2 * q]), __uint_as_float(r[1][2 * q + 1]))));
 #pragma unroll
             for (int j = 0; j < 2; j++) {
               const int t = 16 * j + 8 * (lane >> 4) + (lane & 7), u = (lane >> 3) & 1;
-              tc::stmatrix_x4_trans(sbuf + 2048 + t * 32 + ((u ^ ((t >> 2) & 1)) << 4), x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+              tc::stmatrix_x4_trans(tc::smem_u32(hplace) + t * 32 + ((u ^ ((t >> 2) & 1)) << 4), x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
             }
-          }
-          __syncwarp();
-          if (MODE != GATE_UP || g.out != nullptr) {
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (g.out != nullptr) tc::tma_store_2d(&tmOut, place, m0, w.row0 + c);
+              tc::tma_store_2d(&tmB1, hplace, m0 / 2, w.row0 + c);
+              tc::tma_commit_group();
+            }
+          } else if constexpr (MODE == DOWN_T) {
+            uint8_t* gu = buf + n % S::PLACES * S::PLACE;
+            __syncwarp();
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(&place_full[(warp - 2) * S::PLACES + n % S::PLACES], (n / S::PLACES) & 1, 0x75))) { ok = false; break; }
+            const int ch = (unit >> 1) * 4 + (unit & 1);      // 16-byte unit of the gate's features in a row of [16 gate | 16 up | 16 gate | 16 up]
+            // (all loads before the first store: behind one they would be waited for a token at a time)
+            uint4 x[CHUNK / 8][3];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const int t = 8 * i + tok;
-              const uint4 v = *reinterpret_cast<const uint4*>(buf + t * 64 + ((unit ^ ((t >> 1) & 3)) << 4));
-              if (c + t < w.rows && m0 + unit * 8 < g.M) *reinterpret_cast<uint4*>(g.out + (size_t)(w.row0 + c + t) * g.M + m0 + unit * 8) = v;
+            for (int i = 0; i < CHUNK / 8; i++) {
+              const int t = 8 * i + tok, sw = t & 7;
+              x[i][0] = *reinterpret_cast<const uint4*>(gu + t * 128 + ((ch ^ sw) << 4));
+              x[i][1] = *reinterpret_cast<const uint4*>(gu + t * 128 + (((ch + 2) ^ sw) << 4));
+              x[i][2] = *reinterpret_cast<const uint4*>(place + unit_at(t, unit));
             }
-          }
-          if constexpr (MODE == GATE_UP) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-              const int t = 16 * i + (lane >> 1), u = lane & 1;
-              const uint4 v = *reinterpret_cast<const uint4*>(buf + 2048 + t * 32 + ((u ^ ((t >> 2) & 1)) << 4));
-              if (c + t < w.rows) *reinterpret_cast<uint4*>(g.h + (size_t)(w.row0 + c + t) * (g.M / 2) + m0 / 2 + u * 8) = v;
+            for (int i = 0; i < CHUNK / 8; i++) {
+              swiglu_bwd8(x[i][0], x[i][1], x[i][2]);
+              if (c + 8 * i + tok >= w.rows) x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);      // (rows that fill up an expert's: zeros, whatever stands in them)
+            }
+            if (lane == 0) tc::tma_wait_group_read<0>();      // the chunk before has left its place: the next one may arrive there
+            __syncwarp();
+            ask();
+#pragma unroll
+            for (int i = 0; i < CHUNK / 8; i++) {
+              const int t = 8 * i + tok, sw = t & 7;
+              *reinterpret_cast<uint4*>(gu + t * 128 + ((ch ^ sw) << 4)) = x[i][0];
+              *reinterpret_cast<uint4*>(gu + t * 128 + (((ch + 2) ^ sw) << 4)) = x[i][1];
+            }
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tc::tma_store_2d(&tmOut, gu, 2 * m0, w.row0 + c);
+              tc::tma_commit_group();
+            }
+          } else {
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tc::tma_store_2d(&tmOut, place, m0, w.row0 + c);
+              tc::tma_commit_group();
             }
           }
-          __syncwarp();
+          n++;
         }
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_u32(tc::smem_u32(&acc_empty[acc]), 0));
-      } else {
-        const int n0 = w.nt * 256 + half * 128;
-        bf16* out = g.out + (size_t)w.e * g.M * g.N;
+      } else if constexpr (MODE == BACK) {
+        const bool gu = w.type == D_GATE_UP;
+        const int M = gu ? 2 * g.I : g.C, N = gu ? g.C : g.I;
 #pragma unroll 1
         for (int c = 0; c < 2; c++) {
           uint32_t r[32], r2[32];
@@ -523,62 +672,58 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
 #pragma unroll
             for (int i = 0; i < 32; i++) r[i] = r2[i] = 0;
           }
-          const int col0 = n0 + c * 64;
-          if (m0 >= g.M || col0 >= g.N) continue;      // (warp-uniform)
-          uint8_t* rowp = buf + lane * 128;
-#pragma unroll
-          for (int v = 0; v < 8; v++) {
-            const uint32_t* s = v < 4 ? &r[v * 8] : &r2[(v - 4) * 8];
-            uint4 pk;
-            pk.x = pack_bf16(__uint_as_float(s[0]), __uint_as_float(s[1]));
-            pk.y = pack_bf16(__uint_as_float(s[2]), __uint_as_float(s[3]));
-            pk.z = pack_bf16(__uint_as_float(s[4]), __uint_as_float(s[5]));
-            pk.w = pack_bf16(__uint_as_float(s[6]), __uint_as_float(s[7]));
-            *reinterpret_cast<uint4*>(rowp + ((v ^ (lane & 7)) << 4)) = pk;
-          }
+          const int col0 = w.nt * 256 + half * 128 + c * 64;
+          if (m0 >= M || col0 >= N) continue;      // (warp-uniform)
+          if (lane == 0) tc::tma_wait_group_read<0>();
           __syncwarp();
-          const int ch = lane & 7, col = col0 + ch * 8;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int row = i * 4 + (lane >> 3), m = m0 + row;
-            const uint4 v = *reinterpret_cast<const uint4*>(buf + row * 128 + ((ch ^ (row & 7)) << 4));
-            // the rows of dWgu come in groups of 16 gate rows and 16 up rows
-            const int to = MODE == D_GATE_UP ? (m >> 5) * 16 + (m & 15) + (m & 16 ? g.M / 2 : 0) : m;
-            if (m < g.M && col < g.N) *reinterpret_cast<uint4*>(out + (size_t)to * g.N + col) = v;
-          }
+          put_rows(buf, lane, r, r2);
+          tc::fence_async_smem();
           __syncwarp();
+          if (lane == 0) {
+            if (gu) tc::tma_store_5d(&tmOut1, buf, col0, 0, 0, m0 >> 5, w.e);      // (rows of 16 of the gate and 16 of the up projection)
+            else tc::tma_store_3d(&tmOut2, buf, col0, m0, w.e);
+            tc::tma_commit_group();
+          }
         }
       }
     }
+    if (lane == 0) tc::tma_wait_group<0>();
   }
   tc::tc_fence_before();
   tc::cluster_sync();      // no CTA frees tensor memory or leaves while its peer may still signal or read it
   if (warp == 1) tc::tmem_dealloc_pair(tmem_base, 2 * ACC);
 }
 
+struct Maps { CUtensorMap a, b, b16, a1, b1, a2, b2, out, out1, out2; };
 template <int MODE>
-int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& g, long items, cudaStream_t st) {
+int launch_gemm(const Maps& m, const GemmArgs& g, long items, cudaStream_t st) {
   auto kern = moe_gemm_k<MODE>;
   static std::atomic<unsigned long long> done{0};
-  cudaError_t e = mlb_allow_smem(kern, Smem::TOTAL, done);
+  cudaError_t e = mlb_allow_smem(kern, Smem<MODE>::TOTAL, done);
   if (e != cudaSuccess) return (int)e;
   static const int most = [&] {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(mlb_sm_count() & ~1);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Smem::TOTAL;
+    cfg.blockDim = dim3(Smem<MODE>::THREADS);
+    cfg.dynamicSmemBytes = Smem<MODE>::TOTAL;
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) { cudaGetLastError(); n = mlb_sm_count() / 2; }
     return std::min(n, mlb_sm_count() / 2);
   }();
   if (items <= 0) return 0;
-  return (int)mlb_launch_tmem(true, kern, dim3(2 * (unsigned)std::min<long>(items, most)), dim3(THREADS), (size_t)Smem::TOTAL, st, a, b, g);
+  return (int)mlb_launch_tmem(true, kern, dim3(2 * (unsigned)std::min<long>(items, most)), dim3(Smem<MODE>::THREADS), (size_t)Smem<MODE>::TOTAL, st, m.a, m.b, m.b16, m.a1, m.b1, m.a2, m.b2, m.out, m.out1, m.out2, g);
 }
 
-bool map_tokens(CUtensorMap* m, const bf16* base, long rows, int K) {      // [rows, K], K-major
+bool map_tokens(Maps& m, const bf16* base, long rows, int K) {      // [rows, K], K-major
   const uint64_t d[2] = {(uint64_t)K, (uint64_t)rows}, s[1] = {2ull * K};
-  const uint32_t b[2] = {64, 128};
-  return mlb_make_tmap_nd(m, base, 2, d, s, b);
+  const uint32_t b[2] = {64, 128}, b16[2] = {64, 16};
+  return mlb_make_tmap_nd(&m.b, base, 2, d, s, b) && mlb_make_tmap_nd(&m.b16, base, 2, d, s, b16);
+}
+// the same for what leaves an epilogue warp or arrives there: some tokens of `width` columns
+bool map_chunk(CUtensorMap* m, const bf16* base, long rows, int cols, uint32_t width, uint32_t tokens = 32) {
+  const uint64_t d[2] = {(uint64_t)cols, (uint64_t)rows}, s[1] = {2ull * cols};
+  const uint32_t b[2] = {width, tokens};
+  return mlb_make_tmap_nd(m, base, 2, d, s, b, 2 * (int)width);
 }
 bool map_rows(CUtensorMap* m, const bf16* base, long rows, int cols) {      // the same, its columns M or N and its rows the reduction
   const uint64_t d[2] = {(uint64_t)cols, (uint64_t)rows}, s[1] = {2ull * cols};
@@ -615,10 +760,14 @@ int dispatch(bf16* out, const bf16* x, const PlanArgs& P, const Sizes& z, long l
   return (int)mlb_launch(moe_dispatch_k, dim3((unsigned)((z.p.rows + 7) / 8)), dim3(256), 0, st, out, x, (const int*)P.source, (const int*)(P.start + z.E), ldx, z.k, z.C);
 }
 template <typename W>
+int dispatch_bwd(bf16* out, W* dw, const bf16* dout, const bf16* y, const W* weights, const PlanArgs& P, const Sizes& z, long ldo, cudaStream_t st) {
+  return (int)mlb_launch(moe_dispatch_bwd_k<W>, dim3((unsigned)((z.NK + z.p.rows + 7) / 8)), dim3(256), 0, st, out, dw, dout, y, weights, (const int*)P.place, (const int*)P.source,
+                         (const int*)(P.start + z.E), ldo, z.NK, z.k, z.C);
+}
+template <typename W>
 int combine(bf16* out, const bf16* y, const W* w, const PlanArgs& P, const Sizes& z, cudaStream_t st) {
   return (int)mlb_launch(moe_combine_k<W>, dim3((unsigned)((z.N * (z.C / 8) + 255) / 256)), dim3(256), 0, st, out, y, w, (const int*)P.place, z.N, z.k, z.C);
 }
-
 }  // namespace
 
 #define MLB_TRY(x) do { const int rc_ = (x); if (rc_ != 0) return rc_; } while (0)
@@ -643,7 +792,7 @@ MLB_API int mlb_moe_plan(int* plan, const int* idx, long N, int k, int E, cudaSt
   if (z.p.blocks > 1) MLB_TRY((int)mlb_launch(moe_hist_k, dim3(z.p.blocks), dim3(PLAN_THREADS), (size_t)4 * E, st, P));
   return (int)mlb_launch(moe_place_k, dim3(z.p.blocks), dim3(PLAN_THREADS), (size_t)4 * E * (2 + PLAN_WARPS), st, P);
 }
-// xs [R, C], gu [R, 2 I] (null: not kept), h [R, I], y [R, C] are workspace, the first two what backward needs
+// xs [R, C], gu [R, 2 I] (null: not kept), h [R, I] and y [R, C] are workspace, and what backward needs
 MLB_API int mlb_moe_fwd(void* out, void* xs, void* gu, void* h, void* y, const void* x, const void* weights, const void* gate_up, const void* down, const int* plan, long N, long ldx, int k,
                         int E, int C, int I, int wbits, cudaStream_t st) {
   Sizes z;
@@ -651,53 +800,51 @@ MLB_API int mlb_moe_fwd(void* out, void* xs, void* gu, void* h, void* y, const v
   if (off16({out, xs, gu, h, y, x, gate_up, down, plan}) || ldx % 8 != 0 || (wbits != 16 && wbits != 32)) return -7;
   if (z.NK == 0) return 0;
   const PlanArgs P = plan_args(const_cast<int*>(plan), nullptr, z);
-  alignas(64) CUtensorMap a, b;
+  alignas(64) Maps m = {};
   MLB_TRY(dispatch((bf16*)xs, (const bf16*)x, P, z, ldx, st));
-  GemmArgs g = {P.start, P.tiles, P.ntiles, (bf16*)gu, (bf16*)h, E, 2 * I, 0, C, (2 * I + 255) / 256, 1};
-  if (!map_gate_up(&a, (const bf16*)gate_up, E, C, I, 4) || !map_tokens(&b, (const bf16*)xs, z.p.rows, C)) return -2;
-  MLB_TRY(launch_gemm<GATE_UP>(a, b, g, (long)z.p.max_tiles * g.tiles_m, st));
-  g = {P.start, P.tiles, P.ntiles, (bf16*)y, nullptr, E, C, 0, I, (C + 255) / 256, 1};
-  if (!map_down(&a, (const bf16*)down, E, C, I, 128) || !map_tokens(&b, (const bf16*)h, z.p.rows, I)) return -2;
-  MLB_TRY(launch_gemm<DOWN>(a, b, g, (long)z.p.max_tiles * g.tiles_m, st));
+  GemmArgs g = {};
+  g.start = P.start, g.order = P.order, g.tiles = P.tiles, g.ntiles = P.ntiles, g.E = E;
+  g.out = (bf16*)gu, g.h = (bf16*)h, g.M = 2 * I, g.K = C, g.tiles_m = (2 * I + 255) / 256;
+  if (!map_gate_up(&m.a, (const bf16*)gate_up, E, C, I, 4) || !map_tokens(m, (const bf16*)xs, z.p.rows, C) || !map_chunk(&m.b1, g.h, z.p.rows, I, 16) ||
+      (g.out != nullptr && !map_chunk(&m.out, g.out, z.p.rows, 2 * I, 32)))
+    return -2;
+  MLB_TRY(launch_gemm<GATE_UP>(m, g, (long)z.p.max_tiles * g.tiles_m, st));
+  g.out = (bf16*)y, g.h = nullptr, g.M = C, g.K = I, g.tiles_m = (C + 255) / 256;
+  if (!map_down(&m.a, (const bf16*)down, E, C, I, 128) || !map_tokens(m, (const bf16*)h, z.p.rows, I) || !map_chunk(&m.out, g.out, z.p.rows, C, 32)) return -2;
+  MLB_TRY(launch_gemm<DOWN>(m, g, (long)z.p.max_tiles * g.tiles_m, st));
   return wbits == 16 ? combine((bf16*)out, (const bf16*)y, (const bf16*)weights, P, z, st) : combine((bf16*)out, (const bf16*)y, (const float*)weights, P, z, st);
 }
-// ys [R, C], dh [R, I], dgu [R, 2 I], hw [R, I], dxs [R, C]: workspace.  dx, dgate_up and ddown that are null are not formed
-MLB_API int mlb_moe_bwd(void* dx, void* dweights, void* dgate_up, void* ddown, void* ys, void* dh, void* dgu, void* hw, void* dxs, const void* dout, const void* xs, const void* gu,
-                        const void* weights, const void* gate_up, const void* down, const int* plan, long N, long ldo, int k, int E, int C, int I, int wbits, cudaStream_t st) {
+// ys [R, C], dgu [R, 2 I], dxs [R, C]: workspace.  dx, dgate_up and ddown that are null are not formed
+MLB_API int mlb_moe_bwd(void* dx, void* dweights, void* dgate_up, void* ddown, void* ys, void* dgu, void* dxs, const void* dout, const void* xs, const void* gu, const void* h,
+                        const void* y, const void* weights, const void* gate_up, const void* down, const int* plan, long N, long ldo, int k, int E, int C, int I, int wbits, cudaStream_t st) {
   Sizes z;
   MLB_TRY(sizes(z, N, k, E, C, I));
-  if (off16({dx, dgate_up, ddown, ys, dh, dgu, hw, dxs, dout, xs, gu, gate_up, down, plan}) || ldo % 8 != 0 || (wbits != 16 && wbits != 32)) return -7;
+  if (off16({dx, dgate_up, ddown, ys, dgu, dxs, dout, xs, gu, h, y, gate_up, down, plan}) || ldo % 8 != 0 || (wbits != 16 && wbits != 32)) return -7;
   if (z.NK == 0) return 0;
   const PlanArgs P = plan_args(const_cast<int*>(plan), nullptr, z);
-  const int* rows = P.start + E;
-  alignas(64) CUtensorMap a, b;
-  MLB_TRY(dispatch((bf16*)ys, (const bf16*)dout, P, z, ldo, st));
-  GemmArgs g = {P.start, P.tiles, P.ntiles, (bf16*)dh, nullptr, E, I, 0, C, (I + 255) / 256, 1};
-  if (!map_down(&a, (const bf16*)down, E, C, I, 64) || !map_tokens(&b, (const bf16*)ys, z.p.rows, C)) return -2;
-  MLB_TRY(launch_gemm<DOWN_T>(a, b, g, (long)z.p.max_tiles * g.tiles_m, st));
-  const dim3 every((unsigned)z.p.rows), copies((unsigned)((z.NK + 255) / 256));
-  if (wbits == 16) {
-    MLB_TRY((int)mlb_launch(moe_swiglu_bwd_k<bf16>, every, dim3(128), 0, st, (bf16*)dgu, (bf16*)hw, (bf16*)dweights, (const bf16*)dh, (const bf16*)gu, (const bf16*)weights, (const int*)P.source, rows, I));
-    MLB_TRY((int)mlb_launch(moe_no_place_k<bf16>, copies, dim3(256), 0, st, (bf16*)dweights, (const int*)P.place, z.NK));
-  } else {
-    MLB_TRY((int)mlb_launch(moe_swiglu_bwd_k<float>, every, dim3(128), 0, st, (bf16*)dgu, (bf16*)hw, (float*)dweights, (const bf16*)dh, (const bf16*)gu, (const float*)weights, (const int*)P.source, rows, I));
-    MLB_TRY((int)mlb_launch(moe_no_place_k<float>, copies, dim3(256), 0, st, (float*)dweights, (const int*)P.place, z.NK));
+  const long R = z.p.rows;
+  alignas(64) Maps m = {};
+  MLB_TRY(wbits == 16 ? dispatch_bwd((bf16*)ys, (bf16*)dweights, (const bf16*)dout, (const bf16*)y, (const bf16*)weights, P, z, ldo, st)
+                      : dispatch_bwd((bf16*)ys, (float*)dweights, (const bf16*)dout, (const bf16*)y, (const float*)weights, P, z, ldo, st));
+  if (dx == nullptr && dgate_up == nullptr && ddown == nullptr) return 0;
+  GemmArgs g = {};
+  g.start = P.start, g.order = P.order, g.tiles = P.tiles, g.ntiles = P.ntiles, g.E = E;
+  g.out = (bf16*)dgu, g.M = I, g.K = C, g.tiles_m = (I + 255) / 256;
+  if (dx != nullptr || dgate_up != nullptr) {
+    constexpr int chunk = Smem<DOWN_T>::CHUNK;
+    if (!map_down(&m.a, (const bf16*)down, E, C, I, 64) || !map_tokens(m, (const bf16*)ys, R, C) || !map_chunk(&m.a1, (const bf16*)gu, R, 2 * I, 64, chunk) ||
+        !map_chunk(&m.out, g.out, R, 2 * I, 64, chunk))
+      return -2;
+    MLB_TRY(launch_gemm<DOWN_T>(m, g, (long)z.p.max_tiles * g.tiles_m, st));
   }
-  if (dx != nullptr) {
-    g = {P.start, P.tiles, P.ntiles, (bf16*)dxs, nullptr, E, C, 0, 2 * I, (C + 255) / 256, 1};
-    if (!map_gate_up(&a, (const bf16*)gate_up, E, C, I, 2) || !map_tokens(&b, (const bf16*)dgu, z.p.rows, 2 * I)) return -2;
-    MLB_TRY(launch_gemm<GATE_UP_T>(a, b, g, (long)z.p.max_tiles * g.tiles_m, st));
-    MLB_TRY(combine((bf16*)dx, (const bf16*)dxs, (const float*)nullptr, P, z, st));
-  }
-  if (dgate_up != nullptr) {
-    g = {P.start, P.tiles, P.ntiles, (bf16*)dgate_up, nullptr, E, 2 * I, C, 0, (2 * I + 255) / 256, (C + 255) / 256};
-    if (!map_rows(&a, (const bf16*)dgu, z.p.rows, 2 * I) || !map_rows(&b, (const bf16*)xs, z.p.rows, C)) return -2;
-    MLB_TRY(launch_gemm<D_GATE_UP>(a, b, g, (long)E * g.tiles_m * g.tiles_n, st));
-  }
-  if (ddown != nullptr) {
-    g = {P.start, P.tiles, P.ntiles, (bf16*)ddown, nullptr, E, C, I, 0, (C + 255) / 256, (I + 255) / 256};
-    if (!map_rows(&a, (const bf16*)ys, z.p.rows, C) || !map_rows(&b, (const bf16*)hw, z.p.rows, I)) return -2;
-    MLB_TRY(launch_gemm<D_DOWN>(a, b, g, (long)E * g.tiles_m * g.tiles_n, st));
-  }
-  return 0;
+  g.out = (bf16*)dxs, g.M = C, g.K = 2 * I, g.tiles_m = dx != nullptr ? (C + 255) / 256 : 0;
+  g.C = C, g.I = I;
+  g.per_gate_up = dgate_up != nullptr ? ((2 * I + 255) / 256) * ((C + 255) / 256) : 0;
+  g.per_down = ddown != nullptr ? ((C + 255) / 256) * ((I + 255) / 256) : 0;
+  if (!map_gate_up(&m.a, (const bf16*)gate_up, E, C, I, 2) || !map_tokens(m, (const bf16*)dgu, R, 2 * I) || !map_rows(&m.a1, (const bf16*)dgu, R, 2 * I) ||
+      !map_rows(&m.b1, (const bf16*)xs, R, C) || !map_rows(&m.a2, (const bf16*)ys, R, C) || !map_rows(&m.b2, (const bf16*)h, R, I) || (dx != nullptr && !map_chunk(&m.out, g.out, R, C, 32)) ||
+      (dgate_up != nullptr && !map_gate_up(&m.out1, (const bf16*)dgate_up, E, C, I, 1)) || (ddown != nullptr && !map_down(&m.out2, (const bf16*)ddown, E, C, I, 32)))
+    return -2;
+  MLB_TRY(launch_gemm<BACK>(m, g, (long)E * (g.per_gate_up + g.per_down) + (long)z.p.max_tiles * g.tiles_m, st));
+  return dx != nullptr ? combine((bf16*)dx, (const bf16*)dxs, (const float*)nullptr, P, z, st) : 0;
 }

@@ -119,6 +119,15 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                "r"(x), "r"(y)
                : "memory");
 }
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* smem_src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_5d(const CUtensorMap* map, const void* smem_src, int x, int y, int z, int u, int v) {
+  asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];" ::"l"(map), "r"(smem_u32(smem_src)), "r"(x), "r"(y),
+               "r"(z), "r"(u), "r"(v)
+               : "memory");
+}
 __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, const void* smem_src, int x, int y) {
   asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
                "r"(smem_u32(smem_src)), "r"(x), "r"(y)
@@ -293,6 +302,17 @@ __device__ __forceinline__ void tmem_ld_pairs_wait(uint32_t taddr_a, uint32_t (&
         "=&r"(b[0][0]), "=&r"(b[0][1]), "=&r"(b[0][2]), "=&r"(b[0][3]), "=&r"(b[0][4]), "=&r"(b[0][5]), "=&r"(b[0][6]), "=&r"(b[0][7]),
         "=&r"(b[1][0]), "=&r"(b[1][1]), "=&r"(b[1][2]), "=&r"(b[1][3]), "=&r"(b[1][4]), "=&r"(b[1][5]), "=&r"(b[1][6]), "=&r"(b[1][7])
       : "r"(taddr_a), "r"(taddr_a + (16u << 16)), "r"(taddr_b), "r"(taddr_b + (16u << 16))
+      : "memory");
+}
+// 16 columns of them
+__device__ __forceinline__ void tmem_ld_frag_wait(uint32_t taddr, uint32_t (&r)[2][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=&r"(r[0][0]), "=&r"(r[0][1]), "=&r"(r[0][2]), "=&r"(r[0][3]), "=&r"(r[0][4]), "=&r"(r[0][5]), "=&r"(r[0][6]), "=&r"(r[0][7]),
+        "=&r"(r[1][0]), "=&r"(r[1][1]), "=&r"(r[1][2]), "=&r"(r[1][3]), "=&r"(r[1][4]), "=&r"(r[1][5]), "=&r"(r[1][6]), "=&r"(r[1][7])
+      : "r"(taddr), "r"(taddr + (16u << 16))
       : "memory");
 }
 // Four 8 x 8 bf16 matrices of such a fragment to shared memory: lane l gives the 16 bytes of row l % 8 of matrix l / 8.
@@ -553,6 +573,6 @@ const CUtensorMap* mlb_tmap_cached(const void* base, uint64_t rows, uint64_t col
 // [seqs][rows][cols] bf16, contiguous, box {64 columns, 64 rows, 1 sequence}, 128-byte swizzle: rows past a sequence's end read as
 // zeros instead of the next sequence's.  Needs a 16-byte aligned base and cols a multiple of 8.
 const CUtensorMap* mlb_tmap_seq3d_cached(const void* base, uint64_t seqs, uint64_t rows, uint64_t cols);
-// Any bf16 tensor of up to five dimensions, innermost first, 128-byte swizzle; `strides` (bytes) of the dimensions behind the first.  Encoded anew each time, a
+// Any bf16 tensor of up to five dimensions, innermost first, rows of a box swizzled over 128, 64 or 32 bytes; `strides` (bytes) of the dimensions behind the first.  Encoded anew each time, a
 // fraction of a microsecond.  false: refused.
-bool mlb_make_tmap_nd(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
+bool mlb_make_tmap_nd(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, int swizzle = 128);

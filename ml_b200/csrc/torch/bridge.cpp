@@ -98,8 +98,8 @@ typedef std::optional<Tensor> Maybe;      // (an undefined tensor is no argument
   X(mlb_moe_plan_rows, long, (long, int, int))                                                                                                 \
   X(mlb_moe_plan, int, (int*, const int*, long, int, int, St))                                                                                 \
   X(mlb_moe_fwd, int, (void*, void*, void*, void*, void*, const void*, const void*, const void*, const void*, const int*, long, long, int, int, int, int, int, St)) \
-  X(mlb_moe_bwd, int, (void*, void*, void*, void*, void*, void*, void*, void*, void*, const void*, const void*, const void*, const void*, const void*, const void*, const int*, long, long, \
-                       int, int, int, int, int, St))
+  X(mlb_moe_bwd, int, (void*, void*, void*, void*, void*, void*, void*, const void*, const void*, const void*, const void*, const void*, const void*, const void*, const void*, const int*, \
+                       long, long, int, int, int, int, int, St))
 #define MLB_POINTER(name, ret, args) ret(*name) args = nullptr;
 struct Entries { MLB_ENTRIES(MLB_POINTER) MLB_GENERATION(MLB_POINTER) MLB_MOE(MLB_POINTER) } K;
 

@@ -107,7 +107,7 @@ def _fwd(out, x, weights, idx, gate_up, down, keep):
     new = lambda c: torch.empty(R, c, dtype=BF16, device=x.device)
     xs, gu, h, y = new(C), new(2 * I) if keep else None, new(I), new(C)
     _took(_n._entries().mlb_moe_fwd(out, xs, _at(gu), h, y, _at(x), _at(weights), gate_up, down, plan, N, ldx, k, E, C, I, _bits(weights)), "moe_mlp")
-    return plan, xs, gu
+    return plan, xs, gu, h, y
 
 
 def moe_mlp(out, x, weights, idx, gate_up, down):
@@ -132,13 +132,13 @@ def moe_mlp_bwd(dx, dweights, dgate_up, ddown, dout, x, weights, idx, gate_up, d
             if t is not None:
                 t.zero_()
         return
-    plan, xs, gu = saved
+    plan, xs, gu, h, y = saved
     e = _n._entries()
     R = e.mlb_moe_plan_rows(N, k, E)
     _need(plan, (e.mlb_moe_plan_ints(N, k, E),), "saved plan", (I32,))
-    _need(xs, (R, C), "saved rows", (BF16,))
-    _need(gu, (R, 2 * I), "saved products", (BF16,))
+    for t, c in ((xs, C), (gu, 2 * I), (h, I), (y, C)):
+        _need(t, (R, c), "saved rows", (BF16,))
     new = lambda c: torch.empty(R, c, dtype=BF16, device=x.device)
-    ys, dh, dgu, hw, dxs = new(C), new(I), new(2 * I), new(I), new(C)
-    _took(e.mlb_moe_bwd(_at(dx), _at(dweights), _at(dgate_up), _at(ddown), ys, dh, dgu, hw, dxs, _at(dout), xs, gu, _at(weights), gate_up, down, plan, N, _rows(dout, "dout"), k, E, C, I,
+    ys, dgu, dxs = new(C), new(2 * I), new(C)
+    _took(e.mlb_moe_bwd(_at(dx), _at(dweights), _at(dgate_up), _at(ddown), ys, dgu, dxs, _at(dout), xs, gu, h, y, _at(weights), gate_up, down, plan, N, _rows(dout, "dout"), k, E, C, I,
                         _bits(weights)), "moe_mlp_bwd")
