@@ -571,9 +571,12 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
         const int last = (w.rows + 31) & ~31;      // (what fills up an expert's rows belongs to it)
         for (int c = half * CHUNK; c < last; c += PASS) {
           if (!live) break;      // (warp-uniform)
-          // what left two chunks ago (a tile's rows: before) has been read, its places are free
+          // what left two chunks ago has been read, its place is free; before the first chunk so have a weight gradient's rows, which had both places
           if constexpr (MODE != DOWN_T) {
-            if (lane == 0) tc::tma_wait_group_read<1>();
+            if (lane == 0) {
+              if (MODE == BACK && n == 0) tc::tma_wait_group_read<0>();
+              else tc::tma_wait_group_read<1>();
+            }
             __syncwarp();
           }
           uint8_t* place = buf + (MODE == DOWN_T ? S::PLACES * S::PLACE : (n & 1) * 2048);
@@ -692,6 +695,177 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
   tc::tc_fence_before();
   tc::cluster_sync();      // no CTA frees tensor memory or leaves while its peer may still signal or read it
   if (warp == 1) tc::tmem_dealloc_pair(tmem_base, 2 * ACC);
+}
+
+// ------------------------------------------------------------------ few tokens
+// A step of a few tokens reads the weights of the experts that they chose, once, and that is all its time: the products are m16n8k16 instructions whose 16 rows of weights come
+// straight from memory to registers, 16 bytes a lane (which eight elements of the reduction an instruction has is the same for both operands, so a lane's eight
+// neighbouring ones serve as those of two instructions) and whose 8 columns are tokens of one expert.  A thread block shares the reduction of 16 rows among its
+// eight warps and adds up their parts in shared memory; 64 KB are on their way for each block at 2048 columns.  Two launches: h of all copies, a row of gate and of up
+// projection each in the instruction's halves; then y, whose last block for 16 columns forms the weighted sums of its 16 columns.
+// An expert's copies are found by each block for itself: 256 at most.
+constexpr int FEW_TOKENS = 32, FEW_COPIES = 256, FEW_THREADS = 256, FEW_BATCH = 6;
+struct FewArgs {
+  bf16* out;            // DOWN: [N, C]
+  bf16* h;              // [N k, I]
+  float* y;             // [N k, C]
+  int* count;           // [C / 16] blocks that are done with 16 columns; 0 between calls
+  const bf16 *x, *W;
+  const void* weights;
+  const int* idx;
+  long ldx;
+  int N, k, E, C, I, wide_w;
+};
+__device__ __forceinline__ uint4 load_weights(const bf16* p) {      // (each is used once: it stays out of the L1, which holds the tokens)
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int NT, bool DOWN_>
+__global__ void __launch_bounds__(FEW_THREADS, 3) moe_few_k(const FewArgs A) {
+  mlb_pdl_sync();
+  __shared__ __align__(16) int expert[FEW_COPIES];
+  __shared__ int list[FEW_COPIES], nth[FEW_COPIES], first[FEW_COPIES + 1], of[FEW_COPIES], sums[FEW_THREADS / 32], last;
+  __shared__ float part[8][NT * 128];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, NK = A.N * A.k;
+  // the copies by expert: a copy's place is the number of those before it.  More copies than an instruction's columns (a token may name an expert twice) are dealt with as if
+  // another expert had them.
+  int e = tid < NK ? A.idx[tid] : -1;
+  if (e >= A.E) {
+    if (blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xD1);
+    e = -1;
+  }
+  expert[tid] = e < 0 ? 0x7fffffff : e;
+  list[tid] = -1;
+  __syncthreads();
+  int less = 0, equal = 0;
+#pragma unroll 4
+  for (int i = 0; i < NK; i += 4) {
+    const int4 x = *reinterpret_cast<const int4*>(expert + i);
+    less += (x.x < e) + (x.y < e) + (x.z < e) + (x.w < e);
+    equal += (x.x == e && i < tid) + (x.y == e && i + 1 < tid) + (x.z == e && i + 2 < tid) + (x.w == e && i + 3 < tid);
+  }
+  nth[tid] = equal;
+  if (e >= 0) list[less + equal] = tid;
+  __syncthreads();
+  const int here = list[tid];
+  const bool begins = here >= 0 && nth[here] % (8 * NT) == 0;
+  const unsigned b = __ballot_sync(0xffffffffu, begins);
+  if (lane == 0) sums[w] = __popc(b);
+  const int held = __syncthreads_count(here >= 0);
+  int experts = 0, before = __popc(b & ((1u << lane) - 1));
+#pragma unroll
+  for (int i = 0; i < FEW_THREADS / 32; i++) {
+    before += i < w ? sums[i] : 0;
+    experts += sums[i];
+  }
+  if (begins) first[before] = tid, of[before] = expert[here];
+  if (tid == 0) first[experts] = held;
+  __syncthreads();
+
+  const int K = DOWN_ ? A.I : A.C, groups = DOWN_ ? A.C / 16 : A.I / 8, kbs = (K + 31) / 32, r = lane >> 2, t = lane & 3;
+  if (DOWN_ && experts == 0) {      // nothing for anybody
+    for (long i = (long)blockIdx.x * FEW_THREADS + tid; i < (long)A.N * A.C; i += (long)gridDim.x * FEW_THREADS) A.out[i] = __float2bfloat16(0.f);
+    return;
+  }
+  const int units = experts * groups;
+  uint4 wa[FEW_BATCH], wb[FEW_BATCH];
+  auto ask = [&](int unit, int kb0) {      // this warp's part of a batch of the unit's weights
+    const int a = unit / groups, g = unit - a * groups;
+    const bf16 *row0 = A.W + (size_t)of[a] * (DOWN_ ? (size_t)A.C * A.I : 2 * (size_t)A.I * A.C) + (size_t)(g * (DOWN_ ? 16 : 8) + r) * K, *row1 = row0 + (size_t)(DOWN_ ? 8 : A.I) * K;
+#pragma unroll
+    for (int i = 0; i < FEW_BATCH; i++) {
+      const int k = (kb0 + 8 * i) * 32 + t * 8;
+      wa[i] = k < K ? load_weights(row0 + k) : make_uint4(0, 0, 0, 0);
+      wb[i] = k < K ? load_weights(row1 + k) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  if (blockIdx.x < units) ask(blockIdx.x, w);
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int a = unit / groups, g = unit - a * groups, f0 = first[a], copies = first[a + 1] - f0;
+    const bf16* col[NT];      // (columns behind the last copy: any row, nothing of theirs is used)
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const int c = list[f0 + min(n * 8 + r, copies - 1)];
+      col[n] = DOWN_ ? A.h + (size_t)c * A.I : A.x + (size_t)(c / A.k) * A.ldx;
+    }
+    float d[NT][4] = {};
+#pragma unroll 1
+    for (int kb0 = w; kb0 < kbs || kb0 == w; kb0 += 8 * FEW_BATCH) {
+#pragma unroll
+      for (int i = 0; i < FEW_BATCH; i++) {
+        const int k = (kb0 + 8 * i) * 32 + t * 8;
+        if ((kb0 + 8 * i) * 32 >= K) break;      // (the warp's)
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          if (n * 8 >= copies) break;            // (the block's)
+          const uint4 v = k < K ? __ldg(reinterpret_cast<const uint4*>(col[n] + k)) : make_uint4(0, 0, 0, 0);
+          mma_16816(d[n], wa[i].x, wb[i].x, wa[i].y, wb[i].y, v.x, v.y);
+          mma_16816(d[n], wa[i].z, wb[i].z, wa[i].w, wb[i].w, v.z, v.w);
+        }
+      }
+      // what comes next is on its way while the parts are added up
+      if (kb0 + 8 * FEW_BATCH < kbs) ask(unit, kb0 + 8 * FEW_BATCH);
+      else if (unit + (int)gridDim.x < units) ask(unit + gridDim.x, w);
+    }
+    // d[n][2 h + x]: row 8 h + lane / 4, column 8 n + 2 (lane % 4) + x
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int x = 0; x < 4; x++) part[w][n * 128 + x * 32 + lane] = d[n][x];
+    __syncthreads();
+    if (DOWN_) {
+      for (int i = tid; i < NT * 128; i += FEW_THREADS) {
+        const int n = i >> 7, x = (i >> 5) & 3, l = i & 31, c = n * 8 + 2 * (l & 3) + (x & 1);
+        if (c >= copies) continue;
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) s += part[j][i];
+        A.y[(size_t)list[f0 + c] * A.C + g * 16 + (x >> 1) * 8 + (l >> 2)] = s;
+      }
+      __syncthreads();
+      if (tid == 0) last = mlb_count_block(A.count + g) == experts - 1;
+      __syncthreads();
+      if (last) {      // all experts are done with these 16 columns
+        for (int i = tid; i < A.N * 16; i += FEW_THREADS) {
+          const int n = i >> 4, c = g * 16 + (i & 15);
+          float s = 0.f;
+          for (int j = 0; j < A.k; j++) {
+            const int q = n * A.k + j;
+            if (expert[q] == 0x7fffffff) continue;
+            const float wq = A.wide_w ? ((const float*)A.weights)[q] : __bfloat162float(((const bf16*)A.weights)[q]);
+            s = fmaf(wq, __ldcg(A.y + (size_t)q * A.C + c), s);
+          }
+          A.out[(size_t)n * A.C + c] = __float2bfloat16(s);
+        }
+        if (tid == 0) A.count[g] = 0;
+      }
+    } else {
+      for (int i = tid; i < NT * 64; i += FEW_THREADS) {      // row lane / 4 is the gate's, row 8 + lane / 4 the up projection's
+        const int n = i >> 6, x = (i >> 5) & 1, l = i & 31, c = n * 8 + 2 * (l & 3) + x;
+        if (c >= copies) continue;
+        float gate = 0.f, up = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) gate += part[j][n * 128 + x * 32 + l], up += part[j][n * 128 + (x + 2) * 32 + l];
+        A.h[(size_t)list[f0 + c] * A.I + g * 8 + (l >> 2)] = __float2bfloat16(gate * rcp(1.f + ex2(-1.44269504f * gate)) * up);
+      }
+    }
+    __syncthreads();
+  }
+}
+template <int NT>
+int launch_few(FewArgs g, const bf16* gate_up, const bf16* down, cudaStream_t st) {
+  const int experts = std::min(g.N * g.k, g.E), resident = mlb_sm_count() * 3;
+  g.W = gate_up;
+  cudaError_t e = mlb_launch(moe_few_k<NT, false>, dim3(std::min(experts * (g.I / 8), resident)), dim3(FEW_THREADS), 0, st, g);
+  if (e != cudaSuccess) return (int)e;
+  g.W = down;
+  return (int)mlb_launch(moe_few_k<NT, true>, dim3(std::min(experts * (g.C / 16), resident)), dim3(FEW_THREADS), 0, st, g);
 }
 
 struct Maps { CUtensorMap a, b, b16, a1, b1, a2, b2, out, out1, out2; };
@@ -847,4 +1021,17 @@ MLB_API int mlb_moe_bwd(void* dx, void* dweights, void* dgate_up, void* ddown, v
     return -2;
   MLB_TRY(launch_gemm<BACK>(m, g, (long)E * (g.per_gate_up + g.per_down) + (long)z.p.max_tiles * g.tiles_m, st));
   return dx != nullptr ? combine((bf16*)dx, (const bf16*)dxs, (const float*)nullptr, P, z, st) : 0;
+}
+// floats of the workspace of the form for few tokens: y, h and (the first C / 16 ints, 0 before the first call, left so by each) counters; 0: the sizes take the other form
+MLB_API long mlb_moe_few_floats(long N, int k, int E, int C, int I) {
+  Sizes z;
+  if (sizes(z, N, k, E, C, I) != 0 || N < 1 || N > FEW_TOKENS || z.NK > FEW_COPIES) return 0;
+  return z.NK * C + (z.NK * I + 1) / 2;
+}
+MLB_API int mlb_moe_few(void* out, const void* x, const void* weights, const int* idx, const void* gate_up, const void* down, float* part, int* count, long N, long ldx, int k, int E, int C,
+                        int I, int wbits, cudaStream_t st) {
+  if (mlb_moe_few_floats(N, k, E, C, I) == 0 || off16({out, x, gate_up, down, part}) || ldx % 8 != 0 || (wbits != 16 && wbits != 32)) return -7;
+  FewArgs g = {(bf16*)out, (bf16*)(part + N * k * C), part, count, (const bf16*)x, nullptr, weights, idx, ldx, (int)N, k, E, C, I, wbits == 32};
+  const bf16 *a = (const bf16*)gate_up, *b = (const bf16*)down;
+  return N <= 8 ? launch_few<1>(g, a, b, st) : N <= 16 ? launch_few<2>(g, a, b, st) : launch_few<4>(g, a, b, st);
 }

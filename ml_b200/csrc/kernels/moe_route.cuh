@@ -38,11 +38,11 @@ __device__ __forceinline__ float exp_fine(float x) {
 __device__ __forceinline__ float exp_from(float a, float b) { return a == b ? 1.f : a == -INFINITY ? 0.f : exp_fine(fmaxf(a - b, -200.f)); }
 __device__ __forceinline__ float sigmoid_fine(float z) {
   const float e = exp_fine(fmaxf(-fabsf(z), -200.f));
-  return __fdiv_rn(z >= 0.f ? 1.f : e, 1.f + e);
+  return __fdividef(z >= 0.f ? 1.f : e, 1.f + e);      // (2 steps of 2^-23; the denominator is 1 to 2)
 }
 // sigmoid(z) / exp(top) for top = min(0, largest z): scores for shares, whose sum is not too small for fp32
 __device__ __forceinline__ float sigmoid_from(float z, float top) {
-  return z == -INFINITY ? 0.f : z >= 0.f ? sigmoid_fine(z) : __fdiv_rn(exp_from(z, top), 1.f + exp_fine(fmaxf(z, -200.f)));
+  return z == -INFINITY ? 0.f : z >= 0.f ? sigmoid_fine(z) : __fdividef(exp_from(z, top), 1.f + exp_fine(fmaxf(z, -200.f)));
 }
 // numbers in the order of their values, as unsigned ones
 __device__ __forceinline__ uint32_t order32(float v) {
@@ -53,9 +53,10 @@ __device__ __forceinline__ uint64_t order64(double v) {
   const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
   return u ^ ((u >> 63) ? ~0ull : 1ull << 63);
 }
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu)); }
+__device__ __forceinline__ double value64(uint64_t key) { return __longlong_as_double((long long)(key ^ ((key >> 63) ? 1ull << 63 : ~0ull))); }
 constexpr uint32_t GONE32 = 0x007fffffu;                    // order32(-inf)
 constexpr uint64_t GONE64 = 0x000fffffffffffffull;          // order64(-inf)
-template <typename K> __device__ __forceinline__ constexpr K gone() { return sizeof(K) == 4 ? (K)GONE32 : (K)GONE64; }
 __device__ __forceinline__ uint32_t warp_best(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint64_t warp_best(uint64_t v) {
   const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
@@ -63,9 +64,10 @@ __device__ __forceinline__ uint64_t warp_best(uint64_t v) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// The k best of the warp's keys, best first: lane j keeps the index of the j-th (-1: none left).
-template <int V, typename K>
-__device__ __forceinline__ int choose(K (&key)[V], int k, int lane) {
+// The k best of the warp's keys, best first: lane j keeps the index of the j-th (-1: none left)
+template <int V>
+__device__ __forceinline__ int choose(uint32_t (&key)[V], int k, int lane) {
+  typedef uint32_t K;
   int mine = -1;
   K best = key[0];
   int at = 0;
@@ -74,7 +76,7 @@ __device__ __forceinline__ int choose(K (&key)[V], int k, int lane) {
     if (key[v] > best) best = key[v], at = v;
   for (int j = 0; j < k; j++) {
     const K top = warp_best(best);
-    if (top <= gone<K>()) break;
+    if (top <= GONE32) break;
     const unsigned i = __reduce_min_sync(0xffffffffu, best == top ? (unsigned)(at * 32 + lane) : 0xffffffffu);
     if (lane == j) mine = (int)i;
     if ((int)(i & 31) == lane) {
@@ -90,11 +92,176 @@ __device__ __forceinline__ int choose(K (&key)[V], int k, int lane) {
   return mine;
 }
 
-template <int V, typename T>
-__global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_k(const RouteArgs A) {
+// What may be chosen of many keys a lane.  A bound that k + 1 lanes' best keys or a few more reach is no better than the k + 1-th best key, so what is chosen, and what comes
+// behind it, is among the keys that reach it (or, with `below`, come near it): usually some more than k.  They are put side by side, a lane each.  Returns how many;
+// over 32 (many equal ones): the list is not complete.  8192 tokens, 8 of 256 experts, by logits: 13.3 us with the bound out of a sort of the lanes' best, 9.2 so.
+template <int V>
+__device__ __forceinline__ int candidates(const uint32_t (&key)[V], int k, int lane, uint2* s, float below) {
+  uint32_t best = key[0];
+#pragma unroll
+  for (int v = 1; v < V; v++) best = max(best, key[v]);
+  uint32_t least = max(__reduce_min_sync(0xffffffffu, best), GONE32 + 1), over = __reduce_max_sync(0xffffffffu, best);
+  if (over < least) return 0;
+#pragma unroll 1
+  for (int i = 0; i < 12 && least < over; i++) {      // (a bound that is kept is reached by k + 1 lanes, or by all)
+    const uint32_t mid = least + ((over - least + 1) >> 1);
+    const int n = __popc(__ballot_sync(0xffffffffu, best >= mid));
+    if (n > k) least = mid;
+    else over = mid - 1;
+    if (n > k && n <= k + 4) break;
+  }
+  if (below > 0.f) least = max(order32(value_of(least) - below), GONE32 + 1);
+  int count = 0;
+  __syncwarp();
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const bool here = key[v] >= least;
+    const unsigned all = __ballot_sync(0xffffffffu, here);
+    if (here) {
+      const int at = count + __popc(all & ((1u << lane) - 1));
+      if (at < 32) s[at] = make_uint2(key[v], v * 32 + lane);
+    }
+    count += __popc(all);
+  }
+  __syncwarp();
+  return count;
+}
+// The k best of them, as choose() returns them
+template <int V>
+__device__ __forceinline__ int choose_many(uint32_t (&key)[V], int k, int lane, uint2* s) {
+  const int count = k < 32 ? candidates(key, k, lane, s, 0.f) : 33;
+  if (count > 32) return choose<V>(key, k, lane);
+  const uint2 own = lane < count ? s[lane] : make_uint2(0, 0);
+  int rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < count; j++) {
+    const uint2 x = s[j];
+    rank += x.x > own.x || (x.x == own.x && x.y < own.y);
+  }
+  __syncwarp();
+  if (lane < count) s[rank] = own;
+  __syncwarp();
+  return lane < k && lane < count ? (int)s[lane].y : -1;
+}
+
+// Groups: the experts' choice numbers t stand in s[E].  As many lanes as go into 32 share a group.  Lane l gets group l's three best numbers, and the indices of the first two.
+struct Best { float a, b, c; int ai, bi; };
+__device__ __forceinline__ Best best_of_groups(const float* s, int size, int groups, int lane) {
+  int share = 32;
+  while (share * groups > 32) share >>= 1;
+  const int g = lane / share, sub = lane % share, steps = (size + share - 1) / share;
+  Best r = {-INFINITY, -INFINITY, -INFINITY, 0, 0};
+  if (g < groups)
+    for (int j = 0, x = g % steps; j < steps; j++, x = x + 1 == steps ? 0 : x + 1) {      // (begun at another place by each group: other banks)
+      const int i = x * share + sub;
+      const float t = i < size ? s[g * size + i] : -INFINITY;
+      if (t > r.b) {
+        r.c = r.b;
+        if (t > r.a) r.b = r.a, r.bi = r.ai, r.a = t, r.ai = g * size + i;
+        else r.b = t, r.bi = g * size + i;
+      } else {
+        r.c = fmaxf(r.c, t);
+      }
+    }
+  for (int o = 1; o < share; o <<= 1) {
+    const float x = __shfl_xor_sync(0xffffffffu, r.a, o), y = __shfl_xor_sync(0xffffffffu, r.b, o), z = __shfl_xor_sync(0xffffffffu, r.c, o);
+    const int xi = __shfl_xor_sync(0xffffffffu, r.ai, o), yi = __shfl_xor_sync(0xffffffffu, r.bi, o);
+    const float low = fminf(r.a, x), mid = fmaxf(r.b, y);      // the second best of all is one of these, and the third the other one or a third
+    const int li = r.a < x ? r.ai : xi, mi = r.b < y ? yi : r.bi;
+    if (r.a < x) r.a = x, r.ai = xi;
+    r.c = fmaxf(fminf(low, mid), fmaxf(r.c, z));
+    r.b = fmaxf(low, mid);
+    r.bi = low < mid ? mi : li;
+  }
+  const int from = (lane * share) & 31;
+  return {__shfl_sync(0xffffffffu, r.a, from), __shfl_sync(0xffffffffu, r.b, from), __shfl_sync(0xffffffffu, r.c, from), __shfl_sync(0xffffffffu, r.ai, from),
+          __shfl_sync(0xffffffffu, r.bi, from)};
+}
+// The bits of the groups that stay, by the sums of their two best (lane l: of group l); `margin`: by how much the worst of them is ahead of the best of the others
+__device__ __forceinline__ unsigned keep_groups(double sum, int groups, int top, int lane, double& margin) {
+  uint64_t key = lane < groups ? order64(sum) : 0;
+  unsigned stays = 0;
+  for (int j = 0; j < top; j++) {
+    const uint64_t best = warp_best(key);
+    const int g = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
+    stays |= 1u << g;
+    if (lane == g) key = 0;
+  }
+  const uint64_t low = ~warp_best((stays >> lane) & 1 ? ~order64(sum) : 0), high = warp_best(key);
+  margin = high <= GONE64 ? INFINITY : value64(low) - value64(high);
+  return stays;
+}
+
+// The choice by score + bias, in 64 bits throughout, the numbers in shared memory (s[E]).  For softmax with a bias where 32 bits leave it open, and many equal numbers.
+template <typename T>
+__device__ __noinline__ int choose_exact(const RouteArgs& A, const T* row, double* s, float m) {
+  const int lane = threadIdx.x & 31, E = A.E;
+  double all = 0;
+  __syncwarp();
+#pragma unroll 1
+  for (int i = lane; i < E; i += 32) {
+    const float z = seen(logit(row, i));
+    const double x = exp(A.sigmoid ? -(double)z : z == m ? 0.0 : (double)z - (double)m);
+    const double t = z == -INFINITY ? 0.0 : A.sigmoid ? 1.0 / (1.0 + x) : x;
+    all += t;
+    s[i] = t;
+  }
+  if (!A.sigmoid)
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+#pragma unroll 1
+  for (int i = lane; i < E; i += 32) {
+    const float z = seen(logit(row, i));
+    const double t = A.sigmoid ? s[i] : all > 0 ? s[i] / all : 0.0;
+    s[i] = z == -INFINITY ? -INFINITY : A.bias != nullptr ? t + (double)__ldg(A.bias + i) : t;
+  }
+  __syncwarp();
+  unsigned stays = 0xffffffffu;
+  const int size = E / A.groups;
+  if (A.groups > 1) {
+    double a = -INFINITY, b = -INFINITY, margin;
+#pragma unroll 1
+    for (int i = 0; lane < A.groups && i < size; i++) {
+      const double t = s[lane * size + i];
+      if (t > a) b = a, a = t;
+      else if (t > b) b = t;
+    }
+    stays = keep_groups(a + (b > -INFINITY ? b : 0.0), A.groups, A.top, lane, margin);
+  }
+  int mine = -1;
+#pragma unroll 1
+  for (int j = 0; j < A.k; j++) {
+    double best = -INFINITY;
+    int at = 0;
+#pragma unroll 1
+    for (int i = lane; i < E; i += 32)
+      if (s[i] > best && ((stays >> (A.groups > 1 ? i / size : 0)) & 1)) best = s[i], at = i;
+    const uint64_t key = order64(best), top = warp_best(key);
+    if (top <= GONE64) break;
+    const unsigned i = __reduce_min_sync(0xffffffffu, key == top ? (unsigned)at : 0xffffffffu);
+    if (lane == j) mine = (int)i;
+    if ((int)(i & 31) == lane) s[i] = -INFINITY;
+    __syncwarp();
+  }
+  __syncwarp();
+  return mine;
+}
+
+// An expert's number in 64 bits where that is the expert's own affair: sigmoids; a softmax without bias over its common factor
+template <typename T>
+__device__ __forceinline__ double own_number(const RouteArgs& A, const T* row, int i, float m) {
+  const double z = (double)seen(logit(row, i)), x = exp(A.sigmoid ? -z : z - (double)m);
+  return A.sigmoid ? 1.0 / (1.0 + x) + (A.bias != nullptr ? (double)__ldg(A.bias + i) : 0.0) : x;
+}
+
+// PLAIN: by the logits alone
+template <int V, typename T, bool PLAIN>
+__global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2) moe_route_k(const RouteArgs A) {
   mlb_pdl_sync();
-  extern __shared__ double route_sm[];      // with groups: the scores of each warp's token; behind the loop: sums of probabilities
+  extern __shared__ double route_sm[];      // not PLAIN: the scores of each warp's token; lists of candidates; behind the loop: sums of probabilities
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, E = A.E;
+  const uint32_t magic = 0xffffffffu / (uint32_t)(E / A.groups) + 1;      // (0, and not used so, where a group is one expert)
+  uint2* list = (uint2*)(route_sm + (PLAIN ? 0 : ROUTE_WARPS * E)) + 32 * w;
   float sum_p[V];
 #pragma unroll
   for (int v = 0; v < V; v++) sum_p[v] = 0.f;
@@ -108,76 +275,99 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_k(const RouteArgs 
       m = fmaxf(m, z[v]);
     }
     m = warp_max(m);
-    float total = 0.f;      // of exp(z - m), or of scores relative to the largest
-    if (A.part != nullptr || (!A.sigmoid && !A.renorm)) {
-      float e[V];
+    float e[V], total = 0.f;      // exp(z - m) or scores, and their sum (for shares of sigmoids, below: relative to the largest)
+    const bool sums = !A.sigmoid && (A.part != nullptr || !A.renorm || !PLAIN);
+    if (sums || !PLAIN) {
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        e[v] = z[v] == -INFINITY ? 0.f : A.sigmoid ? sigmoid_from(z[v], fminf(m, 0.f)) : exp_from(z[v], m);
+        e[v] = z[v] == -INFINITY ? 0.f : A.sigmoid ? sigmoid_fine(z[v]) : exp_from(z[v], m);
         total += e[v];
       }
-      total = warp_sum(total);
-      if (A.part != nullptr) {
-        const float inv = total > 0.f ? __fdiv_rn(1.f, total) : 0.f;
+      if (sums) total = warp_sum(total);
+    }
+    if (A.part != nullptr) {
+      float x[V], all = total;
+      if (A.sigmoid) {
+        all = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; v++) sum_p[v] = fmaf(e[v], inv, sum_p[v]);
+        for (int v = 0; v < V; v++) x[v] = z[v] == -INFINITY ? 0.f : sigmoid_from(z[v], fminf(m, 0.f)), all += x[v];
+        all = warp_sum(all);
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; v++) x[v] = e[v];
       }
+      const float inv = all > 0.f ? __fdiv_rn(1.f, all) : 0.f;
+#pragma unroll
+      for (int v = 0; v < V; v++) sum_p[v] = fmaf(x[v], inv, sum_p[v]);
     }
     int mine;
-    if (A.bias == nullptr && A.groups == 1) {
+    if constexpr (PLAIN) {
       uint32_t key[V];
 #pragma unroll
       for (int v = 0; v < V; v++) key[v] = order32(z[v]);
-      mine = choose<V>(key, A.k, lane);
+      if constexpr (V >= 4) mine = choose_many<V>(key, A.k, lane, list);
+      else mine = choose<V>(key, A.k, lane);
     } else {
-      double t[V], all = 0;
-#pragma unroll
-      for (int v = 0; v < V; v++) {
-        t[v] = z[v] == -INFINITY ? 0.0 : A.sigmoid ? 1.0 / (1.0 + exp(-(double)z[v])) : z[v] == m ? 1.0 : exp((double)z[v] - (double)m);
-        all += t[v];
-      }
-      if (!A.sigmoid) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-      }
+      // 32 bits say what may be chosen, 64 bits what is.  In 32 a score is off by less than 2^-22 of itself (6 roundings, and a sum's), score + bias by less than slack = 2^-21 of the
+      // row's largest score + |bias|.  (With 64 bits for the few tokens alone that 32 leave open, these wait some 10 us for code that no cache has.)
+      float t[V], size = 0.f;
+      const float inv = A.sigmoid || A.bias == nullptr ? 1.f : total > 0.f ? __fdiv_rn(1.f, total) : 0.f;
 #pragma unroll
       for (int v = 0; v < V; v++) {
         const int i = v * 32 + lane;
-        if (!A.sigmoid) t[v] = all > 0 ? t[v] / all : 0.0;
-        if (i < E && A.bias != nullptr) t[v] += (double)__ldg(A.bias + i);
-        if (z[v] == -INFINITY) t[v] = -INFINITY;
+        const float b = i < E && A.bias != nullptr ? __ldg(A.bias + i) : 0.f, s = e[v] * inv;
+        t[v] = z[v] == -INFINITY ? -INFINITY : s + b;
+        if (z[v] > -INFINITY) size = fmaxf(size, s + fabsf(b));
       }
-      if (A.groups > 1) {      // lane l has group l: its two best
-        double* s = route_sm + w * E;
-        const int size = E / A.groups;
+      const float slack = 4.7683716e-7f * __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size)));
+      const bool single = A.sigmoid || A.bias == nullptr;      // own_number() has them
+      bool sure = slack < 1e30f && m < INFINITY;
+      if (A.groups > 1) {
+        float* s = (float*)(route_sm + w * E);
+        __syncwarp();
 #pragma unroll
         for (int v = 0; v < V; v++)
           if (v * 32 + lane < E) s[v * 32 + lane] = t[v];
         __syncwarp();
-        double a = -INFINITY, b = -INFINITY;
-        if (lane < A.groups)
-          for (int j = 0, i = lane % size; j < size; j++, i = i + 1 == size ? 0 : i + 1) {      // (begun at another place by each lane: other banks)
-            const double x = s[lane * size + i];
-            if (x > a) b = a, a = x;
-            else if (x > b) b = x;
-          }
-        __syncwarp();
-        uint64_t key[1] = {lane < A.groups ? order64(a + (b > -INFINITY ? b : 0.0)) : 0};
-        unsigned stays = 0;
-        for (int j = 0; j < A.top; j++) {
-          const uint64_t best = warp_best(key[0]);
-          const int g = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
-          stays |= 1u << g;
-          if (lane == g) key[0] = 0;
+        const Best g = best_of_groups(s, E / A.groups, A.groups, lane);
+        double sum = g.a, margin;
+        if (single) {      // (a group without experts stays at -inf)
+          if (lane < A.groups && g.a > -INFINITY) sum = own_number(A, row, g.ai, m) + (g.b > -INFINITY ? own_number(A, row, g.bi, m) : 0.0);
+        } else if (g.b > -INFINITY) {
+          sum += g.b;
         }
+        const unsigned stays = keep_groups(sum, A.groups, A.top, lane, margin);
+        // which two are a group's best is open where the third comes near the second, and then matters where groups come near each other
+        if (margin <= 4.0 * slack && (!single || __any_sync(0xffffffffu, lane < A.groups && g.c > -INFINITY && g.b - g.c <= 2.f * slack))) sure = false;
 #pragma unroll
-        for (int v = 0; v < V; v++)
-          if (v * 32 + lane < E && !((stays >> ((v * 32 + lane) / size)) & 1)) t[v] = -INFINITY;
+        for (int v = 0; v < V; v++)      // ((i magic) >> 32 is i / (experts of a group) for i < 2^16)
+          if (!((stays >> ((magic ? __umulhi(v * 32 + lane, magic) : v * 32 + lane) & 31)) & 1)) t[v] = -INFINITY;
       }
-      uint64_t key[V];
+      uint32_t key[V];
 #pragma unroll
-      for (int v = 0; v < V; v++) key[v] = order64(t[v]);
-      mine = choose<V>(key, A.k, lane);
+      for (int v = 0; v < V; v++) key[v] = order32(t[v]);
+      const int count = A.k < 32 && sure ? candidates(key, A.k, lane, list, 4.f * slack) : 33;
+      mine = -1;
+      if (count <= 32) {
+        const uint2 c = lane < count ? list[lane] : make_uint2(0, 0);
+        double own = value_of(c.x);
+        if (single && lane < count) own = own_number(A, row, (int)c.y, m);
+        const uint64_t k64 = lane < count ? order64(own) : 0;
+        double near = INFINITY;      // (softmax with a bias: the distance to the next better one)
+        int rank = 0;
+        for (int j = 0; j < count; j++) {
+          const uint64_t x = (uint64_t)__shfl_sync(0xffffffffu, (uint32_t)(k64 >> 32), j) << 32 | __shfl_sync(0xffffffffu, (uint32_t)k64, j);
+          const uint32_t xi = __shfl_sync(0xffffffffu, c.y, j);
+          rank += x > k64 || (x == k64 && xi < c.y);
+          if (!single && j != lane) near = fmin(near, fabs(value64(x) - own));
+        }
+        if (!single) sure = !__any_sync(0xffffffffu, lane < count && rank <= A.k && near <= 2.0 * slack);
+        __syncwarp();
+        if (lane < count) list[rank].x = c.y;
+        __syncwarp();
+        if (lane < A.k && lane < count) mine = (int)list[lane].x;
+      }
+      if (count > 32 || !sure) mine = choose_exact(A, row, route_sm + w * E, m);
     }
     // lane j: the weight of the j-th
     const float zj = mine >= 0 ? seen(logit(row, mine)) : -INFINITY;
@@ -212,24 +402,20 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_k(const RouteArgs 
     }
   }
 }
-// mean[e] = the blocks' sums / N: 8 threads to an expert, always the same blocks to a thread
-__global__ void __launch_bounds__(256) moe_mean_k(float* mean, const float* __restrict__ part, int blocks, int E, float inv) {
+// mean[e] = the blocks' sums / N: 32 threads to an expert, always the same blocks to a thread
+__global__ void __launch_bounds__(1024) moe_mean_k(float* mean, const float* __restrict__ part, int blocks, int E, float inv) {
   mlb_pdl_sync();
-  const int e = blockIdx.x * 32 + (threadIdx.x & 31), s = threadIdx.x >> 5;
-  __shared__ float red[8][32];
+  const int lane = threadIdx.x & 31, e = blockIdx.x * 32 + lane, s = threadIdx.x >> 5;
+  __shared__ float red[32][33];
   float t = 0.f;
   if (e < E) {
-#pragma unroll 8
-    for (int b = s; b < blocks; b += 8) t += part[(long)b * E + e];
+#pragma unroll 10
+    for (int b = s; b < blocks; b += 32) t += part[(long)b * E + e];
   }
-  red[s][threadIdx.x & 31] = t;
+  red[s][lane] = t;
   __syncthreads();
-  if (s == 0 && e < E) {
-    t = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; k++) t += red[k][threadIdx.x];
-    mean[e] = t * inv;
-  }
+  t = warp_sum(red[lane][s]);      // (expert s of these 32)
+  if (lane == 0 && blockIdx.x * 32 + s < E) mean[blockIdx.x * 32 + s] = t * inv;
 }
 
 // ------------------------------------------------------------------ backward
@@ -332,9 +518,20 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_bwd_k(const RouteB
   }
 }
 
-int route_blocks(long N, int E) {
-  const long want = (N + ROUTE_WARPS - 1) / ROUTE_WARPS, most = (long)mlb_sm_count() * 6;
+// A warp has a token, or some where the blocks' sums of probabilities are to be added up (or there are very many tokens)
+int route_blocks(long N, bool sums) {
+  const long want = (N + ROUTE_WARPS - 1) / ROUTE_WARPS, most = sums ? (long)mlb_sm_count() * 4 : 1L << 16;
   return (int)std::max(1L, std::min(want, most));
+}
+constexpr size_t ROUTE_LISTS = sizeof(uint2) * ROUTE_WARPS * 32;
+template <auto KERN>
+int launch_route(const RouteArgs& A, int blocks, size_t smem, cudaStream_t st) {
+  if (smem > 48 * 1024) {
+    static std::atomic<unsigned long long> done{0};
+    const cudaError_t e = mlb_allow_smem(KERN, ROUTE_LISTS + sizeof(double) * ROUTE_WARPS * MAX_E, done);
+    if (e != cudaSuccess) return (int)e;
+  }
+  return (int)mlb_launch(KERN, dim3(blocks), dim3(32 * ROUTE_WARPS), smem, st, A);
 }
 template <typename F>
 int by_width(int E, F&& f) {
@@ -349,7 +546,7 @@ int by_width(int E, F&& f) {
 }  // namespace
 
 // floats of the workspace of a call with means
-MLB_API long mlb_moe_route_part(long N, int E) { return (long)route_blocks(N, E) * E; }
+MLB_API long mlb_moe_route_part(long N, int E) { return (long)route_blocks(N, true) * E; }
 MLB_API int mlb_moe_route(void* weights, int* idx, float* mean, float* part, const void* logits, const float* bias, long N, long ld, int E, int k, int sigmoid, int groups, int top, int renorm,
                           float scale, int zbits, int wbits, cudaStream_t st) {
   if (N < 0 || E < 1 || E > MAX_E || k < 1 || k > MAX_K || k > E || groups < 1 || groups > MAX_GROUPS || E % groups != 0 || top < 1 || top > groups || (zbits != 16 && zbits != 32) ||
@@ -357,21 +554,15 @@ MLB_API int mlb_moe_route(void* weights, int* idx, float* mean, float* part, con
     return -7;
   if (N == 0) return 0;
   const RouteArgs A = {logits, bias, weights, idx, mean ? part : nullptr, N, ld, E, k, groups, top, sigmoid, renorm, wbits == 32, scale};
-  const int blocks = route_blocks(N, E);
-  const size_t smem = std::max(groups > 1 ? sizeof(double) * ROUTE_WARPS * E : 0, mean ? sizeof(float) * ROUTE_WARPS * E : 0);
+  const int blocks = route_blocks(N, mean != nullptr);
+  const bool plain = bias == nullptr && groups == 1;
+  const size_t smem = std::max(ROUTE_LISTS + (plain ? 0 : sizeof(double) * ROUTE_WARPS * E), mean ? sizeof(float) * ROUTE_WARPS * E : 0);
   int rc = by_width(E, [&](auto V) {
-    auto go = [&](auto kern) {
-      if (smem > 48 * 1024) {
-        static std::atomic<unsigned long long> done{0};
-        const cudaError_t e = mlb_allow_smem(kern, sizeof(double) * ROUTE_WARPS * MAX_E, done);
-        if (e != cudaSuccess) return (int)e;
-      }
-      return (int)mlb_launch(kern, dim3(blocks), dim3(32 * ROUTE_WARPS), smem, st, A);
-    };
-    return zbits == 16 ? go(moe_route_k<V.value, bf16>) : go(moe_route_k<V.value, float>);
+    if (plain) return zbits == 16 ? launch_route<moe_route_k<V.value, bf16, true>>(A, blocks, smem, st) : launch_route<moe_route_k<V.value, float, true>>(A, blocks, smem, st);
+    return zbits == 16 ? launch_route<moe_route_k<V.value, bf16, false>>(A, blocks, smem, st) : launch_route<moe_route_k<V.value, float, false>>(A, blocks, smem, st);
   });
   if (rc == 0 && mean != nullptr)
-    rc = (int)mlb_launch(moe_mean_k, dim3((E + 31) / 32), dim3(256), 0, st, mean, (const float*)part, blocks, E, 1.f / (float)N);
+    rc = (int)mlb_launch(moe_mean_k, dim3((E + 31) / 32), dim3(1024), 0, st, mean, (const float*)part, blocks, E, 1.f / (float)N);
   return rc;
 }
 MLB_API int mlb_moe_route_bwd(void* dlogits, const void* dweights, const float* dmean, const void* logits, const int* idx, long N, long ld, int E, int k, int sigmoid, int renorm, float scale,
@@ -380,7 +571,7 @@ MLB_API int mlb_moe_route_bwd(void* dlogits, const void* dweights, const float* 
   if (N == 0) return 0;
   const RouteBwdArgs A = {dlogits, dweights, logits, dmean, idx, N, ld, E, k, sigmoid, renorm, wbits == 32, scale};
   return by_width(E, [&](auto V) {
-    auto go = [&](auto kern) { return (int)mlb_launch(kern, dim3(route_blocks(N, E)), dim3(32 * ROUTE_WARPS), 0, st, A); };
+    auto go = [&](auto kern) { return (int)mlb_launch(kern, dim3(route_blocks(N, false)), dim3(32 * ROUTE_WARPS), 0, st, A); };
     return zbits == 16 ? go(moe_route_bwd_k<V.value, bf16>) : go(moe_route_bwd_k<V.value, float>);
   });
 }

@@ -99,7 +99,9 @@ typedef std::optional<Tensor> Maybe;      // (an undefined tensor is no argument
   X(mlb_moe_plan, int, (int*, const int*, long, int, int, St))                                                                                 \
   X(mlb_moe_fwd, int, (void*, void*, void*, void*, void*, const void*, const void*, const void*, const void*, const int*, long, long, int, int, int, int, int, St)) \
   X(mlb_moe_bwd, int, (void*, void*, void*, void*, void*, void*, void*, const void*, const void*, const void*, const void*, const void*, const void*, const void*, const void*, const int*, \
-                       long, long, int, int, int, int, int, St))
+                       long, long, int, int, int, int, int, St))                                                                              \
+  X(mlb_moe_few_floats, long, (long, int, int, int, int))                                                                                      \
+  X(mlb_moe_few, int, (void*, const void*, const void*, const int*, const void*, const void*, float*, int*, long, long, int, int, int, int, int, St))
 #define MLB_POINTER(name, ret, args) ret(*name) args = nullptr;
 struct Entries { MLB_ENTRIES(MLB_POINTER) MLB_GENERATION(MLB_POINTER) MLB_MOE(MLB_POINTER) } K;
 
@@ -407,6 +409,104 @@ struct CrossEntropyFn : torch::autograd::Function<CrossEntropyFn> {
   }
 };
 
+// ------------------------------------------------------------------ experts
+struct Routing { int k, sigmoid, groups, top, renorm, wide; double scale; };
+struct Routed { Tensor weights, idx, mean; };
+int bits(const Tensor& t) { return t.scalar_type() == at::kFloat ? 32 : 16; }
+// Rows that the kernels of routing read: neighbouring elements, any distance
+Tensor plain_rows(const Tensor& z) { return z.size(1) == 1 || z.stride(1) == 1 ? z : z.contiguous(); }
+long row_step(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+Routed route_forward(const Tensor& logits, const Tensor& bias, const Routing& r) {
+  const Tensor z = plain_rows(logits);
+  const long N = z.size(0), E = z.size(1);
+  Routed out{at::empty({N, r.k}, z.options().dtype(r.wide ? at::kFloat : at::kBFloat16)), at::empty({N, r.k}, z.options().dtype(at::kInt)), f32(z, {E})};
+  const Tensor part = f32(z, {K.mlb_moe_route_part(N, (int)E)});
+  check(K.mlb_moe_route(out.weights.data_ptr(), (int*)out.idx.data_ptr(), (float*)out.mean.data_ptr(), (float*)part.data_ptr(), z.data_ptr(),
+                        bias.defined() ? (const float*)bias.data_ptr() : nullptr, N, row_step(z), (int)E, r.k, r.sigmoid, r.groups, r.top, r.renorm, (float)r.scale, bits(z), bits(out.weights),
+                        stream()),
+        "moe_route");
+  return out;
+}
+struct RouteFn : torch::autograd::Function<RouteFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Maybe& bias, int64_t k, int64_t sigmoid, int64_t groups, int64_t top, int64_t renorm, int64_t wide, double scale) {
+    const Routing r{(int)k, (int)sigmoid, (int)groups, (int)top, (int)renorm, (int)wide, scale};
+    const Routed out = route_forward(logits, bias.value_or(Tensor()), r);
+    ctx->save_for_backward({logits, out.idx});
+    ctx->saved_data["how"] = std::vector<int64_t>{logits.size(0), logits.size(1), k, sigmoid, renorm, wide, logits.scalar_type() == at::kFloat};
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({out.idx});
+    ctx->set_materialize_grads(false);
+    return {out.weights, out.idx, out.mean};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list none(9);
+    const Tensor &dw_ = g[0], &dm_ = g[2];
+    if (!dw_.defined() && !dm_.defined()) return none;
+    const auto how = ctx->saved_data["how"].toIntVector();
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& like = dw_.defined() ? dw_ : dm_;
+    const long N = how[0], E = how[1], k = how[2];
+    const Tensor z = unpacked(saved[0], like, how[6] ? at::kFloat : at::kBFloat16, {N, E}), idx = unpacked(saved[1], like, at::kInt, {N, k});
+    const auto wide = how[5] ? at::kFloat : at::kBFloat16;
+    const Tensor dw = dw_.defined() ? dw_.to(wide).contiguous() : at::zeros({N, k}, z.options().dtype(wide)), dm = dm_.defined() ? dm_.to(at::kFloat).contiguous() : Tensor();
+    none[0] = at::empty({N, E}, z.options());
+    check(K.mlb_moe_route_bwd(none[0].data_ptr(), dw.data_ptr(), dm.defined() ? (const float*)dm.data_ptr() : nullptr, z.data_ptr(), (const int*)idx.data_ptr(), N, E, (int)E, (int)k, (int)how[3],
+                              (int)how[4], (float)ctx->saved_data["scale"].toDouble(), bits(z), bits(dw), stream()),
+          "moe_route_bwd");
+    return none;
+  }
+};
+struct Experts { Tensor x, weights, idx, gate_up, down; };
+struct Held { Tensor plan, xs, gu, h, y; };      // what backward needs
+Tensor experts_forward(const Experts& a, Held* held, Tensor out) {
+  const long N = a.x.size(0), C = a.x.size(1), I = a.down.size(2);
+  const int k = (int)a.idx.size(1), E = (int)a.down.size(0);
+  const St st = stream();
+  Held t;
+  const auto ints = a.idx.options();
+  const long R = K.mlb_moe_plan_rows(N, k, E);
+  t.plan = at::empty({K.mlb_moe_plan_ints(N, k, E)}, ints);
+  check(K.mlb_moe_plan((int*)t.plan.data_ptr(), (const int*)a.idx.data_ptr(), N, k, E, st), "moe_plan");
+  const auto rows = [&](long c) { return at::empty({R, c}, a.x.options()); };
+  t.xs = rows(C), t.h = rows(I), t.y = rows(C);
+  if (held) t.gu = rows(2 * I);
+  if (!out.defined()) out = at::empty({N, C}, a.x.options());
+  check(K.mlb_moe_fwd(out.data_ptr(), t.xs.data_ptr(), held ? t.gu.data_ptr() : nullptr, t.h.data_ptr(), t.y.data_ptr(), a.x.data_ptr(), a.weights.data_ptr(), a.gate_up.data_ptr(),
+                      a.down.data_ptr(), (const int*)t.plan.data_ptr(), N, row_step(a.x), k, E, (int)C, (int)I, bits(a.weights), st),
+        "moe_mlp");
+  if (held) *held = t;
+  return out;
+}
+struct ExpertsFn : torch::autograd::Function<ExpertsFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weights, const Tensor& idx, const Tensor& gate_up, const Tensor& down) {
+    Held t;
+    const Tensor out = experts_forward({x, weights, idx, gate_up, down}, &t, Tensor());
+    ctx->save_for_backward({weights, gate_up, down, t.plan, t.xs, t.gu, t.h, t.y});
+    ctx->saved_data["dims"] = std::vector<int64_t>{x.size(0), idx.size(1), down.size(0), x.size(1), down.size(2), weights.scalar_type() == at::kFloat};
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto d = ctx->saved_data["dims"].toIntVector();
+    const long N = d[0], k = d[1], E = d[2], C = d[3], I = d[4], R = K.mlb_moe_plan_rows(N, (int)k, (int)E);
+    const auto saved = ctx->get_saved_variables();
+    const Tensor dout = rows_of(g[0]);
+    const Tensor w = unpacked(saved[0], dout, d[5] ? at::kFloat : at::kBFloat16, {N, k}), gate_up = unpacked_bf(saved[1], dout, {E, 2 * I, C}), down = unpacked_bf(saved[2], dout, {E, C, I}),
+                 plan = unpacked(saved[3], dout, at::kInt, {K.mlb_moe_plan_ints(N, (int)k, (int)E)}), xs = unpacked_bf(saved[4], dout, {R, C}), gu = unpacked_bf(saved[5], dout, {R, 2 * I}),
+                 h = unpacked_bf(saved[6], dout, {R, I}), y = unpacked_bf(saved[7], dout, {R, C});
+    const auto rows = [&](long c) { return at::empty({R, c}, dout.options()); };
+    Tensor dx, dw = at::empty_like(w), dgate_up, ddown;
+    if (ctx->needs_input_grad(0)) dx = at::empty({N, C}, dout.options());
+    if (ctx->needs_input_grad(3)) dgate_up = at::empty({E, 2 * I, C}, dout.options());
+    if (ctx->needs_input_grad(4)) ddown = at::empty({E, C, I}, dout.options());
+    const Tensor ys = rows(C), dgu = rows(2 * I), dxs = rows(C);
+    const auto at_ = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    check(K.mlb_moe_bwd(at_(dx), dw.data_ptr(), at_(dgate_up), at_(ddown), ys.data_ptr(), dgu.data_ptr(), dxs.data_ptr(), dout.data_ptr(), xs.data_ptr(), gu.data_ptr(), h.data_ptr(),
+                        y.data_ptr(), w.data_ptr(), gate_up.data_ptr(), down.data_ptr(), (const int*)plan.data_ptr(), N, C, (int)k, (int)E, (int)C, (int)I, bits(w), stream()),
+          "moe_mlp_bwd");
+    return {dx, ctx->needs_input_grad(1) ? dw : Tensor(), Tensor(), dgate_up, ddown};
+  }
+};
+
 // ------------------------------------------------------------------ Python entry points
 PyObject* declined() { Py_RETURN_NOTIMPLEMENTED; }
 template <typename F>
@@ -591,7 +691,7 @@ bool pool_given(PyObject* o, Pool& p, int dim) {
 }
 // Workspace of the calling thread on its current stream, kept from call to call; counters are zero between calls (never given back: the thread may end after torch)
 struct Kept { int op; c10::DeviceIndex device; St st; Tensor part, count; };
-enum { KEPT_ATTN, KEPT_TABLES, KEPT_SELECT };
+enum { KEPT_ATTN, KEPT_TABLES, KEPT_SELECT, KEPT_EXPERTS };
 Kept& kept(int op, const Tensor& like, St st, long floats, long counters) {
   static thread_local auto* all = new std::vector<Kept>();
   Kept* k = nullptr;
@@ -749,6 +849,109 @@ PyObject* py_beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {      //
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------ experts
+bool flag_arg(PyObject* o, int& v) {
+  if (!PyBool_Check(o)) return false;
+  v = o == Py_True;
+  return true;
+}
+bool score_arg(PyObject* o, int& sigmoid) {
+  if (!PyUnicode_CheckExact(o)) return false;
+  sigmoid = PyUnicode_CompareWithASCIIString(o, "sigmoid") == 0;
+  return sigmoid || PyUnicode_CompareWithASCIIString(o, "softmax") == 0;
+}
+bool wide_or_half(PyObject* o, Tensor& t, int dim) { return plain(o, t, at::kFloat, dim) || plain(o, t, at::kBFloat16, dim); }
+// logits, and what follows them: (bias, score, groups, top_groups, renorm, scale)
+bool routing_given(PyObject* logits, PyObject* const* a, Tensor& z, Tensor& bias, Routing& r) {
+  long groups, top;
+  if (!wide_or_half(logits, z, 2) || !score_arg(a[1], r.sigmoid) || !int_arg(a[2], groups) || !int_arg(a[3], top) || !flag_arg(a[4], r.renorm) || !PyFloat_CheckExact(a[5])) return false;
+  r.scale = PyFloat_AS_DOUBLE(a[5]);
+  const long E = z.size(1);
+  if (E > 1024 || groups < 1 || groups > 32 || E % groups != 0 || top < 1 || top > groups) return false;
+  r.groups = (int)groups, r.top = (int)top;
+  if (a[0] != Py_None && !given(a[0], bias, at::kFloat, {E})) return false;
+  return r.k >= 1 && r.k <= 32 && r.k <= top * (E / groups);
+}
+PyObject* py_moe_route(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (logits, k, bias, score, groups, top_groups, renorm, scale, fp32 weights) -> (weights, idx, mean)
+  HANDLE_TH_ERRORS
+  Tensor z, bias;
+  Routing r{};
+  long k;
+  if (n != 9 || transformed() || !int_arg(a[1], k) || k > 32) return declined();
+  r.k = (int)k;
+  if (!routing_given(a[0], a + 2, z, bias, r) || !flag_arg(a[8], r.wide) || bias.requires_grad()) return declined();
+  Routed out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (wants_grad({&z})) {
+      const variable_list v = RouteFn::apply(z, maybe(bias), r.k, r.sigmoid, r.groups, r.top, r.renorm, r.wide, r.scale);
+      out = {v[0], v[1], v[2]};
+    } else {
+      out = route_forward(z, bias, r);
+    }
+  }
+  PyObject* t = PyTuple_New(3);
+  if (!t) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(out.weights)));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(out.idx)));
+  PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(std::move(out.mean)));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_moe_route_out(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (weights, idx, logits, bias, score, groups, top_groups, renorm, scale): no means
+  HANDLE_TH_ERRORS
+  Tensor w, idx, z, bias;
+  Routing r{};
+  if (n != 9 || transformed() || !wide_or_half(a[0], w, 2) || !plain(a[1], idx, at::kInt, 2)) return declined();
+  r.k = (int)std::min<long>(idx.size(1), 33);
+  if (!routing_given(a[2], a + 3, z, bias, r)) return declined();
+  const long N = z.size(0), E = z.size(1);
+  if (!sized(w, {N, r.k}) || !sized(idx, {N, r.k}) || (E > 1 && z.stride(1) != 1) || (N > 1 && z.stride(0) < E)) return declined();
+  return launched("moe_route", [&] {
+    return K.mlb_moe_route(w.data_ptr(), (int*)idx.data_ptr(), nullptr, nullptr, z.data_ptr(), bias.defined() ? (const float*)bias.data_ptr() : nullptr, N, row_step(z), (int)E, r.k, r.sigmoid,
+                           r.groups, r.top, r.renorm, (float)r.scale, bits(z), bits(w), stream());
+  });
+  END_HANDLE_TH_ERRORS
+}
+bool experts_given(PyObject* const* a, Experts& e) {      // (x, weights, idx, gate_up, down)
+  if (!plain_bf(a[0], e.x, 2) || !wide_or_half(a[1], e.weights, 2) || !plain(a[2], e.idx, at::kInt, 2) || !plain_bf(a[3], e.gate_up, 3) || !plain_bf(a[4], e.down, 3)) return false;
+  const long N = e.x.size(0), C = e.x.size(1), E = e.down.size(0), I = e.down.size(2), k = e.idx.size(1);
+  return sized(e.weights, {N, k}) && sized(e.idx, {N, k}) && sized(e.down, {E, C, I}) && sized(e.gate_up, {E, 2 * I, C}) && (C == 1 || e.x.stride(1) == 1) && row_step(e.x) % 8 == 0 &&
+         row_step(e.x) >= C && C % 16 == 0 && I % 16 == 0 && C <= (1 << 20) && I <= (1 << 20) && E <= 1024 && N < (1L << 31) && N * k + 32 * E < (1L << 31);
+}
+PyObject* py_moe_mlp(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (x, weights, idx, gate_up, down) -> out, in training
+  HANDLE_TH_ERRORS
+  Experts e;
+  if (n != 5 || transformed() || !experts_given(a, e)) return declined();
+  return released([&] { return ExpertsFn::apply(e.x, e.weights, e.idx, e.gate_up, e.down); });
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_moe_mlp_out(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (out, x, weights, idx, gate_up, down)
+  HANDLE_TH_ERRORS
+  Experts e;
+  Tensor out;
+  if (n != 6 || transformed() || !experts_given(a + 1, e)) return declined();
+  const long N = e.x.size(0), C = e.x.size(1), I = e.down.size(2);
+  const int k = (int)e.idx.size(1), E = (int)e.down.size(0);
+  if (!given(a[0], out, at::kBFloat16, {N, C}) || !aligned(out)) return declined();
+  const St st = stream();
+  const long few = K.mlb_moe_few_floats(N, k, E, (int)C, (int)I);
+  if (few > 0) {
+    if (K.mlb_capture_id(st) != 0) return declined();
+    const Kept& w = kept(KEPT_EXPERTS, e.x, st, few, C / 16);
+    return launched("moe_mlp", [&] {
+      return K.mlb_moe_few(out.data_ptr(), e.x.data_ptr(), e.weights.data_ptr(), (const int*)e.idx.data_ptr(), e.gate_up.data_ptr(), e.down.data_ptr(), (float*)w.part.data_ptr(),
+                           (int*)w.count.data_ptr(), N, row_step(e.x), k, E, (int)C, (int)I, bits(e.weights), st);
+    });
+  }
+  {
+    pybind11::gil_scoped_release no_gil;
+    experts_forward(e, nullptr, out);
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(path, settings): the kernel library whose functions are called, the module with the variables above
 PyObject* py_bind(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
@@ -802,6 +1005,7 @@ PyObject* py_moe_signatures(PyObject*, PyObject*) {
 #define MLB_METHOD(name, ret, args) {#name, (PyCFunction)(void (*)(void))call_##name, METH_FASTCALL, nullptr},
 PyMethodDef methods[] = {MLB_FAST(linear), MLB_FAST(rmsnorm), MLB_FAST(layer_norm), MLB_FAST(swiglu), MLB_FAST(rope_causal_attention), MLB_FAST(bidir_attention),
                          MLB_FAST(cross_entropy), MLB_FAST(kv4_append), MLB_FAST(kv4_read), MLB_FAST(kv4_attn), MLB_FAST(block_tables), MLB_FAST(beam_select), MLB_FAST(beam_reorder),
+                         MLB_FAST(moe_route), MLB_FAST(moe_route_out), MLB_FAST(moe_mlp), MLB_FAST(moe_mlp_out),
                          MLB_ENTRIES(MLB_METHOD) MLB_GENERATION(MLB_METHOD) MLB_MOE(MLB_METHOD) {"bind", py_bind, METH_VARARGS, nullptr}, {"signatures", py_signatures, METH_NOARGS, nullptr},
                          {"generation_signatures", py_generation_signatures, METH_NOARGS, nullptr}, {"moe_signatures", py_moe_signatures, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mlb_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

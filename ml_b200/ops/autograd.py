@@ -304,13 +304,16 @@ embedding = Embedding.apply
 def moe_route(logits, k, bias=None, score="softmax", groups=1, top_groups=1, renorm=True, scale=1.0, dtype=None):
     """(weights [N, k], idx int32 [N, k], mean fp32 [E]): each token's k experts, best first, their weights in `dtype` (None: that of the logits), and the experts' mean
     probabilities, from which a loss that balances them is formed.  ops/ref_moe.py says what they are."""
-    return MoERoute.apply(logits, k, bias, score, groups, top_groups, renorm, scale, dtype or logits.dtype)
+    dtype = dtype or logits.dtype
+    y = _plain("moe_route", logits, k, bias, score, groups, top_groups, renorm, scale, dtype is torch.float32) if dtype in (torch.float32, torch.bfloat16) else NotImplemented
+    return MoERoute.apply(logits, k, bias, score, groups, top_groups, renorm, scale, dtype) if y is NotImplemented else y
 
 
 def moe_mlp(x, weights, idx, gate_up, down):
     """x [N, C] through the SwiGLU experts gate_up [E, 2 I, C], down [E, C, I] that `moe_route` chose, weighted and added up."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weights, gate_up, down)):
-        return MoEMLP.apply(x, weights, idx, gate_up, down)
+        y = _plain("moe_mlp", x, weights, idx, gate_up, down)
+        return MoEMLP.apply(x, weights, idx, gate_up, down) if y is NotImplemented else y
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     ops.moe_mlp(out, x, weights.contiguous(), idx.contiguous(), gate_up.contiguous(), down.contiguous())
     return out

@@ -49,7 +49,8 @@ _GEN_KINDS = {
 # ... and those of the experts of a mixture (ops/native_moe.py)
 _MOE_KINDS = {
     "moe_route_part": "ln", "moe_route": "biffbfllnnnnnndnns", "moe_route_bwd": "bbfbillnnnndnns", "moe_plan_ints": "lnn", "moe_plan_rows": "lnn", "moe_plan": "iilnns",
-    "moe_fwd": "bbbbbbbbbillnnnnns", "moe_bwd": "bbbbbbbbbbbbbbbillnnnnns"}
+    "moe_fwd": "bbbbbbbbbillnnnnns", "moe_bwd": "bbbbbbbbbbbbbbbillnnnnns",
+    "moe_few_floats": "lnnnn", "moe_few": "bbbibbfillnnnnns"}
 _CTYPES = {"n": _i32, "l": _i64, "d": _f32}      # (else a pointer)
 
 
@@ -104,7 +105,7 @@ def lib():
         fn.argtypes = args
         fn.restype = _i32
     L.mlb_attn_bwd_scratch_bytes.restype = L.mlb_kv4_attn_scratch.restype = _i64
-    L.mlb_moe_route_part.restype = L.mlb_moe_plan_ints.restype = L.mlb_moe_plan_rows.restype = _i64
+    L.mlb_moe_route_part.restype = L.mlb_moe_plan_ints.restype = L.mlb_moe_plan_rows.restype = L.mlb_moe_few_floats.restype = _i64
     L.mlb_capture_id.restype = C.c_ulonglong
     for tag in _ERROR_WORDS:
         for pre in ("mlb_get_error_", "mlb_clear_error_"):

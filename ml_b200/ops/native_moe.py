@@ -50,8 +50,18 @@ def _rows(t, what, eights=True):
     return ld
 
 
+def _plain(name, *args):
+    e = _n._entries()
+    if e is not _n.bridge() or getattr(e, name)(*args) is NotImplemented:
+        return False
+    _n.LAUNCHES += 1
+    return True
+
+
 # ------------------------------------------------------------------ routing
 def moe_route(weights, idx, mean, logits, bias=None, score="softmax", groups=1, top_groups=1, renorm=True, scale=1.0):
+    if mean is None and _plain("moe_route_out", weights, idx, logits, bias, score, groups, top_groups, renorm, scale):
+        return
     N, E, k = check_route(weights, idx, mean, logits, bias, score, groups, top_groups)
     _here(weights, idx, mean, logits, bias)
     _dense(weights=weights, idx=idx, mean=mean, bias=bias)
@@ -103,14 +113,22 @@ def _fwd(out, x, weights, idx, gate_up, down, keep):
     ldx = _rows(x, "x")
     if N == 0:
         return None
+    e = _n._entries()
+    few = 0 if keep else e.mlb_moe_few_floats(N, k, E, C, I)
+    if few:
+        part, count = _n.scratch("moe_few", few, F32, x.device), _n.scratch("moe_count", C // 16, I32, x.device, zero=True)
+        _took(e.mlb_moe_few(out, _at(x), _at(weights), idx, gate_up, down, part, count, N, ldx, k, E, C, I, _bits(weights)), "moe_mlp")
+        return None
     plan, R = _plan(idx, E)
     new = lambda c: torch.empty(R, c, dtype=BF16, device=x.device)
     xs, gu, h, y = new(C), new(2 * I) if keep else None, new(I), new(C)
-    _took(_n._entries().mlb_moe_fwd(out, xs, _at(gu), h, y, _at(x), _at(weights), gate_up, down, plan, N, ldx, k, E, C, I, _bits(weights)), "moe_mlp")
+    _took(e.mlb_moe_fwd(out, xs, _at(gu), h, y, _at(x), _at(weights), gate_up, down, plan, N, ldx, k, E, C, I, _bits(weights)), "moe_mlp")
     return plan, xs, gu, h, y
 
 
 def moe_mlp(out, x, weights, idx, gate_up, down):
+    if _plain("moe_mlp_out", out, x, weights, idx, gate_up, down):
+        return
     _fwd(out, x, weights, idx, gate_up, down, False)
 
 
