@@ -698,69 +698,72 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
 }
 
 // ------------------------------------------------------------------ few tokens
-// A step of a few tokens reads the weights of the experts that they chose, once, and that is all its time: the products are m16n8k16 instructions whose 16 rows of weights come
-// straight from memory to registers, 16 bytes a lane (which eight elements of the reduction an instruction has is the same for both operands, so a lane's eight
-// neighbouring ones serve as those of two instructions) and whose 8 columns are tokens of one expert.  A thread block shares the reduction of 16 rows among its
-// eight warps and adds up their parts in shared memory; 64 KB are on their way for each block at 2048 columns.  Two launches: h of all copies, a row of gate and of up
-// projection each in the instruction's halves; then y, whose last block for 16 columns forms the weighted sums of its 16 columns.
-// An expert's copies are found by each block for itself: 256 at most.
-constexpr int FEW_TOKENS = 32, FEW_COPIES = 256, FEW_THREADS = 256, FEW_BATCH = 6;
+// A step of a few tokens reads the weights of the experts that they chose, once, and that is all its time.  One, two, four or eight warps share units of 16 rows of one
+// expert, each the boxes of 16 rows x 64 columns of its part of the reduction, which it fetches into shared memory of its own: three stages of four boxes a warp, 192 KB an SM on
+// their way.  The products are m16n8k16 instructions whose 16 rows are weights and whose 8 columns are tokens (which eight elements of the reduction an instruction
+// has is the same for both operands: 16 neighbouring bytes a lane serve two instructions).  Three launches: h of all copies, with 8 rows of the gate and 8 of the up
+// projection to a unit; y; their weighted sums.  An expert's copies are found by each block for itself: 256 at most.
+constexpr int FEW_TOKENS = 8, FEW_COPIES = 256, FEW_WARPS = 8, FEW_THREADS = 32 * FEW_WARPS, FEW_BOX = 2048, FEW_BOXES = 4, FEW_STAGES = 3;
+constexpr int FEW_SMEM = FEW_WARPS * FEW_STAGES * FEW_BOXES * FEW_BOX + 1024;
 struct FewArgs {
-  bf16* out;            // DOWN: [N, C]
   bf16* h;              // [N k, I]
   float* y;             // [N k, C]
-  int* count;           // [C / 16] blocks that are done with 16 columns; 0 between calls
-  const bf16 *x, *W;
-  const void* weights;
+  const bf16* x;
   const int* idx;
   long ldx;
-  int N, k, E, C, I, wide_w;
+  int N, k, E, C, I, ways;      // ways: warps that share a unit
 };
-__device__ __forceinline__ uint4 load_weights(const bf16* p) {      // (each is used once: it stays out of the L1, which holds the tokens)
-  uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <int NT, bool DOWN_>
-__global__ void __launch_bounds__(FEW_THREADS, 3) moe_few_k(const FewArgs A) {
-  mlb_pdl_sync();
+template <bool DOWN_>
+__global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_k(const __grid_constant__ CUtensorMap tmW, const FewArgs A) {
+  // The kernel before the one for y is that for h, which has waited for all before it: idx and the weights stand, and only h has to be waited for.  (Past the L1, of
+  // which nothing is known so early.)
+  if (!DOWN_) mlb_pdl_sync();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(16) int expert[FEW_COPIES];
-  __shared__ int list[FEW_COPIES], nth[FEW_COPIES], first[FEW_COPIES + 1], of[FEW_COPIES], sums[FEW_THREADS / 32], last;
-  __shared__ float part[8][NT * 128];
+  __shared__ int list[FEW_COPIES], nth[FEW_COPIES], first[FEW_COPIES + 1], of[FEW_COPIES], sums[FEW_WARPS];
+  __shared__ uint64_t full[FEW_WARPS][FEW_STAGES];
+  __shared__ float4 part[2][FEW_WARPS][32];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, NK = A.N * A.k;
   // the copies by expert: a copy's place is the number of those before it.  More copies than an instruction's columns (a token may name an expert twice) are dealt with as if
   // another expert had them.
-  int e = tid < NK ? A.idx[tid] : -1;
+  int e = tid < NK ? __ldcg(A.idx + tid) : -1;
   if (e >= A.E) {
-    if (blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xD1);
+    if (!DOWN_ && blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xD1);
     e = -1;
   }
-  expert[tid] = e < 0 ? 0x7fffffff : e;
-  list[tid] = -1;
-  __syncthreads();
-  int less = 0, equal = 0;
-#pragma unroll 4
-  for (int i = 0; i < NK; i += 4) {
-    const int4 x = *reinterpret_cast<const int4*>(expert + i);
-    less += (x.x < e) + (x.y < e) + (x.z < e) + (x.w < e);
-    equal += (x.x == e && i < tid) + (x.y == e && i + 1 < tid) + (x.z == e && i + 2 < tid) + (x.w == e && i + 3 < tid);
+  expert[tid] = e < 0 ? 0x7fffffff : e, list[tid] = -1;
+  if (lane == 0) {
+    for (int i = 0; i < FEW_STAGES; i++) tc::mbar_init(&full[w][i], 1);
+    tc::mbar_fence_init();
+    if (w == 0) tc::tma_prefetch_desc(&tmW);
   }
-  nth[tid] = equal;
-  if (e >= 0) list[less + equal] = tid;
+  __syncthreads();
+  if (e >= 0) {
+    int less = 0, equal = 0;
+#pragma unroll 4
+    for (int i = 0; i < NK; i += 4) {
+      const int4 x = *reinterpret_cast<const int4*>(expert + i);
+      less += (x.x < e) + (x.y < e) + (x.z < e) + (x.w < e);
+      equal += (x.x == e && i < tid) + (x.y == e && i + 1 < tid) + (x.z == e && i + 2 < tid) + (x.w == e && i + 3 < tid);
+    }
+    nth[tid] = equal;
+    list[less + equal] = tid;
+  }
   __syncthreads();
   const int here = list[tid];
-  const bool begins = here >= 0 && nth[here] % (8 * NT) == 0;
+  const bool begins = here >= 0 && nth[here] % 8 == 0;
   const unsigned b = __ballot_sync(0xffffffffu, begins);
   if (lane == 0) sums[w] = __popc(b);
   const int held = __syncthreads_count(here >= 0);
   int experts = 0, before = __popc(b & ((1u << lane) - 1));
 #pragma unroll
-  for (int i = 0; i < FEW_THREADS / 32; i++) {
+  for (int i = 0; i < FEW_WARPS; i++) {
     before += i < w ? sums[i] : 0;
     experts += sums[i];
   }
@@ -768,104 +771,115 @@ __global__ void __launch_bounds__(FEW_THREADS, 3) moe_few_k(const FewArgs A) {
   if (tid == 0) first[experts] = held;
   __syncthreads();
 
-  const int K = DOWN_ ? A.I : A.C, groups = DOWN_ ? A.C / 16 : A.I / 8, kbs = (K + 31) / 32, r = lane >> 2, t = lane & 3;
-  if (DOWN_ && experts == 0) {      // nothing for anybody
-    for (long i = (long)blockIdx.x * FEW_THREADS + tid; i < (long)A.N * A.C; i += (long)gridDim.x * FEW_THREADS) A.out[i] = __float2bfloat16(0.f);
-    return;
-  }
-  const int units = experts * groups;
-  uint4 wa[FEW_BATCH], wb[FEW_BATCH];
-  auto ask = [&](int unit, int kb0) {      // this warp's part of a batch of the unit's weights
-    const int a = unit / groups, g = unit - a * groups;
-    const bf16 *row0 = A.W + (size_t)of[a] * (DOWN_ ? (size_t)A.C * A.I : 2 * (size_t)A.I * A.C) + (size_t)(g * (DOWN_ ? 16 : 8) + r) * K, *row1 = row0 + (size_t)(DOWN_ ? 8 : A.I) * K;
+  const int K = DOWN_ ? A.I : A.C, groups = DOWN_ ? A.C / 16 : A.I / 8, units = experts * groups, boxes = (K + 63) / 64, steps = (boxes + FEW_BOXES - 1) / FEW_BOXES;
+  // the units of this warp and those beside it; of each it has the steps `part_of`, part_of + ways, ...
+  const int r = lane >> 2, t = lane & 3, ways = A.ways, part_of = w % ways, begin = blockIdx.x + w / ways * gridDim.x, every = gridDim.x * (FEW_WARPS / ways);
+  uint8_t* ring = smem + w * (FEW_STAGES * FEW_BOXES * FEW_BOX);
+  int next_unit = begin, next_s = part_of, asked = 0, n = 0, turn = 0;      // the step that is asked for next; how many have been, and have been dealt with
+  auto ask = [&]() {
+    if (next_unit >= units || part_of >= steps) return;
+    if (lane == 0) {
+      const int a = next_unit / groups, g = next_unit - a * groups, stage = asked % FEW_STAGES, some = min(FEW_BOXES, boxes - next_s * FEW_BOXES);
+      uint64_t* bar = &full[w][stage];
+      tc::mbar_expect_tx(bar, some * FEW_BOX);
+      for (int j = 0; j < some; j++) {
+        uint8_t* to = ring + (stage * FEW_BOXES + j) * FEW_BOX;
+        if (DOWN_) tc::tma_load_3d(to, &tmW, bar, (next_s * FEW_BOXES + j) * 64, g * 16, of[a]);
+        else tc::tma_load_5d(to, &tmW, bar, (next_s * FEW_BOXES + j) * 64, 0, 0, g, of[a]);
+      }
+    }
+    asked++;
+    if ((next_s += ways) >= steps) next_s = part_of, next_unit += every;
+  };
+  for (int i = 0; i < FEW_STAGES; i++) ask();
+  if (DOWN_) mlb_pdl_sync();
+  bool ok = true;
+  uint4 ahead[FEW_BOXES][2] = {};      // the tokens' part of the next step, asked for while this one goes on
+  auto tokens = [&](int unit, int s) {
+    const int a = unit / groups, f0 = first[a], c = list[f0 + min(r, first[a + 1] - f0 - 1)];      // (columns behind the last copy: its row, nothing of theirs is used)
+    const bf16* col = DOWN_ ? A.h + (size_t)c * A.I : A.x + (size_t)(c / A.k) * A.ldx;
 #pragma unroll
-    for (int i = 0; i < FEW_BATCH; i++) {
-      const int k = (kb0 + 8 * i) * 32 + t * 8;
-      wa[i] = k < K ? load_weights(row0 + k) : make_uint4(0, 0, 0, 0);
-      wb[i] = k < K ? load_weights(row1 + k) : make_uint4(0, 0, 0, 0);
+    for (int x = 0; x < 2 * FEW_BOXES; x++) {
+      const int k = (s * FEW_BOXES + x / 2) * 64 + x % 2 * 32 + t * 8;
+      ahead[x / 2][x % 2] = k < K ? __ldg(reinterpret_cast<const uint4*>(col + k)) : make_uint4(0, 0, 0, 0);
     }
   };
-  if (blockIdx.x < units) ask(blockIdx.x, w);
-  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+  if (begin < units && part_of < steps) tokens(begin, part_of);
+  for (int unit = begin; unit < units; unit += every, turn ^= 1) {
     const int a = unit / groups, g = unit - a * groups, f0 = first[a], copies = first[a + 1] - f0;
-    const bf16* col[NT];      // (columns behind the last copy: any row, nothing of theirs is used)
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      const int c = list[f0 + min(n * 8 + r, copies - 1)];
-      col[n] = DOWN_ ? A.h + (size_t)c * A.I : A.x + (size_t)(c / A.k) * A.ldx;
-    }
-    float d[NT][4] = {};
+    float d[2][4] = {};      // (two sums: neighbouring instructions do not wait for one another)
 #pragma unroll 1
-    for (int kb0 = w; kb0 < kbs || kb0 == w; kb0 += 8 * FEW_BATCH) {
+    for (int s = part_of; s < steps; s += ways, n++) {
+      uint4 v[FEW_BOXES][2];
 #pragma unroll
-      for (int i = 0; i < FEW_BATCH; i++) {
-        const int k = (kb0 + 8 * i) * 32 + t * 8;
-        if ((kb0 + 8 * i) * 32 >= K) break;      // (the warp's)
+      for (int x = 0; x < 2 * FEW_BOXES; x++) v[x / 2][x % 2] = ahead[x / 2][x % 2];
+      if (s + ways < steps) tokens(unit, s + ways);
+      else if (unit + every < units) tokens(unit + every, part_of);
+      const int stage = n % FEW_STAGES;
+      if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[w][stage], (n / FEW_STAGES) & 1, 0x76));
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          if (n * 8 >= copies) break;            // (the block's)
-          const uint4 v = k < K ? __ldg(reinterpret_cast<const uint4*>(col[n] + k)) : make_uint4(0, 0, 0, 0);
-          mma_16816(d[n], wa[i].x, wb[i].x, wa[i].y, wb[i].y, v.x, v.y);
-          mma_16816(d[n], wa[i].z, wb[i].z, wa[i].w, wb[i].w, v.z, v.w);
+      for (int x = 0; x < FEW_BOXES; x++) {
+        if (s * FEW_BOXES + x >= boxes) break;
+        const uint8_t* box = ring + (stage * FEW_BOXES + x) * FEW_BOX + r * 128;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int at = ((t + 4 * j) ^ r) << 4;
+          const uint4 p = *reinterpret_cast<const uint4*>(box + at), q = *reinterpret_cast<const uint4*>(box + 1024 + at);
+          mma_16816(d[0], p.x, q.x, p.y, q.y, v[x][j].x, v[x][j].y);
+          mma_16816(d[1], p.z, q.z, p.w, q.w, v[x][j].z, v[x][j].w);
         }
       }
-      // what comes next is on its way while the parts are added up
-      if (kb0 + 8 * FEW_BATCH < kbs) ask(unit, kb0 + 8 * FEW_BATCH);
-      else if (unit + (int)gridDim.x < units) ask(unit + gridDim.x, w);
+      __syncwarp();
+      ask();
     }
-    // d[n][2 h + x]: row 8 h + lane / 4, column 8 n + 2 (lane % 4) + x
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int x = 0; x < 4; x++) part[w][n * 128 + x * 32 + lane] = d[n][x];
-    __syncthreads();
-    if (DOWN_) {
-      for (int i = tid; i < NT * 128; i += FEW_THREADS) {
-        const int n = i >> 7, x = (i >> 5) & 3, l = i & 31, c = n * 8 + 2 * (l & 3) + (x & 1);
-        if (c >= copies) continue;
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) s += part[j][i];
-        A.y[(size_t)list[f0 + c] * A.C + g * 16 + (x >> 1) * 8 + (l >> 2)] = s;
-      }
-      __syncthreads();
-      if (tid == 0) last = mlb_count_block(A.count + g) == experts - 1;
-      __syncthreads();
-      if (last) {      // all experts are done with these 16 columns
-        for (int i = tid; i < A.N * 16; i += FEW_THREADS) {
-          const int n = i >> 4, c = g * 16 + (i & 15);
-          float s = 0.f;
-          for (int j = 0; j < A.k; j++) {
-            const int q = n * A.k + j;
-            if (expert[q] == 0x7fffffff) continue;
-            const float wq = A.wide_w ? ((const float*)A.weights)[q] : __bfloat162float(((const bf16*)A.weights)[q]);
-            s = fmaf(wq, __ldcg(A.y + (size_t)q * A.C + c), s);
-          }
-          A.out[(size_t)n * A.C + c] = __float2bfloat16(s);
-        }
-        if (tid == 0) A.count[g] = 0;
-      }
-    } else {
-      for (int i = tid; i < NT * 64; i += FEW_THREADS) {      // row lane / 4 is the gate's, row 8 + lane / 4 the up projection's
-        const int n = i >> 6, x = (i >> 5) & 1, l = i & 31, c = n * 8 + 2 * (l & 3) + x;
-        if (c >= copies) continue;
-        float gate = 0.f, up = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) gate += part[j][n * 128 + x * 32 + l], up += part[j][n * 128 + (x + 2) * 32 + l];
-        A.h[(size_t)list[f0 + c] * A.I + g * 8 + (l >> 2)] = __float2bfloat16(gate * rcp(1.f + ex2(-1.44269504f * gate)) * up);
+    // d[..][2 h + x]: row 8 h + lane / 4, column 2 (lane % 4) + x.  Of h's rows the first half is the gate's, the second the up projection's.
+    float4 sum = make_float4(d[0][0] + d[1][0], d[0][1] + d[1][1], d[0][2] + d[1][2], d[0][3] + d[1][3]);
+    if (ways > 1) {      // (two places in turn: whoever writes to one again has met the others behind their reading of it)
+      part[turn][w][lane] = sum;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + w / ways), "r"(32 * ways) : "memory");
+      if (part_of != 0) continue;
+      for (int j = 1; j < ways; j++) {
+        const float4 x = part[turn][w + j][lane];
+        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
       }
     }
-    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      if (2 * t + x >= copies) continue;
+      const float p = x ? sum.y : sum.x, q = x ? sum.w : sum.z;
+      const size_t to = list[f0 + 2 * t + x];
+      if (DOWN_) A.y[to * A.C + g * 16 + r] = p, A.y[to * A.C + g * 16 + 8 + r] = q;
+      else A.h[to * A.I + g * 8 + r] = __float2bfloat16(p * rcp(1.f + ex2(-1.44269504f * p)) * q);
+    }
   }
 }
-template <int NT>
-int launch_few(FewArgs g, const bf16* gate_up, const bf16* down, cudaStream_t st) {
-  const int experts = std::min(g.N * g.k, g.E), resident = mlb_sm_count() * 3;
-  g.W = gate_up;
-  cudaError_t e = mlb_launch(moe_few_k<NT, false>, dim3(std::min(experts * (g.I / 8), resident)), dim3(FEW_THREADS), 0, st, g);
+// out[n] = the weighted sum of its copies' y, four columns a thread
+template <typename W>
+__global__ void __launch_bounds__(128) moe_few_sum_k(bf16* __restrict__ out, const float* __restrict__ y, const W* __restrict__ weights, const int* __restrict__ idx, int N, int k, int E, int C) {
+  mlb_pdl_sync();
+  const int at = blockIdx.x * 128 + threadIdx.x, n = at / (C / 4), c = at - n * (C / 4);
+  if (n >= N) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int q = n * k; q < (n + 1) * k; q++) {
+    const int e = idx[q];
+    if (e < 0 || e >= E) continue;
+    const float w = as_float(weights[q]);
+    const float4 x = reinterpret_cast<const float4*>(y + (size_t)q * C)[c];
+    s.x = fmaf(w, x.x, s.x), s.y = fmaf(w, x.y, s.y), s.z = fmaf(w, x.z, s.z), s.w = fmaf(w, x.w, s.w);
+  }
+  reinterpret_cast<uint2*>(out + (size_t)n * C)[c] = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+}
+template <bool DOWN_>
+int launch_few(const CUtensorMap& m, FewArgs g, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = mlb_allow_smem(moe_few_k<DOWN_>, FEW_SMEM, done);
   if (e != cudaSuccess) return (int)e;
-  g.W = down;
-  return (int)mlb_launch(moe_few_k<NT, true>, dim3(std::min(experts * (g.C / 16), resident)), dim3(FEW_THREADS), 0, st, g);
+  const int units = std::min(g.N * g.k, g.E) * (DOWN_ ? g.C / 16 : g.I / 8), steps = ((DOWN_ ? g.I : g.C) + 255) / 256;
+  // As few warps to a unit as give most of an SM's warps one.  One token, us, by ways: 6 of 64 experts (1032 and 768 units) 28.3, 30.2, 31.9, 34.7; 2 of 8 experts of 5504 behind
+  // 2048 columns (1376 and 256) 53.5, 37.7, 33.3, 37.1; of 2048 behind 768 (512 and 96) 17.7, 12.8, 11.4, 13.3.
+  for (g.ways = 1; g.ways < FEW_WARPS && units * g.ways < 5 * mlb_sm_count() && 2 * g.ways <= steps;) g.ways *= 2;
+  return (int)mlb_launch(moe_few_k<DOWN_>, dim3(std::min(units, mlb_sm_count())), dim3(FEW_THREADS), (size_t)FEW_SMEM, st, m, g);
 }
 
 struct Maps { CUtensorMap a, b, b16, a1, b1, a2, b2, out, out1, out2; };
@@ -1022,16 +1036,24 @@ MLB_API int mlb_moe_bwd(void* dx, void* dweights, void* dgate_up, void* ddown, v
   MLB_TRY(launch_gemm<BACK>(m, g, (long)E * (g.per_gate_up + g.per_down) + (long)z.p.max_tiles * g.tiles_m, st));
   return dx != nullptr ? combine((bf16*)dx, (const bf16*)dxs, (const float*)nullptr, P, z, st) : 0;
 }
-// floats of the workspace of the form for few tokens: y, h and (the first C / 16 ints, 0 before the first call, left so by each) counters; 0: the sizes take the other form
+// floats of the workspace of the form for few tokens: y and h; 0: the sizes take the other form
 MLB_API long mlb_moe_few_floats(long N, int k, int E, int C, int I) {
   Sizes z;
   if (sizes(z, N, k, E, C, I) != 0 || N < 1 || N > FEW_TOKENS || z.NK > FEW_COPIES) return 0;
   return z.NK * C + (z.NK * I + 1) / 2;
 }
-MLB_API int mlb_moe_few(void* out, const void* x, const void* weights, const int* idx, const void* gate_up, const void* down, float* part, int* count, long N, long ldx, int k, int E, int C,
-                        int I, int wbits, cudaStream_t st) {
+MLB_API int mlb_moe_few(void* out, const void* x, const void* weights, const int* idx, const void* gate_up, const void* down, float* part, long N, long ldx, int k, int E, int C, int I,
+                        int wbits, cudaStream_t st) {
   if (mlb_moe_few_floats(N, k, E, C, I) == 0 || off16({out, x, gate_up, down, part}) || ldx % 8 != 0 || (wbits != 16 && wbits != 32)) return -7;
-  FewArgs g = {(bf16*)out, (bf16*)(part + N * k * C), part, count, (const bf16*)x, nullptr, weights, idx, ldx, (int)N, k, E, C, I, wbits == 32};
-  const bf16 *a = (const bf16*)gate_up, *b = (const bf16*)down;
-  return N <= 8 ? launch_few<1>(g, a, b, st) : N <= 16 ? launch_few<2>(g, a, b, st) : launch_few<4>(g, a, b, st);
+  const FewArgs g = {(bf16*)(part + N * k * C), part, (const bf16*)x, idx, ldx, (int)N, k, E, C, I, 1};
+  const uint64_t c = C, i = I, n = E;
+  const uint64_t da[5] = {c, 8, 2, i / 8, n}, sa[4] = {2 * c, 2 * i * c, 16 * c, 4 * i * c}, db[3] = {i, c, n}, sb[2] = {2 * i, 2 * c * i};
+  const uint32_t ba[5] = {64, 8, 2, 1, 1}, bb[3] = {64, 16, 1};
+  alignas(64) CUtensorMap a, b;
+  if (!mlb_make_tmap_nd(&a, gate_up, 5, da, sa, ba) || !mlb_make_tmap_nd(&b, down, 3, db, sb, bb)) return -2;
+  MLB_TRY(launch_few<false>(a, g, st));
+  MLB_TRY(launch_few<true>(b, g, st));
+  const dim3 blocks((unsigned)((N * (C / 4) + 127) / 128));
+  if (wbits == 16) return (int)mlb_launch(moe_few_sum_k<bf16>, blocks, dim3(128), 0, st, (bf16*)out, (const float*)part, (const bf16*)weights, idx, (int)N, k, E, C);
+  return (int)mlb_launch(moe_few_sum_k<float>, blocks, dim3(128), 0, st, (bf16*)out, (const float*)part, (const float*)weights, idx, (int)N, k, E, C);
 }

@@ -101,7 +101,7 @@ typedef std::optional<Tensor> Maybe;      // (an undefined tensor is no argument
   X(mlb_moe_bwd, int, (void*, void*, void*, void*, void*, void*, void*, const void*, const void*, const void*, const void*, const void*, const void*, const void*, const void*, const int*, \
                        long, long, int, int, int, int, int, St))                                                                              \
   X(mlb_moe_few_floats, long, (long, int, int, int, int))                                                                                      \
-  X(mlb_moe_few, int, (void*, const void*, const void*, const int*, const void*, const void*, float*, int*, long, long, int, int, int, int, int, St))
+  X(mlb_moe_few, int, (void*, const void*, const void*, const int*, const void*, const void*, float*, long, long, int, int, int, int, int, St))
 #define MLB_POINTER(name, ret, args) ret(*name) args = nullptr;
 struct Entries { MLB_ENTRIES(MLB_POINTER) MLB_GENERATION(MLB_POINTER) MLB_MOE(MLB_POINTER) } K;
 
@@ -702,7 +702,7 @@ Kept& kept(int op, const Tensor& like, St st, long floats, long counters) {
     k = &all->back();
   }
   if (floats > 0 && (!k->part.defined() || k->part.numel() < floats)) k->part = at::empty({floats}, like.options().dtype(at::kFloat));
-  if (!k->count.defined() || k->count.numel() < counters) k->count = at::zeros({counters}, like.options().dtype(at::kInt));
+  if (counters > 0 && (!k->count.defined() || k->count.numel() < counters)) k->count = at::zeros({counters}, like.options().dtype(at::kInt));
   return *k;
 }
 template <typename F>
@@ -938,10 +938,10 @@ PyObject* py_moe_mlp_out(PyObject*, PyObject* const* a, Py_ssize_t n) {      // 
   const long few = K.mlb_moe_few_floats(N, k, E, (int)C, (int)I);
   if (few > 0) {
     if (K.mlb_capture_id(st) != 0) return declined();
-    const Kept& w = kept(KEPT_EXPERTS, e.x, st, few, C / 16);
+    const Kept& w = kept(KEPT_EXPERTS, e.x, st, few, 0);
     return launched("moe_mlp", [&] {
       return K.mlb_moe_few(out.data_ptr(), e.x.data_ptr(), e.weights.data_ptr(), (const int*)e.idx.data_ptr(), e.gate_up.data_ptr(), e.down.data_ptr(), (float*)w.part.data_ptr(),
-                           (int*)w.count.data_ptr(), N, row_step(e.x), k, E, (int)C, (int)I, bits(e.weights), st);
+                           N, row_step(e.x), k, E, (int)C, (int)I, bits(e.weights), st);
     });
   }
   {

@@ -50,7 +50,7 @@ _GEN_KINDS = {
 _MOE_KINDS = {
     "moe_route_part": "ln", "moe_route": "biffbfllnnnnnndnns", "moe_route_bwd": "bbfbillnnnndnns", "moe_plan_ints": "lnn", "moe_plan_rows": "lnn", "moe_plan": "iilnns",
     "moe_fwd": "bbbbbbbbbillnnnnns", "moe_bwd": "bbbbbbbbbbbbbbbillnnnnns",
-    "moe_few_floats": "lnnnn", "moe_few": "bbbibbfillnnnnns"}
+    "moe_few_floats": "lnnnn", "moe_few": "bbbibbfllnnnnns"}
 _CTYPES = {"n": _i32, "l": _i64, "d": _f32}      # (else a pointer)
 
 

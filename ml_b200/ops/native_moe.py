@@ -116,8 +116,8 @@ def _fwd(out, x, weights, idx, gate_up, down, keep):
     e = _n._entries()
     few = 0 if keep else e.mlb_moe_few_floats(N, k, E, C, I)
     if few:
-        part, count = _n.scratch("moe_few", few, F32, x.device), _n.scratch("moe_count", C // 16, I32, x.device, zero=True)
-        _took(e.mlb_moe_few(out, _at(x), _at(weights), idx, gate_up, down, part, count, N, ldx, k, E, C, I, _bits(weights)), "moe_mlp")
+        part = _n.scratch("moe_few", few, F32, x.device)
+        _took(e.mlb_moe_few(out, _at(x), _at(weights), idx, gate_up, down, part, N, ldx, k, E, C, I, _bits(weights)), "moe_mlp")
         return None
     plan, R = _plan(idx, E)
     new = lambda c: torch.empty(R, c, dtype=BF16, device=x.device)

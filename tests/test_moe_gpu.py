@@ -266,7 +266,7 @@ def test_experts_of_many_copies(N, E, k):
     close((out, *grads), oracle.mlp_grads(dout, x, w, idx, gate_up, down), oracle.mlp_sizes(dout, x, w, idx, gate_up, down))
 
 
-@pytest.mark.parametrize("N,E,k", [(8, 3, 3), (16, 4, 8), (30, 2, 8), (5, 2, 32)])
+@pytest.mark.parametrize("N,E,k", [(8, 3, 3), (6, 4, 8), (8, 2, 20), (8, 1, 32)])
 def test_few_tokens_with_an_expert_many_times(N, E, k):
     x, w, idx, gate_up, down = experts(N, max(E, k), k, 96, 48, F32)
     idx.copy_(torch.randint(-1, E, idx.shape, generator=torch.Generator().manual_seed(N), dtype=I32))
@@ -275,10 +275,10 @@ def test_few_tokens_with_an_expert_many_times(N, E, k):
     close([out], [oracle.mlp(x.double(), w.double(), idx, gate_up.double(), down.double())], oracle.mlp_sizes(out, x, w, idx, gate_up, down))
 
 
-@pytest.mark.parametrize("N", [1, 7, 8, 9, 16, 17, 31, 32, 33])
-@pytest.mark.parametrize("C,I,E,k", [(16, 16, 4, 2), (80, 528, 12, 3), (1040, 96, 6, 1), (2048, 1376, 16, 6)])
+@pytest.mark.parametrize("N", [1, 2, 7, 8, 9, 33])
+@pytest.mark.parametrize("C,I,E,k", [(16, 16, 4, 2), (80, 528, 12, 3), (1040, 96, 6, 1), (2048, 1376, 16, 6), (256, 2816, 2, 2)])
 def test_few_tokens(N, C, I, E, k):
-    """The form for few tokens, and the first number of tokens for the other one: sizes that end inside an instruction's and a thread block's share, all of them twice (counters)."""
+    """The form for few tokens, and the first number of tokens for the other one: sizes that end inside a stage, a warp's and a thread block's share, and leave some without any."""
     x, w, idx, gate_up, down = experts(N, E, k, C, I, F32, drop=N // 4)
     want, sizes = [oracle.mlp(x.double(), w.double(), idx, gate_up.double(), down.double())], oracle.mlp_sizes(x, x, w, idx, gate_up, down)
     for _ in range(2):
