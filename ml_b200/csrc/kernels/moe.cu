@@ -24,13 +24,16 @@ struct PlanShape {
   long rows, tiles, place, source, hist, total;      // R; offsets of the parts in ints
   int max_tiles, blocks, per_block;
 };
-constexpr int PLAN_THREADS = 256, PLAN_WARPS = PLAN_THREADS / 32;
+// PLAN_BATCH: copies that a lane asks for at a time.  A block that has all copies to itself has 32 warps, whose copies go to their rows 32 at a time, one behind the other (1806 copies to 64
+// experts: 10.4 us with 8 warps, 8.7 with 32); where there are several, or more lists of counts than shared memory takes, it has 8 (16384 copies to 8 experts: 5.3 us, 6.4 with 32).
+constexpr int PLAN_BATCH = 8;
+inline int plan_warps(int E, int blocks) { return E <= 256 && blocks == 1 ? 32 : 8; }
 inline PlanShape plan_shape(long NK, int E) {
   PlanShape p;
   const long used = NK < E ? NK : E;
   p.rows = (NK + (PAD - 1) * used) / PAD * PAD;
   p.max_tiles = (int)(NK / TILE_TOKENS + used);
-  p.per_block = NK <= 4096 ? 4096 : (int)std::max(1024L, ((NK + 127) / 128 + PLAN_THREADS - 1) / PLAN_THREADS * PLAN_THREADS);
+  p.per_block = NK <= 2048 ? 2048 : (int)std::max(1024L, ((NK + 127) / 128 + 1023) / 1024 * 1024);
   p.blocks = (int)((NK + p.per_block - 1) / p.per_block);
   p.tiles = (2L * E + 2 + 3) / 4 * 4;
   p.place = p.tiles + 4L * p.max_tiles;
@@ -57,38 +60,42 @@ __device__ __forceinline__ int expert_of(const PlanArgs& A, long i) {
   }
   return e;
 }
-__global__ void __launch_bounds__(PLAN_THREADS) moe_hist_k(const PlanArgs A) {
+__global__ void __launch_bounds__(256) moe_hist_k(const PlanArgs A) {
   mlb_pdl_sync();
   extern __shared__ int cnt[];
-  for (int e = threadIdx.x; e < A.E; e += PLAN_THREADS) cnt[e] = 0;
+  for (int e = threadIdx.x; e < A.E; e += (int)blockDim.x) cnt[e] = 0;
   __syncthreads();
   const long i0 = (long)blockIdx.x * A.per_block;
-  for (int i = threadIdx.x; i < A.per_block; i += PLAN_THREADS) {
+  for (int i = threadIdx.x; i < A.per_block; i += (int)blockDim.x) {
     const int e = expert_of(A, i0 + i);
     if (e >= 0) atomicAdd(&cnt[e], 1);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < A.E; e += PLAN_THREADS) A.hist[(long)blockIdx.x * A.E + e] = cnt[e];
+  for (int e = threadIdx.x; e < A.E; e += (int)blockDim.x) A.hist[(long)blockIdx.x * A.E + e] = cnt[e];
 }
 // Every block adds up all blocks' counts for itself and puts its copies behind those of the blocks before it, in order: the same rows on every run.
-__global__ void __launch_bounds__(PLAN_THREADS) moe_place_k(const PlanArgs A) {
+__global__ void __launch_bounds__(1024) moe_place_k(const PlanArgs A) {
   mlb_pdl_sync();
   extern __shared__ int sm[];
-  const int E = A.E, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  int *total = sm, *base = sm + E, *mine = sm + 2 * E;      // mine[PLAN_WARPS][E]
-  __shared__ int2 warps[PLAN_WARPS];
-  for (int e = tid; e < (2 + PLAN_WARPS) * E; e += PLAN_THREADS) sm[e] = 0;
+  const int E = A.E, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, threads = blockDim.x, nw = threads >> 5;
+  int *total = sm, *base = sm + E, *mine = sm + 2 * E;      // mine[nw][E]
+  __shared__ int2 warps[32];
+  for (int e = tid; e < (2 + nw) * E; e += (int)blockDim.x) sm[e] = 0;
   __syncthreads();
   // the copies of this block, a run of them to each warp
-  const int run = A.per_block / PLAN_WARPS;
+  const int run = A.per_block / nw;
   const long i0 = (long)blockIdx.x * A.per_block + (long)w * run;
-  for (int i = lane; i < run; i += 32) {
-    const int e = expert_of(A, i0 + i);
-    if (e >= 0) atomicAdd(&mine[w * E + e], 1);
+  for (int i = lane; i < run; i += 32 * PLAN_BATCH) {
+    int e[PLAN_BATCH];
+#pragma unroll
+    for (int j = 0; j < PLAN_BATCH; j++) e[j] = i + 32 * j < run ? expert_of(A, i0 + i + 32 * j) : -1;
+#pragma unroll
+    for (int j = 0; j < PLAN_BATCH; j++)
+      if (e[j] >= 0) atomicAdd(&mine[w * E + e[j]], 1);
   }
   if (A.blocks > 1) {
-    if (E >= PLAN_THREADS / 2) {
-      for (int e = tid; e < E; e += PLAN_THREADS) {
+    if (E >= 128) {
+      for (int e = tid; e < E; e += (int)blockDim.x) {
         int all = 0, before = 0;
 #pragma unroll 8
         for (int b = 0; b < A.blocks; b++) {
@@ -101,7 +108,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_place_k(const PlanArgs A) {
     } else {
       const int n = A.blocks * E;
 #pragma unroll 4
-      for (int i = tid; i < n; i += PLAN_THREADS) {
+      for (int i = tid; i < n; i += (int)blockDim.x) {
         const int v = A.hist[i], b = i / E, e = i - b * E;
         if (v) {
           atomicAdd(&total[e], v);
@@ -112,15 +119,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_place_k(const PlanArgs A) {
   }
   __syncthreads();
   if (A.blocks == 1) {
-    for (int e = tid; e < E; e += PLAN_THREADS) {
+    for (int e = tid; e < E; e += (int)blockDim.x) {
       int all = 0;
-      for (int k = 0; k < PLAN_WARPS; k++) all += mine[k * E + e];
+      for (int k = 0; k < nw; k++) all += mine[k * E + e];
       total[e] = all;
     }
     __syncthreads();
   }
   // rows and tiles of the experts before each (a thread has `per` experts, one behind the other)
-  const int per = (E + PLAN_THREADS - 1) / PLAN_THREADS, e0 = tid * per, e1 = min(e0 + per, E);
+  const int per = (E + threads - 1) / threads, e0 = tid * per, e1 = min(e0 + per, E);
   int2 own = make_int2(0, 0);
   for (int e = e0; e < e1; e++) {
     own.x += (total[e] + PAD - 1) / PAD * PAD;
@@ -148,29 +155,37 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_place_k(const PlanArgs A) {
       for (int t = n; t < padded; t++) A.source[row + t] = -1;
     }
     int at = row + base[e];
-    for (int k = 0; k < PLAN_WARPS; k++) {
+    for (int k = 0; k < nw; k++) {
       const int v = mine[k * E + e];
       mine[k * E + e] = at;
       at += v;
     }
     row += padded;
   }
-  if (writes && tid == PLAN_THREADS - 1) A.start[E] = sum.x, *A.ntiles = sum.y;
+  if (writes && tid == threads - 1) A.start[E] = sum.x, *A.ntiles = sum.y;
   __syncthreads();
-  for (int i = lane; i < run; i += 32) {      // (run is a multiple of 32)
-    const int e = expert_of(A, i0 + i);
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int first = e >= 0 ? mine[w * E + e] : 0;
-    __syncwarp();
-    const int rank = __popc(same & ((1u << lane) - 1));
-    if (e >= 0) {
-      if (rank == 0) mine[w * E + e] = first + __popc(same);
-      A.place[i0 + i] = first + rank;
-      A.source[first + rank] = (int)(i0 + i);
-    } else if (i0 + i < A.NK) {
-      A.place[i0 + i] = -1;
+  for (int i = lane; i < run; i += 32 * PLAN_BATCH) {      // (run is a multiple of 32)
+    int es[PLAN_BATCH];
+#pragma unroll
+    for (int j = 0; j < PLAN_BATCH; j++) es[j] = i + 32 * j < run ? expert_of(A, i0 + i + 32 * j) : -1;
+#pragma unroll
+    for (int j = 0; j < PLAN_BATCH; j++) {
+      if (i - lane + 32 * j >= run) break;      // (the warp's)
+      const long at = i0 + i + 32 * j;
+      const int e = es[j];
+      const unsigned same = __match_any_sync(0xffffffffu, e);
+      const int first = e >= 0 ? mine[w * E + e] : 0;
+      __syncwarp();
+      const int rank = __popc(same & ((1u << lane) - 1));
+      if (e >= 0) {
+        if (rank == 0) mine[w * E + e] = first + __popc(same);
+        A.place[at] = first + rank;
+        A.source[first + rank] = (int)at;
+      } else if (at < A.NK) {
+        A.place[at] = -1;
+      }
+      __syncwarp();
     }
-    __syncwarp();
   }
 }
 
@@ -801,7 +816,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_k(const __grid_constan
 #pragma unroll
     for (int x = 0; x < 2 * FEW_BOXES; x++) {
       const int k = (s * FEW_BOXES + x / 2) * 64 + x % 2 * 32 + t * 8;
-      ahead[x / 2][x % 2] = k < K ? __ldg(reinterpret_cast<const uint4*>(col + k)) : make_uint4(0, 0, 0, 0);
+      ahead[x / 2][x % 2] = k < K ? *reinterpret_cast<const uint4*>(col + k) : make_uint4(0, 0, 0, 0);
     }
   };
   if (begin < units && part_of < steps) tokens(begin, part_of);
@@ -977,8 +992,8 @@ MLB_API int mlb_moe_plan(int* plan, const int* idx, long N, int k, int E, cudaSt
   if (off16({plan})) return -7;
   if (z.NK == 0) return 0;
   const PlanArgs P = plan_args(plan, idx, z);
-  if (z.p.blocks > 1) MLB_TRY((int)mlb_launch(moe_hist_k, dim3(z.p.blocks), dim3(PLAN_THREADS), (size_t)4 * E, st, P));
-  return (int)mlb_launch(moe_place_k, dim3(z.p.blocks), dim3(PLAN_THREADS), (size_t)4 * E * (2 + PLAN_WARPS), st, P);
+  if (z.p.blocks > 1) MLB_TRY((int)mlb_launch(moe_hist_k, dim3(z.p.blocks), dim3(256), (size_t)4 * E, st, P));
+  return (int)mlb_launch(moe_place_k, dim3(z.p.blocks), dim3(32 * plan_warps(E, z.p.blocks)), (size_t)4 * E * (2 + plan_warps(E, z.p.blocks)), st, P);
 }
 // xs [R, C], gu [R, 2 I] (null: not kept), h [R, I] and y [R, C] are workspace, and what backward needs
 MLB_API int mlb_moe_fwd(void* out, void* xs, void* gu, void* h, void* y, const void* x, const void* weights, const void* gate_up, const void* down, const int* plan, long N, long ldx, int k,

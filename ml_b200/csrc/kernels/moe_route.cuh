@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
       for (int v = 0; v < V; v++) {
         const int i = v * 32 + lane;
         const float b = i < E && A.bias != nullptr ? __ldg(A.bias + i) : 0.f, s = e[v] * inv;
-        t[v] = z[v] == -INFINITY ? -INFINITY : s + b;
+        t[v] = z[v] == -INFINITY ? -INFINITY : fmaxf(s + b, -INFINITY);      // (NaN, of a bias: not there)
         if (z[v] > -INFINITY) size = fmaxf(size, s + fabsf(b));
       }
       const float slack = 4.7683716e-7f * __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size)));

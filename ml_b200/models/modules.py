@@ -50,9 +50,9 @@ class Block(nn.Module):
         a = F.rope_causal_attention(qkv, cos, sin, B, c.T, c.H, c.hd, self.Hkv)
         x = x + F.linear(a, self.o)
         h = F.rmsnorm(x, self.ln2, c.eps)
-        if self.moe is not None:
-            y, self.aux = self.moe(h)
-            return x + y
+        if self.moe is not None:      # (the balancing loss is handed on, not kept: a graph that outlives its step stands in the way of capturing the next)
+            y, aux = self.moe(h)
+            return x + y, aux
         return x + F.linear(F.swiglu(F.linear(h, self.gate_up)), self.down)
 
 
@@ -101,12 +101,14 @@ class Decoder(nn.Module):
         c = self.cfg
         B = ids.numel() // c.T
         x = F.embedding(self.wte, ids.view(-1), c.T)
+        aux = 0.0
         for b in self.blocks:
             x = b(x, self.cos, self.sin, B)
+            if b.moe is not None:
+                x, more = x
+                aux = aux + more
         logits = F.linear(F.rmsnorm(x, self.lnf, c.eps), self.lm)
         if tgt is None:
             return logits
         loss = F.cross_entropy(logits, tgt.view(-1))
-        if self.blocks[0].moe is not None:
-            loss = loss + self.aux_coef * sum(b.aux for b in self.blocks)
-        return loss
+        return loss if self.blocks[0].moe is None else loss + self.aux_coef * aux

@@ -3,7 +3,7 @@
 Signatures and checks are those of `ops.native_moe`; what CPU tensors get and what the kernels are compared with.  (The reference's prototype has a softmax router and
 expert kernels that nothing calls, csrc/kernels/moe_kernels.cu:18-194.)
 
-Routing.  A logit of NaN counts as -inf, and an expert at -inf is not there.  Scores s are a softmax over the experts or a sigmoid each.  A token's k experts are those of
+Routing.  A logit of NaN counts as -inf, and an expert at -inf, or with a bias of NaN or -inf, is not there for the choice.  Scores s are a softmax over the experts or a sigmoid each.  A token's k experts are those of
 the largest logits, or, with `bias` (fp32 [E]; for the choice only) or groups, of the largest s + bias in 64 bits; equal ones go to the lowest index.  Of `groups` equal
 groups of neighbouring experts the `top_groups` best stay, by the sum of their two best s + bias.  Weights are scale * s, with `renorm` scale * s / (sum of the chosen
 experts' s).  Where fewer than k experts are left, the index is -1 and the weight 0.  `mean` is the mean over all tokens of softmax(z), or of s / (sum of s).
@@ -148,7 +148,7 @@ def moe_route(weights, idx, mean, logits, bias=None, score="softmax", groups=1, 
     else:
         zd = _seen(logits, torch.float64)
         t = _scores(zd, score) + (0.0 if bias is None else bias.double())
-        t = torch.where(zd > NEG, t, NEG)
+        t = torch.where((zd > NEG) & ~torch.isnan(t), t, NEG)
     if groups > 1:
         parts = t.view(N, groups, -1)
         two = parts.sort(dim=2, descending=True).values[..., :2]

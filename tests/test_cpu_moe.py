@@ -38,6 +38,20 @@ def test_plain_routing(N, E, k, groups, top, score, renorm, biased):
     assert torch.allclose(dz.double(), torch.nan_to_num(ez), atol=2e-6, rtol=1e-5)
 
 
+@pytest.mark.parametrize("groups", [1, 4])
+def test_bias_that_is_no_number(groups):
+    z = torch.randn(6, 64, generator=torch.Generator().manual_seed(1))
+    bias = torch.zeros(64)
+    bias[3], bias[40], bias[50], bias[20] = math.nan, -math.inf, math.inf, math.inf
+    w, idx = torch.empty(6, 4), torch.empty(6, 4, dtype=I32)
+    ops.moe_route(w, idx, None, z, bias, "sigmoid", groups, groups, False)
+    free = torch.sigmoid(z.double())
+    free[:, [3, 40]] = -1
+    free[:, [20, 50]] = 2
+    at = free.sort(dim=1, descending=True, stable=True).indices[:, :4]
+    assert torch.equal(idx.long(), at) and torch.allclose(w, torch.sigmoid(z).gather(1, at), rtol=1e-5)
+
+
 def test_routing_gradient_against_differences():
     torch.manual_seed(3)
     for score in ("softmax", "sigmoid"):

@@ -171,6 +171,20 @@ def test_gradient_of_routing_of_one_output():
         assert torch.allclose(dz.cpu().double(), ez, atol=1e-6, rtol=1e-5)
 
 
+@pytest.mark.parametrize("groups", [1, 4])
+def test_bias_that_is_no_number(groups):
+    z = torch.randn(6, 64, generator=torch.Generator().manual_seed(1)).to(dev())
+    bias = torch.zeros(64, device=dev())
+    bias[3], bias[40], bias[50], bias[20] = math.nan, -math.inf, math.inf, math.inf
+    w, idx = torch.empty(6, 4, device=dev()), torch.empty(6, 4, dtype=I32, device=dev())
+    ops.moe_route(w, idx, None, z, bias, "sigmoid", groups, groups, False)
+    free = torch.sigmoid(z.double())
+    free[:, [3, 40]] = -1
+    free[:, [20, 50]] = 2
+    at = free.sort(dim=1, descending=True, stable=True).indices[:, :4]
+    assert torch.equal(idx.long(), at) and torch.allclose(w, torch.sigmoid(z).gather(1, at), rtol=1e-5)
+
+
 def test_routing_of_no_tokens():
     w, idx, mean = routed(torch.empty(0, 8), 2)
     assert w.shape == (0, 2) and mean.abs().sum() == 0
@@ -467,3 +481,74 @@ def test_entry_points_are_called_alike_through_python_and_the_extension_module(m
         monkeypatch.setattr(n, "_E", entries)
         outs.append(work())
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+# ------------------------------------------------------------------ together
+@pytest.mark.parametrize("how", [dict(), dict(score="sigmoid", balanced=True, groups=4, top_groups=2, scale=2.5), dict(renorm=False)])
+@pytest.mark.parametrize("N", [1, 5, 300])
+def test_block_of_experts(how, N):
+    """Router, experts and balancing loss together, forward and backward, against the definitions with the logits and weights that the block has."""
+    from ml_b200.models.moe import MoE
+    torch.manual_seed(N)
+    m = MoE(128, 96, 8, 2, device=dev(), dtype=BF16, std=0.1, **how)
+    if m.bias is not None:
+        m.bias.normal_(std=0.05)
+    x = torch.randn(N, 128, device=dev()).to(BF16).requires_grad_()
+    y, aux = m(x)
+    dout = torch.randn(N, 128, device=dev()).to(BF16)
+    grads = torch.autograd.grad([y, aux], [x, m.gate_up, m.down, m.router], [dout, torch.ones_like(aux)])
+    z = (x.detach() @ m.router.detach().T)      # what the block's product gives, to a rounding: the choice is compared where it is clear
+    logits = F.linear(x.detach(), m.router.detach())
+    assert torch.allclose(z.float(), logits.float(), atol=0.05, rtol=0.02)
+    kw = {k: v for k, v in m.how.items()}
+    zd = logits.double().cpu().requires_grad_()
+    w, idx, mean = oracle.route(zd, 2, None if m.bias is None else m.bias.cpu(), **kw)
+    wb = w.detach().to(BF16).to(dev())
+    want, sizes = (f(dout, x, wb, idx.to(dev()), m.gate_up, m.down) for f in (oracle.mlp_grads, oracle.mlp_sizes))
+    close([y, grads[1], grads[2]], want, sizes, ["out", "dgate_up", "ddown"])
+    load = torch.bincount(idx[idx >= 0].long().flatten(), minlength=8).double()
+    assert torch.equal(m.load.cpu().double(), load)
+    want_aux = float(8 * (mean.detach() * load).sum() / idx.numel())
+    assert abs(float(aux.detach()) - want_aux) < 1e-4 * max(1.0, want_aux)
+    # the router: the weights' and the loss's gradients through the logits, rounded to bf16 on their way (5 roundings: weights', logits', a product's each)
+    back = 8 * (mean * load).sum() / idx.numel()
+    dz, = torch.autograd.grad([w, back], zd, [want[2].cpu(), torch.ones_like(back)])
+    dr = dz.T @ x.detach().double().cpu()
+    assert float((grads[3].double().cpu() - dr).norm()) <= 8 * HALF[BF16] * float(dr.norm()) + 1e-6
+    m.eval()
+    with torch.no_grad():
+        served, _ = m(x.detach())
+    close([served], want[:1], sizes, ["out"])
+
+
+def test_decoder_with_experts_trains_and_is_captured():
+    from ml_b200 import Config
+    from ml_b200.models.modules import Decoder
+    cfg = Config(V=512, C=128, L=2, H=2, I=192, T=64)
+    torch.manual_seed(0)
+    m = Decoder(cfg, device="cuda:0", experts=dict(n_experts=8, top_k=2, std=0.05))
+    for n, p in m.named_parameters():
+        if "moe" not in n:
+            torch.nn.init.normal_(p, std=0.05)
+    ids = torch.randint(0, 512, (2, 64), dtype=I32, device=dev())
+    tgt = torch.roll(ids, -1).contiguous()
+    ps = list(m.parameters())
+
+    def step():
+        loss = m(ids, tgt)
+        return [loss.detach(), *torch.autograd.grad(loss, ps)]
+
+    first = step()
+    assert all(bool(torch.isfinite(t).all()) for t in first) and all(float(t.float().abs().sum()) > 0 for t in first)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    for (n, _), a, b in zip([("loss", None), *m.named_parameters()], first, got):      # (products whose sums are split add up in the order of arrival: equal to a rounding)
+        assert torch.allclose(a.float(), b.float(), atol=2e-2 * float(a.float().abs().max()), rtol=2e-2), n
