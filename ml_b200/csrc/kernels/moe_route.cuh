@@ -3,6 +3,8 @@
 // A warp has a token, lane l the experts l, l + 32, ...  A logit of NaN counts as -inf and an expert at -inf is not there.  Scores are a softmax over the experts or a
 // sigmoid each.  Experts are chosen by their logits, or, with a bias or groups, by score + bias in 64 bits: in 32 the last bits of two roundings would decide between
 // neighbours, and another way of adding up would choose other experts.  Equal ones go to the lowest index.
+// Bound by instructions: 8192 tokens to 8 of 256 experts 7.8 us by logits (700 a token; 1.3 for the bytes), 17.3 with a bias and 4 of 8 groups (1550; with 64 bits for
+// every expert 31.0, with them for the candidates and two experts of each group 21.5); 16 tokens 3.1 and 5.6, of which a launch is 2.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -11,7 +13,7 @@
 
 namespace {
 
-constexpr int ROUTE_WARPS = 8, MAX_E = 1024, MAX_K = 32, MAX_GROUPS = 32;      // (ops/ref_moe.py refuses more)
+constexpr int ROUTE_WARPS = 8, MAX_E = 1024, MAX_K = 32, MAX_GROUPS = 32, LIST = 34;      // (ops/ref_moe.py refuses more)
 struct RouteArgs {
   const void* logits;
   const float* bias;
@@ -22,11 +24,12 @@ struct RouteArgs {
   int E, k, groups, top, sigmoid, renorm, wide_w;
   float scale;
 };
+__host__ __device__ constexpr int own_doubles(int E) { return E > 32 ? E : 32; }      // a warp's shared memory where the choice is not by logits: numbers of the experts, or of candidates
 template <typename T> __device__ __forceinline__ float logit(const T* z, int i);
 template <> __device__ __forceinline__ float logit<float>(const float* z, int i) { return __ldg(z + i); }
 template <> __device__ __forceinline__ float logit<bf16>(const bf16* z, int i) { return __bfloat162float(z[i]); }
 // (NaN -> -inf, -0 -> 0)
-__device__ __forceinline__ float seen(float z) { return z != z ? -INFINITY : z + 0.f; }
+__device__ __forceinline__ float seen(float z) { return fmaxf(z, -INFINITY) + 0.f; }
 // exp(x) for x <= 0 to a few 2^-24: the product with log2 e in two parts
 __device__ __forceinline__ float exp_fine(float x) {
   const float hi = x * 1.44269504f, lo = fmaf(x, 1.44269504f, -hi) + x * 1.92596299e-8f;
@@ -39,6 +42,13 @@ __device__ __forceinline__ float exp_from(float a, float b) { return a == b ? 1.
 __device__ __forceinline__ float sigmoid_fine(float z) {
   const float e = exp_fine(fmaxf(-fabsf(z), -200.f));
   return __fdividef(z >= 0.f ? 1.f : e, 1.f + e);      // (2 steps of 2^-23; the denominator is 1 to 2)
+}
+// The same to 2^-21 or so of itself (2 steps of ex2, 1 of rcp, and the product's rounding, which matters where the score is small), 0 for -inf: says what may be chosen
+__device__ __forceinline__ float sigmoid_fast(float z) {
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+  return s;
 }
 // sigmoid(z) / exp(top) for top = min(0, largest z): scores for shares, whose sum is not too small for fp32
 __device__ __forceinline__ float sigmoid_from(float z, float top) {
@@ -94,7 +104,7 @@ __device__ __forceinline__ int choose(uint32_t (&key)[V], int k, int lane) {
 
 // What may be chosen of many keys a lane.  A bound that k + 1 lanes' best keys or a few more reach is no better than the k + 1-th best key, so what is chosen, and what comes
 // behind it, is among the keys that reach it (or, with `below`, come near it): usually some more than k.  They are put side by side, a lane each.  Returns how many;
-// over 32 (many equal ones): the list is not complete.  8192 tokens, 8 of 256 experts, by logits: 13.3 us with the bound out of a sort of the lanes' best, 9.2 so.
+// over 32 (many equal ones): the list is not complete.  8192 tokens, 8 of 256 experts, by logits: 13.3 us with the bound out of a sort of the lanes' best, 7.8 so.
 template <int V>
 __device__ __forceinline__ int candidates(const uint32_t (&key)[V], int k, int lane, uint2* s, float below) {
   uint32_t best = key[0];
@@ -117,10 +127,7 @@ __device__ __forceinline__ int candidates(const uint32_t (&key)[V], int k, int l
   for (int v = 0; v < V; v++) {
     const bool here = key[v] >= least;
     const unsigned all = __ballot_sync(0xffffffffu, here);
-    if (here) {
-      const int at = count + __popc(all & ((1u << lane) - 1));
-      if (at < 32) s[at] = make_uint2(key[v], v * 32 + lane);
-    }
+    s[here ? min(count + __popc(all & ((1u << lane) - 1)), 32) : 32] = make_uint2(key[v], v * 32 + lane);      // (place 32: for those that are none)
     count += __popc(all);
   }
   __syncwarp();
@@ -144,51 +151,47 @@ __device__ __forceinline__ int choose_many(uint32_t (&key)[V], int k, int lane, 
   return lane < k && lane < count ? (int)s[lane].y : -1;
 }
 
-// Groups: the experts' choice numbers t stand in s[E].  As many lanes as go into 32 share a group.  Lane l gets group l's three best numbers, and the indices of the first two.
-struct Best { float a, b, c; int ai, bi; };
+// Groups: the experts' choice numbers t stand in s[E].  As many lanes as go into 32 share a group.  Lane l gets group l's three best numbers.
+struct Best { float a, b, c; };
 __device__ __forceinline__ Best best_of_groups(const float* s, int size, int groups, int lane) {
-  int share = 32;
-  while (share * groups > 32) share >>= 1;
-  const int g = lane / share, sub = lane % share, steps = (size + share - 1) / share;
-  Best r = {-INFINITY, -INFINITY, -INFINITY, 0, 0};
+  const int bits = groups > 1 ? 32 - __clz(groups - 1) : 0, shift = 5 - bits, share = 1 << shift;
+  const int g = lane >> shift, sub = lane & (share - 1), steps = (size + share - 1) >> shift;
+  Best r = {-INFINITY, -INFINITY, -INFINITY};
   if (g < groups)
-    for (int j = 0, x = g % steps; j < steps; j++, x = x + 1 == steps ? 0 : x + 1) {      // (begun at another place by each group: other banks)
+    for (int j = 0, x = (g * steps) >> bits; j < steps; j++, x = x + 1 == steps ? 0 : x + 1) {      // (begun at another place by each group: other banks)
       const int i = x * share + sub;
       const float t = i < size ? s[g * size + i] : -INFINITY;
-      if (t > r.b) {
-        r.c = r.b;
-        if (t > r.a) r.b = r.a, r.bi = r.ai, r.a = t, r.ai = g * size + i;
-        else r.b = t, r.bi = g * size + i;
-      } else {
-        r.c = fmaxf(r.c, t);
-      }
+      r.c = fmaxf(r.c, fminf(r.b, t));
+      r.b = fmaxf(r.b, fminf(r.a, t));
+      r.a = fmaxf(r.a, t);
     }
   for (int o = 1; o < share; o <<= 1) {
     const float x = __shfl_xor_sync(0xffffffffu, r.a, o), y = __shfl_xor_sync(0xffffffffu, r.b, o), z = __shfl_xor_sync(0xffffffffu, r.c, o);
-    const int xi = __shfl_xor_sync(0xffffffffu, r.ai, o), yi = __shfl_xor_sync(0xffffffffu, r.bi, o);
     const float low = fminf(r.a, x), mid = fmaxf(r.b, y);      // the second best of all is one of these, and the third the other one or a third
-    const int li = r.a < x ? r.ai : xi, mi = r.b < y ? yi : r.bi;
-    if (r.a < x) r.a = x, r.ai = xi;
+    r.a = fmaxf(r.a, x);
     r.c = fmaxf(fminf(low, mid), fmaxf(r.c, z));
     r.b = fmaxf(low, mid);
-    r.bi = low < mid ? mi : li;
   }
-  const int from = (lane * share) & 31;
-  return {__shfl_sync(0xffffffffu, r.a, from), __shfl_sync(0xffffffffu, r.b, from), __shfl_sync(0xffffffffu, r.c, from), __shfl_sync(0xffffffffu, r.ai, from),
-          __shfl_sync(0xffffffffu, r.bi, from)};
+  const int from = (lane << shift) & 31;
+  return {__shfl_sync(0xffffffffu, r.a, from), __shfl_sync(0xffffffffu, r.b, from), __shfl_sync(0xffffffffu, r.c, from)};
 }
 // The bits of the groups that stay, by the sums of their two best (lane l: of group l); `margin`: by how much the worst of them is ahead of the best of the others
-__device__ __forceinline__ unsigned keep_groups(double sum, int groups, int top, int lane, double& margin) {
-  uint64_t key = lane < groups ? order64(sum) : 0;
+__device__ __forceinline__ uint32_t order(float v) { return order32(v); }
+__device__ __forceinline__ uint64_t order(double v) { return order64(v); }
+__device__ __forceinline__ float value_of(uint64_t key) { return (float)value64(key); }
+template <typename R>
+__device__ __forceinline__ unsigned keep_groups(R sum, int groups, int top, int lane, float& margin) {
+  auto key = lane < groups ? order(sum) : 0;
+  auto low = key;
   unsigned stays = 0;
   for (int j = 0; j < top; j++) {
-    const uint64_t best = warp_best(key);
-    const int g = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
+    low = warp_best(key);
+    const int g = __ffs(__ballot_sync(0xffffffffu, key == low)) - 1;
     stays |= 1u << g;
     if (lane == g) key = 0;
   }
-  const uint64_t low = ~warp_best((stays >> lane) & 1 ? ~order64(sum) : 0), high = warp_best(key);
-  margin = high <= GONE64 ? INFINITY : value64(low) - value64(high);
+  const auto high = warp_best(key);
+  margin = high == 0 ? INFINITY : value_of(low) - value_of(high);
   return stays;
 }
 
@@ -219,7 +222,8 @@ __device__ __noinline__ int choose_exact(const RouteArgs& A, const T* row, doubl
   unsigned stays = 0xffffffffu;
   const int size = E / A.groups;
   if (A.groups > 1) {
-    double a = -INFINITY, b = -INFINITY, margin;
+    double a = -INFINITY, b = -INFINITY;
+    float margin;
 #pragma unroll 1
     for (int i = 0; lane < A.groups && i < size; i++) {
       const double t = s[lane * size + i];
@@ -248,8 +252,9 @@ __device__ __noinline__ int choose_exact(const RouteArgs& A, const T* row, doubl
 }
 
 // An expert's number in 64 bits where that is the expert's own affair: sigmoids; a softmax without bias over its common factor
+// (one function: every token asks for it, so its code is at hand for the few that do so for groups, too)
 template <typename T>
-__device__ __forceinline__ double own_number(const RouteArgs& A, const T* row, int i, float m) {
+__device__ __noinline__ double own_number(const RouteArgs& A, const T* row, int i, float m) {
   const double z = (double)seen(logit(row, i)), x = exp(A.sigmoid ? -z : z - (double)m);
   return A.sigmoid ? 1.0 / (1.0 + x) + (A.bias != nullptr ? (double)__ldg(A.bias + i) : 0.0) : x;
 }
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
   extern __shared__ double route_sm[];      // not PLAIN: the scores of each warp's token; lists of candidates; behind the loop: sums of probabilities
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, E = A.E;
   const uint32_t magic = 0xffffffffu / (uint32_t)(E / A.groups) + 1;      // (0, and not used so, where a group is one expert)
-  uint2* list = (uint2*)(route_sm + (PLAIN ? 0 : ROUTE_WARPS * E)) + 32 * w;
+  uint2* list = (uint2*)(route_sm + (PLAIN ? 0 : ROUTE_WARPS * own_doubles(E))) + LIST * w;
   float sum_p[V];
 #pragma unroll
   for (int v = 0; v < V; v++) sum_p[v] = 0.f;
@@ -280,7 +285,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
     if (sums || !PLAIN) {
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        e[v] = z[v] == -INFINITY ? 0.f : A.sigmoid ? sigmoid_fine(z[v]) : exp_from(z[v], m);
+        e[v] = A.sigmoid ? sigmoid_fast(z[v]) : z[v] == -INFINITY ? 0.f : exp_from(z[v], m);
         total += e[v];
       }
       if (sums) total = warp_sum(total);
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
 #pragma unroll
         for (int v = 0; v < V; v++) x[v] = e[v];
       }
-      const float inv = all > 0.f ? __fdiv_rn(1.f, all) : 0.f;
+      const float inv = all > 0.f ? __fdividef(1.f, all) : 0.f;
 #pragma unroll
       for (int v = 0; v < V; v++) sum_p[v] = fmaf(x[v], inv, sum_p[v]);
     }
@@ -308,10 +313,10 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
       if constexpr (V >= 4) mine = choose_many<V>(key, A.k, lane, list);
       else mine = choose<V>(key, A.k, lane);
     } else {
-      // 32 bits say what may be chosen, 64 bits what is.  In 32 a score is off by less than 2^-22 of itself (6 roundings, and a sum's), score + bias by less than slack = 2^-21 of the
-      // row's largest score + |bias|.  (With 64 bits for the few tokens alone that 32 leave open, these wait some 10 us for code that no cache has.)
+      // 32 bits say what may be chosen, 64 bits what is.  In 32 a score is off by less than 2^-21 of itself, or of 1/4 where it is smaller, score + bias by less than slack = 2^-20 of
+      // the row's largest score + |bias|.  (With 64 bits for the few tokens alone that 32 leave open, these wait some 10 us for code that no cache has.)
       float t[V], size = 0.f;
-      const float inv = A.sigmoid || A.bias == nullptr ? 1.f : total > 0.f ? __fdiv_rn(1.f, total) : 0.f;
+      const float inv = A.sigmoid || A.bias == nullptr ? 1.f : total > 0.f ? __fdividef(1.f, total) : 0.f;
 #pragma unroll
       for (int v = 0; v < V; v++) {
         const int i = v * 32 + lane;
@@ -319,26 +324,36 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
         t[v] = z[v] == -INFINITY ? -INFINITY : fmaxf(s + b, -INFINITY);      // (NaN, of a bias: not there)
         if (z[v] > -INFINITY) size = fmaxf(size, s + fabsf(b));
       }
-      const float slack = 4.7683716e-7f * __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size)));
+      const float slack = 9.5367432e-7f * __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size)));
       const bool single = A.sigmoid || A.bias == nullptr;      // own_number() has them
       bool sure = slack < 1e30f && m < INFINITY;
       if (A.groups > 1) {
-        float* s = (float*)(route_sm + w * E);
+        float* s = (float*)(route_sm + w * own_doubles(E));
         __syncwarp();
 #pragma unroll
         for (int v = 0; v < V; v++)
           if (v * 32 + lane < E) s[v * 32 + lane] = t[v];
         __syncwarp();
         const Best g = best_of_groups(s, E / A.groups, A.groups, lane);
-        double sum = g.a, margin;
-        if (single) {      // (a group without experts stays at -inf)
-          if (lane < A.groups && g.a > -INFINITY) sum = own_number(A, row, g.ai, m) + (g.b > -INFINITY ? own_number(A, row, g.bi, m) : 0.0);
-        } else if (g.b > -INFINITY) {
-          sum += g.b;
+        float margin;
+        unsigned stays = keep_groups(g.b > -INFINITY ? g.a + g.b : g.a, A.groups, A.top, lane, margin);      // (a group without experts stays at -inf)
+        if (!(margin > 4.f * slack)) {      // sums of two come near each other: 64 bits, where no third number comes near a group's second
+          if (!single || __any_sync(0xffffffffu, lane < A.groups && g.c > -INFINITY && g.b - g.c <= 2.f * slack)) {
+            sure = false;
+          } else {
+            const int size = E / A.groups;
+            int ai = -1, bi = -1;
+            for (int i = lane * size; lane < A.groups && i < lane * size + size; i++) {
+              const float t = s[i];
+              if (ai < 0 && t == g.a) ai = i;
+              else if (bi < 0 && t == g.b) bi = i;
+            }
+            double sum = g.a;
+            if (lane < A.groups && g.a > -INFINITY) sum = own_number(A, row, ai, m);
+            if (lane < A.groups && g.b > -INFINITY) sum += own_number(A, row, bi, m);
+            stays = keep_groups(sum, A.groups, A.top, lane, margin);
+          }
         }
-        const unsigned stays = keep_groups(sum, A.groups, A.top, lane, margin);
-        // which two are a group's best is open where the third comes near the second, and then matters where groups come near each other
-        if (margin <= 4.0 * slack && (!single || __any_sync(0xffffffffu, lane < A.groups && g.c > -INFINITY && g.b - g.c <= 2.f * slack))) sure = false;
 #pragma unroll
         for (int v = 0; v < V; v++)      // ((i magic) >> 32 is i / (experts of a group) for i < 2^16)
           if (!((stays >> ((magic ? __umulhi(v * 32 + lane, magic) : v * 32 + lane) & 31)) & 1)) t[v] = -INFINITY;
@@ -353,12 +368,16 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
         double own = value_of(c.x);
         if (single && lane < count) own = own_number(A, row, (int)c.y, m);
         const uint64_t k64 = lane < count ? order64(own) : 0;
+        uint64_t* keys = (uint64_t*)(route_sm + w * own_doubles(E));
+        __syncwarp();
+        keys[lane] = k64;
+        __syncwarp();
         double near = INFINITY;      // (softmax with a bias: the distance to the next better one)
         int rank = 0;
-        for (int j = 0; j < count; j++) {
-          const uint64_t x = (uint64_t)__shfl_sync(0xffffffffu, (uint32_t)(k64 >> 32), j) << 32 | __shfl_sync(0xffffffffu, (uint32_t)k64, j);
-          const uint32_t xi = __shfl_sync(0xffffffffu, c.y, j);
-          rank += x > k64 || (x == k64 && xi < c.y);
+#pragma unroll 4
+        for (int j = 0; j < count; j++) {      // (the list is in the order of the experts but for v: of equal ones the index decides)
+          const uint64_t x = keys[j];
+          rank += x > k64 || (x == k64 && list[j].y < c.y);
           if (!single && j != lane) near = fmin(near, fabs(value64(x) - own));
         }
         if (!single) sure = !__any_sync(0xffffffffu, lane < count && rank <= A.k && near <= 2.0 * slack);
@@ -367,7 +386,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
         __syncwarp();
         if (lane < A.k && lane < count) mine = (int)list[lane].x;
       }
-      if (count > 32 || !sure) mine = choose_exact(A, row, route_sm + w * E, m);
+      if (count > 32 || !sure) mine = choose_exact(A, row, route_sm + w * own_doubles(E), m);
     }
     // lane j: the weight of the j-th
     const float zj = mine >= 0 ? seen(logit(row, mine)) : -INFINITY;
@@ -376,9 +395,9 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
       const float top = warp_max(zj);
       wj = zj == -INFINITY ? 0.f : A.sigmoid ? sigmoid_from(zj, fminf(top, 0.f)) : exp_from(zj, top);
       const float sum = warp_sum(wj);
-      wj = sum > 0.f ? __fdiv_rn(wj, sum) : 0.f;
+      wj = sum > 0.f ? __fdividef(wj, sum) : 0.f;
     } else if (zj > -INFINITY) {
-      wj = A.sigmoid ? sigmoid_fine(zj) : __fdiv_rn(exp_from(zj, m), total);
+      wj = A.sigmoid ? sigmoid_fine(zj) : __fdividef(exp_from(zj, m), total);
     }
     if (lane < A.k) {
       A.idx[n * A.k + lane] = mine;
@@ -462,7 +481,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_bwd_k(const RouteB
         total += p[v];
       }
       total = warp_sum(total);
-      inv = total > 0.f ? __fdiv_rn(1.f, total) : 0.f;
+      inv = total > 0.f ? __fdividef(1.f, total) : 0.f;
 #pragma unroll
       for (int v = 0; v < V; v++) p[v] *= inv;
     }
@@ -471,7 +490,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_bwd_k(const RouteB
       const float top = warp_max(zj);
       float q = zj == -INFINITY ? 0.f : A.sigmoid ? sigmoid_from(zj, fminf(top, 0.f)) : exp_from(zj, top);
       const float sum = warp_sum(q);
-      q = sum > 0.f ? __fdiv_rn(q, sum) : 0.f;
+      q = sum > 0.f ? __fdividef(q, sum) : 0.f;
       own = q * (g - warp_sum(q * g));
       if (A.sigmoid) own *= sigmoid_fine(-zj);
     } else if (A.sigmoid) {
@@ -523,7 +542,7 @@ int route_blocks(long N, bool sums) {
   const long want = (N + ROUTE_WARPS - 1) / ROUTE_WARPS, most = sums ? (long)mlb_sm_count() * 4 : 1L << 16;
   return (int)std::max(1L, std::min(want, most));
 }
-constexpr size_t ROUTE_LISTS = sizeof(uint2) * ROUTE_WARPS * 32;
+constexpr size_t ROUTE_LISTS = sizeof(uint2) * ROUTE_WARPS * LIST;
 template <auto KERN>
 int launch_route(const RouteArgs& A, int blocks, size_t smem, cudaStream_t st) {
   if (smem > 48 * 1024) {
@@ -556,7 +575,7 @@ MLB_API int mlb_moe_route(void* weights, int* idx, float* mean, float* part, con
   const RouteArgs A = {logits, bias, weights, idx, mean ? part : nullptr, N, ld, E, k, groups, top, sigmoid, renorm, wbits == 32, scale};
   const int blocks = route_blocks(N, mean != nullptr);
   const bool plain = bias == nullptr && groups == 1;
-  const size_t smem = std::max(ROUTE_LISTS + (plain ? 0 : sizeof(double) * ROUTE_WARPS * E), mean ? sizeof(float) * ROUTE_WARPS * E : 0);
+  const size_t smem = std::max(ROUTE_LISTS + (plain ? 0 : sizeof(double) * ROUTE_WARPS * own_doubles(E)), mean ? sizeof(float) * ROUTE_WARPS * E : 0);
   int rc = by_width(E, [&](auto V) {
     if (plain) return zbits == 16 ? launch_route<moe_route_k<V.value, bf16, true>>(A, blocks, smem, st) : launch_route<moe_route_k<V.value, float, true>>(A, blocks, smem, st);
     return zbits == 16 ? launch_route<moe_route_k<V.value, bf16, false>>(A, blocks, smem, st) : launch_route<moe_route_k<V.value, float, false>>(A, blocks, smem, st);
