@@ -204,12 +204,20 @@ class Embedding(torch.autograd.Function):
         return dw.to(ctx.dtype), None, None
 
 
+def _rows_of(x):
+    """A matrix as the kernels of routing and of the experts read it: rows of neighbouring elements, side by side or apart, that begin on 16-byte boundaries."""
+    if x.stride(1) == 1 and x.stride(0) >= x.shape[1] and x.stride(0) * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return x.contiguous() if not x.is_contiguous() or x.data_ptr() % 16 == 0 else x.clone()
+
+
 class MoERoute(torch.autograd.Function):
     """logits [N, E] -> weights [N, k], idx int32 [N, k], mean fp32 [E] (ops/ref_moe.py has what they are).  The choice has no gradient, and neither has the bias."""
 
     @staticmethod
     def forward(ctx, logits, k, bias, score, groups, top_groups, renorm, scale, dtype):
         N, E = logits.shape
+        logits = _rows_of(logits)
         weights, idx = _like(logits, N, k, dtype=dtype), _like(logits, N, k, dtype=torch.int32)
         mean = _like(logits, E, dtype=torch.float32)
         ops.moe_route(weights, idx, mean, logits, bias, score, groups, top_groups, renorm, scale)
@@ -237,7 +245,7 @@ class MoEMLP(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weights, idx, gate_up, down):
-        weights, idx, gate_up, down = weights.contiguous(), idx.contiguous(), gate_up.contiguous(), down.contiguous()
+        x, weights, idx, gate_up, down = _rows_of(x), weights.contiguous(), idx.contiguous(), gate_up.contiguous(), down.contiguous()
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         saved = ops.moe_mlp_fwd(out, x, weights, idx, gate_up, down)
         ctx.save_for_backward(x, weights, idx, gate_up, down, *saved)
@@ -315,5 +323,5 @@ def moe_mlp(x, weights, idx, gate_up, down):
         y = _plain("moe_mlp", x, weights, idx, gate_up, down)
         return MoEMLP.apply(x, weights, idx, gate_up, down) if y is NotImplemented else y
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    ops.moe_mlp(out, x, weights.contiguous(), idx.contiguous(), gate_up.contiguous(), down.contiguous())
+    ops.moe_mlp(out, _rows_of(x), weights.contiguous(), idx.contiguous(), gate_up.contiguous(), down.contiguous())
     return out

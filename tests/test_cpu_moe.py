@@ -137,6 +137,47 @@ def test_entry_points_have_one_signature():
         assert all(d == k or (d == "p" and k in "bfiu") for d, k in zip(defined["mlb_" + name], kinds)), name
 
 
+def test_entries_refuse_what_they_cannot_address():
+    """-7, before anything is launched: memory off 16 bytes, rows apart by no multiple of 8, sizes out of range."""
+    from ml_b200.ops import native
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are nobody's memory: asked only where no kernel can run")
+    L, ok, off = native.lib(), 1 << 20, (1 << 20) + 2
+    sizes = dict(N=40, ld=64, k=2, E=4, C=64, I=48, bits=16)
+    fwd = lambda **kw: L.mlb_moe_fwd(*{**{n: ok for n in ("out", "xs", "gu", "h", "y", "x", "weights", "gate_up", "down", "plan")}, **sizes, **kw}.values(), None)
+    bwd = lambda **kw: L.mlb_moe_bwd(*{**{n: ok for n in ("dx", "dweights", "dgate_up", "ddown", "ys", "dgu", "dxs", "dout", "xs", "gu", "h", "y", "weights", "gate_up", "down", "plan")}, **sizes,
+                                       **kw}.values(), None)
+    few = lambda **kw: L.mlb_moe_few(*{**{n: ok for n in ("out", "x", "weights", "idx", "gate_up", "down", "part")}, **sizes, "N": 4, **kw}.values(), None)
+    for call, names in ((fwd, ("out", "xs", "gu", "h", "y", "x", "gate_up", "down", "plan")),
+                        (bwd, ("dx", "dgate_up", "ddown", "ys", "dgu", "dxs", "dout", "xs", "gu", "h", "y", "gate_up", "down", "plan")), (few, ("out", "x", "gate_up", "down", "part"))):
+        for bad in [{n: off} for n in names] + [dict(ld=68), dict(C=72), dict(I=40), dict(E=1025), dict(E=0), dict(k=0), dict(bits=8), dict(N=1 << 31)]:
+            assert call(**bad) == -7, (names, bad)
+    assert few(N=9) == -7 and few(N=8, k=33) == -7
+    assert L.mlb_moe_plan_ints(1 << 31, 2, 4) == L.mlb_moe_plan_rows(1 << 31, 2, 4) == -7
+    assert L.mlb_moe_plan(off, ok, 40, 2, 4, None) == -7
+    route = lambda **kw: L.mlb_moe_route(*{**dict(w=ok, idx=ok, mean=None, part=None, z=ok, bias=None, N=4, ld=64, E=64, k=2, sigmoid=0, groups=1, top=1, renorm=1, scale=1.0, zb=32, wb=32), **kw}.values(),
+                                         None)
+    for bad in (dict(E=1025), dict(k=0), dict(k=33), dict(E=1), dict(groups=3), dict(groups=64), dict(top=2), dict(zb=64), dict(N=-1)):
+        assert route(**bad) == -7, bad
+
+
+def test_a_plan_has_room_for_every_distribution():
+    """Rows and tiles that the plan's buffers have, against the worst distributions of copies over experts."""
+    from ml_b200.ops import native
+    L = native.lib()
+    for NK in (1, 2, 31, 32, 33, 255, 256, 257, 2048, 2049, 5000, 131073):
+        for E in (1, 2, 7, 64, 1024):
+            rows = L.mlb_moe_plan_rows(NK, 1, E)
+            spread = [NK // E + (i < NK % E) for i in range(E)]
+            ones = [1] * min(E - 1, NK - 1) + [NK - min(E - 1, NK - 1)]
+            odd = [33] * min(E - 1, (NK - 1) // 33) + [NK - 33 * min(E - 1, (NK - 1) // 33)]
+            tiles = NK // 256 + min(NK, E)
+            for d in (spread, ones, odd):
+                assert sum(-(-n // 32) * 32 for n in d) <= rows and rows % 32 == 0
+                assert sum(-(-n // 256) for n in d) <= tiles
+            assert L.mlb_moe_plan_ints(NK, 1, E) >= 2 * E + 2 + 4 * tiles + NK + rows
+
+
 # ------------------------------------------------------------------ the block, the decoder
 def test_block_gives_what_the_loop_over_experts_gives():
     from ml_b200.models.moe import MoE, MoEBlock

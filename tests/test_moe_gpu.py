@@ -379,6 +379,48 @@ def test_rows_of_a_wider_tensor_and_frozen_weights():
     close(torch.autograd.grad(y, down, torch.ones_like(y)), want, sizes, ["ddown"])
 
 
+def test_inputs_of_any_layout():
+    """Broadcast, transposed and unaligned tensors, through the differentiable operators."""
+    x, w, idx, gate_up, down = experts(40, 4, 2, 64, 48)
+    one = x[:1].clone().requires_grad_()
+    y = F.moe_mlp(one.expand(40, 64), w, idx, gate_up, down)
+    d, = torch.autograd.grad(y, one, dout := torch.randn(40, 64, device=dev()).to(BF16))
+    want = oracle.mlp_grads(dout, one.detach().expand(40, 64), w, idx, gate_up, down)
+    assert float((d.double() - want[1].sum(0, keepdim=True)).norm()) <= 8 * HALF[BF16] * float(want[1].sum(0).norm())
+    for t in (x.T.contiguous().T, torch.cat([x.flatten()[:1], x.flatten()])[1:].view(40, 64)):
+        with torch.no_grad():
+            assert torch.equal(F.moe_mlp(t, w, idx, gate_up, down), F.moe_mlp(x, w, idx, gate_up, down))
+        g, = torch.autograd.grad(F.moe_mlp(t.requires_grad_(), w.T.contiguous().T, idx.T.contiguous().T, gate_up.transpose(1, 2).contiguous().transpose(1, 2), down), t, dout)
+        assert torch.equal(g, torch.autograd.grad(F.moe_mlp(xr := x.clone().requires_grad_(), w, idx, gate_up, down), xr, dout)[0])
+    z = torch.randn(8, 40, device=dev()).T.requires_grad_()
+    a, b = F.moe_route(z, 2), F.moe_route(zc := z.detach().contiguous().requires_grad_(), 2)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    assert torch.equal(torch.autograd.grad(a[0].sum() + a[2][0], z)[0], torch.autograd.grad(b[0].sum() + b[2][0], zc)[0])
+
+
+@pytest.mark.parametrize("which", [(0,), (1,), (2,), (3,), (0, 2), (1, 3)])
+def test_any_of_the_gradients(which):
+    x, w, idx, gate_up, down = experts(70, 5, 2, 128, 80)
+    leaves = [x, w, gate_up, down]
+    for i in which:
+        leaves[i].requires_grad_()
+    y = F.moe_mlp(x, w, idx, gate_up, down)
+    wanted = [leaves[i] for i in which]
+    first = torch.autograd.grad(y, wanted, dout := torch.randn(70, 128, device=dev()).to(BF16), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, wanted, dout)))      # (nothing kept for it has changed)
+    want, sizes = (f(dout, x, w, idx, gate_up, down) for f in (oracle.mlp_grads, oracle.mlp_sizes))
+    close(first, want, sizes, [WHAT[1 + i] for i in which])
+
+
+@pytest.mark.parametrize("N", [3, 60])
+def test_negative_indices_of_any_size_are_none(N):
+    x, w, idx, gate_up, down = experts(N, 4, 2, 64, 48, drop=2)
+    a, b = torch.empty_like(x), torch.empty_like(x)
+    ops.moe_mlp(a, x, w, idx, gate_up, down)
+    ops.moe_mlp(b, x, w, torch.where(idx < 0, -(1 << 31), idx.long()).to(I32), gate_up, down)
+    assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("N,E,k,C,I", [(1, 8, 2, 256, 128), (16, 8, 2, 256, 128), (900, 8, 3, 128, 256), (257, 64, 8, 64, 96)])
 def test_the_same_bits_on_every_run_and_from_a_graph(N, E, k, C, I):
     x, w, idx, gate_up, down = leaves = experts(N, E, k, C, I, F32)
