@@ -733,80 +733,107 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
 }
 
 // ------------------------------------------------------------------ few tokens
-// A step of a few tokens reads the weights of the experts that they chose, once, and that is all its time.  One, two, four or eight warps share units of 16 rows of one
-// expert, each the boxes of 16 rows x 64 columns of its part of the reduction, which it fetches into shared memory of its own: three stages of four boxes a warp, 192 KB an SM on
-// their way.  The products are m16n8k16 instructions whose 16 rows are weights and whose 8 columns are tokens (which eight elements of the reduction an instruction
-// has is the same for both operands: 16 neighbouring bytes a lane serve two instructions).  Three launches: h of all copies, with 8 rows of the gate and 8 of the up
-// projection to a unit; y; their weighted sums.  An expert's copies are found by each block for itself: 256 at most.
+// A step of a few tokens reads the weights of the experts that they chose, once, and that is all its time.  Warps read boxes of 16 rows x 64 columns of the weights, each into shared memory
+// of its own: three stages of four boxes, 192 KB an SM on their way.  The products are m16n8k16 instructions whose 16 rows are weights and whose 8 columns are tokens (which eight
+// elements of the reduction an instruction has is the same for both operands: 16 neighbouring bytes a lane serve two instructions).  Two launches: h of all copies, then
+// the tokens' weighted sums.  An expert's copies are found by each block for itself: 256 at most.
 constexpr int FEW_TOKENS = 8, FEW_COPIES = 256, FEW_WARPS = 8, FEW_THREADS = 32 * FEW_WARPS, FEW_BOX = 2048, FEW_BOXES = 4, FEW_STAGES = 3;
 constexpr int FEW_SMEM = FEW_WARPS * FEW_STAGES * FEW_BOXES * FEW_BOX + 1024;
 struct FewArgs {
-  bf16* h;              // [N k, I]
-  float* y;             // [N k, C]
+  bf16 *out, *h;        // h [N k, I]
   const bf16* x;
+  const void* weights;
   const int* idx;
   long ldx;
-  int N, k, E, C, I, ways;      // ways: warps that share a unit
+  int N, k, E, C, I, wbits;
+  int ways;             // h: warps that share a unit
 };
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <bool DOWN_>
-__global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_k(const __grid_constant__ CUtensorMap tmW, const FewArgs A) {
-  // The kernel before the one for y is that for h, which has waited for all before it: idx and the weights stand, and only h has to be waited for.  (Past the L1, of
-  // which nothing is known so early.)
-  if (!DOWN_) mlb_pdl_sync();
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(16) int expert[FEW_COPIES];
-  __shared__ int list[FEW_COPIES], nth[FEW_COPIES], first[FEW_COPIES + 1], of[FEW_COPIES], sums[FEW_WARPS];
-  __shared__ uint64_t full[FEW_WARPS][FEW_STAGES];
-  __shared__ float4 part[2][FEW_WARPS][32];
+// The copies by expert: list[first[a] ..] are those of of[a].  More copies than an instruction's columns (a token may name an expert twice) are dealt with as if another expert had them.
+struct FewLists {
+  __align__(16) int expert[FEW_COPIES];
+  int list[FEW_COPIES], nth[FEW_COPIES], first[FEW_COPIES + 1], of[FEW_COPIES], sums[FEW_WARPS];
+};
+__device__ __forceinline__ int few_lists(FewLists& L, const FewArgs& A, bool reports) {      // by 256 threads; how many experts
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, NK = A.N * A.k;
-  // the copies by expert: a copy's place is the number of those before it.  More copies than an instruction's columns (a token may name an expert twice) are dealt with as if
-  // another expert had them.
   int e = tid < NK ? __ldcg(A.idx + tid) : -1;
   if (e >= A.E) {
-    if (!DOWN_ && blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xD1);
+    if (reports && blockIdx.x == 0) mlb_set_error(MLB_ERR_BOUNDS, 0xD1);
     e = -1;
   }
-  expert[tid] = e < 0 ? 0x7fffffff : e, list[tid] = -1;
+  L.expert[tid] = e < 0 ? 0x7fffffff : e, L.list[tid] = -1;
+  __syncthreads();
+  if (e >= 0) {      // a copy's place is the number of those before it
+    int less = 0, equal = 0;
+#pragma unroll 4
+    for (int i = 0; i < NK; i += 4) {
+      const int4 x = *reinterpret_cast<const int4*>(L.expert + i);
+      less += (x.x < e) + (x.y < e) + (x.z < e) + (x.w < e);
+      equal += (x.x == e && i < tid) + (x.y == e && i + 1 < tid) + (x.z == e && i + 2 < tid) + (x.w == e && i + 3 < tid);
+    }
+    L.nth[tid] = equal;
+    L.list[less + equal] = tid;
+  }
+  __syncthreads();
+  const int here = L.list[tid];
+  const bool begins = here >= 0 && L.nth[here] % 8 == 0;
+  const unsigned b = __ballot_sync(0xffffffffu, begins);
+  if (lane == 0) L.sums[w] = __popc(b);
+  const int held = __syncthreads_count(here >= 0);
+  int experts = 0, before = __popc(b & ((1u << lane) - 1));
+#pragma unroll
+  for (int i = 0; i < FEW_WARPS; i++) {
+    before += i < w ? L.sums[i] : 0;
+    experts += L.sums[i];
+  }
+  if (begins) L.first[before] = tid, L.of[before] = L.expert[here];
+  if (tid == 0) L.first[experts] = held;
+  __syncthreads();
+  return experts;
+}
+// Eight tokens' part of one step (the reduction's columns 256 s ...): `col` is this lane's token's row
+__device__ __forceinline__ void few_tokens(uint4 (&v)[FEW_BOXES][2], const bf16* col, int s, int K, int t) {
+#pragma unroll
+  for (int x = 0; x < 2 * FEW_BOXES; x++) {
+    const int k = (s * FEW_BOXES + x / 2) * 64 + x % 2 * 32 + t * 8;
+    v[x / 2][x % 2] = k < K ? *reinterpret_cast<const uint4*>(col + k) : make_uint4(0, 0, 0, 0);
+  }
+}
+// d += the products of one step, `some` boxes (two sums: neighbouring instructions do not wait for one another)
+__device__ __forceinline__ void few_products(float (&d)[2][4], const uint8_t* stage, const uint4 (&v)[FEW_BOXES][2], int some, int r, int t) {
+#pragma unroll
+  for (int x = 0; x < FEW_BOXES; x++) {
+    if (x >= some) break;
+    const uint8_t* box = stage + x * FEW_BOX + r * 128;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int at = ((t + 4 * j) ^ r) << 4;
+      const uint4 p = *reinterpret_cast<const uint4*>(box + at), q = *reinterpret_cast<const uint4*>(box + 1024 + at);
+      mma_16816(d[0], p.x, q.x, p.y, q.y, v[x][j].x, v[x][j].y);
+      mma_16816(d[1], p.z, q.z, p.w, q.w, v[x][j].z, v[x][j].w);
+    }
+  }
+}
+// h: a unit is 8 rows of the gate and 8 of the up projection of an expert; one, two, four or eight warps share it, each with some steps of its reduction
+__global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_h_k(const __grid_constant__ CUtensorMap tmW, const FewArgs A) {
+  mlb_pdl_sync();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ FewLists L;
+  __shared__ uint64_t full[FEW_WARPS][FEW_STAGES];
+  __shared__ float4 part[2][FEW_WARPS][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   if (lane == 0) {
     for (int i = 0; i < FEW_STAGES; i++) tc::mbar_init(&full[w][i], 1);
     tc::mbar_fence_init();
     if (w == 0) tc::tma_prefetch_desc(&tmW);
   }
-  __syncthreads();
-  if (e >= 0) {
-    int less = 0, equal = 0;
-#pragma unroll 4
-    for (int i = 0; i < NK; i += 4) {
-      const int4 x = *reinterpret_cast<const int4*>(expert + i);
-      less += (x.x < e) + (x.y < e) + (x.z < e) + (x.w < e);
-      equal += (x.x == e && i < tid) + (x.y == e && i + 1 < tid) + (x.z == e && i + 2 < tid) + (x.w == e && i + 3 < tid);
-    }
-    nth[tid] = equal;
-    list[less + equal] = tid;
-  }
-  __syncthreads();
-  const int here = list[tid];
-  const bool begins = here >= 0 && nth[here] % 8 == 0;
-  const unsigned b = __ballot_sync(0xffffffffu, begins);
-  if (lane == 0) sums[w] = __popc(b);
-  const int held = __syncthreads_count(here >= 0);
-  int experts = 0, before = __popc(b & ((1u << lane) - 1));
-#pragma unroll
-  for (int i = 0; i < FEW_WARPS; i++) {
-    before += i < w ? sums[i] : 0;
-    experts += sums[i];
-  }
-  if (begins) first[before] = tid, of[before] = expert[here];
-  if (tid == 0) first[experts] = held;
-  __syncthreads();
-
-  const int K = DOWN_ ? A.I : A.C, groups = DOWN_ ? A.C / 16 : A.I / 8, units = experts * groups, boxes = (K + 63) / 64, steps = (boxes + FEW_BOXES - 1) / FEW_BOXES;
+  const int experts = few_lists(L, A, true);
+  const int K = A.C, groups = A.I / 8, units = experts * groups, boxes = (K + 63) / 64, steps = (boxes + FEW_BOXES - 1) / FEW_BOXES;
   // the units of this warp and those beside it; of each it has the steps `part_of`, part_of + ways, ...
   const int r = lane >> 2, t = lane & 3, ways = A.ways, part_of = w % ways, begin = blockIdx.x + w / ways * gridDim.x, every = gridDim.x * (FEW_WARPS / ways);
   uint8_t* ring = smem + w * (FEW_STAGES * FEW_BOXES * FEW_BOX);
@@ -817,32 +844,22 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_k(const __grid_constan
       const int a = next_unit / groups, g = next_unit - a * groups, stage = asked % FEW_STAGES, some = min(FEW_BOXES, boxes - next_s * FEW_BOXES);
       uint64_t* bar = &full[w][stage];
       tc::mbar_expect_tx(bar, some * FEW_BOX);
-      for (int j = 0; j < some; j++) {
-        uint8_t* to = ring + (stage * FEW_BOXES + j) * FEW_BOX;
-        if (DOWN_) tc::tma_load_3d(to, &tmW, bar, (next_s * FEW_BOXES + j) * 64, g * 16, of[a]);
-        else tc::tma_load_5d(to, &tmW, bar, (next_s * FEW_BOXES + j) * 64, 0, 0, g, of[a]);
-      }
+      for (int j = 0; j < some; j++) tc::tma_load_5d(ring + (stage * FEW_BOXES + j) * FEW_BOX, &tmW, bar, (next_s * FEW_BOXES + j) * 64, 0, 0, g, L.of[a]);
     }
     asked++;
     if ((next_s += ways) >= steps) next_s = part_of, next_unit += every;
   };
   for (int i = 0; i < FEW_STAGES; i++) ask();
-  if (DOWN_) mlb_pdl_sync();
   bool ok = true;
   uint4 ahead[FEW_BOXES][2] = {};      // the tokens' part of the next step, asked for while this one goes on
   auto tokens = [&](int unit, int s) {
-    const int a = unit / groups, f0 = first[a], c = list[f0 + min(r, first[a + 1] - f0 - 1)];      // (columns behind the last copy: its row, nothing of theirs is used)
-    const bf16* col = DOWN_ ? A.h + (size_t)c * A.I : A.x + (size_t)(c / A.k) * A.ldx;
-#pragma unroll
-    for (int x = 0; x < 2 * FEW_BOXES; x++) {
-      const int k = (s * FEW_BOXES + x / 2) * 64 + x % 2 * 32 + t * 8;
-      ahead[x / 2][x % 2] = k < K ? *reinterpret_cast<const uint4*>(col + k) : make_uint4(0, 0, 0, 0);
-    }
+    const int a = unit / groups, f0 = L.first[a], c = L.list[f0 + min(r, L.first[a + 1] - f0 - 1)];      // (columns behind the last copy: its row, nothing of theirs is used)
+    few_tokens(ahead, A.x + (size_t)(c / A.k) * A.ldx, s, K, t);
   };
   if (begin < units && part_of < steps) tokens(begin, part_of);
   for (int unit = begin; unit < units; unit += every, turn ^= 1) {
-    const int a = unit / groups, g = unit - a * groups, f0 = first[a], copies = first[a + 1] - f0;
-    float d[2][4] = {};      // (two sums: neighbouring instructions do not wait for one another)
+    const int a = unit / groups, g = unit - a * groups, f0 = L.first[a], copies = L.first[a + 1] - f0;
+    float d[2][4] = {};
 #pragma unroll 1
     for (int s = part_of; s < steps; s += ways, n++) {
       uint4 v[FEW_BOXES][2];
@@ -852,22 +869,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_k(const __grid_constan
       else if (unit + every < units) tokens(unit + every, part_of);
       const int stage = n % FEW_STAGES;
       if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[w][stage], (n / FEW_STAGES) & 1, 0x76));
-#pragma unroll
-      for (int x = 0; x < FEW_BOXES; x++) {
-        if (s * FEW_BOXES + x >= boxes) break;
-        const uint8_t* box = ring + (stage * FEW_BOXES + x) * FEW_BOX + r * 128;
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const int at = ((t + 4 * j) ^ r) << 4;
-          const uint4 p = *reinterpret_cast<const uint4*>(box + at), q = *reinterpret_cast<const uint4*>(box + 1024 + at);
-          mma_16816(d[0], p.x, q.x, p.y, q.y, v[x][j].x, v[x][j].y);
-          mma_16816(d[1], p.z, q.z, p.w, q.w, v[x][j].z, v[x][j].w);
-        }
-      }
+      few_products(d, ring + stage * FEW_BOXES * FEW_BOX, v, boxes - s * FEW_BOXES, r, t);
       __syncwarp();
       ask();
     }
-    // d[..][2 h + x]: row 8 h + lane / 4, column 2 (lane % 4) + x.  Of h's rows the first half is the gate's, the second the up projection's.
+    // d[..][2 h + x]: row 8 h + lane / 4, column 2 (lane % 4) + x.  The first half of the rows is the gate's, the second the up projection's.
     float4 sum = make_float4(d[0][0] + d[1][0], d[0][1] + d[1][1], d[0][2] + d[1][2], d[0][3] + d[1][3]);
     if (ways > 1) {      // (two places in turn: whoever writes to one again has met the others behind their reading of it)
       part[turn][w][lane] = sum;
@@ -882,39 +888,123 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_k(const __grid_constan
     for (int x = 0; x < 2; x++) {
       if (2 * t + x >= copies) continue;
       const float p = x ? sum.y : sum.x, q = x ? sum.w : sum.z;
-      const size_t to = list[f0 + 2 * t + x];
-      if (DOWN_) A.y[to * A.C + g * 16 + r] = p, A.y[to * A.C + g * 16 + 8 + r] = q;
-      else A.h[to * A.I + g * 8 + r] = __float2bfloat16(p * rcp(1.f + ex2(-1.44269504f * p)) * q);
+      A.h[(size_t)L.list[f0 + 2 * t + x] * A.I + g * 8 + r] = __float2bfloat16(p * rcp(1.f + ex2(-1.44269504f * p)) * q);
     }
   }
 }
-// out[n] = the weighted sum of its copies' y, four columns a thread
-template <typename W>
-__global__ void __launch_bounds__(128) moe_few_sum_k(bf16* __restrict__ out, const float* __restrict__ y, const W* __restrict__ weights, const int* __restrict__ idx, int N, int k, int E, int C) {
-  mlb_pdl_sync();
-  const int at = blockIdx.x * 128 + threadIdx.x, n = at / (C / 4), c = at - n * (C / 4);
-  if (n >= N) return;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int q = n * k; q < (n + 1) * k; q++) {
-    const int e = idx[q];
-    if (e < 0 || e >= E) continue;
-    const float w = as_float(weights[q]);
-    const float4 x = reinterpret_cast<const float4*>(y + (size_t)q * C)[c];
-    s.x = fmaf(w, x.x, s.x), s.y = fmaf(w, x.y, s.y), s.z = fmaf(w, x.z, s.z), s.w = fmaf(w, x.w, s.w);
+// out: a cluster of SPLIT blocks has 16 columns of all tokens, and its warps share the steps of all experts' reductions, a run of neighbouring ones each.  Sums of products are
+// sums of their parts, so a warp adds what it has of an expert, times the weight, to sums of its own, in fp32; those of all warps are added in their order.
+template <int SPLIT>
+__global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(FEW_THREADS, 1) moe_few_out_k(const __grid_constant__ CUtensorMap tmW, const FewArgs A) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ FewLists L;
+  __shared__ uint64_t full[FEW_WARPS][FEW_STAGES];
+  __shared__ float weight[FEW_COPIES], part[FEW_WARPS][8][16], sums[FEW_WARPS][FEW_TOKENS][16], from[2][SPLIT][FEW_TOKENS * 16];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rank = SPLIT > 1 ? (int)tc::cluster_ctarank() : 0;
+  // The kernel before is that for h, which has waited for all before it: idx and the weights stand, and only h has to be waited for.  (Past the L1, of which nothing is known so early.)
+  if (tid < A.N * A.k) weight[tid] = A.wbits == 32 ? __ldcg((const float*)A.weights + tid) : __uint_as_float((uint32_t)__ldcg((const unsigned short*)A.weights + tid) << 16);
+  if (lane == 0) {
+    for (int i = 0; i < FEW_STAGES; i++) tc::mbar_init(&full[w][i], 1);
+    tc::mbar_fence_init();
+    if (w == 0) tc::tma_prefetch_desc(&tmW);
   }
-  reinterpret_cast<uint2*>(out + (size_t)n * C)[c] = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+  const int experts = few_lists(L, A, false);
+  const int K = A.I, groups = A.C / 16, boxes = (K + 63) / 64, steps = (boxes + FEW_BOXES - 1) / FEW_BOXES, all = experts * steps;
+  const int share = (all + FEW_WARPS * SPLIT - 1) / (FEW_WARPS * SPLIT), begin = min((rank * FEW_WARPS + w) * share, all), end = min(begin + share, all), every = gridDim.x / SPLIT;
+  const int r = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + w * (FEW_STAGES * FEW_BOXES * FEW_BOX);
+  int next_g = blockIdx.x / SPLIT, next = begin, asked = 0, n = 0;
+  auto ask = [&]() {
+    if (next_g >= groups || begin >= end) return;
+    if (lane == 0) {
+      const int a = next / steps, box = (next - a * steps) * FEW_BOXES, stage = asked % FEW_STAGES, some = min(FEW_BOXES, boxes - box);
+      uint64_t* bar = &full[w][stage];
+      tc::mbar_expect_tx(bar, some * FEW_BOX);
+      for (int j = 0; j < some; j++) tc::tma_load_3d(ring + (stage * FEW_BOXES + j) * FEW_BOX, &tmW, bar, (box + j) * 64, next_g * 16, L.of[a]);
+    }
+    asked++;
+    if (++next >= end) next = begin, next_g += every;
+  };
+  for (int i = 0; i < FEW_STAGES; i++) ask();
+  if (SPLIT > 1) tc::cluster_sync();      // (the first block of the cluster is there to be written to)
+  mlb_pdl_sync();
+  bool ok = true;
+  uint4 ahead[FEW_BOXES][2] = {};
+  auto tokens = [&](int i) {
+    const int a = i / steps, f0 = L.first[a], c = L.list[f0 + min(r, L.first[a + 1] - f0 - 1)];      // (columns behind the last copy: its row, nothing of theirs is used)
+    few_tokens(ahead, A.h + (size_t)c * A.I, i - a * steps, K, t);
+  };
+  if (begin < end) tokens(begin);
+  int turn = 0;
+  for (int g = blockIdx.x / SPLIT; g < groups; g += every, turn ^= 1) {
+    for (int i = lane; i < FEW_TOKENS * 16; i += 32) (&sums[w][0][0])[i] = 0.f;
+    float d[2][4] = {};
+    int a = begin / steps, s = begin - a * steps;
+#pragma unroll 1
+    for (int i = begin; i < end; i++, n++) {
+      uint4 v[FEW_BOXES][2];
+#pragma unroll
+      for (int x = 0; x < 2 * FEW_BOXES; x++) v[x / 2][x % 2] = ahead[x / 2][x % 2];
+      tokens(i + 1 < end ? i + 1 : begin);
+      const int stage = n % FEW_STAGES;
+      if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[w][stage], (n / FEW_STAGES) & 1, 0x76));
+      few_products(d, ring + stage * FEW_BOXES * FEW_BOX, v, boxes - s * FEW_BOXES, r, t);
+      __syncwarp();
+      ask();
+      if (++s < steps && i + 1 < end) continue;
+      // the expert's copies are done, as far as this warp has them.  d[..][2 h + x]: row 8 h + lane / 4, column 2 (lane % 4) + x
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        part[w][2 * t + (q & 1)][r + 4 * (q & 2)] = d[0][q] + d[1][q];
+        d[0][q] = d[1][q] = 0.f;
+      }
+      __syncwarp();
+      const int f0 = L.first[a], copies = L.first[a + 1] - f0, row = lane & 15;
+      for (int c = 0; c < copies; c++) {      // even tokens to one half of the warp, odd ones to the other: a token that names an expert twice meets itself in order
+        const int copy = L.list[f0 + c], token = copy / A.k;
+        if ((token & 1) == lane >> 4) sums[w][token][row] = fmaf(weight[copy], part[w][c][row], sums[w][token][row]);
+      }
+      __syncwarp();
+      s = 0, a++;
+    }
+    __syncthreads();
+    float sum = 0.f;
+    if (tid < FEW_TOKENS * 16) {
+#pragma unroll
+      for (int i = 0; i < FEW_WARPS; i++) sum += (&sums[i][0][0])[tid];
+      if (SPLIT > 1 && rank != 0) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(tc::mapa_u32(tc::smem_u32(&from[turn][rank][tid]), 0)), "f"(sum) : "memory");
+    }
+    if (SPLIT > 1) tc::cluster_sync();      // (two places in turn: whoever writes to one again has met the first block behind its reading of it)
+    else __syncthreads();
+    if (rank == 0 && tid < 16 * A.N) {
+#pragma unroll
+      for (int i = 1; i < SPLIT; i++) sum += from[turn][i][tid];
+      A.out[(size_t)(tid / 16) * A.C + g * 16 + tid % 16] = __float2bfloat16(sum);
+    }
+  }
 }
-template <bool DOWN_>
-int launch_few(const CUtensorMap& m, FewArgs g, cudaStream_t st) {
+int launch_few_h(const CUtensorMap& m, FewArgs g, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  const cudaError_t e = mlb_allow_smem(moe_few_k<DOWN_>, FEW_SMEM, done);
+  const cudaError_t e = mlb_allow_smem(moe_few_h_k, FEW_SMEM, done);
   if (e != cudaSuccess) return (int)e;
-  const int units = std::min(g.N * g.k, g.E) * (DOWN_ ? g.C / 16 : g.I / 8), steps = ((DOWN_ ? g.I : g.C) + 255) / 256;
-  // As few warps to a unit as give most of an SM's warps one.  One token, us, by ways: 6 of 64 experts (1032 and 768 units) 28.3, 30.2, 31.9, 34.7; 2 of 8 experts of 5504 behind
-  // 2048 columns (1376 and 256) 53.5, 37.7, 33.3, 37.1; of 2048 behind 768 (512 and 96) 17.7, 12.8, 11.4, 13.3.
-  for (g.ways = 1; g.ways < FEW_WARPS && units * g.ways < 5 * mlb_sm_count() && 2 * g.ways <= steps;) g.ways *= 2;
-  return (int)mlb_launch(moe_few_k<DOWN_>, dim3(std::min(units, mlb_sm_count())), dim3(FEW_THREADS), (size_t)FEW_SMEM, st, m, g);
+  const int units = std::min(g.N * g.k, g.E) * (g.I / 8), steps = (g.C + 255) / 256;
+  // The number of warps to a unit with which the last round of units leaves least idle, two at least of long reductions, eight only where one round is all.  One token, whole call, us, with
+  // 1, 2 and 4: 6 of 64 experts of 1376 behind 2048 columns 26.7, 26.6, 26.7 (takes 2); 8 of 128 of 768 behind 2048 23.5, 24.0, 21.9 (4); 2 of 8 of 5504 behind 2048 37.3, 32.8, 31.6 (4), of
+  // 2048 behind 768 11.0, 10.3, 11.0 (2).
+  const long warps = (long)FEW_WARPS * mlb_sm_count();
+  auto rounds = [&](int ways) { return (units * (long)ways + warps - 1) / warps; };
+  g.ways = steps >= 8 ? 2 : 1;
+  for (int ways = 2 * g.ways; ways <= std::min(steps, FEW_WARPS) && (ways < FEW_WARPS || units * (long)ways <= warps); ways *= 2)
+    if (g.ways * rounds(ways) < ways * rounds(g.ways)) g.ways = ways;
+  return (int)mlb_launch(moe_few_h_k, dim3(std::min(units, mlb_sm_count())), dim3(FEW_THREADS), (size_t)FEW_SMEM, st, m, g);
+}
+template <int SPLIT>
+int launch_few_out(const CUtensorMap& m, const FewArgs& g, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = mlb_allow_smem(moe_few_out_k<SPLIT>, FEW_SMEM, done);
+  if (e != cudaSuccess) return (int)e;
+  return (int)mlb_launch(moe_few_out_k<SPLIT>, dim3(SPLIT * std::min(g.C / 16, mlb_sm_count() / SPLIT)), dim3(FEW_THREADS), (size_t)FEW_SMEM, st, m, g);
 }
 
 struct Maps { CUtensorMap a, b, b16, a1, b1, a2, b2, out, out1, out2; };
@@ -1075,24 +1165,24 @@ MLB_API int mlb_moe_bwd(void* dx, void* dweights, void* dgate_up, void* ddown, v
   MLB_TRY(launch_gemm<BACK>(m, g, (long)E * (g.per_gate_up + g.per_down) + (long)z.p.max_tiles * g.tiles_m, st));
   return dx != nullptr ? combine((bf16*)dx, (const bf16*)dxs, (const float*)nullptr, P, z, st) : 0;
 }
-// floats of the workspace of the form for few tokens: y and h; 0: the sizes take the other form
+// floats of the workspace of the form for few tokens; 0: the sizes take the other form
 MLB_API long mlb_moe_few_floats(long N, int k, int E, int C, int I) {
   Sizes z;
   if (sizes(z, N, k, E, C, I) != 0 || N < 1 || N > FEW_TOKENS || z.NK > FEW_COPIES) return 0;
-  return z.NK * C + (z.NK * I + 1) / 2;
+  return z.NK * I / 2;      // (h)
 }
 MLB_API int mlb_moe_few(void* out, const void* x, const void* weights, const int* idx, const void* gate_up, const void* down, float* part, long N, long ldx, int k, int E, int C, int I,
                         int wbits, cudaStream_t st) {
   if (mlb_moe_few_floats(N, k, E, C, I) == 0 || off16({out, x, gate_up, down, part}) || ldx % 8 != 0 || (wbits != 16 && wbits != 32)) return -7;
-  const FewArgs g = {(bf16*)(part + N * k * C), part, (const bf16*)x, idx, ldx, (int)N, k, E, C, I, 1};
+  const FewArgs g = {(bf16*)out, (bf16*)part, (const bf16*)x, weights, idx, ldx, (int)N, k, E, C, I, wbits, 1};
   const uint64_t c = C, i = I, n = E;
   const uint64_t da[5] = {c, 8, 2, i / 8, n}, sa[4] = {2 * c, 2 * i * c, 16 * c, 4 * i * c}, db[3] = {i, c, n}, sb[2] = {2 * i, 2 * c * i};
   const uint32_t ba[5] = {64, 8, 2, 1, 1}, bb[3] = {64, 16, 1};
   alignas(64) CUtensorMap a, b;
   if (!mlb_make_tmap_nd(&a, gate_up, 5, da, sa, ba) || !mlb_make_tmap_nd(&b, down, 3, db, sb, bb)) return -2;
-  MLB_TRY(launch_few<false>(a, g, st));
-  MLB_TRY(launch_few<true>(b, g, st));
-  const dim3 blocks((unsigned)((N * (C / 4) + 127) / 128));
-  if (wbits == 16) return (int)mlb_launch(moe_few_sum_k<bf16>, blocks, dim3(128), 0, st, (bf16*)out, (const float*)part, (const bf16*)weights, idx, (int)N, k, E, C);
-  return (int)mlb_launch(moe_few_sum_k<float>, blocks, dim3(128), 0, st, (bf16*)out, (const float*)part, (const float*)weights, idx, (int)N, k, E, C);
+  MLB_TRY(launch_few_h(a, g, st));
+  // Blocks for most SMs, whole call, us, by 1, 2 and 4 blocks to 16 columns: 2048 columns of 6 experts 26.6, 31.1, 45.5; 768 of 8 tokens' 8 experts 23.8, 20.6, 24.0
+  int split = 1;
+  while (split < 4 && C / 16 * split * 2 <= mlb_sm_count()) split *= 2;
+  return split == 1 ? launch_few_out<1>(b, g, st) : split == 2 ? launch_few_out<2>(b, g, st) : launch_few_out<4>(b, g, st);
 }
