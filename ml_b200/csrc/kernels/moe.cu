@@ -900,7 +900,7 @@ __global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(FEW_THREADS, 1) 
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ FewLists L;
   __shared__ uint64_t full[FEW_WARPS][FEW_STAGES];
-  __shared__ float weight[FEW_COPIES], part[FEW_WARPS][8][16], sums[FEW_WARPS][FEW_TOKENS][16], from[2][SPLIT][FEW_TOKENS * 16];
+  __shared__ float weight[FEW_COPIES], part[FEW_WARPS][8][16], sums[FEW_WARPS][FEW_TOKENS][16], from[SPLIT][FEW_TOKENS * 16];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rank = SPLIT > 1 ? (int)tc::cluster_ctarank() : 0;
   // The kernel before is that for h, which has waited for all before it: idx and the weights stand, and only h has to be waited for.  (Past the L1, of which nothing is known so early.)
   if (tid < A.N * A.k) weight[tid] = A.wbits == 32 ? __ldcg((const float*)A.weights + tid) : __uint_as_float((uint32_t)__ldcg((const unsigned short*)A.weights + tid) << 16);
@@ -936,8 +936,7 @@ __global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(FEW_THREADS, 1) 
     few_tokens(ahead, A.h + (size_t)c * A.I, i - a * steps, K, t);
   };
   if (begin < end) tokens(begin);
-  int turn = 0;
-  for (int g = blockIdx.x / SPLIT; g < groups; g += every, turn ^= 1) {
+  for (int g = blockIdx.x / SPLIT; g < groups; g += every) {
     for (int i = lane; i < FEW_TOKENS * 16; i += 32) (&sums[w][0][0])[i] = 0.f;
     float d[2][4] = {};
     int a = begin / steps, s = begin - a * steps;
@@ -973,13 +972,13 @@ __global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(FEW_THREADS, 1) 
     if (tid < FEW_TOKENS * 16) {
 #pragma unroll
       for (int i = 0; i < FEW_WARPS; i++) sum += (&sums[i][0][0])[tid];
-      if (SPLIT > 1 && rank != 0) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(tc::mapa_u32(tc::smem_u32(&from[turn][rank][tid]), 0)), "f"(sum) : "memory");
+      if (SPLIT > 1 && rank != 0) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(tc::mapa_u32(tc::smem_u32(&from[rank][tid]), 0)), "f"(sum) : "memory");
     }
-    if (SPLIT > 1) tc::cluster_sync();      // (two places in turn: whoever writes to one again has met the first block behind its reading of it)
+    if (SPLIT > 1) tc::cluster_sync();      // (where blocks share columns each has one turn: `from` is not written again)
     else __syncthreads();
     if (rank == 0 && tid < 16 * A.N) {
 #pragma unroll
-      for (int i = 1; i < SPLIT; i++) sum += from[turn][i][tid];
+      for (int i = 1; i < SPLIT; i++) sum += from[i][tid];
       A.out[(size_t)(tid / 16) * A.C + g * 16 + tid % 16] = __float2bfloat16(sum);
     }
   }
@@ -1004,7 +1003,7 @@ int launch_few_out(const CUtensorMap& m, const FewArgs& g, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = mlb_allow_smem(moe_few_out_k<SPLIT>, FEW_SMEM, done);
   if (e != cudaSuccess) return (int)e;
-  return (int)mlb_launch(moe_few_out_k<SPLIT>, dim3(SPLIT * std::min(g.C / 16, mlb_sm_count() / SPLIT)), dim3(FEW_THREADS), (size_t)FEW_SMEM, st, m, g);
+  return (int)mlb_launch(moe_few_out_k<SPLIT>, dim3(SPLIT > 1 ? SPLIT * (g.C / 16) : std::min(g.C / 16, mlb_sm_count())), dim3(FEW_THREADS), (size_t)FEW_SMEM, st, m, g);
 }
 
 struct Maps { CUtensorMap a, b, b16, a1, b1, a2, b2, out, out1, out2; };

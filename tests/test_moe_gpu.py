@@ -290,7 +290,7 @@ def test_few_tokens_with_an_expert_many_times(N, E, k):
 
 
 @pytest.mark.parametrize("N", [1, 2, 7, 8, 9, 33])
-@pytest.mark.parametrize("C,I,E,k", [(16, 16, 4, 2), (80, 528, 12, 3), (1040, 96, 6, 1), (2048, 1376, 16, 6), (256, 2816, 2, 2)])
+@pytest.mark.parametrize("C,I,E,k", [(16, 16, 4, 2), (80, 528, 12, 3), (1040, 96, 6, 1), (2048, 1376, 16, 6), (256, 2816, 2, 2), (4112, 64, 9, 4)])
 def test_few_tokens(N, C, I, E, k):
     """The form for few tokens, and the first number of tokens for the other one: sizes that end inside a stage, a warp's and a thread block's share, and leave some without any."""
     x, w, idx, gate_up, down = experts(N, E, k, C, I, F32, drop=N // 4)
