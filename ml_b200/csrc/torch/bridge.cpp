@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -427,6 +428,19 @@ Routed route_forward(const Tensor& logits, const Tensor& bias, const Routing& r)
         "moe_route");
   return out;
 }
+// Gradients from kernels that have none themselves: they raise where they are differentiated again
+variable_list first_order(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list there;
+  for (const Tensor& g : grads)
+    if (g.defined()) there.push_back(g.detach().set_requires_grad(true));
+  const auto n = (int64_t)there.size();
+  there = torch::autograd::DelayedError("routing and experts have no second derivative", n).apply(std::move(there));
+  auto next = there.begin();
+  for (Tensor& g : grads)
+    if (g.defined()) g = *next++;
+  return grads;
+}
 struct RouteFn : torch::autograd::Function<RouteFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Maybe& bias, int64_t k, int64_t sigmoid, int64_t groups, int64_t top, int64_t renorm, int64_t wide, double scale) {
     const Routing r{(int)k, (int)sigmoid, (int)groups, (int)top, (int)renorm, (int)wide, scale};
@@ -453,7 +467,7 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
     check(K.mlb_moe_route_bwd(none[0].data_ptr(), dw.data_ptr(), dm.defined() ? (const float*)dm.data_ptr() : nullptr, z.data_ptr(), (const int*)idx.data_ptr(), N, E, (int)E, (int)k, (int)how[3],
                               (int)how[4], (float)ctx->saved_data["scale"].toDouble(), bits(z), bits(dw), stream()),
           "moe_route_bwd");
-    return none;
+    return first_order(none);
   }
 };
 struct Experts { Tensor x, weights, idx, gate_up, down; };
@@ -503,7 +517,7 @@ struct ExpertsFn : torch::autograd::Function<ExpertsFn> {
     check(K.mlb_moe_bwd(at_(dx), dw.data_ptr(), at_(dgate_up), at_(ddown), ys.data_ptr(), dgu.data_ptr(), dxs.data_ptr(), dout.data_ptr(), xs.data_ptr(), gu.data_ptr(), h.data_ptr(),
                         y.data_ptr(), w.data_ptr(), gate_up.data_ptr(), down.data_ptr(), (const int*)plan.data_ptr(), N, C, (int)k, (int)E, (int)C, (int)I, bits(w), stream()),
           "moe_mlp_bwd");
-    return {dx, ctx->needs_input_grad(1) ? dw : Tensor(), Tensor(), dgate_up, ddown};
+    return first_order({dx, ctx->needs_input_grad(1) ? dw : Tensor(), Tensor(), dgate_up, ddown});
   }
 };
 

@@ -9,7 +9,6 @@ backward kernels need.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -211,6 +210,23 @@ def _rows_of(x):
     return x.contiguous() if not x.is_contiguous() or x.data_ptr() % 16 == 0 else x.clone()
 
 
+def _first_order(backward):
+    """A backward pass on kernels that have none themselves: what it gives raises where it is differentiated again."""
+
+    def run(ctx, *grads):
+        again = torch.is_grad_enabled()
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        there = [t for t in out if t is not None]
+        if not again or not there:
+            return out
+        back = torch._C._functions.DelayedError(b"routing and experts have no second derivative", len(there))(*[t.detach().requires_grad_() for t in there])
+        back = iter((back,) if torch.is_tensor(back) else back)
+        return tuple(None if t is None else next(back) for t in out)
+
+    return run
+
+
 class MoERoute(torch.autograd.Function):
     """logits [N, E] -> weights [N, k], idx int32 [N, k], mean fp32 [E] (ops/ref_moe.py has what they are).  The choice has no gradient, and neither has the bias."""
 
@@ -229,7 +245,7 @@ class MoERoute(torch.autograd.Function):
         return weights, idx, mean
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dweights, _, dmean):
         logits, idx = ctx.saved_tensors
         if dweights is None and dmean is None:
@@ -252,7 +268,7 @@ class MoEMLP(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         x, weights, idx, gate_up, down, *saved = ctx.saved_tensors
         new = lambda t, wanted=True: torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None

@@ -242,3 +242,15 @@ def test_decoder_with_experts_trains():
             p[at] += d
             both.append(float(m(ids, torch.roll(ids, -1))))
     assert abs((both[0] - both[1]) / 2e-2 - float(p.grad[at])) < 1e-3
+
+
+def test_there_is_no_second_derivative():
+    torch.manual_seed(0)
+    x, w, idx = torch.randn(6, 8, requires_grad=True), torch.rand(6, 2, requires_grad=True), torch.randint(0, 3, (6, 2), dtype=torch.int32)
+    gate_up, down, z = torch.randn(3, 8, 8, requires_grad=True), torch.randn(3, 8, 4, requires_grad=True), torch.randn(6, 3, requires_grad=True)
+    for out, of in ((F.moe_mlp(x, w, idx, gate_up, down), [x, w, gate_up, down]), (F.moe_mlp(x, w, idx, gate_up, down), [x]), (F.moe_route(z, 2)[0], [z])):
+        dout = torch.randn_like(out)
+        plain, grads = (torch.autograd.grad(out, of, dout, retain_graph=True, create_graph=c) for c in (False, True))
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads)) and not any(g.requires_grad for g in plain)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            sum(g.square().sum() for g in grads).backward()

@@ -412,6 +412,21 @@ def test_any_of_the_gradients(which):
     close(first, want, sizes, [WHAT[1 + i] for i in which])
 
 
+@pytest.mark.parametrize("extension", [True, False])
+def test_there_is_no_second_derivative(extension):
+    x, w, idx, gate_up, down = experts(20, 4, 2, 64, 48)
+    z = torch.randn(20, 4, device=dev()).requires_grad_()
+    x.requires_grad_(), down.requires_grad_()
+    y = F.moe_mlp(x, w, idx, gate_up, down) if extension else F.MoEMLP.apply(x, w, idx, gate_up, down)
+    p = F.moe_route(z, 2)[0] if extension else F.MoERoute.apply(z, 2, None, "softmax", 1, 1, True, 1.0, F32)[0]
+    for out, of in ((y, [x, down]), (y, [x]), (p, [z])):
+        dout = torch.randn_like(out)
+        plain, grads = (torch.autograd.grad(out, of, dout, retain_graph=True, create_graph=c) for c in (False, True))
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            sum(g.float().square().sum() for g in grads).backward()
+
+
 @pytest.mark.parametrize("N", [3, 60])
 def test_negative_indices_of_any_size_are_none(N):
     x, w, idx, gate_up, down = experts(N, 4, 2, 64, 48, drop=2)
@@ -466,6 +481,53 @@ def test_experts_on_another_stream():
     ops.moe_mlp(ref, x, w, idx, gate_up, down)      # at the same time
     torch.cuda.synchronize()
     assert torch.equal(ref, out)
+
+
+@pytest.mark.parametrize("N", [1, 6, 200])
+def test_two_graphs_at_once(N):
+    """Two captured calls, each with its own inputs, replayed on two streams beside one another and an uncaptured call: no workspace is another's."""
+    calls = []
+    for seed in range(2):
+        torch.manual_seed(seed)
+        x, w, idx, gate_up, down = experts(N, 8, 2, 512, 768)
+        idx = (idx + seed) % 8
+        z = torch.randn(N, 8, device=dev())
+        outs = [torch.zeros_like(x), torch.zeros(N, 2, device=dev()), torch.zeros(N, 2, dtype=I32, device=dev()), torch.zeros(8, device=dev())]
+
+        def work(outs=outs, x=x, w=w, idx=idx, gate_up=gate_up, down=down, z=z):
+            ops.moe_mlp(outs[0], x, w, idx, gate_up, down)
+            ops.moe_route(outs[1], outs[2], outs[3], z, score="sigmoid", groups=4, top_groups=2)
+
+        work()
+        want = [t.clone() for t in outs]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(8):
+                work()
+        calls.append((work, graph, outs, want, torch.cuda.Stream()))
+    for _, _, outs, _, _ in calls:
+        for t in outs:
+            t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for _, graph, _, _, stream in calls:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        mine = [torch.zeros_like(t) for t in calls[0][2]]
+        calls[0][0](mine)
+        assert all(torch.equal(a, b) for a, b in zip(mine, calls[0][3]))
+    torch.cuda.synchronize()
+    for _, _, outs, want, _ in calls:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("N", [1, 8, 100])
+def test_the_output_in_the_tokens_place(N):
+    x, w, idx, gate_up, down = experts(N, 4, 2, 320, 64)
+    out = torch.empty_like(x)
+    ops.moe_mlp(out, x, w, idx, gate_up, down)
+    ops.moe_mlp(x, x, w, idx, gate_up, down)
+    assert torch.equal(out, x)
 
 
 def test_a_token_costs_the_same_bits_in_any_batch_of_the_kind():
