@@ -620,6 +620,11 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
           uint8_t* place = MODE == DOWN_T ? buf + S::PLACES * S::PLACE : staging + half * (4 * S::WARP_BYTES) + (n & 1) * (2 * S::WARP_BYTES);
           const uint32_t splace = tc::smem_u32(place);
           uint32_t r[2][CHUNK / 2];
+          if constexpr (MODE == DOWN_T) {
+            if (lane == 0) tc::tma_wait_group_read<0>();      // the chunk before has left its place: the next one may arrive there
+            __syncwarp();
+            ask();
+          }
           tc::tmem_ld_frag_wait(taddr + c, r);
           if constexpr (MODE != DOWN_T) {
             // what left two chunks ago has been read, its place is free; before the first chunk so have weight gradients' rows, which had all places
@@ -670,9 +675,6 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
               swiglu_bwd8(x[i][0], x[i][1], x[i][2]);
               if (c + 8 * i + tok >= w.rows) x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);      // (rows that fill up an expert's: zeros, whatever stands in them)
             }
-            if (lane == 0) tc::tma_wait_group_read<0>();      // the chunk before has left its place: the next one may arrive there
-            __syncwarp();
-            ask();
 #pragma unroll
             for (int i = 0; i < CHUNK / 8; i++) {
               const int t = 8 * i + tok, sw = t & 7;
