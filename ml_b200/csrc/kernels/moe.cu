@@ -319,7 +319,7 @@ struct Smem {
   static constexpr int EPI = MODE == DOWN_T ? 16 : 8, THREADS = 64 + 32 * EPI;      // epilogue warps
   static constexpr int CHUNK = MODE == DOWN_T ? 16 : 32;
   static constexpr int A_BYTES = 128 * BK * 2, STAGE_BYTES = 2 * A_BYTES, STAGES = MODE == DOWN_T ? 4 : MODE == GATE_UP ? 5 : 6;
-  static constexpr int PLACES = 2, PLACE = 128 * CHUNK, WARP_BYTES = MODE == DOWN_T ? PLACES * PLACE + PLACE / 2 : MODE == GATE_UP ? 2 * 2048 + 2 * 1024 : 4096;
+  static constexpr int PLACES = 3, PLACE = 128 * CHUNK, WARP_BYTES = MODE == DOWN_T ? PLACES * PLACE : MODE == GATE_UP ? 2 * 2048 + 2 * 1024 : 4096;
   static constexpr int TOTAL = STAGES * STAGE_BYTES + EPI * WARP_BYTES + 512 + 1024;
   static_assert(WARP_BYTES % 1024 == 0 && TOTAL <= 232448, "shared memory of an SM");
 };
@@ -386,9 +386,8 @@ __device__ __forceinline__ void put_rows(uint8_t* buf, int lane, const uint32_t 
     *reinterpret_cast<uint4*>(rowp + ((v ^ (lane & 7)) << 4)) = pk;
   }
 }
-// Unit u (8 features) of token t in rows of 128 bytes, swizzled as TMA has them, and in rows of 64
+// Unit u (8 features) of token t in rows of 128 bytes, swizzled as TMA has them
 __device__ __forceinline__ int wide_at(int t, int u) { return t * 128 + ((u ^ (t & 7)) << 4); }
-__device__ __forceinline__ int unit_at(int t, int u) { return t * 64 + ((u ^ ((t >> 1) & 3)) << 4); }
 
 // Two fp32 values an instruction
 typedef uint64_t Two;
@@ -431,19 +430,11 @@ __device__ __forceinline__ Two sigmoid2(Two g) {
 }
 __device__ __forceinline__ Two swiglu2(Two g, Two u) { return mul2(mul2(g, sigmoid2(g)), u); }
 
-// SwiGLU's gradient, 8 neighbouring features of a row.  With s = sigmoid(g) and d = dh:  dg = d u s (1 + g (1 - s)),  du = d g s
-__device__ __forceinline__ void swiglu_bwd8(uint4& g4, uint4& u4, const uint4& d4) {
-  const uint32_t gq[4] = {g4.x, g4.y, g4.z, g4.w}, uq[4] = {u4.x, u4.y, u4.z, u4.w}, dq[4] = {d4.x, d4.y, d4.z, d4.w};
-  uint32_t a[4], b[4];
-  const Two one = two(1.f, 1.f), minus = two(-1.f, -1.f);
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const Two g = two_bf16(gq[i]), u = two_bf16(uq[i]), d = two_bf16(dq[i]);
-    const Two s = sigmoid2(g), silu = mul2(g, s);
-    a[i] = pack_two(mul2(mul2(d, u), fma2(silu, fma2(s, minus, one), s)));
-    b[i] = pack_two(mul2(d, silu));
-  }
-  g4 = make_uint4(a[0], a[1], a[2], a[3]), u4 = make_uint4(b[0], b[1], b[2], b[3]);
+// SwiGLU's gradient, one feature of two tokens.  With s = sigmoid(g) and d = dh:  dg = d u s (1 + g (1 - s)),  du = d g s
+__device__ __forceinline__ void swiglu_bwd2(uint32_t& gq, uint32_t& uq, Two d) {
+  const Two g = two_bf16(gq), u = two_bf16(uq), s = sigmoid2(g), silu = mul2(g, s);
+  gq = pack_two(mul2(mul2(d, u), fma2(silu, fma2(s, two(-1.f, -1.f), two(1.f, 1.f)), s)));
+  uq = pack_two(mul2(d, silu));
 }
 
 template <int MODE>
@@ -568,7 +559,6 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
     // barriers none of them leaves by itself: after a wait that ran out they go on without waiting, and nothing is stored.
     const int lg = warp & 3, half = (warp - 2) >> 2;
     uint8_t* buf = staging + (warp - 2) * S::WARP_BYTES;
-    const int tok = (lane >> 4) | (lane >> 1 & 6), unit = lane & 3;      // of four tokens 8 i + tok this lane has features m0 + 8 unit ... (tokens in an order that spares banks)
     int it = 0, n = 0;      // items that had products; chunks of 32 tokens
     bool ok = true;
     Items<MODE> items(g, cid, ncl);
@@ -598,7 +588,7 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
     };
     if constexpr (MODE == DOWN_T) {
       advance();
-      ask();
+      for (int i = 1; i < S::PLACES; i++) ask();
     }
     while ((MODE != DOWN_T || ok) && items.next(w)) {
       const bool grad = MODE == BACK && w.type != TOKENS;
@@ -617,7 +607,7 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
         const int last = (w.rows + 31) & ~31;      // (what fills up an expert's rows belongs to it)
         for (int c = half * CHUNK; c < last; c += PASS) {
           if (MODE == DOWN_T ? !live : m0 - lg * 32 >= g.M) break;      // (the four warps')
-          uint8_t* place = MODE == DOWN_T ? buf + S::PLACES * S::PLACE : staging + half * (4 * S::WARP_BYTES) + (n & 1) * (2 * S::WARP_BYTES);
+          uint8_t* place = MODE == DOWN_T ? buf + n % S::PLACES * S::PLACE : staging + half * (4 * S::WARP_BYTES) + (n & 1) * (2 * S::WARP_BYTES);
           const uint32_t splace = tc::smem_u32(place);
           uint32_t r[2][CHUNK / 2];
           if constexpr (MODE == DOWN_T) {
@@ -636,14 +626,14 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
             meet();
           }
           // r[h][4 j + 2 v + x]: token 8 j + 2 (lane % 4) + x of feature 16 h + 8 v + lane / 4
-          if (MODE != GATE_UP || g.out != nullptr) {
+          if (MODE != DOWN_T && (MODE != GATE_UP || g.out != nullptr)) {
 #pragma unroll
             for (int j = 0; j < CHUNK / 8; j++) {
               uint32_t p[4];
 #pragma unroll
               for (int q = 0; q < 4; q++) p[q] = pack_bf16(__uint_as_float(r[q >> 1][4 * j + 2 * (q & 1)]), __uint_as_float(r[q >> 1][4 * j + 2 * (q & 1) + 1]));
               const int t = 8 * j + (lane & 7), u = lane >> 3;
-              tc::stmatrix_x4_trans(splace + (MODE == DOWN_T ? unit_at(t, u) : (lg >> 1) * 4096 + wide_at(t, (lg & 1) * 4 + u)), p[0], p[1], p[2], p[3]);
+              tc::stmatrix_x4_trans(splace + (lg >> 1) * 4096 + wide_at(t, (lg & 1) * 4 + u), p[0], p[1], p[2], p[3]);
             }
           }
           if constexpr (MODE == GATE_UP) {      // feature 8 v + lane / 4: h = 0 its gate, h = 1 its up value
@@ -657,34 +647,27 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
               tc::stmatrix_x4_trans(splace + 8192 + wide_at(t, lg * 2 + u), x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
             }
           } else if constexpr (MODE == DOWN_T) {
-            uint8_t* gu = buf + n % S::PLACES * S::PLACE;
-            __syncwarp();
             if (!__all_sync(0xffffffffu, tc::mbar_wait(&place_full[(warp - 2) * S::PLACES + n % S::PLACES], (n / S::PLACES) & 1, 0x75))) { ok = false; break; }
-            const int ch = (unit >> 1) * 4 + (unit & 1);      // 16-byte unit of the gate's features in a row of [16 gate | 16 up | 16 gate | 16 up]
-            // (all loads before the first store: behind one they would be waited for a token at a time)
-            uint4 x[CHUNK / 8][3];
+            const int t = 8 * (lane >> 4) + (lane & 7), v = (lane >> 3) & 1;      // rows of [16 gate | 16 up | 16 gate | 16 up]; matrices of 8 tokens x 8 features, which is how the accumulators lie
+            uint32_t gate[2][4], up[2][4];
 #pragma unroll
-            for (int i = 0; i < CHUNK / 8; i++) {
-              const int t = 8 * i + tok, sw = t & 7;
-              x[i][0] = *reinterpret_cast<const uint4*>(gu + t * 128 + ((ch ^ sw) << 4));
-              x[i][1] = *reinterpret_cast<const uint4*>(gu + t * 128 + (((ch + 2) ^ sw) << 4));
-              x[i][2] = *reinterpret_cast<const uint4*>(place + unit_at(t, unit));
-            }
+            for (int h = 0; h < 2; h++) tc::ldmatrix_x4_trans(splace + wide_at(t, 4 * h + v), gate[h]), tc::ldmatrix_x4_trans(splace + wide_at(t, 4 * h + 2 + v), up[h]);
 #pragma unroll
-            for (int i = 0; i < CHUNK / 8; i++) {
-              swiglu_bwd8(x[i][0], x[i][1], x[i][2]);
-              if (c + 8 * i + tok >= w.rows) x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);      // (rows that fill up an expert's: zeros, whatever stands in them)
-            }
+            for (int h = 0; h < 2; h++) {
 #pragma unroll
-            for (int i = 0; i < CHUNK / 8; i++) {
-              const int t = 8 * i + tok, sw = t & 7;
-              *reinterpret_cast<uint4*>(gu + t * 128 + ((ch ^ sw) << 4)) = x[i][0];
-              *reinterpret_cast<uint4*>(gu + t * 128 + (((ch + 2) ^ sw) << 4)) = x[i][1];
+              for (int q = 0; q < 4; q++) {
+                swiglu_bwd2(gate[h][q], up[h][q], two(__uint_as_float(r[h][2 * q]), __uint_as_float(r[h][2 * q + 1])));
+                const int left = w.rows - (c + 8 * (q >> 1) + 2 * (lane & 3));      // (rows that fill up an expert's: zeros, whatever stands in them)
+                const uint32_t keep = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+                gate[h][q] &= keep, up[h][q] &= keep;
+              }
+              tc::stmatrix_x4_trans(splace + wide_at(t, 4 * h + v), gate[h][0], gate[h][1], gate[h][2], gate[h][3]);
+              tc::stmatrix_x4_trans(splace + wide_at(t, 4 * h + 2 + v), up[h][0], up[h][1], up[h][2], up[h][3]);
             }
             tc::fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tc::tma_store_2d(&tmOut, gu, 2 * m0, w.row0 + c);
+              tc::tma_store_2d(&tmOut, place, 2 * m0, w.row0 + c);
               tc::tma_commit_group();
             }
           }
