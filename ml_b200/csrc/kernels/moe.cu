@@ -318,8 +318,8 @@ template <int MODE>
 struct Smem {
   static constexpr int EPI = MODE == DOWN_T ? 16 : 8, THREADS = 64 + 32 * EPI;      // epilogue warps
   static constexpr int CHUNK = MODE == DOWN_T ? 16 : 32;
-  static constexpr int A_BYTES = 128 * BK * 2, STAGE_BYTES = 2 * A_BYTES, STAGES = MODE == DOWN_T ? 4 : MODE == GATE_UP ? 5 : 6;
-  static constexpr int PLACES = 3, PLACE = 128 * CHUNK, WARP_BYTES = MODE == DOWN_T ? PLACES * PLACE : MODE == GATE_UP ? 2 * 2048 + 2 * 1024 : 4096;
+  static constexpr int A_BYTES = 128 * BK * 2, STAGE_BYTES = 2 * A_BYTES, STAGES = MODE == DOWN_T || MODE == GATE_UP ? 5 : 6;
+  static constexpr int PLACES = 2, PLACE = 128 * CHUNK, WARP_BYTES = MODE == DOWN_T ? PLACES * PLACE : MODE == GATE_UP ? 2 * 2048 + 2 * 1024 : 4096;
   static constexpr int TOTAL = STAGES * STAGE_BYTES + EPI * WARP_BYTES + 512 + 1024;
   static_assert(WARP_BYTES % 1024 == 0 && TOTAL <= 232448, "shared memory of an SM");
 };
