@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(256) moe_combine_k(bf16* __restrict__ out, con
 // each CTA stages its 128 rows of A and its half of B and drains its own 128 tensor-memory lanes.  The weights are A and the tokens B, whose number
 // an instruction takes in steps of 32: an expert's last tile, and that of an expert with few tokens, is no wider than its rows.  Two accumulators, so that a tile's
 // epilogue runs under the next one's products.
-//   GATE_UP  [g | u] = xs Wgu^T, kept for backward or not, and h = silu(g) u
+//   GATE_UP  [g | u] = xs Wgu^T and h = silu(g) u;  H  the same, of which only h is kept
 //   DOWN     y = h Wd^T
 //   DOWN_T   dh = ys Wd, and from it dgu
 //   BACK     dWgu, dWd and dxs = dgu Wgu, one launch: tiles of all three behind one another, so that only one last wave leaves SMs idle
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(256) moe_combine_k(bf16* __restrict__ out, con
 //   DOWN      82 (1.26)   134 (1.03)
 //   DOWN_T   132 (0.78)   170 (0.82)      memory: 573 MB in the first, 4.3 TB/s
 //   BACK     356 (1.45)   668 (1.04)      1.08 GB of weight gradients in the second
-enum { GATE_UP, DOWN, DOWN_T, BACK };
+enum { GATE_UP, DOWN, DOWN_T, BACK, H };
 constexpr int BK = 64;
 // An epilogue warp has 32 features, of CHUNK tokens at a time.  GATE_UP, DOWN and BACK: four warps have the same tokens and put what leaves side by side, rows of 128 bytes in boxes of
 // 4 KB (two, and one of h), two places in turn; by itself a warp would have rows of 64 bytes, and of 32 of h, which the L2 takes as slowly as whole ones (GATE_UP, 16384 tokens to
@@ -319,7 +319,7 @@ struct Smem {
   static constexpr int EPI = MODE == DOWN_T ? 16 : 8, THREADS = 64 + 32 * EPI;      // epilogue warps
   static constexpr int CHUNK = MODE == DOWN_T ? 16 : 32;
   static constexpr int A_BYTES = 128 * BK * 2, STAGE_BYTES = 2 * A_BYTES, STAGES = MODE == DOWN_T || MODE == GATE_UP ? 5 : 6;
-  static constexpr int PLACES = 2, PLACE = 128 * CHUNK, WARP_BYTES = MODE == DOWN_T ? PLACES * PLACE : MODE == GATE_UP ? 2 * 2048 + 2 * 1024 : 4096;
+  static constexpr int PLACES = 2, PLACE = 128 * CHUNK, WARP_BYTES = MODE == DOWN_T ? PLACES * PLACE : MODE == GATE_UP ? 2 * 2048 + 2 * 1024 : MODE == H ? 2 * 1024 : 4096;
   static constexpr int TOTAL = STAGES * STAGE_BYTES + EPI * WARP_BYTES + 512 + 1024;
   static_assert(WARP_BYTES % 1024 == 0 && TOTAL <= 232448, "shared memory of an SM");
 };
@@ -327,7 +327,7 @@ struct GemmArgs {
   const int *start, *order;      // rows of the experts [E + 1]; the experts, those with the most rows first
   const int4* tiles;
   const int* ntiles;
-  bf16 *out, *h;         // [R, M]; GATE_UP (whose out may be null): h [R, M / 2].  DOWN_T: dgu [R, 2 M].  BACK: dxs
+  bf16 *out, *h;         // [R, M]; GATE_UP, H (which has no out): h [R, M / 2].  DOWN_T: dgu [R, 2 M].  BACK: dxs
   int E, M, K, tiles_m;  // token products: M features over K
   // BACK
   int C, I, per_gate_up, per_down;      // tiles of one expert (0: not asked for)
@@ -500,7 +500,7 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
             for (int c = 0; c < 2; c++) tc::tma_load_2d_pair(sA + c * 8192, a, bar, m0 + c * 64, y);
             for (int c = 0; c < 2; c++) tc::tma_load_2d_pair(sB + c * 8192, b, bar, n0 + c * 64, y);
           } else {
-            if (MODE == GATE_UP) {      // rows in groups of 16 gate rows and the matching 16 up rows
+            if (MODE == GATE_UP || MODE == H) {      // rows in groups of 16 gate rows and the matching 16 up rows
               tc::tma_load_5d_pair(sA, &tmA, bar, kb * BK, 0, 0, m0 / 32, w.e);
             } else if (MODE == DOWN) {
               tc::tma_load_3d_pair(sA, &tmA, bar, kb * BK, m0, w.e);
@@ -626,7 +626,7 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
             meet();
           }
           // r[h][4 j + 2 v + x]: token 8 j + 2 (lane % 4) + x of feature 16 h + 8 v + lane / 4
-          if (MODE != DOWN_T && (MODE != GATE_UP || g.out != nullptr)) {
+          if (MODE != DOWN_T && MODE != H) {
 #pragma unroll
             for (int j = 0; j < CHUNK / 8; j++) {
               uint32_t p[4];
@@ -636,7 +636,8 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
               tc::stmatrix_x4_trans(splace + (lg >> 1) * 4096 + wide_at(t, (lg & 1) * 4 + u), p[0], p[1], p[2], p[3]);
             }
           }
-          if constexpr (MODE == GATE_UP) {      // feature 8 v + lane / 4: h = 0 its gate, h = 1 its up value
+          uint8_t* hs = place + (MODE == GATE_UP ? 8192 : 0);
+          if constexpr (MODE == GATE_UP || MODE == H) {      // feature 8 v + lane / 4: h = 0 its gate, h = 1 its up value
             uint32_t x[8];
 #pragma unroll
             for (int q = 0; q < 8; q++)
@@ -644,7 +645,7 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
 #pragma unroll
             for (int j = 0; j < 2; j++) {
               const int t = 16 * j + 8 * (lane >> 4) + (lane & 7), u = (lane >> 3) & 1;
-              tc::stmatrix_x4_trans(splace + 8192 + wide_at(t, lg * 2 + u), x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+              tc::stmatrix_x4_trans(tc::smem_u32(hs) + wide_at(t, lg * 2 + u), x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
             }
           } else if constexpr (MODE == DOWN_T) {
             if (!__all_sync(0xffffffffu, tc::mbar_wait(&place_full[(warp - 2) * S::PLACES + n % S::PLACES], (n / S::PLACES) & 1, 0x75))) { ok = false; break; }
@@ -675,9 +676,9 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
             tc::fence_async_smem();
             meet();
             if (ok && lg == 0 && lane == 0) {
-              if (MODE != GATE_UP || g.out != nullptr)
+              if (MODE != H)
                 for (int i = 0; i < 2 && m0 + 64 * i < g.M; i++) tc::tma_store_2d(&tmOut, place + 4096 * i, m0 + 64 * i, w.row0 + c);
-              if (MODE == GATE_UP) tc::tma_store_2d(&tmB1, place + 8192, m0 / 2, w.row0 + c);
+              if (MODE == GATE_UP || MODE == H) tc::tma_store_2d(&tmB1, hs, m0 / 2, w.row0 + c);
               tc::tma_commit_group();
             }
           }
@@ -1117,7 +1118,7 @@ MLB_API int mlb_moe_fwd(void* out, void* xs, void* gu, void* h, void* y, const v
   if (!map_gate_up(&m.a, (const bf16*)gate_up, E, C, I, 4) || !map_tokens(m, (const bf16*)xs, z.p.rows, C) || !map_chunk(&m.b1, g.h, z.p.rows, I, 64) ||
       (g.out != nullptr && !map_chunk(&m.out, g.out, z.p.rows, 2 * I, 64)))
     return -2;
-  MLB_TRY(launch_gemm<GATE_UP>(m, g, (long)z.p.max_tiles * g.tiles_m, st));
+  MLB_TRY(gu != nullptr ? launch_gemm<GATE_UP>(m, g, (long)z.p.max_tiles * g.tiles_m, st) : launch_gemm<H>(m, g, (long)z.p.max_tiles * g.tiles_m, st));
   g.out = (bf16*)y, g.h = nullptr, g.M = C, g.K = I, g.tiles_m = (C + 255) / 256;
   if (!map_down(&m.a, (const bf16*)down, E, C, I, 128) || !map_tokens(m, (const bf16*)h, z.p.rows, I) || !map_chunk(&m.out, g.out, z.p.rows, C, 64)) return -2;
   MLB_TRY(launch_gemm<DOWN>(m, g, (long)z.p.max_tiles * g.tiles_m, st));
