@@ -8,7 +8,7 @@
 //   backward   ys = rows of w dout, dw = dout . y;  dh = ys Wd and from it dgu;  dxs = dgu Wgu, dx = sums of it;  dWgu = dgu^T xs;  dWd = ys^T h
 // Of the forward pass xs, [g | u], h and y are kept: with h and y the gradient of a weight and that of Wd need neither SwiGLU again nor a second set of rows.
 // Rounded to bf16 on the way, all sums being fp32: h, ys and dgu, which the tensor cores take in no wider form that is as fast; [g | u], from whose rounded values backward forms
-// the gradient again; y and dxs, which in fp32 would be 50 MB more to write and to read each at 16384 x 2 copies of 768 (some 15 us).  Outputs are 0.0029, gradients 0.0042 of their norm from
+// the gradient again; y and dxs, which in fp32 would be 50 MB more to write and to read each at 16384 x 2 copies of 768 (some 15 us).  Outputs are 0.0029, gradients 0.0039 of their norm from
 // 64 bits, of which the last rounding is 0.0017.
 // Counts are known on the device only: grids are sized by what there may be at most, and blocks that find nothing leave.
 #include "../tc.cuh"
@@ -306,14 +306,14 @@ __global__ void __launch_bounds__(256) moe_combine_k(bf16* __restrict__ out, con
 // us (PFLOP/s) with 16384 tokens to 2 of 8 experts of 2048 behind 768 columns, and with 4096 to 6 of 64 of 1376 behind 2048, whose rows are 1 to 2900:
 //   GATE_UP  152 (1.36)   248 (1.12)      a tile's operands are 62 bytes a clock and SM from the L2, all that it gives; what is stored and few rows to a tile come on top
 //   DOWN      82 (1.26)   134 (1.03)
-//   DOWN_T   132 (0.78)   170 (0.82)      memory: 573 MB in the first, 4.3 TB/s
+//   DOWN_T   110 (0.94)   154 (0.90)      memory: 573 MB in the first, 5.2 TB/s
 //   BACK     356 (1.45)   668 (1.04)      1.08 GB of weight gradients in the second
 enum { GATE_UP, DOWN, DOWN_T, BACK, H };
 constexpr int BK = 64;
 // An epilogue warp has 32 features, of CHUNK tokens at a time.  GATE_UP, DOWN and BACK: four warps have the same tokens and put what leaves side by side, rows of 128 bytes in boxes of
 // 4 KB (two, and one of h), two places in turn; by itself a warp would have rows of 64 bytes, and of 32 of h, which the L2 takes as slowly as whole ones (GATE_UP, 16384 tokens to
-// 2 of 8 experts of 2048 behind 768 columns: 159 us, 126 with nothing stored, 149 so).  A weight gradient's rows: 4 KB a warp.  DOWN_T: two places for [g | u], which arrive, become
-// their gradients and leave, and one for dh, a warp.
+// 2 of 8 experts of 2048 behind 768 columns: 159 us, 126 with nothing stored, 149 so).  A weight gradient's rows: 4 KB a warp.  DOWN_T: two places a warp for [g | u], which arrive, become
+// their gradients where they stand and leave; what comes next is asked for before the arithmetic (132 us behind it, 116 so; with five stages of operands instead of four 110).
 template <int MODE>
 struct Smem {
   static constexpr int EPI = MODE == DOWN_T ? 16 : 8, THREADS = 64 + 32 * EPI;      // epilogue warps
