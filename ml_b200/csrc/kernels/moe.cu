@@ -27,16 +27,17 @@ struct PlanShape {
   long rows, tiles, place, source, hist, total;      // R; offsets of the parts in ints
   int max_tiles, blocks, per_block;
 };
-// PLAN_BATCH: copies that a lane asks for at a time.  A block that has all copies to itself has 32 warps, whose copies go to their rows 32 at a time, one behind the other (1806 copies to 64
-// experts: 10.4 us with 8 warps, 8.7 with 32); where there are several, or more lists of counts than shared memory takes, it has 8 (16384 copies to 8 experts: 5.3 us, 6.4 with 32).
+// PLAN_BATCH: copies that a lane asks for at a time.  One block takes up to 2048 copies, with a run of 32 to 256 of them to each of its 8 warps, which put theirs in rows one 32 behind the other; of
+// more than 1024 it has 32 warps (32 copies to 8 experts: 4.7 us with 32 warps, 3.1 with 8; 1024 of 64: 6.6 and 5.7; 1806 of 64, by themselves: 8.7 and 10.4), unless there are more lists of
+// counts than shared memory takes.
 constexpr int PLAN_BATCH = 8;
-inline int plan_warps(int E, int blocks) { return E <= 256 && blocks == 1 ? 32 : 8; }
+inline int plan_warps(int E, long NK) { return E <= 256 && NK > 1024 && NK <= 2048 ? 32 : 8; }
 inline PlanShape plan_shape(long NK, int E) {
   PlanShape p;
-  const long used = NK < E ? NK : E;
+  const long used = NK < E ? NK : E, step = NK <= 2048 ? 32 * plan_warps(E, NK) : 1024;
   p.rows = (NK + (PAD - 1) * used) / PAD * PAD;
   p.max_tiles = (int)(NK / TILE_TOKENS + used);
-  p.per_block = NK <= 2048 ? 2048 : (int)std::max(1024L, ((NK + 127) / 128 + 1023) / 1024 * 1024);
+  p.per_block = (int)std::max(step, ((NK <= 2048 ? NK : (NK + 127) / 128) + step - 1) / step * step);
   p.blocks = (int)((NK + p.per_block - 1) / p.per_block);
   p.tiles = (2L * E + 2 + 3) / 4 * 4;
   p.place = p.tiles + 4L * p.max_tiles;
@@ -1100,7 +1101,7 @@ MLB_API int mlb_moe_plan(int* plan, const int* idx, long N, int k, int E, cudaSt
   if (z.NK == 0) return 0;
   const PlanArgs P = plan_args(plan, idx, z);
   if (z.p.blocks > 1) MLB_TRY((int)mlb_launch(moe_hist_k, dim3(z.p.blocks), dim3(256), (size_t)4 * E, st, P));
-  return (int)mlb_launch(moe_place_k, dim3(z.p.blocks), dim3(32 * plan_warps(E, z.p.blocks)), (size_t)4 * E * (2 + plan_warps(E, z.p.blocks)), st, P);
+  return (int)mlb_launch(moe_place_k, dim3(z.p.blocks), dim3(32 * plan_warps(E, z.NK)), (size_t)4 * E * (2 + plan_warps(E, z.NK)), st, P);
 }
 // xs [R, C], gu [R, 2 I] (null: not kept), h [R, I] and y [R, C] are workspace, and what backward needs
 MLB_API int mlb_moe_fwd(void* out, void* xs, void* gu, void* h, void* y, const void* x, const void* weights, const void* gate_up, const void* down, const int* plan, long N, long ldx, int k,
