@@ -43,7 +43,8 @@ __device__ __forceinline__ float sigmoid_fine(float z) {
   const float e = exp_fine(fmaxf(-fabsf(z), -200.f));
   return __fdividef(z >= 0.f ? 1.f : e, 1.f + e);      // (2 steps of 2^-23; the denominator is 1 to 2)
 }
-// The same to 2^-21 or so of itself (2 steps of ex2, 1 of rcp, and the product's rounding, which matters where the score is small), 0 for -inf: says what may be chosen
+// The same to (7 + 1.23 |z|) 2^-24 of itself below 0 (ex2 4, the sum 1, rcp 2; the product with log2 e is rounded, and so is log2 e: an exponent's error grows with it), 0 for -inf and
+// below 2^-126: says what may be chosen
 __device__ __forceinline__ float sigmoid_fast(float z) {
   float e, s;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.44269504f));
@@ -313,8 +314,9 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
       if constexpr (V >= 4) mine = choose_many<V>(key, A.k, lane, list);
       else mine = choose<V>(key, A.k, lane);
     } else {
-      // 32 bits say what may be chosen, 64 bits what is.  In 32 a score is off by less than 2^-21 of itself, or of 1/4 where it is smaller, score + bias by less than slack = 2^-20 of
-      // the row's largest score + |bias|.  (With 64 bits for the few tokens alone that 32 leave open, these wait some 10 us for code that no cache has.)
+      // 32 bits say what may be chosen, 64 bits what is.  In 32 score + bias is off by less than slack, in steps of 2^-24 of `size`, the row's largest score + |bias|, of which the addition
+      // is one.  An exponential of z - m has 7.  Sigmoids: of s |z| (1 - s) none is over size max(1.28, -m), so 8 + 1.23 max(1.28, -m) is all.  2^-124 stands for what is flushed to 0.
+      // (With 64 bits for the few tokens alone that 32 leave open, these wait some 10 us for code that no cache has.)
       float t[V], size = 0.f;
       const float inv = A.sigmoid || A.bias == nullptr ? 1.f : total > 0.f ? __fdividef(1.f, total) : 0.f;
 #pragma unroll
@@ -324,7 +326,8 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
         t[v] = z[v] == -INFINITY ? -INFINITY : fmaxf(s + b, -INFINITY);      // (NaN, of a bias: not there)
         if (z[v] > -INFINITY) size = fmaxf(size, s + fabsf(b));
       }
-      const float slack = 9.5367432e-7f * __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size)));
+      const float steps = A.sigmoid ? 16.f + 1.3f * fminf(fmaxf(-m, 0.f), 128.f) : 16.f;      // (below -128 all scores are 0)
+      const float slack = fmaf(5.9604645e-8f * steps, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))), 4.7019774e-38f);
       const bool single = A.sigmoid || A.bias == nullptr;      // own_number() has them
       bool sure = slack < 1e30f && m < INFINITY;
       if (A.groups > 1) {

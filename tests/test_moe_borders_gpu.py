@@ -1,0 +1,91 @@
+"""Routing on the GPU against its definition in 64 bits, all tokens at once: many tokens, and choices that lie next to a border."""
+import math
+
+import pytest
+import torch
+
+from ml_b200 import ops
+from ml_b200.ops import autograd as F
+
+pytestmark = pytest.mark.gpu
+BF16, F32, F64, I32 = torch.bfloat16, torch.float32, torch.float64, torch.int32
+NEG = -math.inf
+STEP = 2.0 ** -24      # half a step of fp32, relative
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+@pytest.fixture(autouse=True)
+def no_errors():
+    from ml_b200.ops import native
+    yield
+    torch.cuda.synchronize()
+    err = native.get_error()
+    native.clear_error()
+    assert err == 0, native.describe_error(err)
+
+
+def scores(z, score):
+    there = z > NEG
+    if score == "sigmoid":
+        return torch.where(there, 1 / (1 + torch.exp(-z)), 0.0)
+    m = z.amax(1, keepdim=True)
+    e = torch.where(there, torch.exp(z - torch.where(m > NEG, m, 0.0)), 0.0)
+    return e / e.sum(1, keepdim=True).clamp(min=1e-300)
+
+
+def chosen(z, k, bias=None, score="softmax", groups=1, top_groups=1):
+    """idx of logits in 64 bits without NaN"""
+    N, E = z.shape
+    t = z if bias is None and groups == 1 else scores(z, score) + (0.0 if bias is None else bias.double())
+    t = torch.where(z > NEG, t, NEG)
+    if groups > 1:
+        parts = t.view(N, groups, E // groups)
+        best = parts.sort(dim=2, descending=True).values[..., :2]
+        second = best[..., 1] if best.shape[2] > 1 else torch.full_like(best[..., 0], NEG)
+        of = best[..., 0] + torch.where(second > NEG, second, 0.0)
+        at = of.sort(dim=1, descending=True, stable=True).indices[:, :top_groups]
+        t = torch.where(torch.zeros_like(of, dtype=torch.bool).scatter_(1, at, True)[..., None], parts, NEG).view(N, E)
+    best, at = t.sort(dim=1, descending=True, stable=True)
+    return torch.where(best[:, :k] > NEG, at[:, :k], -1).to(I32)
+
+
+def routed(z, k, **how):
+    w, idx = torch.empty(len(z), k, device=dev()), torch.empty(len(z), k, dtype=I32, device=dev())
+    ops.moe_route(w, idx, None, z, **how)
+    return idx
+
+
+def same(idx, want):
+    wrong = (idx != want).any(1)
+    assert not bool(wrong.any()), (int(wrong.sum()), idx[wrong][:4].tolist(), want[wrong][:4].tolist())
+
+
+# ------------------------------------------------------------------ borders
+@pytest.mark.parametrize("level", [-2.0, -10.0, -30.0, -50.0, -80.0, -87.6, -95.0])
+@pytest.mark.parametrize("biased", [False, True])
+def test_groups_whose_sums_are_nearly_equal(level, biased):
+    """Sigmoids far below 0: a rounding of the logit's product with log2 e is |z| 2^-24 of the score, and below e^-87 there are no normal numbers.  Four groups' sums of two, a few 1e-6 apart."""
+    g = torch.Generator(device="cuda").manual_seed(int(-10 * level))
+    N, groups, size = 40000, 4, 4
+    a = level + 0.6 * torch.rand(N, groups, generator=g, device=dev(), dtype=F64)
+    both = 2.2 * math.exp(level + 0.6) * (1 + 3e-6 * torch.randn(N, groups, generator=g, device=dev(), dtype=F64))
+    z = torch.full((N, groups, size), level - 4.0, device=dev())
+    s = torch.sigmoid(a.float().double())
+    rest = (both - s).clamp(min=0.2 * both.min())
+    z[..., 1], z[..., 2] = a.float(), (torch.log(rest) - torch.log1p(-rest)).float()
+    z = z.view(N, groups * size)
+    bias = torch.zeros(groups * size, device=dev()) if biased else None
+    for top in (1, 2, 3):
+        how = dict(score="sigmoid", groups=groups, top_groups=top, bias=bias)
+        same(routed(z, 2, **how), chosen(z.double(), 2, **how))
+
+
+@pytest.mark.parametrize("level", [-30.0, -50.0, -87.6])
+def test_sigmoids_that_are_nearly_equal(level):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    z = level + 1e-4 * torch.randint(0, 3, (20000, 64), generator=g, device=dev()) + torch.randint(-2, 2, (20000, 64), generator=g, device=dev()).float() * abs(level) * 2.0 ** -23
+    how = dict(score="sigmoid", bias=torch.zeros(64, device=dev()))
+    same(routed(z, 6, **how), chosen(z.double(), 6, **how))
