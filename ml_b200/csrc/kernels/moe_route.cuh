@@ -315,8 +315,9 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
       else mine = choose<V>(key, A.k, lane);
     } else {
       // 32 bits say what may be chosen, 64 bits what is.  In 32 score + bias is off by less than slack, in steps of 2^-24 of `size`, the row's largest score + |bias|, of which the addition
-      // is one.  An exponential of z - m has 7.  Sigmoids: of s |z| (1 - s) none is over size max(1.28, -m), so 8 + 1.23 max(1.28, -m) is all.  2^-124 stands for what is flushed to 0.
-      // (With 64 bits for the few tokens alone that 32 leave open, these wait some 10 us for code that no cache has.)
+      // is one.  An exponential of z - m has 7, and where the sum does not cancel (softmax with a bias) as much in its terms, 4.5 for their arguments' roundings (on average, of 1024 terms at
+      // most), V + 4 for its additions, and 5 for the division and the product.  Sigmoids: of s |z| (1 - s) none is over size max(1.28, -m), so 8 + 1.23 max(1.28, -m) is all.
+      // 2^-124 stands for what is flushed to 0.  (With 64 bits for the few tokens alone that 32 leave open, these wait some 10 us for code that no cache has.)
       float t[V], size = 0.f;
       const float inv = A.sigmoid || A.bias == nullptr ? 1.f : total > 0.f ? __fdividef(1.f, total) : 0.f;
 #pragma unroll
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 4 ? 6 : V == 8 ? 4 : 2)
         t[v] = z[v] == -INFINITY ? -INFINITY : fmaxf(s + b, -INFINITY);      // (NaN, of a bias: not there)
         if (z[v] > -INFINITY) size = fmaxf(size, s + fabsf(b));
       }
-      const float steps = A.sigmoid ? 16.f + 1.3f * fminf(fmaxf(-m, 0.f), 128.f) : 16.f;      // (below -128 all scores are 0)
+      const float steps = A.sigmoid ? 16.f + 1.3f * fminf(fmaxf(-m, 0.f), 128.f) : A.bias != nullptr ? 32.f + V : 16.f;      // (below -128 all scores are 0)
       const float slack = fmaf(5.9604645e-8f * steps, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))), 4.7019774e-38f);
       const bool single = A.sigmoid || A.bias == nullptr;      // own_number() has them
       bool sure = slack < 1e30f && m < INFINITY;

@@ -89,3 +89,32 @@ def test_sigmoids_that_are_nearly_equal(level):
     z = level + 1e-4 * torch.randint(0, 3, (20000, 64), generator=g, device=dev()) + torch.randint(-2, 2, (20000, 64), generator=g, device=dev()).float() * abs(level) * 2.0 ** -23
     how = dict(score="sigmoid", bias=torch.zeros(64, device=dev()))
     same(routed(z, 6, **how), chosen(z.double(), 6, **how))
+
+
+@pytest.mark.parametrize("E", [512, 1024])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_softmax_with_a_bias_next_to_a_border(E, groups):
+    """An expert's number is all score and another's all but all bias, by one step of fp32 the larger, so that what a sum of exponentials has lost in 32 bits does not cancel: a lane's first
+    terms add up to a little over 1, and each of the others is less than half a step of that."""
+    g = torch.Generator().manual_seed(E + groups)
+    tiny, size = -16.64, E // groups
+    for v in (math.log(0.5) + 1e-4 + 2e-3 * torch.rand(1500, generator=g)).tolist():
+        z = torch.full((1, E), tiny)
+        z[0, 1:64], z[0, 0], z[0, 32] = v, 0.0, tiny
+        if groups > 1:                                                # the group's second as good as its first
+            z[0, 1], z[0, 33] = 0.0, tiny
+        p = torch.softmax(z.double(), 1)[0]
+        bias = torch.zeros(E)
+        if groups == 1:
+            bias[E - 1] = p[0] - p[E - 1]
+            at = [E - 1]
+        else:
+            bias[E - 1] = (p[0] + p[1] - p[E - 1] - p[E - 2]) / 2
+            bias[E - 2] = p[0] + p[1] - p[E - 1] - p[E - 2] - bias[E - 1].double()
+            at = [E - 2]
+        bias[at] = torch.nextafter(bias[at], torch.ones(1))
+        t = p + bias.double()
+        group = int(t.view(groups, size).sort(1, descending=True).values[:, :2].sum(1).argmax())
+        want = group * size + int(t.view(groups, size)[group].argmax()) if groups > 1 else int(t.argmax())
+        got = routed(z.to(dev()), 1, bias=bias.to(dev()), groups=groups, top_groups=1)
+        assert int(got) == want, (v, int(got), want)
