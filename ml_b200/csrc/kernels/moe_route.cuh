@@ -28,8 +28,18 @@ __host__ __device__ constexpr int own_doubles(int E) { return E > 32 ? E : 32; }
 template <typename T> __device__ __forceinline__ float logit(const T* z, int i);
 template <> __device__ __forceinline__ float logit<float>(const float* z, int i) { return __ldg(z + i); }
 template <> __device__ __forceinline__ float logit<bf16>(const bf16* z, int i) { return __bfloat162float(z[i]); }
-// (NaN -> -inf, -0 -> 0)
-__device__ __forceinline__ float seen(float z) { return fmaxf(z, -INFINITY) + 0.f; }
+// NaN -> -inf, -0 -> 0.  Numbers below the normal ones stay: these are compared, too, and the compiler's own instructions take them for 0.
+__device__ __forceinline__ float seen(float z) {
+  float r;
+  asm("max.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(-INFINITY));
+  asm("add.f32 %0, %0, %1;" : "+f"(r) : "f"(0.f));
+  return r;
+}
+__device__ __forceinline__ double wide(float v) {
+  double r;
+  asm("cvt.f64.f32 %0, %1;" : "=d"(r) : "f"(v));
+  return r;
+}
 // exp(x) for x <= 0 to a few 2^-24: the product with log2 e in two parts
 __device__ __forceinline__ float exp_fine(float x) {
   const float hi = x * 1.44269504f, lo = fmaf(x, 1.44269504f, -hi) + x * 1.92596299e-8f;
@@ -217,7 +227,7 @@ __device__ __noinline__ int choose_exact(const RouteArgs& A, const T* row, doubl
   for (int i = lane; i < E; i += 32) {
     const float z = seen(logit(row, i));
     const double t = A.sigmoid ? s[i] : all > 0 ? s[i] / all : 0.0;
-    s[i] = z == -INFINITY ? -INFINITY : A.bias != nullptr ? t + (double)__ldg(A.bias + i) : t;
+    s[i] = z == -INFINITY ? -INFINITY : A.bias != nullptr ? t + wide(__ldg(A.bias + i)) : t;
   }
   __syncwarp();
   unsigned stays = 0xffffffffu;
@@ -257,7 +267,7 @@ __device__ __noinline__ int choose_exact(const RouteArgs& A, const T* row, doubl
 template <typename T>
 __device__ __noinline__ double own_number(const RouteArgs& A, const T* row, int i, float m) {
   const double z = (double)seen(logit(row, i)), x = exp(A.sigmoid ? -z : z - (double)m);
-  return A.sigmoid ? 1.0 / (1.0 + x) + (A.bias != nullptr ? (double)__ldg(A.bias + i) : 0.0) : x;
+  return A.sigmoid ? 1.0 / (1.0 + x) + (A.bias != nullptr ? wide(__ldg(A.bias + i)) : 0.0) : x;
 }
 
 // PLAIN: by the logits alone

@@ -118,3 +118,20 @@ def test_softmax_with_a_bias_next_to_a_border(E, groups):
         want = group * size + int(t.view(groups, size)[group].argmax()) if groups > 1 else int(t.argmax())
         got = routed(z.to(dev()), 1, bias=bias.to(dev()), groups=groups, top_groups=1)
         assert int(got) == want, (v, int(got), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_logits_and_biases_below_the_normal_numbers(dtype):
+    z = torch.zeros(3, 40, device=dev())
+    z[0, 7], z[0, 30], z[0, 3] = 3e-39, 2e-39, -1e-39
+    z[1], z[1, 5], z[1, 20] = -2e-39, -1e-39, 1e-39
+    z[2, ::2] = -0.0
+    z = z.to(dtype)
+    same(routed(z, 3), chosen(z.double(), 3))
+    z = torch.full((2, 40), -95.0, device=dev(), dtype=dtype)
+    bias = torch.zeros(40, device=dev())
+    bias[9], bias[4], bias[30] = 3e-40, 2e-40, -1e-40
+    how = dict(score="sigmoid", bias=bias)
+    same(routed(z, 4, **how), chosen(z.double(), 4, **how))
+    how = dict(score="sigmoid", bias=bias, groups=5, top_groups=2)
+    same(routed(z, 4, **how), chosen(z.double(), 4, **how))
