@@ -933,35 +933,51 @@ bool experts_given(PyObject* const* a, Experts& e) {      // (x, weights, idx, g
   return sized(e.weights, {N, k}) && sized(e.idx, {N, k}) && sized(e.down, {E, C, I}) && sized(e.gate_up, {E, 2 * I, C}) && (C == 1 || e.x.stride(1) == 1) && row_step(e.x) % 8 == 0 &&
          row_step(e.x) >= C && C % 16 == 0 && I % 16 == 0 && C <= (1 << 20) && I <= (1 << 20) && E <= 1024 && N < (1L << 31) && N * k + 32 * E < (1L << 31);
 }
-PyObject* py_moe_mlp(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (x, weights, idx, gate_up, down) -> out, in training
+// Without a gradient, to `out`.  false: few tokens inside a capture, whose workspace is that capture's
+bool experts_served(const Experts& e, const Tensor& out) {
+  const long N = e.x.size(0), C = e.x.size(1), I = e.down.size(2);
+  const int k = (int)e.idx.size(1), E = (int)e.down.size(0);
+  const St st = stream();
+  const long few = K.mlb_moe_few_floats(N, k, E, (int)C, (int)I);
+  if (few == 0) {
+    experts_forward(e, nullptr, out);
+    return true;
+  }
+  if (K.mlb_capture_id(st) != 0) return false;
+  const Kept& w = kept(KEPT_EXPERTS, e.x, st, few, 0);
+  check(K.mlb_moe_few(out.data_ptr(), e.x.data_ptr(), e.weights.data_ptr(), (const int*)e.idx.data_ptr(), e.gate_up.data_ptr(), e.down.data_ptr(), (float*)w.part.data_ptr(), N, row_step(e.x), k,
+                      E, (int)C, (int)I, bits(e.weights), st),
+        "moe_mlp");
+  return true;
+}
+PyObject* py_moe_mlp(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (x, weights, idx, gate_up, down) -> out
   HANDLE_TH_ERRORS
   Experts e;
   if (n != 5 || transformed() || !experts_given(a, e)) return declined();
-  return released([&] { return ExpertsFn::apply(e.x, e.weights, e.idx, e.gate_up, e.down); });
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (wants_grad({&e.x, &e.weights, &e.gate_up, &e.down})) {
+      out = ExpertsFn::apply(e.x, e.weights, e.idx, e.gate_up, e.down);
+    } else {
+      out = at::empty(e.x.sizes(), e.x.options());
+      if (!experts_served(e, out)) out = Tensor();
+    }
+  }
+  return out.defined() ? THPVariable_Wrap(std::move(out)) : declined();
   END_HANDLE_TH_ERRORS
 }
 PyObject* py_moe_mlp_out(PyObject*, PyObject* const* a, Py_ssize_t n) {      // (out, x, weights, idx, gate_up, down)
   HANDLE_TH_ERRORS
   Experts e;
   Tensor out;
-  if (n != 6 || transformed() || !experts_given(a + 1, e)) return declined();
-  const long N = e.x.size(0), C = e.x.size(1), I = e.down.size(2);
-  const int k = (int)e.idx.size(1), E = (int)e.down.size(0);
-  if (!given(a[0], out, at::kBFloat16, {N, C}) || !aligned(out)) return declined();
-  const St st = stream();
-  const long few = K.mlb_moe_few_floats(N, k, E, (int)C, (int)I);
-  if (few > 0) {
-    if (K.mlb_capture_id(st) != 0) return declined();
-    const Kept& w = kept(KEPT_EXPERTS, e.x, st, few, 0);
-    return launched("moe_mlp", [&] {
-      return K.mlb_moe_few(out.data_ptr(), e.x.data_ptr(), e.weights.data_ptr(), (const int*)e.idx.data_ptr(), e.gate_up.data_ptr(), e.down.data_ptr(), (float*)w.part.data_ptr(),
-                           N, row_step(e.x), k, E, (int)C, (int)I, bits(e.weights), st);
-    });
-  }
+  if (n != 6 || transformed() || !experts_given(a + 1, e) || !given(a[0], out, at::kBFloat16, {e.x.size(0), e.x.size(1)}) || !aligned(out)) return declined();
+  bool done;
   {
     pybind11::gil_scoped_release no_gil;
-    experts_forward(e, nullptr, out);
+    done = experts_served(e, out);
   }
+  if (!done) return declined();
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

@@ -260,9 +260,12 @@ class MoEMLP(torch.autograd.Function):
     """x [N, C] through the experts idx [N, k] with weights [N, k]: sum_j w_nj down[e] (silu(gate) * up), [gate | up] = gate_up[e] x_n (ops/ref_moe.py)."""
 
     @staticmethod
-    def forward(ctx, x, weights, idx, gate_up, down):
+    def forward(ctx, x, weights, idx, gate_up, down, keep=True):
         x, weights, idx, gate_up, down = _rows_of(x), weights.contiguous(), idx.contiguous(), gate_up.contiguous(), down.contiguous()
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _like(x, *x.shape)
+        if not keep:      # (no gradient is asked for: nothing is kept for it, and few tokens have a form of their own)
+            ops.moe_mlp(out, x, weights, idx, gate_up, down)
+            return out
         saved = ops.moe_mlp_fwd(out, x, weights, idx, gate_up, down)
         ctx.save_for_backward(x, weights, idx, gate_up, down, *saved)
         return out
@@ -275,7 +278,7 @@ class MoEMLP(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx, dweights, dgate_up, ddown = new(x, need[0]), new(weights), new(gate_up, need[3]), new(down, need[4])
         ops.moe_mlp_bwd(dx, dweights, dgate_up, ddown, dout.contiguous(), x, weights, idx, gate_up, down, saved)
-        return dx, dweights if need[1] else None, None, dgate_up, ddown
+        return dx, dweights if need[1] else None, None, dgate_up, ddown, None
 
 
 # What programs call.  Plain calls on CUDA tensors go through the extension module (csrc/torch/bridge.cpp), which runs the same kernels
@@ -335,9 +338,7 @@ def moe_route(logits, k, bias=None, score="softmax", groups=1, top_groups=1, ren
 
 def moe_mlp(x, weights, idx, gate_up, down):
     """x [N, C] through the SwiGLU experts gate_up [E, 2 I, C], down [E, C, I] that `moe_route` chose, weighted and added up."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weights, gate_up, down)):
-        y = _plain("moe_mlp", x, weights, idx, gate_up, down)
-        return MoEMLP.apply(x, weights, idx, gate_up, down) if y is NotImplemented else y
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    ops.moe_mlp(out, _rows_of(x), weights.contiguous(), idx.contiguous(), gate_up.contiguous(), down.contiguous())
-    return out
+    y = _plain("moe_mlp", x, weights, idx, gate_up, down)
+    if y is not NotImplemented:
+        return y
+    return MoEMLP.apply(x, weights, idx, gate_up, down, torch.is_grad_enabled() and any(t.requires_grad for t in (x, weights, gate_up, down)))

@@ -254,3 +254,23 @@ def test_there_is_no_second_derivative():
         assert all(torch.equal(a, b) for a, b in zip(plain, grads)) and not any(g.requires_grad for g in plain)
         with pytest.raises(RuntimeError, match="no second derivative"):
             sum(g.square().sum() for g in grads).backward()
+
+
+def test_tangents_and_traces_meet_the_functions():
+    """Where nothing asks for a gradient, too: a tangent is refused as the other operators refuse it, and a trace holds the operator."""
+    import torch.autograd.forward_ad as fwAD
+    x, w, idx, gate_up, down = case(9, 4, 2, 16, 16)
+    z = torch.randn(9, 4)
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), fwAD.dual_level():
+            dual = lambda t: fwAD.make_dual(t, torch.ones_like(t))
+            for call in (lambda: F.moe_mlp(dual(x), w, idx, gate_up, down), lambda: F.moe_mlp(x, dual(w), idx, gate_up, down), lambda: F.moe_mlp(x, w, idx, gate_up, dual(down)),
+                         lambda: F.moe_route(dual(z), 2)):
+                with pytest.raises(NotImplementedError):
+                    call()
+    for call, args in ((F.moe_mlp, (x, w, idx, gate_up, down)), (lambda t: F.moe_route(t, 2)[0], (z,))):
+        graph = torch.jit.trace(call, args, check_trace=False).graph
+        assert any(n.kind() == "prim::PythonOp" for n in graph.nodes()), graph
+    with torch.inference_mode():
+        served = F.moe_mlp(x * 1, w, idx, gate_up, down)
+    assert torch.equal(served, F.moe_mlp(x, w, idx, gate_up.requires_grad_(), down).detach())
