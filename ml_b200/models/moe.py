@@ -62,10 +62,11 @@ class MoE(nn.Module):
         self.register_buffer("load", torch.zeros(n_experts, device=device), persistent=False)
 
     def _apply(self, fn, recurse=True):
+        held = {n: t for n in ("bias", "load") if (t := getattr(self, n)) is not None}
         super()._apply(fn, recurse)
-        for n in ("bias", "load"):      # (a change of the weights' type leaves these in 32 bits)
-            if getattr(self, n) is not None:
-                setattr(self, n, getattr(self, n).float())
+        for n, t in held.items():      # (a change of the weights' type leaves these as they are, in 32 bits)
+            if getattr(self, n).dtype != torch.float32:
+                setattr(self, n, t.to(getattr(self, n).device))
         return self
 
     def forward(self, x):

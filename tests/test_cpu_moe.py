@@ -274,3 +274,21 @@ def test_tangents_and_traces_meet_the_functions():
     with torch.inference_mode():
         served = F.moe_mlp(x * 1, w, idx, gate_up, down)
     assert torch.equal(served, F.moe_mlp(x, w, idx, gate_up.requires_grad_(), down).detach())
+
+
+def test_another_type_of_weights_leaves_the_balance_as_it_is():
+    from ml_b200.models.moe import MoE
+    m = MoE(16, 16, 8, 2, score="sigmoid", balanced=True)
+    m.bias.copy_(0.5 + 1e-3 * torch.arange(8))
+    m.load.copy_(70001.0 + torch.arange(8))
+    bias, load = m.bias.clone(), m.load.clone()
+    outer = torch.nn.Sequential(torch.nn.Sequential(m))
+    for change in (torch.nn.Module.bfloat16, torch.nn.Module.half, torch.nn.Module.double, torch.nn.Module.float, lambda t: t.to(torch.bfloat16), lambda t: t.to("cpu", torch.float16),
+                   lambda t: t.to(torch.device("cpu"))):
+        change(outer)
+        assert torch.equal(m.bias, bias) and torch.equal(m.load, load) and m.bias.dtype == m.load.dtype == torch.float32
+    m.to("meta", torch.bfloat16)
+    assert m.bias.is_meta and m.bias.dtype == torch.float32 and m.router.dtype == torch.bfloat16
+    m.to_empty(device="cpu")
+    assert m.bias.device.type == "cpu" and m.bias.dtype == torch.float32
+    assert {n for n, _ in m.named_buffers()} == {"bias", "load"} and "load" not in m.state_dict()
