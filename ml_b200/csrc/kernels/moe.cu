@@ -821,7 +821,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_h_k(const __grid_const
   __shared__ FewLists L;
   __shared__ uint64_t full[FEW_WARPS][FEW_STAGES];
   __shared__ float4 part[2][FEW_WARPS][32];
+  __shared__ volatile int late;      // a wait of some warp ran out: what it shares units of is not stored
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  if (threadIdx.x == 0) late = 0;
   if (lane == 0) {
     for (int i = 0; i < FEW_STAGES; i++) tc::mbar_init(&full[w][i], 1);
     tc::mbar_fence_init();
@@ -845,7 +847,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_h_k(const __grid_const
     if ((next_s += ways) >= steps) next_s = part_of, next_unit += every;
   };
   for (int i = 0; i < FEW_STAGES; i++) ask();
-  bool ok = true;
   uint4 ahead[FEW_BOXES][2] = {};      // the tokens' part of the next step, asked for while this one goes on
   auto tokens = [&](int unit, int s) {
     const int a = unit / groups, f0 = L.first[a], c = L.list[f0 + min(r, L.first[a + 1] - f0 - 1)];      // (columns behind the last copy: its row, nothing of theirs is used)
@@ -863,7 +864,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_h_k(const __grid_const
       if (s + ways < steps) tokens(unit, s + ways);
       else if (unit + every < units) tokens(unit + every, part_of);
       const int stage = n % FEW_STAGES;
-      if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[w][stage], (n / FEW_STAGES) & 1, 0x76));
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[w][stage], (n / FEW_STAGES) & 1, 0x76))) {
+        // nothing more is asked for or stored; what is on its way is waited for, the late one once more, and so are the warps that share units with this one
+        late = 1;
+        for (int x = n; x < asked; x++) tc::mbar_wait(&full[w][x % FEW_STAGES], (x / FEW_STAGES) & 1, 0x77);
+        __syncwarp();
+        for (; ways > 1 && unit < units; unit += every) asm volatile("bar.sync %0, %1;" ::"r"(1 + w / ways), "r"(32 * ways) : "memory");
+        return;
+      }
       few_products(d, ring + stage * FEW_BOXES * FEW_BOX, v, boxes - s * FEW_BOXES, r, t);
       __syncwarp();
       ask();
@@ -873,7 +881,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) moe_few_h_k(const __grid_const
     if (ways > 1) {      // (two places in turn: whoever writes to one again has met the others behind their reading of it)
       part[turn][w][lane] = sum;
       asm volatile("bar.sync %0, %1;" ::"r"(1 + w / ways), "r"(32 * ways) : "memory");
-      if (part_of != 0) continue;
+      if (part_of != 0 || late) continue;
       for (int j = 1; j < ways; j++) {
         const float4 x = part[turn][w + j][lane];
         sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
@@ -896,7 +904,9 @@ __global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(FEW_THREADS, 1) 
   __shared__ FewLists L;
   __shared__ uint64_t full[FEW_WARPS][FEW_STAGES];
   __shared__ float weight[FEW_COPIES], part[FEW_WARPS][8][16], sums[FEW_WARPS][FEW_TOKENS][16], from[SPLIT][FEW_TOKENS * 16];
+  __shared__ volatile int late;      // a wait of some warp of the cluster ran out: nothing more is stored (asked in its first block)
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rank = SPLIT > 1 ? (int)tc::cluster_ctarank() : 0;
+  if (tid == 0) late = 0;
   // The kernel before is that for h, which has waited for all before it: idx and the weights stand, and only h has to be waited for.  (Past the L1, of which nothing is known so early.)
   if (tid < A.N * A.k) weight[tid] = A.wbits == 32 ? __ldcg((const float*)A.weights + tid) : __uint_as_float((uint32_t)__ldcg((const unsigned short*)A.weights + tid) << 16);
   if (lane == 0) {
@@ -924,7 +934,6 @@ __global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(FEW_THREADS, 1) 
   for (int i = 0; i < FEW_STAGES; i++) ask();
   if (SPLIT > 1) tc::cluster_sync();      // (the first block of the cluster is there to be written to)
   mlb_pdl_sync();
-  bool ok = true;
   uint4 ahead[FEW_BOXES][2] = {};
   auto tokens = [&](int i) {
     const int a = i / steps, f0 = L.first[a], c = L.list[f0 + min(r, L.first[a + 1] - f0 - 1)];      // (columns behind the last copy: its row, nothing of theirs is used)
@@ -942,7 +951,18 @@ __global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(FEW_THREADS, 1) 
       for (int x = 0; x < 2 * FEW_BOXES; x++) v[x / 2][x % 2] = ahead[x / 2][x % 2];
       tokens(i + 1 < end ? i + 1 : begin);
       const int stage = n % FEW_STAGES;
-      if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[w][stage], (n / FEW_STAGES) & 1, 0x76));
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[w][stage], (n / FEW_STAGES) & 1, 0x78))) {
+        // nothing more is asked for or stored; what is on its way is waited for, the late one once more, and so are the other warps
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::mapa_u32(tc::smem_u32((const void*)&late), 0)), "r"(1) : "memory");
+        for (int x = n; x < asked; x++) tc::mbar_wait(&full[w][x % FEW_STAGES], (x / FEW_STAGES) & 1, 0x79);
+        __syncwarp();
+        for (; g < groups; g += every) {
+          __syncthreads();
+          if (SPLIT > 1) tc::cluster_sync();
+          else __syncthreads();
+        }
+        return;
+      }
       few_products(d, ring + stage * FEW_BOXES * FEW_BOX, v, boxes - s * FEW_BOXES, r, t);
       __syncwarp();
       ask();
@@ -971,7 +991,7 @@ __global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(FEW_THREADS, 1) 
     }
     if (SPLIT > 1) tc::cluster_sync();      // (where blocks share columns each has one turn: `from` is not written again)
     else __syncthreads();
-    if (rank == 0 && tid < 16 * A.N) {
+    if (rank == 0 && tid < 16 * A.N && !late) {
 #pragma unroll
       for (int i = 1; i < SPLIT; i++) sum += from[i][tid];
       A.out[(size_t)(tid / 16) * A.C + g * 16 + tid % 16] = __float2bfloat16(sum);

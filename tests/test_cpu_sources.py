@@ -130,3 +130,27 @@ def test_untiled_copies_on_their_way_are_waited_for_when_a_wait_has_run_out():
         assert re.search(r"some && !dead|tid == 0 && whole > 0 && !late", body), (file, name)
         seen.add(name)
     assert seen == {"kv4_attn_k", "beam_select_k"}
+
+
+def test_few_tokens_of_experts_that_wait_in_vain_store_nothing():
+    """A warp whose wait has run out says so, waits for all that is on its way, the late one as well, keeps meeting the others, and leaves; what they had together is not stored."""
+    seen = set()
+    for file, name, body, _ in _kernels():
+        if not name.startswith("moe_few_"):
+            continue
+        waits = [m for m in WAIT.finditer(body) if "mbar_wait" in m.group(0)]
+        assert len(waits) == 2 and list(_heads(body, waits[0].start()))[0].strip() == "if (!__all_sync(0xffffffffu,", name
+        begin = body.index("{", waits[0].end())
+        depth, end = 1, begin + 1
+        while depth:
+            depth += {"{": 1, "}": -1}.get(body[end], 0)
+            end += 1
+        block = body[begin:end]
+        assert re.search(r"\blate\b", block) and "for (int x = n; x < asked; x++) tc::mbar_wait(" in block and re.search(r"return;\s*\}$", block), name
+        met = ["bar.sync"] if name == "moe_few_h_k" else ["__syncthreads()", "cluster_sync()"]
+        assert all(b in block for b in met), name
+        stores = [m.start() for m in re.finditer(r"\bA\.(h|out)\[[^;]*\] = ", body)]
+        assert len(stores) == 1, name
+        assert "!late" in "".join(_heads(body, stores[0])) or "|| late) continue;" in body[body.rindex("bar.sync", 0, stores[0]):stores[0]], name
+        seen.add(name)
+    assert seen == {"moe_few_h_k", "moe_few_out_k"}
