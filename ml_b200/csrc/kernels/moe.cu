@@ -455,6 +455,7 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* place_full = acc_empty + 2;      // [EPI][PLACES]
   uint32_t* tmem_slot = (uint32_t*)(place_full + (MODE == DOWN_T ? S::EPI * S::PLACES : 0));
+  volatile uint32_t* late = tmem_slot + 1;      // the accumulators of some epilogue warp did not come: no tokens' tile is stored
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_ctarank();
@@ -463,6 +464,7 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; i++) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; i++) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 2 * S::EPI); }
+    *late = 0;
     if (MODE == DOWN_T)
       for (int i = 0; i < S::EPI * S::PLACES; i++) tc::mbar_init(&place_full[i], 1);
     tc::mbar_fence_init();
@@ -518,6 +520,8 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
+      if (rank == 0)      // what was asked for last has arrived (both CTAs' part) when the kernel ends, whoever has given up on it
+        for (int i = 0; i < STAGES; i++) tc::mbar_wait(&full[i], i < stage ? phase : phase ^ 1, 0x7A);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- products (one thread of the leader)
@@ -599,7 +603,7 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
       const bool live = m0 < g.M;
       if (some) {
         it++;
-        if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[acc], acc_phase, 0x74));
+        if (ok && !__all_sync(0xffffffffu, tc::mbar_wait(&acc_full[acc], acc_phase, 0x74))) ok = false, *late = 1;
         if (MODE == DOWN_T && !ok) break;
         tc::tc_fence_after();
       }
@@ -676,7 +680,7 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
           if constexpr (MODE != DOWN_T) {
             tc::fence_async_smem();
             meet();
-            if (ok && lg == 0 && lane == 0) {
+            if (lg == 0 && lane == 0 && !*late) {
               if (MODE != H)
                 for (int i = 0; i < 2 && m0 + 64 * i < g.M; i++) tc::tma_store_2d(&tmOut, place + 4096 * i, m0 + 64 * i, w.row0 + c);
               if (MODE == GATE_UP || MODE == H) tc::tma_store_2d(&tmB1, hs, m0 / 2, w.row0 + c);
@@ -719,6 +723,10 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
           }
         }
       }
+    }
+    if constexpr (MODE == DOWN_T) {
+      for (; n < ahead_n; n++) tc::mbar_wait(&place_full[(warp - 2) * S::PLACES + n % S::PLACES], (n / S::PLACES) & 1, 0x7B);      // (of a warp that has given up: what is on its way, the late one once more)
+      __syncwarp();
     }
     if (lane == 0) tc::tma_wait_group<0>();
   }

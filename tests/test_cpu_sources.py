@@ -154,3 +154,17 @@ def test_few_tokens_of_experts_that_wait_in_vain_store_nothing():
         assert "!late" in "".join(_heads(body, stores[0])) or "|| late) continue;" in body[body.rindex("bar.sync", 0, stores[0]):stores[0]], name
         seen.add(name)
     assert seen == {"moe_few_h_k", "moe_few_out_k"}
+
+
+def test_products_of_experts_that_wait_in_vain_store_no_tile():
+    """Four epilogue warps put a tile side by side: one whose accumulators did not come says so to the one that stores.  What was asked for has arrived when the kernel ends."""
+    (body,) = [b for _, name, b, _ in _kernels() if name == "moe_gemm_k"]
+    assert re.search(r"mbar_wait\(&acc_full\[acc\], acc_phase, 0x74\)\)\) ok = false, \*late = 1;", body) and "*late = 0;" in body[:body.index("cluster_sync")]
+    for m in re.finditer(r"tc::tma_store_\dd\(", body):
+        heads = "".join(_heads(body, m.start()))
+        asked = "!*late" in heads or "if (ok &&" in heads      # (ok: rows that a warp has for itself)
+        alone = "MODE == DOWN_T" in heads                      # (a warp that has given up has left the loop)
+        assert asked or alone, body[m.start():m.start() + 60]
+    loader = body[body.index("tc::elect_one()"):body.index("warp == 1) {", body.index("tc::elect_one()"))]
+    assert re.search(r"for \(int i = 0; i < STAGES; i\+\+\) tc::mbar_wait\(&full\[i\], i < stage \? phase : phase \^ 1", loader)
+    assert re.search(r"for \(; n < ahead_n; n\+\+\) tc::mbar_wait\(&place_full\[", body)
