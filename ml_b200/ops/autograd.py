@@ -277,7 +277,7 @@ class MoEMLP(torch.autograd.Function):
         new = lambda t, wanted=True: torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None
         need = ctx.needs_input_grad
         dx, dweights, dgate_up, ddown = new(x, need[0]), new(weights), new(gate_up, need[3]), new(down, need[4])
-        ops.moe_mlp_bwd(dx, dweights, dgate_up, ddown, dout.contiguous(), x, weights, idx, gate_up, down, saved)
+        ops.moe_mlp_bwd(dx, dweights, dgate_up, ddown, _rows_of(dout), x, weights, idx, gate_up, down, saved)
         return dx, dweights if need[1] else None, None, dgate_up, ddown, None
 
 

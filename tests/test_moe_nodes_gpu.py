@@ -128,3 +128,24 @@ def test_without_a_gradient_the_operator_is_the_entry_point(N):
     with torch.inference_mode():
         assert torch.equal(F.moe_mlp(x * 1, w, idx, gate_up, down), want)
         assert torch.equal(F.moe_mlp(x, w, idx, gate_up, down), want)
+
+
+@pytest.mark.parametrize("form", [offset, strided, lambda t: t[:1].expand_as(t)], ids=["offset", "strided", "broadcast"])
+@pytest.mark.parametrize("extension", [True, False])
+def test_gradients_that_arrive_in_any_layout(form, extension):
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g).to(dev())
+    N = 40
+    x, w, gate_up, down = r(N, 96).to(BF16), torch.softmax(r(N, 2), 1), (r(6, 160, 96) / 10).to(BF16), (r(6, 96, 80) / 9).to(BF16)
+    idx = torch.stack([torch.randperm(6, generator=g)[:2] for _ in range(N)]).to(dev(), I32)
+    dout = form(r(N, 96).to(BF16))
+    leaves = [t.requires_grad_() for t in (x, w, gate_up, down)]
+    # (tokens off a 16-byte boundary are no plain call)
+    y = F.moe_mlp(x if extension else offset(x), w, idx, gate_up, down)
+    assert ("CppNode" in y.grad_fn.name()) == extension
+    want = torch.autograd.grad(F.moe_mlp(x, w, idx, gate_up, down), leaves, dout.contiguous().clone())
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dout), want))
+    z = r(N, 6).requires_grad_()
+    p = F.moe_route(z, 2)[0] if extension else F.MoERoute.apply(z, 2, None, "softmax", 1, 1, True, 1.0, F32)[0]
+    dp = form(r(N, 2))
+    assert torch.equal(*(torch.autograd.grad(p, z, d, retain_graph=True)[0] for d in (dp, dp.contiguous().clone())))
