@@ -809,8 +809,14 @@ def scale_(x, s):
     _chk(lib().mlb_scale_f32(_f(x), x.numel(), s, _st()), "scale_f32")
 
 
-# ------------------------------------------------------------------ generation
-from .native_gen import beam_reorder, beam_select, block_tables, kv4_append, kv4_attn, kv4_read  # noqa: E402,F401
+# ------------------------------------------------------------------ generation, experts
+_ELSEWHERE = {**dict.fromkeys(("beam_reorder", "beam_select", "block_tables", "kv4_append", "kv4_attn", "kv4_read"), "native_gen"),
+              **dict.fromkeys(("moe_mlp", "moe_mlp_bwd", "moe_mlp_fwd", "moe_route", "moe_route_bwd"), "native_moe")}
 
-# ------------------------------------------------------------------ experts
-from .native_moe import moe_mlp, moe_mlp_bwd, moe_mlp_fwd, moe_route, moe_route_bwd  # noqa: E402,F401
+
+def __getattr__(name):      # (these modules import this one, and either may come first)
+    if name not in _ELSEWHERE:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    import importlib
+    fn = globals()[name] = getattr(importlib.import_module("." + _ELSEWHERE[name], __package__), name)
+    return fn

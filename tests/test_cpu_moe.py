@@ -292,3 +292,12 @@ def test_another_type_of_weights_leaves_the_balance_as_it_is():
     m.to_empty(device="cpu")
     assert m.bias.device.type == "cpu" and m.bias.dtype == torch.float32
     assert {n for n, _ in m.named_buffers()} == {"bias", "load"} and "load" not in m.state_dict()
+
+
+@pytest.mark.parametrize("first", ["native_moe", "native_gen", "native"])
+def test_modules_of_operators_are_imported_in_any_order(first):
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = f"from ml_b200.ops import {first}; from ml_b200.ops import native as n, native_moe as m, native_gen as g; assert n.moe_mlp is m.moe_mlp and n.kv4_attn is g.kv4_attn and not hasattr(n, 'none')"
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=Path(__file__).resolve().parent.parent, timeout=300)
