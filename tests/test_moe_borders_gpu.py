@@ -135,3 +135,77 @@ def test_logits_and_biases_below_the_normal_numbers(dtype):
     same(routed(z, 4, **how), chosen(z.double(), 4, **how))
     how = dict(score="sigmoid", bias=bias, groups=5, top_groups=2)
     same(routed(z, 4, **how), chosen(z.double(), 4, **how))
+
+
+# ------------------------------------------------------------------ several tokens to a warp
+MANY = [(5001, 8, 2, 1, 1), (5001, 60, 4, 1, 1), (20000, 60, 4, 6, 3), (9600, 256, 8, 8, 4), (20000, 256, 8, 1, 1), (5001, 1000, 5, 1, 1), (530001, 8, 2, 1, 1)]      # (the last: several in the backward pass, too)
+
+
+@pytest.mark.parametrize("N,E,k,groups,top", MANY)
+@pytest.mark.parametrize("score,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_more_tokens_than_warps(N, E, k, groups, top, score, renorm, biased):
+    """Indices, weights, means and gradient of as many tokens as give every warp several, rows of NaN, -inf and equal logits between ordinary ones."""
+    dtype = BF16 if N == 5001 else F32
+    g = torch.Generator(device="cuda").manual_seed(N + E)
+    z = (2 * torch.randn(N, E, generator=g, device=dev())).to(dtype)
+    kind = torch.randint(0, 12, (N,), generator=g, device=dev())
+    z[kind == 0] = NEG
+    z[kind == 1] = torch.where(torch.rand(int((kind == 1).sum()), E, generator=g, device=dev()) < 0.5, math.nan, z[kind == 1].float()).to(dtype)
+    z[kind == 2] = 0.5
+    z[kind == 3, 1:] = NEG
+    z[kind == 4] = z[kind == 4].clamp(min=-1, max=1).round()
+    bias = 0.1 * torch.randn(E, generator=g, device=dev()) if biased else None
+    how = dict(bias=bias, score=score, groups=groups, top_groups=top)
+    scale = 1.5
+    zr = z.clone().requires_grad_()
+    w, idx, mean = F.moe_route(zr, k, renorm=renorm, scale=scale, dtype=F32, **how)
+    dw, dm = torch.randn(N, k, generator=g, device=dev()), torch.randn(E, generator=g, device=dev()) * E
+    dz, = torch.autograd.grad([w, mean], [zr], [dw, dm])
+
+    zd = torch.where(torch.isnan(z), NEG, z.double())
+    want = chosen(zd, k, **how)
+    same(idx, want)
+    s, has, at = scores(zd, score), want >= 0, want.clamp(min=0).long()
+    sj = torch.where(has, s.gather(1, at), 0.0)
+    q = sj / sj.sum(1, keepdim=True).clamp(min=1e-300)
+    p = s / s.sum(1, keepdim=True).clamp(min=1e-300)
+    # exp and a division 10 half steps; sums of E terms 5 + E / 32 additions and its terms; the difference of a logit and the largest, rounded, |z| + |m| half steps of an exponential
+    span = torch.where(zd > NEG, zd.abs() + zd.amax(1, keepdim=True).abs(), 0.0)
+    tol = STEP * (10 + 2 * (5 + E / 32) + 4)
+    ew = scale * (q if renorm else sj)
+    spread = span.amax(1, keepdim=True)
+    assert torch.all((w.double() - ew).abs() <= (tol + 2 * STEP * spread) * ew + 1e-37)
+    # a warp's running sum, those of 8 warps, and 32 threads' of the blocks'
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    adds = N / (32 * sms) + 1 + 8 + sms / 8 + 1 + 5 + 2
+    assert torch.all((mean.double() - p.mean(0)).abs() <= STEP * (adds * p.mean(0)) + tol * p.mean(0) + 2 * STEP * (p * spread).mean(0) + 1e-37)
+
+    gw = torch.zeros_like(s).scatter_add_(1, at, torch.where(has, dw.double() * scale, 0.0))
+    qf = torch.zeros_like(s).scatter_add_(1, at, q)
+    h, rest = dm.double() / N, (1.0 if score == "softmax" else 1 - s)
+    if renorm:
+        ez = qf * (gw - (qf * gw).sum(1, keepdim=True)) * rest
+    elif score == "softmax":
+        ez = s * (gw - (s * gw).sum(1, keepdim=True))
+    else:
+        ez = s * rest * gw
+    ez = ez + p * (h - (p * h).sum(1, keepdim=True)) * rest
+    # two differences p (g - sum p g), whose terms are off by as much as a weight is, relative to the largest g of the row; then the rounding to the logits' type
+    size = scale * dw.abs().amax(1, keepdim=True).double() + dm.abs().max().double() / N
+    half = 2.0 ** -8 if dtype == BF16 else STEP
+    assert torch.all((dz.double() - ez).abs() <= half * ez.abs() + 3 * (tol + 4 * STEP + 2 * STEP * spread) * size + 1e-37)
+
+
+def test_routing_gives_the_same_bits_on_every_run():
+    z = torch.randn(20000, 60, device=dev()).requires_grad_()
+    bias = torch.randn(60, device=dev()) * 0.1
+    dw, dm = torch.randn(20000, 4, device=dev()), torch.randn(60, device=dev())
+
+    def step():
+        w, idx, mean = F.moe_route(z, 4, bias=bias, score="sigmoid")
+        return [w.detach(), idx, mean.detach(), *torch.autograd.grad([w, mean], [z], [dw, dm])]
+
+    first = step()
+    for _ in range(10):
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
