@@ -1003,7 +1003,7 @@ bool mlb_make_tmap(CUtensorMap* out, const void* base, uint64_t rows, uint64_t c
   return r == CUDA_SUCCESS;
 }
 
-bool mlb_make_tmap_nd(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, int swizzle) {
+bool mlb_make_tmap_nd(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
   EncodeTiledFn enc = get_encode();
   if (!enc || rank < 2 || rank > 5 || ((uintptr_t)base & 15)) return false;
   cuuint64_t d[5], s[4];
@@ -1013,7 +1013,7 @@ bool mlb_make_tmap_nd(CUtensorMap* out, const void* base, int rank, const uint64
     if (i > 0) s[i - 1] = strides[i - 1];
   }
   return encode_map(enc, out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    swizzle == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 const CUtensorMap* mlb_tmap_cached(const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_elems,

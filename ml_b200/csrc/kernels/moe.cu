@@ -1054,11 +1054,11 @@ bool map_tokens(Maps& m, const bf16* base, long rows, int K) {      // [rows, K]
   const uint32_t b[2] = {64, 128}, b16[2] = {64, 16};
   return mlb_make_tmap_nd(&m.b, base, 2, d, s, b) && mlb_make_tmap_nd(&m.b16, base, 2, d, s, b16);
 }
-// the same for what leaves an epilogue warp or arrives there: some tokens of `width` columns
-bool map_chunk(CUtensorMap* m, const bf16* base, long rows, int cols, uint32_t width, uint32_t tokens = 32) {
+// the same for what leaves an epilogue warp or arrives there: 64 columns of some tokens
+bool map_chunk(CUtensorMap* m, const bf16* base, long rows, int cols, uint32_t tokens = 32) {
   const uint64_t d[2] = {(uint64_t)cols, (uint64_t)rows}, s[1] = {2ull * cols};
-  const uint32_t b[2] = {width, tokens};
-  return mlb_make_tmap_nd(m, base, 2, d, s, b, 2 * (int)width);
+  const uint32_t b[2] = {64, tokens};
+  return mlb_make_tmap_nd(m, base, 2, d, s, b);
 }
 bool map_rows(CUtensorMap* m, const bf16* base, long rows, int cols) {      // the same, its columns M or N and its rows the reduction
   const uint64_t d[2] = {(uint64_t)cols, (uint64_t)rows}, s[1] = {2ull * cols};
@@ -1144,12 +1144,12 @@ MLB_API int mlb_moe_fwd(void* out, void* xs, void* gu, void* h, void* y, const v
   GemmArgs g = {};
   g.start = P.start, g.order = P.order, g.tiles = P.tiles, g.ntiles = P.ntiles, g.E = E;
   g.out = (bf16*)gu, g.h = (bf16*)h, g.M = 2 * I, g.K = C, g.tiles_m = (2 * I + 255) / 256;
-  if (!map_gate_up(&m.a, (const bf16*)gate_up, E, C, I, 4) || !map_tokens(m, (const bf16*)xs, z.p.rows, C) || !map_chunk(&m.b1, g.h, z.p.rows, I, 64) ||
-      (g.out != nullptr && !map_chunk(&m.out, g.out, z.p.rows, 2 * I, 64)))
+  if (!map_gate_up(&m.a, (const bf16*)gate_up, E, C, I, 4) || !map_tokens(m, (const bf16*)xs, z.p.rows, C) || !map_chunk(&m.b1, g.h, z.p.rows, I) ||
+      (g.out != nullptr && !map_chunk(&m.out, g.out, z.p.rows, 2 * I)))
     return -2;
   MLB_TRY(gu != nullptr ? launch_gemm<GATE_UP>(m, g, (long)z.p.max_tiles * g.tiles_m, st) : launch_gemm<H>(m, g, (long)z.p.max_tiles * g.tiles_m, st));
   g.out = (bf16*)y, g.h = nullptr, g.M = C, g.K = I, g.tiles_m = (C + 255) / 256;
-  if (!map_down(&m.a, (const bf16*)down, E, C, I, 128) || !map_tokens(m, (const bf16*)h, z.p.rows, I) || !map_chunk(&m.out, g.out, z.p.rows, C, 64)) return -2;
+  if (!map_down(&m.a, (const bf16*)down, E, C, I, 128) || !map_tokens(m, (const bf16*)h, z.p.rows, I) || !map_chunk(&m.out, g.out, z.p.rows, C)) return -2;
   MLB_TRY(launch_gemm<DOWN>(m, g, (long)z.p.max_tiles * g.tiles_m, st));
   return wbits == 16 ? combine((bf16*)out, (const bf16*)y, (const bf16*)weights, P, z, st) : combine((bf16*)out, (const bf16*)y, (const float*)weights, P, z, st);
 }
@@ -1171,8 +1171,8 @@ MLB_API int mlb_moe_bwd(void* dx, void* dweights, void* dgate_up, void* ddown, v
   g.out = (bf16*)dgu, g.M = I, g.K = C, g.tiles_m = (I + 255) / 256;
   if (dx != nullptr || dgate_up != nullptr) {
     constexpr int chunk = Smem<DOWN_T>::CHUNK;
-    if (!map_down(&m.a, (const bf16*)down, E, C, I, 64) || !map_tokens(m, (const bf16*)ys, R, C) || !map_chunk(&m.a1, (const bf16*)gu, R, 2 * I, 64, chunk) ||
-        !map_chunk(&m.out, g.out, R, 2 * I, 64, chunk))
+    if (!map_down(&m.a, (const bf16*)down, E, C, I, 64) || !map_tokens(m, (const bf16*)ys, R, C) || !map_chunk(&m.a1, (const bf16*)gu, R, 2 * I, chunk) ||
+        !map_chunk(&m.out, g.out, R, 2 * I, chunk))
       return -2;
     MLB_TRY(launch_gemm<DOWN_T>(m, g, (long)z.p.max_tiles * g.tiles_m, st));
   }
@@ -1181,7 +1181,7 @@ MLB_API int mlb_moe_bwd(void* dx, void* dweights, void* dgate_up, void* ddown, v
   g.per_gate_up = dgate_up != nullptr ? ((2 * I + 255) / 256) * ((C + 255) / 256) : 0;
   g.per_down = ddown != nullptr ? ((C + 255) / 256) * ((I + 255) / 256) : 0;
   if (!map_gate_up(&m.a, (const bf16*)gate_up, E, C, I, 2) || !map_tokens(m, (const bf16*)dgu, R, 2 * I) || !map_rows(&m.a1, (const bf16*)dgu, R, 2 * I) ||
-      !map_rows(&m.b1, (const bf16*)xs, R, C) || !map_rows(&m.a2, (const bf16*)ys, R, C) || !map_rows(&m.b2, (const bf16*)h, R, I) || (dx != nullptr && !map_chunk(&m.out, g.out, R, C, 64)) ||
+      !map_rows(&m.b1, (const bf16*)xs, R, C) || !map_rows(&m.a2, (const bf16*)ys, R, C) || !map_rows(&m.b2, (const bf16*)h, R, I) || (dx != nullptr && !map_chunk(&m.out, g.out, R, C)) ||
       (dgate_up != nullptr && !map_gate_up(&m.out1, (const bf16*)dgate_up, E, C, I, 1)) || (ddown != nullptr && !map_down(&m.out2, (const bf16*)ddown, E, C, I, 32)))
     return -2;
   MLB_TRY(launch_gemm<BACK>(m, g, (long)E * (g.per_gate_up + g.per_down) + (long)z.p.max_tiles * g.tiles_m, st));

@@ -583,6 +583,6 @@ const CUtensorMap* mlb_tmap_cached(const void* base, uint64_t rows, uint64_t col
 // [seqs][rows][cols] bf16, contiguous, box {64 columns, 64 rows, 1 sequence}, 128-byte swizzle: rows past a sequence's end read as
 // zeros instead of the next sequence's.  Needs a 16-byte aligned base and cols a multiple of 8.
 const CUtensorMap* mlb_tmap_seq3d_cached(const void* base, uint64_t seqs, uint64_t rows, uint64_t cols);
-// Any bf16 tensor of up to five dimensions, innermost first, rows of a box swizzled over 128, 64 or 32 bytes; `strides` (bytes) of the dimensions behind the first.  Encoded anew each time, a
+// Any bf16 tensor of up to five dimensions, innermost first, rows of a box swizzled over 128 bytes; `strides` (bytes) of the dimensions behind the first.  Encoded anew each time, a
 // fraction of a microsecond.  false: refused.
-bool mlb_make_tmap_nd(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, int swizzle = 128);
+bool mlb_make_tmap_nd(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
