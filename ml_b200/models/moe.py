@@ -71,7 +71,8 @@ class MoE(nn.Module):
 
     def forward(self, x):
         """x: [N, C] -> [N, C]; also returns the load-balancing auxiliary loss (mean prob * mean assignment per expert)."""
-        weights, idx, mean = F.moe_route(F.linear(x, self.router), self.k, bias=self.bias, **self.how)
+        logits = F.linear(x, self.router) if len(x) else x @ self.router.T      # (the kernels' product takes one row at least)
+        weights, idx, mean = F.moe_route(logits, self.k, bias=self.bias, **self.how)
         out = F.moe_mlp(x, weights, idx, self.gate_up, self.down)
         chosen = idx.flatten()
         load = torch.zeros_like(self.load).scatter_add_(0, chosen.clamp(min=0).long(), (chosen >= 0).float())

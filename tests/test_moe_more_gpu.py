@@ -70,3 +70,16 @@ def test_block_of_any_number_of_experts(E, k, N):
     with torch.no_grad():
         served, _ = m(x.detach())
     assert float((served.double() - want).norm()) <= 3 * HALF * float(want.norm())
+
+
+@pytest.mark.parametrize("device,dtype", [("cpu", F32), ("cuda:0", BF16)])
+def test_block_of_no_tokens(device, dtype):
+    from ml_b200.models.moe import MoE
+    m = MoE(64, 48, 6, 2, score="sigmoid", balanced=True, device=device, dtype=dtype)
+    x = torch.empty(0, 64, device=device, dtype=dtype, requires_grad=True)
+    y, aux = m(x)
+    assert y.shape == (0, 64) and float(aux.detach()) == 0 and m.load.sum() == 0
+    grads = torch.autograd.grad(y.sum() + aux, [x, *m.parameters()])
+    assert all(bool((t == 0).all()) for t in grads)
+    with torch.no_grad():
+        assert m.eval()(x)[0].shape == (0, 64)
