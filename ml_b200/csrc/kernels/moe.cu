@@ -739,7 +739,11 @@ moe_gemm_k(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
 // A step of a few tokens reads the weights of the experts that they chose, once, and that is all its time.  Warps read boxes of 16 rows x 64 columns of the weights, each into shared memory
 // of its own: three stages of four boxes, 192 KB an SM on their way.  The products are m16n8k16 instructions whose 16 rows are weights and whose 8 columns are tokens (which eight
 // elements of the reduction an instruction has is the same for both operands: 16 neighbouring bytes a lane serve two instructions).  Two launches: h of all copies, then
-// the tokens' weighted sums.  An expert's copies are found by each block for itself: 256 at most.
+// the tokens' weighted sums.  An expert's copies are found by each block for itself: 256 at most.  Up to eight tokens, the instruction's columns, as one more brings a second turn at an expert's weights
+// where all go to few.  Eight tokens so, and nine by the other form, us in a graph: 6 of 64 experts of 1376 behind 2048 columns 103.9, 124.2; 2 of 8 of 5504 behind 2048 99.2, 100.5, of
+// 2048 behind 768 22.9, 28.8; 2 of 2 of 5504 behind 2048 36.4, 50.6; 1 of 4 of 11008 behind 4096 109.4, 117.1.
+// A warp whose wait has run out stores nothing, waits for what is on its way and leaves, meeting those that it shares barriers with until the end: 1.2 per cent of the time, the code around the
+// loops' waits (one token to 6 of 64 experts 25.3 -> 25.5, eight 102.8 -> 104.0; asking for nothing more and going on was no faster).
 constexpr int FEW_TOKENS = 8, FEW_COPIES = 256, FEW_WARPS = 8, FEW_THREADS = 32 * FEW_WARPS, FEW_BOX = 2048, FEW_BOXES = 4, FEW_STAGES = 3;
 constexpr int FEW_SMEM = FEW_WARPS * FEW_STAGES * FEW_BOXES * FEW_BOX + 1024;
 struct FewArgs {
